@@ -341,6 +341,65 @@ int sp_decode_attn_static_bf16(const void* q, const void* k, const void* v, int6
                                int64_t v_stride_n, int64_t v_stride_h, float softmax_scale, void* out,
                                sp_stream_t stream);
 
+/* ---- serving from a key / value cache in pages -----------------------------------------------------
+ * (no counterpart in the reference, whose decode step reads a contiguous cache, shareprefill_attn.py:146-155)
+ * A cache is a pool of num_pages pages of page_size tokens (a power of two from 16 to 1024), one for K and one for V: bf16
+ * [num_pages][hkv][page_size][d] with element strides for the page, head and slot axes and a contiguous head_dim axis.  Row b of
+ * block_table (int32, table_width entries at a row stride of table_stride elements) names the pages of sequence b in order; an entry
+ * outside [0, num_pages) is no page.  At most 4096 sequences a call. */
+
+/* The bookkeeping of a step: sequence b has lens[b] tokens in the cache and new_lens[b] (0 is allowed) to be added.
+ * free_pages[0 .. *free_count) is a stack of unused pages, at most free_room; the pages that the new tokens open come off its top, in the
+ * order of the sequences, and are entered into block_table in place.  A page that the stack does not hold is entered as -1.
+ * Written: seq_lens[b] = lens[b] + new_lens[b]; cu_new[0 .. batch] = prefix sums of new_lens; per new token t < max_tokens, in the order
+ * of the sequences, slots[t] = page * page_size + position % page_size (-1: no page, or beyond the table's width) and positions[t] (its
+ * place in its sequence); tokens behind the last one get -1 and 0.  *free_left = pages left on the stack (negative: so many were missing).
+ * Negative lengths count as 0.  The outputs must not overlap the inputs. */
+int sp_paged_tables(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t page_size, int32_t num_pages,
+                    int32_t* block_table, int64_t table_stride, int32_t table_width, const int32_t* free_pages,
+                    int32_t free_room, const int32_t* free_count, int32_t max_tokens, int32_t* seq_lens, int32_t* cu_new,
+                    int64_t* slots, int32_t* positions, int32_t* free_left, sp_stream_t stream);
+
+/* k, v: bf16 [tokens][hkv][d] (token and head strides) copied to slots[t] of the pools; a slot outside the pool is skipped.  Slots
+ * must differ from each other: where two tokens name the same one, its contents are parts of either.  d a multiple of 8. */
+int sp_paged_cache_write_bf16(const void* k, const void* v, int64_t tokens, int32_t hkv, int32_t d, int64_t k_stride_n,
+                              int64_t k_stride_h, int64_t v_stride_n, int64_t v_stride_h, void* k_pages, void* v_pages,
+                              int32_t num_pages, int32_t page_size, int64_t k_stride_page, int64_t k_stride_slot,
+                              int64_t k_stride_page_h, int64_t v_stride_page, int64_t v_stride_slot,
+                              int64_t v_stride_page_h, const int64_t* slots, sp_stream_t stream);
+
+/* Attention of the new tokens over everything cached, them included.  q: bf16 [tokens][hq][d], the sequences one behind the other:
+ * sequence b has rows cu_q[b] .. cu_q[b + 1] (null: one row each, tokens == batch) and seq_lens[b] keys; its query i stands at position
+ * p = seq_lens[b] - its rows + i and sees the keys j <= p with j > p - window or j < sinks (window 0: all j <= p).  Keys without a page
+ * are not seen; a query that sees nothing gives zeros.  out: bf16 [tokens][hq][d] contiguous; rows outside every sequence stay as they
+ * were.  Device values out of range (lengths, offsets, pages) are held to what the arguments allow.  head_dim 64 or 128. */
+typedef struct sp_paged_attn_args {
+  const void *q, *k_pages, *v_pages;
+  const int32_t *block_table, *seq_lens, *cu_q;
+  void *out, *workspace;
+  uint64_t workspace_bytes;
+  int64_t tokens, batch, hq, hkv, d, num_pages, page_size, table_width, table_stride, window, sinks;
+  int64_t q_stride_n, q_stride_h, k_stride_page, k_stride_slot, k_stride_h, v_stride_page, v_stride_slot, v_stride_h;
+  double softmax_scale;
+  sp_stream_t stream;
+} sp_paged_attn_args;
+size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d);
+int sp_paged_attn_bf16(const sp_paged_attn_args* args /* host */);
+
+/* The same mask over contiguous tensors: q bf16 [batch][n][hq][d], k / v bf16 [batch][n_keys][hkv][d] (strides for all axes but the last);
+ * the queries are the last n of the n_keys positions.  out: bf16 [batch][n][hq][d] contiguous. */
+typedef struct sp_window_attn_args {
+  const void *q, *k, *v;
+  void *out, *workspace;
+  uint64_t workspace_bytes;
+  int64_t batch, n, n_keys, hq, hkv, d, window, sinks;
+  int64_t q_stride_b, q_stride_n, q_stride_h, k_stride_b, k_stride_n, k_stride_h, v_stride_b, v_stride_n, v_stride_h;
+  double softmax_scale;
+  sp_stream_t stream;
+} sp_window_attn_args;
+size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d);
+int sp_window_attn_bf16(const sp_window_attn_args* args /* host */);
+
 /* ---- rotary position embedding in front of the attention function ---------------------------------
  * The reference's patched model produces (cos, sin) per position (model_patch.py:121) and leaves the rotation to
  * the Hugging Face attention layer, which evaluates  x*cos + rotate_half(x)*sin  (rotate_half(x) =

@@ -1,0 +1,203 @@
+// The bookkeeping of a key / value cache in pages: which pages a step's new tokens open and where each of them goes
+// (sp_paged_tables), and the copy of their keys and values there (sp_paged_cache_write_bf16).
+#include "sp_common.h"
+#include "sp_paged_plan.h"
+
+#define PT_THREADS 256
+
+struct TablesArgs {
+  const int32_t *lens, *new_lens;
+  int32_t* table;
+  int64_t table_stride;
+  const int32_t *free_pages, *free_count;
+  int batch, shift, width, num_pages, free_room, max_tokens;
+  int32_t *seq_lens, *cu_new;
+  int64_t* slots;
+  int32_t *positions, *free_left;
+};
+
+// With len, new >= 0 of a request and pages of P tokens, W of them in its row of the table:
+//   have = min(ceil(len / P), W), need = min(ceil((len + new) / P), W) - have;
+// the pages of all requests in order come off the top of the stack, token t of the step belongs to the request whose prefix sum of `new`
+// it lies behind.  Latency is all there is to it (some 130 KB for 256 requests): one launch, and every workgroup forms the two prefix sums over the
+// requests for itself, which costs less than a launch that hands them over.  A new token's slot is taken from the stack itself, not from the
+// table's entry, so nothing that another workgroup of the launch writes is read.
+__global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs a) {
+  extern __shared__ int sh[];  // prefix sums over the requests: [batch + 1] tokens, [batch + 1] pages
+  __shared__ int64_t wave_sums[2][PT_THREADS / SP_WAVE];
+  int* const tok = sh;
+  int* const pgs = sh + a.batch + 1;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, P = 1 << a.shift;
+  const int per = (a.batch + PT_THREADS - 1) / PT_THREADS;
+  auto length = [](int x) { return pg_max(0, pg_min(x, PG_MAX_KEYS - 1)); };
+  auto pages = [&](int n) { return pg_min((int)(((int64_t)n + P - 1) >> a.shift), a.width); };
+  int64_t tokens = 0, opened = 0;
+  for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
+    const int len = length(a.lens[i]), n = length(a.new_lens[i]);
+    tokens += n;
+    opened += pages(len + n) - pages(len);
+  }
+  int64_t tok_at = tokens, page_at = opened;  // inclusive sums over the wave's lanes
+#pragma unroll
+  for (int o = 1; o < SP_WAVE; o <<= 1) {
+    const int64_t x = __shfl_up(tok_at, o, SP_WAVE), y = __shfl_up(page_at, o, SP_WAVE);
+    if (lane >= o) tok_at += x, page_at += y;
+  }
+  if (lane == SP_WAVE - 1) wave_sums[0][wave] = tok_at, wave_sums[1][wave] = page_at;
+  __syncthreads();
+  tok_at -= tokens, page_at -= opened;
+  for (int w = 0; w < wave; ++w) tok_at += wave_sums[0][w], page_at += wave_sums[1][w];
+  auto capped = [](int64_t x) { return (int)(x < PG_MAX_KEYS ? x : PG_MAX_KEYS); };
+  for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
+    const int len = length(a.lens[i]), n = length(a.new_lens[i]);
+    tok[i] = capped(tok_at), pgs[i] = capped(page_at);
+    if (blockIdx.x == 0) a.seq_lens[i] = len + n;
+    tok_at += n, page_at += pages(len + n) - pages(len);
+  }
+  if (t == PT_THREADS - 1) tok[a.batch] = capped(tok_at), pgs[a.batch] = capped(page_at);
+  __syncthreads();
+  const int count = pg_max(0, pg_min(a.free_count[0], a.free_room));
+  if (blockIdx.x == 0) {
+    for (int i = t; i <= a.batch; i += PT_THREADS) a.cu_new[i] = tok[i];
+    if (t == 0) a.free_left[0] = count - pgs[a.batch];  // (below zero: as many pages were missing)
+  }
+  auto from_stack = [&](int i) {  // the i-th page that the step opens
+    const int id = i < count ? a.free_pages[count - 1 - i] : -1;
+    return (unsigned)id < (unsigned)a.num_pages ? id : -1;
+  };
+  auto request = [&](const int* sums, int x) {  // the last request that starts at or in front of x
+    int lo = 0, hi = a.batch;                   // sums[lo] <= x < sums[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (sums[mid] <= x)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  const int gid = blockIdx.x * PT_THREADS + t;
+  for (int i = gid; i < pgs[a.batch]; i += gridDim.x * PT_THREADS) {  // (as many as tokens at most, unless those are capped)
+    const int b = request(pgs, i);
+    a.table[b * a.table_stride + pages(length(a.lens[b])) + (i - pgs[b])] = from_stack(i);
+  }
+  if (gid >= a.max_tokens) return;
+  int64_t slot = -1;
+  int pos = 0;
+  if (gid < tok[a.batch]) {
+    const int b = request(tok, gid), len = length(a.lens[b]);
+    pos = len + (gid - tok[b]);
+    const int page = pos >> a.shift, have = pages(len);
+    if (page < a.width) {
+      int id = page < have ? a.table[b * a.table_stride + page] : from_stack(pgs[b] + page - have);
+      if ((unsigned)id < (unsigned)a.num_pages) slot = ((int64_t)id << a.shift) + (pos & (P - 1));
+    }
+  }
+  a.slots[gid] = slot;
+  a.positions[gid] = pos;
+}
+
+static int page_shift(int32_t page_size) {  // -1: not a page size
+  for (int s = 4; s <= 10; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+
+extern "C" int sp_paged_tables(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t page_size, int32_t num_pages,
+                               int32_t* block_table, int64_t table_stride, int32_t table_width, const int32_t* free_pages,
+                               int32_t free_room, const int32_t* free_count, int32_t max_tokens, int32_t* seq_lens, int32_t* cu_new,
+                               int64_t* slots, int32_t* positions, int32_t* free_left, sp_stream_t stream) {
+  const char* who = "sp_paged_tables";
+  SP_REQUIRE(batch > 0 && table_width > 0 && num_pages >= 0 && free_room >= 0 && max_tokens >= 0, SP_ERR_INVALID_ARGUMENT,
+             "%s: batch=%d table_width=%d num_pages=%d free_room=%d max_tokens=%d", who, batch, table_width, num_pages, free_room, max_tokens);
+  SP_REQUIRE(lens && new_lens && block_table && (free_pages || free_room == 0) && free_count && seq_lens && cu_new && free_left &&
+                 ((slots && positions) || max_tokens == 0),
+             SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE((const void*)seq_lens != lens && (const void*)seq_lens != new_lens && (const void*)free_left != free_count && cu_new != new_lens && cu_new != lens,
+             SP_ERR_INVALID_ARGUMENT, "%s: an output is an input", who);
+  SP_REQUIRE(table_stride >= table_width || batch == 1, SP_ERR_INVALID_ARGUMENT, "%s: rows of %d entries overlap at a stride of %lld", who,
+             table_width, (long long)table_stride);
+  SP_REQUIRE(batch <= PG_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %d (at most %d)", who, batch, PG_MAX_SEQS);
+  const int shift = page_shift(page_size);
+  SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %d (a power of two from 16 to 1024)", who, page_size);
+  SP_REQUIRE(((int64_t)table_width << shift) <= PG_MAX_KEYS && max_tokens <= PG_MAX_KEYS, SP_ERR_UNSUPPORTED,
+             "%s: %d pages a request, %d tokens", who, table_width, max_tokens);
+  const TablesArgs a = {lens, new_lens, block_table, table_stride, free_pages, free_count, batch, shift, table_width, num_pages, free_room,
+                        max_tokens, seq_lens, cu_new, slots, positions, free_left};
+  const unsigned grid = max_tokens > 0 ? (unsigned)sp_ceil_div(max_tokens, PT_THREADS) : 1u;
+  hipLaunchKernelGGL(sp_paged_tables_kernel, dim3(grid), dim3(PT_THREADS), 2 * (batch + 1) * sizeof(int), (hipStream_t)stream, a);
+  SP_LAUNCH_CHECK();
+  return SP_OK;
+}
+
+// ---- new keys and values into their pages ---------------------------------------------------------------------------------
+#define PW_THREADS 256
+#define PW_ITEMS 4
+
+typedef uint32_t pw_u32x4 __attribute__((ext_vector_type(4)));
+
+struct WriteArgs {
+  const sp_bf16 *k, *v;
+  sp_bf16 *k_pages, *v_pages;
+  const int64_t* slots;
+  int64_t items, room;  // 16-byte chunks of k; tokens of the pool
+  int hkv, chunks, shift;
+  int64_t k_n, k_h, v_n, v_h;
+  int64_t kp_p, kp_n, kp_h, vp_p, vp_n, vp_h;
+};
+
+// pages[slot / P][h][slot % P] = x[t][h] for k and v: a copy, HBM-bound.  A thread moves PW_ITEMS chunks of 16 bytes of either, all loads
+// in front of the first store; the chunks of a token's heads lie side by side over the lanes, as projections leave them.
+__global__ __launch_bounds__(PW_THREADS) void sp_paged_write_kernel(WriteArgs a) {
+  const int64_t first = (int64_t)blockIdx.x * (PW_THREADS * PW_ITEMS) + threadIdx.x;
+  pw_u32x4 kx[PW_ITEMS], vx[PW_ITEMS];
+  sp_bf16 *kd[PW_ITEMS], *vd[PW_ITEMS];
+#pragma unroll
+  for (int i = 0; i < PW_ITEMS; ++i) {
+    const int64_t item = first + i * PW_THREADS;
+    kd[i] = vd[i] = nullptr;
+    if (item >= a.items) continue;
+    const int64_t row = item / a.chunks, t = row / a.hkv;  // (token, head)
+    const int c = (int)(item - row * a.chunks) * 8, h = (int)(row - t * a.hkv);
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.room) continue;
+    const int64_t page = slot >> a.shift, in = slot & ((1 << a.shift) - 1);
+    kx[i] = *reinterpret_cast<const pw_u32x4*>(a.k + t * a.k_n + h * a.k_h + c);
+    vx[i] = *reinterpret_cast<const pw_u32x4*>(a.v + t * a.v_n + h * a.v_h + c);
+    kd[i] = a.k_pages + page * a.kp_p + in * a.kp_n + h * a.kp_h + c;
+    vd[i] = a.v_pages + page * a.vp_p + in * a.vp_n + h * a.vp_h + c;
+  }
+#pragma unroll
+  for (int i = 0; i < PW_ITEMS; ++i)
+    if (kd[i] != nullptr) {
+      *reinterpret_cast<pw_u32x4*>(kd[i]) = kx[i];
+      *reinterpret_cast<pw_u32x4*>(vd[i]) = vx[i];
+    }
+}
+
+extern "C" int sp_paged_cache_write_bf16(const void* k, const void* v, int64_t tokens, int32_t hkv, int32_t d, int64_t k_stride_n,
+                                         int64_t k_stride_h, int64_t v_stride_n, int64_t v_stride_h, void* k_pages, void* v_pages,
+                                         int32_t num_pages, int32_t page_size, int64_t k_stride_page, int64_t k_stride_slot,
+                                         int64_t k_stride_page_h, int64_t v_stride_page, int64_t v_stride_slot, int64_t v_stride_page_h,
+                                         const int64_t* slots, sp_stream_t stream) {
+  const char* who = "sp_paged_cache_write_bf16";
+  SP_REQUIRE(tokens >= 0 && hkv > 0 && num_pages >= 0, SP_ERR_INVALID_ARGUMENT, "%s: tokens=%lld hkv=%d num_pages=%d", who,
+             (long long)tokens, hkv, num_pages);
+  SP_REQUIRE(d > 0 && d % 8 == 0, SP_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 8)", who, d);
+  const int shift = page_shift(page_size);
+  SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %d (a power of two from 16 to 1024)", who, page_size);
+  if (tokens == 0 || num_pages == 0) return SP_OK;
+  SP_REQUIRE(k && v && k_pages && v_pages && slots, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 &&
+                 (k_stride_n | k_stride_h | v_stride_n | v_stride_h | k_stride_page | k_stride_slot | k_stride_page_h | v_stride_page |
+                  v_stride_slot | v_stride_page_h) % 8 == 0,
+             SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
+  const int64_t items = tokens * hkv * (d / 8), grid = sp_ceil_div(items, PW_THREADS * PW_ITEMS);
+  SP_REQUIRE(grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: tokens=%lld too many", who, (long long)tokens);
+  const WriteArgs a = {(const sp_bf16*)k, (const sp_bf16*)v, (sp_bf16*)k_pages, (sp_bf16*)v_pages, slots, items, (int64_t)num_pages << shift,
+                       hkv, d / 8, shift, k_stride_n, k_stride_h, v_stride_n, v_stride_h, k_stride_page, k_stride_slot, k_stride_page_h,
+                       v_stride_page, v_stride_slot, v_stride_page_h};
+  hipLaunchKernelGGL(sp_paged_write_kernel, dim3((unsigned)grid), dim3(PW_THREADS), 0, (hipStream_t)stream, a);
+  SP_LAUNCH_CHECK();
+  return SP_OK;
+}

@@ -1,0 +1,69 @@
+// How attention over pages and windows is cut into work (sp_chunk.hip, sp_paged_decode.hip): arithmetic on positions and lengths that the
+// kernels and the host share and a plain C++ compiler takes as well.
+#pragma once
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define PG_FN __host__ __device__ static inline
+#else
+#define PG_FN static inline
+#endif
+
+#define PG_MAX_SEQS 4096           // sequences of a call
+#define PG_MAX_KEYS (1 << 30)      // keys of a sequence: positions and their differences have 31 bits
+#define PG_NO_WINDOW PG_MAX_KEYS   // every key in front of a query lies inside it
+#define PG_TILE 64                 // keys of a tile
+#define PG_ROWS 128                // rows of a row tile: (token, query head of the kv group), the heads of a token side by side
+
+PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
+PG_FN int pg_max(int a, int b) { return a > b ? a : b; }
+
+// The query at position p sees key j: causal, inside its window or among the first `sinks`.
+PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j <= p && (j > p - window || j < sinks); }
+
+// Units of `unit` keys that queries at positions p0 .. p1 see something of, as two runs: [0, front) holds sinks, [lo, hi) the windows.
+struct PgSpan {
+  int front, lo, hi;
+};
+PG_FN int pg_span_units(const PgSpan& s) { return s.front + s.hi - s.lo; }
+PG_FN int pg_span_unit(const PgSpan& s, int i) { return i < s.front ? i : s.lo + (i - s.front); }
+PG_FN PgSpan pg_span(int p0, int p1, int window, int sinks, int unit) {
+  PgSpan s = {0, 0, 0};
+  if (p1 < 0) return s;
+  s.hi = p1 / unit + 1;
+  const int first = p0 - window + 1;  // of the windows
+  s.lo = first > 0 ? first / unit : 0;
+  const int k = pg_min(sinks, p1 + 1);
+  s.front = pg_min((k + unit - 1) / unit, s.lo);
+  return s;
+}
+
+// Row tiles are numbered so that a workgroup finds its own without a scan: those of sequence b, whose tokens start at `start`, begin at
+// floor(start * g / 128) + b.  Every sequence has room for its last, partly filled tile; numbers left over stand for nothing.
+PG_FN int64_t pg_first_slot(int64_t start, int g, int b) { return start * g / PG_ROWS + b; }
+PG_FN int64_t pg_slots(int64_t tokens, int g, int batch) { return tokens * g / PG_ROWS + batch; }
+PG_FN int64_t pg_row_tiles(int64_t q_len, int g) { return (q_len * g + PG_ROWS - 1) / PG_ROWS; }
+
+// Positions of a row tile's first and last row: row r of a sequence is token r / g.
+PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int* p0, int* p1) {
+  const int64_t r0 = (int64_t)rt * PG_ROWS, rows = (int64_t)q_len * g, r1 = r0 + PG_ROWS < rows ? r0 + PG_ROWS : rows;
+  *p0 = len - q_len + (int)(r0 / g);
+  *p1 = len - q_len + (int)((r1 - 1) / g);
+}
+
+// A launch of few row tiles cuts the line of all their tiles, one line per kv head, into equal parts: part p of `parts` starts at unit
+// total * p / parts.  A row tile counts its tiles and PG_OVERHEAD units for its queries, its first loads and its output; a cut within
+// PG_MIN_PART tiles of a row tile's start or end goes there.
+#define PG_OVERHEAD 2
+#define PG_MIN_PART 4
+#define PG_MIN_SHARE 8  // units of a part at least
+PG_FN int64_t pg_parts(int64_t total, int64_t room) {
+  const int64_t parts = (total + PG_MIN_SHARE - 1) / PG_MIN_SHARE;
+  return parts < room ? (parts < 1 ? 1 : parts) : room;
+}
+PG_FN int64_t pg_cut(int64_t total, int64_t parts, int64_t p) { return total / parts * p + total % parts * p / parts; }
+// Where a cut `off` units into a row tile of n tiles stands: tile 0 .. n - 1 of it, or n: the start of what follows.
+PG_FN int pg_snap(int64_t off, int n) {
+  const int64_t t = off - PG_OVERHEAD;
+  return t < PG_MIN_PART ? 0 : t > n - PG_MIN_PART ? n : (int)t;
+}

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -521,6 +521,181 @@ def decode_attention_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, so
         k_n, k_h, v_b, v_n, v_h, softmax_scale, stream))
     if st:
         _lib.check(st, "sp_decode_attn_batch_bf16")
+    return out
+
+
+class PageTables(NamedTuple):
+    """What page_tables finds for a step's new tokens."""
+    seq_lens: torch.Tensor   # int32 [B]: tokens of every request, the new ones included
+    cu_new: torch.Tensor     # int32 [B + 1]: where a request's new tokens start among the step's
+    slots: torch.Tensor      # int64 [T]: page * page_size + place in the page, -1 where there is none
+    positions: torch.Tensor  # int32 [T]: place in the request
+    free_left: torch.Tensor  # int32 [1]: pages left on the stack; below zero: so many were missing
+
+
+def _check_int(t: torch.Tensor, name: str, dtype, shape, device) -> None:
+    if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}, "
+                         f"got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def _check_table(block_table: torch.Tensor, batch: int, device) -> None:
+    if (block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] != batch or block_table.device != device
+            or block_table.shape[1] < 1 or block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows on {device}")
+
+
+def page_tables(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                free_count: torch.Tensor, page_size: int, num_pages: int, max_new_tokens: int) -> PageTables:
+    """The bookkeeping of a serving step over a key / value cache in pages, on the GPU: request b has lens[b] tokens cached and
+    new_lens[b] to come (int32 [B] each).  The pages that the new tokens open come off the top of the stack
+    free_pages[:free_count] (int32 [F], int32 [1]; free_count stays as it is, free_left is what it becomes), in the order of the requests,
+    and are entered into block_table int32 [B, W] in place (-1 where the stack is empty).  max_new_tokens: length of slots and positions;
+    places behind the last new token hold -1 and 0, new tokens beyond it none.
+
+    page_size: a power of two from 16 to 1024; at most 4096 requests.  Nothing synchronises: lengths may change under a captured graph."""
+    lib = _lib.load()
+    if not lens.is_cuda:
+        raise ValueError("lens must live on the GPU")
+    dev, batch = lens.device, lens.shape[0] if lens.dim() == 1 else -1
+    _check_int(lens, "lens", torch.int32, (max(batch, 0),), dev)
+    _check_int(new_lens, "new_lens", torch.int32, (batch,), dev)
+    _check_int(free_pages, "free_pages", torch.int32, (free_pages.numel(),), dev)
+    _check_int(free_count, "free_count", torch.int32, (1,), dev)
+    _check_table(block_table, batch, dev)
+    if max_new_tokens < 0:
+        raise ValueError(f"max_new_tokens {max_new_tokens}")
+    stream = _stream_handle(dev)
+    seq_lens, cu_new, free_left, positions = torch.empty(2 * batch + 2 + max_new_tokens, dtype=torch.int32, device=dev).split(
+        [batch, batch + 1, 1, max_new_tokens])
+    slots = torch.empty(max_new_tokens, dtype=torch.int64, device=dev)
+    st = lib.sp_paged_tables(lens.data_ptr(), new_lens.data_ptr(), batch, page_size, num_pages, block_table.data_ptr(), block_table.stride(0),
+                             block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), max_new_tokens,
+                             seq_lens.data_ptr(), cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_left.data_ptr(), stream)
+    _lib.check(st, "sp_paged_tables")
+    return PageTables(seq_lens, cu_new, slots, positions, free_left)
+
+
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, d: int, device) -> None:
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [num_pages, Hkv, page_size, D], got {tuple(t.shape)}")
+        if t.dtype is not torch.bfloat16:
+            raise AssertionError(f"{name} must be bfloat16, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} must live on {device}")
+        if t.stride(3) != 1:
+            raise ValueError(f"{name} must have a contiguous head_dim axis")
+    if k_pages.shape != v_pages.shape or k_pages.shape[3] != d:
+        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must agree, with head_dim {d}")
+
+
+def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor) -> None:
+    """Copies a step's keys and values, bf16 [Hkv, T, D] views, to their slots (int64 [T], page_tables) of the pools, bf16
+    [num_pages, Hkv, page_size, D] views with any strides and a contiguous head_dim axis.  Tokens whose slot is outside the pool are left out.
+    Slots must differ from each other: of two tokens with the same one the pool keeps parts of either."""
+    lib = _lib.load()
+    _check_hnd(k, "k")
+    _check_hnd(v, "v")
+    hkv, n, d = k.shape
+    if v.shape != k.shape or v.device != k.device:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must agree")
+    _check_pages(k_pages, v_pages, d, k.device)
+    pages, heads, page_size, _ = k_pages.shape
+    if heads != hkv:
+        raise ValueError(f"the pools hold {heads} heads, k has {hkv}")
+    _check_int(slots, "slots", torch.int64, (n,), k.device)
+    (k_h, k_n, _), (v_h, v_n, _) = k.stride(), v.stride()
+    (kp_p, kp_h, kp_n, _), (vp_p, vp_h, vp_n, _) = k_pages.stride(), v_pages.stride()
+    st = lib.sp_paged_cache_write_bf16(k.data_ptr(), v.data_ptr(), n, hkv, d, k_n, k_h, v_n, v_h, k_pages.data_ptr(), v_pages.data_ptr(), pages,
+                                       page_size, kp_p, kp_n, kp_h, vp_p, vp_n, vp_h, slots.data_ptr(), _stream_handle(k.device))
+    _lib.check(st, "sp_paged_cache_write_bf16")
+
+
+def _window_of(window: Optional[int], sinks: int) -> int:
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1 (None: no window), got {window}")
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
+    return 0 if window is None else window
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    softmax_scale: float, cu_q: Optional[torch.Tensor] = None, window: Optional[int] = None, sinks: int = 0,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of new tokens over a cache in pages that holds them and everything in front of them: q bf16 [Hq, T, D] view, the requests'
+    tokens one behind the other, pools bf16 [num_pages, Hkv, page_size, D] views -> out bf16 [T, Hq, D].
+
+    Request b has rows cu_q[b] .. cu_q[b + 1] of q (int32 [B + 1]; None: one row each, T == B) and seq_lens[b] keys (int32 [B]), those
+    in the pages that block_table[b] (int32 [B, W]) names; its rows are its last positions.  A row at position p sees keys j <= p and,
+    with a window, of those j > p - window and j < sinks.  Keys without a page (an entry outside the pool) are not seen; a row that sees
+    nothing is zero.  Rows of `out` outside every request stay as they were (undefined in a tensor made here).
+    head_dim 64 or 128, page_size a power of two from 16 to 1024, at most 4096 requests.  Lengths and pages are read on the device."""
+    lib = _lib.load()
+    _check_hnd(q, "q")
+    hq, n, d = q.shape
+    dev = q.device
+    _check_pages(k_pages, v_pages, d, dev)
+    pages, hkv, page_size, _ = k_pages.shape
+    batch = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
+    _check_int(seq_lens, "seq_lens", torch.int32, (max(batch, 0),), dev)
+    _check_table(block_table, batch, dev)
+    if cu_q is not None:
+        _check_int(cu_q, "cu_q", torch.int32, (batch + 1,), dev)
+    elif n != batch:
+        raise ValueError(f"without cu_q every request has one row: q has {n}, seq_lens {batch}")
+    span = _window_of(window, sinks)
+    stream = _stream_handle(dev)
+    if out is None:
+        out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
+    elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (n, hq, d) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bfloat16 [{n}, {hq}, {d}] tensor on {dev}")
+    need = lib.sp_paged_attn_workspace_bytes(n, batch, hq, hkv, d)
+    # a buffer of this call's own: graphs captured on one stream may be replayed on two, so they must not meet in a kept one
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    (q_h, q_n, _), (k_p, k_h, k_n, _), (v_p, v_h, v_n, _) = q.stride(), k_pages.stride(), v_pages.stride()
+    st = lib.sp_paged_attn_bf16(_lib.PAGED_ATTN_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+        out.data_ptr(), 0 if ws is None else ws.data_ptr(), need, n, batch, hq, hkv, d, pages, page_size, block_table.shape[1],
+        block_table.stride(0), span, sinks, q_n, q_h, k_p, k_n, k_h, v_p, v_n, v_h, softmax_scale, stream))
+    _lib.check(st, "sp_paged_attn_bf16")
+    return out
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, window: Optional[int] = None,
+                     sinks: int = 0) -> torch.Tensor:
+    """Causal attention in a sliding window with the first `sinks` tokens kept in sight: q bf16 [B, Hq, N, D], k / v bf16 [B, Hkv, Nk, D]
+    views, N <= Nk, the queries being the last N positions -> out bf16 [B, N, Hq, D].  The query at position p sees keys j <= p with
+    j > p - window or j < sinks; window None: all j <= p (a prompt's next chunk over a contiguous cache).
+
+    Prompts (N = Nk), chunks and single tokens (N = 1) alike; head_dim 64 or 128, any strides with a contiguous head_dim axis."""
+    lib = _lib.load()
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [B, H, N, D], got {tuple(t.shape)}")
+        if t.dtype is not torch.bfloat16:
+            raise AssertionError(f"{name} must be bfloat16, got {t.dtype}")
+        if not t.is_cuda or t.device != q.device:
+            raise ValueError(f"{name} must live on the GPU the queries are on")
+        if t.stride(3) != 1:
+            raise ValueError(f"{name} must have a contiguous head_dim axis")
+    b, hq, n, d = q.shape
+    _, hkv, nk, _ = k.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    if n > nk:
+        raise ValueError(f"{n} queries are more than the {nk} positions there are")
+    span = _window_of(window, sinks)
+    dev = q.device
+    stream = _stream_handle(dev)
+    out = torch.empty(b, n, hq, d, dtype=torch.bfloat16, device=dev)
+    need = lib.sp_window_attn_workspace_bytes(b, n, nk, hq, hkv, d)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
+    (q_b, q_h, q_n, _), (k_b, k_h, k_n, _), (v_b, v_h, v_n, _) = q.stride(), k.stride(), v.stride()
+    st = lib.sp_window_attn_bf16(_lib.WINDOW_ATTN_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if ws is None else ws.data_ptr(), need, b, n, nk, hq, hkv, d, span, sinks,
+        q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, softmax_scale, stream))
+    _lib.check(st, "sp_window_attn_bf16")
     return out
 
 

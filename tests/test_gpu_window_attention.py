@@ -1,0 +1,121 @@
+"""Sliding-window attention with sinks over contiguous keys and values against its definition in 64 bits (paged_reference.py)."""
+
+import pytest
+import torch
+
+from paged_reference import check, default_scale, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _run(dev, batch, n, nk, hq, hkv, d, window, sinks, seed=0, token_major=True):
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(seed)
+
+    def make(heads, length):
+        if token_major:
+            return torch.randn(batch, length, heads, d, generator=gen).to(torch.bfloat16).transpose(1, 2)
+        return torch.randn(batch, heads, length, d, generator=gen).to(torch.bfloat16)
+
+    q, k, v = make(hq, n), make(hkv, nk), make(hkv, nk)
+    got = ops.window_attention(q.to(dev), k.to(dev), v.to(dev), default_scale(d), window=window or None, sinks=sinks).cpu()
+    assert got.shape == (batch, n, hq, d)
+    for b in range(batch):
+        check(got[b], *reference(q[b], k[b], v[b], default_scale(d), window, sinks), f"sequence {b}")
+
+
+@pytest.mark.parametrize("n,nk", [(1, 1), (7, 7), (64, 64), (65, 65), (200, 200), (50, 170), (1, 130), (33, 300)])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (7, 1, 64), (2, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (16, 4), (64, 0), (100, 70)])
+def test_prompts_and_chunks_match_the_definition(gpu_device, n, nk, hq, hkv, d, window, sinks):
+    _run(gpu_device, 2, n, nk, hq, hkv, d, window, sinks, seed=n + nk)
+
+
+@pytest.mark.parametrize("nk", [1, 31, 32, 33, 64, 500, 4000])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (14, 2, 64), (32, 2, 128), (34, 2, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 2), (40, 4), (1000, 33)])
+def test_single_tokens_match_the_definition(gpu_device, nk, hq, hkv, d, window, sinks):
+    _run(gpu_device, 3, 1, nk, hq, hkv, d, window, sinks, seed=nk, token_major=False)
+
+
+def test_a_long_prompt_in_rows_spread_over_many_workgroups(gpu_device):
+    """Enough row tiles that no cut is needed, and a few rows of them checked."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(1)
+    n, hq, hkv, d = 9001, 32, 8, 128
+    q, k, v = (torch.randn(n, h, d, generator=gen).to(torch.bfloat16).transpose(0, 1) for h in (hq, hkv, hkv))
+    for window, sinks in ((700, 4), (0, 0)):
+        got = ops.window_attention(*(t[None].to(gpu_device) for t in (q, k, v)), default_scale(d), window=window or None, sinks=sinks)[0].cpu()
+        for p in (0, 1, 63, 64, 699, 700, 703, 704, 4095, 8999, 9000):
+            want, bound = reference(q[:, p:p + 1], k[:, :p + 1], v[:, :p + 1], default_scale(d), window, sinks)
+            check(got[p:p + 1], want, bound, f"position {p}")
+
+
+def test_every_row_is_the_mean_of_what_it_sees(gpu_device):
+    """With q = 0 all weights are equal: every row of a long prompt in closed form.  The weights are powers of two and sums of them, exact, so
+    what is left is the output's rounding and fp32 sums of up to n values, and the division's rounding."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(1)
+    for n, hq, hkv, d, window, sinks in ((6000, 28, 4, 128, 1000, 70), (5003, 4, 1, 64, 0, 0), (3333, 8, 8, 64, 65, 1)):
+        q = torch.zeros(1, hq, n, d, dtype=torch.bfloat16, device=gpu_device)
+        k = torch.randn(1, hkv, n, d, generator=gen).to(torch.bfloat16).to(gpu_device)
+        v = torch.randn(1, hkv, n, d, generator=gen).to(torch.bfloat16).to(gpu_device)
+        got = ops.window_attention(q, k, v, 0.1, window=window or None, sinks=sinks)[0].double()
+        sums = torch.cat((torch.zeros(hkv, 1, d, device=gpu_device, dtype=torch.float64), v[0].double().cumsum(1)), 1)
+        p = torch.arange(n, device=gpu_device)
+        lo = (p - (window or n + 1) + 1).clamp(min=0)
+        front = torch.minimum(lo, torch.full_like(lo, sinks))
+        total = sums[:, p + 1] - sums[:, lo] + sums[:, front]
+        want = (total / (p + 1 - lo + front)[None, :, None]).transpose(0, 1).repeat_interleave(hq // hkv, 1)
+        mean_abs = v.double().abs().mean().item()
+        err = (got - want).abs()
+        assert (err <= want.abs() * 2.0 ** -8 * 1.01 + n * 2.0 ** -24 * mean_abs).all(), (n, window, err.max().item())
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_out_of_sight_do_not_matter(gpu_device, bad):
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(3)
+    n, hq, hkv, d, window = 140, 4, 2, 128, 30
+    q, k, v = (torch.randn(h, n, d, generator=gen).to(torch.bfloat16) for h in (hq, hkv, hkv))
+    k[:, 50] = bad
+    v[:, 50] = bad
+    got = ops.window_attention(*(t[None].to(gpu_device) for t in (q, k, v)), default_scale(d), window=window)[0].cpu()
+    want, bound = reference(q, k, v, default_scale(d), window, 0)
+    clean = (torch.arange(n) < 50) | (torch.arange(n) >= 80)
+    check(got[clean], want[clean], bound[clean])
+    assert not torch.isfinite(got[~clean].float()).any()
+    # the next token: position 139 does not see it
+    one = ops.window_attention(q[None, :, -1:].to(gpu_device), k[None].to(gpu_device), v[None].to(gpu_device), default_scale(d), window=window)[0].cpu()
+    check(one, want[-1:], bound[-1:])
+
+
+def test_a_window_as_long_as_the_prompt_is_none(gpu_device):
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(1, h, 333, 64, generator=gen).to(torch.bfloat16).to(gpu_device) for h in (6, 3, 3))
+    a = ops.window_attention(q, k, v, 0.1)
+    for window, sinks in ((333, 0), (10 ** 12, 5), (1, 333), (5, 10 ** 12)):
+        assert torch.equal(a, ops.window_attention(q, k, v, 0.1, window=window, sinks=sinks))
+
+
+def test_empty_and_refused_calls(gpu_device):
+    from shareprefill_amd import ops
+
+    make = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=gpu_device)
+    assert ops.window_attention(make(2, 4, 0, 64), make(2, 2, 5, 64), make(2, 2, 5, 64), 0.1, window=3).shape == (2, 0, 4, 64)
+    assert ops.window_attention(make(2, 4, 0, 64), make(2, 2, 0, 64), make(2, 2, 0, 64), 0.1, window=3).shape == (2, 0, 4, 64)
+    q, k = make(1, 4, 8, 64), make(1, 2, 8, 64)
+    for error, args, kw in [
+        (ValueError, (make(1, 4, 9, 64), k, k), {}), (ValueError, (q, k, k[:, :1]), {}), (ValueError, (make(2, 4, 8, 64), k, k), {}),
+        (ValueError, (q[0], k, k), {}), (AssertionError, (q.half(), k, k), {}), (ValueError, (q.cpu(), k, k), {}), (ValueError, (q, k, k.cpu()), {}),
+        (ValueError, (make(1, 3, 8, 64), k, k), {}), (ValueError, (q, k, k), dict(window=0)), (ValueError, (q, k, k), dict(sinks=-2)),
+        (ValueError, (q.transpose(2, 3).contiguous().transpose(2, 3), k, k), {}),
+        (NotImplementedError, (make(1, 4, 8, 96), make(1, 2, 8, 96), make(1, 2, 8, 96)), {})]:
+        with pytest.raises(error):
+            ops.window_attention(*args, 0.1, **kw)

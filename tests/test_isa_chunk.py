@@ -1,0 +1,15 @@
+"""CPU-only checks of the generated code of the chunk attention kernel, whose operands are read by LDS reads in inline assembly as the
+short-prompt kernel's are (test_isa_hazards.py, test_isa_operand_reads.py)."""
+
+from test_isa_hazards import _kernels, touched_in_flight
+from test_isa_operand_reads import _inline_reads_as_transposing
+
+
+def test_nothing_touches_a_read_in_flight_in_the_chunk_kernel():
+    kernels = _kernels("sp_chunk.hip", "sp_chunk_kernel")
+    assert len(kernels) == 4, "64 / 128 channels x pages / contiguous"
+    for name, body in kernels.items():
+        for lines, least in ((_inline_reads_as_transposing(body), 8), (body, 16)):
+            count, found = touched_in_flight(lines)
+            assert count >= least
+            assert not found, f"{name}: '{found[0][1]}' while '{found[0][0]}' is in flight"
