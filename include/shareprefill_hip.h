@@ -383,7 +383,8 @@ typedef struct sp_paged_attn_args {
   double softmax_scale;
   sp_stream_t stream;
 } sp_paged_attn_args;
-size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d);
+/* single_tokens: for calls without cu_q */
+size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens);
 int sp_paged_attn_bf16(const sp_paged_attn_args* args /* host */);
 
 /* The same mask over contiguous tensors: q bf16 [batch][n][hq][d], k / v bf16 [batch][n_keys][hkv][d] (strides for all axes but the last);

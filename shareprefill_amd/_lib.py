@@ -101,7 +101,7 @@ SIGNATURES = {
     "sp_paged_tables": (_I32, [_P, _P, _I32, _I32, _I32, _P, _I64, _I32, _P, _I32, _P, _I32, _P, _P, _P, _P, _P, _P]),
     "sp_paged_cache_write_bf16": (_I32, [_P, _P, _I64, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _I32, _I64, _I64, _I64,
                                          _I64, _I64, _I64, _P, _P]),
-    "sp_paged_attn_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32]),
+    "sp_paged_attn_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32]),
     "sp_paged_attn_bf16": (_I32, [C.c_char_p]),  # (PAGED_ATTN_ARGS.pack(...))
     "sp_window_attn_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I32, _I32, _I32]),
     "sp_window_attn_bf16": (_I32, [C.c_char_p]),  # (WINDOW_ATTN_ARGS.pack(...))

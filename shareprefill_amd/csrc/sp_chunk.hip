@@ -14,49 +14,10 @@
 //   * where a launch has few row tiles their tiles form a line that is cut into equal parts, one workgroup each (sp_paged_plan.h): every CU
 //     has as much to do as the others, whatever the sequences' lengths, which only the device knows.  A row tile that a cut goes through
 //     leaves fp32 partials that a second launch merges; the lengths need no host, so the call can be captured into a graph.
-#include "sp_paged_plan.h"
+#include "sp_chunk.h"
 #include "sp_tiles.h"
 
-struct CkArgs {
-  const sp_bf16 *q, *k, *v;
-  const int32_t* table;     // [batch][width] pages of 1 << shift keys; null: page i of a sequence is its keys i << shift ..
-  const int32_t *lens, *cu;  // per sequence, or null: n_keys keys and n_queries queries each
-  sp_bf16* out;             // [tokens][hq][D]
-  int64_t table_stride;
-  int64_t sq_b, sq_n, sq_h, sk_b, sk_p, sk_n, sk_h, sv_b, sv_p, sv_n, sv_h;  // elements; _b between sequences, _p between pages
-  int batch, tokens, width, num_pages, shift, n_keys, n_queries;
-  int hkv, group, window, sinks;
-  int slots, parts;         // row tiles per kv head; parts of their line at most, or 0: a workgroup per row tile
-  float scale_log2;
-  float* o_part;            // [workgroup][2][128][D]: its first row tile where that began in an earlier part, its last where that goes on
-  float2* ml_part;          // [workgroup][2][128]
-  int4* notes;              // [workgroup]
-};
-// notes of a workgroup: x: its first row tile's part is 0 no partial, 1 the last of the row tile, 2 one in the middle;
-// y: >= 0: its last row tile starts here and goes on in the next part: sequence y, row tile z
-#define CK_NONE 0
-#define CK_LAST 1
-#define CK_MIDDLE 2
-
 #define CK_LDS_BYTES(D) (4 * AS_TILE * (D) * 2)
-
-__device__ __forceinline__ int ck_start(const CkArgs& a, int b) {
-  return a.cu != nullptr ? pg_max(0, pg_min(a.cu[b], a.tokens)) : b * a.n_queries;
-}
-__device__ __forceinline__ int ck_len(const CkArgs& a, int b) { return a.lens != nullptr ? pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS)) : a.n_keys; }
-
-// tiles that a row tile sees something of; none behind the table's last page
-__device__ __forceinline__ PgSpan ck_span(const CkArgs& a, int rt, int q_len, int len) {
-  int p0, p1;
-  pg_tile_positions(rt, q_len, len, a.group, &p0, &p1);
-  PgSpan s = pg_span(p0, p1, a.window, a.sinks, PG_TILE);
-  if (a.table != nullptr) {
-    s.hi = pg_min(s.hi, (int)((((int64_t)a.width << a.shift) + PG_TILE - 1) / PG_TILE));
-    s.lo = pg_min(s.lo, s.hi);
-    s.front = pg_min(s.front, s.lo);
-  }
-  return s;
-}
 
 // the sequence that row tile number x belongs to, by 64 candidates at a time
 __device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
@@ -117,7 +78,9 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
         while (b + 1 < a.batch && pg_first_slot(cu_s[b + 1], a.group, b + 1) <= i) ++b;
         const int q_len = pg_max(0, cu_s[b + 1] - cu_s[b]), rt = (int)(i - pg_first_slot(cu_s[b], a.group, b));
         if (rt < 0 || rt >= pg_row_tiles(q_len, a.group)) continue;
-        const int tiles = pg_span_units(ck_span(a, rt, q_len, len_s[b]));
+        int p0, p1;
+        pg_tile_positions(rt, q_len, len_s[b], a.group, &p0, &p1);
+        const int tiles = pg_span_units(ck_span(a, p0, p1, PG_TILE));
         visit(i, tiles + PG_OVERHEAD, tiles);
       }
     };
@@ -139,13 +102,13 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
       total += wave_sums[w];
     }
     at -= mine;
-    const int64_t parts = pg_parts(total, a.parts);
+    const int64_t parts = pg_parts(total, a.parts, PG_MIN_SHARE);
     const int64_t cut[2] = {part < parts ? pg_cut(total, parts, part) : total, part < parts ? pg_cut(total, parts, part + 1) : total};
     walk([&](int i, int units, int tiles) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (cut[e] >= at && cut[e] < at + units) {
-          const int tile = pg_snap(cut[e] - at, tiles);
+          const int tile = pg_snap(cut[e] - at, tiles, PG_OVERHEAD);
           found[e][0] = tile < tiles || tile == 0 ? i : i + 1;
           found[e][1] = tile < tiles ? tile : 0;
         }
@@ -177,7 +140,9 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
     const int rt = (int)(x - pg_first_slot(start, a.group, b));
     const int rows = q_len * a.group - rt * PG_ROWS;  // from here to the sequence's end
     if (rt < 0 || rows <= 0) continue;
-    const PgSpan span = ck_span(a, rt, q_len, len);
+    int p0, p1;
+    pg_tile_positions(rt, q_len, len, a.group, &p0, &p1);
+    const PgSpan span = ck_span(a, p0, p1, PG_TILE);
     const int tiles = pg_span_units(span);
     const int i_end = x == x_end ? pg_min(tile_end, tiles) : tiles;
     const bool from_start = tile_begin == 0, to_end = i_end == tiles;  // (uniform)
@@ -517,54 +482,6 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
   if (a.parts != 0 && t == 0) a.notes[blockIdx.x] = note;
 }
 
-// Row tiles that cuts went through: the workgroup whose part such a row tile starts in has noted it, those of the following parts that they
-// hold a middle or the last of it.  grid (workgroups of the main launch, bands of 16 rows); sixteen threads a row, the parts in order.
-#define CM_ROWS 16
-template <int D>
-__global__ __launch_bounds__(AS_THREADS) void sp_chunk_merge_kernel(const CkArgs a, int workgroups) {
-  const int4 note = a.notes[blockIdx.x];
-  if (note.y < 0) return;
-  const int b = note.y, rt = note.z, t = threadIdx.x, lane = t & 63;
-  const int kvh = blockIdx.x % a.hkv;
-  const int start = ck_start(a, b), q_len = pg_max(0, ck_start(a, b + 1) - start);
-  const int rows = pg_min(q_len * a.group - rt * PG_ROWS, PG_ROWS), row0 = blockIdx.y * CM_ROWS;
-  if (row0 >= rows) return;
-  int more = 0;  // parts behind the first
-  for (;;) {
-    const int64_t w = blockIdx.x + (int64_t)(more + 1 + lane) * a.hkv;
-    const uint64_t ends = __ballot(w >= workgroups || a.notes[w < workgroups ? w : 0].x != CK_MIDDLE);
-    if (ends != 0ull) {
-      more += __builtin_ctzll(ends) + 1;
-      break;
-    }
-    more += SP_WAVE;
-  }
-  const int row = row0 + (t >> 4), c0 = (t & 15) * 4;
-  if (row >= rows) return;
-  auto slab = [&](int i) { return i == 0 ? (int64_t)blockIdx.x * 2 + 1 : ((int64_t)blockIdx.x + (int64_t)i * a.hkv) * 2; };
-  float top = AS_NO_MAX;
-  for (int i = 0; i <= more; ++i) top = fmaxf(top, a.ml_part[slab(i) * PG_ROWS + row].x);
-  as_floatx4 acc[D / 64];
-  float sum = 0.f;
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c) acc[c] = (as_floatx4){0, 0, 0, 0};
-#pragma unroll 4
-  for (int i = 0; i <= more; ++i) {
-    const float2 ml = a.ml_part[slab(i) * PG_ROWS + row];
-    const float w = __builtin_amdgcn_exp2f(ml.x - top);
-    sum += ml.y * w;
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c)
-      acc[c] += *reinterpret_cast<const as_floatx4*>(a.o_part + (slab(i) * PG_ROWS + row) * D + 64 * c + c0) * w;
-  }
-  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-  const int r = rt * PG_ROWS + row, token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
-  sp_bf16* dst = a.out + ((int64_t)(start + token) * (a.hkv * a.group) + head) * D + c0;
-#pragma unroll
-  for (int c = 0; c < D / 64; ++c)
-    *reinterpret_cast<uint2*>(dst + 64 * c) = make_uint2(as_pack2(acc[c][0] * inv, acc[c][1] * inv), as_pack2(acc[c][2] * inv, acc[c][3] * inv));
-}
-
 // ---- host -------------------------------------------------------------------------------------------------
 struct CkPlan {
   int64_t slots, grid;
@@ -586,8 +503,7 @@ static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int3
   return p.parts == 0 ? 0 : (size_t)p.grid * (2 * PG_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
-static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, float softmax_scale, void* workspace, size_t workspace_bytes,
-                     hipStream_t s) {
+static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* workspace, size_t workspace_bytes, hipStream_t s) {
   const CkPlan plan = ck_plan(a.tokens, a.batch, a.hkv, a.group, d);
   SP_REQUIRE(plan.grid <= 0x7fffffffll && (int64_t)a.tokens * a.group < (1ll << 31), SP_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are too many",
              who, a.tokens, hq);
@@ -596,7 +512,6 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, float so
              "%s: workspace too small or misaligned", who);
   a.slots = (int)plan.slots;
   a.parts = plan.parts;
-  a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.o_part = (float*)workspace;
   a.ml_part = (float2*)(a.o_part + (size_t)plan.grid * 2 * PG_ROWS * d);
   a.notes = (int4*)(a.ml_part + (size_t)plan.grid * 2 * PG_ROWS);
@@ -604,7 +519,7 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, float so
   const size_t lds = plan_lds > (size_t)CK_LDS_BYTES(d) ? plan_lds : (size_t)CK_LDS_BYTES(d);
   auto go = [&](auto kernel, auto merge) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(AS_THREADS), lds, s, a);
-    if (plan.parts != 0) hipLaunchKernelGGL(merge, dim3((unsigned)plan.grid, PG_ROWS / CM_ROWS), dim3(AS_THREADS), 0, s, a, (int)plan.grid);
+    if (plan.parts != 0) hipLaunchKernelGGL(merge, dim3((unsigned)plan.grid, PG_ROWS / CM_ROWS), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
   };
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -617,9 +532,9 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, float so
     attr_set[dev] = true;
   }
   if (d == 64)
-    a.table != nullptr ? go(sp_chunk_kernel<64, true>, sp_chunk_merge_kernel<64>) : go(sp_chunk_kernel<64, false>, sp_chunk_merge_kernel<64>);
+    a.table != nullptr ? go(sp_chunk_kernel<64, true>, sp_chunk_merge_kernel<64, PG_ROWS>) : go(sp_chunk_kernel<64, false>, sp_chunk_merge_kernel<64, PG_ROWS>);
   else
-    a.table != nullptr ? go(sp_chunk_kernel<128, true>, sp_chunk_merge_kernel<128>) : go(sp_chunk_kernel<128, false>, sp_chunk_merge_kernel<128>);
+    a.table != nullptr ? go(sp_chunk_kernel<128, true>, sp_chunk_merge_kernel<128, PG_ROWS>) : go(sp_chunk_kernel<128, false>, sp_chunk_merge_kernel<128, PG_ROWS>);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
@@ -637,7 +552,9 @@ static int ck_window(int64_t window) { return window == 0 || window > PG_NO_WIND
 // offsets inside the rows of a load have 32 bits
 static bool ck_rows_ok(int64_t stride_n) { return stride_n >= 0 && stride_n < (1ll << 24) && stride_n % 8 == 0; }
 
-extern "C" size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d) {
+extern "C" size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens) {
+  if (single_tokens && tokens > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128))
+    return pd_workspace_bytes(hkv, d);
   return ck_workspace_bytes(tokens, batch, hq, hkv, d);
 }
 
@@ -675,12 +592,14 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   a.batch = (int)x->batch, a.tokens = (int)x->tokens, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
   a.n_queries = 1;
   a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.window = ck_window(x->window), a.sinks = (int)(x->sinks < PG_MAX_KEYS ? x->sinks : PG_MAX_KEYS);
-  return ck_launch(who, a, (int)x->hq, (int)x->d, (float)x->softmax_scale, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
+  a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
+  if (pd_takes(a)) return pd_launch(who, a, x->table_width << shift, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
+  return ck_launch(who, a, (int)x->hq, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
 }
 
 extern "C" size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d) {
   (void)n_keys;
-  return batch <= 0 || n <= 0 ? 0 : ck_workspace_bytes(batch * n, batch, hq, hkv, d);
+  return batch <= 0 || n <= 0 ? 0 : sp_paged_attn_workspace_bytes(batch * n, batch, hq, hkv, d, n == 1);
 }
 
 extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
@@ -708,5 +627,7 @@ extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
   a.sv_b = x->v_stride_b, a.sv_n = x->v_stride_n, a.sv_h = x->v_stride_h, a.sv_p = x->v_stride_n << a.shift;
   a.batch = (int)x->batch, a.tokens = (int)(x->batch * x->n), a.n_keys = (int)x->n_keys, a.n_queries = (int)x->n;
   a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.window = ck_window(x->window), a.sinks = (int)(x->sinks < PG_MAX_KEYS ? x->sinks : PG_MAX_KEYS);
-  return ck_launch(who, a, (int)x->hq, (int)x->d, (float)x->softmax_scale, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
+  a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
+  if (pd_takes(a)) return pd_launch(who, a, x->n_keys, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
+  return ck_launch(who, a, (int)x->hq, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
 }

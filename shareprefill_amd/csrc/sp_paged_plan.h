@@ -57,13 +57,13 @@ PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int* p0, int* p1
 #define PG_OVERHEAD 2
 #define PG_MIN_PART 4
 #define PG_MIN_SHARE 8  // units of a part at least
-PG_FN int64_t pg_parts(int64_t total, int64_t room) {
-  const int64_t parts = (total + PG_MIN_SHARE - 1) / PG_MIN_SHARE;
+PG_FN int64_t pg_parts(int64_t total, int64_t room, int share) {
+  const int64_t parts = (total + share - 1) / share;
   return parts < room ? (parts < 1 ? 1 : parts) : room;
 }
 PG_FN int64_t pg_cut(int64_t total, int64_t parts, int64_t p) { return total / parts * p + total % parts * p / parts; }
 // Where a cut `off` units into a row tile of n tiles stands: tile 0 .. n - 1 of it, or n: the start of what follows.
-PG_FN int pg_snap(int64_t off, int n) {
-  const int64_t t = off - PG_OVERHEAD;
+PG_FN int pg_snap(int64_t off, int n, int overhead) {
+  const int64_t t = off - overhead;
   return t < PG_MIN_PART ? 0 : t > n - PG_MIN_PART ? n : (int)t;
 }

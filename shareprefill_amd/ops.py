@@ -650,7 +650,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
     elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (n, hq, d) or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out must be a contiguous bfloat16 [{n}, {hq}, {d}] tensor on {dev}")
-    need = lib.sp_paged_attn_workspace_bytes(n, batch, hq, hkv, d)
+    need = lib.sp_paged_attn_workspace_bytes(n, batch, hq, hkv, d, cu_q is None)
     # a buffer of this call's own: graphs captured on one stream may be replayed on two, so they must not meet in a kept one
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     (q_h, q_n, _), (k_p, k_h, k_n, _), (v_p, v_h, v_n, _) = q.stride(), k_pages.stride(), v_pages.stride()

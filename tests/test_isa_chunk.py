@@ -13,3 +13,13 @@ def test_nothing_touches_a_read_in_flight_in_the_chunk_kernel():
             count, found = touched_in_flight(lines)
             assert count >= least
             assert not found, f"{name}: '{found[0][1]}' while '{found[0][0]}' is in flight"
+
+
+def test_nothing_touches_a_read_in_flight_in_the_single_token_kernel():
+    kernels = _kernels("sp_paged_decode.hip", "sp_paged_decode_kernel")
+    assert len(kernels) == 4, "64 / 128 channels x pages / contiguous"
+    for name, body in kernels.items():
+        for lines, least in ((_inline_reads_as_transposing(body), 4), (body, 8)):
+            count, found = touched_in_flight(lines)
+            assert count >= least
+            assert not found, f"{name}: '{found[0][1]}' while '{found[0][0]}' is in flight"

@@ -22,9 +22,9 @@ int main() {
     } else if (what == 'f') {
       printf("%ld %ld %ld\\n", (long)pg_first_slot(a, (int)b, (int)c), (long)pg_slots(a, (int)b, (int)c), (long)pg_row_tiles(a, (int)b));
     } else if (what == 'c') {
-      printf("%ld %ld\\n", (long)pg_parts(a, b), (long)pg_cut(a, pg_parts(a, b), c));
+      printf("%ld %ld\\n", (long)pg_parts(a, b, 8), (long)pg_cut(a, pg_parts(a, b, 8), c));
     } else if (what == 'n') {
-      printf("%d\\n", pg_snap(a, (int)b));
+      printf("%d\\n", pg_snap(a, (int)b, 2));
     } else {
       int p0, p1;
       pg_tile_positions((int)a, (int)b, (int)c, (int)d, &p0, &p1);

@@ -63,8 +63,8 @@ def test_nothing_to_do_is_no_error():
     assert _paged(tokens=0, q=0, out=0, workspace=0, workspace_bytes=0) == 0
     assert _window(n=0, q=0, out=0, workspace=0, workspace_bytes=0) == 0
     lib = _lib.load()
-    assert lib.sp_paged_attn_workspace_bytes(0, 4, 8, 2, 128) == 0 == lib.sp_window_attn_workspace_bytes(0, 4, 4, 8, 2, 128)
-    assert lib.sp_paged_attn_workspace_bytes(4, 4, 7, 2, 128) == 0
+    assert lib.sp_paged_attn_workspace_bytes(0, 4, 8, 2, 128, 0) == 0 == lib.sp_window_attn_workspace_bytes(0, 4, 4, 8, 2, 128)
+    assert lib.sp_paged_attn_workspace_bytes(4, 4, 7, 2, 128, 1) == 0
 
 
 def test_tables_and_writes_refuse():
