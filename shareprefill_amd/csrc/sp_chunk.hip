@@ -15,17 +15,111 @@
 //     has as much to do as the others, whatever the sequences' lengths, which only the device knows.  A row tile that a cut goes through
 //     leaves fp32 partials that a second launch merges; the lengths need no host, so the call can be captured into a graph.
 #include "sp_chunk.h"
-#include "sp_tiles.h"
+#include "sp_pipeline.h"
 
-#define CK_LDS_BYTES(D) (4 * AS_TILE * (D) * 2)
+#define CK_WAVES 8
+#define CK_THREADS (CK_WAVES * SP_WAVE)
+#define CK_ROWS (32 * CK_WAVES)  // of a row tile
+#define CK_SUB 64                // keys of a sub-tile
+#define CK_BLOCK (2 * CK_SUB)    // keys of a block: what lies between two barriers
+#define CK_RING 4                // sub-tiles of K in LDS, and of V
+#define CK_SUB_BYTES(D) (CK_SUB * (D) * 2)
+#define CK_LDS_BYTES(D) (2 * CK_RING * CK_SUB_BYTES(D))
+
+typedef __attribute__((address_space(3))) void* ck_lds_ptr;
+typedef uint32_t ck_u32x2 __attribute__((ext_vector_type(2)));
+
+// K and V sub-tiles are [64 keys][D] bf16 in 16-byte chunks, the chunk index XOR-swizzled by the row so that each kind of operand read is
+// free of bank conflicts: K's single chunks (16 rows of one chunk), V's pairs (the transposing read takes two neighbouring chunks of
+// 8 rows).  Rows of 64 channels are half a bank cycle long: two of them share a swizzle.
+template <int D>
+__device__ __forceinline__ int ck_swz_k(int row) {
+  return D == 128 ? (row & 15) : ((row >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int ck_swz_v(int row) {
+  return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3);
+}
+
+// Operands of a block (sp_pipeline.h): sub-tiles 2b and 2b + 1 of K, 2b - 1 (VB 0) and 2b (VB 1) of V.  A V^T operand is two transposing
+// reads of 16 keys each; S^T leaves a lane with keys 4g .. 4g + 3 of either 16-key tile, which is what the two deliver.
+template <int D>
+struct CkAddr {
+  static constexpr int V_READS = 2;
+  uint32_t ka, va[2];
+  template <int KQ, int KS, int T>
+  __device__ __forceinline__ bf16x8 k() const {
+    return at_lds128_async<(KQ >> 1) * CK_SUB_BYTES(D) + ((KQ & 1) * 32 + T * 16) * (D * 2)>(ka ^ (uint32_t)(KS << 6));
+  }
+  template <int VB, int KT, int I>
+  __device__ __forceinline__ bf16x8 v() const {
+    const uint32_t at = va[VB] ^ (uint32_t)(I << 5);
+    ck_u32x2 lo, hi;
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(lo) : "v"(at), "n"(KT * 32 * (D * 2)));
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(hi) : "v"(at), "n"((KT * 32 + 16) * (D * 2)));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3));
+  }
+};
+
+// stages of matrix instructions alone: a walk's first S, its last P . V
+template <int KQ, bool HALF, class Addr>
+__device__ __forceinline__ void ck_qk_only(const Addr& ad, const bf16x8 (&qb)[2][4], floatx4 (&s_out)[2][2]) {
+  constexpr int QS = HALF ? 4 : 8;
+  bf16x8 a[QS];  // slot i: channel step i / 2, key tile i % 2
+  auto fetch = [&](auto kc) {
+    constexpr int i = decltype(kc)::value;
+    a[i] = ad.template k<KQ, (i >> 1), (i & 1)>();
+  };
+  at_static_for<0, 2>(fetch);
+  AT_PIN();
+  at_static_for<0, QS>([&](auto kc) {
+    constexpr int i = decltype(kc)::value;
+    AT_WAIT_LGKM(i + 1 < QS ? 1 : 0);
+    AT_PIN();
+    if constexpr (i + 2 < QS) fetch(std::integral_constant<int, i + 2>{});
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) {
+      if ((i >> 1) == 0)
+        at_mfma_first(s_out[i & 1][qt], a[i], qb[qt][0]);
+      else if (i == QS - 1 && qt == 1)  // the last one: the softmax of the next stage reads S_out right away
+        at_mfma_acc_settled(s_out[i & 1][qt], a[i], qb[qt][i >> 1]);
+      else
+        at_mfma_acc(s_out[i & 1][qt], a[i], qb[qt][i >> 1]);
+    }
+    AT_PIN();
+  });
+}
+template <int VB, int KT, bool HALF, class Addr>
+__device__ __forceinline__ void ck_pv_only(const Addr& ad, const bf16x8 (&p)[2], floatx4 (&o)[9][2], const bf16x8& ones) {
+  constexpr int PS = HALF ? 4 : 8;
+  bf16x8 a[PS];  // slot i: channel tile i
+  auto fetch = [&](auto kc) {
+    constexpr int i = decltype(kc)::value;
+    a[i] = ad.template v<VB, KT, i>();
+  };
+  at_static_for<0, 2>(fetch);
+  AT_PIN();
+  at_static_for<0, PS>([&](auto kc) {
+    constexpr int i = decltype(kc)::value;
+    AT_WAIT_LGKM(i + 1 < PS ? Addr::V_READS : 0);
+    AT_PIN();
+    if constexpr (i + 2 < PS) fetch(std::integral_constant<int, i + 2>{});
+#pragma unroll
+    for (int qt = 0; qt < 2; ++qt) at_mfma_acc(o[i][qt], a[i], p[qt]);
+    AT_PIN();
+  });
+  at_mfma_acc(o[8][0], ones, p[0]);
+  at_mfma_acc_settled(o[8][1], ones, p[1]);  // the end of the walk: the epilogue reads O next
+}
 
 // the sequence that row tile number x belongs to, by 64 candidates at a time
+template <int ROWS>
 __device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
   int lo = 0, span = a.batch;  // it is one of lo .. lo + span - 1
   while (span > 1) {
     const int step = (span + SP_WAVE - 1) / SP_WAVE;
     const int b = lo + lane * step;
-    const bool at_or_behind = lane * step < span && pg_first_slot(ck_start(a, b), a.group, b) <= x;
+    const bool at_or_behind = lane * step < span && pg_first_slot(ck_start(a, b), a.group, b, ROWS) <= x;
     const int n = __builtin_popcountll(__ballot(at_or_behind));
     const int at = pg_max(n - 1, 0) * step;
     span = pg_min(step, span - at);
@@ -35,13 +129,15 @@ __device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
 }
 
 template <int D, bool PAGED>
-__global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a) {
+__global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a) {
+  constexpr int WAVES = CK_WAVES, THREADS = CK_THREADS, TILE_ROWS = CK_ROWS;
+  constexpr bool HALF = D == 64;
   constexpr int QT = 2;                    // 16-row tiles per wave
   constexpr int KS = D / 32, CT = D / 16;  // channel steps of S, channel tiles of O
-  constexpr int TILE_BYTES = AS_TILE * D * 2;
-  constexpr int CHUNKS = D / 8, ROWS = SP_WAVE / CHUNKS;          // of a row; rows of a load instruction
-  constexpr int ITS = AS_TILE / (ROWS * AS_WAVES);                // instructions of a wave for a tile
-  extern __shared__ __attribute__((aligned(1024))) char lds[];  // [buffer][K | V]
+  constexpr int SUB_BYTES = CK_SUB_BYTES(D);
+  constexpr int CHUNKS = D / 8, ROWS = SP_WAVE / CHUNKS;        // of a row; rows of a load instruction
+  constexpr int ITS = CK_SUB / (ROWS * WAVES);                  // instructions of a wave for a sub-tile
+  extern __shared__ __attribute__((aligned(1024))) char lds[];  // rings of K and of V
   const int t = threadIdx.x, lane = t & 63, lq = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t lds_base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
@@ -55,32 +151,32 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
   } else {
     int* const cu_s = reinterpret_cast<int*>(lds);
     int* const len_s = cu_s + a.batch + 1;
-    __shared__ int64_t wave_sums[AS_WAVES];
+    __shared__ int64_t wave_sums[WAVES];
     __shared__ int found[2][2];
-    for (int i = t; i <= a.batch; i += AS_THREADS) {
+    for (int i = t; i <= a.batch; i += THREADS) {
       cu_s[i] = ck_start(a, i);
       if (i < a.batch) len_s[i] = ck_len(a, i);
     }
     __syncthreads();
     // every thread some row tiles in a row: their units, then the line's prefix sums
-    const int per = (a.slots + AS_THREADS - 1) / AS_THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
+    const int per = (a.slots + THREADS - 1) / THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
     auto walk = [&](auto&& visit) {  // visit(x, units in the line, tiles)
       if (x0 >= x1) return;
       int b = 0, hi = a.batch;
       while (hi - b > 1) {
         const int mid = (b + hi) >> 1;
-        if (pg_first_slot(cu_s[mid], a.group, mid) <= x0)
+        if (pg_first_slot(cu_s[mid], a.group, mid, TILE_ROWS) <= x0)
           b = mid;
         else
           hi = mid;
       }
       for (int i = x0; i < x1; ++i) {
-        while (b + 1 < a.batch && pg_first_slot(cu_s[b + 1], a.group, b + 1) <= i) ++b;
-        const int q_len = pg_max(0, cu_s[b + 1] - cu_s[b]), rt = (int)(i - pg_first_slot(cu_s[b], a.group, b));
-        if (rt < 0 || rt >= pg_row_tiles(q_len, a.group)) continue;
+        while (b + 1 < a.batch && pg_first_slot(cu_s[b + 1], a.group, b + 1, TILE_ROWS) <= i) ++b;
+        const int q_len = pg_max(0, cu_s[b + 1] - cu_s[b]), rt = (int)(i - pg_first_slot(cu_s[b], a.group, b, TILE_ROWS));
+        if (rt < 0 || rt >= pg_row_tiles(q_len, a.group, TILE_ROWS)) continue;
         int p0, p1;
-        pg_tile_positions(rt, q_len, len_s[b], a.group, &p0, &p1);
-        const int tiles = pg_span_units(ck_span(a, p0, p1, PG_TILE));
+        pg_tile_positions(rt, q_len, len_s[b], a.group, TILE_ROWS, &p0, &p1);
+        const int tiles = pg_span_units(ck_span(a, p0, p1, CK_BLOCK));
         visit(i, tiles + PG_OVERHEAD, tiles);
       }
     };
@@ -97,7 +193,7 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
     __syncthreads();
     int64_t total = 0;
 #pragma unroll
-    for (int w = 0; w < AS_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       if (w == wave) at += total;
       total += wave_sums[w];
     }
@@ -124,34 +220,35 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
 
   const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
   const int in_tile = wave * ROWS + lane / CHUNKS;                               // the lane's row of its wave's first instruction
-  const uint32_t k_lane = (uint32_t)(lane / CHUNKS) * k_row + 16u * ((lane % CHUNKS) ^ as_swz<D>(in_tile));
-  const uint32_t v_lane = (uint32_t)(lane / CHUNKS) * v_row + 16u * ((lane % CHUNKS) ^ as_swz_v<D>(in_tile));
-  // LDS byte offsets of the lane's operands: K row lq, logical chunk 4 ks + g; V row 4 g + lq / 4, 8-byte piece lq % 4 of the
-  // 32 bytes of channel tile ct.  Rows 16 further have the same swizzle.
-  const int koff = lq * (D * 2), kswz = as_swz<D>(lq);
+  const uint32_t k_lane = (uint32_t)(lane / CHUNKS) * k_row + 16u * ((lane % CHUNKS) ^ ck_swz_k<D>(in_tile));
+  const uint32_t v_lane = (uint32_t)(lane / CHUNKS) * v_row + 16u * ((lane % CHUNKS) ^ ck_swz_v<D>(in_tile));
+  // LDS byte offsets of the lane's operands inside a sub-tile: K row lq, chunk g; V row 4 g + lq / 4, 8-byte piece lq % 4 of the 32 bytes of
+  // channel tile 0.  Other steps and tiles are one XOR away, rows 16 further have the same swizzle.
+  const uint32_t koff = (uint32_t)(lq * (D * 2) + ((g ^ ck_swz_k<D>(lq)) << 4));
   const int vrow = 4 * g + (lq >> 2);
-  const int voff = vrow * (D * 2) + 8 * (lq & 1), vswz = as_swz_v<D>(vrow), vhalf = (lq >> 1) & 1;
-  const as_bf16x8 ones = __builtin_bit_cast(as_bf16x8, (as_u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  const uint32_t voff = (uint32_t)(vrow * (D * 2) + ((((lq >> 1) & 1) ^ ck_swz_v<D>(vrow)) << 4) + 8 * (lq & 1));
+  bf16x8 ones = __builtin_bit_cast(bf16x8, (at_u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  asm volatile("" : "+v"(ones));  // one register set throughout
 
-  int b = x < a.slots ? __builtin_amdgcn_readfirstlane(ck_sequence(a, x, lane)) : 0;
+  int b = x < a.slots ? __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, x, lane)) : 0;
   for (; x < a.slots && (x < x_end || (x == x_end && tile_end > 0)); ++x, tile_begin = 0) {
-    while (b + 1 < a.batch && pg_first_slot(ck_start(a, b + 1), a.group, b + 1) <= x) ++b;
+    while (b + 1 < a.batch && pg_first_slot(ck_start(a, b + 1), a.group, b + 1, TILE_ROWS) <= x) ++b;
     const int start = ck_start(a, b), q_len = pg_max(0, ck_start(a, b + 1) - start), len = ck_len(a, b);
-    const int rt = (int)(x - pg_first_slot(start, a.group, b));
-    const int rows = q_len * a.group - rt * PG_ROWS;  // from here to the sequence's end
+    const int rt = (int)(x - pg_first_slot(start, a.group, b, TILE_ROWS));
+    const int rows = q_len * a.group - rt * TILE_ROWS;  // from here to the sequence's end
     if (rt < 0 || rows <= 0) continue;
     int p0, p1;
-    pg_tile_positions(rt, q_len, len, a.group, &p0, &p1);
-    const PgSpan span = ck_span(a, p0, p1, PG_TILE);
+    pg_tile_positions(rt, q_len, len, a.group, TILE_ROWS, &p0, &p1);
+    const PgSpan span = ck_span(a, p0, p1, CK_BLOCK);
     const int tiles = pg_span_units(span);
     const int i_end = x == x_end ? pg_min(tile_end, tiles) : tiles;
     const bool from_start = tile_begin == 0, to_end = i_end == tiles;  // (uniform)
 
     // the lane's rows: token, head and position
     int pos[QT];
-    as_bf16x8 qb[QT][KS];
+    bf16x8 qb[QT][4];
     auto row_of = [&](int qt, int* token, int* head) {
-      const int r = rt * PG_ROWS + pg_min(wave * 32 + 16 * qt + lq, rows - 1);
+      const int r = rt * TILE_ROWS + pg_min(wave * 32 + 16 * qt + lq, rows - 1);
       *token = (int)((unsigned)r / (unsigned)a.group);
       *head = kvh * a.group + (r - *token * a.group);
     };
@@ -162,12 +259,12 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
       pos[qt] = len - q_len + token;
       const sp_bf16* src = a.q + b * a.sq_b + (int64_t)((PAGED ? start : 0) + token) * a.sq_n + head * a.sq_h + 8 * g;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qb[qt][ks] = __builtin_bit_cast(as_bf16x8, *reinterpret_cast<const uint4*>(src + 32 * ks));
+      for (int ks = 0; ks < KS; ++ks) qb[qt][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 32 * ks));
     }
     const bool has_rows = wave * 32 < rows;  // (uniform in the wave)
     // positions of the wave's first and last row
-    const int w0 = len - q_len + (int)((unsigned)(rt * PG_ROWS + pg_min(wave * 32, rows - 1)) / (unsigned)a.group);
-    const int w1 = len - q_len + (int)((unsigned)(rt * PG_ROWS + pg_min(wave * 32 + 31, rows - 1)) / (unsigned)a.group);
+    const int w0 = len - q_len + (int)((unsigned)(rt * TILE_ROWS + pg_min(wave * 32, rows - 1)) / (unsigned)a.group);
+    const int w1 = len - q_len + (int)((unsigned)(rt * TILE_ROWS + pg_min(wave * 32 + 31, rows - 1)) / (unsigned)a.group);
 
     // ---- the sequence's pages: 64 entries of its table at hand, a lane each, and the 64 behind them on their way ----
     const int32_t* const table = PAGED ? a.table + b * a.table_stride : nullptr;
@@ -177,209 +274,177 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
       const int id = table[pg_min(i, a.width - 1)];
       return i < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
     };
-    auto turn_to = [&](int tile) {  // (a tile's pages lie in one group of 64)
-      if constexpr (PAGED) {
-        const int group = (int)(((int64_t)tile * AS_TILE) >> a.shift) >> 6;
-        if (group != ids_group) {
-          ids = group == ids_group + 1 ? ids_next : entries(group);
-          ids_next = entries(group + 1);
-          ids_group = group;
-        }
+    auto turn_to = [&](int page) {  // (a block's pages lie in one group of 64)
+      const int group = page >> 6;
+      if (group != ids_group) {
+        ids = group == ids_group + 1 ? ids_next : entries(group);
+        ids_next = entries(group + 1);
+        ids_group = group;
       }
     };
     const char* const kh = (const char*)(a.k + b * a.sk_b + kvh * a.sk_h);
     const char* const vh = (const char*)(a.v + b * a.sv_b + kvh * a.sv_h);
-    auto issue = [&](int tile, int buf) {
-      turn_to(tile);
-      const uint32_t at = lds_base + (uint32_t)(buf * 2 * TILE_BYTES + wave * 1024);
+    // A block of the walk: its first key, the pages of this wave's instructions (-1: none), and which 16-key groups have none (bits).
+    struct Block {
+      int key0, id[2][ITS];
+      uint32_t lost;
+    };
+    auto block = [&](int i) {
+      Block c;
+      c.key0 = pg_span_unit(span, i) * CK_BLOCK;
+      c.lost = 0;
+      if constexpr (PAGED) turn_to(c.key0 >> a.shift);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const int page = (c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS) >> a.shift;
+          c.id[hf][it] = PAGED ? __builtin_amdgcn_readlane(ids, page & 63) : page;
+        }
+      if constexpr (PAGED) {
+#pragma unroll
+        for (int i16 = 0; i16 < 8; ++i16)
+          c.lost |= (uint32_t)(__builtin_amdgcn_readlane(ids, ((c.key0 + 16 * i16) >> a.shift) & 63) < 0) << i16;
+      }
+      return c;
+    };
+    // half hf of a block into slot `sub` % 4 of a ring; want false: zeros, without a read
+    auto load = [&](const Block& c, int hf, int sub, bool want, const char* x, int64_t stride_page, uint32_t row_bytes, uint32_t lane_off,
+                    uint32_t to) {
+      to += (uint32_t)((sub & 3) * SUB_BYTES + wave * 1024);
 #pragma unroll
       for (int it = 0; it < ITS; ++it) {
-        const int key = tile * AS_TILE + (it * AS_WAVES + wave) * ROWS;  // the instruction's first
-        const int page = key >> a.shift, in = key & ((1 << a.shift) - 1);
-        const int id = PAGED ? __builtin_amdgcn_readlane(ids, page & 63) : page;
-        // rows from here that are there, as far as this instruction goes
-        const int there = id < 0 ? 0 : pg_max(0, pg_min(len - key, ROWS));
-        auto load = [&](const char* x, int64_t stride_page, uint32_t row_bytes, uint32_t lane_off, uint32_t to) {
-          const char* p = x + (int64_t)pg_max(id, 0) * (stride_page * 2) + (uint64_t)(uint32_t)in * row_bytes;
-          const __amdgpu_buffer_rsrc_t rsrc =
-              __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, there > 0 ? (int)((uint32_t)(there - 1) * row_bytes + 2u * D) : 0, 0x00027000);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (as_lds_ptr)(uintptr_t)(to + it * AS_WAVES * 1024), 16, (int)lane_off, 0, 0, 0);
-        };
-        load(kh, a.sk_p, k_row, k_lane, at);
-        load(vh, a.sv_p, v_row, v_lane, at + TILE_BYTES);
+        const int key = c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS, in = key & ((1 << a.shift) - 1), id = c.id[hf][it];
+        const int there = id < 0 || !want ? 0 : pg_max(0, pg_min(len - key, ROWS));  // rows that are there, as far as this instruction goes
+        const char* p = x + (int64_t)pg_max(id, 0) * (stride_page * 2) + (uint64_t)(uint32_t)in * row_bytes;
+        const __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, there > 0 ? (int)((uint32_t)(there - 1) * row_bytes + 2u * D) : 0, 0x00027000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ck_lds_ptr)(uintptr_t)(to + it * WAVES * 1024), 16, (int)lane_off, 0, 0, 0);
       }
     };
-    auto missing = [&](int tile) {  // bit kt: keys 16 kt .. 16 kt + 15 of the tile have no page
-      uint32_t m = 0;
-      if constexpr (PAGED) {
-        turn_to(tile);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-          m |= (uint32_t)(__builtin_amdgcn_readlane(ids, ((tile * AS_TILE + 16 * kt) >> a.shift) & 63) < 0) << kt;
-      }
-      return m;
+    auto load_k = [&](const Block& c, int hf, int sub, bool want) { load(c, hf, sub, want, kh, a.sk_p, k_row, k_lane, lds_base); };
+    auto load_v = [&](const Block& c, int hf, int sub, bool want) {
+      load(c, hf, sub, want, vh, a.sv_p, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
     };
 
-    as_floatx4 o[CT][QT], l[QT];  // l: row sums (ones . P, every row of the tile holds the sum)
-    float m[QT];
+    floatx4 o[9][2];  // [channel tile][row tile]; o[8]: the row sums (ones . P)
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
+    for (int ct = 0; ct < 9; ++ct)
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[ct][qt] = (as_floatx4){0, 0, 0, 0};
-      l[qt] = (as_floatx4){0, 0, 0, 0};
-      m[qt] = AS_NO_MAX;
-    }
+      for (int qt = 0; qt < QT; ++qt) o[ct][qt] = (floatx4){0, 0, 0, 0};
+    float m[QT] = {AT_NO_MAX, AT_NO_MAX}, l_mark[QT] = {0.f, 0.f};
+    uint32_t det[2] = {0u, 0u};
 
-    __syncthreads();  // the LDS is free: the plan has been read, the row tile in front is done with its last tile
-    uint32_t lost_next = 0;
-    if (tile_begin < i_end) {
-      const int tile = pg_span_unit(span, tile_begin);
-      issue(tile, 0);
-      lost_next = missing(tile);
-    }
-    for (int i = tile_begin; i < i_end; ++i) {
-      const int buf = (i - tile_begin) & 1, tile = pg_span_unit(span, i);
-      const uint32_t lost = lost_next;
-      // this wave's loads of the tile have landed, and everybody's; the other buffer's readers are done
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (i + 1 < i_end) {
-        const int next = pg_span_unit(span, i + 1);
-        issue(next, buf ^ 1);
-        lost_next = missing(next);
-      }
-      const int key0 = tile * AS_TILE, key1 = key0 + AS_TILE - 1;
-      // (a tile that no row of the wave sees anything of: behind them all, or between the sinks and all windows)
-      if (!has_rows || key0 > w1 || (key1 <= w0 - a.window && key0 >= a.sinks)) continue;
-      const bool masked = key1 > w0 || (key0 <= w1 - a.window && key1 >= a.sinks) || lost != 0;
-      const uint32_t kt_addr = lds_base + (uint32_t)(buf * 2 * TILE_BYTES);
-      const uint32_t vt_addr = lds_base + (uint32_t)(buf * 2 * TILE_BYTES + TILE_BYTES + voff);
-      constexpr int GR = CT / 4;  // groups of four channel tiles
-      as_u32x2 vr[2][8];
-      auto fetch_v = [&](auto hc, auto gc) {  // group gc of half hc, into vr[gc & 1] (the first of the next half: where it is free)
-        constexpr int hh = decltype(hc)::value, gi = decltype(gc)::value, to = GR == 1 ? hh & 1 : gi & 1;
-        as_static_for<0, 4>([&](auto uc) {
-          constexpr int u = decltype(uc)::value;
-          const uint32_t ad = vt_addr + (uint32_t)(((2 * (4 * gi + u) + vhalf) ^ vswz) << 4);
-          vr[to][2 * u] = as_read_tr<hh * 32 * (D * 2)>(ad);
-          vr[to][2 * u + 1] = as_read_tr<hh * 32 * (D * 2) + 16 * (D * 2)>(ad);
-        });
+    __syncthreads();  // the LDS is free: the plan has been read, the row tile in front is done with its last block
+    const int n_blk = i_end - tile_begin;
+    if (n_blk > 0) {
+      // Block bb of the walk is sub-tiles 2 bb and 2 bb + 1; sub-tile s lives in slot s % 4 of either ring.  One wait and barrier per block:
+      // while it is computed on (K of 2 bb, 2 bb + 1, V of 2 bb - 1, 2 bb: P . V trails by a sub-tile) K of 2 bb + 2, 2 bb + 3 and V of
+      // 2 bb + 1, 2 bb + 2 are on their way, sent out in four parts between the block's steps.
+      Block cur = block(tile_begin), nxt = cur;
+      load_k(cur, 0, 0, true);
+      load_k(cur, 1, 1, true);
+      load_v(cur, 0, 0, true);
+      int bb = 0;
+      bool more = false;  // there is a block behind this one
+      CkAddr<D> ad;
+      auto top = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");  // everybody's loads have landed, everybody is past the block in front
+        more = bb + 1 < n_blk;
+        if (more) nxt = block(tile_begin + bb + 1);
+        const uint32_t k_at = lds_base + (uint32_t)(((2 * bb) & 3) * SUB_BYTES), v_at = lds_base + CK_RING * SUB_BYTES;
+        ad.ka = k_at + koff;
+        ad.va[0] = v_at + (uint32_t)(((2 * bb + 3) & 3) * SUB_BYTES) + voff;
+        ad.va[1] = v_at + (uint32_t)(((2 * bb) & 3) * SUB_BYTES) + voff;
       };
-      as_floatx4 s[4][QT];
-      {
-        as_u32x4 kr[2][KS];
-        auto fetch_k = [&](auto kc) {
-          constexpr int kt = decltype(kc)::value;
-          as_static_for<0, KS>([&](auto sc) {
-            constexpr int ks = decltype(sc)::value;
-            kr[kt & 1][ks] = as_read_k<kt * 16 * (D * 2)>(kt_addr + (uint32_t)(koff + (((4 * ks + g) ^ kswz) << 4)));
-          });
-        };
-        fetch_k(std::integral_constant<int, 0>{});
-        fetch_k(std::integral_constant<int, 1>{});
-        __builtin_amdgcn_s_setprio(1);
-        as_static_for<0, 4>([&](auto kc) {
-          constexpr int kt = decltype(kc)::value;
-          as_wait_k<(kt < 3 ? KS : 0)>(kr[kt & 1]);
+      auto feed = [&](int part) {
+        if (part == 0) load_k(nxt, 0, 2 * bb + 2, more);
+        if (part == 1) load_k(nxt, 1, 2 * bb + 3, more);
+        if (part == 2) load_v(cur, 1, 2 * bb + 1, true);
+        if (part == 3) load_v(nxt, 0, 2 * bb + 2, more);
+      };
+      // what the wave's rows do not see of a block: nothing to take out in most of them
+      auto partly = [&](const Block& c) {
+        const int key0 = c.key0, key1 = key0 + CK_BLOCK - 1;
+        return key1 > w0 || (key0 <= w1 - a.window && key1 >= a.sinks) || c.lost != 0;
+      };
+      struct Mask {
+        bool some;
+        int key0, window, sinks, p0, p1;  // (of the half-tile; positions of the lane's rows)
+        uint32_t lost;
+        __device__ __forceinline__ void operator()(floatx4 (&s)[2][2]) const {
+          if (!some) return;
+          const int key = key0 + 4 * ((threadIdx.x >> 4) & 3);
 #pragma unroll
-          for (int qt = 0; qt < QT; ++qt) s[kt][qt] = (as_floatx4){0, 0, 0, 0};
+          for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-              s[kt][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(as_bf16x8, kr[kt & 1][ks]), qb[qt][ks], s[kt][qt], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (kt + 2 < 4) fetch_k(std::integral_constant<int, kt + 2>{});
-        });
-      }
-      if (masked) {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (((lost >> kt) & 1u) || !pg_sees(pos[qt], key0 + 16 * kt + 4 * g + j, a.window, a.sinks)) s[kt][qt][j] = -INFINITY;
-      }
-      __builtin_amdgcn_s_setprio(0);
-      fetch_v(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
-      uint32_t pk[QT][8];
-      auto softmax = [&](int qt, int hh) {  // half hh: 32 keys
-#pragma unroll
-        for (int kt = 2 * hh; kt < 2 * hh + 2; ++kt) {
-          float e[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][qt][j], a.scale_log2, -m[qt]));
-          pk[qt][2 * kt] = as_pack2(e[0], e[1]);
-          pk[qt][2 * kt + 1] = as_pack2(e[2], e[3]);
+            for (int j = 0; j < 4; ++j) {
+              const bool gone = (lost >> kt) & 1u;
+              if (gone || !pg_sees(p0, key + 16 * kt + j, window, sinks)) s[kt][0][j] = -INFINITY;
+              if (gone || !pg_sees(p1, key + 16 * kt + j, window, sinks)) s[kt][1][j] = -INFINITY;
+            }
         }
       };
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        softmax(qt, 0);
-        softmax(qt, 1);
-      }
-      __builtin_amdgcn_s_setprio(1);
-      as_static_for<0, 2>([&](auto hc) {
-        constexpr int hh = decltype(hc)::value;
-        // The running max is lazy: it moves only when some probability came out at 2 or more (or is inf: a row's first keys), and then
-        // the probabilities are formed again before they are used.  P enters the product as bf16, rounded at 2^-9 of its value at most;
-        // the sums are those of the rounded values.
-        uint32_t det = 0u;
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-          for (int i = 4 * hh; i < 4 * hh + 4; i += 2) det |= pk[qt][i] | pk[qt][i + 1];
-        as_wait_v<0>(vr[GR == 1 ? hh & 1 : 0]);  // the half's first group (no read may be in flight across the branch)
-        if (__ballot((det & AS_P_TOO_LARGE) != 0u) != 0ull) {
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kt = 2 * hh; kt < 2 * hh + 2; ++kt)
-              mx = fmaxf(mx, fmaxf(fmaxf(s[kt][qt][0], s[kt][qt][1]), fmaxf(s[kt][qt][2], s[kt][qt][3])));
-            const float m_new = fmaxf(m[qt], as_groupmax(mx * a.scale_log2));
-            const float alpha = __builtin_amdgcn_exp2f(m[qt] - m_new);
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) o[ct][qt] *= alpha;
-            l[qt] *= alpha;
-            m[qt] = m_new;
-            softmax(qt, hh);
-            if constexpr (hh == 0) softmax(qt, 1);
-          }
+      auto masked = [&](const Block& c, bool some, int quarter) {
+        return Mask{some, c.key0 + 32 * quarter, a.window, a.sinks, pos[0], pos[1], c.lost >> (2 * quarter)};
+      };
+      constexpr int MODE = HALF ? 2 : 0;
+      if (!has_rows) {
+        for (; bb < n_blk; ++bb) {
+          top();
+          feed(0), feed(1), feed(2), feed(3);
+          cur = nxt;
         }
-        // O += V^T . P: groups of four channel tiles, the next group's operands on their way
-        as_bf16x8 p[QT];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-          p[qt] = __builtin_bit_cast(as_bf16x8, (as_u32x4){pk[qt][4 * hh], pk[qt][4 * hh + 1], pk[qt][4 * hh + 2], pk[qt][4 * hh + 3]});
-        as_static_for<0, GR>([&](auto gc) {
-          constexpr int gi = decltype(gc)::value, from = GR == 1 ? hh & 1 : gi & 1;
-          if constexpr (gi > 0) as_wait_v<0>(vr[from]);
-          if constexpr (gi + 1 < GR)
-            fetch_v(hc, std::integral_constant<int, gi + 1>{});
-          else if constexpr (hh == 0)
-            fetch_v(std::integral_constant<int, 1>{}, std::integral_constant<int, 0>{});
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const as_u32x4 raw = __builtin_shufflevector(vr[from][2 * u], vr[from][2 * u + 1], 0, 1, 2, 3);
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt)
-              o[4 * gi + u][qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(as_bf16x8, raw), p[qt], o[4 * gi + u][qt], 0, 0, 0);
-          }
-          if constexpr (gi == 0) {
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) l[qt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[qt], l[qt], 0, 0, 0);
-          }
-        });
-      });
-      __builtin_amdgcn_s_setprio(0);
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      } else {
+        floatx4 sa[2][2], sb[2][2];  // [key tile][row tile]
+        bf16x8 pa[2], pb[2];         // [row tile]
+        bf16x8 pre[2];               // the next stage's first two LDS operands, in flight (at_prefetch_qk)
+        Block old = cur;
+        bool some = partly(cur), some_old = some;
+        // ---- start: S of the first half-tile, nothing to overlap with yet ----
+        top();
+        feed(0);
+        ck_qk_only<0, HALF>(ad, qb, sa);
+        feed(1);
+        at_step<true, false, 1, 0, 0, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+        feed(2);
+        at_step<true, true, 2, 1, 0, MODE, false, -1>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
+        feed(3);
+        at_step<true, true, 3, 1, 1, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
+        // ---- steady: four steps per block ----
+        for (bb = 1; bb < n_blk; ++bb) {
+          old = cur, some_old = some;
+          cur = nxt;
+          some = partly(cur);
+          top();
+          if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(1);
+          at_step<true, true, 0, 0, 0, MODE, false, -1>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(old, some_old, 3), l_mark, pre);
+          feed(0);
+          at_step<true, true, 1, 0, 1, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+          if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(0);
+          feed(1);
+          feed(2);
+          at_step<true, true, 2, 1, 0, MODE, false, -1>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
+          feed(3);
+          at_step<true, true, 3, 1, 1, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
+        }
+        // ---- drain: the last half-tile and its P . V (V of sub-tile 2 n_blk - 1) ----
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        ad.va[0] = lds_base + CK_RING * SUB_BYTES + (uint32_t)(((2 * n_blk + 3) & 3) * SUB_BYTES) + voff;
+        at_step<false, true, 0, 0, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 3), l_mark, pre);
+        at_commit<MODE>(sb, pb, det, o, a.scale_log2, m, l_mark);
+        ck_pv_only<0, 1, HALF>(ad, pb, o, ones);
+        at_settle_o(o);
+      }
     }
+    const float l[QT] = {o[8][0][0], o[8][1][0]};
 
     // ---- what has come of it: the rows, or a partial ----
     const bool whole = from_start && to_end;  // (uniform)
     const int64_t slab = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
-    float* const o_to = a.o_part + slab * (PG_ROWS * D);
-    float2* const ml_to = a.ml_part + slab * PG_ROWS;
+    float* const o_to = a.o_part + slab * (TILE_ROWS * D);
+    float2* const ml_to = a.ml_part + slab * TILE_ROWS;
     if (!whole) {
       if (from_start)
         note.y = b, note.z = rt;
@@ -400,7 +465,7 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
         for (int j = 0; j < 4; ++j) spoilt[qt] |= o[ct][qt][j] != o[ct][qt][j];
       spoilt[qt] &= mine;
       if (whole) {
-        const float inv_l = l[qt][0] > 0.f || l[qt][0] != l[qt][0] ? 1.0f / l[qt][0] : 0.f;
+        const float inv_l = l[qt] > 0.f || l[qt] != l[qt] ? 1.0f / l[qt] : 0.f;
         // (lane groups 2i and 2i + 1 trade halves of two neighbouring channel tiles: 16 bytes a store, 64 contiguous ones a row)
         sp_bf16* dst = a.out + ((int64_t)(start + token) * (a.hkv * a.group) + head) * D + 16 * (g & 1) + 8 * (g >> 1);
 #pragma unroll
@@ -408,8 +473,8 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
           uint32_t w[2][2];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            w[u][0] = as_pack2(o[ct + u][qt][0] * inv_l, o[ct + u][qt][1] * inv_l);
-            w[u][1] = as_pack2(o[ct + u][qt][2] * inv_l, o[ct + u][qt][3] * inv_l);
+            w[u][0] = at_pack2(o[ct + u][qt][0] * inv_l, o[ct + u][qt][1] * inv_l);
+            w[u][1] = at_pack2(o[ct + u][qt][2] * inv_l, o[ct + u][qt][3] * inv_l);
           }
           const auto lo = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false);
           const auto hi = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
@@ -417,8 +482,8 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
         }
       } else if (mine) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<as_floatx4*>(o_to + in_rows * D + 16 * ct + 4 * g) = o[ct][qt];
-        if (g == 0) ml_to[in_rows] = make_float2(m[qt], l[qt][0]);
+        for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<floatx4*>(o_to + in_rows * D + 16 * ct + 4 * g) = o[ct][qt];
+        if (g == 0) ml_to[in_rows] = make_float2(m[qt], l[qt]);
       }
     }
     // A masked key weighs 0, and 0 times an infinity or a NaN of its value has made a NaN of the sum.  Such rows are formed again key by key,
@@ -432,13 +497,13 @@ __global__ __launch_bounds__(AS_THREADS, 2) void sp_chunk_kernel(const CkArgs a)
       while (rows_left != 0ull) {
         const int in_rows = wave * 32 + 16 * qt + __builtin_ctzll(rows_left);
         rows_left &= rows_left - 1ull;
-        const int r = rt * PG_ROWS + in_rows, token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
+        const int r = rt * TILE_ROWS + in_rows, token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
         const int p = len - q_len + token;
         const sp_bf16* qrow = a.q + b * a.sq_b + (int64_t)((PAGED ? start : 0) + token) * a.sq_n + head * a.sq_h;
         constexpr int CL = D / SP_WAVE;  // channels of a lane
-        float acc[CL] = {0.f}, sum = 0.f, top = AS_NO_MAX;
-        for (int i = tile_begin; i < i_end; ++i) {
-          const int key = pg_span_unit(span, i) * AS_TILE + lane, page = key >> a.shift;
+        float acc[CL] = {0.f}, sum = 0.f, top = CK_NO_MAX;
+        for (int i = 2 * tile_begin; i < 2 * i_end; ++i) {
+          const int key = pg_span_unit(span, i >> 1) * CK_BLOCK + (i & 1) * SP_WAVE + lane, page = key >> a.shift;
           int id = page;
           if constexpr (PAGED) {
             id = page < a.width ? table[page] : -1;
@@ -488,19 +553,19 @@ struct CkPlan {
   int parts;
 };
 // Workgroups that are resident at once: two a CU with 128 channels.
-static int ck_places(int d) { return d == 64 ? 768 : 512; }
+#define CK_PLACES 256
 static CkPlan ck_plan(int64_t tokens, int32_t batch, int32_t hkv, int32_t group, int32_t d) {
   CkPlan p;
-  p.slots = pg_slots(tokens, group, batch);
-  const int64_t room = ck_places(d) / hkv;
-  p.parts = p.slots * hkv >= 4 * ck_places(d) ? 0 : (int)(room < 1 ? 1 : room);
+  p.slots = pg_slots(tokens, group, batch, CK_ROWS);
+  const int64_t room = CK_PLACES / hkv;
+  p.parts = p.slots * hkv >= 4 * CK_PLACES ? 0 : (int)(room < 1 ? 1 : room);
   p.grid = (p.parts == 0 ? p.slots : p.parts) * hkv;
   return p;
 }
 static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d) {
   if (tokens <= 0 || batch <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || (d != 64 && d != 128)) return 0;
   const CkPlan p = ck_plan(tokens, batch, hkv, hq / hkv, d);
-  return p.parts == 0 ? 0 : (size_t)p.grid * (2 * PG_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + sizeof(int4));
+  return p.parts == 0 ? 0 : (size_t)p.grid * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
 static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* workspace, size_t workspace_bytes, hipStream_t s) {
@@ -513,13 +578,13 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* wo
   a.slots = (int)plan.slots;
   a.parts = plan.parts;
   a.o_part = (float*)workspace;
-  a.ml_part = (float2*)(a.o_part + (size_t)plan.grid * 2 * PG_ROWS * d);
-  a.notes = (int4*)(a.ml_part + (size_t)plan.grid * 2 * PG_ROWS);
+  a.ml_part = (float2*)(a.o_part + (size_t)plan.grid * 2 * (size_t)CK_ROWS * d);
+  a.notes = (int4*)(a.ml_part + (size_t)plan.grid * 2 * CK_ROWS);
   const size_t plan_lds = (size_t)(2 * a.batch + 1) * sizeof(int);
   const size_t lds = plan_lds > (size_t)CK_LDS_BYTES(d) ? plan_lds : (size_t)CK_LDS_BYTES(d);
   auto go = [&](auto kernel, auto merge) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(AS_THREADS), lds, s, a);
-    if (plan.parts != 0) hipLaunchKernelGGL(merge, dim3((unsigned)plan.grid, PG_ROWS / CM_ROWS), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(CK_THREADS), lds, s, a);
+    if (plan.parts != 0) hipLaunchKernelGGL(merge, dim3((unsigned)plan.grid, CK_ROWS / CM_ROWS), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
   };
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -532,9 +597,9 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* wo
     attr_set[dev] = true;
   }
   if (d == 64)
-    a.table != nullptr ? go(sp_chunk_kernel<64, true>, sp_chunk_merge_kernel<64, PG_ROWS>) : go(sp_chunk_kernel<64, false>, sp_chunk_merge_kernel<64, PG_ROWS>);
+    a.table != nullptr ? go(sp_chunk_kernel<64, true>, sp_chunk_merge_kernel<64, CK_ROWS>) : go(sp_chunk_kernel<64, false>, sp_chunk_merge_kernel<64, CK_ROWS>);
   else
-    a.table != nullptr ? go(sp_chunk_kernel<128, true>, sp_chunk_merge_kernel<128, PG_ROWS>) : go(sp_chunk_kernel<128, false>, sp_chunk_merge_kernel<128, PG_ROWS>);
+    a.table != nullptr ? go(sp_chunk_kernel<128, true>, sp_chunk_merge_kernel<128, CK_ROWS>) : go(sp_chunk_kernel<128, false>, sp_chunk_merge_kernel<128, CK_ROWS>);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }

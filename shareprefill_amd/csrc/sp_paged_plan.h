@@ -13,7 +13,7 @@
 #define PG_MAX_KEYS (1 << 30)      // keys of a sequence: positions and their differences have 31 bits
 #define PG_NO_WINDOW PG_MAX_KEYS   // every key in front of a query lies inside it
 #define PG_TILE 64                 // keys of a tile
-#define PG_ROWS 128                // rows of a row tile: (token, query head of the kv group), the heads of a token side by side
+                                   // a row tile has `tile` rows: (token, query head of the kv group) pairs, the heads of a token side by side
 
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
 PG_FN int pg_max(int a, int b) { return a > b ? a : b; }
@@ -39,14 +39,14 @@ PG_FN PgSpan pg_span(int p0, int p1, int window, int sinks, int unit) {
 }
 
 // Row tiles are numbered so that a workgroup finds its own without a scan: those of sequence b, whose tokens start at `start`, begin at
-// floor(start * g / 128) + b.  Every sequence has room for its last, partly filled tile; numbers left over stand for nothing.
-PG_FN int64_t pg_first_slot(int64_t start, int g, int b) { return start * g / PG_ROWS + b; }
-PG_FN int64_t pg_slots(int64_t tokens, int g, int batch) { return tokens * g / PG_ROWS + batch; }
-PG_FN int64_t pg_row_tiles(int64_t q_len, int g) { return (q_len * g + PG_ROWS - 1) / PG_ROWS; }
+// floor(start * g / tile) + b.  Every sequence has room for its last, partly filled tile; numbers left over stand for nothing.
+PG_FN int64_t pg_first_slot(int64_t start, int g, int b, int tile) { return start * g / tile + b; }
+PG_FN int64_t pg_slots(int64_t tokens, int g, int batch, int tile) { return tokens * g / tile + batch; }
+PG_FN int64_t pg_row_tiles(int64_t q_len, int g, int tile) { return (q_len * g + tile - 1) / tile; }
 
 // Positions of a row tile's first and last row: row r of a sequence is token r / g.
-PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int* p0, int* p1) {
-  const int64_t r0 = (int64_t)rt * PG_ROWS, rows = (int64_t)q_len * g, r1 = r0 + PG_ROWS < rows ? r0 + PG_ROWS : rows;
+PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int tile, int* p0, int* p1) {
+  const int64_t r0 = (int64_t)rt * tile, rows = (int64_t)q_len * g, r1 = r0 + tile < rows ? r0 + tile : rows;
   *p0 = len - q_len + (int)(r0 / g);
   *p1 = len - q_len + (int)((r1 - 1) / g);
 }

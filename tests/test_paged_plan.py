@@ -20,14 +20,14 @@ int main() {
       const PgSpan s = pg_span((int)a, (int)b, (int)c, (int)d, (int)e);
       printf("%d %d %d %d\\n", s.front, s.lo, s.hi, pg_span_units(s));
     } else if (what == 'f') {
-      printf("%ld %ld %ld\\n", (long)pg_first_slot(a, (int)b, (int)c), (long)pg_slots(a, (int)b, (int)c), (long)pg_row_tiles(a, (int)b));
+      printf("%ld %ld %ld\\n", (long)pg_first_slot(a, (int)b, (int)c, (int)d), (long)pg_slots(a, (int)b, (int)c, (int)d), (long)pg_row_tiles(a, (int)b, (int)d));
     } else if (what == 'c') {
       printf("%ld %ld\\n", (long)pg_parts(a, b, 8), (long)pg_cut(a, pg_parts(a, b, 8), c));
     } else if (what == 'n') {
       printf("%d\\n", pg_snap(a, (int)b, 2));
     } else {
       int p0, p1;
-      pg_tile_positions((int)a, (int)b, (int)c, (int)d, &p0, &p1);
+      pg_tile_positions((int)a, (int)b, (int)c, (int)d, (int)e, &p0, &p1);
       printf("%d %d\\n", p0, p1);
     }
   }
@@ -72,26 +72,27 @@ def test_spans_hold_every_key_that_is_seen_and_no_unit_twice(ask, unit):
         assert all(u in seen for u in units), (p0, p1, window, sinks)
 
 
-def test_row_tiles_number_without_a_clash(ask):
+@pytest.mark.parametrize("tile", [128, 256])
+def test_row_tiles_number_without_a_clash(ask, tile):
     rng = random.Random(1)
     for _ in range(60):
         g, lens = rng.choice((1, 4, 7, 8, 20, 160)), [rng.choice((0, 1, 2, rng.randrange(300))) for _ in range(rng.randrange(1, 40))]
         at = [0]
         for n in lens:
             at.append(at[-1] + n)
-        firsts = [r[0] for r in ask([("f", s, g, b) for b, s in enumerate(at)])]
-        tiles = [r[2] for r in ask([("f", n, g, 0) for n in lens])]
-        slots = ask([("f", at[-1], g, len(lens))])[0][1]
+        firsts = [r[0] for r in ask([("f", s, g, b, tile) for b, s in enumerate(at)])]
+        tiles = [r[2] for r in ask([("f", n, g, 0, tile) for n in lens])]
+        slots = ask([("f", at[-1], g, len(lens), tile)])[0][1]
         for b, n in enumerate(lens):
-            assert tiles[b] == -(-n * g // 128)
+            assert tiles[b] == -(-n * g // tile)
             assert firsts[b] + tiles[b] <= firsts[b + 1], "room for the tiles of every sequence"
             assert firsts[b] < firsts[b + 1]
         assert firsts[-1] == slots
         # positions of a tile's rows
         b = rng.randrange(len(lens))
         for rt in range(tiles[b]):
-            rows = range(rt * 128, min(rt * 128 + 128, lens[b] * g))
-            assert ask([("p", rt, lens[b], 1000, g)])[0] == (1000 - lens[b] + rows[0] // g, 1000 - lens[b] + rows[-1] // g)
+            rows = range(rt * tile, min(rt * tile + tile, lens[b] * g))
+            assert ask([("p", rt, lens[b], 1000, g, tile)])[0] == (1000 - lens[b] + rows[0] // g, 1000 - lens[b] + rows[-1] // g)
 
 
 def test_cuts_cover_the_line_once(ask):
