@@ -24,7 +24,8 @@
 #define CK_BLOCK (2 * CK_SUB)    // keys of a block: what lies between two barriers
 #define CK_RING 4                // sub-tiles of K in LDS, and of V
 #define CK_SUB_BYTES(D) (CK_SUB * (D) * 2)
-#define CK_LDS_BYTES(D) (2 * CK_RING * CK_SUB_BYTES(D))
+#define CK_LDS_BYTES(D) (2 * CK_RING * CK_SUB_BYTES(D))  // the rings; offsets and lengths of the sequences stand behind them
+#define CK_MAX_SEQS 2048
 
 typedef __attribute__((address_space(3))) void* ck_lds_ptr;
 typedef uint32_t ck_u32x2 __attribute__((ext_vector_type(2)));
@@ -143,13 +144,12 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   const uint32_t lds_base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
   const int kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv;  // (workgroups of a kv head share an XCD where that works out)
 
-  // ---- which row tiles, and which tiles of the first and the last ----
-  int x, x_end, tile_begin = 0, tile_end = 0;  // row tiles x .. x_end, of the last the tiles in front of tile_end
-  if (a.parts == 0) {
-    x = a.slots - 1 - part;  // (the last rows of a prompt see the most keys)
-    x_end = x + 1;
-  } else {
-    int* const cu_s = reinterpret_cast<int*>(lds);
+  // ---- which row tiles, and which blocks of the first and the last ----
+  // On a line: row tiles x .. x_end, the first from block tile_begin on, of the last the blocks in front of tile_end.
+  int x = 0, x_end = 0, tile_begin = 0, tile_end = 0, turn = 0;
+  const uint32_t lds_cu = lds_base + CK_LDS_BYTES(D), lds_len = lds_cu + 4u * (uint32_t)(a.batch + 1);
+  if (a.parts != 0) {
+    int* const cu_s = reinterpret_cast<int*>(lds + CK_LDS_BYTES(D));
     int* const len_s = cu_s + a.batch + 1;
     __shared__ int64_t wave_sums[WAVES];
     __shared__ int found[2][2];
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     __syncthreads();
     // every thread some row tiles in a row: their units, then the line's prefix sums
     const int per = (a.slots + THREADS - 1) / THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
-    auto walk = [&](auto&& visit) {  // visit(x, units in the line, tiles)
+    auto walk = [&](auto&& visit) {  // visit(x, units in the line, blocks)
       if (x0 >= x1) return;
       int b = 0, hi = a.batch;
       while (hi - b > 1) {
@@ -176,8 +176,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         if (rt < 0 || rt >= pg_row_tiles(q_len, a.group, TILE_ROWS)) continue;
         int p0, p1;
         pg_tile_positions(rt, q_len, len_s[b], a.group, TILE_ROWS, &p0, &p1);
-        const int tiles = pg_span_units(ck_span(a, p0, p1, CK_BLOCK));
-        visit(i, tiles + PG_OVERHEAD, tiles);
+        const int blocks = pg_span_units(ck_span(a, p0, p1, CK_BLOCK));
+        visit(i, blocks + PG_OVERHEAD, blocks);
       }
     };
     int64_t mine = 0;
@@ -200,13 +200,13 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     at -= mine;
     const int64_t parts = pg_parts(total, a.parts, PG_MIN_SHARE);
     const int64_t cut[2] = {part < parts ? pg_cut(total, parts, part) : total, part < parts ? pg_cut(total, parts, part + 1) : total};
-    walk([&](int i, int units, int tiles) {
+    walk([&](int i, int units, int blocks) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (cut[e] >= at && cut[e] < at + units) {
-          const int tile = pg_snap(cut[e] - at, tiles, PG_OVERHEAD);
-          found[e][0] = tile < tiles || tile == 0 ? i : i + 1;
-          found[e][1] = tile < tiles ? tile : 0;
+          const int tile = pg_snap(cut[e] - at, blocks, PG_OVERHEAD);
+          found[e][0] = tile < blocks || tile == 0 ? i : i + 1;
+          found[e][1] = tile < blocks ? tile : 0;
         }
       at += units;
     });
@@ -217,6 +217,54 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     tile_end = __builtin_amdgcn_readfirstlane(found[1][1]);
   }
   int4 note = make_int4(CK_NONE, -1, 0, 0);
+
+  // A row tile, or what of it falls to this workgroup: blocks i0 .. i1 - 1 of its walk.
+  struct Piece {
+    int b, rt, start, q_len, len, i0, i1, blocks;
+    PgSpan span;
+  };
+  // (LDS reads of its own: the compiler would wait for all that is in flight in front of them)
+  auto from_lds = [&](uint32_t at) {
+    int v;
+    asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(at));
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  auto start_of = [&](int b) { return a.cu != nullptr ? from_lds(lds_cu + 4u * b) : b * a.n_queries; };
+  int seq = a.parts == 0 || x >= a.slots ? 0 : __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, x, lane));
+  auto next_piece = [&](Piece& p) {  // false: there is none
+    for (;;) {
+      int begin = 0, here = x, end = -1;
+      if (a.parts == 0) {
+        // whole row tiles, there and back over the workgroups of the kv head: their work is even, and those that run at a time are neighbours
+        const int wgs = (int)(gridDim.x / a.hkv), place = turn * wgs + (turn & 1 ? wgs - 1 - part : part);
+        if (turn * (int64_t)wgs >= a.slots) return false;
+        ++turn;
+        if (place >= a.slots) continue;
+        here = a.slots - 1 - place;  // (the last rows of a prompt see the most keys)
+        seq = pg_min((int)((unsigned)here * (unsigned)TILE_ROWS / (unsigned)(a.n_queries * a.group + TILE_ROWS)), a.batch - 1);  // (or the one behind)
+      } else {
+        if (x >= a.slots || !(x < x_end || (x == x_end && tile_end > 0))) return false;
+        begin = tile_begin;
+        if (x == x_end) end = tile_end;
+        tile_begin = 0;
+        ++x;
+      }
+      while (seq + 1 < a.batch && pg_first_slot(start_of(seq + 1), a.group, seq + 1, TILE_ROWS) <= here) ++seq;
+      p.b = seq;
+      p.start = start_of(seq);
+      p.q_len = pg_max(0, start_of(seq + 1) - p.start);
+      p.len = a.lens != nullptr ? from_lds(lds_len + 4u * seq) : a.n_keys;
+      p.rt = (int)(here - pg_first_slot(p.start, a.group, seq, TILE_ROWS));
+      if (p.rt < 0 || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
+      int p0, p1;
+      pg_tile_positions(p.rt, p.q_len, p.len, a.group, TILE_ROWS, &p0, &p1);
+      p.span = ck_span(a, p0, p1, CK_BLOCK);
+      p.blocks = pg_span_units(p.span);
+      p.i0 = begin;
+      p.i1 = end >= 0 ? pg_min(end, p.blocks) : p.blocks;
+      return true;
+    }
+  };
 
   const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
   const int in_tile = wave * ROWS + lane / CHUNKS;                               // the lane's row of its wave's first instruction
@@ -230,101 +278,123 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   bf16x8 ones = __builtin_bit_cast(bf16x8, (at_u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   asm volatile("" : "+v"(ones));  // one register set throughout
 
-  int b = x < a.slots ? __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, x, lane)) : 0;
-  for (; x < a.slots && (x < x_end || (x == x_end && tile_end > 0)); ++x, tile_begin = 0) {
-    while (b + 1 < a.batch && pg_first_slot(ck_start(a, b + 1), a.group, b + 1, TILE_ROWS) <= x) ++b;
-    const int start = ck_start(a, b), q_len = pg_max(0, ck_start(a, b + 1) - start), len = ck_len(a, b);
-    const int rt = (int)(x - pg_first_slot(start, a.group, b, TILE_ROWS));
-    const int rows = q_len * a.group - rt * TILE_ROWS;  // from here to the sequence's end
-    if (rt < 0 || rows <= 0) continue;
-    int p0, p1;
-    pg_tile_positions(rt, q_len, len, a.group, TILE_ROWS, &p0, &p1);
-    const PgSpan span = ck_span(a, p0, p1, CK_BLOCK);
-    const int tiles = pg_span_units(span);
-    const int i_end = x == x_end ? pg_min(tile_end, tiles) : tiles;
-    const bool from_start = tile_begin == 0, to_end = i_end == tiles;  // (uniform)
-
-    // the lane's rows: token, head and position
-    int pos[QT];
-    bf16x8 qb[QT][4];
-    auto row_of = [&](int qt, int* token, int* head) {
-      const int r = rt * TILE_ROWS + pg_min(wave * 32 + 16 * qt + lq, rows - 1);
-      *token = (int)((unsigned)r / (unsigned)a.group);
-      *head = kvh * a.group + (r - *token * a.group);
-    };
+  // row of the lane's tile qt in a piece: token and head
+  auto row_of = [&](const Piece& c, int in_rows, int* token, int* head) {
+    const int r = c.rt * TILE_ROWS + pg_min(in_rows, c.q_len * a.group - c.rt * TILE_ROWS - 1);
+    *token = (int)((unsigned)r / (unsigned)a.group);
+    *head = kvh * a.group + (r - *token * a.group);
+  };
+  bf16x8 qb[QT][4];
+  auto load_q = [&](const Piece& c) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       int token, head;
-      row_of(qt, &token, &head);
-      pos[qt] = len - q_len + token;
-      const sp_bf16* src = a.q + b * a.sq_b + (int64_t)((PAGED ? start : 0) + token) * a.sq_n + head * a.sq_h + 8 * g;
+      row_of(c, wave * 32 + 16 * qt + lq, &token, &head);
+      const sp_bf16* src = a.q + c.b * a.sq_b + (int64_t)((PAGED ? c.start : 0) + token) * a.sq_n + head * a.sq_h + 8 * g;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qb[qt][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 32 * ks));
     }
+  };
+
+  // ---- a sequence's pages: 64 entries of its table at hand, a lane each, and the 64 behind them on their way ----
+  auto entries = [&](int b, int group) {
+    const int i = group * SP_WAVE + lane;
+    const int id = a.table[b * a.table_stride + pg_min(i, a.width - 1)];
+    return i < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
+  };
+  auto group_of = [&](int key) { return (key >> a.shift) >> 6; };  // (a block's pages lie in one group of 64)
+  // A block of a walk: its first key, its sequence's keys, the pages of this wave's instructions (-1: none), and which 16-key groups have
+  // none (bits).
+  struct Block {
+    int b, key0, len, id[2][ITS];
+    uint32_t lost;
+  };
+  auto block = [&](const Piece& p, int i, int ids) {
+    Block c;
+    c.b = p.b;
+    c.key0 = pg_span_unit(p.span, i) * CK_BLOCK;
+    c.len = p.len;
+    c.lost = 0;
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const int page = (c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS) >> a.shift;
+        c.id[hf][it] = PAGED ? __builtin_amdgcn_readlane(ids, page & 63) : page;
+      }
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i16 = 0; i16 < 8; ++i16)
+        c.lost |= (uint32_t)(__builtin_amdgcn_readlane(ids, ((c.key0 + 16 * i16) >> a.shift) & 63) < 0) << i16;
+    }
+    return c;
+  };
+  // half hf of a block into slot `sub` % 4 of a ring; want false: zeros, without a read
+  auto load = [&](const Block& c, int hf, int sub, bool want, const sp_bf16* x, int64_t stride_b, int64_t stride_page, int64_t stride_h,
+                  uint32_t row_bytes, uint32_t lane_off, uint32_t to) {
+    to += (uint32_t)((sub & 3) * SUB_BYTES + wave * 1024);
+    const char* const base = (const char*)(x + (PAGED ? 0 : c.b * stride_b) + kvh * stride_h);
+#pragma unroll
+    for (int it = 0; it < ITS; ++it) {
+      const int key = c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS, in = key & ((1 << a.shift) - 1), id = c.id[hf][it];
+      const int there = id < 0 || !want ? 0 : pg_max(0, pg_min(c.len - key, ROWS));  // rows that are there, as far as this instruction goes
+      const char* p = base + (int64_t)pg_max(id, 0) * (stride_page * 2) + (uint64_t)(uint32_t)in * row_bytes;
+      const __amdgpu_buffer_rsrc_t rsrc =
+          __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, there > 0 ? (int)((uint32_t)(there - 1) * row_bytes + 2u * D) : 0, 0x00027000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ck_lds_ptr)(uintptr_t)(to + it * WAVES * 1024), 16, (int)lane_off, 0, 0, 0);
+    }
+  };
+  auto load_k = [&](const Block& c, int hf, int sub, bool want) {
+    load(c, hf, sub, want, a.k, a.sk_b, a.sk_p, a.sk_h, k_row, k_lane, lds_base);
+  };
+  auto load_v = [&](const Block& c, int hf, int sub, bool want) {
+    load(c, hf, sub, want, a.v, a.sv_b, a.sv_p, a.sv_h, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
+  };
+
+  // Block n of the workgroup (over all its pieces) is sub-tiles 2 n and 2 n + 1; sub-tile s lives in slot s % 4 of either ring.  One wait and
+  // barrier per block: while it is computed on (K of 2 n, 2 n + 1, V of 2 n - 1, 2 n: P . V trails by a sub-tile) K of 2 n + 2, 2 n + 3 and V of
+  // 2 n + 1, 2 n + 2 are on their way, sent out in four parts between the block's steps.  Behind a piece's last block that is the next piece's
+  // first one: its tiles land, and its queries, under the end of the piece in front.
+  Piece cur_p, next_p;
+  bool have = next_piece(cur_p), primed = false;
+  Block cur = {}, nxt = {};
+  int n = 0, ids_first = 0;
+  if (have) load_q(cur_p);
+  if (PAGED && have) ids_first = entries(cur_p.b, group_of(pg_span_unit(cur_p.span, cur_p.i0) * CK_BLOCK));
+  while (have) {
+    const Piece pc = cur_p;
+    const bool have_next = next_piece(next_p);
+    const int b = pc.b, rt = pc.rt, start = pc.start, q_len = pc.q_len, len = pc.len, n_blk = pc.i1 - pc.i0;
+    const int rows = q_len * a.group - rt * TILE_ROWS;  // from here to the sequence's end
+    const bool from_start = pc.i0 == 0, to_end = pc.i1 == pc.blocks;  // (uniform)
     const bool has_rows = wave * 32 < rows;  // (uniform in the wave)
     // positions of the wave's first and last row
     const int w0 = len - q_len + (int)((unsigned)(rt * TILE_ROWS + pg_min(wave * 32, rows - 1)) / (unsigned)a.group);
     const int w1 = len - q_len + (int)((unsigned)(rt * TILE_ROWS + pg_min(wave * 32 + 31, rows - 1)) / (unsigned)a.group);
-
-    // ---- the sequence's pages: 64 entries of its table at hand, a lane each, and the 64 behind them on their way ----
-    const int32_t* const table = PAGED ? a.table + b * a.table_stride : nullptr;
-    int ids = 0, ids_next = 0, ids_group = -2;
-    auto entries = [&](int group) {
-      const int i = group * SP_WAVE + lane;
-      const int id = table[pg_min(i, a.width - 1)];
-      return i < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
-    };
-    auto turn_to = [&](int page) {  // (a block's pages lie in one group of 64)
-      const int group = page >> 6;
-      if (group != ids_group) {
-        ids = group == ids_group + 1 ? ids_next : entries(group);
-        ids_next = entries(group + 1);
-        ids_group = group;
-      }
-    };
-    const char* const kh = (const char*)(a.k + b * a.sk_b + kvh * a.sk_h);
-    const char* const vh = (const char*)(a.v + b * a.sv_b + kvh * a.sv_h);
-    // A block of the walk: its first key, the pages of this wave's instructions (-1: none), and which 16-key groups have none (bits).
-    struct Block {
-      int key0, id[2][ITS];
-      uint32_t lost;
-    };
-    auto block = [&](int i) {
-      Block c;
-      c.key0 = pg_span_unit(span, i) * CK_BLOCK;
-      c.lost = 0;
-      if constexpr (PAGED) turn_to(c.key0 >> a.shift);
+    int pos[QT];
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-        for (int it = 0; it < ITS; ++it) {
-          const int page = (c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS) >> a.shift;
-          c.id[hf][it] = PAGED ? __builtin_amdgcn_readlane(ids, page & 63) : page;
-        }
+    for (int qt = 0; qt < QT; ++qt) {
+      int token, head;
+      row_of(pc, wave * 32 + 16 * qt + lq, &token, &head);
+      pos[qt] = len - q_len + token;
+    }
+    const int key_first = n_blk > 0 ? pg_span_unit(pc.span, pc.i0) * CK_BLOCK : 0;
+    int ids = ids_first, ids_group = group_of(key_first), ids_next = 0;
+    const bool next_blocks = have_next && next_p.i1 > next_p.i0;  // the next piece has a first block to fetch
+    if constexpr (PAGED) {
+      ids_next = entries(b, ids_group + 1);
+      if (next_blocks) ids_first = entries(next_p.b, group_of(pg_span_unit(next_p.span, next_p.i0) * CK_BLOCK));
+    }
+    auto block_at = [&](int i) {
       if constexpr (PAGED) {
-#pragma unroll
-        for (int i16 = 0; i16 < 8; ++i16)
-          c.lost |= (uint32_t)(__builtin_amdgcn_readlane(ids, ((c.key0 + 16 * i16) >> a.shift) & 63) < 0) << i16;
+        const int group = group_of(pg_span_unit(pc.span, i) * CK_BLOCK);
+        if (group != ids_group) {
+          ids = group == ids_group + 1 ? ids_next : entries(b, group);
+          ids_next = entries(b, group + 1);
+          ids_group = group;
+        }
       }
-      return c;
-    };
-    // half hf of a block into slot `sub` % 4 of a ring; want false: zeros, without a read
-    auto load = [&](const Block& c, int hf, int sub, bool want, const char* x, int64_t stride_page, uint32_t row_bytes, uint32_t lane_off,
-                    uint32_t to) {
-      to += (uint32_t)((sub & 3) * SUB_BYTES + wave * 1024);
-#pragma unroll
-      for (int it = 0; it < ITS; ++it) {
-        const int key = c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS, in = key & ((1 << a.shift) - 1), id = c.id[hf][it];
-        const int there = id < 0 || !want ? 0 : pg_max(0, pg_min(len - key, ROWS));  // rows that are there, as far as this instruction goes
-        const char* p = x + (int64_t)pg_max(id, 0) * (stride_page * 2) + (uint64_t)(uint32_t)in * row_bytes;
-        const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, there > 0 ? (int)((uint32_t)(there - 1) * row_bytes + 2u * D) : 0, 0x00027000);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ck_lds_ptr)(uintptr_t)(to + it * WAVES * 1024), 16, (int)lane_off, 0, 0, 0);
-      }
-    };
-    auto load_k = [&](const Block& c, int hf, int sub, bool want) { load(c, hf, sub, want, kh, a.sk_p, k_row, k_lane, lds_base); };
-    auto load_v = [&](const Block& c, int hf, int sub, bool want) {
-      load(c, hf, sub, want, vh, a.sv_p, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
+      return block(pc, i, ids);
     };
 
     floatx4 o[9][2];  // [channel tile][row tile]; o[8]: the row sums (ones . P)
@@ -335,109 +405,137 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     float m[QT] = {AT_NO_MAX, AT_NO_MAX}, l_mark[QT] = {0.f, 0.f};
     uint32_t det[2] = {0u, 0u};
 
-    __syncthreads();  // the LDS is free: the plan has been read, the row tile in front is done with its last block
-    const int n_blk = i_end - tile_begin;
     if (n_blk > 0) {
-      // Block bb of the walk is sub-tiles 2 bb and 2 bb + 1; sub-tile s lives in slot s % 4 of either ring.  One wait and barrier per block:
-      // while it is computed on (K of 2 bb, 2 bb + 1, V of 2 bb - 1, 2 bb: P . V trails by a sub-tile) K of 2 bb + 2, 2 bb + 3 and V of
-      // 2 bb + 1, 2 bb + 2 are on their way, sent out in four parts between the block's steps.
-      Block cur = block(tile_begin), nxt = cur;
-      load_k(cur, 0, 0, true);
-      load_k(cur, 1, 1, true);
-      load_v(cur, 0, 0, true);
-      int bb = 0;
+      if (primed) {
+        cur = nxt;
+      } else {
+        __syncthreads();  // the rings are free
+        cur = block_at(pc.i0);
+        load_k(cur, 0, 2 * n, true);
+        load_k(cur, 1, 2 * n + 1, true);
+        load_v(cur, 0, 2 * n, true);
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      }
+      const int n_last = n + n_blk - 1;
       bool more = false;  // there is a block behind this one
       CkAddr<D> ad;
-      auto top = [&]() {
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");  // everybody's loads have landed, everybody is past the block in front
-        more = bb + 1 < n_blk;
-        if (more) nxt = block(tile_begin + bb + 1);
-        const uint32_t k_at = lds_base + (uint32_t)(((2 * bb) & 3) * SUB_BYTES), v_at = lds_base + CK_RING * SUB_BYTES;
+      auto top = [&](bool wait) {
+        // everybody's loads have landed, everybody is past the block in front
+        if (wait) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        more = n < n_last || next_blocks;
+        if (n < n_last)
+          nxt = block_at(pc.i1 - (n_last - n));
+        else if (next_blocks)
+          nxt = block(next_p, next_p.i0, ids_first);
+        const uint32_t k_at = lds_base + (uint32_t)(((2 * n) & 3) * SUB_BYTES), v_at = lds_base + CK_RING * SUB_BYTES;
         ad.ka = k_at + koff;
-        ad.va[0] = v_at + (uint32_t)(((2 * bb + 3) & 3) * SUB_BYTES) + voff;
-        ad.va[1] = v_at + (uint32_t)(((2 * bb) & 3) * SUB_BYTES) + voff;
+        ad.va[0] = v_at + (uint32_t)(((2 * n + 3) & 3) * SUB_BYTES) + voff;
+        ad.va[1] = v_at + (uint32_t)(((2 * n) & 3) * SUB_BYTES) + voff;
       };
       auto feed = [&](int part) {
-        if (part == 0) load_k(nxt, 0, 2 * bb + 2, more);
-        if (part == 1) load_k(nxt, 1, 2 * bb + 3, more);
-        if (part == 2) load_v(cur, 1, 2 * bb + 1, true);
-        if (part == 3) load_v(nxt, 0, 2 * bb + 2, more);
+        if (part == 0) load_k(nxt, 0, 2 * n + 2, more);
+        if (part == 1) load_k(nxt, 1, 2 * n + 3, more);
+        if (part == 2) load_v(cur, 1, 2 * n + 1, true);
+        if (part == 3) load_v(nxt, 0, 2 * n + 2, more);
       };
       // what the wave's rows do not see of a block: nothing to take out in most of them
       auto partly = [&](const Block& c) {
         const int key0 = c.key0, key1 = key0 + CK_BLOCK - 1;
-        return key1 > w0 || (key0 <= w1 - a.window && key1 >= a.sinks) || c.lost != 0;
+        return (key1 > w0 ? 1 : 0) | (key0 <= w1 - a.window && key1 >= a.sinks ? 2 : 0) | (c.lost != 0 ? 4 : 0);
       };
       struct Mask {
-        bool some;
-        int key0, window, sinks, p0, p1;  // (of the half-tile; positions of the lane's rows)
+        int what;            // 1: keys behind rows, 2: keys in front of windows, 4: keys without a page
+        int key0, p0, p1, window, sinks;  // the half-tile's first key, positions of the lane's rows
         uint32_t lost;
         __device__ __forceinline__ void operator()(floatx4 (&s)[2][2]) const {
-          if (!some) return;
+          if (what == 0) return;
           const int key = key0 + 4 * ((threadIdx.x >> 4) & 3);
+          const int h[2] = {p0 - key, p1 - key};
+          if (what & 1) {
 #pragma unroll
-          for (int kt = 0; kt < 2; ++kt)
+            for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const bool gone = (lost >> kt) & 1u;
-              if (gone || !pg_sees(p0, key + 16 * kt + j, window, sinks)) s[kt][0][j] = -INFINITY;
-              if (gone || !pg_sees(p1, key + 16 * kt + j, window, sinks)) s[kt][1][j] = -INFINITY;
-            }
+              for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[kt][qt][j] = 16 * kt + j <= h[qt] ? s[kt][qt][j] : -INFINITY;
+          }
+          if (what & 2) {
+            const int front = sinks - key, lo[2] = {h[0] - window, h[1] - window};
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int qt = 0; qt < 2; ++qt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  s[kt][qt][j] = 16 * kt + j > lo[qt] || 16 * kt + j < front ? s[kt][qt][j] : -INFINITY;
+          }
+          if (what & 4) {
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+              if ((lost >> kt) & 1u) s[kt][0] = s[kt][1] = (floatx4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          }
         }
       };
-      auto masked = [&](const Block& c, bool some, int quarter) {
-        return Mask{some, c.key0 + 32 * quarter, a.window, a.sinks, pos[0], pos[1], c.lost >> (2 * quarter)};
+      auto masked = [&](const Block& c, int what, int quarter) {
+        return Mask{what, c.key0 + 32 * quarter, pos[0], pos[1], a.window, a.sinks, c.lost >> (2 * quarter)};
       };
       constexpr int MODE = HALF ? 2 : 0;
       if (!has_rows) {
-        for (; bb < n_blk; ++bb) {
-          top();
-          feed(0), feed(1), feed(2), feed(3);
+        top(false);
+        feed(0), feed(1), feed(2), feed(3);
+        for (++n; n <= n_last; ++n) {
           cur = nxt;
+          top(true);
+          feed(0), feed(1), feed(2), feed(3);
         }
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (have_next) load_q(next_p);
       } else {
         floatx4 sa[2][2], sb[2][2];  // [key tile][row tile]
         bf16x8 pa[2], pb[2];         // [row tile]
-        bf16x8 pre[2];               // the next stage's first two LDS operands, in flight (at_prefetch_qk)
+        bf16x8 pre[2];
         Block old = cur;
-        bool some = partly(cur), some_old = some;
+        int some = partly(cur), some_old = some;
         // ---- start: S of the first half-tile, nothing to overlap with yet ----
-        top();
+        top(false);
         feed(0);
         ck_qk_only<0, HALF>(ad, qb, sa);
         feed(1);
-        at_step<true, false, 1, 0, 0, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+        at_step<true, false, 1, 0, 0, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
         feed(2);
-        at_step<true, true, 2, 1, 0, MODE, false, -1>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
+        at_step<true, true, 2, 1, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
         feed(3);
-        at_step<true, true, 3, 1, 1, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
+        at_step<true, true, 3, 1, 1, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
         // ---- steady: four steps per block ----
-        for (bb = 1; bb < n_blk; ++bb) {
+        for (++n; n <= n_last; ++n) {
           old = cur, some_old = some;
           cur = nxt;
           some = partly(cur);
-          top();
+          top(true);
           if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(1);
-          at_step<true, true, 0, 0, 0, MODE, false, -1>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(old, some_old, 3), l_mark, pre);
+          at_step<true, true, 0, 0, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(old, some_old, 3), l_mark, pre);
           feed(0);
-          at_step<true, true, 1, 0, 1, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+          at_step<true, true, 1, 0, 1, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
           if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(0);
           feed(1);
           feed(2);
-          at_step<true, true, 2, 1, 0, MODE, false, -1>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
+          at_step<true, true, 2, 1, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
           feed(3);
-          at_step<true, true, 3, 1, 1, MODE, false, -1>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
+          at_step<true, true, 3, 1, 1, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
         }
-        // ---- drain: the last half-tile and its P . V (V of sub-tile 2 n_blk - 1) ----
+        // ---- drain: the last half-tile and its P . V (V of the last block's second sub-tile) ----
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        ad.va[0] = lds_base + CK_RING * SUB_BYTES + (uint32_t)(((2 * n_blk + 3) & 3) * SUB_BYTES) + voff;
+        if (have_next) load_q(next_p);
+        ad.va[0] = lds_base + CK_RING * SUB_BYTES + (uint32_t)(((2 * n + 3) & 3) * SUB_BYTES) + voff;
         at_step<false, true, 0, 0, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 3), l_mark, pre);
         at_commit<MODE>(sb, pb, det, o, a.scale_log2, m, l_mark);
         ck_pv_only<0, 1, HALF>(ad, pb, o, ones);
         at_settle_o(o);
       }
+    } else if (have_next) {
+      load_q(next_p);
     }
+    primed = n_blk > 0 && next_blocks;
     const float l[QT] = {o[8][0][0], o[8][1][0]};
 
     // ---- what has come of it: the rows, or a partial ----
@@ -457,7 +555,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       const int in_rows = wave * 32 + 16 * qt + lq;
       const bool mine = in_rows < rows;
       int token, head;
-      row_of(qt, &token, &head);
+      row_of(pc, in_rows, &token, &head);
       spoilt[qt] = false;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
@@ -502,18 +600,18 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         const sp_bf16* qrow = a.q + b * a.sq_b + (int64_t)((PAGED ? start : 0) + token) * a.sq_n + head * a.sq_h;
         constexpr int CL = D / SP_WAVE;  // channels of a lane
         float acc[CL] = {0.f}, sum = 0.f, top = CK_NO_MAX;
-        for (int i = 2 * tile_begin; i < 2 * i_end; ++i) {
-          const int key = pg_span_unit(span, i >> 1) * CK_BLOCK + (i & 1) * SP_WAVE + lane, page = key >> a.shift;
+        for (int i = 2 * pc.i0; i < 2 * pc.i1; ++i) {
+          const int key = pg_span_unit(pc.span, i >> 1) * CK_BLOCK + (i & 1) * SP_WAVE + lane, page = key >> a.shift;
           int id = page;
           if constexpr (PAGED) {
-            id = page < a.width ? table[page] : -1;
+            id = page < a.width ? a.table[b * a.table_stride + page] : -1;
             if ((unsigned)id >= (unsigned)a.num_pages) id = -1;
           }
           const bool seen = id >= 0 && key < len && pg_sees(p, key, a.window, a.sinks);
           const int64_t in = key & ((1 << a.shift) - 1);
           float logit = -INFINITY;
           if (seen) {
-            const sp_bf16* krow = (const sp_bf16*)kh + id * a.sk_p + in * a.sk_n;
+            const sp_bf16* krow = a.k + b * a.sk_b + kvh * a.sk_h + id * a.sk_p + in * a.sk_n;
             float dot = 0.f;
             for (int c = 0; c < D; ++c) dot = __builtin_fmaf(sp_bf16_to_f32(qrow[c]), sp_bf16_to_f32(krow[c]), dot);
             logit = dot * a.scale_log2;
@@ -527,7 +625,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           const int64_t v_at = id < 0 ? 0 : id * a.sv_p + in * a.sv_n;
           for (uint64_t left = __ballot(seen); left != 0ull; left &= left - 1ull) {
             const int j = __builtin_ctzll(left);
-            const sp_bf16* vrow_j = (const sp_bf16*)vh + __shfl(v_at, j, SP_WAVE) + lane * CL;
+            const sp_bf16* vrow_j = a.v + b * a.sv_b + kvh * a.sv_h + __shfl(v_at, j, SP_WAVE) + lane * CL;
             const float w = __shfl(weight, j, SP_WAVE);
 #pragma unroll
             for (int c = 0; c < CL; ++c) acc[c] = __builtin_fmaf(w, sp_bf16_to_f32(vrow_j[c]), acc[c]);
@@ -543,6 +641,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         if (!whole && lane == 0) ml_to[in_rows] = make_float2(top, sum);
       }
     }
+    cur_p = next_p;
+    have = have_next;
   }
   if (a.parts != 0 && t == 0) a.notes[blockIdx.x] = note;
 }
@@ -554,25 +654,27 @@ struct CkPlan {
 };
 // Workgroups that are resident at once: two a CU with 128 channels.
 #define CK_PLACES 256
-static CkPlan ck_plan(int64_t tokens, int32_t batch, int32_t hkv, int32_t group, int32_t d) {
+static CkPlan ck_plan(int64_t tokens, int32_t batch, int32_t hkv, int32_t group, bool uniform) {
   CkPlan p;
   p.slots = pg_slots(tokens, group, batch, CK_ROWS);
   const int64_t room = CK_PLACES / hkv;
-  p.parts = p.slots * hkv >= 4 * CK_PLACES ? 0 : (int)(room < 1 ? 1 : room);
-  p.grid = (p.parts == 0 ? p.slots : p.parts) * hkv;
+  const int64_t wgs = room < 1 ? 1 : room;  // of a kv head
+  p.parts = uniform && p.slots >= 4 * wgs ? 0 : (int)wgs;
+  p.grid = wgs * hkv;
   return p;
 }
-static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d) {
+static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, bool uniform) {
   if (tokens <= 0 || batch <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || (d != 64 && d != 128)) return 0;
-  const CkPlan p = ck_plan(tokens, batch, hkv, hq / hkv, d);
+  const CkPlan p = ck_plan(tokens, batch, hkv, hq / hkv, uniform);
   return p.parts == 0 ? 0 : (size_t)p.grid * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
 static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* workspace, size_t workspace_bytes, hipStream_t s) {
-  const CkPlan plan = ck_plan(a.tokens, a.batch, a.hkv, a.group, d);
+  const bool uniform = a.cu == nullptr && a.lens == nullptr;  // as many queries and keys in every sequence
+  const CkPlan plan = ck_plan(a.tokens, a.batch, a.hkv, a.group, uniform);
   SP_REQUIRE(plan.grid <= 0x7fffffffll && (int64_t)a.tokens * a.group < (1ll << 31), SP_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are too many",
              who, a.tokens, hq);
-  const size_t need = ck_workspace_bytes(a.tokens, a.batch, hq, a.hkv, d);
+  const size_t need = ck_workspace_bytes(a.tokens, a.batch, hq, a.hkv, d, uniform);
   SP_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), SP_ERR_WORKSPACE,
              "%s: workspace too small or misaligned", who);
   a.slots = (int)plan.slots;
@@ -580,8 +682,8 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* wo
   a.o_part = (float*)workspace;
   a.ml_part = (float2*)(a.o_part + (size_t)plan.grid * 2 * (size_t)CK_ROWS * d);
   a.notes = (int4*)(a.ml_part + (size_t)plan.grid * 2 * CK_ROWS);
-  const size_t plan_lds = (size_t)(2 * a.batch + 1) * sizeof(int);
-  const size_t lds = plan_lds > (size_t)CK_LDS_BYTES(d) ? plan_lds : (size_t)CK_LDS_BYTES(d);
+  SP_REQUIRE(a.batch <= CK_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %d (at most %d, single tokens %d)", who, a.batch, CK_MAX_SEQS, PG_MAX_SEQS);
+  const size_t lds = CK_LDS_BYTES(d) + (plan.parts != 0 ? (size_t)(2 * a.batch + 1) * sizeof(int) : 0);
   auto go = [&](auto kernel, auto merge) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(CK_THREADS), lds, s, a);
     if (plan.parts != 0) hipLaunchKernelGGL(merge, dim3((unsigned)plan.grid, CK_ROWS / CM_ROWS), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
@@ -593,7 +695,7 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* wo
   if (!attr_set[dev]) {
     const void* kernels[4] = {(const void*)sp_chunk_kernel<64, false>, (const void*)sp_chunk_kernel<64, true>,
                               (const void*)sp_chunk_kernel<128, false>, (const void*)sp_chunk_kernel<128, true>};
-    for (const void* f : kernels) SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, CK_LDS_BYTES(128)));
+    for (const void* f : kernels) SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, CK_LDS_BYTES(128) + (2 * CK_MAX_SEQS + 1) * (int)sizeof(int)));
     attr_set[dev] = true;
   }
   if (d == 64)
@@ -620,7 +722,7 @@ static bool ck_rows_ok(int64_t stride_n) { return stride_n >= 0 && stride_n < (1
 extern "C" size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens) {
   if (single_tokens && tokens > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128))
     return pd_workspace_bytes(hkv, d);
-  return ck_workspace_bytes(tokens, batch, hq, hkv, d);
+  return ck_workspace_bytes(tokens, batch, hq, hkv, d, false);
 }
 
 extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
@@ -664,7 +766,7 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
 
 extern "C" size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d) {
   (void)n_keys;
-  return batch <= 0 || n <= 0 ? 0 : sp_paged_attn_workspace_bytes(batch * n, batch, hq, hkv, d, n == 1);
+  return batch <= 0 || n <= 0 ? 0 : n == 1 ? sp_paged_attn_workspace_bytes(batch, batch, hq, hkv, d, 1) : ck_workspace_bytes(batch * n, batch, hq, hkv, d, true);
 }
 
 extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
