@@ -267,9 +267,11 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   };
 
   const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
-  const int in_tile = wave * ROWS + lane / CHUNKS;                               // the lane's row of its wave's first instruction
-  const uint32_t k_lane = (uint32_t)(lane / CHUNKS) * k_row + 16u * ((lane % CHUNKS) ^ ck_swz_k<D>(in_tile));
-  const uint32_t v_lane = (uint32_t)(lane / CHUNKS) * v_row + 16u * ((lane % CHUNKS) ^ ck_swz_v<D>(in_tile));
+  // The lane's place in what its wave's instructions fetch: its row of the page where a page is smaller than a sub-tile (an instruction of all
+  // waves is 32 rows, 64 of 64 channels: the place in the page is the same for all), of the sub-tile else.
+  const int in_sub = wave * ROWS + lane / CHUNKS, in_page = 1 << a.shift < CK_SUB ? in_sub & ((1 << a.shift) - 1) : in_sub;
+  const uint32_t k_lane = (uint32_t)in_page * k_row + 16u * ((lane % CHUNKS) ^ ck_swz_k<D>(in_sub));
+  const uint32_t v_lane = (uint32_t)in_page * v_row + 16u * ((lane % CHUNKS) ^ ck_swz_v<D>(in_sub));
   // LDS byte offsets of the lane's operands inside a sub-tile: K row lq, chunk g; V row 4 g + lq / 4, 8-byte piece lq % 4 of the 32 bytes of
   // channel tile 0.  Other steps and tiles are one XOR away, rows 16 further have the same swizzle.
   const uint32_t koff = (uint32_t)(lq * (D * 2) + ((g ^ ck_swz_k<D>(lq)) << 4));
@@ -296,71 +298,90 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     }
   };
 
-  // ---- a sequence's pages: 64 entries of its table at hand, a lane each, and the 64 behind them on their way ----
+  // ---- a sequence's pages: 64 of them at hand, a lane each ----
+  // A lane knows where its page's rows of K and V start and how many bytes of them there are, up to the sequence's end (none: no page): that is
+  // what a load's buffer descriptor is made of, three lane reads a load.  Formed from scalars where it is needed it took a fifth of the waves'
+  // instructions (65001 keys in pages of 128 2036 -> 1885 us with one descriptor a sub-tile instead of two).
+  // Without a table a page is 64 keys of the tensor.
+  struct Window {
+    int k_lo, k_hi, k_bytes, v_lo, v_hi, v_bytes, group;  // group: pages 64 group .. 64 group + 63
+    uint64_t lost;                                        // lanes without a page
+  };
+  Window win = {0, 0, 0, 0, 0, 0, -2, 0ull};
   auto entries = [&](int b, int group) {
     const int i = group * SP_WAVE + lane;
+    if constexpr (!PAGED) return i;
     const int id = a.table[b * a.table_stride + pg_min(i, a.width - 1)];
     return i < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
   };
-  auto group_of = [&](int key) { return (key >> a.shift) >> 6; };  // (a block's pages lie in one group of 64)
-  // A block of a walk: its first key, its sequence's keys, the pages of this wave's instructions (-1: none), and which 16-key groups have
-  // none (bits).
-  struct Block {
-    int b, key0, len, id[2][ITS];
-    uint32_t lost;
+  auto turn_to = [&](int b, int len, int group, int id) {
+    const int rows = id < 0 ? 0 : pg_max(0, pg_min(len - ((group * SP_WAVE + lane) << a.shift), 1 << a.shift));
+    auto at = [&](const sp_bf16* x, int64_t stride_b, int64_t stride_page, int64_t stride_h) {
+      return (uint64_t)(x + (PAGED ? 0 : b * stride_b) + kvh * stride_h) + (uint64_t)pg_max(id, 0) * (uint64_t)(stride_page * 2);
+    };
+    const uint64_t k_at = at(a.k, a.sk_b, a.sk_p, a.sk_h), v_at = at(a.v, a.sv_b, a.sv_p, a.sv_h);
+    win.k_lo = (int)(uint32_t)k_at, win.k_hi = (int)(uint32_t)(k_at >> 32);
+    win.v_lo = (int)(uint32_t)v_at, win.v_hi = (int)(uint32_t)(v_at >> 32);
+    win.k_bytes = rows > 0 ? (int)((uint32_t)(rows - 1) * k_row + 2u * D) : 0;
+    win.v_bytes = rows > 0 ? (int)((uint32_t)(rows - 1) * v_row + 2u * D) : 0;
+    win.group = group;
+    if constexpr (PAGED) win.lost = __ballot(id < 0);
   };
-  auto block = [&](const Piece& p, int i, int ids) {
-    Block c;
-    c.b = p.b;
-    c.key0 = pg_span_unit(p.span, i) * CK_BLOCK;
-    c.len = p.len;
-    c.lost = 0;
+  auto group_of = [&](int key) { return (key >> a.shift) >> 6; };  // (a block's pages lie in one group of 64)
+  // half hf of the block at key0 into slot `sub` % 4 of a ring; want false: zeros, without a read
+  auto load = [&](int key0, int hf, int sub, bool want, int lo, int hi, int bytes, uint32_t row_bytes, uint32_t lane_off, uint32_t to) {
+    to += (uint32_t)((sub & 3) * SUB_BYTES + wave * 1024);
+    auto rsrc_of = [&](int key) {
+      const int i = (key >> a.shift) & 63;
+      const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, i) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32;
+      return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, want ? __builtin_amdgcn_readlane(bytes, i) : 0, 0x00027000);
+    };
+    const int first = key0 + hf * CK_SUB;
+    if (!PAGED || 1 << a.shift >= CK_SUB) {  // (uniform)
+      const __amdgpu_buffer_rsrc_t rsrc = rsrc_of(first);
+      const uint32_t off = lane_off + (PAGED ? (uint32_t)(first & ((1 << a.shift) - 1)) * row_bytes : 0u);
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf)
+      for (int it = 0; it < ITS; ++it)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ck_lds_ptr)(uintptr_t)(to + it * WAVES * 1024), 16,
+                                                 (int)(off + (uint32_t)(it * WAVES * ROWS) * row_bytes), 0, 0, 0);
+    } else {
 #pragma unroll
       for (int it = 0; it < ITS; ++it) {
-        const int page = (c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS) >> a.shift;
-        c.id[hf][it] = PAGED ? __builtin_amdgcn_readlane(ids, page & 63) : page;
+        const __amdgpu_buffer_rsrc_t rsrc = rsrc_of(first + (it * WAVES + wave) * ROWS);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ck_lds_ptr)(uintptr_t)(to + it * WAVES * 1024), 16, (int)lane_off, 0, 0, 0);
       }
-    if constexpr (PAGED) {
+    }
+  };
+  auto load_k = [&](int key0, int hf, int sub, bool want) { load(key0, hf, sub, want, win.k_lo, win.k_hi, win.k_bytes, k_row, k_lane, lds_base); };
+  auto load_v = [&](int key0, int hf, int sub, bool want) {
+    load(key0, hf, sub, want, win.v_lo, win.v_hi, win.v_bytes, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
+  };
+  // A block of a walk: its first key, and which of its 16-key groups have no page (bits).
+  struct Block {
+    int key0;
+    uint32_t lost;
+  };
+  auto block = [&](int key0) {
+    Block c = {key0, 0u};
+    if (PAGED && win.lost != 0ull) {  // (uniform)
 #pragma unroll
-      for (int i16 = 0; i16 < 8; ++i16)
-        c.lost |= (uint32_t)(__builtin_amdgcn_readlane(ids, ((c.key0 + 16 * i16) >> a.shift) & 63) < 0) << i16;
+      for (int i16 = 0; i16 < 8; ++i16) c.lost |= (uint32_t)((win.lost >> (((key0 + 16 * i16) >> a.shift) & 63)) & 1ull) << i16;
     }
     return c;
   };
-  // half hf of a block into slot `sub` % 4 of a ring; want false: zeros, without a read
-  auto load = [&](const Block& c, int hf, int sub, bool want, const sp_bf16* x, int64_t stride_b, int64_t stride_page, int64_t stride_h,
-                  uint32_t row_bytes, uint32_t lane_off, uint32_t to) {
-    to += (uint32_t)((sub & 3) * SUB_BYTES + wave * 1024);
-    const char* const base = (const char*)(x + (PAGED ? 0 : c.b * stride_b) + kvh * stride_h);
-#pragma unroll
-    for (int it = 0; it < ITS; ++it) {
-      const int key = c.key0 + hf * CK_SUB + (it * WAVES + wave) * ROWS, in = key & ((1 << a.shift) - 1), id = c.id[hf][it];
-      const int there = id < 0 || !want ? 0 : pg_max(0, pg_min(c.len - key, ROWS));  // rows that are there, as far as this instruction goes
-      const char* p = base + (int64_t)pg_max(id, 0) * (stride_page * 2) + (uint64_t)(uint32_t)in * row_bytes;
-      const __amdgpu_buffer_rsrc_t rsrc =
-          __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, there > 0 ? (int)((uint32_t)(there - 1) * row_bytes + 2u * D) : 0, 0x00027000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ck_lds_ptr)(uintptr_t)(to + it * WAVES * 1024), 16, (int)lane_off, 0, 0, 0);
-    }
-  };
-  auto load_k = [&](const Block& c, int hf, int sub, bool want) {
-    load(c, hf, sub, want, a.k, a.sk_b, a.sk_p, a.sk_h, k_row, k_lane, lds_base);
-  };
-  auto load_v = [&](const Block& c, int hf, int sub, bool want) {
-    load(c, hf, sub, want, a.v, a.sv_b, a.sv_p, a.sv_h, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
-  };
+  auto key_of = [&](const Piece& p, int i) { return pg_span_unit(p.span, i) * CK_BLOCK; };
 
   // Block n of the workgroup (over all its pieces) is sub-tiles 2 n and 2 n + 1; sub-tile s lives in slot s % 4 of either ring.  One wait and
   // barrier per block: while it is computed on (K of 2 n, 2 n + 1, V of 2 n - 1, 2 n: P . V trails by a sub-tile) K of 2 n + 2, 2 n + 3 and V of
-  // 2 n + 1, 2 n + 2 are on their way, sent out in four parts between the block's steps.  Behind a piece's last block that is the next piece's
+  // 2 n + 1, 2 n + 2 are on their way, sent out in four parts between the block's steps, V of 2 n + 1 first: the others are the next block's, whose
+  // pages may be others.  Behind a piece's last block that is the next piece's
   // first one: its tiles land, and its queries, under the end of the piece in front.
   Piece cur_p, next_p;
   bool have = next_piece(cur_p), primed = false;
-  Block cur = {}, nxt = {};
+  Block cur = {0, 0u}, nxt = {0, 0u};
   int n = 0, ids_first = 0;
   if (have) load_q(cur_p);
-  if (PAGED && have) ids_first = entries(cur_p.b, group_of(pg_span_unit(cur_p.span, cur_p.i0) * CK_BLOCK));
+  if (have) ids_first = entries(cur_p.b, group_of(key_of(cur_p, cur_p.i0)));
   while (have) {
     const Piece pc = cur_p;
     const bool have_next = next_piece(next_p);
@@ -378,24 +399,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       row_of(pc, wave * 32 + 16 * qt + lq, &token, &head);
       pos[qt] = len - q_len + token;
     }
-    const int key_first = n_blk > 0 ? pg_span_unit(pc.span, pc.i0) * CK_BLOCK : 0;
-    int ids = ids_first, ids_group = group_of(key_first), ids_next = 0;
     const bool next_blocks = have_next && next_p.i1 > next_p.i0;  // the next piece has a first block to fetch
-    if constexpr (PAGED) {
-      ids_next = entries(b, ids_group + 1);
-      if (next_blocks) ids_first = entries(next_p.b, group_of(pg_span_unit(next_p.span, next_p.i0) * CK_BLOCK));
-    }
-    auto block_at = [&](int i) {
-      if constexpr (PAGED) {
-        const int group = group_of(pg_span_unit(pc.span, i) * CK_BLOCK);
-        if (group != ids_group) {
-          ids = group == ids_group + 1 ? ids_next : entries(b, group);
-          ids_next = entries(b, group + 1);
-          ids_group = group;
-        }
-      }
-      return block(pc, i, ids);
-    };
+    int ids_next = 0, ids_here = ids_first;
+    if (n_blk > 0) ids_next = entries(b, group_of(key_of(pc, pc.i0)) + 1);
+    if (next_blocks) ids_first = entries(next_p.b, group_of(key_of(next_p, next_p.i0)));
 
     floatx4 o[9][2];  // [channel tile][row tile]; o[8]: the row sums (ones . P)
 #pragma unroll
@@ -410,10 +417,12 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         cur = nxt;
       } else {
         __syncthreads();  // the rings are free
-        cur = block_at(pc.i0);
-        load_k(cur, 0, 2 * n, true);
-        load_k(cur, 1, 2 * n + 1, true);
-        load_v(cur, 0, 2 * n, true);
+        const int key0 = key_of(pc, pc.i0);
+        turn_to(b, len, group_of(key0), ids_here);
+        cur = block(key0);
+        load_k(key0, 0, 2 * n, true);
+        load_k(key0, 1, 2 * n + 1, true);
+        load_v(key0, 0, 2 * n, true);
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
       }
       const int n_last = n + n_blk - 1;
@@ -422,21 +431,30 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       auto top = [&](bool wait) {
         // everybody's loads have landed, everybody is past the block in front
         if (wait) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        load_v(cur.key0, 1, 2 * n + 1, true);
         more = n < n_last || next_blocks;
-        if (n < n_last)
-          nxt = block_at(pc.i1 - (n_last - n));
-        else if (next_blocks)
-          nxt = block(next_p, next_p.i0, ids_first);
+        if (n < n_last) {
+          const int key0 = key_of(pc, pc.i1 - (n_last - n)), group = group_of(key0);
+          if (group != win.group) {  // (uniform)
+            const bool following = group == win.group + 1;
+            turn_to(b, len, group, following ? ids_next : entries(b, group));
+            ids_next = entries(b, group + 1);
+          }
+          nxt = block(key0);
+        } else if (next_blocks) {
+          const int key0 = key_of(next_p, next_p.i0);
+          turn_to(next_p.b, next_p.len, group_of(key0), ids_first);
+          nxt = block(key0);
+        }
         const uint32_t k_at = lds_base + (uint32_t)(((2 * n) & 3) * SUB_BYTES), v_at = lds_base + CK_RING * SUB_BYTES;
         ad.ka = k_at + koff;
         ad.va[0] = v_at + (uint32_t)(((2 * n + 3) & 3) * SUB_BYTES) + voff;
         ad.va[1] = v_at + (uint32_t)(((2 * n) & 3) * SUB_BYTES) + voff;
       };
       auto feed = [&](int part) {
-        if (part == 0) load_k(nxt, 0, 2 * n + 2, more);
-        if (part == 1) load_k(nxt, 1, 2 * n + 3, more);
-        if (part == 2) load_v(cur, 1, 2 * n + 1, true);
-        if (part == 3) load_v(nxt, 0, 2 * n + 2, more);
+        if (part == 0) load_k(nxt.key0, 0, 2 * n + 2, more);
+        if (part == 1) load_k(nxt.key0, 1, 2 * n + 3, more);
+        if (part == 2) load_v(nxt.key0, 0, 2 * n + 2, more);
       };
       // what the wave's rows do not see of a block: nothing to take out in most of them
       auto partly = [&](const Block& c) {
@@ -482,11 +500,11 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       constexpr int MODE = HALF ? 2 : 0;
       if (!has_rows) {
         top(false);
-        feed(0), feed(1), feed(2), feed(3);
+        feed(0), feed(1), feed(2);
         for (++n; n <= n_last; ++n) {
           cur = nxt;
           top(true);
-          feed(0), feed(1), feed(2), feed(3);
+          feed(0), feed(1), feed(2);
         }
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         if (have_next) load_q(next_p);
@@ -501,11 +519,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         feed(0);
         ck_qk_only<0, HALF>(ad, qb, sa);
         feed(1);
-        at_step<true, false, 1, 0, 0, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+        at_step<true, false, 1, 0, 0, MODE, false, 2, true>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+        at_step<true, true, 2, 1, 0, MODE, true, 3, true>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
         feed(2);
-        at_step<true, true, 2, 1, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
-        feed(3);
-        at_step<true, true, 3, 1, 1, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
+        at_step<true, true, 3, 1, 1, MODE, true>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
         // ---- steady: four steps per block ----
         for (++n; n <= n_last; ++n) {
           old = cur, some_old = some;
@@ -513,15 +530,14 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           some = partly(cur);
           top(true);
           if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(1);
-          at_step<true, true, 0, 0, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(old, some_old, 3), l_mark, pre);
+          at_step<true, true, 0, 0, 0, MODE, false, 1, true>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(old, some_old, 3), l_mark, pre);
           feed(0);
-          at_step<true, true, 1, 0, 1, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
+          at_step<true, true, 1, 0, 1, MODE, true, 2, true>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 0), l_mark, pre);
           if (wave >= WAVES / 2) __builtin_amdgcn_s_setprio(0);
           feed(1);
+          at_step<true, true, 2, 1, 0, MODE, true, 3, true>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
           feed(2);
-          at_step<true, true, 2, 1, 0, MODE>(ad, qb, sa, sb, pa, pb, o, a.scale_log2, m, det, ones, masked(cur, some, 1), l_mark, pre);
-          feed(3);
-          at_step<true, true, 3, 1, 1, MODE>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
+          at_step<true, true, 3, 1, 1, MODE, true>(ad, qb, sb, sa, pb, pa, o, a.scale_log2, m, det, ones, masked(cur, some, 2), l_mark, pre);
         }
         // ---- drain: the last half-tile and its P . V (V of the last block's second sub-tile) ----
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
@@ -695,13 +711,16 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* wo
   if (!attr_set[dev]) {
     const void* kernels[4] = {(const void*)sp_chunk_kernel<64, false>, (const void*)sp_chunk_kernel<64, true>,
                               (const void*)sp_chunk_kernel<128, false>, (const void*)sp_chunk_kernel<128, true>};
-    for (const void* f : kernels) SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, CK_LDS_BYTES(128) + (2 * CK_MAX_SEQS + 1) * (int)sizeof(int)));
+    for (const void* f : kernels)
+      SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, CK_LDS_BYTES(128) + (2 * CK_MAX_SEQS + 1) * (int)sizeof(int)));
     attr_set[dev] = true;
   }
-  if (d == 64)
-    a.table != nullptr ? go(sp_chunk_kernel<64, true>, sp_chunk_merge_kernel<64, CK_ROWS>) : go(sp_chunk_kernel<64, false>, sp_chunk_merge_kernel<64, CK_ROWS>);
-  else
-    a.table != nullptr ? go(sp_chunk_kernel<128, true>, sp_chunk_merge_kernel<128, CK_ROWS>) : go(sp_chunk_kernel<128, false>, sp_chunk_merge_kernel<128, CK_ROWS>);
+  auto pick = [&](auto width) {
+    constexpr int D = decltype(width)::value;
+    auto merge = sp_chunk_merge_kernel<D, CK_ROWS>;
+    a.table != nullptr ? go(sp_chunk_kernel<D, true>, merge) : go(sp_chunk_kernel<D, false>, merge);
+  };
+  d == 64 ? pick(std::integral_constant<int, 64>{}) : pick(std::integral_constant<int, 128>{});
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
@@ -716,8 +735,8 @@ static int ck_check(const char* who, int64_t hq, int64_t hkv, int64_t d, int64_t
   return SP_OK;
 }
 static int ck_window(int64_t window) { return window == 0 || window > PG_NO_WINDOW ? PG_NO_WINDOW : (int)window; }
-// offsets inside the rows of a load have 32 bits
-static bool ck_rows_ok(int64_t stride_n) { return stride_n >= 0 && stride_n < (1ll << 24) && stride_n % 8 == 0; }
+// offsets inside a page (`rows` of them) have 32 bits
+static bool ck_rows_ok(int64_t stride_n, int64_t rows) { return stride_n >= 0 && stride_n * rows < (1ll << 30) && stride_n % 8 == 0; }
 
 extern "C" size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens) {
   if (single_tokens && tokens > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128))
@@ -747,7 +766,7 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k_pages | (uintptr_t)x->v_pages | (uintptr_t)x->out) % 16 == 0 &&
                  (x->q_stride_n | x->q_stride_h | x->k_stride_page | x->k_stride_h | x->v_stride_page | x->v_stride_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
-  SP_REQUIRE(ck_rows_ok(x->k_stride_slot) && ck_rows_ok(x->v_stride_slot), SP_ERR_UNSUPPORTED, "%s: slot strides %lld / %lld unsupported", who,
+  SP_REQUIRE(ck_rows_ok(x->k_stride_slot, x->page_size) && ck_rows_ok(x->v_stride_slot, x->page_size), SP_ERR_UNSUPPORTED, "%s: slot strides %lld / %lld unsupported", who,
              (long long)x->k_stride_slot, (long long)x->v_stride_slot);
   CkArgs a = {};
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k_pages, a.v = (const sp_bf16*)x->v_pages;
@@ -784,7 +803,7 @@ extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
   SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k | (uintptr_t)x->v | (uintptr_t)x->out) % 16 == 0 &&
                  (x->q_stride_b | x->q_stride_n | x->q_stride_h | x->k_stride_b | x->k_stride_h | x->v_stride_b | x->v_stride_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
-  SP_REQUIRE(ck_rows_ok(x->k_stride_n) && ck_rows_ok(x->v_stride_n), SP_ERR_UNSUPPORTED, "%s: token strides %lld / %lld unsupported", who,
+  SP_REQUIRE(ck_rows_ok(x->k_stride_n, CK_SUB) && ck_rows_ok(x->v_stride_n, CK_SUB), SP_ERR_UNSUPPORTED, "%s: token strides %lld / %lld unsupported", who,
              (long long)x->k_stride_n, (long long)x->v_stride_n);
   CkArgs a = {};
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k, a.v = (const sp_bf16*)x->v, a.out = (sp_bf16*)x->out;

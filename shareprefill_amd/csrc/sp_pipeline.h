@@ -132,7 +132,8 @@ __device__ __forceinline__ void at_prefetch_qk(const Addr& ad, bf16x8 (&pre)[2])
 // (a run's first stage, whose S the next stage's softmax reads at once; a pivot head's stage in front of the block sums).
 // Addr: where the operands of a block lie in LDS.  k<KQ, KS, T>() fetches channel step KS of key tile T of quarter KQ, v<VB, KT, I>() channel
 // tile I of half KT of buffer VB, both unseen by the compiler; V_READS: LDS reads of the latter.
-template <bool DO_QK, bool DO_PV, int KQ, int VB, int KT, bool PRE, int NEXT, bool HALF, bool SETTLE, class Addr>
+// EARLY: they are asked for two slots in front of the stage's end, and have landed there: no branch finds them on their way.
+template <bool DO_QK, bool DO_PV, int KQ, int VB, int KT, bool PRE, int NEXT, bool HALF, bool SETTLE, bool EARLY, class Addr>
 __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4], floatx4 (&s_out)[2][2],
                                          const floatx4 (&s_in)[2][2], const bf16x8 (&p_prev)[2], bf16x8 (&p_out)[2],
                                          floatx4 (&o)[9][2], float sc, const float (&neg_m)[2], uint32_t (&det)[2],
@@ -168,7 +169,8 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
     constexpr int k = decltype(kc)::value;
     constexpr bool qk = k < QS;
     constexpr int i = qk ? k : k - QS;
-    constexpr int in_flight_after = k + 1 == NP ? 0 : k + 1 < QS ? 1 : Addr::V_READS;  // reads of operand k + 1
+    constexpr bool ahead = EARLY && NEXT >= 0;  // the next stage's operands go out in slot NP - 2
+    constexpr int in_flight_after = k + 1 == NP ? (ahead ? 2 : 0) : k + 1 < QS ? 1 : Addr::V_READS;  // reads of operand k + 1, those
     AT_WAIT_LGKM(in_flight_after);  // operand k has landed
     AT_PIN();
     auto mfma = [&](auto qc, auto lastc) {
@@ -189,6 +191,7 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
     // stays the same for two MFMAs in a row, as the A operand does inside a slot (+0.5 % under the power cap)
     mfma(std::integral_constant<int, (k & 1)>{}, std::false_type{});
     if constexpr (k + AHEAD < NP) fetch(std::integral_constant<int, k + AHEAD>{});
+    if constexpr (ahead && k + AHEAD == NP) at_prefetch_qk<NEXT>(ad, pre);
 #pragma unroll
     for (int u = 0; u < EPS; ++u) {
       const int idx = k * EPS + u;
@@ -230,7 +233,10 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
     }
     AT_PIN();
   });
-  if constexpr (NEXT >= 0) {
+  if constexpr (NEXT >= 0 && EARLY) {
+    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(pre[0]), "+v"(pre[1]));
+    AT_PIN();
+  } else if constexpr (NEXT >= 0) {
     at_prefetch_qk<NEXT>(ad, pre);
     AT_PIN();
   }
@@ -335,7 +341,7 @@ __device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 
 // packed words; s_out still holds S(j-1) on entry and S(j+1) on return, p_out = P(j) with its OR in det.
 // The fused stage exists once per step: O never lives in two register sets that would have to be merged.
 // mask(s): takes out what the half-tile's queries do not see of its keys.
-template <bool DO_QK, bool HAVE_PREV, int KQ, int VB, int KT, int MODE, bool PRE = false, int NEXT = -1, class Addr, class Mask>
+template <bool DO_QK, bool HAVE_PREV, int KQ, int VB, int KT, int MODE, bool PRE = false, int NEXT = -1, bool EARLY = false, class Addr, class Mask>
 __device__ __forceinline__ void at_step(const Addr& ad, const bf16x8 (&qb)[2][4], floatx4 (&s_out)[2][2],
                                         floatx4 (&s_in)[2][2], bf16x8 (&p_prev)[2], bf16x8 (&p_out)[2],
                                         floatx4 (&o)[9][2], float scale_log2, float (&m_run)[2], uint32_t (&det)[2],
@@ -346,6 +352,6 @@ __device__ __forceinline__ void at_step(const Addr& ad, const bf16x8 (&qb)[2][4]
   // wait states inside the stage's last MFMA: a run's first stage (S read at once), and for pivot heads the stage
   // behind which the block sums are taken (emit in the kernel: the second stage of a block in the steady state)
   constexpr bool SETTLE = (DO_QK && !HAVE_PREV) || ((MODE & 1) != 0 && DO_QK && HAVE_PREV && KQ == 1);
-  at_fused<DO_QK, HAVE_PREV, KQ, VB, KT, PRE, NEXT, (MODE & 2) != 0, SETTLE>(ad, qb, s_out, s_in, p_prev, p_out, o,
+  at_fused<DO_QK, HAVE_PREV, KQ, VB, KT, PRE, NEXT, (MODE & 2) != 0, SETTLE, EARLY>(ad, qb, s_out, s_in, p_prev, p_out, o,
                                                                               scale_log2, neg_m, det, ones, pre);
 }
