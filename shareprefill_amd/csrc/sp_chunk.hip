@@ -160,7 +160,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     __syncthreads();
     // every thread some row tiles in a row: their units, then the line's prefix sums
     const int per = (a.slots + THREADS - 1) / THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
-    auto walk = [&](auto&& visit) {  // visit(x, units in the line, blocks)
+    auto walk = [&](auto&& visit) {  // visit(x, units in the line, 0: no row tile has the number, blocks)
       if (x0 >= x1) return;
       int b = 0, hi = a.batch;
       while (hi - b > 1) {
@@ -173,7 +173,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       for (int i = x0; i < x1; ++i) {
         while (b + 1 < a.batch && pg_first_slot(cu_s[b + 1], a.group, b + 1, TILE_ROWS) <= i) ++b;
         const int q_len = pg_max(0, cu_s[b + 1] - cu_s[b]), rt = (int)(i - pg_first_slot(cu_s[b], a.group, b, TILE_ROWS));
-        if (rt < 0 || rt >= pg_row_tiles(q_len, a.group, TILE_ROWS)) continue;
+        if (rt < 0 || (a.split && q_len == 1) || rt >= pg_row_tiles(q_len, a.group, TILE_ROWS)) {
+          visit(i, 0, 0);
+          continue;
+        }
         int p0, p1;
         pg_tile_positions(rt, q_len, len_s[b], a.group, TILE_ROWS, &p0, &p1);
         const int blocks = pg_span_units(ck_span(a, p0, p1, CK_BLOCK));
@@ -181,7 +184,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       }
     };
     int64_t mine = 0;
-    walk([&](int, int units, int) { mine += units; });
+    walk([&](int i, int units, int) {
+      mine += units;
+      if (units == 0 && part == 0 && a.by_slot != nullptr) a.by_slot[(int64_t)i * a.hkv + kvh].y = 0;  // (no row tile: nothing to merge)
+    });
     int64_t at = mine;
 #pragma unroll
     for (int o = 1; o < SP_WAVE; o <<= 1) {
@@ -204,7 +210,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (cut[e] >= at && cut[e] < at + units) {
-          const int tile = pg_snap(cut[e] - at, blocks, PG_OVERHEAD);
+          const int tile = pg_snap(cut[e] - at, blocks, PG_OVERHEAD, pg_near(total, parts));
           found[e][0] = tile < blocks || tile == 0 ? i : i + 1;
           found[e][1] = tile < blocks ? tile : 0;
         }
@@ -216,11 +222,11 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     x_end = __builtin_amdgcn_readfirstlane(found[1][0]);
     tile_end = __builtin_amdgcn_readfirstlane(found[1][1]);
   }
-  int4 note = make_int4(CK_NONE, -1, 0, 0);
+  int4 note = make_int4(CK_NONE, 0, 0, 0);
 
   // A row tile, or what of it falls to this workgroup: blocks i0 .. i1 - 1 of its walk.
   struct Piece {
-    int b, rt, start, q_len, len, i0, i1, blocks;
+    int slot, b, rt, start, q_len, len, i0, i1, blocks;
     PgSpan span;
   };
   // (LDS reads of its own: the compiler would wait for all that is in flight in front of them)
@@ -250,12 +256,13 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         ++x;
       }
       while (seq + 1 < a.batch && pg_first_slot(start_of(seq + 1), a.group, seq + 1, TILE_ROWS) <= here) ++seq;
+      p.slot = here;
       p.b = seq;
       p.start = start_of(seq);
       p.q_len = pg_max(0, start_of(seq + 1) - p.start);
       p.len = a.lens != nullptr ? from_lds(lds_len + 4u * seq) : a.n_keys;
       p.rt = (int)(here - pg_first_slot(p.start, a.group, seq, TILE_ROWS));
-      if (p.rt < 0 || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
+      if (p.rt < 0 || (a.split && p.q_len == 1) || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
       int p0, p1;
       pg_tile_positions(p.rt, p.q_len, p.len, a.group, TILE_ROWS, &p0, &p1);
       p.span = ck_span(a, p0, p1, CK_BLOCK);
@@ -559,9 +566,11 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     const int64_t slab = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
     float* const o_to = a.o_part + slab * (TILE_ROWS * D);
     float2* const ml_to = a.ml_part + slab * TILE_ROWS;
+    if (from_start && a.by_slot != nullptr && t == 0)
+      a.by_slot[(int64_t)pc.slot * a.hkv + kvh] = make_int4(blockIdx.x, whole ? 0 : pg_min(rows, TILE_ROWS), 0, 0);
     if (!whole) {
       if (from_start)
-        note.y = b, note.z = rt;
+        note.y = pg_min(rows, TILE_ROWS), note.z = rt * TILE_ROWS, note.w = start;
       else
         note.x = to_end ? CK_LAST : CK_MIDDLE;
     }
@@ -665,7 +674,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
 
 // ---- host -------------------------------------------------------------------------------------------------
 struct CkPlan {
-  int64_t slots, grid;
+  int64_t slots, grid, merges;  // merges: workgroups of the merging launch, a band of rows
   int parts;
 };
 // Workgroups that are resident at once: two a CU with 128 channels.
@@ -677,32 +686,43 @@ static CkPlan ck_plan(int64_t tokens, int32_t batch, int32_t hkv, int32_t group,
   const int64_t wgs = room < 1 ? 1 : room;  // of a kv head
   p.parts = uniform && p.slots >= 4 * wgs ? 0 : (int)wgs;
   p.grid = wgs * hkv;
+  p.merges = p.slots * hkv < p.grid ? p.slots * hkv : p.grid;
   return p;
 }
 static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, bool uniform) {
   if (tokens <= 0 || batch <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || (d != 64 && d != 128)) return 0;
   const CkPlan p = ck_plan(tokens, batch, hkv, hq / hkv, uniform);
-  return p.parts == 0 ? 0 : (size_t)p.grid * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + sizeof(int4));
+  return p.parts == 0 ? 0 : (size_t)p.grid * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + 2 * sizeof(int4));
 }
 
-static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* workspace, size_t workspace_bytes, hipStream_t s) {
+// what a launch needs, checked before anything is launched
+static int ck_check_launch(const char* who, const CkArgs& a, size_t need, const void* workspace, size_t workspace_bytes) {
+  const int hq = a.hkv * a.group;
+  SP_REQUIRE(pg_slots(a.tokens, a.group, a.batch, CK_ROWS) <= 0x7fffffffll && (int64_t)a.tokens * a.group < (1ll << 31) &&
+                 (int64_t)a.batch * a.hkv <= 0x7fffffffll,
+             SP_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are too many", who, a.tokens, hq);
+  SP_REQUIRE(pd_takes(a) || a.batch <= CK_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %d (at most %d, single tokens %d)", who, a.batch, CK_MAX_SEQS,
+             PG_MAX_SEQS);
+  SP_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), SP_ERR_WORKSPACE,
+             "%s: workspace missing, too small or misaligned", who);
+  return SP_OK;
+}
+
+static int ck_launch(const char* who, CkArgs& a, int32_t d, void* workspace, hipStream_t s) {
   const bool uniform = a.cu == nullptr && a.lens == nullptr;  // as many queries and keys in every sequence
   const CkPlan plan = ck_plan(a.tokens, a.batch, a.hkv, a.group, uniform);
-  SP_REQUIRE(plan.grid <= 0x7fffffffll && (int64_t)a.tokens * a.group < (1ll << 31), SP_ERR_UNSUPPORTED, "%s: %d tokens of %d heads are too many",
-             who, a.tokens, hq);
-  const size_t need = ck_workspace_bytes(a.tokens, a.batch, hq, a.hkv, d, uniform);
-  SP_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), SP_ERR_WORKSPACE,
-             "%s: workspace too small or misaligned", who);
   a.slots = (int)plan.slots;
   a.parts = plan.parts;
   a.o_part = (float*)workspace;
   a.ml_part = (float2*)(a.o_part + (size_t)plan.grid * 2 * (size_t)CK_ROWS * d);
   a.notes = (int4*)(a.ml_part + (size_t)plan.grid * 2 * CK_ROWS);
-  SP_REQUIRE(a.batch <= CK_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %d (at most %d, single tokens %d)", who, a.batch, CK_MAX_SEQS, PG_MAX_SEQS);
   const size_t lds = CK_LDS_BYTES(d) + (plan.parts != 0 ? (size_t)(2 * a.batch + 1) * sizeof(int) : 0);
-  auto go = [&](auto kernel, auto merge) {
+  a.by_slot = plan.parts != 0 && plan.merges < plan.grid ? a.notes + plan.grid : nullptr;
+  const int band = plan.merges <= 128 ? 16 : 64;
+  auto go = [&](auto kernel, auto few, auto many) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(CK_THREADS), lds, s, a);
-    if (plan.parts != 0) hipLaunchKernelGGL(merge, dim3((unsigned)plan.grid, CK_ROWS / CM_ROWS), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
+    if (plan.parts != 0)
+      hipLaunchKernelGGL(band == 16 ? few : many, dim3((unsigned)plan.merges, CK_ROWS / band), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
   };
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -717,8 +737,8 @@ static int ck_launch(const char* who, CkArgs& a, int32_t hq, int32_t d, void* wo
   }
   auto pick = [&](auto width) {
     constexpr int D = decltype(width)::value;
-    auto merge = sp_chunk_merge_kernel<D, CK_ROWS>;
-    a.table != nullptr ? go(sp_chunk_kernel<D, true>, merge) : go(sp_chunk_kernel<D, false>, merge);
+    auto few = sp_chunk_merge_kernel<D, CK_ROWS, 16>, many = sp_chunk_merge_kernel<D, CK_ROWS, 64>;
+    a.table != nullptr ? go(sp_chunk_kernel<D, true>, few, many) : go(sp_chunk_kernel<D, false>, few, many);
   };
   d == 64 ? pick(std::integral_constant<int, 64>{}) : pick(std::integral_constant<int, 128>{});
   SP_LAUNCH_CHECK();
@@ -736,12 +756,17 @@ static int ck_check(const char* who, int64_t hq, int64_t hkv, int64_t d, int64_t
 }
 static int ck_window(int64_t window) { return window == 0 || window > PG_NO_WINDOW ? PG_NO_WINDOW : (int)window; }
 // offsets inside a page (`rows` of them) have 32 bits
-static bool ck_rows_ok(int64_t stride_n, int64_t rows) { return stride_n >= 0 && stride_n * rows < (1ll << 30) && stride_n % 8 == 0; }
+static bool ck_rows_ok(int64_t stride_n, int64_t rows) { return stride_n >= 0 && stride_n < (1ll << 24) && stride_n * rows < (1ll << 30) && stride_n % 8 == 0; }
+
+// Sequences of one row among others go to the single-token kernel, in launches of their own, where there can be many: a row tile of the
+// chunk kernel that holds one token is nearly empty.  The lengths are the device's; what the host knows is the average.
+static bool ck_splits(int64_t tokens, int32_t batch) { return batch >= 4 && tokens < 256ll * batch; }
 
 extern "C" size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens) {
-  if (single_tokens && tokens > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128))
-    return pd_workspace_bytes(hkv, d);
-  return ck_workspace_bytes(tokens, batch, hq, hkv, d, false);
+  const size_t chunks = ck_workspace_bytes(tokens, batch, hq, hkv, d, false);
+  if (tokens > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128))
+    return single_tokens ? pd_workspace_bytes(hkv, d) : ck_splits(tokens, batch) ? chunks + pd_workspace_bytes(hkv, d) : chunks;
+  return chunks;
 }
 
 extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
@@ -779,8 +804,20 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   a.n_queries = 1;
   a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.window = ck_window(x->window), a.sinks = (int)(x->sinks < PG_MAX_KEYS ? x->sinks : PG_MAX_KEYS);
   a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
-  if (pd_takes(a)) return pd_launch(who, a, x->table_width << shift, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
-  return ck_launch(who, a, (int)x->hq, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
+  rc = ck_check_launch(who, a, sp_paged_attn_workspace_bytes(x->tokens, (int)x->batch, (int)x->hq, (int)x->hkv, (int)x->d, a.cu == nullptr),
+                       x->workspace, (size_t)x->workspace_bytes);
+  if (rc) return rc;
+  const int64_t room = x->table_width << shift;
+  if (pd_takes(a)) return pd_launch(a, room, (int)x->d, x->workspace, (hipStream_t)x->stream);
+  char* workspace = (char*)x->workspace;
+  if (a.cu != nullptr && a.group <= PD_MAX_GROUP && ck_splits(a.tokens, a.batch)) {
+    a.split = 1;
+    CkArgs singles = a;
+    rc = pd_launch(singles, room, (int)x->d, workspace, (hipStream_t)x->stream);
+    if (rc) return rc;
+    workspace += pd_workspace_bytes(a.hkv, (int)x->d);
+  }
+  return ck_launch(who, a, (int)x->d, workspace, (hipStream_t)x->stream);
 }
 
 extern "C" size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d) {
@@ -814,6 +851,9 @@ extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
   a.batch = (int)x->batch, a.tokens = (int)(x->batch * x->n), a.n_keys = (int)x->n_keys, a.n_queries = (int)x->n;
   a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.window = ck_window(x->window), a.sinks = (int)(x->sinks < PG_MAX_KEYS ? x->sinks : PG_MAX_KEYS);
   a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
-  if (pd_takes(a)) return pd_launch(who, a, x->n_keys, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
-  return ck_launch(who, a, (int)x->hq, (int)x->d, x->workspace, (size_t)x->workspace_bytes, (hipStream_t)x->stream);
+  rc = ck_check_launch(who, a, sp_window_attn_workspace_bytes((int)x->batch, x->n, x->n_keys, (int)x->hq, (int)x->hkv, (int)x->d),
+                       x->workspace, (size_t)x->workspace_bytes);
+  if (rc) return rc;
+  if (pd_takes(a)) return pd_launch(a, x->n_keys, (int)x->d, x->workspace, (hipStream_t)x->stream);
+  return ck_launch(who, a, (int)x->d, x->workspace, (hipStream_t)x->stream);
 }

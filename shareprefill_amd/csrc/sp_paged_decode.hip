@@ -36,6 +36,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
 
   // ---- which sequences, and which steps of the first and the last ----
   auto span_of = [&](int len) { return ck_span(a, len - 1, len - 1, DS_KEYS); };
+  auto single = [&](int i) { return !a.split || ck_start(a, i + 1) - ck_start(a, i) == 1; };
   int b, b_end, begin = 0, end = 0;
   if (a.parts == 0) {
     b = part;
@@ -44,7 +45,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     // every wave for itself, 64 sequences at a time
     auto sums = [&](int b0, int* steps, int64_t* upto) {  // of the lane's sequence; units up to it, it included
       const int i = b0 + lane;
-      *steps = i < a.batch ? pg_span_units(span_of(ck_len(a, i))) : -PD_OVERHEAD;
+      *steps = i < a.batch && single(i) ? pg_span_units(span_of(ck_len(a, i))) : -PD_OVERHEAD;  // (others take no room in the line)
       int64_t at = *steps + PD_OVERHEAD;
 #pragma unroll
       for (int o = 1; o < SP_WAVE; o <<= 1) {
@@ -72,7 +73,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
           const uint64_t here = __ballot(cut < before + upto);
           if (here != 0ull) {
             const int i = __builtin_ctzll(here), n = __shfl(steps, i, SP_WAVE);
-            const int at = pg_snap(cut - (before + __shfl(upto, i, SP_WAVE) - n - PD_OVERHEAD), n, PD_OVERHEAD);
+            const int at = pg_snap(cut - (before + __shfl(upto, i, SP_WAVE) - n - PD_OVERHEAD), n, PD_OVERHEAD, pg_near(total, parts));
             seq[e] = b0 + i + (at < n || at == 0 ? 0 : 1);
             step[e] = at < n ? at : 0;
             break;
@@ -83,7 +84,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     b = __builtin_amdgcn_readfirstlane(seq[0]), begin = __builtin_amdgcn_readfirstlane(step[0]);
     b_end = __builtin_amdgcn_readfirstlane(seq[1]), end = __builtin_amdgcn_readfirstlane(step[1]);
   }
-  int4 note = make_int4(CK_NONE, -1, 0, 0);
+  int4 note = make_int4(CK_NONE, 0, 0, 0);
 
   const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
   const uint32_t ring = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)ring_lds + wave * NB * Shape::STEP_BYTES;
@@ -91,7 +92,8 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
   const int v_key = 4 * gr + (lq >> 2);  // row of the transposing read; 16 rows further the swizzle is the same
   const uint32_t v_at = ring + Shape::K_BYTES + v_key * (CT * 32) + 8 * (lq & 3);
 
-  for (bool first = true; b < a.batch && (b < b_end || (b == b_end && end > 0)); ++b, begin = 0, first = false) {
+  for (bool first = true; b < a.batch && (b < b_end || (b == b_end && end > 0)); ++b, begin = 0) {
+    if (!single(b)) continue;
     const int len = ck_len(a, b), pos = len - 1;
     const PgSpan span = span_of(len);
     const int steps = pg_span_units(span), s_end = b == b_end ? pg_min(end, steps) : steps;
@@ -100,7 +102,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
 
     dc_bf16x8 qb[KS];
     {
-      const sp_bf16* src = a.q + (int64_t)b * (PAGED ? a.sq_n : a.sq_b) + (int64_t)(kvh * g + (lq < g ? lq : 0)) * a.sq_h + 8 * gr;
+      const sp_bf16* src = a.q + (int64_t)(PAGED ? ck_start(a, b) : b) * (PAGED ? a.sq_n : a.sq_b) + (int64_t)(kvh * g + (lq < g ? lq : 0)) * a.sq_h + 8 * gr;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const dc_u32x4 raw = *reinterpret_cast<const dc_u32x4*>(src + 32 * ks);
@@ -167,6 +169,8 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     };
 
     if (!first) __syncthreads();  // the rings are free
+    first = false;
+    const int64_t row = ck_start(a, b);  // of q and out
     const int s0 = begin + wave;
     uint32_t seen[NB - 1];
 #pragma unroll
@@ -278,7 +282,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     const int64_t slab = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
     if (!whole) {
       if (from_start)
-        note.y = b;
+        note.y = g, note.w = (int)row;
       else
         note.x = to_end ? CK_LAST : CK_MIDDLE;
     }
@@ -297,7 +301,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // (a sequence without keys: zeros)
-        *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hkv * g + kvh * g + h) * D + c) =
+        *reinterpret_cast<uint2*>(a.out + (row * a.hkv * g + kvh * g + h) * D + c) =
             make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
       } else {
         *reinterpret_cast<ds_floatx4*>(a.o_part + (slab * PD_ROWS + h) * D + c) = acc;
@@ -314,35 +318,26 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
 template <int D>
 __global__ __launch_bounds__(PD_MERGE_THREADS) void sp_paged_decode_merge_kernel(const CkArgs a, int workgroups) {
   constexpr int WIDTH = D / 4, GROUPS = PD_MERGE_THREADS / WIDTH;
-  const int b = a.notes[blockIdx.x].y;
-  if (b < 0) return;
   __shared__ float2 ml_s[PD_MAX_PARTS];
   __shared__ __attribute__((aligned(16))) float o_s[GROUPS][D];
-  const int t = threadIdx.x, lane = t & 63, h = blockIdx.y;
-  int more = 0;  // parts behind the first
-  for (;;) {
-    const int64_t w = blockIdx.x + (int64_t)(more + 1 + lane) * a.hkv;
-    const uint64_t ends = __ballot(w >= workgroups || a.notes[w < workgroups ? w : 0].x != CK_MIDDLE);
-    if (ends != 0ull) {
-      more += __builtin_ctzll(ends) + 1;
-      break;
-    }
-    more += SP_WAVE;
-  }
+  const int t = threadIdx.x, h = blockIdx.y;
+  int4 note;
+  const int parts = cm_parts(a, workgroups, t & 63, blockIdx.x, &note);
+  if (parts == 0) return;
   auto row = [&](int i) {
     return (i == 0 ? (int64_t)blockIdx.x * 2 + 1 : ((int64_t)blockIdx.x + (int64_t)i * a.hkv) * 2) * PD_ROWS + h;
   };
-  if (t <= more) ml_s[t] = a.ml_part[row(t)];
+  if (t < parts) ml_s[t] = a.ml_part[row(t)];
   __syncthreads();
   float top = CK_NO_MAX;
-  for (int i = 0; i <= more; ++i) top = fmaxf(top, ml_s[i].x);
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, ml_s[i].x);
   const int grp = t / WIDTH, c = t % WIDTH * 4;
   ds_floatx4 acc = {0, 0, 0, 0};
   float sum = 0.f;
 #pragma unroll 4
-  for (int i = grp; i <= more; i += GROUPS)
+  for (int i = grp; i < parts; i += GROUPS)
     acc += *reinterpret_cast<const ds_floatx4*>(a.o_part + row(i) * D + c) * __builtin_amdgcn_exp2f(ml_s[i].x - top);
-  for (int i = 0; i <= more; ++i) sum += ml_s[i].y * __builtin_amdgcn_exp2f(ml_s[i].x - top);
+  for (int i = 0; i < parts; ++i) sum += ml_s[i].y * __builtin_amdgcn_exp2f(ml_s[i].x - top);
   *reinterpret_cast<ds_floatx4*>(&o_s[grp][c]) = acc;
   __syncthreads();
   if (t >= WIDTH) return;
@@ -350,7 +345,7 @@ __global__ __launch_bounds__(PD_MERGE_THREADS) void sp_paged_decode_merge_kernel
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i) acc += *reinterpret_cast<const ds_floatx4*>(&o_s[i][c]);
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hkv * a.group + (blockIdx.x % a.hkv) * a.group + h) * D + c) =
+  *reinterpret_cast<uint2*>(a.out + ((int64_t)note.w * a.hkv * a.group + (blockIdx.x % a.hkv) * a.group + h) * D + c) =
       make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
 }
 
@@ -363,7 +358,7 @@ size_t pd_workspace_bytes(int32_t hkv, int32_t d) {
   return (size_t)pd_parts(hkv) * hkv * (2 * PD_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + sizeof(int4));
 }
 
-int pd_launch(const char* who, CkArgs& a, int64_t max_keys, int32_t d, void* workspace, size_t workspace_bytes, hipStream_t s) {
+int pd_launch(CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream_t s) {
   if (a.window < PG_NO_WINDOW && (int64_t)a.window + a.sinks + 2 * DS_KEYS < max_keys) max_keys = (int64_t)a.window + a.sinks + 2 * DS_KEYS;
   const int64_t pairs = (int64_t)a.batch * a.hkv, units = sp_ceil_div(max_keys, DS_KEYS) + PD_OVERHEAD;
   const int64_t most = pg_parts(units * a.batch, pd_parts(a.hkv), PD_MIN_SHARE);
@@ -371,9 +366,6 @@ int pd_launch(const char* who, CkArgs& a, int64_t max_keys, int32_t d, void* wor
   const int64_t whole = sp_ceil_div(pairs, 256) * units, cut = sp_ceil_div(pairs * units, 256) + 16;
   a.parts = whole <= cut || most == 1 ? 0 : (int)most;
   const int64_t grid = a.parts == 0 ? pairs : (int64_t)a.parts * a.hkv;
-  SP_REQUIRE(grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %d sequences of %d kv heads are too many", who, a.batch, a.hkv);
-  SP_REQUIRE(a.parts == 0 || (workspace != nullptr && workspace_bytes >= pd_workspace_bytes(a.hkv, d) && (uintptr_t)workspace % 16 == 0),
-             SP_ERR_WORKSPACE, "%s: workspace too small or misaligned", who);
   a.o_part = (float*)workspace;
   a.ml_part = (float2*)(a.o_part + (size_t)grid * 2 * PD_ROWS * d);
   a.notes = (int4*)(a.ml_part + (size_t)grid * 2 * PD_ROWS);

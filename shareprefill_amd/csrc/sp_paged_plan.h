@@ -12,7 +12,6 @@
 #define PG_MAX_SEQS 4096           // sequences of a call
 #define PG_MAX_KEYS (1 << 30)      // keys of a sequence: positions and their differences have 31 bits
 #define PG_NO_WINDOW PG_MAX_KEYS   // every key in front of a query lies inside it
-#define PG_TILE 64                 // keys of a tile
                                    // a row tile has `tile` rows: (token, query head of the kv group) pairs, the heads of a token side by side
 
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
@@ -51,19 +50,23 @@ PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int tile, int* p
   *p1 = len - q_len + (int)((r1 - 1) / g);
 }
 
-// A launch of few row tiles cuts the line of all their tiles, one line per kv head, into equal parts: part p of `parts` starts at unit
-// total * p / parts.  A row tile counts its tiles and PG_OVERHEAD units for its queries, its first loads and its output; a cut within
-// PG_MIN_PART tiles of a row tile's start or end goes there.
+// A launch cuts the line of all its row tiles' blocks, one line per kv head, into equal parts: part p of `parts` starts at unit
+// total * p / parts.  A row tile counts its blocks and PG_OVERHEAD units for its queries, its first loads and its output; a cut near a row
+// tile's start or end goes there (pg_near).
 #define PG_OVERHEAD 2
-#define PG_MIN_PART 4
-#define PG_MIN_SHARE 8  // units of a part at least
+#define PG_MIN_SHARE 3  // units of a part at least
 PG_FN int64_t pg_parts(int64_t total, int64_t room, int share) {
   const int64_t parts = (total + share - 1) / share;
   return parts < room ? (parts < 1 ? 1 : parts) : room;
 }
 PG_FN int64_t pg_cut(int64_t total, int64_t parts, int64_t p) { return total / parts * p + total % parts * p / parts; }
-// Where a cut `off` units into a row tile of n tiles stands: tile 0 .. n - 1 of it, or n: the start of what follows.
-PG_FN int pg_snap(int64_t off, int n, int overhead) {
+// How near: a cut leaves partials behind that are written, read and merged, some four units' worth, and is not worth a quarter of a part.
+PG_FN int pg_near(int64_t total, int64_t parts) {
+  const int64_t quarter = total / parts / 4;
+  return quarter < 1 ? 1 : quarter > 4 ? 4 : (int)quarter;
+}
+// Where a cut `off` units into a row tile of n blocks stands: block 0 .. n - 1 of it, or n: the start of what follows.
+PG_FN int pg_snap(int64_t off, int n, int overhead, int near) {
   const int64_t t = off - overhead;
-  return t < PG_MIN_PART ? 0 : t > n - PG_MIN_PART ? n : (int)t;
+  return t < near ? 0 : t > n - near ? n : (int)t;
 }

@@ -22,9 +22,9 @@ int main() {
     } else if (what == 'f') {
       printf("%ld %ld %ld\\n", (long)pg_first_slot(a, (int)b, (int)c, (int)d), (long)pg_slots(a, (int)b, (int)c, (int)d), (long)pg_row_tiles(a, (int)b, (int)d));
     } else if (what == 'c') {
-      printf("%ld %ld\\n", (long)pg_parts(a, b, 8), (long)pg_cut(a, pg_parts(a, b, 8), c));
+      printf("%ld %ld\\n", (long)pg_parts(a, b, 3), (long)pg_cut(a, pg_parts(a, b, 3), c));
     } else if (what == 'n') {
-      printf("%d\\n", pg_snap(a, (int)b, 2));
+      printf("%d %d\\n", pg_snap(a, (int)b, 2, pg_near(c, d)), pg_near(c, d));
     } else {
       int p0, p1;
       pg_tile_positions((int)a, (int)b, (int)c, (int)d, (int)e, &p0, &p1);
@@ -114,14 +114,14 @@ def test_cuts_cover_the_line_once(ask):
                 places.append((len(tiles), 0))
                 continue
             x = max(i for i, s in enumerate(starts[:-1]) if s <= cut)
-            tile = ask([("n", cut - starts[x], tiles[x])])[0][0]
+            tile, near = ask([("n", cut - starts[x], tiles[x], total, parts)])[0]
             assert 0 <= tile <= tiles[x]
             places.append((x, tile) if tile < tiles[x] or tile == 0 else (x + 1, 0))
         assert places[0] == (0, 0) and places == sorted(places)
-        # no piece of a row tile is shorter than four tiles, unless two cuts meet
-        for (x0, t0), (x1, t1) in zip(places, places[1:]):
-            if t0:
-                assert 4 <= t0 <= tiles[x0] - 4
+        # no cut lies within a quarter of a part of a row tile's start or end, four blocks at most
+        near = max(1, min(4, total // parts // 4))
+        for x, t in places:
+            assert t == 0 or near <= t <= tiles[x] - near
 
 
 def test_a_line_past_32_bits_is_cut_evenly(ask):
