@@ -54,8 +54,12 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
       }
       *upto = at;
     };
-    int steps;
-    int64_t upto, total = 0;
+    int steps = 0;
+    int64_t upto = 0, total = 0;
+    if (a.batch == 1) {  // (no sums to form: half a microsecond of a chat's step)
+      steps = single(0) ? pg_span_units(span_of(ck_len(a, 0))) : -PD_OVERHEAD;
+      upto = total = steps + PD_OVERHEAD;
+    } else
     for (int b0 = 0; b0 < a.batch; b0 += SP_WAVE) {
       sums(b0, &steps, &upto);
       total += __shfl(upto, SP_WAVE - 1, SP_WAVE);
@@ -363,7 +367,8 @@ int pd_launch(CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream
   const int64_t pairs = (int64_t)a.batch * a.hkv, units = sp_ceil_div(max_keys, DS_KEYS) + PD_OVERHEAD;
   const int64_t most = pg_parts(units * a.batch, pd_parts(a.hkv), PD_MIN_SHARE);
   // A workgroup a sequence where that takes the longest of them no longer than even parts and their merging launch (units).
-  const int64_t whole = sp_ceil_div(pairs, 256) * units, cut = sp_ceil_div(pairs * units, 256) + 16;
+  // A table's width only bounds the lengths: sequences are taken for five eighths of it on average.
+  const int64_t whole = sp_ceil_div(pairs, 256) * units, cut = sp_ceil_div(pairs * units, 256) * (a.lens != nullptr ? 5 : 8) / 8 + 16;
   a.parts = whole <= cut || most == 1 ? 0 : (int)most;
   const int64_t grid = a.parts == 0 ? pairs : (int64_t)a.parts * a.hkv;
   a.o_part = (float*)workspace;

@@ -55,15 +55,24 @@ PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int tile, int* p
 // tile's start or end goes there (pg_near).
 #define PG_OVERHEAD 2
 #define PG_MIN_SHARE 3  // units of a part at least
+// (Quotients of 64 bits take the device a hundred instructions each, and every workgroup forms them: lines that fit 31 bits do without.)
+#define PG_SHORT_LINE (1ll << 31)
 PG_FN int64_t pg_parts(int64_t total, int64_t room, int share) {
-  const int64_t parts = (total + share - 1) / share;
+  const int64_t parts = total < PG_SHORT_LINE ? (int64_t)(((unsigned)total + (unsigned)share - 1u) / (unsigned)share) : room;
   return parts < room ? (parts < 1 ? 1 : parts) : room;
 }
-PG_FN int64_t pg_cut(int64_t total, int64_t parts, int64_t p) { return total / parts * p + total % parts * p / parts; }
+// (at most 2^15 parts)
+PG_FN int64_t pg_cut(int64_t total, int64_t parts, int64_t p) {
+  if (total < PG_SHORT_LINE) {
+    const unsigned t = (unsigned)total, n = (unsigned)parts, at = (unsigned)p, each = t / n;
+    return (int64_t)(each * at + (t - each * n) * at / n);
+  }
+  return total / parts * p + total % parts * p / parts;
+}
 // How near: a cut leaves partials behind that are written, read and merged, some four units' worth, and is not worth a quarter of a part.
 PG_FN int pg_near(int64_t total, int64_t parts) {
-  const int64_t quarter = total / parts / 4;
-  return quarter < 1 ? 1 : quarter > 4 ? 4 : (int)quarter;
+  const int64_t four = 16 * parts;
+  return total >= four ? 4 : total >= 12 * parts ? 3 : total >= 8 * parts ? 2 : 1;
 }
 // Where a cut `off` units into a row tile of n blocks stands: block 0 .. n - 1 of it, or n: the start of what follows.
 PG_FN int pg_snap(int64_t off, int n, int overhead, int near) {
