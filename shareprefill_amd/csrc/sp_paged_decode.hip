@@ -16,8 +16,8 @@
 #include "sp_ring.h"
 
 #define PD_ROWS PD_MAX_GROUP
-#define PD_OVERHEAD 8   // units of a line that a sequence counts beside its steps: queries, first loads, the waves' meeting
-#define PD_MIN_SHARE 8  // units of a part at least
+#define PD_OVERHEAD 4   // units of a line that a sequence counts beside its steps: queries, first loads, the waves' meeting
+#define PD_MIN_SHARE 4  // units of a part at least
 
 template <int D>
 using PdShape = DsShape<D, D / 16, D == 64 ? 8 : 4, 152>;
