@@ -355,18 +355,30 @@ int sp_decode_attn_static_bf16(const void* q, const void* k, const void* v, int6
  * of the sequences, slots[t] = page * page_size + position % page_size (-1: no page, or beyond the table's width) and positions[t] (its
  * place in its sequence); tokens behind the last one get -1 and 0.  *free_left = pages left on the stack (negative: so many were missing).
  * Negative lengths count as 0.  The outputs must not overlap the inputs. */
-int sp_paged_tables(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t page_size, int32_t num_pages,
-                    int32_t* block_table, int64_t table_stride, int32_t table_width, const int32_t* free_pages,
-                    int32_t free_room, const int32_t* free_count, int32_t max_tokens, int32_t* seq_lens, int32_t* cu_new,
-                    int64_t* slots, int32_t* positions, int32_t* free_left, sp_stream_t stream);
+typedef struct sp_paged_tables_args {
+  const int32_t *lens, *new_lens;
+  int32_t* block_table;
+  const int32_t *free_pages, *free_count;
+  int32_t *seq_lens, *cu_new;
+  int64_t* slots;
+  int32_t *positions, *free_left;
+  int64_t batch, page_size, num_pages, table_width, table_stride, free_room, max_tokens;
+  sp_stream_t stream;
+} sp_paged_tables_args;
+int sp_paged_tables(const sp_paged_tables_args* args /* host */);
 
 /* k, v: bf16 [tokens][hkv][d] (token and head strides) copied to slots[t] of the pools; a slot outside the pool is skipped.  Slots
  * must differ from each other: where two tokens name the same one, its contents are parts of either.  d a multiple of 8. */
-int sp_paged_cache_write_bf16(const void* k, const void* v, int64_t tokens, int32_t hkv, int32_t d, int64_t k_stride_n,
-                              int64_t k_stride_h, int64_t v_stride_n, int64_t v_stride_h, void* k_pages, void* v_pages,
-                              int32_t num_pages, int32_t page_size, int64_t k_stride_page, int64_t k_stride_slot,
-                              int64_t k_stride_page_h, int64_t v_stride_page, int64_t v_stride_slot,
-                              int64_t v_stride_page_h, const int64_t* slots, sp_stream_t stream);
+typedef struct sp_paged_write_args {
+  const void *k, *v;
+  void *k_pages, *v_pages;
+  const int64_t* slots;
+  int64_t tokens, hkv, d, num_pages, page_size;
+  int64_t k_stride_n, k_stride_h, v_stride_n, v_stride_h;
+  int64_t k_stride_page, k_stride_slot, k_stride_page_h, v_stride_page, v_stride_slot, v_stride_page_h;
+  sp_stream_t stream;
+} sp_paged_write_args;
+int sp_paged_cache_write_bf16(const sp_paged_write_args* args /* host */);
 
 /* Attention of the new tokens over everything cached, them included.  q: bf16 [tokens][hq][d], the sequences one behind the other:
  * sequence b has rows cu_q[b] .. cu_q[b + 1] (null: one row each, tokens == batch) and seq_lens[b] keys; its query i stands at position

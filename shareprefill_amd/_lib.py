@@ -98,13 +98,12 @@ SIGNATURES = {
                                          _I64, _I64, _F, _P, _P, _SZ, _P]),
     "sp_decode_attn_batch_args_bf16": (_I32, [C.c_char_p]),  # (DECODE_BATCH_ARGS.pack(...))
     "sp_decode_attn_static_bf16": (_I32, [_P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _F, _P, _P]),
-    "sp_paged_tables": (_I32, [_P, _P, _I32, _I32, _I32, _P, _I64, _I32, _P, _I32, _P, _I32, _P, _P, _P, _P, _P, _P]),
-    "sp_paged_cache_write_bf16": (_I32, [_P, _P, _I64, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _I32, _I64, _I64, _I64,
-                                         _I64, _I64, _I64, _P, _P]),
+    "sp_paged_tables": (_I32, [C.c_char_p]),  # (PAGED_TABLES_ARGS.pack(...), and so on)
+    "sp_paged_cache_write_bf16": (_I32, [C.c_char_p]),
     "sp_paged_attn_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32]),
-    "sp_paged_attn_bf16": (_I32, [C.c_char_p]),  # (PAGED_ATTN_ARGS.pack(...))
+    "sp_paged_attn_bf16": (_I32, [C.c_char_p]),
     "sp_window_attn_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I32, _I32, _I32]),
-    "sp_window_attn_bf16": (_I32, [C.c_char_p]),  # (WINDOW_ATTN_ARGS.pack(...))
+    "sp_window_attn_bf16": (_I32, [C.c_char_p]),
     "sp_rope_inplace_bf16": (_I32, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _P]),
     "sp_pivot_update": (_I32, [_ST, _P, _P, _P, _I32, _I32, _F, _P]),
     "sp_cover_select_rows": (_I32, [_P, _I32, _F, _P, _P]),
@@ -115,7 +114,9 @@ SIGNATURES = {
 
 # sp_decode_batch_args
 DECODE_BATCH_ARGS = struct.Struct("@5PQ13qdP")
-# sp_paged_attn_args, sp_window_attn_args
+# sp_paged_tables_args, sp_paged_write_args, sp_paged_attn_args, sp_window_attn_args
+PAGED_TABLES_ARGS = struct.Struct("@10P7qP")
+PAGED_WRITE_ARGS = struct.Struct("@5P15qP")
 PAGED_ATTN_ARGS = struct.Struct("@8PQ19qdP")
 WINDOW_ATTN_ARGS = struct.Struct("@5PQ17qdP")
 

@@ -97,35 +97,38 @@ __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs 
   a.positions[gid] = pos;
 }
 
-static int page_shift(int32_t page_size) {  // -1: not a page size
+static int page_shift(int64_t page_size) {  // -1: not a page size
   for (int s = 4; s <= 10; ++s)
-    if (page_size == 1 << s) return s;
+    if (page_size == 1ll << s) return s;
   return -1;
 }
 
-extern "C" int sp_paged_tables(const int32_t* lens, const int32_t* new_lens, int32_t batch, int32_t page_size, int32_t num_pages,
-                               int32_t* block_table, int64_t table_stride, int32_t table_width, const int32_t* free_pages,
-                               int32_t free_room, const int32_t* free_count, int32_t max_tokens, int32_t* seq_lens, int32_t* cu_new,
-                               int64_t* slots, int32_t* positions, int32_t* free_left, sp_stream_t stream) {
+extern "C" int sp_paged_tables(const sp_paged_tables_args* x) {
   const char* who = "sp_paged_tables";
-  SP_REQUIRE(batch > 0 && table_width > 0 && num_pages >= 0 && free_room >= 0 && max_tokens >= 0, SP_ERR_INVALID_ARGUMENT,
-             "%s: batch=%d table_width=%d num_pages=%d free_room=%d max_tokens=%d", who, batch, table_width, num_pages, free_room, max_tokens);
-  SP_REQUIRE(lens && new_lens && block_table && (free_pages || free_room == 0) && free_count && seq_lens && cu_new && free_left &&
-                 ((slots && positions) || max_tokens == 0),
+  SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(x->batch > 0 && x->table_width > 0 && x->num_pages >= 0 && x->free_room >= 0 && x->max_tokens >= 0, SP_ERR_INVALID_ARGUMENT,
+             "%s: batch=%lld table_width=%lld num_pages=%lld free_room=%lld max_tokens=%lld", who, (long long)x->batch, (long long)x->table_width,
+             (long long)x->num_pages, (long long)x->free_room, (long long)x->max_tokens);
+  SP_REQUIRE(x->lens && x->new_lens && x->block_table && (x->free_pages || x->free_room == 0) && x->free_count && x->seq_lens && x->cu_new &&
+                 x->free_left && ((x->slots && x->positions) || x->max_tokens == 0),
              SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  SP_REQUIRE((const void*)seq_lens != lens && (const void*)seq_lens != new_lens && (const void*)free_left != free_count && cu_new != new_lens && cu_new != lens,
-             SP_ERR_INVALID_ARGUMENT, "%s: an output is an input", who);
-  SP_REQUIRE(table_stride >= table_width || batch == 1, SP_ERR_INVALID_ARGUMENT, "%s: rows of %d entries overlap at a stride of %lld", who,
-             table_width, (long long)table_stride);
-  SP_REQUIRE(batch <= PG_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %d (at most %d)", who, batch, PG_MAX_SEQS);
-  const int shift = page_shift(page_size);
-  SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %d (a power of two from 16 to 1024)", who, page_size);
-  SP_REQUIRE(((int64_t)table_width << shift) <= PG_MAX_KEYS && max_tokens <= PG_MAX_KEYS, SP_ERR_UNSUPPORTED,
-             "%s: %d pages a request, %d tokens", who, table_width, max_tokens);
-  const TablesArgs a = {lens, new_lens, block_table, table_stride, free_pages, free_count, batch, shift, table_width, num_pages, free_room,
-                        max_tokens, seq_lens, cu_new, slots, positions, free_left};
-  const unsigned grid = max_tokens > 0 ? (unsigned)sp_ceil_div(max_tokens, PT_THREADS) : 1u;
-  hipLaunchKernelGGL(sp_paged_tables_kernel, dim3(grid), dim3(PT_THREADS), 2 * (batch + 1) * sizeof(int), (hipStream_t)stream, a);
+  const int32_t* const in[3] = {x->lens, x->new_lens, x->free_count};
+  for (const int32_t* p : in)
+    SP_REQUIRE(p != x->seq_lens && p != x->cu_new && p != x->free_left, SP_ERR_INVALID_ARGUMENT, "%s: an output is an input", who);
+  SP_REQUIRE(x->table_stride >= x->table_width || x->batch == 1, SP_ERR_INVALID_ARGUMENT, "%s: rows of %lld entries overlap at a stride of %lld", who,
+             (long long)x->table_width, (long long)x->table_stride);
+  SP_REQUIRE(x->batch <= PG_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %lld (at most %d)", who, (long long)x->batch, PG_MAX_SEQS);
+  const int shift = page_shift(x->page_size);
+  SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
+  SP_REQUIRE(x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS && x->max_tokens <= PG_MAX_KEYS && x->num_pages <= 0x7fffffffll &&
+                 x->free_room <= 0x7fffffffll,
+             SP_ERR_UNSUPPORTED, "%s: table_width=%lld max_tokens=%lld num_pages=%lld free_room=%lld too large", who, (long long)x->table_width,
+             (long long)x->max_tokens, (long long)x->num_pages, (long long)x->free_room);
+  const TablesArgs a = {x->lens, x->new_lens, x->block_table, x->table_stride, x->free_pages, x->free_count, (int)x->batch, shift,
+                        (int)x->table_width, (int)x->num_pages, (int)x->free_room, (int)x->max_tokens, x->seq_lens, x->cu_new, x->slots,
+                        x->positions, x->free_left};
+  const unsigned grid = x->max_tokens > 0 ? (unsigned)sp_ceil_div(x->max_tokens, PT_THREADS) : 1u;
+  hipLaunchKernelGGL(sp_paged_tables_kernel, dim3(grid), dim3(PT_THREADS), 2 * (x->batch + 1) * sizeof(int), (hipStream_t)x->stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
@@ -175,29 +178,28 @@ __global__ __launch_bounds__(PW_THREADS) void sp_paged_write_kernel(WriteArgs a)
     }
 }
 
-extern "C" int sp_paged_cache_write_bf16(const void* k, const void* v, int64_t tokens, int32_t hkv, int32_t d, int64_t k_stride_n,
-                                         int64_t k_stride_h, int64_t v_stride_n, int64_t v_stride_h, void* k_pages, void* v_pages,
-                                         int32_t num_pages, int32_t page_size, int64_t k_stride_page, int64_t k_stride_slot,
-                                         int64_t k_stride_page_h, int64_t v_stride_page, int64_t v_stride_slot, int64_t v_stride_page_h,
-                                         const int64_t* slots, sp_stream_t stream) {
+extern "C" int sp_paged_cache_write_bf16(const sp_paged_write_args* x) {
   const char* who = "sp_paged_cache_write_bf16";
-  SP_REQUIRE(tokens >= 0 && hkv > 0 && num_pages >= 0, SP_ERR_INVALID_ARGUMENT, "%s: tokens=%lld hkv=%d num_pages=%d", who,
-             (long long)tokens, hkv, num_pages);
-  SP_REQUIRE(d > 0 && d % 8 == 0, SP_ERR_UNSUPPORTED, "%s: head_dim %d (a multiple of 8)", who, d);
-  const int shift = page_shift(page_size);
-  SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %d (a power of two from 16 to 1024)", who, page_size);
-  if (tokens == 0 || num_pages == 0) return SP_OK;
-  SP_REQUIRE(k && v && k_pages && v_pages && slots, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
-  SP_REQUIRE(((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16 == 0 &&
-                 (k_stride_n | k_stride_h | v_stride_n | v_stride_h | k_stride_page | k_stride_slot | k_stride_page_h | v_stride_page |
-                  v_stride_slot | v_stride_page_h) % 8 == 0,
+  SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(x->tokens >= 0 && x->hkv > 0 && x->num_pages >= 0, SP_ERR_INVALID_ARGUMENT, "%s: tokens=%lld hkv=%lld num_pages=%lld", who,
+             (long long)x->tokens, (long long)x->hkv, (long long)x->num_pages);
+  SP_REQUIRE(x->d > 0 && x->d % 8 == 0 && x->d <= 65536, SP_ERR_UNSUPPORTED, "%s: head_dim %lld (a multiple of 8)", who, (long long)x->d);
+  const int shift = page_shift(x->page_size);
+  SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
+  if (x->tokens == 0 || x->num_pages == 0) return SP_OK;
+  SP_REQUIRE(x->k && x->v && x->k_pages && x->v_pages && x->slots, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(((uintptr_t)x->k | (uintptr_t)x->v | (uintptr_t)x->k_pages | (uintptr_t)x->v_pages) % 16 == 0 &&
+                 (x->k_stride_n | x->k_stride_h | x->v_stride_n | x->v_stride_h | x->k_stride_page | x->k_stride_slot | x->k_stride_page_h |
+                  x->v_stride_page | x->v_stride_slot | x->v_stride_page_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
-  const int64_t items = tokens * hkv * (d / 8), grid = sp_ceil_div(items, PW_THREADS * PW_ITEMS);
-  SP_REQUIRE(grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: tokens=%lld too many", who, (long long)tokens);
-  const WriteArgs a = {(const sp_bf16*)k, (const sp_bf16*)v, (sp_bf16*)k_pages, (sp_bf16*)v_pages, slots, items, (int64_t)num_pages << shift,
-                       hkv, d / 8, shift, k_stride_n, k_stride_h, v_stride_n, v_stride_h, k_stride_page, k_stride_slot, k_stride_page_h,
-                       v_stride_page, v_stride_slot, v_stride_page_h};
-  hipLaunchKernelGGL(sp_paged_write_kernel, dim3((unsigned)grid), dim3(PW_THREADS), 0, (hipStream_t)stream, a);
+  SP_REQUIRE(x->tokens <= (1ll << 40) && x->hkv <= 65536 && x->num_pages <= 0x7fffffffll, SP_ERR_UNSUPPORTED,
+             "%s: tokens=%lld hkv=%lld num_pages=%lld too many", who, (long long)x->tokens, (long long)x->hkv, (long long)x->num_pages);
+  const int64_t items = x->tokens * x->hkv * (x->d / 8), grid = sp_ceil_div(items, PW_THREADS * PW_ITEMS);
+  SP_REQUIRE(grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: tokens=%lld too many", who, (long long)x->tokens);
+  const WriteArgs a = {(const sp_bf16*)x->k, (const sp_bf16*)x->v, (sp_bf16*)x->k_pages, (sp_bf16*)x->v_pages, x->slots, items, x->num_pages << shift,
+                       (int)x->hkv, (int)(x->d / 8), shift, x->k_stride_n, x->k_stride_h, x->v_stride_n, x->v_stride_h, x->k_stride_page,
+                       x->k_stride_slot, x->k_stride_page_h, x->v_stride_page, x->v_stride_slot, x->v_stride_page_h};
+  hipLaunchKernelGGL(sp_paged_write_kernel, dim3((unsigned)grid), dim3(PW_THREADS), 0, (hipStream_t)x->stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }

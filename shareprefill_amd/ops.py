@@ -533,10 +533,15 @@ class PageTables(NamedTuple):
     free_left: torch.Tensor  # int32 [1]: pages left on the stack; below zero: so many were missing
 
 
-def _check_int(t: torch.Tensor, name: str, dtype, shape, device) -> None:
-    if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}, "
-                         f"got {t.dtype} {list(t.shape)} on {t.device}")
+def _is_int(t: torch.Tensor, dtype, n: int, device) -> bool:
+    return t.dtype is dtype and t.device == device and t.dim() == 1 and t.shape[0] == n and (n == 1 or t.stride(0) == 1)
+
+
+def _check_ints(device, *named) -> None:
+    """(name, tensor, dtype, length) each; asked only where a call's own check says that something is amiss."""
+    for name, t, dtype, n in named:
+        if not _is_int(t, dtype, n, device):
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _check_table(block_table: torch.Tensor, batch: int, device) -> None:
@@ -558,25 +563,32 @@ def page_tables(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
     if not lens.is_cuda:
         raise ValueError("lens must live on the GPU")
     dev, batch = lens.device, lens.shape[0] if lens.dim() == 1 else -1
-    _check_int(lens, "lens", torch.int32, (max(batch, 0),), dev)
-    _check_int(new_lens, "new_lens", torch.int32, (batch,), dev)
-    _check_int(free_pages, "free_pages", torch.int32, (free_pages.numel(),), dev)
-    _check_int(free_count, "free_count", torch.int32, (1,), dev)
+    room = free_pages.numel()
+    i32 = torch.int32
+    if not (_is_int(lens, i32, batch, dev) and _is_int(new_lens, i32, batch, dev) and _is_int(free_pages, i32, room, dev)
+            and _is_int(free_count, i32, 1, dev)):
+        _check_ints(dev, ("lens", lens, i32, batch), ("new_lens", new_lens, i32, batch), ("free_pages", free_pages, i32, room),
+                    ("free_count", free_count, i32, 1))
     _check_table(block_table, batch, dev)
     if max_new_tokens < 0:
         raise ValueError(f"max_new_tokens {max_new_tokens}")
     stream = _stream_handle(dev)
-    seq_lens, cu_new, free_left, positions = torch.empty(2 * batch + 2 + max_new_tokens, dtype=torch.int32, device=dev).split(
+    seq_lens, cu_new, free_left, positions = torch.empty(2 * batch + 2 + max_new_tokens, dtype=i32, device=dev).split_with_sizes(
         [batch, batch + 1, 1, max_new_tokens])
     slots = torch.empty(max_new_tokens, dtype=torch.int64, device=dev)
-    st = lib.sp_paged_tables(lens.data_ptr(), new_lens.data_ptr(), batch, page_size, num_pages, block_table.data_ptr(), block_table.stride(0),
-                             block_table.shape[1], free_pages.data_ptr(), free_pages.numel(), free_count.data_ptr(), max_new_tokens,
-                             seq_lens.data_ptr(), cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_left.data_ptr(), stream)
-    _lib.check(st, "sp_paged_tables")
+    st = lib.sp_paged_tables(_lib.PAGED_TABLES_ARGS.pack(
+        lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), seq_lens.data_ptr(),
+        cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_left.data_ptr(), batch, page_size, num_pages, block_table.shape[1],
+        block_table.stride(0), room, max_new_tokens, stream))
+    if st:
+        _lib.check(st, "sp_paged_tables")
     return PageTables(seq_lens, cu_new, slots, positions, free_left)
 
 
 def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, d: int, device) -> None:
+    if (k_pages.dtype is v_pages.dtype is torch.bfloat16 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == d
+            and k_pages.stride(3) == v_pages.stride(3) == 1 and k_pages.device == device and v_pages.device == device):
+        return
     for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         if t.dim() != 4:
             raise ValueError(f"{name} must be [num_pages, Hkv, page_size, D], got {tuple(t.shape)}")
@@ -586,8 +598,7 @@ def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, d: int, device) -
             raise ValueError(f"{name} must live on {device}")
         if t.stride(3) != 1:
             raise ValueError(f"{name} must have a contiguous head_dim axis")
-    if k_pages.shape != v_pages.shape or k_pages.shape[3] != d:
-        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must agree, with head_dim {d}")
+    raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must agree, with head_dim {d}")
 
 
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor) -> None:
@@ -604,12 +615,15 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     pages, heads, page_size, _ = k_pages.shape
     if heads != hkv:
         raise ValueError(f"the pools hold {heads} heads, k has {hkv}")
-    _check_int(slots, "slots", torch.int64, (n,), k.device)
+    if not _is_int(slots, torch.int64, n, k.device):
+        _check_ints(k.device, ("slots", slots, torch.int64, n))
     (k_h, k_n, _), (v_h, v_n, _) = k.stride(), v.stride()
     (kp_p, kp_h, kp_n, _), (vp_p, vp_h, vp_n, _) = k_pages.stride(), v_pages.stride()
-    st = lib.sp_paged_cache_write_bf16(k.data_ptr(), v.data_ptr(), n, hkv, d, k_n, k_h, v_n, v_h, k_pages.data_ptr(), v_pages.data_ptr(), pages,
-                                       page_size, kp_p, kp_n, kp_h, vp_p, vp_n, vp_h, slots.data_ptr(), _stream_handle(k.device))
-    _lib.check(st, "sp_paged_cache_write_bf16")
+    st = lib.sp_paged_cache_write_bf16(_lib.PAGED_WRITE_ARGS.pack(
+        k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), n, hkv, d, pages, page_size, k_n, k_h, v_n, v_h,
+        kp_p, kp_n, kp_h, vp_p, vp_n, vp_h, _stream_handle(k.device)))
+    if st:
+        _lib.check(st, "sp_paged_cache_write_bf16")
 
 
 def _window_of(window: Optional[int], sinks: int) -> int:
@@ -638,10 +652,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _check_pages(k_pages, v_pages, d, dev)
     pages, hkv, page_size, _ = k_pages.shape
     batch = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    _check_int(seq_lens, "seq_lens", torch.int32, (max(batch, 0),), dev)
+    if not _is_int(seq_lens, torch.int32, batch, dev):
+        _check_ints(dev, ("seq_lens", seq_lens, torch.int32, batch))
     _check_table(block_table, batch, dev)
     if cu_q is not None:
-        _check_int(cu_q, "cu_q", torch.int32, (batch + 1,), dev)
+        if not _is_int(cu_q, torch.int32, batch + 1, dev):
+            _check_ints(dev, ("cu_q", cu_q, torch.int32, batch + 1))
     elif n != batch:
         raise ValueError(f"without cu_q every request has one row: q has {n}, seq_lens {batch}")
     span = _window_of(window, sinks)
@@ -658,7 +674,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
         out.data_ptr(), 0 if ws is None else ws.data_ptr(), need, n, batch, hq, hkv, d, pages, page_size, block_table.shape[1],
         block_table.stride(0), span, sinks, q_n, q_h, k_p, k_n, k_h, v_p, v_n, v_h, softmax_scale, stream))
-    _lib.check(st, "sp_paged_attn_bf16")
+    if st:
+        _lib.check(st, "sp_paged_attn_bf16")
     return out
 
 
@@ -670,15 +687,18 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_
 
     Prompts (N = Nk), chunks and single tokens (N = 1) alike; head_dim 64 or 128, any strides with a contiguous head_dim axis."""
     lib = _lib.load()
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [B, H, N, D], got {tuple(t.shape)}")
-        if t.dtype is not torch.bfloat16:
-            raise AssertionError(f"{name} must be bfloat16, got {t.dtype}")
-        if not t.is_cuda or t.device != q.device:
-            raise ValueError(f"{name} must live on the GPU the queries are on")
-        if t.stride(3) != 1:
-            raise ValueError(f"{name} must have a contiguous head_dim axis")
+    dev = q.device
+    if not (q.dtype is k.dtype is v.dtype is torch.bfloat16 and q.is_cuda and q.dim() == k.dim() == v.dim() == 4 and k.device == dev
+            and v.device == dev and q.stride(3) == k.stride(3) == v.stride(3) == 1):
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            if t.dim() != 4:
+                raise ValueError(f"{name} must be [B, H, N, D], got {tuple(t.shape)}")
+            if t.dtype is not torch.bfloat16:
+                raise AssertionError(f"{name} must be bfloat16, got {t.dtype}")
+            if not t.is_cuda or t.device != dev:
+                raise ValueError(f"{name} must live on the GPU the queries are on")
+            if t.stride(3) != 1:
+                raise ValueError(f"{name} must have a contiguous head_dim axis")
     b, hq, n, d = q.shape
     _, hkv, nk, _ = k.shape
     if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
@@ -686,7 +706,6 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_
     if n > nk:
         raise ValueError(f"{n} queries are more than the {nk} positions there are")
     span = _window_of(window, sinks)
-    dev = q.device
     stream = _stream_handle(dev)
     out = torch.empty(b, n, hq, d, dtype=torch.bfloat16, device=dev)
     need = lib.sp_window_attn_workspace_bytes(b, n, nk, hq, hkv, d)
@@ -695,7 +714,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_
     st = lib.sp_window_attn_bf16(_lib.WINDOW_ATTN_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if ws is None else ws.data_ptr(), need, b, n, nk, hq, hkv, d, span, sinks,
         q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, softmax_scale, stream))
-    _lib.check(st, "sp_window_attn_bf16")
+    if st:
+        _lib.check(st, "sp_window_attn_bf16")
     return out
 
 

@@ -71,23 +71,23 @@ def test_tables_and_writes_refuse():
     lib = _lib.load()
 
     def tables(**kw):
-        a = dict(lens=P, new=P, batch=4, page=16, pages=50, table=P, stride=9, width=9, free=P, room=50, count=P, tokens=10, seq=P + 64, cu=P + 128,
-                 slots=P + 256, positions=P + 512, left=P + 1024, stream=None)
+        a = dict(lens=P, new=P, table=P, free=P, count=P, seq=P + 64, cu=P + 128, slots=P + 256, positions=P + 512, left=P + 1024, batch=4, page=16,
+                 pages=50, width=9, stride=9, room=50, tokens=10, stream=0)
         a.update(kw)
-        return lib.sp_paged_tables(*a.values())
+        return lib.sp_paged_tables(_lib.PAGED_TABLES_ARGS.pack(*a.values()))
 
-    for code, kw in [(-1, dict(batch=0)), (-2, dict(batch=4097)), (-1, dict(lens=None)), (-1, dict(free=None)), (-1, dict(slots=None)), (-1, dict(stride=8)),
+    for code, kw in [(-1, dict(batch=0)), (-2, dict(batch=4097)), (-1, dict(lens=0)), (-1, dict(free=0)), (-1, dict(slots=0)), (-1, dict(stride=8)),
                      (-1, dict(width=0)), (-2, dict(page=17)), (-2, dict(page=2048)), (-1, dict(tokens=-1)), (-1, dict(room=-1)),
                      (-2, dict(width=1 << 27, stride=1 << 27)), (-1, dict(left=P)), (-1, dict(seq=P))]:
         assert tables(**kw) == code, (kw, _message())
 
     def write(**kw):
-        a = dict(k=P, v=P, tokens=5, hkv=2, d=128, k_n=256, k_h=128, v_n=256, v_h=128, kp=P, vp=P, pages=9, page=16, kp_p=4096, kp_n=128, kp_h=2048,
-                 vp_p=4096, vp_n=128, vp_h=2048, slots=P, stream=None)
+        a = dict(k=P, v=P, kp=P, vp=P, slots=P, tokens=5, hkv=2, d=128, pages=9, page=16, k_n=256, k_h=128, v_n=256, v_h=128, kp_p=4096, kp_n=128,
+                 kp_h=2048, vp_p=4096, vp_n=128, vp_h=2048, stream=0)
         a.update(kw)
-        return lib.sp_paged_cache_write_bf16(*a.values())
+        return lib.sp_paged_cache_write_bf16(_lib.PAGED_WRITE_ARGS.pack(*a.values()))
 
-    for code, kw in [(-1, dict(k=None)), (-1, dict(slots=None)), (-1, dict(tokens=-1)), (-1, dict(hkv=0)), (-2, dict(d=12)), (-2, dict(page=48)),
+    for code, kw in [(-1, dict(k=0)), (-1, dict(slots=0)), (-1, dict(tokens=-1)), (-1, dict(hkv=0)), (-2, dict(d=12)), (-2, dict(page=48)),
                      (-2, dict(kp=P + 8)), (-2, dict(vp_h=2047)), (-2, dict(k_n=250)), (-2, dict(tokens=1 << 45))]:
         assert write(**kw) == code, (kw, _message())
     assert write(tokens=0) == 0 and write(pages=0) == 0
@@ -95,7 +95,8 @@ def test_tables_and_writes_refuse():
 
 def test_argument_structs_are_those_of_the_header():
     header = open(_lib.__file__.replace("shareprefill_amd/_lib.py", "include/shareprefill_hip.h")).read()
-    for name, packed in (("sp_paged_attn_args", _lib.PAGED_ATTN_ARGS), ("sp_window_attn_args", _lib.WINDOW_ATTN_ARGS)):
+    for name, packed in (("sp_paged_tables_args", _lib.PAGED_TABLES_ARGS), ("sp_paged_write_args", _lib.PAGED_WRITE_ARGS),
+                         ("sp_paged_attn_args", _lib.PAGED_ATTN_ARGS), ("sp_window_attn_args", _lib.WINDOW_ATTN_ARGS)):
         body = header[header.index("typedef struct %s {" % name):header.index("} %s;" % name)].split("{")[1]
         size, kinds = 0, ""
         for line in re.findall(r"([^;]+);", body):
