@@ -346,7 +346,8 @@ int sp_decode_attn_static_bf16(const void* q, const void* k, const void* v, int6
  * A cache is a pool of num_pages pages of page_size tokens (a power of two from 16 to 1024), one for K and one for V: bf16
  * [num_pages][hkv][page_size][d] with element strides for the page, head and slot axes and a contiguous head_dim axis.  Row b of
  * block_table (int32, table_width entries at a row stride of table_stride elements) names the pages of sequence b in order; an entry
- * outside [0, num_pages) is no page.  At most 4096 sequences a call. */
+ * outside [0, num_pages) is no page.  At most 4096 sequences a call; attention takes 2048 where they have more than one row, cu_q, or
+ * more than 16 query heads to a kv head. */
 
 /* The bookkeeping of a step: sequence b has lens[b] tokens in the cache and new_lens[b] (0 is allowed) to be added.
  * free_pages[0 .. *free_count) is a stack of unused pages, at most free_room; the pages that the new tokens open come off its top, in the
@@ -384,7 +385,8 @@ int sp_paged_cache_write_bf16(const sp_paged_write_args* args /* host */);
  * sequence b has rows cu_q[b] .. cu_q[b + 1] (null: one row each, tokens == batch) and seq_lens[b] keys; its query i stands at position
  * p = seq_lens[b] - its rows + i and sees the keys j <= p with j > p - window or j < sinks (window 0: all j <= p).  Keys without a page
  * are not seen; a query that sees nothing gives zeros.  out: bf16 [tokens][hq][d] contiguous; rows outside every sequence stay as they
- * were.  Device values out of range (lengths, offsets, pages) are held to what the arguments allow.  head_dim 64 or 128. */
+ * were.  Device values out of range (lengths, offsets, pages) are held to what the arguments allow.  head_dim 64 or 128.
+ * The workspace is 16-byte aligned and the call's own until it has run; out shares no memory with q. */
 typedef struct sp_paged_attn_args {
   const void *q, *k_pages, *v_pages;
   const int32_t *block_table, *seq_lens, *cu_q;

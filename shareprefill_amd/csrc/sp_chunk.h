@@ -15,11 +15,11 @@ struct CkArgs {
   int64_t sq_b, sq_n, sq_h, sk_b, sk_p, sk_n, sk_h, sv_b, sv_p, sv_n, sv_h;  // elements; _b between sequences, _p between pages
   int batch, tokens, width, num_pages, shift, n_keys, n_queries;
   int hkv, group, window, sinks;
-  int split;                // 1: sequences of one row are the single-token kernel's, the others the chunk kernel's
-  int slots, parts;         // row tiles per kv head; parts of their line at most, or 0: a workgroup per row tile
+  int slots, parts;         // row tile numbers per kv head; parts of their line at most, or 0: row tiles stay whole
+  int tiles, together;      // whole ones (pg_deal): of a sequence, sequences dealt at a time
   float scale_log2;
-  float* o_part;            // [workgroup][2][128][D]: its first row tile where that began in an earlier part, its last where that goes on
-  float2* ml_part;          // [workgroup][2][128]
+  float* o_part;            // [workgroup][2][rows of a tile][D]: its first row tile where that began in an earlier part, its last where that goes on
+  float2* ml_part;          // [workgroup][2][rows of a tile]
   int4* notes;              // [workgroup], and where by_slot is not null [row tile number][kv head]
   int4* by_slot;
 };

@@ -3,17 +3,23 @@
 //   j <= p with (j > p - window or j < sinks):   out = sum_j exp(scale q . k_j) v_j / sum_j exp(scale q . k_j)
 // in one pass over the keys with a running maximum and sum; a query that sees nothing is zero.
 //
-// The tile loop is that of the short-prompt kernel (sp_attn_short.hip): 4 waves of 32 rows, K and V tiles of 64 keys double-buffered
-// in LDS by direct loads, S^T = K . Q^T, P^T from its accumulators in place, V by the transposing LDS read.  What differs:
-//   * a row is a (token, query head of the kv group) pair, the heads of a token side by side, so that a few new tokens fill a tile's 128
-//     rows as far as they can and all heads of the group share its keys: a chunk of 32 tokens of 4 heads reads the cache once;
-//   * a load's address comes from the sequence's table.  A wave holds 64 entries of it, a lane each; a load instruction covers 4 rows (8 of
-//     64 channels), which lie in one page, so a page is a scalar: a buffer descriptor of its own, whose length ends with the sequence: rows
-//     behind it, and pages that are none, read as zeros, whatever a page's unused end holds;
-//   * tiles in front of the window that hold no sinks are left out, and only tiles that some row of the wave sees in part are masked;
-//   * where a launch has few row tiles their tiles form a line that is cut into equal parts, one workgroup each (sp_paged_plan.h): every CU
-//     has as much to do as the others, whatever the sequences' lengths, which only the device knows.  A row tile that a cut goes through
-//     leaves fp32 partials that a second launch merges; the lengths need no host, so the call can be captured into a graph.
+// Rows.  A row is a (token, query head of the kv group) pair, the heads of a token side by side: a few new tokens fill a tile's 256 rows as far
+// as they can, and all heads of a group share its keys.  Eight waves of 32 rows work on the same blocks of 128 keys, so K and V are read once
+// per 256 rows: with four waves and 128 rows the loads alone held the loop up (2048 tokens over 65001 keys 2630 -> 2330 us).
+// Keys.  K and V lie in rings of four sub-tiles of 64 keys each (128 KiB of LDS with 128 channels), filled by direct loads a block ahead; one
+// barrier a block.  A wave's own pipeline (sp_pipeline.h: S^T = K . Q^T of a half-tile, the softmax of the one in front and P . V of the one
+// in front of that, interleaved instruction by instruction, P^T taken from the accumulators in place, V by the transposing LDS read) keeps the
+// matrix cores fed: 2330 -> 2004 us.
+// Pages.  A load's address comes from the sequence's table: a lane holds a page's addresses and length, and a load takes them by lane reads
+// into a buffer descriptor that ends with the sequence, so rows behind it, and pages that are none, read as zeros, whatever stands there.
+// Masks.  Blocks in front of the window that hold no sinks are left out; a wave masks only what its rows see in part.
+// Workgroups, one a CU, stay for the launch: the next row tile's first keys and its queries land under the end of the one in front
+// (30001 tokens in a window of 4096 2282 -> 1811 us).  The row tiles' blocks form a line that is cut into equal parts, one workgroup each
+// (sp_paged_plan.h): every CU has as much to do as the others, whatever the sequences' lengths, which only the device knows; row tiles that a
+// cut goes through leave fp32 partials that a second launch merges.  No length comes to the host, so the call can be captured into a graph.
+// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1765 us, 1216 TFLOP/s, the rate of a large
+// bf16 matrix product on this card; 30001 tokens in a window of 4096 1175 TFLOP/s.  Short calls: some 10 us go by until the line is laid out
+// and the first keys have landed, a row tile's turn takes 5 us beside its blocks of 4 us each.
 #include "sp_chunk.h"
 #include "sp_pipeline.h"
 
@@ -31,7 +37,7 @@
 #define CK_RING 4                // sub-tiles of K in LDS, and of V
 #define CK_SUB_BYTES(D) (CK_SUB * (D) * 2)
 #define CK_LDS_BYTES(D) (2 * CK_RING * CK_SUB_BYTES(D))  // the rings; offsets and lengths of the sequences stand behind them
-#define CK_MAX_SEQS 2048
+#define CK_MAX_SEQS 2048  // their offsets and lengths take 16 KiB of LDS
 
 typedef __attribute__((address_space(3))) void* ck_lds_ptr;
 typedef uint32_t ck_u32x2 __attribute__((ext_vector_type(2)));
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       for (int i = x0; i < x1; ++i) {
         while (b + 1 < a.batch && pg_first_slot(cu_s[b + 1], a.group, b + 1, TILE_ROWS) <= i) ++b;
         const int q_len = pg_max(0, cu_s[b + 1] - cu_s[b]), rt = (int)(i - pg_first_slot(cu_s[b], a.group, b, TILE_ROWS));
-        if (rt < 0 || (a.split && q_len == 1) || rt >= pg_row_tiles(q_len, a.group, TILE_ROWS)) {
+        if (rt < 0 || rt >= pg_row_tiles(q_len, a.group, TILE_ROWS)) {
           visit(i, 0, 0);
           continue;
         }
@@ -245,30 +251,34 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   int seq = a.parts == 0 || x >= a.slots ? 0 : __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, x, lane));
   auto next_piece = [&](Piece& p) {  // false: there is none
     for (;;) {
-      int begin = 0, here = x, end = -1;
+      int begin = 0, end = -1;
       if (a.parts == 0) {
-        // whole row tiles, there and back over the workgroups of the kv head: their work is even, and those that run at a time are neighbours
-        const int wgs = (int)(gridDim.x / a.hkv), place = turn * wgs + (turn & 1 ? wgs - 1 - part : part);
-        if (turn * (int64_t)wgs >= a.slots) return false;
-        ++turn;
-        if (place >= a.slots) continue;
-        here = a.slots - 1 - place;  // (the last rows of a prompt see the most keys)
-        seq = pg_min((int)((unsigned)here * (unsigned)TILE_ROWS / (unsigned)(a.n_queries * a.group + TILE_ROWS)), a.batch - 1);  // (or the one behind)
+        const int wgs = (int)(gridDim.x / a.hkv);
+        if (turn * (int64_t)wgs >= (int64_t)a.tiles * a.batch) return false;
+        int at_b, at_rt;
+        if (!pg_deal(turn++, part, wgs, a.batch, a.tiles, a.together, &at_b, &at_rt)) continue;
+        // (quotients come from vector registers)
+        p.slot = 0;
+        p.b = __builtin_amdgcn_readfirstlane(at_b);
+        p.rt = __builtin_amdgcn_readfirstlane(at_rt);
+        p.start = p.b * a.n_queries;
+        p.q_len = a.n_queries;
+        p.len = a.n_keys;
       } else {
         if (x >= a.slots || !(x < x_end || (x == x_end && tile_end > 0))) return false;
         begin = tile_begin;
         if (x == x_end) end = tile_end;
         tile_begin = 0;
-        ++x;
+        const int here = x++;
+        while (seq + 1 < a.batch && pg_first_slot(start_of(seq + 1), a.group, seq + 1, TILE_ROWS) <= here) ++seq;
+        p.slot = here;
+        p.b = seq;
+        p.start = start_of(seq);
+        p.q_len = pg_max(0, start_of(seq + 1) - p.start);
+        p.len = a.lens != nullptr ? from_lds(lds_len + 4u * seq) : a.n_keys;
+        p.rt = (int)(here - pg_first_slot(p.start, a.group, seq, TILE_ROWS));
+        if (p.rt < 0 || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
       }
-      while (seq + 1 < a.batch && pg_first_slot(start_of(seq + 1), a.group, seq + 1, TILE_ROWS) <= here) ++seq;
-      p.slot = here;
-      p.b = seq;
-      p.start = start_of(seq);
-      p.q_len = pg_max(0, start_of(seq + 1) - p.start);
-      p.len = a.lens != nullptr ? from_lds(lds_len + 4u * seq) : a.n_keys;
-      p.rt = (int)(here - pg_first_slot(p.start, a.group, seq, TILE_ROWS));
-      if (p.rt < 0 || (a.split && p.q_len == 1) || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
       int p0, p1;
       pg_tile_positions(p.rt, p.q_len, p.len, a.group, TILE_ROWS, &p0, &p1);
       p.span = ck_span(a, p0, p1, CK_BLOCK);
@@ -387,8 +397,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   // Block n of the workgroup (over all its pieces) is sub-tiles 2 n and 2 n + 1; sub-tile s lives in slot s % 4 of either ring.  One wait and
   // barrier per block: while it is computed on (K of 2 n, 2 n + 1, V of 2 n - 1, 2 n: P . V trails by a sub-tile) K of 2 n + 2, 2 n + 3 and V of
   // 2 n + 1, 2 n + 2 are on their way, sent out in four parts between the block's steps, V of 2 n + 1 first: the others are the next block's, whose
-  // pages may be others.  Behind a piece's last block that is the next piece's
-  // first one: its tiles land, and its queries, under the end of the piece in front.
+  // pages may be others.  Behind a
+  // piece's last block that is the next piece's first one: its tiles land, and its queries, under the end of the piece in front.
   Piece cur_p, next_p;
   bool have = next_piece(cur_p), primed = false;
   Block cur = {0, 0u}, nxt = {0, 0u};
@@ -592,7 +602,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
         for (int j = 0; j < 4; ++j) spoilt[qt] |= o[ct][qt][j] != o[ct][qt][j];
-      spoilt[qt] &= mine;
+      // (a row whose sum is a NaN saw a logit that is none, or an infinite one: it is a NaN in all its channels as it is)
+      spoilt[qt] = spoilt[qt] && mine && l[qt] == l[qt];
       if (whole) {
         const float inv_l = l[qt] > 0.f || l[qt] != l[qt] ? 1.0f / l[qt] : 0.f;
         // (lane groups 2i and 2i + 1 trade halves of two neighbouring channel tiles: 16 bytes a store, 64 contiguous ones a row)
@@ -679,26 +690,31 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
-struct CkPlan {
-  int64_t slots, grid, merges;  // merges: workgroups of the merging launch, a band of rows
-  int parts;
-};
-// Workgroups that are resident at once: two a CU with 128 channels.
+// Workgroups that are resident at once: one a CU.
 #define CK_PLACES 256
-static CkPlan ck_plan(int64_t tokens, int32_t batch, int32_t hkv, int32_t group, bool uniform) {
-  CkPlan p;
-  p.slots = pg_slots(tokens, group, batch, CK_ROWS);
-  const int64_t room = CK_PLACES / hkv;
-  const int64_t wgs = room < 1 ? 1 : room;  // of a kv head
-  p.parts = uniform && p.slots >= 4 * wgs ? 0 : (int)wgs;
-  p.grid = wgs * hkv;
-  p.merges = p.slots * hkv < p.grid ? p.slots * hkv : p.grid;
-  return p;
-}
-static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, bool uniform) {
+static int ck_workgroups(int32_t hkv) { return hkv < CK_PLACES ? CK_PLACES / hkv : 1; }  // of a kv head
+static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d) {
   if (tokens <= 0 || batch <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || (d != 64 && d != 128)) return 0;
-  const CkPlan p = ck_plan(tokens, batch, hkv, hq / hkv, uniform);
-  return p.parts == 0 ? 0 : (size_t)p.grid * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + 2 * sizeof(int4));
+  return (size_t)ck_workgroups(hkv) * hkv * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + 2 * sizeof(int4));
+}
+
+// Whether row tiles of a call whose sequences have as many rows and keys each stay whole: the longest workgroup against even parts, which take
+// a sixteenth longer a block (their row tiles' keys lie further apart) and a merging launch, eight blocks' time.  us, whole / cut, 32 heads
+// over 8: 2 tokens 9.7 / 13.6, prompts of 2048 59 / 64, 4096 126 / 150, in a window of 1024 75 / 84, 16384 1735 / 1850, 8 of 1024 88 / 98; cut
+// because whole ones are uneven: 64 tokens over 16384, two row tiles a head, 42.
+static bool ck_whole(const CkArgs& a, int wgs) {
+  if ((int64_t)a.tiles * a.batch >= 4 * wgs) return true;
+  int64_t units[CK_PLACES] = {0}, most = 0, total = 0;
+  for (int turn = 0; turn * wgs < a.tiles * a.batch; ++turn)
+    for (int part = 0; part < wgs; ++part) {
+      int b, rt, p0, p1;
+      if (!pg_deal(turn, part, wgs, a.batch, a.tiles, a.together, &b, &rt)) continue;
+      pg_tile_positions(rt, a.n_queries, a.n_keys, a.group, CK_ROWS, &p0, &p1);
+      const int n = pg_span_units(pg_span(p0, p1, a.window, a.sinks, CK_BLOCK)) + PG_OVERHEAD;
+      units[part] += n, total += n;
+      if (units[part] > most) most = units[part];
+    }
+  return most <= total / wgs * 17 / 16 + 8;
 }
 
 // what a launch needs, checked before anything is launched
@@ -716,19 +732,25 @@ static int ck_check_launch(const char* who, const CkArgs& a, size_t need, const 
 
 static int ck_launch(const char* who, CkArgs& a, int32_t d, void* workspace, hipStream_t s) {
   const bool uniform = a.cu == nullptr && a.lens == nullptr;  // as many queries and keys in every sequence
-  const CkPlan plan = ck_plan(a.tokens, a.batch, a.hkv, a.group, uniform);
-  a.slots = (int)plan.slots;
-  a.parts = plan.parts;
+  const int wgs = ck_workgroups(a.hkv), grid = wgs * a.hkv;
+  a.slots = (int)pg_slots(a.tokens, a.group, a.batch, CK_ROWS);
+  a.tiles = uniform ? (int)pg_row_tiles(a.n_queries, a.group, CK_ROWS) : 0;
+  a.together = uniform ? pg_together(a.tiles, wgs, a.batch) : 0;
+  a.parts = uniform && ck_whole(a, wgs) ? 0 : wgs;
   a.o_part = (float*)workspace;
-  a.ml_part = (float2*)(a.o_part + (size_t)plan.grid * 2 * (size_t)CK_ROWS * d);
-  a.notes = (int4*)(a.ml_part + (size_t)plan.grid * 2 * CK_ROWS);
-  const size_t lds = CK_LDS_BYTES(d) + (plan.parts != 0 ? (size_t)(2 * a.batch + 1) * sizeof(int) : 0);
-  a.by_slot = plan.parts != 0 && plan.merges < plan.grid ? a.notes + plan.grid : nullptr;
-  const int band = plan.merges <= 128 ? 16 : 64;
+  a.ml_part = (float2*)(a.o_part + (size_t)grid * 2 * (size_t)CK_ROWS * d);
+  a.notes = (int4*)(a.ml_part + (size_t)grid * 2 * CK_ROWS);
+  const size_t lds = CK_LDS_BYTES(d) + (a.parts != 0 ? (size_t)(2 * a.batch + 1) * sizeof(int) : 0);
+  const bool by_slot = (int64_t)a.slots * a.hkv < grid;
+  const int merges = by_slot ? a.slots * a.hkv : grid;  // workgroups of the merging launch, a band of rows
+  a.by_slot = a.parts != 0 && by_slot ? a.notes + grid : nullptr;
+  // Rows a merging workgroup takes: 16 spread few row tiles of many parts over more workgroups, 64 need fewer launches of them.  us, 16 / 64:
+  // 64 tokens over 16384 keys (merges 16) 42.3 / 50.4, 2 over 8192 (16) 23.6 / 28.3; 512 over 8192 (72) 86 / 81, 2048 over 2048 (256) 74 / 60.
+  const int band = merges <= 32 ? 16 : 64;
   auto go = [&](auto kernel, auto few, auto many) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)plan.grid), dim3(CK_THREADS), lds, s, a);
-    if (plan.parts != 0)
-      hipLaunchKernelGGL(band == 16 ? few : many, dim3((unsigned)plan.merges, CK_ROWS / band), dim3(CM_THREADS), 0, s, a, (int)plan.grid);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(CK_THREADS), lds, s, a);
+    if (a.parts != 0)
+      hipLaunchKernelGGL(band == 16 ? few : many, dim3((unsigned)merges, CK_ROWS / band), dim3(CM_THREADS), 0, s, a, grid);
   };
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -762,17 +784,13 @@ static int ck_check(const char* who, int64_t hq, int64_t hkv, int64_t d, int64_t
 }
 static int ck_window(int64_t window) { return window == 0 || window > PG_NO_WINDOW ? PG_NO_WINDOW : (int)window; }
 // offsets inside a page (`rows` of them) have 32 bits
-static bool ck_rows_ok(int64_t stride_n, int64_t rows) { return stride_n >= 0 && stride_n < (1ll << 24) && stride_n * rows < (1ll << 30) && stride_n % 8 == 0; }
-
-// Sequences of one row among others go to the single-token kernel, in launches of their own, where there can be many: a row tile of the
-// chunk kernel that holds one token is nearly empty.  The lengths are the device's; what the host knows is the average.
-static bool ck_splits(int64_t tokens, int32_t batch) { return batch >= 4 && tokens < 256ll * batch; }
+static bool ck_rows_ok(int64_t stride_n, int64_t rows) {
+  return stride_n >= 0 && stride_n < (1ll << 24) && stride_n * rows < (1ll << 30) && stride_n % 8 == 0;
+}
 
 extern "C" size_t sp_paged_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens) {
-  const size_t chunks = ck_workspace_bytes(tokens, batch, hq, hkv, d, false);
-  if (tokens > 0 && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128))
-    return single_tokens ? pd_workspace_bytes(hkv, d) : ck_splits(tokens, batch) ? chunks + pd_workspace_bytes(hkv, d) : chunks;
-  return chunks;
+  const bool singles = single_tokens && hq > 0 && hkv > 0 && hq % hkv == 0 && hq / hkv <= PD_MAX_GROUP && (d == 64 || d == 128);
+  return singles && tokens > 0 ? pd_workspace_bytes(hkv, d) : ck_workspace_bytes(tokens, batch, hq, hkv, d);
 }
 
 extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
@@ -797,8 +815,8 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k_pages | (uintptr_t)x->v_pages | (uintptr_t)x->out) % 16 == 0 &&
                  (x->q_stride_n | x->q_stride_h | x->k_stride_page | x->k_stride_h | x->v_stride_page | x->v_stride_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
-  SP_REQUIRE(ck_rows_ok(x->k_stride_slot, x->page_size) && ck_rows_ok(x->v_stride_slot, x->page_size), SP_ERR_UNSUPPORTED, "%s: slot strides %lld / %lld unsupported", who,
-             (long long)x->k_stride_slot, (long long)x->v_stride_slot);
+  SP_REQUIRE(ck_rows_ok(x->k_stride_slot, x->page_size) && ck_rows_ok(x->v_stride_slot, x->page_size), SP_ERR_UNSUPPORTED,
+             "%s: slot strides %lld / %lld unsupported", who, (long long)x->k_stride_slot, (long long)x->v_stride_slot);
   CkArgs a = {};
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k_pages, a.v = (const sp_bf16*)x->v_pages;
   a.table = x->block_table, a.lens = x->seq_lens, a.cu = x->cu_q, a.out = (sp_bf16*)x->out;
@@ -815,20 +833,12 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   if (rc) return rc;
   const int64_t room = x->table_width << shift;
   if (pd_takes(a)) return pd_launch(a, room, (int)x->d, x->workspace, (hipStream_t)x->stream);
-  char* workspace = (char*)x->workspace;
-  if (a.cu != nullptr && a.group <= PD_MAX_GROUP && ck_splits(a.tokens, a.batch)) {
-    a.split = 1;
-    CkArgs singles = a;
-    rc = pd_launch(singles, room, (int)x->d, workspace, (hipStream_t)x->stream);
-    if (rc) return rc;
-    workspace += pd_workspace_bytes(a.hkv, (int)x->d);
-  }
-  return ck_launch(who, a, (int)x->d, workspace, (hipStream_t)x->stream);
+  return ck_launch(who, a, (int)x->d, x->workspace, (hipStream_t)x->stream);
 }
 
 extern "C" size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d) {
   (void)n_keys;
-  return batch <= 0 || n <= 0 ? 0 : n == 1 ? sp_paged_attn_workspace_bytes(batch, batch, hq, hkv, d, 1) : ck_workspace_bytes(batch * n, batch, hq, hkv, d, true);
+  return batch <= 0 || n <= 0 ? 0 : n == 1 ? sp_paged_attn_workspace_bytes(batch, batch, hq, hkv, d, 1) : ck_workspace_bytes(batch * n, batch, hq, hkv, d);
 }
 
 extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
@@ -850,7 +860,7 @@ extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
              (long long)x->k_stride_n, (long long)x->v_stride_n);
   CkArgs a = {};
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k, a.v = (const sp_bf16*)x->v, a.out = (sp_bf16*)x->out;
-  a.shift = 6;  // a tile is a page
+  a.shift = 6;  // a sub-tile is a page
   a.sq_b = x->q_stride_b, a.sq_n = x->q_stride_n, a.sq_h = x->q_stride_h;
   a.sk_b = x->k_stride_b, a.sk_n = x->k_stride_n, a.sk_h = x->k_stride_h, a.sk_p = x->k_stride_n << a.shift;
   a.sv_b = x->v_stride_b, a.sv_n = x->v_stride_n, a.sv_h = x->v_stride_h, a.sv_p = x->v_stride_n << a.shift;

@@ -16,8 +16,10 @@
 #include "sp_ring.h"
 
 #define PD_ROWS PD_MAX_GROUP
-#define PD_OVERHEAD 4   // units of a line that a sequence counts beside its steps: queries, first loads, the waves' meeting
-#define PD_MIN_SHARE 4  // units of a part at least
+// Units of a line that a sequence counts beside its steps: queries, first loads, the waves' meeting; units of a part at least.  (us, 8 and 8 /
+// 4 and 4: one token over 1025 keys 11.5 / 9.9, 64 over 500 27.0 / 23.5, 64 over 8192 128.7 either way.)
+#define PD_OVERHEAD 4
+#define PD_MIN_SHARE 4
 
 template <int D>
 using PdShape = DsShape<D, D / 16, D == 64 ? 8 : 4, 152>;
@@ -36,7 +38,6 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
 
   // ---- which sequences, and which steps of the first and the last ----
   auto span_of = [&](int len) { return ck_span(a, len - 1, len - 1, DS_KEYS); };
-  auto single = [&](int i) { return !a.split || ck_start(a, i + 1) - ck_start(a, i) == 1; };
   int b, b_end, begin = 0, end = 0;
   if (a.parts == 0) {
     b = part;
@@ -45,7 +46,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     // every wave for itself, 64 sequences at a time
     auto sums = [&](int b0, int* steps, int64_t* upto) {  // of the lane's sequence; units up to it, it included
       const int i = b0 + lane;
-      *steps = i < a.batch && single(i) ? pg_span_units(span_of(ck_len(a, i))) : -PD_OVERHEAD;  // (others take no room in the line)
+      *steps = i < a.batch ? pg_span_units(span_of(ck_len(a, i))) : -PD_OVERHEAD;  // (none: no room in the line)
       int64_t at = *steps + PD_OVERHEAD;
 #pragma unroll
       for (int o = 1; o < SP_WAVE; o <<= 1) {
@@ -57,12 +58,13 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     int steps = 0;
     int64_t upto = 0, total = 0;
     if (a.batch == 1) {  // (no sums to form: half a microsecond of a chat's step)
-      steps = single(0) ? pg_span_units(span_of(ck_len(a, 0))) : -PD_OVERHEAD;
+      steps = pg_span_units(span_of(ck_len(a, 0)));
       upto = total = steps + PD_OVERHEAD;
-    } else
-    for (int b0 = 0; b0 < a.batch; b0 += SP_WAVE) {
-      sums(b0, &steps, &upto);
-      total += __shfl(upto, SP_WAVE - 1, SP_WAVE);
+    } else {
+      for (int b0 = 0; b0 < a.batch; b0 += SP_WAVE) {
+        sums(b0, &steps, &upto);
+        total += __shfl(upto, SP_WAVE - 1, SP_WAVE);
+      }
     }
     const int64_t parts = pg_parts(total, a.parts, PD_MIN_SHARE);
     int seq[2], step[2];
@@ -97,7 +99,6 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
   const uint32_t v_at = ring + Shape::K_BYTES + v_key * (CT * 32) + 8 * (lq & 3);
 
   for (bool first = true; b < a.batch && (b < b_end || (b == b_end && end > 0)); ++b, begin = 0) {
-    if (!single(b)) continue;
     const int len = ck_len(a, b), pos = len - 1;
     const PgSpan span = span_of(len);
     const int steps = pg_span_units(span), s_end = b == b_end ? pg_min(end, steps) : steps;
@@ -106,7 +107,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
 
     dc_bf16x8 qb[KS];
     {
-      const sp_bf16* src = a.q + (int64_t)(PAGED ? ck_start(a, b) : b) * (PAGED ? a.sq_n : a.sq_b) + (int64_t)(kvh * g + (lq < g ? lq : 0)) * a.sq_h + 8 * gr;
+      const sp_bf16* src = a.q + b * (PAGED ? a.sq_n : a.sq_b) + (int64_t)(kvh * g + (lq < g ? lq : 0)) * a.sq_h + 8 * gr;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const dc_u32x4 raw = *reinterpret_cast<const dc_u32x4*>(src + 32 * ks);
@@ -174,7 +175,6 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
 
     if (!first) __syncthreads();  // the rings are free
     first = false;
-    const int64_t row = ck_start(a, b);  // of q and out
     const int s0 = begin + wave;
     uint32_t seen[NB - 1];
 #pragma unroll
@@ -286,7 +286,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
     const int64_t slab = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
     if (!whole) {
       if (from_start)
-        note.y = g, note.w = (int)row;
+        note.y = g, note.w = b;
       else
         note.x = to_end ? CK_LAST : CK_MIDDLE;
     }
@@ -305,7 +305,7 @@ __global__ __launch_bounds__((PdShape<D>::WAVES * SP_WAVE)) void sp_paged_decode
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // (a sequence without keys: zeros)
-        *reinterpret_cast<uint2*>(a.out + (row * a.hkv * g + kvh * g + h) * D + c) =
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)b * a.hkv * g + kvh * g + h) * D + c) =
             make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
       } else {
         *reinterpret_cast<ds_floatx4*>(a.o_part + (slab * PD_ROWS + h) * D + c) = acc;
@@ -366,9 +366,12 @@ int pd_launch(CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream
   if (a.window < PG_NO_WINDOW && (int64_t)a.window + a.sinks + 2 * DS_KEYS < max_keys) max_keys = (int64_t)a.window + a.sinks + 2 * DS_KEYS;
   const int64_t pairs = (int64_t)a.batch * a.hkv, units = sp_ceil_div(max_keys, DS_KEYS) + PD_OVERHEAD;
   const int64_t most = pg_parts(units * a.batch, pd_parts(a.hkv), PD_MIN_SHARE);
-  // A workgroup a sequence where that takes the longest of them no longer than even parts and their merging launch (units).
-  // A table's width only bounds the lengths: sequences are taken for five eighths of it on average.
-  const int64_t whole = sp_ceil_div(pairs, 256) * units, cut = sp_ceil_div(pairs * units, 256) * (a.lens != nullptr ? 5 : 8) / 8 + 16;
+  // A workgroup a sequence where that takes the longest of them no longer than even parts and their merging launch, in units (of 64 channels
+  // one takes half the time).  A table's width only bounds the lengths: sequences are taken for five eighths of it on average.
+  // us, whole / cut, sequences of up to n keys; 32 heads over 8: 1 of 200 7.3 / 9.7, 1 of 1025 18.8 / 10.0, 16 of 1000 19.7 / 19.2, 64 of 500
+  // 23.6 / 27.2, 128 of 2000 143 / 127; 14 over 2 of 64 channels: 1 of 1025 10.0 / 9.2, 16 of 1000 10.0 / 13.0, 128 of 2000 19.7 / 27.4.
+  const int64_t whole = sp_ceil_div(pairs, 256) * units;
+  const int64_t cut = sp_ceil_div(pairs * units, 256) * (a.lens != nullptr ? 5 : 8) / 8 + (d == 64 ? 34 : 16);
   a.parts = whole <= cut || most == 1 ? 0 : (int)most;
   const int64_t grid = a.parts == 0 ? pairs : (int64_t)a.parts * a.hkv;
   a.o_part = (float*)workspace;

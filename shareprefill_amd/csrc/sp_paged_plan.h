@@ -12,7 +12,8 @@
 #define PG_MAX_SEQS 4096           // sequences of a call
 #define PG_MAX_KEYS (1 << 30)      // keys of a sequence: positions and their differences have 31 bits
 #define PG_NO_WINDOW PG_MAX_KEYS   // every key in front of a query lies inside it
-                                   // a row tile has `tile` rows: (token, query head of the kv group) pairs, the heads of a token side by side
+
+// (A row tile has `tile` rows: (token, query head of the kv group) pairs, the heads of a token side by side.)
 
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
 PG_FN int pg_max(int a, int b) { return a > b ? a : b; }
@@ -78,4 +79,18 @@ PG_FN int pg_near(int64_t total, int64_t parts) {
 PG_FN int pg_snap(int64_t off, int n, int overhead, int near) {
   const int64_t t = off - overhead;
   return t < near ? 0 : t > n - near ? n : (int)t;
+}
+
+// Sequences of as many rows and keys each may keep their row tiles whole: a kv head's workgroups are dealt them turn by turn, there and back,
+// the longest first.  The tiles of `together` sequences, four turns of them, are dealt before the next ones', so that workgroups that run at a
+// time read the same keys.  (32 prompts of 1024 tokens, us, two turns / four / all at once: 32 heads over 8 346 / 351 / 368, in a window of
+// 256 280 / 267 / 272, 28 over 4 336 / 328 / 313, 14 over 2 of 64 channels 123 / 110 / 104.)  false: nothing falls to the workgroup in this turn.
+PG_FN int pg_together(int tiles, int workgroups, int batch) { return pg_min(pg_max(1, (4 * workgroups + tiles - 1) / tiles), batch); }
+PG_FN bool pg_deal(int turn, int part, int workgroups, int batch, int tiles, int together, int* b, int* rt) {
+  const int place = turn * workgroups + (turn & 1 ? workgroups - 1 - part : part);
+  if (place >= tiles * batch) return false;
+  const int deal = place / (together * tiles), at = place - deal * (together * tiles), n = pg_min(together, batch - deal * together);
+  *rt = tiles - 1 - at / n;
+  *b = deal * together + at % n;
+  return true;
 }

@@ -643,8 +643,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Request b has rows cu_q[b] .. cu_q[b + 1] of q (int32 [B + 1]; None: one row each, T == B) and seq_lens[b] keys (int32 [B]), those
     in the pages that block_table[b] (int32 [B, W]) names; its rows are its last positions.  A row at position p sees keys j <= p and,
     with a window, of those j > p - window and j < sinks.  Keys without a page (an entry outside the pool) are not seen; a row that sees
-    nothing is zero.  Rows of `out` outside every request stay as they were (undefined in a tensor made here).
-    head_dim 64 or 128, page_size a power of two from 16 to 1024, at most 4096 requests.  Lengths and pages are read on the device."""
+    nothing is zero.  Rows of `out` outside every request stay as they were (undefined in a tensor made here); `out` shares no memory with q.
+    head_dim 64 or 128, page_size a power of two from 16 to 1024; at most 4096 requests of single tokens without cu_q and groups of up to 16
+    query heads, else 2048.  Lengths and pages are read on the device.  Scratch memory: up to 68 MB, from torch's allocator, for the call."""
     lib = _lib.load()
     _check_hnd(q, "q")
     hq, n, d = q.shape
@@ -685,7 +686,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_
     views, N <= Nk, the queries being the last N positions -> out bf16 [B, N, Hq, D].  The query at position p sees keys j <= p with
     j > p - window or j < sinks; window None: all j <= p (a prompt's next chunk over a contiguous cache).
 
-    Prompts (N = Nk), chunks and single tokens (N = 1) alike; head_dim 64 or 128, any strides with a contiguous head_dim axis."""
+    Prompts (N = Nk), chunks and single tokens (N = 1) alike; head_dim 64 or 128, any strides with a contiguous head_dim axis; B at most 2048
+    (4096 for single tokens of groups of up to 16 query heads)."""
     lib = _lib.load()
     dev = q.device
     if not (q.dtype is k.dtype is v.dtype is torch.bfloat16 and q.is_cuda and q.dim() == k.dim() == v.dim() == 4 and k.device == dev

@@ -7,7 +7,8 @@
         out = cache.attend(layer, q, softmax_scale)
     cache.release(finished)
 
-A step reads no device value on the host, so it can be recorded into a HIP graph and replayed with other lengths.  The reference keeps no
+A step (begin_step, write, attend) reads no device value on the host, so it can be recorded into a HIP graph and replayed with other lengths;
+release runs between steps.  The reference keeps no
 cache of its own (its decode step reads a contiguous one, shareprefill_attn.py:146-155).
 """
 
@@ -72,7 +73,8 @@ class PagedKVCache:
                                    window=window, sinks=sinks, out=out)
 
     def release(self, finished: torch.Tensor) -> None:
-        """Puts the pages of the requests with finished[r] (bool [max_requests]) back on the stack; their rows are empty again."""
+        """Puts the pages of the requests with finished[r] (bool [max_requests]) back on the stack; their rows are empty again.
+        Not for a captured graph."""
         if finished.dtype is not torch.bool or tuple(finished.shape) != (self.max_requests,) or finished.device != self.lens.device:
             raise ValueError(f"finished must be bool [{self.max_requests}] on {self.lens.device}")
         back = finished[:, None] & (self.block_table >= 0)

@@ -75,6 +75,27 @@ def test_every_row_is_the_mean_of_what_it_sees(gpu_device):
         assert (err <= want.abs() * 2.0 ** -8 * 1.01 + n * 2.0 ** -24 * mean_abs).all(), (n, window, err.max().item())
 
 
+@pytest.mark.parametrize("batch,n,nk,hq,hkv,d", [(5, 700, 700, 8, 1, 128), (33, 70, 70, 16, 2, 64), (3, 130, 400, 160, 1, 64), (2, 9, 40, 300, 1, 128),
+                                                (70, 33, 33, 8, 8, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (65, 3)])
+def test_batches(gpu_device, batch, n, nk, hq, hkv, d, window, sinks):
+    """Row tiles kept whole and cut ones, several of a sequence and one, tokens that reach over row tiles; enough sequences that they are dealt
+    to the workgroups in more than one go."""
+    _run(gpu_device, batch, n, nk, hq, hkv, d, window, sinks, seed=batch)
+
+
+def test_many_short_sequences(gpu_device):
+    """4096 single tokens; 2048 sequences where there are more than one or large groups, no more."""
+    from shareprefill_amd import ops
+
+    _run(gpu_device, 2048, 2, 3, 2, 1, 64, 2, 0, seed=1)
+    _run(gpu_device, 4096, 1, 2, 2, 1, 64, 0, 0, seed=1)
+    make = lambda *shape: torch.zeros(*shape, dtype=torch.bfloat16, device=gpu_device)
+    for batch, n, hq in ((4097, 1, 2), (2049, 2, 2), (2049, 1, 17)):
+        with pytest.raises(RuntimeError, match="batch"):
+            ops.window_attention(make(batch, hq, n, 64), make(batch, 1, 2, 64), make(batch, 1, 2, 64), 0.1)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_values_out_of_sight_do_not_matter(gpu_device, bad):
     from shareprefill_amd import ops

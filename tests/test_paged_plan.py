@@ -25,6 +25,11 @@ int main() {
       printf("%ld %ld\\n", (long)pg_parts(a, b, 3), (long)pg_cut(a, pg_parts(a, b, 3), c));
     } else if (what == 'n') {
       printf("%d %d\\n", pg_snap(a, (int)b, 2, pg_near(c, d)), pg_near(c, d));
+    } else if (what == 'd') {
+      const long part = b;
+      int seq = -1, rt = -1;
+      const bool any = pg_deal((int)a, (int)part, (int)c, (int)d, (int)e, pg_together((int)e, (int)c, (int)d), &seq, &rt);
+      printf("%d %d %d\\n", any ? 1 : 0, seq, rt);
     } else {
       int p0, p1;
       pg_tile_positions((int)a, (int)b, (int)c, (int)d, (int)e, &p0, &p1);
@@ -128,3 +133,17 @@ def test_a_line_past_32_bits_is_cut_evenly(ask):
     total, parts = 2 ** 45 + 12345, 512
     cuts = [r[1] for r in ask([("c", total, parts, p) for p in range(parts + 1)])]
     assert cuts[-1] == total and all(abs((b - a) - total / parts) < 1.5 for a, b in zip(cuts, cuts[1:]))
+
+
+def test_whole_row_tiles_are_dealt_once_and_evenly(ask):
+    for workgroups, batch, tiles in ((1, 1, 1), (32, 1, 5), (32, 8, 16), (64, 3, 100), (256, 40, 7), (5, 11, 13), (32, 1, 128), (7, 2048, 1)):
+        turns = -(-batch * tiles // workgroups)
+        asked = [("d", t, p, workgroups, batch, tiles) for t in range(turns) for p in range(workgroups)]
+        answers = ask(asked)
+        dealt = [(b, rt) for there, b, rt in answers if there]
+        assert sorted(dealt) == [(b, rt) for b in range(batch) for rt in range(tiles)]
+        # all but the last turn give every workgroup one, and the tiles of a deal of sequences come longest first
+        assert all(there for there, _, _ in answers[:(turns - 1) * workgroups])
+        if batch == 1:
+            assert [max(rt for there, _, rt in answers[t * workgroups:(t + 1) * workgroups] if there) for t in range(turns)] == \
+                [tiles - 1 - t * workgroups for t in range(turns)]
