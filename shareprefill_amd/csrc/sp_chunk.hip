@@ -196,8 +196,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       }
     };
     int64_t mine = 0;
-    walk([&](int i, int units, int) {
+    int mine_blocks = 0;
+    walk([&](int i, int units, int blocks) {
       mine += units;
+      mine_blocks = blocks;
       if (units == 0 && part == 0 && a.by_slot != nullptr) a.by_slot[(int64_t)i * a.hkv + kvh].y = 0;  // (no row tile: nothing to merge)
     });
     int64_t at = mine;
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     at -= mine;
     const int64_t parts = pg_parts(total, a.parts, PG_MIN_SHARE);
     const int64_t cut[2] = {part < parts ? pg_cut(total, parts, part) : total, part < parts ? pg_cut(total, parts, part + 1) : total};
-    walk([&](int i, int units, int blocks) {
+    auto cuts = [&](int i, int units, int blocks) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (cut[e] >= at && cut[e] < at + units) {
@@ -227,7 +229,11 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           found[e][1] = tile < blocks ? tile : 0;
         }
       at += units;
-    });
+    };
+    if (per > 1)
+      walk(cuts);
+    else if (mine > 0)
+      cuts(x0, (int)mine, mine_blocks);
     __syncthreads();
     x = __builtin_amdgcn_readfirstlane(found[0][0]);
     tile_begin = __builtin_amdgcn_readfirstlane(found[0][1]);

@@ -44,11 +44,11 @@ PG_FN int64_t pg_first_slot(int64_t start, int g, int b, int tile) { return star
 PG_FN int64_t pg_slots(int64_t tokens, int g, int batch, int tile) { return tokens * g / tile + batch; }
 PG_FN int64_t pg_row_tiles(int64_t q_len, int g, int tile) { return (q_len * g + tile - 1) / tile; }
 
-// Positions of a row tile's first and last row: row r of a sequence is token r / g.
+// Positions of a row tile's first and last row: row r of a sequence, fewer than 2^31 of them, is token r / g.
 PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int tile, int* p0, int* p1) {
-  const int64_t r0 = (int64_t)rt * tile, rows = (int64_t)q_len * g, r1 = r0 + tile < rows ? r0 + tile : rows;
-  *p0 = len - q_len + (int)(r0 / g);
-  *p1 = len - q_len + (int)((r1 - 1) / g);
+  const unsigned rows = (unsigned)q_len * (unsigned)g, r0 = (unsigned)rt * (unsigned)tile, r1 = rows - r0 < (unsigned)tile ? rows : r0 + (unsigned)tile;
+  *p0 = len - q_len + (int)(r0 / (unsigned)g);
+  *p1 = len - q_len + (int)((r1 - 1u) / (unsigned)g);
 }
 
 // A launch cuts the line of all its row tiles' blocks, one line per kv head, into equal parts: part p of `parts` starts at unit
