@@ -36,8 +36,10 @@ __device__ __forceinline__ int ck_start(const CkArgs& a, int b) {
 __device__ __forceinline__ int ck_len(const CkArgs& a, int b) { return a.lens != nullptr ? pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS)) : a.n_keys; }
 
 // units of `unit` keys that positions p0 .. p1 see something of; none behind the table's last page
+template <bool WINDOWED = true>
 __device__ __forceinline__ PgSpan ck_span(const CkArgs& a, int p0, int p1, int unit) {
-  PgSpan s = pg_span(p0, p1, a.window, a.sinks, unit);
+  PgSpan s = {0, 0, p1 < 0 ? 0 : p1 / unit + 1};
+  if constexpr (WINDOWED) s = pg_span(p0, p1, a.window, a.sinks, unit);
   if (a.table != nullptr) {
     s.hi = pg_min(s.hi, ((a.width << a.shift) + unit - 1) / unit);
     s.lo = pg_min(s.lo, s.hi);

@@ -33,7 +33,7 @@
 #define CK_THREADS (CK_WAVES * SP_WAVE)
 #define CK_ROWS (32 * CK_WAVES)  // of a row tile
 #define CK_SUB 64                // keys of a sub-tile
-#define CK_BLOCK (2 * CK_SUB)    // keys of a block: what lies between two barriers
+#define CK_BLOCK (2 * CK_SUB)    // keys of a block, two sub-tiles of a walk: what lies between two barriers
 #define CK_RING 4                // sub-tiles of K in LDS, and of V
 #define CK_SUB_BYTES(D) (CK_SUB * (D) * 2)
 #define CK_LDS_BYTES(D) (2 * CK_RING * CK_SUB_BYTES(D))  // the rings; offsets and lengths of the sequences stand behind them
@@ -125,6 +125,9 @@ __device__ __forceinline__ void ck_pv_only(const Addr& ad, const bf16x8 (&p)[2],
   at_mfma_acc_settled(o[8][1], ones, p[1]);  // the end of the walk: the epilogue reads O next
 }
 
+// blocks of a walk of sub-tiles; the second one of the last block may lie behind them all
+__host__ __device__ static inline int ck_blocks(const PgSpan& s) { return (pg_span_units(s) + 1) >> 1; }
+
 // the sequence that row tile number x belongs to, by 64 candidates at a time
 template <int ROWS>
 __device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
@@ -141,7 +144,10 @@ __device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
   return lo;
 }
 
-template <int D, bool PAGED>
+// WINDOWED: blocks are made of any two sub-tiles of a walk, so that a window's start and the sinks cost a sub-tile, not a block: 8192 tokens in a
+// window of 1024 with 4 sinks 155 -> 151 us.  Without a window a block is 128 keys in a row, and nothing asks for windows: 2048 tokens over
+// 65001 keys 1800 -> 1772 us, chunks of 64 channels in a batch 138 -> 132.
+template <int D, bool PAGED, bool WINDOWED>
 __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a) {
   constexpr int WAVES = CK_WAVES, THREADS = CK_THREADS, TILE_ROWS = CK_ROWS;
   constexpr bool HALF = D == 64;
@@ -155,6 +161,14 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t lds_base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
   const int kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv;  // (workgroups of a kv head share an XCD where that works out)
+  // Arguments of what is done once a row tile or a page group are read where they are used: scalar registers do not suffice to keep them, and
+  // what the compiler sets aside for them passes through vector lanes in the loop.
+  const auto kernel_args = (const __attribute__((address_space(4))) CkArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  auto args = [&] {
+    auto p = kernel_args;
+    asm volatile("" : "+s"(p));
+    return p;
+  };
 
   // ---- which row tiles, and which blocks of the first and the last ----
   // On a line: row tiles x .. x_end, the first from block tile_begin on, of the last the blocks in front of tile_end.
@@ -191,7 +205,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         }
         int p0, p1;
         pg_tile_positions(rt, q_len, len_s[b], a.group, TILE_ROWS, &p0, &p1);
-        const int blocks = pg_span_units(ck_span(a, p0, p1, CK_BLOCK));
+        const int blocks = ck_blocks(ck_span<WINDOWED>(a, p0, p1, CK_SUB));
         visit(i, blocks + PG_OVERHEAD, blocks);
       }
     };
@@ -287,8 +301,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       }
       int p0, p1;
       pg_tile_positions(p.rt, p.q_len, p.len, a.group, TILE_ROWS, &p0, &p1);
-      p.span = ck_span(a, p0, p1, CK_BLOCK);
-      p.blocks = pg_span_units(p.span);
+      p.span = ck_span<WINDOWED>(a, p0, p1, CK_SUB);
+      p.blocks = ck_blocks(p.span);
       p.i0 = begin;
       p.i1 = end >= 0 ? pg_min(end, p.blocks) : p.blocks;
       return true;
@@ -317,11 +331,12 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   };
   bf16x8 qb[QT][4];
   auto load_q = [&](const Piece& c) {
+    const auto r = args();
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       int token, head;
       row_of(c, wave * 32 + 16 * qt + lq, &token, &head);
-      const sp_bf16* src = a.q + c.b * a.sq_b + (int64_t)((PAGED ? c.start : 0) + token) * a.sq_n + head * a.sq_h + 8 * g;
+      const sp_bf16* src = r->q + c.b * r->sq_b + (int64_t)((PAGED ? c.start : 0) + token) * r->sq_n + head * r->sq_h + 8 * g;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qb[qt][ks] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(src + 32 * ks));
     }
@@ -340,15 +355,17 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   auto entries = [&](int b, int group) {
     const int i = group * SP_WAVE + lane;
     if constexpr (!PAGED) return i;
-    const int id = a.table[b * a.table_stride + pg_min(i, a.width - 1)];
-    return i < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
+    const auto r = args();
+    const int id = r->table[b * r->table_stride + pg_min(i, r->width - 1)];
+    return i < r->width && (unsigned)id < (unsigned)r->num_pages ? id : -1;
   };
   auto turn_to = [&](int b, int len, int group, int id) {
     const int rows = id < 0 ? 0 : pg_max(0, pg_min(len - ((group * SP_WAVE + lane) << a.shift), 1 << a.shift));
     auto at = [&](const sp_bf16* x, int64_t stride_b, int64_t stride_page, int64_t stride_h) {
       return (uint64_t)(x + (PAGED ? 0 : b * stride_b) + kvh * stride_h) + (uint64_t)pg_max(id, 0) * (uint64_t)(stride_page * 2);
     };
-    const uint64_t k_at = at(a.k, a.sk_b, a.sk_p, a.sk_h), v_at = at(a.v, a.sv_b, a.sv_p, a.sv_h);
+    const auto r = args();
+    const uint64_t k_at = at(r->k, r->sk_b, r->sk_p, r->sk_h), v_at = at(r->v, r->sv_b, r->sv_p, r->sv_h);
     win.k_lo = (int)(uint32_t)k_at, win.k_hi = (int)(uint32_t)(k_at >> 32);
     win.v_lo = (int)(uint32_t)v_at, win.v_hi = (int)(uint32_t)(v_at >> 32);
     win.k_bytes = rows > 0 ? (int)((uint32_t)(rows - 1) * k_row + 2u * D) : 0;
@@ -356,16 +373,15 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     win.group = group;
     if constexpr (PAGED) win.lost = __ballot(id < 0);
   };
-  auto group_of = [&](int key) { return (key >> a.shift) >> 6; };  // (a block's pages lie in one group of 64)
-  // half hf of the block at key0 into slot `sub` % 4 of a ring; want false: zeros, without a read
-  auto load = [&](int key0, int hf, int sub, bool want, int lo, int hi, int bytes, uint32_t row_bytes, uint32_t lane_off, uint32_t to) {
+  auto group_of = [&](int key) { return (key >> a.shift) >> 6; };  // (a sub-tile's pages lie in one group of 64)
+  // the sub-tile at key `first` into slot `sub` % 4 of a ring; want false: zeros, without a read
+  auto load = [&](int first, int sub, bool want, int lo, int hi, int bytes, uint32_t row_bytes, uint32_t lane_off, uint32_t to) {
     to += (uint32_t)((sub & 3) * SUB_BYTES + wave * 1024);
     auto rsrc_of = [&](int key) {
       const int i = (key >> a.shift) & 63;
       const uint64_t at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(lo, i) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, i) << 32;
       return __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, want ? __builtin_amdgcn_readlane(bytes, i) : 0, 0x00027000);
     };
-    const int first = key0 + hf * CK_SUB;
     if (!PAGED || 1 << a.shift >= CK_SUB) {  // (uniform)
       const __amdgpu_buffer_rsrc_t rsrc = rsrc_of(first);
       const uint32_t off = lane_off + (PAGED ? (uint32_t)(first & ((1 << a.shift) - 1)) * row_bytes : 0u);
@@ -381,36 +397,36 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       }
     }
   };
-  auto load_k = [&](int key0, int hf, int sub, bool want) { load(key0, hf, sub, want, win.k_lo, win.k_hi, win.k_bytes, k_row, k_lane, lds_base); };
-  auto load_v = [&](int key0, int hf, int sub, bool want) {
-    load(key0, hf, sub, want, win.v_lo, win.v_hi, win.v_bytes, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
+  auto load_k = [&](int first, int sub, bool want) { load(first, sub, want, win.k_lo, win.k_hi, win.k_bytes, k_row, k_lane, lds_base); };
+  auto load_v = [&](int first, int sub, bool want) {
+    load(first, sub, want, win.v_lo, win.v_hi, win.v_bytes, v_row, v_lane, lds_base + CK_RING * SUB_BYTES);
   };
-  // A block of a walk: its first key, and which of its 16-key groups have no page (bits).
+  // A block of a walk: its sub-tiles' first keys, and which of its 16-key groups have no page (bits).
   struct Block {
-    int key0;
+    int key[2];
     uint32_t lost;
   };
-  auto block = [&](int key0) {
-    Block c = {key0, 0u};
+  auto lost_of = [&](int first) {  // of a sub-tile of the pages at hand
+    uint32_t lost = 0;
     if (PAGED && win.lost != 0ull) {  // (uniform)
 #pragma unroll
-      for (int i16 = 0; i16 < 8; ++i16) c.lost |= (uint32_t)((win.lost >> (((key0 + 16 * i16) >> a.shift) & 63)) & 1ull) << i16;
+      for (int i16 = 0; i16 < 4; ++i16) lost |= (uint32_t)((win.lost >> (((first + 16 * i16) >> a.shift) & 63)) & 1ull) << i16;
     }
-    return c;
+    return lost;
   };
-  auto key_of = [&](const Piece& p, int i) { return pg_span_unit(p.span, i) * CK_BLOCK; };
+  auto key_of = [&](const Piece& p, int i, int hf) { return (WINDOWED ? pg_span_unit(p.span, 2 * i + hf) : 2 * i + hf) * CK_SUB; };
 
   // Block n of the workgroup (over all its pieces) is sub-tiles 2 n and 2 n + 1; sub-tile s lives in slot s % 4 of either ring.  One wait and
   // barrier per block: while it is computed on (K of 2 n, 2 n + 1, V of 2 n - 1, 2 n: P . V trails by a sub-tile) K of 2 n + 2, 2 n + 3 and V of
-  // 2 n + 1, 2 n + 2 are on their way, sent out in four parts between the block's steps, V of 2 n + 1 first: the others are the next block's, whose
-  // pages may be others.  Behind a
-  // piece's last block that is the next piece's first one: its tiles land, and its queries, under the end of the piece in front.
+  // 2 n + 1, 2 n + 2 are on their way, sent out in four parts between the block's steps: V of 2 n + 1, then the next block's sub-tiles one after
+  // the other, each of which may lie in other pages than the one in front.  Behind a piece's last block that is the next piece's first one: its
+  // tiles land, and its queries, under the end of the piece in front.
   Piece cur_p, next_p;
   bool have = next_piece(cur_p), primed = false;
-  Block cur = {0, 0u}, nxt = {0, 0u};
-  int n = 0, ids_first = 0;
+  Block cur = {{0, 0}, 0u}, nxt = {{0, 0}, 0u};
+  int n = 0, ids_first = 0, ids_next = 0;  // table entries of the pages behind those at hand, if there is a block at hand
   if (have) load_q(cur_p);
-  if (have) ids_first = entries(cur_p.b, group_of(key_of(cur_p, cur_p.i0)));
+  if (have) ids_first = entries(cur_p.b, group_of(key_of(cur_p, cur_p.i0, 0)));
   while (have) {
     const Piece pc = cur_p;
     const bool have_next = next_piece(next_p);
@@ -429,9 +445,9 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       pos[qt] = len - q_len + token;
     }
     const bool next_blocks = have_next && next_p.i1 > next_p.i0;  // the next piece has a first block to fetch
-    int ids_next = 0, ids_here = ids_first;
-    if (n_blk > 0) ids_next = entries(b, group_of(key_of(pc, pc.i0)) + 1);
-    if (next_blocks) ids_first = entries(next_p.b, group_of(key_of(next_p, next_p.i0)));
+    const int ids_here = ids_first;
+    if (n_blk > 0 && !primed) ids_next = entries(b, group_of(key_of(pc, pc.i0, 0)) + 1);
+    if (next_blocks) ids_first = entries(next_p.b, group_of(key_of(next_p, next_p.i0, 0)));
 
     floatx4 o[9][2];  // [channel tile][row tile]; o[8]: the row sums (ones . P)
 #pragma unroll
@@ -441,17 +457,27 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     float m[QT] = {AT_NO_MAX, AT_NO_MAX}, l_mark[QT] = {0.f, 0.f};
     uint32_t det[2] = {0u, 0u};
 
+    // to the pages of a block's second sub-tile
+    auto turn_on = [&](int of_b, int of_len, Block& c) {
+      const int group = group_of(c.key[1]);
+      if (WINDOWED && group != win.group) {  // (uniform)
+        turn_to(of_b, of_len, group, group == win.group + 1 ? ids_next : entries(of_b, group));
+        ids_next = entries(of_b, group + 1);
+      }
+      c.lost |= lost_of(c.key[1]) << 4;
+    };
     if (n_blk > 0) {
       if (primed) {
         cur = nxt;
       } else {
         __syncthreads();  // the rings are free
-        const int key0 = key_of(pc, pc.i0);
-        turn_to(b, len, group_of(key0), ids_here);
-        cur = block(key0);
-        load_k(key0, 0, 2 * n, true);
-        load_k(key0, 1, 2 * n + 1, true);
-        load_v(key0, 0, 2 * n, true);
+        cur = {{key_of(pc, pc.i0, 0), key_of(pc, pc.i0, 1)}, 0u};
+        turn_to(b, len, group_of(cur.key[0]), ids_here);
+        cur.lost = lost_of(cur.key[0]);
+        load_k(cur.key[0], 2 * n, true);
+        load_v(cur.key[0], 2 * n, true);
+        turn_on(b, len, cur);
+        load_k(cur.key[1], 2 * n + 1, true);
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
       }
       const int n_last = n + n_blk - 1;
@@ -460,20 +486,23 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       auto top = [&](bool wait) {
         // everybody's loads have landed, everybody is past the block in front
         if (wait) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        load_v(cur.key0, 1, 2 * n + 1, true);
+        load_v(cur.key[1], 2 * n + 1, true);
         more = n < n_last || next_blocks;
         if (n < n_last) {
-          const int key0 = key_of(pc, pc.i1 - (n_last - n)), group = group_of(key0);
+          const int i = pc.i1 - (n_last - n);
+          nxt = {{key_of(pc, i, 0), key_of(pc, i, 1)}, 0u};
+          const int group = group_of(nxt.key[0]);
           if (group != win.group) {  // (uniform)
-            const bool following = group == win.group + 1;
-            turn_to(b, len, group, following ? ids_next : entries(b, group));
+            turn_to(b, len, group, group == win.group + 1 ? ids_next : entries(b, group));
             ids_next = entries(b, group + 1);
           }
-          nxt = block(key0);
+          nxt.lost = lost_of(nxt.key[0]);
         } else if (next_blocks) {
-          const int key0 = key_of(next_p, next_p.i0);
-          turn_to(next_p.b, next_p.len, group_of(key0), ids_first);
-          nxt = block(key0);
+          nxt = {{key_of(next_p, next_p.i0, 0), key_of(next_p, next_p.i0, 1)}, 0u};
+          const int group = group_of(nxt.key[0]);
+          turn_to(next_p.b, next_p.len, group, ids_first);
+          ids_next = entries(next_p.b, group + 1);
+          nxt.lost = lost_of(nxt.key[0]);
         }
         const uint32_t k_at = lds_base + (uint32_t)(((2 * n) & 3) * SUB_BYTES), v_at = lds_base + CK_RING * SUB_BYTES;
         ad.ka = k_at + koff;
@@ -481,24 +510,39 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         ad.va[1] = v_at + (uint32_t)(((2 * n) & 3) * SUB_BYTES) + voff;
       };
       auto feed = [&](int part) {
-        if (part == 0) load_k(nxt.key0, 0, 2 * n + 2, more);
-        if (part == 1) load_k(nxt.key0, 1, 2 * n + 3, more);
-        if (part == 2) load_v(nxt.key0, 0, 2 * n + 2, more);
+        if (part == 0) load_k(nxt.key[0], 2 * n + 2, more);
+        if (part == 1) load_v(nxt.key[0], 2 * n + 2, more);
+        if (part == 2) {
+          if (more) turn_on(n < n_last ? b : next_p.b, n < n_last ? len : next_p.len, nxt);
+          load_k(nxt.key[1], 2 * n + 3, more);
+        }
       };
       // what the wave's rows do not see of a block: nothing to take out in most of them
       auto partly = [&](const Block& c) {
-        const int key0 = c.key0, key1 = key0 + CK_BLOCK - 1;
-        return (key1 > w0 ? 1 : 0) | (key0 <= w1 - a.window && key1 >= a.sinks ? 2 : 0) | (c.lost != 0 ? 4 : 0);
+        bool some = c.lost != 0;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int key1 = c.key[hf] + CK_SUB - 1;
+          some |= key1 > w0 || (WINDOWED && c.key[hf] <= w1 - a.window && key1 >= a.sinks);
+        }
+        return some;
       };
+      // A half-tile of a block that holds unseen keys: none of its keys may be seen, or all, or some; most need one comparison a key or less.
       struct Mask {
-        int what;            // 1: keys behind rows, 2: keys in front of windows, 4: keys without a page
-        int key0, p0, p1, window, sinks;  // the half-tile's first key, positions of the lane's rows
-        uint32_t lost;
+        bool some;                                // the block holds unseen keys
+        int key0, w0, w1, p0, p1, window, sinks;  // the half-tile's first key, positions of the wave's first and last row and of the lane's rows
+        uint32_t lost;                            // halves of it without a page (bits)
         __device__ __forceinline__ void operator()(floatx4 (&s)[2][2]) const {
-          if (what == 0) return;
+          if (!some) return;
+          const floatx4 unseen = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          const int key1 = key0 + 31;
+          if (key0 > w1 || (WINDOWED && key1 <= w0 - window && key0 >= sinks) || (lost & 3u) == 3u) {
+            s[0][0] = s[0][1] = s[1][0] = s[1][1] = unseen;
+            return;
+          }
           const int key = key0 + 4 * ((threadIdx.x >> 4) & 3);
           const int h[2] = {p0 - key, p1 - key};
-          if (what & 1) {
+          if (key1 > w0) {
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -506,7 +550,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[kt][qt][j] = 16 * kt + j <= h[qt] ? s[kt][qt][j] : -INFINITY;
           }
-          if (what & 2) {
+          if (WINDOWED && key0 <= w1 - window && key1 >= sinks) {
             const int front = sinks - key, lo[2] = {h[0] - window, h[1] - window};
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
@@ -516,15 +560,13 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
                 for (int j = 0; j < 4; ++j)
                   s[kt][qt][j] = 16 * kt + j > lo[qt] || 16 * kt + j < front ? s[kt][qt][j] : -INFINITY;
           }
-          if (what & 4) {
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-              if ((lost >> kt) & 1u) s[kt][0] = s[kt][1] = (floatx4){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          }
+          for (int kt = 0; kt < 2; ++kt)
+            if ((lost >> kt) & 1u) s[kt][0] = s[kt][1] = unseen;
         }
       };
-      auto masked = [&](const Block& c, int what, int quarter) {
-        return Mask{what, c.key0 + 32 * quarter, pos[0], pos[1], a.window, a.sinks, c.lost >> (2 * quarter)};
+      auto masked = [&](const Block& c, bool some, int quarter) {
+        return Mask{some, c.key[quarter >> 1] + 32 * (quarter & 1), w0, w1, pos[0], pos[1], a.window, a.sinks, c.lost >> (2 * quarter)};
       };
       constexpr int MODE = (HALF ? 2 : 0) | (CK_SLACK << 4);
       if (!has_rows) {
@@ -542,7 +584,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         bf16x8 pa[2], pb[2];         // [row tile]
         bf16x8 pre[2];
         Block old = cur;
-        int some = partly(cur), some_old = some;
+        bool some = partly(cur), some_old = some;
         // ---- start: S of the first half-tile, nothing to overlap with yet ----
         top(false);
         feed(0);
@@ -586,10 +628,12 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     // ---- what has come of it: the rows, or a partial ----
     const bool whole = from_start && to_end;  // (uniform)
     const int64_t slab = (int64_t)blockIdx.x * 2 + (from_start ? 1 : 0);
-    float* const o_to = a.o_part + slab * (TILE_ROWS * D);
-    float2* const ml_to = a.ml_part + slab * TILE_ROWS;
-    if (from_start && a.by_slot != nullptr && t == 0)
-      a.by_slot[(int64_t)pc.slot * a.hkv + kvh] = make_int4(blockIdx.x, whole ? 0 : pg_min(rows, TILE_ROWS), 0, 0);
+    const auto dst_args = args();
+    float* const o_to = dst_args->o_part + slab * (TILE_ROWS * D);
+    float2* const ml_to = dst_args->ml_part + slab * TILE_ROWS;
+    sp_bf16* const out = dst_args->out;
+    if (from_start && dst_args->by_slot != nullptr && t == 0)
+      dst_args->by_slot[(int64_t)pc.slot * a.hkv + kvh] = make_int4(blockIdx.x, whole ? 0 : pg_min(rows, TILE_ROWS), 0, 0);
     if (!whole) {
       if (from_start)
         note.y = pg_min(rows, TILE_ROWS), note.z = rt * TILE_ROWS, note.w = start;
@@ -613,7 +657,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       if (whole) {
         const float inv_l = l[qt] > 0.f || l[qt] != l[qt] ? 1.0f / l[qt] : 0.f;
         // (lane groups 2i and 2i + 1 trade halves of two neighbouring channel tiles: 16 bytes a store, 64 contiguous ones a row)
-        sp_bf16* dst = a.out + ((int64_t)(start + token) * (a.hkv * a.group) + head) * D + 16 * (g & 1) + 8 * (g >> 1);
+        sp_bf16* dst = out + ((int64_t)(start + token) * (a.hkv * a.group) + head) * D + 16 * (g & 1) + 8 * (g >> 1);
 #pragma unroll
         for (int ct = 0; ct < CT; ct += 2) {
           uint32_t w[2][2];
@@ -645,21 +689,22 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         rows_left &= rows_left - 1ull;
         const int r = rt * TILE_ROWS + in_rows, token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
         const int p = len - q_len + token;
-        const sp_bf16* qrow = a.q + b * a.sq_b + (int64_t)((PAGED ? start : 0) + token) * a.sq_n + head * a.sq_h;
+        const auto c = args();
+        const sp_bf16* qrow = c->q + b * c->sq_b + (int64_t)((PAGED ? start : 0) + token) * c->sq_n + head * c->sq_h;
         constexpr int CL = D / SP_WAVE;  // channels of a lane
         float acc[CL] = {0.f}, sum = 0.f, top = CK_NO_MAX;
         for (int i = 2 * pc.i0; i < 2 * pc.i1; ++i) {
-          const int key = pg_span_unit(pc.span, i >> 1) * CK_BLOCK + (i & 1) * SP_WAVE + lane, page = key >> a.shift;
+          const int key = key_of(pc, 0, i) + lane, page = key >> a.shift;
           int id = page;
           if constexpr (PAGED) {
-            id = page < a.width ? a.table[b * a.table_stride + page] : -1;
-            if ((unsigned)id >= (unsigned)a.num_pages) id = -1;
+            id = page < c->width ? c->table[b * c->table_stride + page] : -1;
+            if ((unsigned)id >= (unsigned)c->num_pages) id = -1;
           }
           const bool seen = id >= 0 && key < len && pg_sees(p, key, a.window, a.sinks);
           const int64_t in = key & ((1 << a.shift) - 1);
           float logit = -INFINITY;
           if (seen) {
-            const sp_bf16* krow = a.k + b * a.sk_b + kvh * a.sk_h + id * a.sk_p + in * a.sk_n;
+            const sp_bf16* krow = c->k + b * c->sk_b + kvh * c->sk_h + id * c->sk_p + in * c->sk_n;
             float dot = 0.f;
             for (int c = 0; c < D; ++c) dot = __builtin_fmaf(sp_bf16_to_f32(qrow[c]), sp_bf16_to_f32(krow[c]), dot);
             logit = dot * a.scale_log2;
@@ -670,10 +715,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           top = new_top;
 #pragma unroll
           for (int c = 0; c < CL; ++c) acc[c] *= alpha;
-          const int64_t v_at = id < 0 ? 0 : id * a.sv_p + in * a.sv_n;
+          const int64_t v_at = id < 0 ? 0 : id * c->sv_p + in * c->sv_n;
           for (uint64_t left = __ballot(seen); left != 0ull; left &= left - 1ull) {
             const int j = __builtin_ctzll(left);
-            const sp_bf16* vrow_j = a.v + b * a.sv_b + kvh * a.sv_h + __shfl(v_at, j, SP_WAVE) + lane * CL;
+            const sp_bf16* vrow_j = c->v + b * c->sv_b + kvh * c->sv_h + __shfl(v_at, j, SP_WAVE) + lane * CL;
             const float w = __shfl(weight, j, SP_WAVE);
 #pragma unroll
             for (int c = 0; c < CL; ++c) acc[c] = __builtin_fmaf(w, sp_bf16_to_f32(vrow_j[c]), acc[c]);
@@ -682,7 +727,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
 #pragma unroll
         for (int c = 0; c < CL; ++c) {
           if (whole)
-            a.out[((int64_t)(start + token) * (a.hkv * a.group) + head) * D + lane * CL + c] = sp_f32_to_bf16(sum == 0.f ? 0.f : acc[c] / sum);
+            out[((int64_t)(start + token) * (a.hkv * a.group) + head) * D + lane * CL + c] = sp_f32_to_bf16(sum == 0.f ? 0.f : acc[c] / sum);
           else
             o_to[in_rows * D + lane * CL + c] = acc[c];
         }
@@ -692,7 +737,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     cur_p = next_p;
     have = have_next;
   }
-  if (a.parts != 0 && t == 0) a.notes[blockIdx.x] = note;
+  if (a.parts != 0 && t == 0) args()->notes[blockIdx.x] = note;
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
@@ -716,7 +761,7 @@ static bool ck_whole(const CkArgs& a, int wgs) {
       int b, rt, p0, p1;
       if (!pg_deal(turn, part, wgs, a.batch, a.tiles, a.together, &b, &rt)) continue;
       pg_tile_positions(rt, a.n_queries, a.n_keys, a.group, CK_ROWS, &p0, &p1);
-      const int n = pg_span_units(pg_span(p0, p1, a.window, a.sinks, CK_BLOCK)) + PG_OVERHEAD;
+      const int n = ck_blocks(pg_span(p0, p1, a.window, a.sinks, CK_SUB)) + PG_OVERHEAD;
       units[part] += n, total += n;
       if (units[part] > most) most = units[part];
     }
@@ -736,7 +781,10 @@ static int ck_check_launch(const char* who, const CkArgs& a, size_t need, const 
   return SP_OK;
 }
 
-static int ck_launch(const char* who, CkArgs& a, int32_t d, void* workspace, hipStream_t s) {
+// max_keys: no sequence has more
+static int ck_launch(const char* who, CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream_t s) {
+  const bool windowed = a.window < max_keys && a.sinks < max_keys;
+  if (!windowed) a.window = PG_NO_WINDOW;
   const bool uniform = a.cu == nullptr && a.lens == nullptr;  // as many queries and keys in every sequence
   const int wgs = ck_workgroups(a.hkv), grid = wgs * a.hkv;
   a.slots = (int)pg_slots(a.tokens, a.group, a.batch, CK_ROWS);
@@ -763,18 +811,22 @@ static int ck_launch(const char* who, CkArgs& a, int32_t d, void* workspace, hip
   SP_HIP(hipGetDevice(&dev));
   SP_REQUIRE(dev >= 0 && dev < 64, SP_ERR_UNSUPPORTED, "%s: device index %d", who, dev);
   if (!attr_set[dev]) {
-    const void* kernels[4] = {(const void*)sp_chunk_kernel<64, false>, (const void*)sp_chunk_kernel<64, true>,
-                              (const void*)sp_chunk_kernel<128, false>, (const void*)sp_chunk_kernel<128, true>};
+    const void* kernels[8] = {(const void*)sp_chunk_kernel<64, false, false>,  (const void*)sp_chunk_kernel<64, true, false>,
+                              (const void*)sp_chunk_kernel<128, false, false>, (const void*)sp_chunk_kernel<128, true, false>,
+                              (const void*)sp_chunk_kernel<64, false, true>,   (const void*)sp_chunk_kernel<64, true, true>,
+                              (const void*)sp_chunk_kernel<128, false, true>,  (const void*)sp_chunk_kernel<128, true, true>};
     for (const void* f : kernels)
       SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, CK_LDS_BYTES(128) + (2 * CK_MAX_SEQS + 1) * (int)sizeof(int)));
     attr_set[dev] = true;
   }
-  auto pick = [&](auto width) {
+  auto pick = [&](auto width, auto in_windows) {
     constexpr int D = decltype(width)::value;
+    constexpr bool WINDOWED = decltype(in_windows)::value;
     auto few = sp_chunk_merge_kernel<D, CK_ROWS, 16>, many = sp_chunk_merge_kernel<D, CK_ROWS, 64>;
-    a.table != nullptr ? go(sp_chunk_kernel<D, true>, few, many) : go(sp_chunk_kernel<D, false>, few, many);
+    a.table != nullptr ? go(sp_chunk_kernel<D, true, WINDOWED>, few, many) : go(sp_chunk_kernel<D, false, WINDOWED>, few, many);
   };
-  d == 64 ? pick(std::integral_constant<int, 64>{}) : pick(std::integral_constant<int, 128>{});
+  auto wide = [&](auto width) { windowed ? pick(width, std::true_type{}) : pick(width, std::false_type{}); };
+  d == 64 ? wide(std::integral_constant<int, 64>{}) : wide(std::integral_constant<int, 128>{});
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
@@ -839,7 +891,7 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   if (rc) return rc;
   const int64_t room = x->table_width << shift;
   if (pd_takes(a)) return pd_launch(a, room, (int)x->d, x->workspace, (hipStream_t)x->stream);
-  return ck_launch(who, a, (int)x->d, x->workspace, (hipStream_t)x->stream);
+  return ck_launch(who, a, room, (int)x->d, x->workspace, (hipStream_t)x->stream);
 }
 
 extern "C" size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d) {
@@ -877,5 +929,5 @@ extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
                        x->workspace, (size_t)x->workspace_bytes);
   if (rc) return rc;
   if (pd_takes(a)) return pd_launch(a, x->n_keys, (int)x->d, x->workspace, (hipStream_t)x->stream);
-  return ck_launch(who, a, (int)x->d, x->workspace, (hipStream_t)x->stream);
+  return ck_launch(who, a, x->n_keys, (int)x->d, x->workspace, (hipStream_t)x->stream);
 }

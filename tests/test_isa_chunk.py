@@ -8,7 +8,7 @@ from test_isa_operand_reads import _inline_reads_as_transposing
 
 def test_nothing_touches_a_read_in_flight_in_the_chunk_kernel():
     kernels = _kernels("sp_chunk.hip", "sp_chunk_kernel")
-    assert len(kernels) == 4, "64 / 128 channels x pages / contiguous"
+    assert len(kernels) == 8, "64 / 128 channels x pages / contiguous x windows / none"
     for name, body in kernels.items():
         for lines, least in ((_inline_reads_as_transposing(body), 8), (body, 16)):
             count, found = touched_in_flight(lines)
