@@ -17,9 +17,9 @@
 // (30001 tokens in a window of 4096 2282 -> 1811 us).  The row tiles' blocks form a line that is cut into equal parts, one workgroup each
 // (sp_paged_plan.h): every CU has as much to do as the others, whatever the sequences' lengths, which only the device knows; row tiles that a
 // cut goes through leave fp32 partials that a second launch merges.  No length comes to the host, so the call can be captured into a graph.
-// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1765 us, 1216 TFLOP/s, the rate of a large
-// bf16 matrix product on this card; 30001 tokens in a window of 4096 1175 TFLOP/s.  Short calls: some 10 us go by until the line is laid out
-// and the first keys have landed, a row tile's turn takes 5 us beside its blocks of 4 us each.
+// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1770 to 1830 us by card, 1170 to 1215 TFLOP/s, the
+// rate of a large bf16 matrix product; 30001 tokens in a window of 4096 1130 to 1175.  Short calls: some 8 us go by until the line is laid out
+// and the first keys have landed, a row tile's turn takes 5 us beside its blocks of 3.5 us each, partials and their merging 15 us.
 #include "sp_chunk.h"
 #include "sp_pipeline.h"
 
@@ -145,8 +145,8 @@ __device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
 }
 
 // WINDOWED: blocks are made of any two sub-tiles of a walk, so that a window's start and the sinks cost a sub-tile, not a block: 8192 tokens in a
-// window of 1024 with 4 sinks 155 -> 151 us.  Without a window a block is 128 keys in a row, and nothing asks for windows: 2048 tokens over
-// 65001 keys 1800 -> 1772 us, chunks of 64 channels in a batch 138 -> 132.
+// window of 1024 with 4 sinks 155 -> 151 us.  Without a window a block is 128 keys in a row, and nothing asks for windows: a mixed batch of 64
+// channels 138 -> 133 us.
 template <int D, bool PAGED, bool WINDOWED>
 __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a) {
   constexpr int WAVES = CK_WAVES, THREADS = CK_THREADS, TILE_ROWS = CK_ROWS;
