@@ -74,6 +74,40 @@ def test_single_tokens_of_long_caches(gpu_device):
     _run(gpu_device, [20011, 5, 9000], [1, 1, 1], 4, 1, 64, 64, 4096, 100, seed=4, singles=True)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 70), (1111, 3), (64, 2000), (100, 64)])
+@pytest.mark.parametrize("d,page", [(128, 16), (64, 32), (128, 64)])
+def test_long_chunks(gpu_device, window, sinks, d, page):
+    """Tables of more pages than a wave has lanes: walks that go from the sinks to a window far behind, begin and end anywhere, and pages
+    that are missing on either side.  K's pool token by token, V's head by head, the table a slice of a wider one."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(window + page)
+    hq, hkv, lens, q_lens = 4, 2, [5003, 2111, 40], [40, 61, 9]
+    kp, vp, table, kv = make_pages(lens, hkv, d, page, gen)
+    gone = [0, 66, lens[0] // page - 3]  # of the first sequence
+    seen = torch.ones(lens[0], dtype=torch.bool)
+    for i in gone:
+        table[0, i] = -1
+        seen[i * page:(i + 1) * page] = False
+    at = starts(q_lens)
+    q = torch.randn(at[-1], hq, d, generator=gen).to(torch.bfloat16).transpose(0, 1)
+    wide = torch.full((3, table.shape[1] + 5), 1, dtype=torch.int32, device=gpu_device)
+    wide[:, 2:-3] = table.to(gpu_device)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu_device)
+    args = [kp.to(gpu_device).transpose(1, 2).contiguous().transpose(1, 2), vp.to(gpu_device), wide[:, 2:-3], ints(lens), default_scale(d)]
+    got = ops.paged_attention(q.contiguous().to(gpu_device), *args, cu_q=ints(at), window=window or None, sinks=sinks).cpu()
+    ones = ops.paged_attention(q[:, [at[b + 1] - 1 for b in range(3)]].to(gpu_device), *args, window=window or None, sinks=sinks).cpu()
+    for b in range(3):
+        want, bound = reference(q[:, at[b]:at[b + 1]], *kv[b], default_scale(d), window, sinks, seen if b == 0 else None)
+        check(got[at[b]:at[b + 1]], want, bound, f"sequence {b}")
+        check(ones[b:b + 1], want[-1:], bound[-1:], f"last token of sequence {b}")
+
+
+def test_more_kv_heads_than_workgroups(gpu_device):
+    _run(gpu_device, [50, 33], [40, 1], 300, 300, 64, 16, 20, 3, seed=1)
+    _run(gpu_device, [50, 33], [1, 1], 300, 300, 64, 16, seed=2, singles=True)
+
+
 @pytest.mark.parametrize("batch", [63, 65, 300])
 def test_many_sequences(gpu_device, batch):
     gen = torch.Generator().manual_seed(batch)

@@ -115,6 +115,62 @@ def test_values_out_of_sight_do_not_matter(gpu_device, bad):
     check(one, want[-1:], bound[-1:])
 
 
+@pytest.mark.parametrize("n,nk", [(900, 900), (40, 3000), (1, 3000)])
+def test_a_captured_call_replays(gpu_device, n, nk):
+    """Whole row tiles, cut ones and single tokens: a replay gives the eager run's bits for whatever stands in its tensors."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(n)
+    make = lambda heads, length: torch.randn(2, length, heads, 128, generator=gen).to(torch.bfloat16).to(gpu_device).transpose(1, 2)
+    sets = [(make(8, n), make(2, nk), make(2, nk)) for _ in range(2)]
+    eager = [ops.window_attention(*s, 0.1, window=500, sinks=4) for s in sets]
+    live = [t.clone() for t in sets[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.window_attention(*live, 0.1, window=500, sinks=4)
+    for i in (0, 1, 1, 0):
+        for a, b in zip(live, sets[i]):
+            a.copy_(b)
+        out.zero_()
+        graph.replay()
+        assert torch.equal(ops.window_attention(*sets[1 - i], 0.1, window=500, sinks=4), eager[1 - i])
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[i])
+
+
+def test_keys_shared_by_a_batch(gpu_device):
+    """A batch stride of zero: samples that go on from one prompt."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(5)
+    q = torch.randn(3, 4, 70, 64, generator=gen).to(torch.bfloat16)
+    k, v = (torch.randn(1, 2, 200, 64, generator=gen).to(torch.bfloat16).expand(3, -1, -1, -1) for _ in range(2))
+    for queries in (q, q[:, :, -1:]):
+        got = ops.window_attention(queries.to(gpu_device), k[:1].to(gpu_device).expand(3, -1, -1, -1), v[:1].to(gpu_device).expand(3, -1, -1, -1),
+                                   0.1, window=90, sinks=2).cpu()
+        for b in range(3):
+            check(got[b], *reference(queries[b], k[b], v[b], 0.1, 90, 2))
+
+
+@pytest.mark.parametrize("window", [0, 70])
+def test_rows_that_are_no_numbers_stay_with_themselves(gpu_device, window):
+    """A query with a NaN, one whose logits overflow: their rows are NaN, the others the definition's."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(6)
+    n, hq, hkv, d = 300, 4, 2, 128
+    q, k, v = (torch.randn(h, n, d, generator=gen).to(torch.bfloat16) for h in (hq, hkv, hkv))
+    q[1, 77, 5] = float("nan")
+    q[2, 200] = float("inf")
+    got = ops.window_attention(*(t[None].to(gpu_device) for t in (q, k, v)), default_scale(d), window=window or None)[0].cpu()
+    want, bound = reference(q, k, v, default_scale(d), window, 0)
+    clean = torch.ones(n, hq, dtype=torch.bool)
+    clean[77, 1] = clean[200, 2] = False
+    check(got[clean], want[clean], bound[clean])
+    assert torch.isnan(got[~clean].float()).all()
+
+
 def test_a_window_as_long_as_the_prompt_is_none(gpu_device):
     from shareprefill_amd import ops
 
