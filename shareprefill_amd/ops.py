@@ -533,14 +533,10 @@ class PageTables(NamedTuple):
     free_left: torch.Tensor  # int32 [1]: pages left on the stack; below zero: so many were missing
 
 
-def _is_int(t: torch.Tensor, dtype, n: int, device) -> bool:
-    return t.dtype is dtype and t.device == device and t.dim() == 1 and t.shape[0] == n and (n == 1 or t.stride(0) == 1)
-
-
 def _check_ints(device, *named) -> None:
-    """(name, tensor, dtype, length) each; asked only where a call's own check says that something is amiss."""
+    """(name, tensor, dtype, length) each.  Asked only where a call's own, shorter check says that something is amiss."""
     for name, t, dtype, n in named:
-        if not _is_int(t, dtype, n, device):
+        if t.dtype is not dtype or t.device != device or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
@@ -562,33 +558,36 @@ def page_tables(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
     lib = _lib.load()
     if not lens.is_cuda:
         raise ValueError("lens must live on the GPU")
-    dev, batch = lens.device, lens.shape[0] if lens.dim() == 1 else -1
-    room = free_pages.numel()
-    i32 = torch.int32
-    if not (_is_int(lens, i32, batch, dev) and _is_int(new_lens, i32, batch, dev) and _is_int(free_pages, i32, room, dev)
-            and _is_int(free_count, i32, 1, dev)):
+    dev, batch, room, i32 = lens.device, lens.numel(), free_pages.numel(), torch.int32
+    if not (lens.dtype is new_lens.dtype is free_pages.dtype is free_count.dtype is block_table.dtype is i32
+            and lens.get_device() == new_lens.get_device() == free_pages.get_device() == free_count.get_device() == block_table.get_device()
+            and lens.dim() == new_lens.dim() == free_pages.dim() == free_count.dim() == 1 and new_lens.numel() == batch
+            and free_count.numel() == 1 and lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
+            and block_table.dim() == 2 and block_table.size(0) == batch and block_table.stride(1) == 1):
         _check_ints(dev, ("lens", lens, i32, batch), ("new_lens", new_lens, i32, batch), ("free_pages", free_pages, i32, room),
                     ("free_count", free_count, i32, 1))
-    _check_table(block_table, batch, dev)
+        _check_table(block_table, batch, dev)
     if max_new_tokens < 0:
         raise ValueError(f"max_new_tokens {max_new_tokens}")
     stream = _stream_handle(dev)
-    seq_lens, cu_new, free_left, positions = torch.empty(2 * batch + 2 + max_new_tokens, dtype=i32, device=dev).split_with_sizes(
-        [batch, batch + 1, 1, max_new_tokens])
+    seq_lens, cu_new, free_left, positions = torch.unsafe_split_with_sizes(
+        torch.empty(2 * batch + 2 + max_new_tokens, dtype=i32, device=dev), [batch, batch + 1, 1, max_new_tokens])
     slots = torch.empty(max_new_tokens, dtype=torch.int64, device=dev)
     st = lib.sp_paged_tables(_lib.PAGED_TABLES_ARGS.pack(
         lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), seq_lens.data_ptr(),
-        cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_left.data_ptr(), batch, page_size, num_pages, block_table.shape[1],
+        cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_left.data_ptr(), batch, page_size, num_pages, block_table.size(1),
         block_table.stride(0), room, max_new_tokens, stream))
     if st:
         _lib.check(st, "sp_paged_tables")
     return PageTables(seq_lens, cu_new, slots, positions, free_left)
 
 
-def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, d: int, device) -> None:
-    if (k_pages.dtype is v_pages.dtype is torch.bfloat16 and k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == d
-            and k_pages.stride(3) == v_pages.stride(3) == 1 and k_pages.device == device and v_pages.device == device):
-        return
+def _check_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, d: int, device):
+    """-> shape and strides of the pools"""
+    shape, k_at, v_at = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if (k_pages.dtype is v_pages.dtype is torch.bfloat16 and len(k_at) == 4 and shape == v_pages.shape and shape[3] == d
+            and k_at[3] == v_at[3] == 1 and k_pages.get_device() == v_pages.get_device() == device.index):
+        return shape, k_at, v_at
     for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         if t.dim() != 4:
             raise ValueError(f"{name} must be [num_pages, Hkv, page_size, D], got {tuple(t.shape)}")
@@ -609,19 +608,18 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v
     _check_hnd(k, "k")
     _check_hnd(v, "v")
     hkv, n, d = k.shape
-    if v.shape != k.shape or v.device != k.device:
+    if v.shape != k.shape or v.get_device() != k.get_device():
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must agree")
-    _check_pages(k_pages, v_pages, d, k.device)
-    pages, heads, page_size, _ = k_pages.shape
+    dev = k.device
+    (pages, heads, page_size, _), (kp_p, kp_h, kp_n, _), (vp_p, vp_h, vp_n, _) = _check_pages(k_pages, v_pages, d, dev)
     if heads != hkv:
         raise ValueError(f"the pools hold {heads} heads, k has {hkv}")
-    if not _is_int(slots, torch.int64, n, k.device):
-        _check_ints(k.device, ("slots", slots, torch.int64, n))
+    if not (slots.dtype is torch.int64 and slots.get_device() == dev.index and slots.dim() == 1 and slots.numel() == n and slots.is_contiguous()):
+        _check_ints(dev, ("slots", slots, torch.int64, n))
     (k_h, k_n, _), (v_h, v_n, _) = k.stride(), v.stride()
-    (kp_p, kp_h, kp_n, _), (vp_p, vp_h, vp_n, _) = k_pages.stride(), v_pages.stride()
     st = lib.sp_paged_cache_write_bf16(_lib.PAGED_WRITE_ARGS.pack(
         k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), n, hkv, d, pages, page_size, k_n, k_h, v_n, v_h,
-        kp_p, kp_n, kp_h, vp_p, vp_n, vp_h, _stream_handle(k.device)))
+        kp_p, kp_n, kp_h, vp_p, vp_n, vp_h, _stream_handle(dev)))
     if st:
         _lib.check(st, "sp_paged_cache_write_bf16")
 
@@ -650,15 +648,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _check_hnd(q, "q")
     hq, n, d = q.shape
     dev = q.device
-    _check_pages(k_pages, v_pages, d, dev)
-    pages, hkv, page_size, _ = k_pages.shape
-    batch = seq_lens.shape[0] if seq_lens.dim() == 1 else -1
-    if not _is_int(seq_lens, torch.int32, batch, dev):
-        _check_ints(dev, ("seq_lens", seq_lens, torch.int32, batch))
-    _check_table(block_table, batch, dev)
+    (pages, hkv, page_size, _), (k_p, k_h, k_n, _), (v_p, v_h, v_n, _) = _check_pages(k_pages, v_pages, d, dev)
+    batch, index, i32 = seq_lens.numel(), dev.index, torch.int32
+    if not (seq_lens.dtype is block_table.dtype is i32 and seq_lens.get_device() == block_table.get_device() == index and seq_lens.dim() == 1
+            and seq_lens.is_contiguous() and block_table.dim() == 2 and block_table.size(0) == batch and block_table.stride(1) == 1):
+        _check_ints(dev, ("seq_lens", seq_lens, i32, batch))
+        _check_table(block_table, batch, dev)
     if cu_q is not None:
-        if not _is_int(cu_q, torch.int32, batch + 1, dev):
-            _check_ints(dev, ("cu_q", cu_q, torch.int32, batch + 1))
+        if not (cu_q.dtype is i32 and cu_q.get_device() == index and cu_q.dim() == 1 and cu_q.numel() == batch + 1 and cu_q.is_contiguous()):
+            _check_ints(dev, ("cu_q", cu_q, i32, batch + 1))
     elif n != batch:
         raise ValueError(f"without cu_q every request has one row: q has {n}, seq_lens {batch}")
     span = _window_of(window, sinks)
@@ -670,10 +668,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     need = lib.sp_paged_attn_workspace_bytes(n, batch, hq, hkv, d, cu_q is None)
     # a buffer of this call's own: graphs captured on one stream may be replayed on two, so they must not meet in a kept one
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    (q_h, q_n, _), (k_p, k_h, k_n, _), (v_p, v_h, v_n, _) = q.stride(), k_pages.stride(), v_pages.stride()
+    q_h, q_n, _ = q.stride()
     st = lib.sp_paged_attn_bf16(_lib.PAGED_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
-        out.data_ptr(), 0 if ws is None else ws.data_ptr(), need, n, batch, hq, hkv, d, pages, page_size, block_table.shape[1],
+        out.data_ptr(), 0 if ws is None else ws.data_ptr(), need, n, batch, hq, hkv, d, pages, page_size, block_table.size(1),
         block_table.stride(0), span, sinks, q_n, q_h, k_p, k_n, k_h, v_p, v_n, v_h, softmax_scale, stream))
     if st:
         _lib.check(st, "sp_paged_attn_bf16")
