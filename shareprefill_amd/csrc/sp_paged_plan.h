@@ -54,7 +54,9 @@ PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int tile, int* p
 // A launch cuts the line of all its row tiles' blocks, one line per kv head, into equal parts: part p of `parts` starts at unit
 // total * p / parts.  A row tile counts its blocks and PG_OVERHEAD units for its queries, its first loads and its output; a cut near a row
 // tile's start or end goes there (pg_near).
-#define PG_OVERHEAD 2
+// (us, 1 / 2 / 3 / 4 units: 512 tokens over 8192 keys 88.6 / 88.3 / 86.5 / 86.7, 16 chunks of 200 over 1000 78.1 / 75.2 / 73.5 / 73.2, one of 900
+// beside three tokens over 4000 80.6 / 83.0 / 85.6 / 88.8, a mixed batch of 64 channels 133.1 / 132.7 / 132.6 / 135.3.)
+#define PG_OVERHEAD 3
 #define PG_MIN_SHARE 3  // units of a part at least
 // (Quotients of 64 bits take the device a hundred instructions each, and every workgroup forms them: lines that fit 31 bits do without.)
 #define PG_SHORT_LINE (1ll << 31)
