@@ -15,6 +15,8 @@ struct CkArgs {
   int64_t sq_b, sq_n, sq_h, sk_b, sk_p, sk_n, sk_h, sv_b, sv_p, sv_n, sv_h;  // elements; _b between sequences, _p between pages
   int batch, tokens, width, num_pages, shift, n_keys, n_queries;
   int hkv, group, window, sinks;
+  PgDivisor by_group;
+  int workgroups;           // of a kv head
   int slots, parts;         // row tile numbers per kv head; parts of their line at most, or 0: row tiles stay whole
   int tiles, together;      // whole ones (pg_deal): of a sequence, sequences dealt at a time
   float scale_log2;
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(CM_THREADS) void sp_chunk_merge_kernel(const CkArgs
     }
   }
   const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
-  const int r = note.z + row, kvh = (int)(w0 % a.hkv), token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
+  const int r = note.z + row, kvh = (int)(w0 % a.hkv), token = (int)pg_div((unsigned)r, a.by_group), head = kvh * a.group + (r - token * a.group);
   sp_bf16* dst = a.out + ((int64_t)(note.w + token) * (a.hkv * a.group) + head) * D + c0;
 #pragma unroll
   for (int c = 0; c < C4; ++c)

@@ -204,7 +204,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           continue;
         }
         int p0, p1;
-        pg_tile_positions(rt, q_len, len_s[b], a.group, TILE_ROWS, &p0, &p1);
+        pg_tile_positions(rt, q_len, len_s[b], a.by_group, TILE_ROWS, &p0, &p1);
         const int blocks = ck_blocks(ck_span<WINDOWED>(a, p0, p1, CK_SUB));
         visit(i, blocks + PG_OVERHEAD, blocks);
       }
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     for (;;) {
       int begin = 0, end = -1;
       if (a.parts == 0) {
-        const int wgs = (int)(gridDim.x / a.hkv);
+        const int wgs = args()->workgroups;
         if (turn * (int64_t)wgs >= (int64_t)a.tiles * a.batch) return false;
         int at_b, at_rt;
         if (!pg_deal(turn++, part, wgs, a.batch, a.tiles, a.together, &at_b, &at_rt)) continue;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         if (p.rt < 0 || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
       }
       int p0, p1;
-      pg_tile_positions(p.rt, p.q_len, p.len, a.group, TILE_ROWS, &p0, &p1);
+      pg_tile_positions(p.rt, p.q_len, p.len, a.by_group, TILE_ROWS, &p0, &p1);
       p.span = ck_span<WINDOWED>(a, p0, p1, CK_SUB);
       p.blocks = ck_blocks(p.span);
       p.i0 = begin;
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   // row of the lane's tile qt in a piece: token and head
   auto row_of = [&](const Piece& c, int in_rows, int* token, int* head) {
     const int r = c.rt * TILE_ROWS + pg_min(in_rows, c.q_len * a.group - c.rt * TILE_ROWS - 1);
-    *token = (int)((unsigned)r / (unsigned)a.group);
+    *token = (int)pg_div((unsigned)r, a.by_group);
     *head = kvh * a.group + (r - *token * a.group);
   };
   bf16x8 qb[QT][4];
@@ -435,8 +435,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     const bool from_start = pc.i0 == 0, to_end = pc.i1 == pc.blocks;  // (uniform)
     const bool has_rows = wave * 32 < rows;  // (uniform in the wave)
     // positions of the wave's first and last row
-    const int w0 = len - q_len + (int)((unsigned)(rt * TILE_ROWS + pg_min(wave * 32, rows - 1)) / (unsigned)a.group);
-    const int w1 = len - q_len + (int)((unsigned)(rt * TILE_ROWS + pg_min(wave * 32 + 31, rows - 1)) / (unsigned)a.group);
+    const int w0 = len - q_len + (int)pg_div((unsigned)(rt * TILE_ROWS + pg_min(wave * 32, rows - 1)), a.by_group);
+    const int w1 = len - q_len + (int)pg_div((unsigned)(rt * TILE_ROWS + pg_min(wave * 32 + 31, rows - 1)), a.by_group);
     int pos[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
@@ -687,7 +687,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       while (rows_left != 0ull) {
         const int in_rows = wave * 32 + 16 * qt + __builtin_ctzll(rows_left);
         rows_left &= rows_left - 1ull;
-        const int r = rt * TILE_ROWS + in_rows, token = (int)((unsigned)r / (unsigned)a.group), head = kvh * a.group + (r - token * a.group);
+        const int r = rt * TILE_ROWS + in_rows, token = (int)pg_div((unsigned)r, a.by_group), head = kvh * a.group + (r - token * a.group);
         const int p = len - q_len + token;
         const auto c = args();
         const sp_bf16* qrow = c->q + b * c->sq_b + (int64_t)((PAGED ? start : 0) + token) * c->sq_n + head * c->sq_h;
@@ -760,7 +760,7 @@ static bool ck_whole(const CkArgs& a, int wgs) {
     for (int part = 0; part < wgs; ++part) {
       int b, rt, p0, p1;
       if (!pg_deal(turn, part, wgs, a.batch, a.tiles, a.together, &b, &rt)) continue;
-      pg_tile_positions(rt, a.n_queries, a.n_keys, a.group, CK_ROWS, &p0, &p1);
+      pg_tile_positions(rt, a.n_queries, a.n_keys, a.by_group, CK_ROWS, &p0, &p1);
       const int n = ck_blocks(pg_span(p0, p1, a.window, a.sinks, CK_SUB)) + PG_OVERHEAD;
       units[part] += n, total += n;
       if (units[part] > most) most = units[part];
@@ -787,6 +787,8 @@ static int ck_launch(const char* who, CkArgs& a, int64_t max_keys, int32_t d, vo
   if (!windowed) a.window = PG_NO_WINDOW;
   const bool uniform = a.cu == nullptr && a.lens == nullptr;  // as many queries and keys in every sequence
   const int wgs = ck_workgroups(a.hkv), grid = wgs * a.hkv;
+  a.workgroups = wgs;
+  a.by_group = pg_divisor((unsigned)a.group);
   a.slots = (int)pg_slots(a.tokens, a.group, a.batch, CK_ROWS);
   a.tiles = uniform ? (int)pg_row_tiles(a.n_queries, a.group, CK_ROWS) : 0;
   a.together = uniform ? pg_together(a.tiles, wgs, a.batch) : 0;

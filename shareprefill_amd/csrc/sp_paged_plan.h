@@ -44,11 +44,25 @@ PG_FN int64_t pg_first_slot(int64_t start, int g, int b, int tile) { return star
 PG_FN int64_t pg_slots(int64_t tokens, int g, int batch, int tile) { return tokens * g / tile + batch; }
 PG_FN int64_t pg_row_tiles(int64_t q_len, int g, int tile) { return (q_len * g + tile - 1) / tile; }
 
+// Quotients by a launch's one divisor: the division takes a wave some 35 instructions, and a row tile needs a dozen.  With 2^l the power of two
+// at or above the divisor, x * ceil(2^(31 + l) / by) / 2^(31 + l) has the quotient for x below 2^31: the multiplier is too large by less than
+// one part in 2^31.
+struct PgDivisor {
+  unsigned by, mul, shift;
+};
+PG_FN PgDivisor pg_divisor(unsigned by) {  // 1 <= by < 2^31
+  PgDivisor d = {by, 0u, 0u};
+  while ((1u << d.shift) < by) ++d.shift;
+  d.mul = (unsigned)((((uint64_t)1 << (31 + d.shift)) + by - 1) / by);
+  return d;
+}
+PG_FN unsigned pg_div(unsigned x, const PgDivisor& d) { return (unsigned)((uint64_t)(x << 1) * d.mul >> 32) >> d.shift; }
+
 // Positions of a row tile's first and last row: row r of a sequence, fewer than 2^31 of them, is token r / g.
-PG_FN void pg_tile_positions(int rt, int q_len, int len, int g, int tile, int* p0, int* p1) {
-  const unsigned rows = (unsigned)q_len * (unsigned)g, r0 = (unsigned)rt * (unsigned)tile, r1 = rows - r0 < (unsigned)tile ? rows : r0 + (unsigned)tile;
-  *p0 = len - q_len + (int)(r0 / (unsigned)g);
-  *p1 = len - q_len + (int)((r1 - 1u) / (unsigned)g);
+PG_FN void pg_tile_positions(int rt, int q_len, int len, const PgDivisor& g, int tile, int* p0, int* p1) {
+  const unsigned rows = (unsigned)q_len * g.by, r0 = (unsigned)rt * (unsigned)tile, r1 = rows - r0 < (unsigned)tile ? rows : r0 + (unsigned)tile;
+  *p0 = len - q_len + (int)pg_div(r0, g);
+  *p1 = len - q_len + (int)pg_div(r1 - 1u, g);
 }
 
 // A launch cuts the line of all its row tiles' blocks, one line per kv head, into equal parts: part p of `parts` starts at unit
@@ -91,6 +105,11 @@ PG_FN int pg_together(int tiles, int workgroups, int batch) { return pg_min(pg_m
 PG_FN bool pg_deal(int turn, int part, int workgroups, int batch, int tiles, int together, int* b, int* rt) {
   const int place = turn * workgroups + (turn & 1 ? workgroups - 1 - part : part);
   if (place >= tiles * batch) return false;
+  if (batch == 1) {
+    *b = 0;
+    *rt = tiles - 1 - place;
+    return true;
+  }
   const int deal = place / (together * tiles), at = place - deal * (together * tiles), n = pg_min(together, batch - deal * together);
   *rt = tiles - 1 - at / n;
   *b = deal * together + at % n;

@@ -25,6 +25,8 @@ int main() {
       printf("%ld %ld\\n", (long)pg_parts(a, b, 3), (long)pg_cut(a, pg_parts(a, b, 3), c));
     } else if (what == 'n') {
       printf("%d %d\\n", pg_snap(a, (int)b, 2, pg_near(c, d)), pg_near(c, d));
+    } else if (what == 'q') {
+      printf("%u\\n", pg_div((unsigned)a, pg_divisor((unsigned)b)));
     } else if (what == 'd') {
       const long part = b;
       int seq = -1, rt = -1;
@@ -32,7 +34,7 @@ int main() {
       printf("%d %d %d\\n", any ? 1 : 0, seq, rt);
     } else {
       int p0, p1;
-      pg_tile_positions((int)a, (int)b, (int)c, (int)d, (int)e, &p0, &p1);
+      pg_tile_positions((int)a, (int)b, (int)c, pg_divisor((unsigned)d), (int)e, &p0, &p1);
       printf("%d %d\\n", p0, p1);
     }
   }
@@ -147,3 +149,12 @@ def test_whole_row_tiles_are_dealt_once_and_evenly(ask):
         if batch == 1:
             assert [max(rt for there, _, rt in answers[t * workgroups:(t + 1) * workgroups] if there) for t in range(turns)] == \
                 [tiles - 1 - t * workgroups for t in range(turns)]
+
+
+def test_quotients_by_a_multiplier(ask):
+    rng = random.Random(3)
+    top = 2 ** 31 - 1
+    pairs = [(x, by) for by in list(range(1, 70)) + [127, 128, 129, 1000, 65535, 65536, 65537, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 1, top]
+             for x in (0, 1, by - 1, by, by + 1, top, top - 1, top // by * by, top // by * by - 1, rng.randrange(top)) if 0 <= x <= top]
+    pairs += [(rng.randrange(2 ** rng.randrange(1, 32)), rng.randrange(1, 2 ** rng.randrange(1, 31) + 1)) for _ in range(20000)]
+    assert [x for x, in ask([("q", x, by) for x, by in pairs])] == [x // by for x, by in pairs]
