@@ -20,43 +20,46 @@ struct TablesArgs {
 //   have = min(ceil(len / P), W), need = min(ceil((len + new) / P), W) - have;
 // the pages of all requests in order come off the top of the stack, token t of the step belongs to the request whose prefix sum of `new`
 // it lies behind.  Latency is all there is to it (some 130 KB for 256 requests): one launch, and every workgroup forms the two prefix sums over the
-// requests for itself, which costs less than a launch that hands them over.  A new token's slot is taken from the stack itself, not from the
-// table's entry, so nothing that another workgroup of the launch writes is read.
+// requests for itself, which costs less than a launch that hands them over.  Sums hold at 2^30 instead of growing past it, which keeps them
+// 32 bits wide and any order of adding the same; what the requests bring is read once and kept in LDS, the stack's height is asked for first.
+// A new token's slot is taken from the stack itself, not from the table's entry, so nothing that another workgroup of the launch writes is read.
 __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs a) {
-  extern __shared__ int sh[];  // prefix sums over the requests: [batch + 1] tokens, [batch + 1] pages
-  __shared__ int64_t wave_sums[2][PT_THREADS / SP_WAVE];
+  extern __shared__ int sh[];  // of the requests: tokens [batch + 1] and pages [batch + 1], then their prefix sums; lengths [batch]
+  __shared__ int wave_sums[2][PT_THREADS / SP_WAVE];
   int* const tok = sh;
-  int* const pgs = sh + a.batch + 1;
+  int* const pgs = tok + a.batch + 1;
+  int* const len_of = pgs + a.batch + 1;
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, P = 1 << a.shift;
+  const int count = pg_max(0, pg_min(a.free_count[0], a.free_room));
   const int per = (a.batch + PT_THREADS - 1) / PT_THREADS;
   auto length = [](int x) { return pg_max(0, pg_min(x, PG_MAX_KEYS - 1)); };
-  auto pages = [&](int n) { return pg_min((int)(((int64_t)n + P - 1) >> a.shift), a.width); };
-  int64_t tokens = 0, opened = 0;
+  auto pages = [&](int n) { return pg_min((int)(((unsigned)n + (unsigned)P - 1u) >> a.shift), a.width); };
+  auto add = [](int x, int y) { return pg_min(x + y, PG_MAX_KEYS); };  // (of two sums up to 2^30; below 2^31)
+  int tokens = 0, opened = 0;
   for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
-    const int len = length(a.lens[i]), n = length(a.new_lens[i]);
-    tokens += n;
-    opened += pages(len + n) - pages(len);
+    const int len = length(a.lens[i]), n = length(a.new_lens[i]), p = pages(len + n) - pages(len);
+    len_of[i] = len, tok[i] = n, pgs[i] = p;
+    tokens = add(tokens, n), opened = add(opened, p);
   }
-  int64_t tok_at = tokens, page_at = opened;  // inclusive sums over the wave's lanes
+  int tok_at = tokens, page_at = opened;  // inclusive sums over the wave's lanes, then what lies in front of the thread
 #pragma unroll
   for (int o = 1; o < SP_WAVE; o <<= 1) {
-    const int64_t x = __shfl_up(tok_at, o, SP_WAVE), y = __shfl_up(page_at, o, SP_WAVE);
-    if (lane >= o) tok_at += x, page_at += y;
+    const int x = __shfl_up(tok_at, o, SP_WAVE), y = __shfl_up(page_at, o, SP_WAVE);
+    if (lane >= o) tok_at = add(tok_at, x), page_at = add(page_at, y);
   }
   if (lane == SP_WAVE - 1) wave_sums[0][wave] = tok_at, wave_sums[1][wave] = page_at;
+  tok_at = __shfl_up(tok_at, 1, SP_WAVE), page_at = __shfl_up(page_at, 1, SP_WAVE);
+  if (lane == 0) tok_at = page_at = 0;
   __syncthreads();
-  tok_at -= tokens, page_at -= opened;
-  for (int w = 0; w < wave; ++w) tok_at += wave_sums[0][w], page_at += wave_sums[1][w];
-  auto capped = [](int64_t x) { return (int)(x < PG_MAX_KEYS ? x : PG_MAX_KEYS); };
+  for (int w = 0; w < wave; ++w) tok_at = add(tok_at, wave_sums[0][w]), page_at = add(page_at, wave_sums[1][w]);
   for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
-    const int len = length(a.lens[i]), n = length(a.new_lens[i]);
-    tok[i] = capped(tok_at), pgs[i] = capped(page_at);
-    if (blockIdx.x == 0) a.seq_lens[i] = len + n;
-    tok_at += n, page_at += pages(len + n) - pages(len);
+    const int n = tok[i], p = pgs[i];
+    tok[i] = tok_at, pgs[i] = page_at;
+    if (blockIdx.x == 0) a.seq_lens[i] = len_of[i] + n;
+    tok_at = add(tok_at, n), page_at = add(page_at, p);
   }
-  if (t == PT_THREADS - 1) tok[a.batch] = capped(tok_at), pgs[a.batch] = capped(page_at);
+  if (t == PT_THREADS - 1) tok[a.batch] = tok_at, pgs[a.batch] = page_at;
   __syncthreads();
-  const int count = pg_max(0, pg_min(a.free_count[0], a.free_room));
   if (blockIdx.x == 0) {
     for (int i = t; i <= a.batch; i += PT_THREADS) a.cu_new[i] = tok[i];
     if (t == 0) a.free_left[0] = count - pgs[a.batch];  // (below zero: as many pages were missing)
@@ -79,13 +82,13 @@ __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs 
   const int gid = blockIdx.x * PT_THREADS + t;
   for (int i = gid; i < pgs[a.batch]; i += gridDim.x * PT_THREADS) {  // (as many as tokens at most, unless those are capped)
     const int b = request(pgs, i);
-    a.table[b * a.table_stride + pages(length(a.lens[b])) + (i - pgs[b])] = from_stack(i);
+    a.table[b * a.table_stride + pages(len_of[b]) + (i - pgs[b])] = from_stack(i);
   }
   if (gid >= a.max_tokens) return;
   int64_t slot = -1;
   int pos = 0;
   if (gid < tok[a.batch]) {
-    const int b = request(tok, gid), len = length(a.lens[b]);
+    const int b = request(tok, gid), len = len_of[b];
     pos = len + (gid - tok[b]);
     const int page = pos >> a.shift, have = pages(len);
     if (page < a.width) {
@@ -128,14 +131,14 @@ extern "C" int sp_paged_tables(const sp_paged_tables_args* x) {
                         (int)x->table_width, (int)x->num_pages, (int)x->free_room, (int)x->max_tokens, x->seq_lens, x->cu_new, x->slots,
                         x->positions, x->free_left};
   const unsigned grid = x->max_tokens > 0 ? (unsigned)sp_ceil_div(x->max_tokens, PT_THREADS) : 1u;
-  hipLaunchKernelGGL(sp_paged_tables_kernel, dim3(grid), dim3(PT_THREADS), 2 * (x->batch + 1) * sizeof(int), (hipStream_t)x->stream, a);
+  hipLaunchKernelGGL(sp_paged_tables_kernel, dim3(grid), dim3(PT_THREADS), (3 * x->batch + 2) * sizeof(int), (hipStream_t)x->stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
 
 // ---- new keys and values into their pages ---------------------------------------------------------------------------------
 #define PW_THREADS 256
-#define PW_ITEMS 4
+#define PW_MAX_ITEMS (1ll << 30)  // of a launch: items and their numbers past the end stay below 2^31
 
 typedef uint32_t pw_u32x4 __attribute__((ext_vector_type(4)));
 
@@ -143,39 +146,30 @@ struct WriteArgs {
   const sp_bf16 *k, *v;
   sp_bf16 *k_pages, *v_pages;
   const int64_t* slots;
-  int64_t items, room;  // 16-byte chunks of k; tokens of the pool
-  int hkv, chunks, shift;
+  int64_t room;               // tokens of the pool
+  int items, shift;           // 16-byte chunks of k, below 2^31
+  PgDivisor chunks, hkv;      // of a row, rows of a token
   int64_t k_n, k_h, v_n, v_h;
   int64_t kp_p, kp_n, kp_h, vp_p, vp_n, vp_h;
 };
 
-// pages[slot / P][h][slot % P] = x[t][h] for k and v: a copy, HBM-bound.  A thread moves PW_ITEMS chunks of 16 bytes of either, all loads
-// in front of the first store; the chunks of a token's heads lie side by side over the lanes, as projections leave them.
+// pages[slot / P][h][slot % P] = x[t][h] for k and v: a copy, HBM-bound.  A thread moves 16 bytes of either; the chunks of a token's heads
+// lie side by side over the lanes, as projections leave them.  us for 16384 tokens of 8 heads of 128 channels, 4 / 2 / 1 chunks a thread 29.8 /
+// 28.5 / 27.4 (4.9 TB/s), for 8 tokens 3.1 / 2.2 / 1.9 (quotients of 64 bits: 3.9).  Stores past the caches would take 25.6 alone, but attention
+// reads the pages next: of both together 4096 tokens 169 / 170.5, 16384 the same.
 __global__ __launch_bounds__(PW_THREADS) void sp_paged_write_kernel(WriteArgs a) {
-  const int64_t first = (int64_t)blockIdx.x * (PW_THREADS * PW_ITEMS) + threadIdx.x;
-  pw_u32x4 kx[PW_ITEMS], vx[PW_ITEMS];
-  sp_bf16 *kd[PW_ITEMS], *vd[PW_ITEMS];
-#pragma unroll
-  for (int i = 0; i < PW_ITEMS; ++i) {
-    const int64_t item = first + i * PW_THREADS;
-    kd[i] = vd[i] = nullptr;
-    if (item >= a.items) continue;
-    const int64_t row = item / a.chunks, t = row / a.hkv;  // (token, head)
-    const int c = (int)(item - row * a.chunks) * 8, h = (int)(row - t * a.hkv);
-    const int64_t slot = a.slots[t];
-    if (slot < 0 || slot >= a.room) continue;
-    const int64_t page = slot >> a.shift, in = slot & ((1 << a.shift) - 1);
-    kx[i] = *reinterpret_cast<const pw_u32x4*>(a.k + t * a.k_n + h * a.k_h + c);
-    vx[i] = *reinterpret_cast<const pw_u32x4*>(a.v + t * a.v_n + h * a.v_h + c);
-    kd[i] = a.k_pages + page * a.kp_p + in * a.kp_n + h * a.kp_h + c;
-    vd[i] = a.v_pages + page * a.vp_p + in * a.vp_n + h * a.vp_h + c;
-  }
-#pragma unroll
-  for (int i = 0; i < PW_ITEMS; ++i)
-    if (kd[i] != nullptr) {
-      *reinterpret_cast<pw_u32x4*>(kd[i]) = kx[i];
-      *reinterpret_cast<pw_u32x4*>(vd[i]) = vx[i];
-    }
+  const unsigned item = blockIdx.x * PW_THREADS + threadIdx.x;
+  if (item >= (unsigned)a.items) return;
+  const unsigned row = pg_div(item, a.chunks);
+  const int64_t t = pg_div(row, a.hkv);  // (token, head)
+  const int c = (int)(item - row * a.chunks.by) * 8, h = (int)(row - (unsigned)t * a.hkv.by);
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= a.room) return;
+  const int64_t page = slot >> a.shift, in = slot & ((1 << a.shift) - 1);
+  const pw_u32x4 kx = *reinterpret_cast<const pw_u32x4*>(a.k + t * a.k_n + h * a.k_h + c);
+  const pw_u32x4 vx = *reinterpret_cast<const pw_u32x4*>(a.v + t * a.v_n + h * a.v_h + c);
+  *reinterpret_cast<pw_u32x4*>(a.k_pages + page * a.kp_p + in * a.kp_n + h * a.kp_h + c) = kx;
+  *reinterpret_cast<pw_u32x4*>(a.v_pages + page * a.vp_p + in * a.vp_n + h * a.vp_h + c) = vx;
 }
 
 extern "C" int sp_paged_cache_write_bf16(const sp_paged_write_args* x) {
@@ -194,12 +188,16 @@ extern "C" int sp_paged_cache_write_bf16(const sp_paged_write_args* x) {
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
   SP_REQUIRE(x->tokens <= (1ll << 40) && x->hkv <= 65536 && x->num_pages <= 0x7fffffffll, SP_ERR_UNSUPPORTED,
              "%s: tokens=%lld hkv=%lld num_pages=%lld too many", who, (long long)x->tokens, (long long)x->hkv, (long long)x->num_pages);
-  const int64_t items = x->tokens * x->hkv * (x->d / 8), grid = sp_ceil_div(items, PW_THREADS * PW_ITEMS);
-  SP_REQUIRE(grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: tokens=%lld too many", who, (long long)x->tokens);
-  const WriteArgs a = {(const sp_bf16*)x->k, (const sp_bf16*)x->v, (sp_bf16*)x->k_pages, (sp_bf16*)x->v_pages, x->slots, items, x->num_pages << shift,
-                       (int)x->hkv, (int)(x->d / 8), shift, x->k_stride_n, x->k_stride_h, x->v_stride_n, x->v_stride_h, x->k_stride_page,
-                       x->k_stride_slot, x->k_stride_page_h, x->v_stride_page, x->v_stride_slot, x->v_stride_page_h};
-  hipLaunchKernelGGL(sp_paged_write_kernel, dim3((unsigned)grid), dim3(PW_THREADS), 0, (hipStream_t)x->stream, a);
+  const int64_t of_token = x->hkv * (x->d / 8), most = PW_MAX_ITEMS / of_token;
+  SP_REQUIRE(most > 0, SP_ERR_UNSUPPORTED, "%s: hkv=%lld head_dim=%lld too large", who, (long long)x->hkv, (long long)x->d);
+  for (int64_t t = 0; t < x->tokens; t += most) {
+    const int items = (int)((x->tokens - t < most ? x->tokens - t : most) * of_token);
+    const WriteArgs a = {(const sp_bf16*)x->k + t * x->k_stride_n, (const sp_bf16*)x->v + t * x->v_stride_n, (sp_bf16*)x->k_pages, (sp_bf16*)x->v_pages,
+                         x->slots + t, x->num_pages << shift, items, shift, pg_divisor((unsigned)(x->d / 8)), pg_divisor((unsigned)x->hkv),
+                         x->k_stride_n, x->k_stride_h, x->v_stride_n, x->v_stride_h, x->k_stride_page, x->k_stride_slot, x->k_stride_page_h,
+                         x->v_stride_page, x->v_stride_slot, x->v_stride_page_h};
+    hipLaunchKernelGGL(sp_paged_write_kernel, dim3((unsigned)sp_ceil_div(items, PW_THREADS)), dim3(PW_THREADS), 0, (hipStream_t)x->stream, a);
+  }
   SP_LAUNCH_CHECK();
   return SP_OK;
 }

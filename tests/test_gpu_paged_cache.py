@@ -117,6 +117,24 @@ def test_write_puts_every_token_in_its_slot(gpu_device, hkv, d, page, tokens, to
         assert torch.equal(got.cpu(), pool)
 
 
+def test_a_write_of_more_than_one_launch(gpu_device):
+    """2100 tokens of 64 heads x 65536 channels are more 16-byte pieces than a launch takes; one token's memory stands for all of them, and
+    all but a few have no slot."""
+    from shareprefill_amd import ops
+
+    hkv, d, tokens = 64, 65536, 2100
+    gen = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(hkv, 1, d, generator=gen).to(torch.bfloat16).to(gpu_device) for _ in range(2))
+    pools = [torch.zeros(1, hkv, 16, d, dtype=torch.bfloat16, device=gpu_device) for _ in range(2)]
+    slots = torch.full((tokens,), -1, dtype=torch.int64)
+    for t, slot in ((0, 3), (2047, 4), (2048, 9), (2099, 15)):
+        slots[t] = slot
+    ops.paged_cache_write(k.expand(-1, tokens, -1), v.expand(-1, tokens, -1), *pools, slots.to(gpu_device))
+    for pool, x in zip(pools, (k, v)):
+        for i in range(16):
+            assert torch.equal(pool[0, :, i], x[:, 0] if i in (3, 4, 9, 15) else torch.zeros_like(x[:, 0])), i
+
+
 def test_write_of_nothing_and_refusals(gpu_device):
     from shareprefill_amd import ops
 
