@@ -25,10 +25,10 @@
 
 // Octaves that a moved maximum is set above the largest logit.  A wave that moves its rows' maxima (some probability came out at 2) forms them
 // again and rescales its sums while the other seven wait at the block's barrier, and in a row's first thousand keys some wave does in nearly
-// every block.  us, 0 / 1 / 2 / 3 octaves: 8192 tokens in a window of 1024 188 / 172 / 165 / 161, 30001 in 4096 1833 / 1740 / 1688 / 1660, 512 over
-// 8192 104 / 98 / 95 / 93, 2048 over 65001 1850 in all.  What it costs: the largest probability need not be a power of two, which bf16 holds
-// exactly; outputs are 2.14e-3 / 2.18e-3 / 2.21e-3 / 2.22e-3 from 64 bits, 1.6e-3 of it their own rounding.
-#define CK_SLACK 3
+// every block.  us, 0 / 3 / 5 / 7 octaves: 8192 tokens in a window of 1024 178 / 151.5 / 148.2 / 147.1, 30001 in 4096 1850 / 1663 / 1657 / 1654, 512
+// over 8192 94.5 / 84.9 / 84.1 / 84.2, 16384 without a window - / 1796 / 1778 / 1777.  What it costs: the largest probability need not be a power of
+// two, which bf16 holds exactly; outputs are 2.14e-3 / 2.22e-3 / 2.23e-3 / 2.23e-3 from 64 bits, 1.6e-3 of it their own rounding.
+#define CK_SLACK 7
 #define CK_WAVES 8
 #define CK_THREADS (CK_WAVES * SP_WAVE)
 #define CK_ROWS (32 * CK_WAVES)  // of a row tile

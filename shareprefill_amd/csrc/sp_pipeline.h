@@ -296,14 +296,14 @@ __device__ __forceinline__ float at_groupmax(float mx) {
 // s_prev = S(j-1) (causal predicate applied), p = P(j-1), det = OR of its packed words.  On return p is safe to use.
 // PIVOT: l_mark (the row sums at the start of the current key block, see the block sums of pivot heads in the
 // kernel) follows every rescale.
-// MODE: bit 0 = PIVOT, bit 1 = HALF (see at_fused), bit 2 = FINE (sp_attn.hip), bits 4, 5 = SLACK: octaves that a moved max is set above the
+// MODE: bit 0 = PIVOT, bit 1 = HALF (see at_fused), bit 2 = FINE (sp_attn.hip), bits 4 .. 6 = SLACK: octaves that a moved max is set above the
 // largest logit
 template <int MODE>
 __device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 (&p)[2], uint32_t (&det)[2],
                                           floatx4 (&o)[9][2], float scale_log2, float (&m_run)[2],
                                           float (&l_mark)[2]) {
   constexpr bool PIVOT = (MODE & 1) != 0, HALF = (MODE & 2) != 0;
-  constexpr int SLACK = (MODE >> 4) & 3;
+  constexpr int SLACK = (MODE >> 4) & 7;
   if (__builtin_amdgcn_ballot_w64(((det[0] | det[1]) & AT_P_TOO_LARGE) != 0u) != 0ull) {
     float mx[2];  // (S(j-1) is a whole stage old: no wait states needed before reading it)
     at_lanemax(s_prev, mx);
