@@ -17,8 +17,8 @@
 // (30001 tokens in a window of 4096 2282 -> 1811 us).  The row tiles' blocks form a line that is cut into equal parts, one workgroup each
 // (sp_paged_plan.h): every CU has as much to do as the others, whatever the sequences' lengths, which only the device knows; row tiles that a
 // cut goes through leave fp32 partials that a second launch merges.  No length comes to the host, so the call can be captured into a graph.
-// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1770 to 1830 us by card, 1170 to 1215 TFLOP/s, the
-// rate of a large bf16 matrix product; 30001 tokens in a window of 4096 1130 to 1175.  Short calls: some 8 us go by until the line is laid out
+// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1760 to 1820 us by card, 1180 to 1220 TFLOP/s, the
+// rate of a large bf16 matrix product; 30001 tokens in a window of 4096 1150 to 1200.  Short calls: some 8 us go by until the line is laid out
 // and the first keys have landed, a row tile's turn takes 5 us beside its blocks of 3.5 us each, partials and their merging 15 us.
 #include "sp_chunk.h"
 #include "sp_pipeline.h"
@@ -751,8 +751,8 @@ static size_t ck_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int3
 
 // Whether row tiles of a call whose sequences have as many rows and keys each stay whole: the longest workgroup against even parts, which take
 // a sixteenth longer a block (their row tiles' keys lie further apart) and a merging launch, eight blocks' time.  us, whole / cut, 32 heads
-// over 8: 2 tokens 9.7 / 13.6, prompts of 2048 59 / 64, 4096 126 / 150, in a window of 1024 75 / 84, 16384 1735 / 1850, 8 of 1024 88 / 98; cut
-// because whole ones are uneven: 64 tokens over 16384, two row tiles a head, 42.
+// over 8: 2 tokens 8.3 / 11.9, prompts of 2048 59 / 67, 4096 127 / 155, in a window of 1024 77 / 88, 16384 1803 / 1899, 8 of 1024 88 / 97; cut
+// because whole ones leave most of the card idle: 64 tokens over 16384, a row tile a head, 41.
 static bool ck_whole(const CkArgs& a, int wgs) {
   if ((int64_t)a.tiles * a.batch >= 4 * wgs) return true;
   int64_t units[CK_PLACES] = {0}, most = 0, total = 0;
