@@ -20,8 +20,8 @@ struct TablesArgs {
 //   have = min(ceil(len / P), W), need = min(ceil((len + new) / P), W) - have;
 // the pages of all requests in order come off the top of the stack, token t of the step belongs to the request whose prefix sum of `new`
 // it lies behind.  Latency is all there is to it (some 130 KB for 256 requests): one launch, and every workgroup forms the two prefix sums over the
-// requests for itself, which costs less than a launch that hands them over.  Sums hold at 2^30 instead of growing past it, which keeps them
-// 32 bits wide and any order of adding the same; what the requests bring is read once and kept in LDS, the stack's height is asked for first.
+// requests for itself, which costs less than a launch that hands them over.  Sums hold at 2^30 (pg_held_sum); what the requests bring is
+// read once and kept in LDS, the stack's height is asked for first.
 // A new token's slot is taken from the stack itself, not from the table's entry, so nothing that another workgroup of the launch writes is read.
 __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs a) {
   extern __shared__ int sh[];  // of the requests: tokens [batch + 1] and pages [batch + 1], then their prefix sums; lengths [batch]
@@ -32,31 +32,29 @@ __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs 
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, P = 1 << a.shift;
   const int count = pg_max(0, pg_min(a.free_count[0], a.free_room));
   const int per = (a.batch + PT_THREADS - 1) / PT_THREADS;
-  auto length = [](int x) { return pg_max(0, pg_min(x, PG_MAX_KEYS - 1)); };
   auto pages = [&](int n) { return pg_min((int)(((unsigned)n + (unsigned)P - 1u) >> a.shift), a.width); };
-  auto add = [](int x, int y) { return pg_min(x + y, PG_MAX_KEYS); };  // (of two sums up to 2^30; below 2^31)
   int tokens = 0, opened = 0;
   for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
-    const int len = length(a.lens[i]), n = length(a.new_lens[i]), p = pages(len + n) - pages(len);
+    const int len = pg_length(a.lens[i]), n = pg_length(a.new_lens[i]), p = pages(len + n) - pages(len);
     len_of[i] = len, tok[i] = n, pgs[i] = p;
-    tokens = add(tokens, n), opened = add(opened, p);
+    tokens = pg_held_sum(tokens, n), opened = pg_held_sum(opened, p);
   }
   int tok_at = tokens, page_at = opened;  // inclusive sums over the wave's lanes, then what lies in front of the thread
 #pragma unroll
   for (int o = 1; o < SP_WAVE; o <<= 1) {
     const int x = __shfl_up(tok_at, o, SP_WAVE), y = __shfl_up(page_at, o, SP_WAVE);
-    if (lane >= o) tok_at = add(tok_at, x), page_at = add(page_at, y);
+    if (lane >= o) tok_at = pg_held_sum(tok_at, x), page_at = pg_held_sum(page_at, y);
   }
   if (lane == SP_WAVE - 1) wave_sums[0][wave] = tok_at, wave_sums[1][wave] = page_at;
   tok_at = __shfl_up(tok_at, 1, SP_WAVE), page_at = __shfl_up(page_at, 1, SP_WAVE);
   if (lane == 0) tok_at = page_at = 0;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) tok_at = add(tok_at, wave_sums[0][w]), page_at = add(page_at, wave_sums[1][w]);
+  for (int w = 0; w < wave; ++w) tok_at = pg_held_sum(tok_at, wave_sums[0][w]), page_at = pg_held_sum(page_at, wave_sums[1][w]);
   for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
     const int n = tok[i], p = pgs[i];
     tok[i] = tok_at, pgs[i] = page_at;
     if (blockIdx.x == 0) a.seq_lens[i] = len_of[i] + n;
-    tok_at = add(tok_at, n), page_at = add(page_at, p);
+    tok_at = pg_held_sum(tok_at, n), page_at = pg_held_sum(page_at, p);
   }
   if (t == PT_THREADS - 1) tok[a.batch] = tok_at, pgs[a.batch] = page_at;
   __syncthreads();
@@ -68,27 +66,16 @@ __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs 
     const int id = i < count ? a.free_pages[count - 1 - i] : -1;
     return (unsigned)id < (unsigned)a.num_pages ? id : -1;
   };
-  auto request = [&](const int* sums, int x) {  // the last request that starts at or in front of x
-    int lo = 0, hi = a.batch;                   // sums[lo] <= x < sums[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (sums[mid] <= x)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    return lo;
-  };
   const int gid = blockIdx.x * PT_THREADS + t;
   for (int i = gid; i < pgs[a.batch]; i += gridDim.x * PT_THREADS) {  // (as many as tokens at most, unless those are capped)
-    const int b = request(pgs, i);
+    const int b = pg_holder(pgs, a.batch, i);
     a.table[b * a.table_stride + pages(len_of[b]) + (i - pgs[b])] = from_stack(i);
   }
   if (gid >= a.max_tokens) return;
   int64_t slot = -1;
   int pos = 0;
   if (gid < tok[a.batch]) {
-    const int b = request(tok, gid), len = len_of[b];
+    const int b = pg_holder(tok, a.batch, gid), len = len_of[b];
     pos = len + (gid - tok[b]);
     const int page = pos >> a.shift, have = pages(len);
     if (page < a.width) {

@@ -18,6 +18,25 @@
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
 PG_FN int pg_max(int a, int b) { return a > b ? a : b; }
 
+// Lengths as the device finds them, and sums of them that hold at 2^30 instead of growing past it: 32 bits wide, sorted, and the same whatever the
+// order of adding.  (Two sums at 2^30 make 2^31, which only unsigned numbers hold.)
+PG_FN int pg_length(int n) { return pg_max(0, pg_min(n, PG_MAX_KEYS - 1)); }
+PG_FN int pg_held_sum(int x, int y) {
+  const unsigned sum = (unsigned)x + (unsigned)y;
+  return sum < (unsigned)PG_MAX_KEYS ? (int)sum : PG_MAX_KEYS;
+}
+PG_FN int pg_holder(const int* sums, int n, int x) {  // the last of n entries that starts at or in front of x: sums[i] <= x < sums[i + 1]
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
 // The query at position p sees key j: causal, inside its window or among the first `sinks`.
 PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j <= p && (j > p - window || j < sinks); }
 
