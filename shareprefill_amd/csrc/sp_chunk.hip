@@ -781,9 +781,10 @@ static int ck_check_launch(const char* who, const CkArgs& a, size_t need, const 
   return SP_OK;
 }
 
-// max_keys: no sequence has more
+// max_keys: no sequence has more that exist.  Behind a table it may be longer, by the lengths that the device holds: its rows' windows lie that much
+// further on, and a window as wide as the table leaves keys out.
 static int ck_launch(const char* who, CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream_t s) {
-  const bool windowed = a.window < max_keys && a.sinks < max_keys;
+  const bool windowed = a.window < (a.table != nullptr ? PG_NO_WINDOW : max_keys) && a.sinks < max_keys;
   if (!windowed) a.window = PG_NO_WINDOW;
   const bool uniform = a.cu == nullptr && a.lens == nullptr;  // as many queries and keys in every sequence
   const int wgs = ck_workgroups(a.hkv), grid = wgs * a.hkv;
