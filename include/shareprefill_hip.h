@@ -385,7 +385,8 @@ int sp_paged_cache_write_bf16(const sp_paged_write_args* args /* host */);
  * sequence b has rows cu_q[b] .. cu_q[b + 1] (null: one row each, tokens == batch) and seq_lens[b] keys; its query i stands at position
  * p = seq_lens[b] - its rows + i and sees the keys j <= p with j > p - window or j < sinks (window 0: all j <= p).  Keys without a page
  * are not seen; a query that sees nothing gives zeros.  out: bf16 [tokens][hq][d] contiguous; rows outside every sequence stay as they
- * were.  Device values out of range (lengths, offsets, pages) are held to what the arguments allow.  head_dim 64 or 128.
+ * were.  Device values out of range (lengths, offsets, pages) are held to what the arguments allow; an offset that goes back counts as the
+ * largest in front of it.  head_dim 64 or 128.
  * The workspace is 16-byte aligned and the call's own until it has run; out shares no memory with q. */
 typedef struct sp_paged_attn_args {
   const void *q, *k_pages, *v_pages;

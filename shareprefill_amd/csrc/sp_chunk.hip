@@ -128,14 +128,14 @@ __device__ __forceinline__ void ck_pv_only(const Addr& ad, const bf16x8 (&p)[2],
 // blocks of a walk of sub-tiles; the second one of the last block may lie behind them all
 __host__ __device__ static inline int ck_blocks(const PgSpan& s) { return (pg_span_units(s) + 1) >> 1; }
 
-// the sequence that row tile number x belongs to, by 64 candidates at a time
+// the sequence that row tile number x belongs to, by 64 candidates at a time.  cu: offsets in order
 template <int ROWS>
-__device__ __forceinline__ int ck_sequence(const CkArgs& a, int x, int lane) {
+__device__ __forceinline__ int ck_sequence(const CkArgs& a, const int* cu, int x, int lane) {
   int lo = 0, span = a.batch;  // it is one of lo .. lo + span - 1
   while (span > 1) {
     const int step = (span + SP_WAVE - 1) / SP_WAVE;
     const int b = lo + lane * step;
-    const bool at_or_behind = lane * step < span && pg_first_slot(ck_start(a, b), a.group, b, ROWS) <= x;
+    const bool at_or_behind = lane * step < span && pg_first_slot(cu[b], a.group, b, ROWS) <= x;
     const int n = __builtin_popcountll(__ballot(at_or_behind));
     const int at = pg_max(n - 1, 0) * step;
     span = pg_min(step, span - at);
@@ -173,17 +173,25 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
   // ---- which row tiles, and which blocks of the first and the last ----
   // On a line: row tiles x .. x_end, the first from block tile_begin on, of the last the blocks in front of tile_end.
   int x = 0, x_end = 0, tile_begin = 0, tile_end = 0, turn = 0;
+  int* const cu_s = reinterpret_cast<int*>(lds + CK_LDS_BYTES(D));
   const uint32_t lds_cu = lds_base + CK_LDS_BYTES(D), lds_len = lds_cu + 4u * (uint32_t)(a.batch + 1);
   if (a.parts != 0) {
-    int* const cu_s = reinterpret_cast<int*>(lds + CK_LDS_BYTES(D));
     int* const len_s = cu_s + a.batch + 1;
     __shared__ int64_t wave_sums[WAVES];
     __shared__ int found[2][2];
+    int back = 0;
     for (int i = t; i <= a.batch; i += THREADS) {
-      cu_s[i] = ck_start(a, i);
-      if (i < a.batch) len_s[i] = ck_len(a, i);
+      const int start = ck_start(a, i);
+      cu_s[i] = start;
+      if (i < a.batch) len_s[i] = ck_len(a, i), back |= ck_start(a, i + 1) < start;
     }
-    __syncthreads();
+    // Searches need the offsets in order, and must all find the same: notes of row tiles that only some of them find stay unwritten, and the
+    // merging launch would read where they happen to point.  An offset that goes back counts as the largest in front of it.
+    if (__syncthreads_or(back)) {
+      if (t == 0)
+        for (int i = 1; i <= a.batch; ++i) cu_s[i] = pg_max(cu_s[i], cu_s[i - 1]);
+      __syncthreads();
+    }
     // every thread some row tiles in a row: their units, then the line's prefix sums
     const int per = (a.slots + THREADS - 1) / THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
     auto walk = [&](auto&& visit) {  // visit(x, units in the line, 0: no row tile has the number, blocks)
@@ -268,7 +276,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     return __builtin_amdgcn_readfirstlane(v);
   };
   auto start_of = [&](int b) { return a.cu != nullptr ? from_lds(lds_cu + 4u * b) : b * a.n_queries; };
-  int seq = a.parts == 0 || x >= a.slots ? 0 : __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, x, lane));
+  int seq = a.parts == 0 || x >= a.slots ? 0 : __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, cu_s, x, lane));
   auto next_piece = [&](Piece& p) {  // false: there is none
     for (;;) {
       int begin = 0, end = -1;
