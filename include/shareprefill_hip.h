@@ -367,6 +367,9 @@ typedef struct sp_paged_tables_args {
   sp_stream_t stream;
 } sp_paged_tables_args;
 int sp_paged_tables(const sp_paged_tables_args* args /* host */);
+/* The same for a step that has max_tokens rows and no more: new tokens from max_tokens on are left out, as if new_lens had ended there.  They open no
+ * page and count neither in seq_lens nor in cu_new, whose last entry is at most max_tokens. */
+int sp_paged_tables_truncated(const sp_paged_tables_args* args /* host */);
 
 /* k, v: bf16 [tokens][hkv][d] (token and head strides) copied to slots[t] of the pools; a slot outside the pool is skipped.  Slots
  * must differ from each other: where two tokens name the same one, its contents are parts of either.  d a multiple of 8. */

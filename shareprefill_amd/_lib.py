@@ -99,6 +99,7 @@ SIGNATURES = {
     "sp_decode_attn_batch_args_bf16": (_I32, [C.c_char_p]),  # (DECODE_BATCH_ARGS.pack(...))
     "sp_decode_attn_static_bf16": (_I32, [_P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _F, _P, _P]),
     "sp_paged_tables": (_I32, [C.c_char_p]),  # (PAGED_TABLES_ARGS.pack(...), and so on)
+    "sp_paged_tables_truncated": (_I32, [C.c_char_p]),
     "sp_paged_cache_write_bf16": (_I32, [C.c_char_p]),
     "sp_paged_attn_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32]),
     "sp_paged_attn_bf16": (_I32, [C.c_char_p]),

@@ -23,6 +23,9 @@ struct TablesArgs {
 // requests for itself, which costs less than a launch that hands them over.  Sums hold at 2^30 (pg_held_sum); what the requests bring is
 // read once and kept in LDS, the stack's height is asked for first.
 // A new token's slot is taken from the stack itself, not from the table's entry, so nothing that another workgroup of the launch writes is read.
+// TRUNCATE: tokens from max_tokens on are none.  What a request keeps of `new` follows from the prefix sums, which are formed first then: offsets
+// held at max_tokens, and their differences.
+template <bool TRUNCATE>
 __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs a) {
   extern __shared__ int sh[];  // of the requests: tokens [batch + 1] and pages [batch + 1], then their prefix sums; lengths [batch]
   __shared__ int wave_sums[2][PT_THREADS / SP_WAVE];
@@ -33,9 +36,30 @@ __global__ __launch_bounds__(PT_THREADS) void sp_paged_tables_kernel(TablesArgs 
   const int count = pg_max(0, pg_min(a.free_count[0], a.free_room));
   const int per = (a.batch + PT_THREADS - 1) / PT_THREADS;
   auto pages = [&](int n) { return pg_min((int)(((unsigned)n + (unsigned)P - 1u) >> a.shift), a.width); };
+  if constexpr (TRUNCATE) {
+    int sum = 0;
+    for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) tok[i] = pg_length(a.new_lens[i]), sum = pg_held_sum(sum, tok[i]);
+    int at = sum;
+#pragma unroll
+    for (int o = 1; o < SP_WAVE; o <<= 1) {
+      const int x = __shfl_up(at, o, SP_WAVE);
+      if (lane >= o) at = pg_held_sum(at, x);
+    }
+    if (lane == SP_WAVE - 1) wave_sums[0][wave] = at;
+    at = __shfl_up(at, 1, SP_WAVE);
+    if (lane == 0) at = 0;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) at = pg_held_sum(at, wave_sums[0][w]);
+    for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
+      const int end = pg_held_sum(at, tok[i]);
+      tok[i] = pg_min(end, a.max_tokens) - pg_min(at, a.max_tokens);
+      at = end;
+    }
+    __syncthreads();  // the waves' sums are free
+  }
   int tokens = 0, opened = 0;
   for (int i = t * per; i < (t + 1) * per && i < a.batch; ++i) {
-    const int len = pg_length(a.lens[i]), n = pg_length(a.new_lens[i]), p = pages(len + n) - pages(len);
+    const int len = pg_length(a.lens[i]), n = TRUNCATE ? tok[i] : pg_length(a.new_lens[i]), p = pages(len + n) - pages(len);
     len_of[i] = len, tok[i] = n, pgs[i] = p;
     tokens = pg_held_sum(tokens, n), opened = pg_held_sum(opened, p);
   }
@@ -93,8 +117,7 @@ static int page_shift(int64_t page_size) {  // -1: not a page size
   return -1;
 }
 
-extern "C" int sp_paged_tables(const sp_paged_tables_args* x) {
-  const char* who = "sp_paged_tables";
+static int tables_launch(const char* who, const sp_paged_tables_args* x, bool truncate) {
   SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   SP_REQUIRE(x->batch > 0 && x->table_width > 0 && x->num_pages >= 0 && x->free_room >= 0 && x->max_tokens >= 0, SP_ERR_INVALID_ARGUMENT,
              "%s: batch=%lld table_width=%lld num_pages=%lld free_room=%lld max_tokens=%lld", who, (long long)x->batch, (long long)x->table_width,
@@ -118,10 +141,14 @@ extern "C" int sp_paged_tables(const sp_paged_tables_args* x) {
                         (int)x->table_width, (int)x->num_pages, (int)x->free_room, (int)x->max_tokens, x->seq_lens, x->cu_new, x->slots,
                         x->positions, x->free_left};
   const unsigned grid = x->max_tokens > 0 ? (unsigned)sp_ceil_div(x->max_tokens, PT_THREADS) : 1u;
-  hipLaunchKernelGGL(sp_paged_tables_kernel, dim3(grid), dim3(PT_THREADS), (3 * x->batch + 2) * sizeof(int), (hipStream_t)x->stream, a);
+  hipLaunchKernelGGL(truncate ? sp_paged_tables_kernel<true> : sp_paged_tables_kernel<false>, dim3(grid), dim3(PT_THREADS),
+                     (3 * x->batch + 2) * sizeof(int), (hipStream_t)x->stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
+
+extern "C" int sp_paged_tables(const sp_paged_tables_args* x) { return tables_launch("sp_paged_tables", x, false); }
+extern "C" int sp_paged_tables_truncated(const sp_paged_tables_args* x) { return tables_launch("sp_paged_tables_truncated", x, true); }
 
 // ---- new keys and values into their pages ---------------------------------------------------------------------------------
 #define PW_THREADS 256

@@ -547,12 +547,13 @@ def _check_table(block_table: torch.Tensor, batch: int, device) -> None:
 
 
 def page_tables(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
-                free_count: torch.Tensor, page_size: int, num_pages: int, max_new_tokens: int) -> PageTables:
+                free_count: torch.Tensor, page_size: int, num_pages: int, max_new_tokens: int, truncate: bool = False) -> PageTables:
     """The bookkeeping of a serving step over a key / value cache in pages, on the GPU: request b has lens[b] tokens cached and
     new_lens[b] to come (int32 [B] each).  The pages that the new tokens open come off the top of the stack
     free_pages[:free_count] (int32 [F], int32 [1]; free_count stays as it is, free_left is what it becomes), in the order of the requests,
     and are entered into block_table int32 [B, W] in place (-1 where the stack is empty).  max_new_tokens: length of slots and positions;
-    places behind the last new token hold -1 and 0, new tokens beyond it none.
+    places behind the last new token hold -1 and 0, new tokens beyond it none.  truncate: new tokens beyond it are left out altogether, as if
+    new_lens had ended there: no page, and neither seq_lens nor cu_new counts them (without it both count all of new_lens).
 
     page_size: a power of two from 16 to 1024; at most 4096 requests.  Nothing synchronises: lengths may change under a captured graph."""
     lib = _lib.load()
@@ -573,7 +574,7 @@ def page_tables(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.T
     seq_lens, cu_new, free_left, positions = torch.unsafe_split_with_sizes(
         torch.empty(2 * batch + 2 + max_new_tokens, dtype=i32, device=dev), [batch, batch + 1, 1, max_new_tokens])
     slots = torch.empty(max_new_tokens, dtype=torch.int64, device=dev)
-    st = lib.sp_paged_tables(_lib.PAGED_TABLES_ARGS.pack(
+    st = (lib.sp_paged_tables_truncated if truncate else lib.sp_paged_tables)(_lib.PAGED_TABLES_ARGS.pack(
         lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), seq_lens.data_ptr(),
         cu_new.data_ptr(), slots.data_ptr(), positions.data_ptr(), free_left.data_ptr(), batch, page_size, num_pages, block_table.size(1),
         block_table.stride(0), room, max_new_tokens, stream))

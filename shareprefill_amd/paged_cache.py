@@ -42,8 +42,9 @@ class PagedKVCache:
 
     def begin_step(self, new_lens: Optional[torch.Tensor] = None, max_new_tokens: Optional[int] = None) -> ops.PageTables:
         """Makes room for new_lens[r] more tokens of every request (int32 [max_requests]; None: one each).  max_new_tokens: how many there can be
-        in all, the T of the step's q, k and v.  Whether the pages sufficed is in the result's free_left (negative: they did not; tokens
-        without a slot are not cached and seen by nobody)."""
+        in all, the T of the step's q, k and v; tokens past it, of the last requests, are left out (the result's cu_new says what each request
+        brought, and its lens grow by that).  Whether the pages sufficed is in the result's free_left (negative: they did not; tokens without a slot
+        are not cached and seen by nobody)."""
         if new_lens is None:
             new_lens, max_new_tokens, singles = self._one_each, self.max_requests, True
         else:
@@ -51,7 +52,7 @@ class PagedKVCache:
             if max_new_tokens is None:
                 raise ValueError("max_new_tokens: how many new tokens there can be in all")
         t = ops.page_tables(self.lens, new_lens, self.block_table, self._stack[:self.num_pages], self.free_count, self.page_size,
-                            self.num_pages, max_new_tokens)
+                            self.num_pages, max_new_tokens, truncate=not singles)
         self.lens.copy_(t.seq_lens)
         torch.clamp(t.free_left, min=0, out=self.free_count)
         self.tables, self._cu_q = t, None if singles else t.cu_new
