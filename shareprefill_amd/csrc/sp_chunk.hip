@@ -685,16 +685,60 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       }
     }
     // A masked key weighs 0, and 0 times an infinity or a NaN of its value has made a NaN of the sum.  Such rows are formed again key by key,
-    // from what they see alone; rows whose NaN is their own come to the same again.
+    // from what they see alone, some 7 us a row and sub-tile: 2048 tokens over 32768 keys with one bad new token 1.1 -> 121 ms.  Rows whose NaN came
+    // from what they do see keep it: with one bad value in a long cache they are all rows of all later calls (256 tokens over 4096 keys 0.06 -> 2.7
+    // ms, with all of them formed again).  Which it was shows in the sub-tiles that not all of the wave's rows see whole, a handful wherever the walk
+    // is long.
+    uint32_t again[QT];
+    {
+      uint32_t no_number[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        const uint64_t lanes = __ballot(spoilt[qt]);
+        no_number[qt] = (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffffu;
+        again[qt] = 0u;
+      }
+      const int units = (no_number[0] | no_number[1]) != 0u ? 2 * pc.i1 : 0;
+#pragma unroll 1
+      for (int i0 = 2 * pc.i0; i0 < units; i0 += SP_WAVE) {
+        const int first = key_of(pc, 0, i0 + lane), last = first + CK_SUB - 1;
+        const bool whole_seen = last <= w0 && (!WINDOWED || first > w1 - a.window || last < a.sinks);
+#pragma unroll 1
+        for (uint64_t left = __ballot(i0 + lane < units && !whole_seen); left != 0ull; left &= left - 1ull) {
+          const int key = key_of(pc, 0, i0 + __builtin_ctzll(left)) + lane, page = key >> a.shift;
+          const auto c = args();
+          int id = page;
+          if constexpr (PAGED) {
+            id = page < c->width ? c->table[b * c->table_stride + page] : -1;
+            if ((unsigned)id >= (unsigned)c->num_pages) id = -1;
+          }
+          uint32_t bad = 0u;  // an exponent of ones: one more carries into the sign
+          if (id >= 0 && key < len) {
+            const sp_bf16* vrow = c->v + b * c->sv_b + kvh * c->sv_h + id * c->sv_p + (int64_t)(key & ((1 << a.shift) - 1)) * c->sv_n;
+            for (int ch = 0; ch < D; ch += 8) {
+              const uint4 x = *reinterpret_cast<const uint4*>(vrow + ch);
+              for (const uint32_t w : {x.x, x.y, x.z, x.w}) bad |= ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+            }
+          }
+          if (__ballot(bad != 0u) == 0ull) continue;
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt)
+            for (uint32_t rows_left = no_number[qt] & ~again[qt]; rows_left != 0u; rows_left &= rows_left - 1u) {
+              const int r = rt * TILE_ROWS + wave * 32 + 16 * qt + __builtin_ctz(rows_left);
+              const int p = len - q_len + (int)pg_div((unsigned)r, a.by_group);
+              if (__ballot(bad != 0u && !pg_sees(p, key, a.window, a.sinks)) != 0ull) again[qt] |= rows_left & (0u - rows_left);
+            }
+        }
+      }
+    }
 #pragma unroll 1
     for (int qt = 0; qt < QT; ++qt) {
-      uint64_t rows_left = __ballot(spoilt[qt]);
-      rows_left = (rows_left | rows_left >> 16 | rows_left >> 32 | rows_left >> 48) & 0xffffull;
-      if (rows_left == 0ull) continue;
+      uint32_t rows_left = again[qt];
+      if (rows_left == 0u) continue;
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the stores above come first
-      while (rows_left != 0ull) {
-        const int in_rows = wave * 32 + 16 * qt + __builtin_ctzll(rows_left);
-        rows_left &= rows_left - 1ull;
+      while (rows_left != 0u) {
+        const int in_rows = wave * 32 + 16 * qt + __builtin_ctz(rows_left);
+        rows_left &= rows_left - 1u;
         const int r = rt * TILE_ROWS + in_rows, token = (int)pg_div((unsigned)r, a.by_group), head = kvh * a.group + (r - token * a.group);
         const int p = len - q_len + token;
         const auto c = args();
@@ -714,7 +758,15 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           if (seen) {
             const sp_bf16* krow = c->k + b * c->sk_b + kvh * c->sk_h + id * c->sk_p + in * c->sk_n;
             float dot = 0.f;
-            for (int c = 0; c < D; ++c) dot = __builtin_fmaf(sp_bf16_to_f32(qrow[c]), sp_bf16_to_f32(krow[c]), dot);
+#pragma unroll 4
+            for (int ch = 0; ch < D; ch += 8) {
+              const at_u32x4 qx = *reinterpret_cast<const at_u32x4*>(qrow + ch), kx = *reinterpret_cast<const at_u32x4*>(krow + ch);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                dot = __builtin_fmaf(__uint_as_float(qx[i] << 16), __uint_as_float(kx[i] << 16), dot);
+                dot = __builtin_fmaf(__uint_as_float(qx[i] & 0xffff0000u), __uint_as_float(kx[i] & 0xffff0000u), dot);
+              }
+            }
             logit = dot * a.scale_log2;
           }
           const float new_top = fmaxf(top, sp_wave_max(logit)), alpha = __builtin_amdgcn_exp2f(top - new_top);
@@ -723,14 +775,31 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           top = new_top;
 #pragma unroll
           for (int c = 0; c < CL; ++c) acc[c] *= alpha;
-          const int64_t v_at = id < 0 ? 0 : id * c->sv_p + in * c->sv_n;
-          for (uint64_t left = __ballot(seen); left != 0ull; left &= left - 1ull) {
-            const int j = __builtin_ctzll(left);
-            const sp_bf16* vrow_j = c->v + b * c->sv_b + kvh * c->sv_h + __shfl(v_at, j, SP_WAVE) + lane * CL;
-            const float w = __shfl(weight, j, SP_WAVE);
+          const uint64_t keys = __ballot(seen);
+          const int64_t v_own = seen ? id * c->sv_p + in * c->sv_n : 0;
+          const int64_t v_first = __shfl(v_own, keys != 0ull ? __builtin_ctzll(keys) : 0, SP_WAVE), v_at = seen ? v_own : v_first;  // (read, not taken)
+          constexpr int AT_ONCE = 8;  // loads in flight
+#pragma unroll 1
+          for (int j0 = 0; j0 < SP_WAVE; j0 += AT_ONCE) {
+            if (((keys >> j0) & ((1ull << AT_ONCE) - 1ull)) == 0ull) continue;
+            float x[AT_ONCE][CL];
 #pragma unroll
-            for (int c = 0; c < CL; ++c) acc[c] = __builtin_fmaf(w, sp_bf16_to_f32(vrow_j[c]), acc[c]);
+            for (int u = 0; u < AT_ONCE; ++u) {
+              const sp_bf16* vrow_j = c->v + b * c->sv_b + kvh * c->sv_h + __shfl(v_at, j0 + u, SP_WAVE) + lane * CL;
+#pragma unroll
+              for (int ch = 0; ch < CL; ++ch) x[u][ch] = sp_bf16_to_f32(vrow_j[ch]);
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+              const float w = __shfl(weight, j0 + u, SP_WAVE);
+#pragma unroll
+              for (int ch = 0; ch < CL; ++ch) acc[ch] = __builtin_fmaf(w, (keys >> (j0 + u)) & 1ull ? x[u][ch] : 0.f, acc[ch]);
+            }
           }
+          bool number = false;  // (a row that is none in any channel stays that)
+#pragma unroll
+          for (int c = 0; c < CL; ++c) number |= acc[c] == acc[c];
+          if (sum > 0.f && __ballot(number) == 0ull) break;
         }
 #pragma unroll
         for (int c = 0; c < CL; ++c) {
