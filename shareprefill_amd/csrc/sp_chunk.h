@@ -4,7 +4,9 @@
 #include "sp_common.h"
 #include "sp_paged_plan.h"
 
-#define CK_NO_MAX (-1.0e30f)  // running maximum of a row without keys: finite, so its partial weighs 0 beside others and nothing is NaN
+// Running maximum of a row without keys: finite, so its partial weighs 0 beside others and nothing is NaN, and below every logit there is, so that the
+// first keys move it and a part's weight is that of its own largest logit.
+#define CK_NO_MAX (-0x1.fffffep127f)
 
 struct CkArgs {
   const sp_bf16 *q, *k, *v;

@@ -29,6 +29,10 @@
 // over 8192 94.5 / 84.9 / 84.1 / 84.2, 16384 without a window - / 1796 / 1778 / 1777.  What it costs: the largest probability need not be a power of
 // two, which bf16 holds exactly; outputs are 2.14e-3 / 2.22e-3 / 2.23e-3 / 2.23e-3 from 64 bits, 1.6e-3 of it their own rounding.
 #define CK_SLACK 7
+// Largest magnitude of a row's maximum, in octaves, up to which its probabilities are what the loop forms: exponents of the exact product less a
+// maximum that is rounded, off by that rounding for all of a row's keys alike and near nothing.  Beyond it they may all be zero, and the rows are
+// formed again from rounded products, whose largest is the maximum itself.
+#define CK_FAR 0x1p24f
 #define CK_WAVES 8
 #define CK_THREADS (CK_WAVES * SP_WAVE)
 #define CK_ROWS (32 * CK_WAVES)  // of a row tile
@@ -462,7 +466,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     for (int ct = 0; ct < 9; ++ct)
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) o[ct][qt] = (floatx4){0, 0, 0, 0};
-    float m[QT] = {AT_NO_MAX, AT_NO_MAX}, l_mark[QT] = {0.f, 0.f};
+    float m[QT] = {CK_NO_MAX, CK_NO_MAX}, l_mark[QT] = {0.f, 0.f};
     uint32_t det[2] = {0u, 0u};
 
     // to the pages of a block's second sub-tile
@@ -648,7 +652,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       else
         note.x = to_end ? CK_LAST : CK_MIDDLE;
     }
-    bool spoilt[QT];  // a NaN in the lane's part of the row
+    bool spoilt[QT], far[QT];  // a NaN in the lane's part of the row; its logits are far from zero
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       const int in_rows = wave * 32 + 16 * qt + lq;
@@ -662,6 +666,8 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         for (int j = 0; j < 4; ++j) spoilt[qt] |= o[ct][qt][j] != o[ct][qt][j];
       // (a row whose sum is a NaN saw a logit that is none, or an infinite one: it is a NaN in all its channels as it is)
       spoilt[qt] = spoilt[qt] && mine && l[qt] == l[qt];
+      const float size = __builtin_fabsf(m[qt]);
+      far[qt] = mine && l[qt] == l[qt] && size >= CK_FAR && size < INFINITY && m[qt] != CK_NO_MAX;
       if (whole) {
         const float inv_l = l[qt] > 0.f || l[qt] != l[qt] ? 1.0f / l[qt] : 0.f;
         // (lane groups 2i and 2i + 1 trade halves of two neighbouring channel tiles: 16 bytes a store, 64 contiguous ones a row)
@@ -696,7 +702,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       for (int qt = 0; qt < QT; ++qt) {
         const uint64_t lanes = __ballot(spoilt[qt]);
         no_number[qt] = (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffffu;
-        again[qt] = 0u;
+        again[qt] = (uint32_t)__ballot(far[qt]) & 0xffffu;  // (the same in all of a row's lanes)
       }
       const int units = (no_number[0] | no_number[1]) != 0u ? 2 * pc.i1 : 0;
 #pragma unroll 1

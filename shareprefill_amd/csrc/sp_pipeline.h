@@ -308,7 +308,15 @@ __device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 
     float mx[2];  // (S(j-1) is a whole stage old: no wait states needed before reading it)
     at_lanemax(s_prev, mx);
     float m_new[2] = {at_groupmax(mx[0] * scale_log2), at_groupmax(mx[1] * scale_log2)};
-    if constexpr (SLACK > 0) m_new[0] += (float)SLACK, m_new[1] += (float)SLACK;
+    // (Past 2^20 a few units in the last place more: the probabilities' exponent has the exact product, and a max rounded down would make them
+    // infinite.  They may come out as zero instead, where the caller forms such rows another way.)
+    if constexpr (SLACK > 0) {
+#pragma unroll
+      for (int qt = 0; qt < 2; ++qt) {
+        m_new[qt] += (float)SLACK;
+        m_new[qt] = __builtin_fmaf(__builtin_amdgcn_fmed3f(__builtin_fabsf(m_new[qt]) - 0x1p20f, 0.f, 0x1.fffffep127f), 0x1p-22f, m_new[qt]);
+      }
+    }
     m_new[0] = at_max2(m_run[0], m_new[0]), m_new[1] = at_max2(m_run[1], m_new[1]);
     at_settle_o(o);
     // m_run = AT_NO_MAX on a row's first keys: alpha = 0 (O and the sums are still zero then)
