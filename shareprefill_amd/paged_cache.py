@@ -5,11 +5,11 @@
     for layer in range(32):                                 # q, k, v of the step's tokens, request after request
         cache.write(layer, k, v)
         out = cache.attend(layer, q, softmax_scale)
+    cache.begin_step(active=running)                        # a token of each running request, rows request by request
     cache.release(finished)
 
 A step (begin_step, write, attend) reads no device value on the host, so it can be recorded into a HIP graph and replayed with other lengths;
-release runs between steps.  The reference keeps no
-cache of its own (its decode step reads a contiguous one, shareprefill_attn.py:146-155).
+release runs between steps.  The reference keeps no cache of its own (its decode step reads a contiguous one, shareprefill_attn.py:146-155).
 """
 
 from __future__ import annotations
@@ -39,22 +39,42 @@ class PagedKVCache:
         self._one_each = torch.ones(max_requests, dtype=torch.int32, device=dev)
         self.tables: Optional[ops.PageTables] = None
         self._cu_q: Optional[torch.Tensor] = None
+        self._seen_lens: Optional[torch.Tensor] = None  # of a step: keys that a request's rows may see
 
-    def begin_step(self, new_lens: Optional[torch.Tensor] = None, max_new_tokens: Optional[int] = None) -> ops.PageTables:
-        """Makes room for new_lens[r] more tokens of every request (int32 [max_requests]; None: one each).  max_new_tokens: how many there can be
+    def _check_mask(self, mask: torch.Tensor, name: str) -> None:
+        if mask.dtype is not torch.bool or tuple(mask.shape) != (self.max_requests,) or mask.device != self.lens.device:
+            raise ValueError(f"{name} must be bool [{self.max_requests}] on {self.lens.device}")
+
+    def begin_step(self, new_lens: Optional[torch.Tensor] = None, max_new_tokens: Optional[int] = None,
+                   active: Optional[torch.Tensor] = None) -> ops.PageTables:
+        """Makes room for new_lens[r] more tokens of every request (int32 [max_requests]).  Without new_lens it is one token of every request that
+        has active[r] (bool [max_requests]), and row r of the step's q, k and v is request r's: rows of the others go nowhere, and come out of attend as
+        zeros.  Without either it is one of each of the max_requests rows, also of those that no request has: for a full server.  (A prompt that
+        comes to such a row later would stand behind what was cached there.)
+
+        max_new_tokens: how many there can be
         in all, the T of the step's q, k and v; tokens past it, of the last requests, are left out (the result's cu_new says what each request
         brought, and its lens grow by that).  Whether the pages sufficed is in the result's free_left (negative: they did not; tokens without a slot
         are not cached and seen by nobody)."""
-        if new_lens is None:
-            new_lens, max_new_tokens, singles = self._one_each, self.max_requests, True
-        else:
-            singles = False
-            if max_new_tokens is None:
-                raise ValueError("max_new_tokens: how many new tokens there can be in all")
+        singles = new_lens is None
+        if active is not None:
+            if not singles:
+                raise ValueError("new_lens already says which requests bring tokens: active is for steps without it")
+            self._check_mask(active, "active")
+        if singles:
+            new_lens, max_new_tokens = self._one_each if active is None else active.to(torch.int32), self.max_requests
+        elif max_new_tokens is None:
+            raise ValueError("max_new_tokens: how many new tokens there can be in all")
         t = ops.page_tables(self.lens, new_lens, self.block_table, self._stack[:self.num_pages], self.free_count, self.page_size,
                             self.num_pages, max_new_tokens, truncate=not singles)
         self.lens.copy_(t.seq_lens)
         torch.clamp(t.free_left, min=0, out=self.free_count)
+        self._seen_lens = t.seq_lens
+        if active is not None:
+            # from places among the step's tokens, which only active requests have, to a row a request
+            place = t.cu_new[:-1].clamp(max=self.max_requests - 1).long()
+            t = t._replace(slots=torch.where(active, t.slots[place], -1), positions=torch.where(active, t.positions[place], 0))
+            self._seen_lens = torch.where(active, t.seq_lens, 0)
         self.tables, self._cu_q = t, None if singles else t.cu_new
         return t
 
@@ -70,14 +90,13 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, window: Optional[int] = None, sinks: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q: bf16 [Hq, T, D] view -> bf16 [T, Hq, D]: every new token over what its request has cached up to it (ops.paged_attention)."""
-        return ops.paged_attention(q, *self._pools_of(layer), self.block_table, self.tables.seq_lens, softmax_scale, cu_q=self._cu_q,
+        return ops.paged_attention(q, *self._pools_of(layer), self.block_table, self._seen_lens, softmax_scale, cu_q=self._cu_q,
                                    window=window, sinks=sinks, out=out)
 
     def release(self, finished: torch.Tensor) -> None:
         """Puts the pages of the requests with finished[r] (bool [max_requests]) back on the stack; their rows are empty again.
         Not for a captured graph."""
-        if finished.dtype is not torch.bool or tuple(finished.shape) != (self.max_requests,) or finished.device != self.lens.device:
-            raise ValueError(f"finished must be bool [{self.max_requests}] on {self.lens.device}")
+        self._check_mask(finished, "finished")
         back = finished[:, None] & (self.block_table >= 0)
         count = torch.cumsum(back.reshape(-1), 0, dtype=torch.int32)
         place = torch.where(back.reshape(-1), self.free_count + count - 1, self.num_pages)
