@@ -955,9 +955,12 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   SP_REQUIRE(x->cu_q != nullptr || x->tokens == x->batch, SP_ERR_INVALID_ARGUMENT, "%s: without cu_q every sequence has one token (%lld for %lld)",
              who, (long long)x->tokens, (long long)x->batch);
   if (x->tokens == 0) return SP_OK;
+  const int64_t q_n = pg_used_stride(x->q_stride_n, x->tokens), q_h = pg_used_stride(x->q_stride_h, x->hq);
+  const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);
+  const int64_t v_p = pg_used_stride(x->v_stride_page, x->num_pages), v_h = pg_used_stride(x->v_stride_h, x->hkv);
   SP_REQUIRE(x->q && x->k_pages && x->v_pages && x->block_table && x->seq_lens && x->out, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k_pages | (uintptr_t)x->v_pages | (uintptr_t)x->out) % 16 == 0 &&
-                 (x->q_stride_n | x->q_stride_h | x->k_stride_page | x->k_stride_h | x->v_stride_page | x->v_stride_h) % 8 == 0,
+                 (q_n | q_h | k_p | k_h | v_p | v_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
   SP_REQUIRE(ck_rows_ok(x->k_stride_slot, x->page_size) && ck_rows_ok(x->v_stride_slot, x->page_size), SP_ERR_UNSUPPORTED,
              "%s: slot strides %lld / %lld unsupported", who, (long long)x->k_stride_slot, (long long)x->v_stride_slot);
@@ -965,9 +968,9 @@ extern "C" int sp_paged_attn_bf16(const sp_paged_attn_args* x) {
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k_pages, a.v = (const sp_bf16*)x->v_pages;
   a.table = x->block_table, a.lens = x->seq_lens, a.cu = x->cu_q, a.out = (sp_bf16*)x->out;
   a.table_stride = x->table_stride;
-  a.sq_n = x->q_stride_n, a.sq_h = x->q_stride_h;
-  a.sk_p = x->k_stride_page, a.sk_n = x->k_stride_slot, a.sk_h = x->k_stride_h;
-  a.sv_p = x->v_stride_page, a.sv_n = x->v_stride_slot, a.sv_h = x->v_stride_h;
+  a.sq_n = q_n, a.sq_h = q_h;
+  a.sk_p = k_p, a.sk_n = x->k_stride_slot, a.sk_h = k_h;
+  a.sv_p = v_p, a.sv_n = x->v_stride_slot, a.sv_h = v_h;
   a.batch = (int)x->batch, a.tokens = (int)x->tokens, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
   a.n_queries = 1;
   a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.window = ck_window(x->window), a.sinks = (int)(x->sinks < PG_MAX_KEYS ? x->sinks : PG_MAX_KEYS);
@@ -996,18 +999,23 @@ extern "C" int sp_window_attn_bf16(const sp_window_attn_args* x) {
   SP_REQUIRE(x->n_keys <= PG_MAX_KEYS && x->batch * x->n <= PG_MAX_KEYS, SP_ERR_UNSUPPORTED, "%s: batch=%lld n=%lld n_keys=%lld too large", who,
              (long long)x->batch, (long long)x->n, (long long)x->n_keys);
   if (x->n == 0) return SP_OK;
+  const int64_t q_b = pg_used_stride(x->q_stride_b, x->batch), q_n = pg_used_stride(x->q_stride_n, x->n), q_h = pg_used_stride(x->q_stride_h, x->hq);
+  const int64_t k_b = pg_used_stride(x->k_stride_b, x->batch), k_h = pg_used_stride(x->k_stride_h, x->hkv);
+  const int64_t v_b = pg_used_stride(x->v_stride_b, x->batch), v_h = pg_used_stride(x->v_stride_h, x->hkv);
+  // (rows behind a sequence's last one are read as what lies behind its end, which a single key has to have too)
+  const int64_t k_n = x->n_keys == 1 ? x->d : x->k_stride_n, v_n = x->n_keys == 1 ? x->d : x->v_stride_n;
   SP_REQUIRE(x->q && x->k && x->v && x->out, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k | (uintptr_t)x->v | (uintptr_t)x->out) % 16 == 0 &&
-                 (x->q_stride_b | x->q_stride_n | x->q_stride_h | x->k_stride_b | x->k_stride_h | x->v_stride_b | x->v_stride_h) % 8 == 0,
+                 (q_b | q_n | q_h | k_b | k_h | v_b | v_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
-  SP_REQUIRE(ck_rows_ok(x->k_stride_n, CK_SUB) && ck_rows_ok(x->v_stride_n, CK_SUB), SP_ERR_UNSUPPORTED, "%s: token strides %lld / %lld unsupported", who,
+  SP_REQUIRE(ck_rows_ok(k_n, CK_SUB) && ck_rows_ok(v_n, CK_SUB), SP_ERR_UNSUPPORTED, "%s: token strides %lld / %lld unsupported", who,
              (long long)x->k_stride_n, (long long)x->v_stride_n);
   CkArgs a = {};
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k, a.v = (const sp_bf16*)x->v, a.out = (sp_bf16*)x->out;
   a.shift = 6;  // a sub-tile is a page
-  a.sq_b = x->q_stride_b, a.sq_n = x->q_stride_n, a.sq_h = x->q_stride_h;
-  a.sk_b = x->k_stride_b, a.sk_n = x->k_stride_n, a.sk_h = x->k_stride_h, a.sk_p = x->k_stride_n << a.shift;
-  a.sv_b = x->v_stride_b, a.sv_n = x->v_stride_n, a.sv_h = x->v_stride_h, a.sv_p = x->v_stride_n << a.shift;
+  a.sq_b = q_b, a.sq_n = q_n, a.sq_h = q_h;
+  a.sk_b = k_b, a.sk_n = k_n, a.sk_h = k_h, a.sk_p = k_n << a.shift;
+  a.sv_b = v_b, a.sv_n = v_n, a.sv_h = v_h, a.sv_p = v_n << a.shift;
   a.batch = (int)x->batch, a.tokens = (int)(x->batch * x->n), a.n_keys = (int)x->n_keys, a.n_queries = (int)x->n;
   a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.window = ck_window(x->window), a.sinks = (int)(x->sinks < PG_MAX_KEYS ? x->sinks : PG_MAX_KEYS);
   a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;

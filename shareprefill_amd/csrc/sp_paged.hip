@@ -195,10 +195,13 @@ extern "C" int sp_paged_cache_write_bf16(const sp_paged_write_args* x) {
   const int shift = page_shift(x->page_size);
   SP_REQUIRE(shift >= 0, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
   if (x->tokens == 0 || x->num_pages == 0) return SP_OK;
+  const int64_t k_n = pg_used_stride(x->k_stride_n, x->tokens), k_h = pg_used_stride(x->k_stride_h, x->hkv);
+  const int64_t v_n = pg_used_stride(x->v_stride_n, x->tokens), v_h = pg_used_stride(x->v_stride_h, x->hkv);
+  const int64_t kp_p = pg_used_stride(x->k_stride_page, x->num_pages), kp_h = pg_used_stride(x->k_stride_page_h, x->hkv);
+  const int64_t vp_p = pg_used_stride(x->v_stride_page, x->num_pages), vp_h = pg_used_stride(x->v_stride_page_h, x->hkv);
   SP_REQUIRE(x->k && x->v && x->k_pages && x->v_pages && x->slots, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   SP_REQUIRE(((uintptr_t)x->k | (uintptr_t)x->v | (uintptr_t)x->k_pages | (uintptr_t)x->v_pages) % 16 == 0 &&
-                 (x->k_stride_n | x->k_stride_h | x->v_stride_n | x->v_stride_h | x->k_stride_page | x->k_stride_slot | x->k_stride_page_h |
-                  x->v_stride_page | x->v_stride_slot | x->v_stride_page_h) % 8 == 0,
+                 (k_n | k_h | v_n | v_h | kp_p | x->k_stride_slot | kp_h | vp_p | x->v_stride_slot | vp_h) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
   SP_REQUIRE(x->tokens <= (1ll << 40) && x->hkv <= 65536 && x->num_pages <= 0x7fffffffll, SP_ERR_UNSUPPORTED,
              "%s: tokens=%lld hkv=%lld num_pages=%lld too many", who, (long long)x->tokens, (long long)x->hkv, (long long)x->num_pages);
@@ -206,10 +209,9 @@ extern "C" int sp_paged_cache_write_bf16(const sp_paged_write_args* x) {
   SP_REQUIRE(most > 0, SP_ERR_UNSUPPORTED, "%s: hkv=%lld head_dim=%lld too large", who, (long long)x->hkv, (long long)x->d);
   for (int64_t t = 0; t < x->tokens; t += most) {
     const int items = (int)((x->tokens - t < most ? x->tokens - t : most) * of_token);
-    const WriteArgs a = {(const sp_bf16*)x->k + t * x->k_stride_n, (const sp_bf16*)x->v + t * x->v_stride_n, (sp_bf16*)x->k_pages, (sp_bf16*)x->v_pages,
+    const WriteArgs a = {(const sp_bf16*)x->k + t * k_n, (const sp_bf16*)x->v + t * v_n, (sp_bf16*)x->k_pages, (sp_bf16*)x->v_pages,
                          x->slots + t, x->num_pages << shift, items, shift, pg_divisor((unsigned)(x->d / 8)), pg_divisor((unsigned)x->hkv),
-                         x->k_stride_n, x->k_stride_h, x->v_stride_n, x->v_stride_h, x->k_stride_page, x->k_stride_slot, x->k_stride_page_h,
-                         x->v_stride_page, x->v_stride_slot, x->v_stride_page_h};
+                         k_n, k_h, v_n, v_h, kp_p, x->k_stride_slot, kp_h, vp_p, x->v_stride_slot, vp_h};
     hipLaunchKernelGGL(sp_paged_write_kernel, dim3((unsigned)sp_ceil_div(items, PW_THREADS)), dim3(PW_THREADS), 0, (hipStream_t)x->stream, a);
   }
   SP_LAUNCH_CHECK();

@@ -37,6 +37,9 @@ PG_FN int pg_holder(const int* sums, int n, int x) {  // the last of n entries t
   return lo;
 }
 
+// A stride as the kernels take it: that of an axis of length one says nothing, and may be anything.
+PG_FN int64_t pg_used_stride(int64_t stride, int64_t length) { return length == 1 ? 0 : stride; }
+
 // The query at position p sees key j: causal, inside its window or among the first `sinks`.
 PG_FN bool pg_sees(int p, int j, int window, int sinks) { return j <= p && (j > p - window || j < sinks); }
 

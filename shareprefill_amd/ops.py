@@ -542,7 +542,7 @@ def _check_ints(device, *named) -> None:
 
 def _check_table(block_table: torch.Tensor, batch: int, device) -> None:
     if (block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] != batch or block_table.device != device
-            or block_table.shape[1] < 1 or block_table.stride(1) != 1):
+            or block_table.shape[1] < 1 or (block_table.stride(1) != 1 and block_table.shape[1] != 1)):
         raise ValueError(f"block_table must be int32 [{batch}, pages of a request] with contiguous rows on {device}")
 
 
