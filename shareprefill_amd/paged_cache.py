@@ -90,7 +90,10 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, window: Optional[int] = None, sinks: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q: bf16 [Hq, T, D] view -> bf16 [T, Hq, D]: every new token over what its request has cached up to it (ops.paged_attention)."""
-        return ops.paged_attention(q, *self._pools_of(layer), self.block_table, self._seen_lens, softmax_scale, cu_q=self._cu_q,
+        pools = self._pools_of(layer)
+        if q.dim() == 3 and q.shape[1] != self.tables.slots.numel():
+            raise ValueError(f"q has {q.shape[1]} rows, the step {self.tables.slots.numel()}")
+        return ops.paged_attention(q, *pools, self.block_table, self._seen_lens, softmax_scale, cu_q=self._cu_q,
                                    window=window, sinks=sinks, out=out)
 
     def release(self, finished: torch.Tensor) -> None:
