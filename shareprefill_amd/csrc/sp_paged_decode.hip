@@ -16,10 +16,6 @@
 #include "sp_ring.h"
 
 #define PD_ROWS PD_MAX_GROUP
-// Units of a line that a sequence counts beside its steps: queries, first loads, the waves' meeting; units of a part at least.  (us, 8 and 8 /
-// 4 and 4: one token over 1025 keys 11.5 / 9.9, 64 over 500 27.0 / 23.5, 64 over 8192 128.7 either way.)
-#define PD_OVERHEAD 4
-#define PD_MIN_SHARE 4
 
 template <int D>
 using PdShape = DsShape<D, D / 16, D == 64 ? 8 : 4, 152>;

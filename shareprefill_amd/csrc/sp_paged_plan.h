@@ -94,6 +94,10 @@ PG_FN void pg_tile_positions(int rt, int q_len, int len, const PgDivisor& g, int
 // beside three tokens over 4000 80.6 / 83.0 / 85.6 / 88.8, a mixed batch of 64 channels 133.1 / 132.7 / 132.6 / 135.3.)
 #define PG_OVERHEAD 3
 #define PG_MIN_SHARE 3  // units of a part at least
+// The same of single tokens, whose line is made of sequences and their steps of 32 keys: queries, first loads, the waves' meeting.  (us, 8 and 8 /
+// 4 and 4: one token over 1025 keys 11.5 / 9.9, 64 over 500 27.0 / 23.5, 64 over 8192 128.7 either way.)
+#define PD_OVERHEAD 4
+#define PD_MIN_SHARE 4
 // (Quotients of 64 bits take the device a hundred instructions each, and every workgroup forms them: lines that fit 31 bits do without.)
 #define PG_SHORT_LINE (1ll << 31)
 PG_FN int64_t pg_parts(int64_t total, int64_t room, int share) {
