@@ -52,10 +52,9 @@ class PagedKVCache:
         zeros.  Without either it is one of each of the max_requests rows, also of those that no request has: for a full server.  (A prompt that
         comes to such a row later would stand behind what was cached there.)
 
-        max_new_tokens: how many there can be
-        in all, the T of the step's q, k and v; tokens past it, of the last requests, are left out (the result's cu_new says what each request
-        brought, and its lens grow by that).  Whether the pages sufficed is in the result's free_left (negative: they did not; tokens without a slot
-        are not cached and seen by nobody)."""
+        max_new_tokens: how many there can be in all, the T of the step's q, k and v; tokens past it, of the last requests, are left out (the
+        result's cu_new says what each request brought, and its lens grow by that).  Whether the pages sufficed is in the result's free_left
+        (negative: they did not; tokens without a slot are not cached and seen by nobody)."""
         singles = new_lens is None
         if active is not None:
             if not singles:
@@ -71,10 +70,10 @@ class PagedKVCache:
         torch.clamp(t.free_left, min=0, out=self.free_count)
         self._seen_lens = t.seq_lens
         if active is not None:
-            # from places among the step's tokens, which only active requests have, to a row a request
-            place = t.cu_new[:-1].clamp(max=self.max_requests - 1).long()
-            t = t._replace(slots=torch.where(active, t.slots[place], -1), positions=torch.where(active, t.positions[place], 0))
-            self._seen_lens = torch.where(active, t.seq_lens, 0)
+            # from a token's place among the step's, which only active requests have, to its request's row (row r has r places in front of it at most)
+            place = t.cu_new[:-1]
+            t = t._replace(slots=torch.where(active, t.slots.index_select(0, place), -1), positions=t.positions.index_select(0, place) * new_lens)
+            self._seen_lens = t.seq_lens * new_lens
         self.tables, self._cu_q = t, None if singles else t.cu_new
         return t
 
