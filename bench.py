@@ -166,7 +166,7 @@ def cpu_baseline(w, q, k, v, mask_bool, decision, kept_blocks, pt):
 # reported only while shareprefill_amd/csrc/sp_attn.hip and the headers of that folder that it includes still have that
 # hash, and is null (with a note) after any change to them until the profile is taken again.
 MEASURED_ATTN_TRAFFIC = {
-    ("C3", 0.95): {"bytes": int((102.5 + 1.0) * 2 ** 30), "attn_sources_sha256_16": "3868e4849c889675",
+    ("C3", 0.95): {"bytes": int((102.9 + 1.0) * 2 ** 30), "attn_sources_sha256_16": "7c37f093df321b8a",
                    "profile": "profiles/attention_layer_C3_hbm_traffic.txt"},
 }
 

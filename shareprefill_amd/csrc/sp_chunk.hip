@@ -17,7 +17,7 @@
 // (30001 tokens in a window of 4096 2282 -> 1811 us).  The row tiles' blocks form a line that is cut into equal parts, one workgroup each
 // (sp_paged_plan.h): every CU has as much to do as the others, whatever the sequences' lengths, which only the device knows; row tiles that a
 // cut goes through leave fp32 partials that a second launch merges.  No length comes to the host, so the call can be captured into a graph.
-// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1760 to 1820 us by card, 1180 to 1220 TFLOP/s, the
+// What it reaches, head_dim 128, 32 heads over 8: 2048 tokens over 65001 keys in pages of 128 1760 to 1830 us by card, 1170 to 1220 TFLOP/s, the
 // rate of a large bf16 matrix product; 30001 tokens in a window of 4096 1150 to 1200.  Short calls: some 8 us go by until the line is laid out
 // and the first keys have landed, a row tile's turn takes 5 us beside its blocks of 3.5 us each, partials and their merging 15 us.
 #include "sp_chunk.h"

@@ -363,7 +363,9 @@ int pd_launch(CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream
   const int64_t pairs = (int64_t)a.batch * a.hkv, units = sp_ceil_div(max_keys, DS_KEYS) + PD_OVERHEAD;
   const int64_t most = pg_parts(units * a.batch, pd_parts(a.hkv), PD_MIN_SHARE);
   // A workgroup a sequence where that takes the longest of them no longer than even parts and their merging launch, in units (of 64 channels
-  // one takes half the time).  A table's width only bounds the lengths: sequences are taken for five eighths of it on average.
+  // one takes half the time).  A table's width only bounds the lengths, which the host does not know: five eighths of it on average is what lengths
+  // spread evenly from a quarter of it up come to, an assumption and no measurement of a server's.  Where it is wider than the caches are long, short
+  // ones are cut though whole ones would be faster.
   // us, whole / cut, sequences of up to n keys; 32 heads over 8: 1 of 200 7.3 / 9.7, 1 of 1025 18.8 / 10.0, 16 of 1000 19.7 / 19.2, 64 of 500
   // 23.6 / 27.2, 128 of 2000 143 / 127; 14 over 2 of 64 channels: 1 of 1025 10.0 / 9.2, 16 of 1000 10.0 / 13.0, 128 of 2000 19.7 / 27.4.
   const int64_t whole = sp_ceil_div(pairs, 256) * units;

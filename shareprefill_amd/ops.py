@@ -644,7 +644,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     with a window, of those j > p - window and j < sinks.  Keys without a page (an entry outside the pool) are not seen; a row that sees
     nothing is zero.  Rows of `out` outside every request stay as they were (undefined in a tensor made here); `out` shares no memory with q.
     head_dim 64 or 128, page_size a power of two from 16 to 1024; at most 4096 requests of single tokens without cu_q and groups of up to 16
-    query heads, else 2048.  Lengths and pages are read on the device.  Scratch memory: up to 68 MB, from torch's allocator, for the call."""
+    query heads, else 2048.  Lengths and pages are read on the device.  Scratch memory, from torch's allocator, for the call: up to 68 MB, with more than 256
+    kv heads 0.27 MB a head.
+
+    Precision: sums, maxima and partial results have 32 bits.  Probabilities enter the product with V as one bf16 value where a request may have
+    several rows (outputs some 2.3e-3 from 64 bits, 1.6e-3 of it their own rounding), and as two without cu_q in groups of up to 16 query heads
+    (1.7e-3).  A value that is not finite makes the rows that see it not finite, and no others."""
     lib = _lib.load()
     _check_hnd(q, "q")
     hq, n, d = q.shape
@@ -683,7 +688,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_
                      sinks: int = 0) -> torch.Tensor:
     """Causal attention in a sliding window with the first `sinks` tokens kept in sight: q bf16 [B, Hq, N, D], k / v bf16 [B, Hkv, Nk, D]
     views, N <= Nk, the queries being the last N positions -> out bf16 [B, N, Hq, D].  The query at position p sees keys j <= p with
-    j > p - window or j < sinks; window None: all j <= p (a prompt's next chunk over a contiguous cache).
+    j > p - window or j < sinks; window None: all j <= p (a prompt's next chunk over a contiguous cache).  Precision as in paged_attention: N = 1 has
+    the two bf16 values.
 
     Prompts (N = Nk), chunks and single tokens (N = 1) alike; head_dim 64 or 128, any strides with a contiguous head_dim axis; B at most 2048
     (4096 for single tokens of groups of up to 16 query heads)."""
