@@ -355,7 +355,7 @@ int sp_decode_attn_static_bf16(const void* q, const void* k, const void* v, int6
  * Written: seq_lens[b] = lens[b] + new_lens[b]; cu_new[0 .. batch] = prefix sums of new_lens; per new token t < max_tokens, in the order
  * of the sequences, slots[t] = page * page_size + position % page_size (-1: no page, or beyond the table's width) and positions[t] (its
  * place in its sequence); tokens behind the last one get -1 and 0.  *free_left = pages left on the stack (negative: so many were missing).
- * Negative lengths count as 0.  The outputs must not overlap the inputs. */
+ * Negative lengths count as 0, longer ones than 2^30 - 1 as that, and sums of them hold at 2^30.  The outputs must not overlap the inputs. */
 typedef struct sp_paged_tables_args {
   const int32_t *lens, *new_lens;
   int32_t* block_table;
