@@ -419,6 +419,30 @@ typedef struct sp_window_attn_args {
 size_t sp_window_attn_workspace_bytes(int32_t batch, int64_t n, int64_t n_keys, int32_t hq, int32_t hkv, int32_t d);
 int sp_window_attn_bf16(const sp_window_attn_args* args /* host */);
 
+/* Attention of new tokens where requests have their first keys in common: as sp_paged_attn_bf16 without a window, the shared keys read once for a
+ * whole group.  Group i is the sequences cu_groups[i] .. cu_groups[i + 1] (int32, groups + 1 of them, in order; sequences outside share
+ * nothing); the first shared_lens[i] keys of each are those that the table row of its first sequence names.  A sequence with a new token at a place
+ * in front of that sees to all of its keys by itself.  At most 1024 sequences.
+ * weights (null, or fp32 [num_pages][hkv][page_size] with element strides for the page and head axes): for calls without cu_q and up to 16
+ * query heads to a kv head.  For every sequence and each of its keys j that is not shared, at its place in the pages,
+ *   weights[j] += sum over the query heads of the kv group of softmax(q . k)[j];
+ * the last key's is set to that sum.  No such key may stand in pages of two sequences.
+ * single_tokens: for calls without cu_q; pool_keys: num_pages * page_size where weights are given, else 0. */
+typedef struct sp_shared_attn_args {
+  const void *q, *k_pages, *v_pages;
+  const int32_t *block_table, *seq_lens, *cu_q, *shared_lens, *cu_groups;
+  float* weights;
+  void *out, *workspace;
+  uint64_t workspace_bytes;
+  int64_t tokens, batch, groups, hq, hkv, d, num_pages, page_size, table_width, table_stride;
+  int64_t q_stride_n, q_stride_h, k_stride_page, k_stride_slot, k_stride_h, v_stride_page, v_stride_slot, v_stride_h, w_stride_page, w_stride_h;
+  double softmax_scale;
+  sp_stream_t stream;
+} sp_shared_attn_args;
+size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t groups, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens,
+                                      int64_t pool_keys);
+int sp_shared_attn_bf16(const sp_shared_attn_args* args /* host */);
+
 /* ---- rotary position embedding in front of the attention function ---------------------------------
  * The reference's patched model produces (cos, sin) per position (model_patch.py:121) and leaves the rotation to
  * the Hugging Face attention layer, which evaluates  x*cos + rotate_half(x)*sin  (rotate_half(x) =

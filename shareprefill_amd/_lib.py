@@ -105,6 +105,8 @@ SIGNATURES = {
     "sp_paged_attn_bf16": (_I32, [C.c_char_p]),
     "sp_window_attn_workspace_bytes": (_SZ, [_I32, _I64, _I64, _I32, _I32, _I32]),
     "sp_window_attn_bf16": (_I32, [C.c_char_p]),
+    "sp_shared_attn_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32, _I32, _I64]),
+    "sp_shared_attn_bf16": (_I32, [C.c_char_p]),
     "sp_rope_inplace_bf16": (_I32, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _P]),
     "sp_pivot_update": (_I32, [_ST, _P, _P, _P, _I32, _I32, _F, _P]),
     "sp_cover_select_rows": (_I32, [_P, _I32, _F, _P, _P]),
@@ -120,6 +122,8 @@ PAGED_TABLES_ARGS = struct.Struct("@10P7qP")
 PAGED_WRITE_ARGS = struct.Struct("@5P15qP")
 PAGED_ATTN_ARGS = struct.Struct("@8PQ19qdP")
 WINDOW_ATTN_ARGS = struct.Struct("@5PQ17qdP")
+# sp_shared_attn_args
+SHARED_ATTN_ARGS = struct.Struct("@11PQ20qdP")
 
 _lib = None
 

@@ -1,0 +1,882 @@
+// Attention of new tokens over a paged cache in which groups of requests have their first keys in common (sp_shared_attn_bf16):
+//   out = sum_j exp(scale q . k_j) v_j / sum_j exp(scale q . k_j) over the keys j <= p of the row's request,
+// the sum over the shared keys formed once for all rows of the group and joined with that over the request's own: with running maxima m and
+// sums l of either side, out = (2^(m1 - m) o1 + 2^(m2 - m) o2) / (2^(m1 - m) l1 + 2^(m2 - m) l2).
+//
+// HBM-bound as long as a group has fewer than some 250 rows a kv head: shared keys are read once per tile of 64 rows, a request's own
+// once.  Tiles of 16 rows or fewer (a request's single token) take the loop of the single-token kernel (sp_paged_decode.hip): waves take steps of 32 keys
+// in turn, each with a ring of operands in LDS that direct loads fill, no barrier between them, and meet in LDS at the end.  In larger tiles a
+// step's operands serve two waves of two row tiles each, so that a group of 16 requests with four heads a kv head costs what one of them does;
+// the two share a SIMD, where the matrix instructions of one run under the exponentials of the other.
+#include "sp_chunk.h"
+#include "sp_ring.h"
+#include "sp_shared_plan.h"
+
+#define SH_WAVES 4  // that share the keys
+#define SH_THREADS (2 * SH_WAVES * SP_WAVE)
+// Octaves by which a row's logits may pass its running maximum before that is moved and what has been summed is scaled: nearly all steps go without.
+// (Probabilities up to 2^7 are as exact in bf16 as those below 1.)
+#define SH_SLACK 7.f
+
+struct ShArgs {
+  const sp_bf16 *q, *k, *v;
+  const int32_t *table, *lens, *cu, *shared, *groups;  // shared: keys of a group, [n_groups]; groups: first requests, [n_groups + 1]
+  sp_bf16* out;
+  int64_t table_stride, sq_n, sq_h, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;  // elements; _p between pages
+  int batch, tokens, width, num_pages, shift, n_groups;
+  int hkv, group, dense;      // dense: single tokens, an item each
+  PgDivisor by_group;
+  int shared_slots, slots;    // items of groups, items in all
+  int parts;                  // of the line at most, and workgroups of a kv head
+  float scale_log2;
+  float* o_part;              // [part][kv head][2][SH_TILE][D]: an item that began in an earlier part, one that goes on in the next
+  float2* ml_part;            // [part][kv head][2][SH_TILE]
+  float* o_row;               // [2][token][query head][D]: items that lie in one part, of groups and of requests
+  float2* ml_row;
+  int64_t* starts;            // [slots + 1]: the items' first units
+  int4* of_request;           // [batch + 1]: first own key, group, the group's first token, the request's first token
+  float* weights;             // null, or [num_pages][kv head][page]
+  float* logits;              // [num_pages][query head][page]: scaled logits of own keys, in octaves
+};
+
+template <int D>
+using ShShape = DsShape<D, D / 16, SH_WAVES, 128>;
+// LDS: the rings, where the waves meet afterwards; their maxima and sums; what is known of the requests and groups
+#define SH_RING 131072
+#define SH_ML (SH_RING)                                      // [2][SH_WAVES][SH_TILE] floats
+#define SH_FOUND (SH_ML + 2 * SH_WAVES * SH_TILE * 4)        // 80 bytes
+#define SH_ARRAYS (SH_FOUND + 80)
+static size_t sh_lds_bytes(int batch, int groups) { return SH_ARRAYS + ((size_t)3 * (batch + 1) + 2 * ((size_t)groups + 1)) * sizeof(int); }
+static_assert(ShShape<128>::LDS_BYTES <= SH_RING && ShShape<64>::LDS_BYTES <= SH_RING && SH_WAVES * SH_TILE * 128 * 4 <= SH_RING, "");
+
+struct ShItem {
+  int table_row;    // of the block table
+  int start;        // first token of the rows
+  int row0, rows;   // first row of the tile, rows from token `start` on
+  int key0, key1;   // keys that some row sees
+  int pos;          // position of token `start`: its row and the following ones see keys up to pos, pos + 1, ..; groups: far behind the last key
+  int lo, n;        // first step, steps
+};
+
+template <int D>
+__global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a) {
+  using Shape = ShShape<D>;
+  constexpr int CT = Shape::CT, KS = D / 32, WAVES = SH_WAVES, NB = Shape::NB;
+  constexpr int CHUNKS = D / 8, ROWS = SP_WAVE / CHUNKS;  // of a row; rows of a load instruction
+  constexpr int HALF = 16 / ROWS;                         // instructions of 16 keys
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lq = lane & 15, gr = lane >> 4;  // head (or key row, channel) in a 16-wide tile, lane group
+  const int g = a.group, kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv;
+  const int room = a.width << a.shift;
+
+  // ---- requests and groups ----
+  int* const start_s = reinterpret_cast<int*>(lds + SH_ARRAYS);  // [batch + 1] first tokens
+  int* const len_s = start_s + a.batch + 1;                      // [batch]
+  int* const first_s = len_s + a.batch + 1;                      // [batch] first own key
+  int* const group_s = first_s + a.batch + 1;                    // [n_groups + 1] first requests
+  int* const shared_s = group_s + a.n_groups + 1;                // [n_groups] shared keys, 0: nobody takes part
+  int back = 0;
+  for (int i = t; i <= a.batch; i += SH_THREADS) {
+    auto start = [&](int j) { return a.cu != nullptr ? pg_max(0, pg_min(a.cu[j], a.tokens)) : j; };
+    start_s[i] = start(i);
+    if (i < a.batch) len_s[i] = pg_max(0, pg_min(a.lens[i], PG_MAX_KEYS)), back |= start(i + 1) < start(i);
+  }
+  for (int i = a.n_groups > 0 ? t : 1; i <= a.n_groups; i += SH_THREADS) {
+    auto first = [&](int j) { return pg_max(0, pg_min(a.groups[j], a.batch)); };
+    group_s[i] = first(i);
+    if (i < a.n_groups) shared_s[i] = 0, back |= first(i + 1) < first(i);
+  }
+  // (offsets that go back count as the largest in front of them: searches need them in order)
+  if (__syncthreads_or(back)) {
+    if (t == 0) {
+      for (int i = 1; i <= a.batch; ++i) start_s[i] = pg_max(start_s[i], start_s[i - 1]);
+      for (int i = 1; i <= a.n_groups; ++i) group_s[i] = pg_max(group_s[i], group_s[i - 1]);
+    }
+    __syncthreads();
+  }
+  const bool tell = blockIdx.x == 0;
+  for (int b = t; b < a.batch; b += SH_THREADS) {
+    int4 what = make_int4(0, 0, 0, start_s[b]);
+    if (a.n_groups > 0) {
+      const int i = pg_holder(group_s, a.n_groups, b);
+      if (group_s[i] <= b && b < group_s[i + 1]) {
+        const int shared = pg_max(0, pg_min(a.shared[i], room));
+        what.x = sh_first_own(len_s[b], start_s[b + 1] - start_s[b], shared);
+        what.y = i, what.z = start_s[group_s[i]];
+        if (what.x > 0 && start_s[b + 1] > start_s[b]) shared_s[i] = shared;  // (the same from all)
+      }
+    }
+    first_s[b] = what.x;
+    if (tell) a.of_request[b] = what;
+  }
+  if (tell && t == 0) a.of_request[a.batch] = make_int4(0, 0, 0, start_s[a.batch]);
+  __syncthreads();
+
+  // ---- items, and which of them fall to this workgroup ----
+  auto item = [&](int x, ShItem& p) {  // false: there is none of this number, or it has no keys
+    if (x < a.shared_slots) {
+      int i = 0, hi = a.n_groups;
+      while (hi - i > 1) {
+        const int mid = (i + hi) >> 1;
+        if (pg_first_slot(start_s[group_s[mid]], g, mid, SH_TILE) <= x)
+          i = mid;
+        else
+          hi = mid;
+      }
+      p.table_row = pg_min(group_s[i], a.batch - 1);
+      p.start = start_s[group_s[i]];
+      p.rows = (start_s[group_s[i + 1]] - p.start) * g;
+      p.row0 = (x - (int)pg_first_slot(p.start, g, i, SH_TILE)) * SH_TILE;
+      if (p.row0 < 0 || p.row0 >= p.rows) return false;
+      p.key0 = 0, p.key1 = shared_s[i], p.pos = PG_MAX_KEYS;
+    } else {
+      const int y = x - a.shared_slots;
+      int b = y;
+      if (!a.dense) {
+        b = 0;
+        int hi = a.batch;
+        while (hi - b > 1) {
+          const int mid = (b + hi) >> 1;
+          if (pg_first_slot(start_s[mid], g, mid, SH_TILE) <= y)
+            b = mid;
+          else
+            hi = mid;
+        }
+      }
+      const int q_len = start_s[b + 1] - start_s[b];
+      p.table_row = b;
+      p.start = start_s[b];
+      p.rows = q_len * g;
+      p.row0 = (y - (int)sh_own_slot(p.start, g, b, a.dense)) * SH_TILE;
+      if (p.row0 < 0 || p.row0 >= p.rows) return false;
+      p.pos = len_s[b] - q_len;
+      p.key0 = first_s[b];
+      p.key1 = pg_min(p.pos + (int)pg_div((unsigned)(pg_min(p.row0 + SH_TILE, p.rows) - 1), a.by_group) + 1, room);
+    }
+    p.lo = p.key0 / SH_KEYS;
+    p.n = p.key1 > p.key0 ? (p.key1 + SH_KEYS - 1) / SH_KEYS - p.lo : 0;
+    return p.n > 0;
+  };
+  int64_t* const found_s = reinterpret_cast<int64_t*>(lds + SH_FOUND);  // the waves' sums; then the first item's start
+  int* const item_s = reinterpret_cast<int*>(lds + SH_FOUND + 72);
+  int64_t cut0, cut1, at_unit;
+  int x, near;
+  {
+    const int per = (a.slots + SH_THREADS - 1) / SH_THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
+    ShItem p;
+    int64_t mine = 0;
+    for (int i = x0; i < x1; ++i) mine += item(i, p) ? p.n + SH_OVERHEAD : 0;
+    int64_t at = mine;
+#pragma unroll
+    for (int o = 1; o < SP_WAVE; o <<= 1) {
+      const int64_t y = __shfl_up(at, o, SP_WAVE);
+      if (lane >= o) at += y;
+    }
+    if (lane == SP_WAVE - 1) found_s[wave] = at;
+    __syncthreads();
+    int64_t total = 0;
+#pragma unroll
+    for (int w = 0; w < 2 * WAVES; ++w) {
+      if (w == wave) at += total;
+      total += found_s[w];
+    }
+    at -= mine;
+    const int64_t parts = pg_parts(total, a.parts, SH_MIN_SHARE);
+    near = pg_near(total, parts);
+    cut0 = part < parts ? pg_cut(total, parts, part) : total;
+    cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
+    if (t == 0) item_s[0] = a.slots;
+    __syncthreads();
+    if (tell || (cut0 < cut1 && cut0 >= at && cut0 < at + mine)) {
+      for (int i = x0; i < x1; ++i) {
+        const int units = item(i, p) ? p.n + SH_OVERHEAD : 0;
+        if (tell) a.starts[i] = at;
+        if (cut0 >= at && cut0 < at + units) item_s[0] = i, found_s[8] = at;
+        at += units;
+      }
+    }
+    if (tell && t == 0) a.starts[a.slots] = total;
+    __syncthreads();
+    x = __builtin_amdgcn_readfirstlane(item_s[0]);
+    at_unit = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)found_s[8]) | (int64_t)__builtin_amdgcn_readfirstlane((int)(found_s[8] >> 32)) << 32;
+  }
+
+  // Arguments of what is done once an item are read where they are used: scalar registers do not suffice to keep them.
+  const auto kernel_args = (const __attribute__((address_space(4))) ShArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  auto args = [&] {
+    auto p = kernel_args;
+    asm volatile("" : "+s"(p));
+    return p;
+  };
+  const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
+  const int slot = wave % WAVES, half = wave / WAVES;  // the wave's keys of a block, and its rows where two waves share them
+  const uint32_t ring = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds + slot * NB * Shape::STEP_BYTES;
+  const uint32_t k_at = ring + lq * (D * 2);
+  const int v_key = 4 * gr + (lq >> 2);  // row of the transposing read; 16 rows further the swizzle is the same
+  const uint32_t v_at = ring + Shape::K_BYTES + v_key * (CT * 32) + 8 * (lq & 3);
+  float* const m_s = reinterpret_cast<float*>(lds + SH_ML);
+  float* const l_s = m_s + WAVES * SH_TILE;
+
+  // RT: row tiles of 16 of a wave.  One: waves 0 .. 3 with a ring each.  Two: the waves of a slot have 32 rows each of its keys, one loads K and the other V, and
+  // all meet at a barrier every block of four steps.
+  auto run = [&](auto tiles, const ShItem& p, int begin, int s_end, bool of_group) {
+    constexpr int RT = decltype(tiles)::value;
+    constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
+    const int tile_row = RT == 1 ? 0 : 16 * RT * half;  // the wave's first row in the tile
+    auto row_of = [&](int in_tile, int* token, int* head) {
+      const int r = pg_min(p.row0 + in_tile, p.rows - 1);
+      *token = (int)pg_div((unsigned)r, a.by_group);
+      *head = kvh * g + (r - *token * g);
+    };
+    dc_bf16x8 qb[RT][KS];
+    int pos[RT];  // last key that the lane's rows see
+    {
+      const auto r = args();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        int token, head;
+        row_of(tile_row + 16 * rt + lq, &token, &head);
+        pos[rt] = p.pos + token;
+        const sp_bf16* src = r->q + (int64_t)(p.start + token) * r->sq_n + (int64_t)head * r->sq_h + 8 * gr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qb[rt][ks] = *reinterpret_cast<const dc_bf16x8*>(src + 32 * ks);
+      }
+    }
+    const int pos0 = p.pos + (int)pg_div((unsigned)p.row0, a.by_group);  // of the tile's first row
+    const char* const kh = (const char*)(a.k + kvh * a.sk_h);
+    const char* const vh = (const char*)(a.v + kvh * a.sv_h);
+    // (scalar loads: nothing writes the table during the launch)
+    const auto table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.table + (int64_t)p.table_row * a.table_stride);
+    struct Ids {
+      int id[2];
+    };
+    auto entries = [&](int s) {  // pages of a step's halves
+      Ids e;
+      const int key0 = (p.lo + s) * SH_KEYS;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) e.id[h] = table[pg_min((key0 + 16 * h) >> a.shift, a.width - 1)];
+      return e;
+    };
+    auto low = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+    // A step's loads, K's or V's or both, and which of its keys any row sees: the others are zeros, without a read, whatever stands there.
+    auto fetch = [&](int buf, int s, Ids ids) {
+      const int key0 = (p.lo + s) * SH_KEYS;
+      uint32_t seen = low(p.key1 - key0) & ~low(p.key0 - key0);
+      const uint32_t at = ring + buf * Shape::STEP_BYTES;
+      int64_t id[2];
+      int in[2], there[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = key0 + 16 * h;
+        const int page = key >> a.shift < a.width && (unsigned)ids.id[h] < (unsigned)a.num_pages ? ids.id[h] : -1;
+        in[h] = key & ((1 << a.shift) - 1);
+        there[h] = page < 0 ? 0 : pg_max(0, pg_min(p.key1 - key, 16));
+        if (page < 0) seen &= h == 0 ? 0xffff0000u : 0x0000ffffu;
+        id[h] = pg_max(page, 0);
+      }
+      auto load = [&](const char* from, int64_t page_bytes, uint32_t row_bytes, uint32_t to, auto&& chunk) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(from + id[h] * page_bytes + (uint64_t)(uint32_t)in[h] * row_bytes), 0,
+              there[h] > 0 ? (int)((uint32_t)(there[h] - 1) * row_bytes + 2u * D) : 0, 0x00027000);
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) {
+            const int row = i * ROWS + lane / CHUNKS;
+            uint32_t off = (uint32_t)row * row_bytes + 16u * (uint32_t)chunk(16 * h + row);
+            off = (seen >> (16 * h + row)) & 1u ? off : 0x7ffffff0u;  // (past the buffer's end: zeros)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ds_lds_ptr)(uintptr_t)(to + (h * HALF + i) * 1024), 16, (int)off, 0, 0, 0);
+          }
+        }
+      };
+      if (RT == 1 || half == 0) load(kh, a.sk_p * 2, k_row, at, [&](int row) { return (lane % CHUNKS) ^ ds_swz_k<D>(row); });
+      if (RT == 1 || half == 1) load(vh, a.sv_p * 2, v_row, at + Shape::K_BYTES, [&](int row) { return (lane % CHUNKS) ^ (2 * ds_swz_v<CT>(row)); });
+      return seen;
+    };
+
+    ds_floatx4 o[RT][CT];
+    float m[RT], l[RT];  // of the lane's rows; l: this lane group's keys
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[rt][ct] = (ds_floatx4){0, 0, 0, 0};
+      m[rt] = -INFINITY, l[rt] = 0.f;
+    }
+
+    // one step of the wave: its operands lie at `off` of its ring, `mine` says which keys are seen
+    auto step = [&](int s, uint32_t mine, uint32_t off) {
+      dc_u32x4 kr[2][KS];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) kr[i][ks] = ds_read_k(k_at + off + i * 16 * (D * 2) + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4));
+      if constexpr (KS == 4)
+        asm volatile("s_waitcnt lgkmcnt(0)"
+                     : "+v"(kr[0][0]), "+v"(kr[0][1]), "+v"(kr[0][2]), "+v"(kr[0][3]), "+v"(kr[1][0]), "+v"(kr[1][1]), "+v"(kr[1][2]), "+v"(kr[1][3]));
+      else
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(kr[0][0]), "+v"(kr[0][1]), "+v"(kr[1][0]), "+v"(kr[1][1]));
+      ds_floatx4 sc[RT][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          sc[rt][i] = (ds_floatx4){0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            sc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, kr[i][ks]), qb[rt][ks], sc[rt][i], 0, 0, 0);
+        }
+      const int key0 = (p.lo + s) * SH_KEYS;
+      const uint32_t bits = mine >> (4 * gr);  // the lane's keys: 16 i + 4 gr + j
+      const bool partly = pg_min(key0 + SH_KEYS, p.key1) - 1 > pos0;  // (uniform: some row does not see a key that others see)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[rt][i][j] *= a.scale_log2;
+      if (mine != ~0u) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[rt][i][j] = bits & (1u << (16 * i + j)) ? sc[rt][i][j] : -INFINITY;
+      }
+      if (partly) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[rt][i][j] = key0 + 4 * gr + 16 * i + j <= pos[rt] ? sc[rt][i][j] : -INFINITY;
+      }
+      if constexpr (RT == 1) {  // the logits themselves, for the keys' weights
+        if (a.weights != nullptr && !of_group) {
+          const auto r = args();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int key = key0 + 16 * i + 4 * gr, page = table[pg_min((key0 + 16 * i) >> a.shift, a.width - 1)];
+            if (((mine >> (16 * i)) & 0xffffu) != 0u && lq < g)  // (no page: no key of it is seen)
+              *reinterpret_cast<ds_floatx4*>(r->logits + (((int64_t)page * a.hkv + kvh) * g + lq) * (1 << a.shift) + (key & ((1 << a.shift) - 1))) = sc[0][i];
+          }
+        }
+      }
+      float mx[RT];
+      bool moves = false;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        mx[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
+                       fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
+        mx[rt] = ds_quad_max(mx[rt]);
+        moves |= mx[rt] > m[rt] + SH_SLACK;
+      }
+      // (a row that has seen no finite logit: m is -inf, every weight exp2(-inf) = 0)
+      if (__ballot(moves) != 0ull) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float to = fmaxf(m[rt], mx[rt]), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
+          m[rt] = to;
+          l[rt] *= alpha;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) o[rt][ct] *= alpha;
+        }
+      }
+      // V is asked for here, under the exponentials: no branch lies between these reads and the wait for them
+      ds_u32x2 vr[CT][2];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        const uint32_t at = v_at + off + ((ct ^ ds_swz_v<CT>(v_key)) << 5);
+        vr[ct][0] = ds_read_v<0>(at);
+        vr[ct][1] = ds_read_v<16 * CT * 32>(at);
+      }
+      dc_bf16x8 ph[RT], pl[1];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float base = m[rt] == -INFINITY ? 0.f : m[rt];
+        uint32_t hi[4], lw[4];
+        float add = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(sc[rt][i][j] - base), p1 = __builtin_amdgcn_exp2f(sc[rt][i][j + 1] - base);
+            const uint32_t w = dc_pack2(p0, p1);
+            hi[2 * i + j / 2] = w;
+            const float q0 = __uint_as_float(w << 16), q1 = __uint_as_float(w & 0xffff0000u);
+            if constexpr (TWO) {
+              lw[2 * i + j / 2] = dc_pack2(p0 - q0, p1 - q1);
+              add += p0 + p1;
+            } else {
+              add += q0 + q1;  // (of what the product takes: an output is a mean of values, whatever its weights' roundings)
+            }
+          }
+        l[rt] += add;
+        ph[rt] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){hi[0], hi[1], hi[2], hi[3]});
+        if constexpr (TWO) pl[0] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){lw[0], lw[1], lw[2], lw[3]});
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[ct][0]), "+v"(vr[ct][1]));
+      // Where a row does not see a key, 0 times a value that is no number would make a NaN of its sum: the product takes zeros in such places, and rows
+      // that do see such a key have a sum of weights that is none.
+      if (partly) {
+        uint32_t odd[2] = {0u, 0u};  // exponents of ones, of the lane's keys 16 h + 4 gr + 0 .. 3: bits 15, 31 of words 0 and 1
+        uint32_t any = 0u;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) any |= ((vr[ct][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        if (__ballot(any != 0u) != 0ull) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t here = 0u;
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct) {
+                const uint32_t ones = ((vr[ct][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                here |= ones;
+                vr[ct][h][e] &= ~((ones >> 15) * 0xffffu);
+              }
+              odd[h] |= here >> (15 * e);  // (keys 2 e and 2 e + 1: bits 15 - 15 e and 31 - 15 e)
+            }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int by = 1; by < 16; by <<= 1) odd[h] |= __shfl_xor(odd[h], by, SP_WAVE);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if ((odd[h] >> (15 - 15 * (j >> 1) + 16 * (j & 1))) & 1u) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                  if (key0 + 16 * h + 4 * gr + j <= pos[rt]) l[rt] = __builtin_nanf("");
+              }
+          }
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, __builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3)),
+                                                              ph[rt], o[rt][ct], 0, 0, 0);
+      if constexpr (TWO) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+          o[0][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(dc_bf16x8, ds_finite(__builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3))), pl[0], o[0][ct], 0, 0, 0);
+      }
+    };
+
+    __syncthreads();  // the rings are free
+    if constexpr (RT == 1) {
+      if (half == 0) {
+        const int s0 = begin + wave;
+        uint32_t seen[NB - 1];
+#pragma unroll
+        for (int i = 0; i < NB - 1; ++i) {
+          seen[i] = 0;
+          if (s0 + i * WAVES < s_end) seen[i] = fetch(i, s0 + i * WAVES, entries(s0 + i * WAVES));
+        }
+        Ids next = {{0, 0}};
+        if (s0 + (NB - 1) * WAVES < s_end) next = entries(s0 + (NB - 1) * WAVES);
+        int buf = 0;
+        for (int s = s0; s < s_end; s += WAVES) {
+          // the step's loads have landed, those of the NB - 2 behind it stay in flight (what is asked for returns in order)
+          if (s + (NB - 2) * WAVES < s_end)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * Shape::LOADS) : "memory");
+          else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          const uint32_t mine = seen[0];
+#pragma unroll
+          for (int i = 0; i + 1 < NB - 1; ++i) seen[i] = seen[i + 1];
+          // (the place that is filled here was read in the step before: those reads' results have been used)
+          if (s + (NB - 1) * WAVES < s_end) {
+            seen[NB - 2] = fetch(buf == 0 ? NB - 1 : buf - 1, s + (NB - 1) * WAVES, next);
+            if (s + NB * WAVES < s_end) next = entries(s + NB * WAVES);
+          }
+          step(s, mine, buf * Shape::STEP_BYTES);
+          buf = buf + 1 == NB ? 0 : buf + 1;
+        }
+      }
+    } else {
+      const int blocks = (s_end - begin + WAVES - 1) / WAVES;
+      const int s0 = begin + slot;
+      uint32_t seen = 0, seen_next = 0;
+      if (s0 < s_end) seen_next = fetch(0, s0, entries(s0));
+      Ids next = {{0, 0}};
+      if (s0 + WAVES < s_end) next = entries(s0 + WAVES);
+      for (int i = 0; i < blocks; ++i) {
+        // everybody's loads of this block have landed, and everybody is past the block in front, whose place the next one's take
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        const int s = s0 + i * WAVES;
+        seen = seen_next;
+        if (s + WAVES < s_end) {
+          seen_next = fetch((i + 1) & 1, s + WAVES, next);
+          if (s + 2 * WAVES < s_end) next = entries(s + 2 * WAVES);
+        }
+        if (s < s_end) step(s, seen, (i & 1) * Shape::STEP_BYTES);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l[rt] = ds_quad_sum(l[rt]);
+    __syncthreads();  // the rings are free
+    // [slot][SH_TILE][D] floats, 16-byte pieces swizzled by the row
+    float* const o_s = reinterpret_cast<float*>(lds);
+    if (RT > 1 || half == 0) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = slot * SH_TILE + tile_row + 16 * rt + lq;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<ds_floatx4*>(o_s + r * D + ((4 * ct + gr) ^ lq) * 4) = o[rt][ct];
+        if (gr == 0) m_s[r] = m[rt], l_s[r] = l[rt];
+      }
+    }
+    __syncthreads();
+    const auto to_args = args();
+    const bool whole = begin == 0 && s_end == p.n;
+    const int rows = pg_min(p.rows - p.row0, RT == 1 ? 16 : SH_TILE);
+    const int64_t slab = ((int64_t)(part * a.hkv + kvh) * 2 + (begin == 0 ? 1 : 0)) * SH_TILE;
+    const bool final = whole && p.key0 == 0 && !of_group;
+    for (int i = t; i < rows * (D / 4); i += SH_THREADS) {
+      const int r = i / (D / 4), c = i % (D / 4);
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, m_s[w * SH_TILE + r]);
+      ds_floatx4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float mw = m_s[w * SH_TILE + r];
+        const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);  // (a wave without keys, or without a finite logit: 0)
+        sum += l_s[w * SH_TILE + r] * f;
+        acc += *reinterpret_cast<const ds_floatx4*>(o_s + (w * SH_TILE + r) * D + (c ^ (r & 15)) * 4) * f;
+      }
+      int token, head;
+      row_of(r, &token, &head);
+      const int64_t row = (int64_t)(p.start + token) * (a.hkv * g) + head;
+      if (final) {
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // (a row without keys: zeros)
+        *reinterpret_cast<uint2*>(to_args->out + row * D + 4 * c) = make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
+      }
+      if (!final || a.weights != nullptr) {
+        const int64_t to = whole ? (of_group ? 0 : (int64_t)a.tokens * (a.hkv * g)) + row : slab + r;
+        if (!final) *reinterpret_cast<ds_floatx4*>((whole ? to_args->o_row : to_args->o_part) + to * D + 4 * c) = acc;
+        if (c == 0) (whole ? to_args->ml_row : to_args->ml_part)[to] = make_float2(fmaxf(top, CK_NO_MAX), sum);
+      }
+    }
+  };
+
+  for (ShItem p; x < a.slots && at_unit < cut1; ++x) {
+    if (!item(x, p)) continue;
+    int begin, end;
+    sh_steps(at_unit, p.n, cut0, cut1, near, &begin, &end);
+    at_unit += p.n + SH_OVERHEAD;
+    if (begin >= end) continue;
+    ShItem u;  // (uniform: out of vector registers)
+    u.table_row = __builtin_amdgcn_readfirstlane(p.table_row), u.start = __builtin_amdgcn_readfirstlane(p.start);
+    u.row0 = __builtin_amdgcn_readfirstlane(p.row0), u.rows = __builtin_amdgcn_readfirstlane(p.rows);
+    u.key0 = __builtin_amdgcn_readfirstlane(p.key0), u.key1 = __builtin_amdgcn_readfirstlane(p.key1);
+    u.pos = __builtin_amdgcn_readfirstlane(p.pos), u.lo = __builtin_amdgcn_readfirstlane(p.lo), u.n = __builtin_amdgcn_readfirstlane(p.n);
+    begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
+    if (u.rows - u.row0 <= 16)
+      run(std::integral_constant<int, 1>{}, u, begin, end, x < a.shared_slots);
+    else
+      run(std::integral_constant<int, SH_TILE / 32>{}, u, begin, end, x < a.shared_slots);
+  }
+}
+
+// ---- joining ----------------------------------------------------------------------------------------------------
+// What the parts of an item left of a row: visit(row of ml_part / o_part, row of ml_row / o_row, whole).
+struct ShLine {
+  int64_t total, parts;
+  int near;
+};
+__device__ __forceinline__ ShLine sh_line(const ShArgs& a) {
+  ShLine s;
+  s.total = a.starts[a.slots];
+  s.parts = s.total > 0 ? pg_parts(s.total, a.parts, SH_MIN_SHARE) : 0;
+  s.near = s.total > 0 ? pg_near(s.total, s.parts) : 0;
+  return s;
+}
+struct ShParts {  // of an item
+  int64_t start, first;
+  int n, count;  // steps; parts that may hold some of them
+};
+__device__ __forceinline__ ShParts sh_parts(const ShArgs& a, const ShLine& s, int x) {
+  ShParts p = {a.starts[x], 0, 0, 0};
+  const int64_t end = a.starts[x + 1];
+  if (end == p.start) return p;
+  p.n = (int)(end - p.start) - SH_OVERHEAD;
+  p.first = sh_part(p.start, s.total, s.parts);
+  p.count = (int)(sh_part(end - 1, s.total, s.parts) - p.first) + 1;
+  return p;
+}
+// Place i of an item's parts holds steps of it: where a row (of kv head kvh, place `in_tile` of its tile, number `row` among all) stands; < 0: it holds none.
+// Rows of ml_part come first, those of ml_row behind them.
+#define SH_NOWHERE (-1)
+__device__ __forceinline__ int64_t sh_place(const ShArgs& a, const ShLine& s, const ShParts& p, int i, int kvh, int in_tile, int64_t row, bool of_group,
+                                            bool* whole) {
+  int begin, end;
+  const int64_t part = p.first + i;
+  sh_steps(p.start, p.n, pg_cut(s.total, s.parts, part), pg_cut(s.total, s.parts, part + 1), s.near, &begin, &end);
+  *whole = begin == 0 && end == p.n;
+  if (begin >= end) return SH_NOWHERE;
+  if (*whole) return (of_group ? 0 : (int64_t)a.tokens * (a.hkv * a.group)) + row;
+  return ((part * a.hkv + kvh) * 2 + (begin == 0 ? 1 : 0)) * SH_TILE + in_tile;
+}
+// the items of a row: its group's (-1: it takes part in none) and its request's, and its places in their tiles
+struct ShRow {
+  int item[2], in_tile[2];
+};
+__device__ __forceinline__ ShRow sh_row(const ShArgs& a, int b, int4 what, int token, int h) {
+  ShRow r;
+  const int in_group = (token - what.z) * a.group + h, in_own = (token - what.w) * a.group + h;
+  r.item[0] = what.x > 0 ? (int)pg_first_slot(what.z, a.group, what.y, SH_TILE) + in_group / SH_TILE : -1;
+  r.in_tile[0] = in_group % SH_TILE;
+  r.item[1] = a.shared_slots + (int)sh_own_slot(what.w, a.group, b, a.dense) + in_own / SH_TILE;
+  r.in_tile[1] = in_own % SH_TILE;
+  return r;
+}
+
+#define SM_THREADS 256
+// A row's parts joined, D / 4 threads a row, and behind those workgroups, where weights are kept, one for every part of the line:
+//   weight[j] += sum over the group's heads of 2^(logit - m) / l for the own keys that fall to the part.
+template <int D>
+__global__ __launch_bounds__(SM_THREADS) void sp_shared_join_kernel(const ShArgs a, int join_blocks) {
+  const int t = threadIdx.x;
+  const int hq = a.hkv * a.group;
+  const ShLine line = sh_line(a);
+  if ((int)blockIdx.x < join_blocks) {
+    constexpr int WIDTH = D / 4, PER = SM_THREADS / WIDTH;
+    const int64_t row = (int64_t)blockIdx.x * PER + t / WIDTH;
+    const int c = t % WIDTH * 4;
+    if (row >= (int64_t)a.tokens * hq) return;
+    const int token = (int)(row / hq), head = (int)(row % hq), kvh = head / a.group;
+    int b = token;
+    if (a.cu != nullptr) {
+      b = 0;
+      int hi = a.batch;
+      while (hi - b > 1) {
+        const int mid = (b + hi) >> 1;
+        if (a.of_request[mid].w <= token)
+          b = mid;
+        else
+          hi = mid;
+      }
+    }
+    const int4 what = a.of_request[b];
+    if (token < what.w || token >= a.of_request[b + 1].w) return;  // (a row outside every request)
+    const ShRow r = sh_row(a, b, what, token, head - kvh * a.group);
+    float top = CK_NO_MAX, sum = 0.f;
+    ds_floatx4 acc = {0, 0, 0, 0};
+    for (int which = 0; which < 2; ++which) {
+      if (r.item[which] < 0) continue;
+      const ShParts p = sh_parts(a, line, r.item[which]);
+#pragma unroll 4
+      for (int i = 0; i < p.count; ++i) {
+        bool whole;
+        const int64_t at = sh_place(a, line, p, i, kvh, r.in_tile[which], row, which == 0, &whole);
+        if (at < 0) continue;
+        if (whole && which == 1 && what.x == 0) return;  // (the row is done)
+        const float2 ml = (whole ? a.ml_row : a.ml_part)[at];
+        const ds_floatx4 o = *reinterpret_cast<const ds_floatx4*>((whole ? a.o_row : a.o_part) + at * D + c);
+        const float to = fmaxf(top, ml.x), f0 = __builtin_amdgcn_exp2f(top - to), f1 = __builtin_amdgcn_exp2f(ml.x - to);
+        sum = sum * f0 + ml.y * f1;
+        acc = acc * f0 + o * f1;
+        top = to;
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    *reinterpret_cast<uint2*>(a.out + row * D + c) = make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
+    return;
+  }
+  // ---- weights of the own keys between two cuts (single tokens) ----
+  __shared__ float m_s[PD_MAX_GROUP], inv_s[PD_MAX_GROUP];
+  const int w = blockIdx.x - join_blocks, kvh = w % a.hkv, part = w / a.hkv, lane = t & 63, wave = t >> 6;
+  if (part >= line.parts) return;
+  const int64_t cut0 = pg_cut(line.total, line.parts, part), cut1 = pg_cut(line.total, line.parts, part + 1);
+  int x = a.shared_slots, hi = a.slots;
+  while (hi - x > 1) {  // the last request's item that starts at or in front of the cut
+    const int mid = (x + hi) >> 1;
+    if (a.starts[mid] <= cut0)
+      x = mid;
+    else
+      hi = mid;
+  }
+  for (; x < a.slots && a.starts[x] < cut1; ++x) {
+    const ShParts p = sh_parts(a, line, x);
+    if (p.count == 0) continue;
+    int begin, end;
+    sh_steps(p.start, p.n, cut0, cut1, line.near, &begin, &end);
+    if (begin >= end) continue;
+    const int b = x - a.shared_slots;
+    const int4 what = a.of_request[b];
+    const int len = pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS)), room = a.width << a.shift;
+    __syncthreads();  // (the rows before are done with)
+    for (int h = wave; h < a.group; h += SM_THREADS / SP_WAVE) {  // a lane a part
+      const ShRow r = sh_row(a, b, what, b, h);
+      float top = CK_NO_MAX, sum = 0.f;
+      for (int which = 0; which < 2; ++which) {
+        if (r.item[which] < 0) continue;
+        const ShParts q = sh_parts(a, line, r.item[which]);
+        for (int i0 = 0; i0 < q.count; i0 += SP_WAVE) {
+          float2 ml = make_float2(CK_NO_MAX, 0.f);
+          bool whole;
+          const int64_t at = i0 + lane < q.count ? sh_place(a, line, q, i0 + lane, kvh, r.in_tile[which], (int64_t)b * hq + kvh * a.group + h, which == 0, &whole)
+                                                 : SH_NOWHERE;
+          if (at >= 0) ml = (whole ? a.ml_row : a.ml_part)[at];
+          const float to = fmaxf(top, sp_wave_max(ml.x));
+          sum = sum * __builtin_amdgcn_exp2f(top - to) + sp_wave_sum(at >= 0 ? ml.y * __builtin_amdgcn_exp2f(ml.x - to) : 0.f);
+          top = to;
+        }
+      }
+      if (lane == 0) m_s[h] = top, inv_s[h] = sum == 0.f ? 0.f : 1.0f / sum;
+    }
+    __syncthreads();
+    const int lo = what.x / SH_KEYS, first = (lo + begin) * SH_KEYS, last = pg_min(pg_min((lo + end) * SH_KEYS, len), room);
+    for (int key = first + 4 * t; key < last; key += 4 * SM_THREADS) {
+      const int id = a.table[b * a.table_stride + (key >> a.shift)], in = key & ((1 << a.shift) - 1);
+      if ((unsigned)id >= (unsigned)a.num_pages) continue;
+      ds_floatx4 sum = {0, 0, 0, 0};
+      for (int h = 0; h < a.group; ++h) {
+        const ds_floatx4 s = *reinterpret_cast<const ds_floatx4*>(a.logits + (((int64_t)id * a.hkv + kvh) * a.group + h) * (1 << a.shift) + in);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - m_s[h]) * inv_s[h];
+      }
+      float* const to = a.weights + id * a.sw_p + kvh * a.sw_h + in;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (key + j >= what.x && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------
+#define SH_PLACES 256  // workgroups that are resident at once: one a CU
+static int sh_workgroups(int64_t hkv) { return hkv < SH_PLACES ? SH_PLACES / (int)hkv : 1; }  // of a kv head
+
+struct ShSizes {
+  int64_t shared_slots, slots, logits;
+  size_t o_part, ml_part, o_row, ml_row, starts, of_request, bytes;
+};
+static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d, bool single, int64_t pool_keys) {
+  ShSizes s;
+  const int64_t g = hq / hkv;
+  s.shared_slots = groups > 0 ? tokens * g / SH_TILE + groups : 0;
+  s.slots = s.shared_slots + (single && g <= SH_TILE ? batch : tokens * g / SH_TILE + batch);
+  const int64_t rows = (int64_t)sh_workgroups(hkv) * hkv * 2 * SH_TILE;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t here = at;
+    at += (n + 255) / 256 * 256;
+    return here;
+  };
+  s.o_part = take((size_t)rows * d * sizeof(float));
+  s.ml_part = take((size_t)rows * sizeof(float2));
+  s.o_row = take(groups > 0 ? (size_t)(2 * tokens * hq) * d * sizeof(float) : 0);
+  s.ml_row = take((size_t)(2 * tokens * hq) * sizeof(float2));
+  s.starts = take((size_t)(s.slots + 1) * sizeof(int64_t));
+  s.of_request = take((size_t)(batch + 1) * sizeof(int4));
+  s.logits = (int64_t)take((size_t)pool_keys * hq * sizeof(float));
+  s.bytes = at;
+  return s;
+}
+static bool sh_shape_ok(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d) {
+  return tokens > 0 && batch > 0 && batch <= SH_MAX_SEQS && groups >= 0 && groups <= batch && hq > 0 && hkv > 0 && hq % hkv == 0 && (d == 64 || d == 128) &&
+         tokens <= PG_MAX_KEYS && hq <= 65536 && tokens * (hq / hkv) < (1ll << 31);
+}
+
+extern "C" size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t groups, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens,
+                                                 int64_t pool_keys) {
+  return sh_shape_ok(tokens, batch, groups, hq, hkv, d) && pool_keys >= 0 && pool_keys <= (1ll << 40)
+             ? sh_sizes(tokens, batch, groups, hq, hkv, d, single_tokens != 0, pool_keys).bytes
+             : 0;
+}
+
+extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
+  const char* who = "sp_shared_attn_bf16";
+  SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(x->hq > 0 && x->hkv > 0 && x->hq % x->hkv == 0, SP_ERR_INVALID_ARGUMENT, "%s: bad shape hq=%lld hkv=%lld", who, (long long)x->hq,
+             (long long)x->hkv);
+  SP_REQUIRE(x->d == 64 || x->d == 128, SP_ERR_UNSUPPORTED, "%s: head_dim %lld unsupported (64 or 128)", who, (long long)x->d);
+  SP_REQUIRE((float)x->softmax_scale > 0.f, SP_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be > 0", who);
+  SP_REQUIRE(x->batch > 0 && x->tokens >= 0 && x->table_width > 0 && x->num_pages > 0 && x->groups >= 0, SP_ERR_INVALID_ARGUMENT,
+             "%s: batch=%lld tokens=%lld table_width=%lld num_pages=%lld groups=%lld", who, (long long)x->batch, (long long)x->tokens,
+             (long long)x->table_width, (long long)x->num_pages, (long long)x->groups);
+  SP_REQUIRE(x->groups <= x->batch, SP_ERR_INVALID_ARGUMENT, "%s: %lld groups of %lld requests", who, (long long)x->groups, (long long)x->batch);
+  SP_REQUIRE(x->batch <= SH_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %lld (at most %d)", who, (long long)x->batch, SH_MAX_SEQS);
+  int shift = 4;
+  while (shift <= 10 && x->page_size != 1ll << shift) ++shift;
+  SP_REQUIRE(shift <= 10, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
+  SP_REQUIRE(x->tokens <= PG_MAX_KEYS && x->num_pages <= 0x7fffffffll && x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS,
+             SP_ERR_UNSUPPORTED, "%s: tokens=%lld num_pages=%lld table_width=%lld too large", who, (long long)x->tokens, (long long)x->num_pages,
+             (long long)x->table_width);
+  SP_REQUIRE(x->cu_q != nullptr || x->tokens == x->batch, SP_ERR_INVALID_ARGUMENT, "%s: without cu_q every sequence has one token (%lld for %lld)",
+             who, (long long)x->tokens, (long long)x->batch);
+  const int64_t g = x->hq / x->hkv;
+  SP_REQUIRE(x->weights == nullptr || (x->cu_q == nullptr && g <= PD_MAX_GROUP), SP_ERR_UNSUPPORTED,
+             "%s: weights go with single tokens of up to %d query heads a kv head", who, PD_MAX_GROUP);
+  if (x->tokens == 0) return SP_OK;
+  SP_REQUIRE(sh_shape_ok(x->tokens, x->batch, x->groups, x->hq, x->hkv, x->d), SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who,
+             (long long)x->tokens, (long long)x->hq);
+  const int64_t q_n = pg_used_stride(x->q_stride_n, x->tokens), q_h = pg_used_stride(x->q_stride_h, x->hq);
+  const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);
+  const int64_t v_p = pg_used_stride(x->v_stride_page, x->num_pages), v_h = pg_used_stride(x->v_stride_h, x->hkv);
+  const int64_t w_p = pg_used_stride(x->w_stride_page, x->num_pages), w_h = pg_used_stride(x->w_stride_h, x->hkv);
+  SP_REQUIRE(x->q && x->k_pages && x->v_pages && x->block_table && x->seq_lens && x->out && ((x->shared_lens && x->cu_groups) || x->groups == 0),
+             SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k_pages | (uintptr_t)x->v_pages | (uintptr_t)x->out) % 16 == 0 &&
+                 (q_n | q_h | k_p | k_h | v_p | v_h) % 8 == 0,
+             SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
+  for (const int64_t n : {x->k_stride_slot, x->v_stride_slot})
+    SP_REQUIRE(n >= 0 && n < (1ll << 24) && n * x->page_size < (1ll << 30) && n % 8 == 0, SP_ERR_UNSUPPORTED, "%s: slot stride %lld unsupported", who,
+               (long long)n);
+  const ShSizes s = sh_sizes(x->tokens, x->batch, x->groups, x->hq, x->hkv, x->d, x->cu_q == nullptr,
+                             x->weights != nullptr ? x->num_pages << shift : 0);
+  SP_REQUIRE(s.slots <= 0x7ffffff0ll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens, (long long)x->hq);
+  SP_REQUIRE(x->workspace != nullptr && x->workspace_bytes >= s.bytes && (uintptr_t)x->workspace % 16 == 0, SP_ERR_WORKSPACE,
+             "%s: workspace missing, too small or misaligned", who);
+  char* const ws = (char*)x->workspace;
+  ShArgs a = {};
+  a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k_pages, a.v = (const sp_bf16*)x->v_pages;
+  a.table = x->block_table, a.lens = x->seq_lens, a.cu = x->cu_q, a.shared = x->shared_lens, a.groups = x->cu_groups;
+  a.out = (sp_bf16*)x->out;
+  a.table_stride = x->table_stride, a.sq_n = q_n, a.sq_h = q_h;
+  a.sk_p = k_p, a.sk_n = x->k_stride_slot, a.sk_h = k_h, a.sv_p = v_p, a.sv_n = x->v_stride_slot, a.sv_h = v_h, a.sw_p = w_p, a.sw_h = w_h;
+  a.batch = (int)x->batch, a.tokens = (int)x->tokens, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
+  a.n_groups = (int)x->groups;
+  a.hkv = (int)x->hkv, a.group = (int)g, a.dense = x->cu_q == nullptr && g <= SH_TILE;
+  a.by_group = pg_divisor((unsigned)g);
+  a.shared_slots = (int)s.shared_slots, a.slots = (int)s.slots;
+  a.parts = sh_workgroups(x->hkv);
+  a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
+  a.o_part = (float*)(ws + s.o_part), a.ml_part = (float2*)(ws + s.ml_part), a.o_row = (float*)(ws + s.o_row), a.ml_row = (float2*)(ws + s.ml_row);
+  a.starts = (int64_t*)(ws + s.starts), a.of_request = (int4*)(ws + s.of_request);
+  a.weights = x->weights, a.logits = (float*)(ws + s.logits);
+  static bool attr_set[64] = {false};  // per device, once (idempotent)
+  int dev = 0;
+  SP_HIP(hipGetDevice(&dev));
+  SP_REQUIRE(dev >= 0 && dev < 64, SP_ERR_UNSUPPORTED, "%s: device index %d", who, dev);
+  if (!attr_set[dev]) {
+    for (const void* f : {(const void*)sp_shared_kernel<64>, (const void*)sp_shared_kernel<128>})
+      SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sh_lds_bytes(SH_MAX_SEQS, SH_MAX_SEQS)));
+    attr_set[dev] = true;
+  }
+  const hipStream_t stream = (hipStream_t)x->stream;
+  const int grid = a.parts * a.hkv;
+  const int64_t join = sp_ceil_div(x->tokens * x->hq, SM_THREADS / (x->d / 4));
+  SP_REQUIRE(join + grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens, (long long)x->hq);
+  const unsigned joins = (unsigned)(join + (a.weights != nullptr ? grid : 0));
+  const size_t lds = sh_lds_bytes(a.batch, a.n_groups);
+  if (x->d == 64) {
+    hipLaunchKernelGGL(sp_shared_kernel<64>, dim3((unsigned)grid), dim3(SH_THREADS), lds, stream, a);
+    hipLaunchKernelGGL(sp_shared_join_kernel<64>, dim3(joins), dim3(SM_THREADS), 0, stream, a, (int)join);
+  } else {
+    hipLaunchKernelGGL(sp_shared_kernel<128>, dim3((unsigned)grid), dim3(SH_THREADS), lds, stream, a);
+    hipLaunchKernelGGL(sp_shared_join_kernel<128>, dim3(joins), dim3(SM_THREADS), 0, stream, a, (int)join);
+  }
+  SP_LAUNCH_CHECK();
+  return SP_OK;
+}

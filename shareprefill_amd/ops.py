@@ -726,6 +726,69 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_
     return out
 
 
+def _check_weights(weights: torch.Tensor, pages: int, hkv: int, page_size: int, device) -> None:
+    if not (weights.dtype is torch.float32 and tuple(weights.shape) == (pages, hkv, page_size) and weights.get_device() == device.index
+            and weights.stride(2) == 1):
+        raise ValueError(f"weights must be float32 [{pages}, {hkv}, {page_size}] with a contiguous last axis on {device}")
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                            shared_lens: torch.Tensor, cu_groups: torch.Tensor, softmax_scale: float, cu_q: Optional[torch.Tensor] = None,
+                            weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention (without a window) where groups of requests have their first keys in common, which are read once for a group instead of once
+    for each of its requests.  Requests cu_groups[i] .. cu_groups[i + 1] - 1 are group i (int32 [G + 1], in order; requests outside share nothing;
+    G may be 0), and the first shared_lens[i] keys (int32 [G]) of each of them are those in the pages that the block table names for the group's
+    first request.  Usually their rows of the table name the same pages; a last one that is shared in part is a copy of everyone's own.  A request
+    with a new token at a place in front of its group's shared_lens takes no part and is computed by itself, so idle rows (seq_lens 0) do no harm.
+
+    weights (fp32 [num_pages, Hkv, page_size] view, for single tokens in groups of up to 16 query heads): what attention each key has received.
+    Every key that a request does not share gets, at its place in the pages, the sum of its softmax weights over the kv group's query heads added; the
+    newest key, whose place may hold what an earlier owner of the page left, is set to it.  Places of no key stay as they are.  Keys of two
+    requests must not lie in one page then, but for shared ones.
+
+    At most 1024 requests; head_dim 64 or 128; lengths, offsets and pages are read on the device.  Scratch memory, from torch's allocator, for the
+    call: 17 MB with 256 kv heads or fewer and 8 Hq (D + 2) bytes a token, with weights 4 Hq num_pages page_size beside it.
+
+    Precision: sums, maxima and partial results have 32 bits; probabilities enter the product with V as one bf16 value, as two where a request (or a
+    group) has no more than 16 rows (tokens times query heads of a kv group).  A value that is not finite makes the rows that see it not finite, and
+    no others."""
+    lib = _lib.load()
+    _check_hnd(q, "q")
+    hq, n, d = q.shape
+    dev = q.device
+    (pages, hkv, page_size, _), (k_p, k_h, k_n, _), (v_p, v_h, v_n, _) = _check_pages(k_pages, v_pages, d, dev)
+    batch, groups = seq_lens.numel(), shared_lens.numel()
+    _check_ints(dev, ("seq_lens", seq_lens, torch.int32, batch), ("shared_lens", shared_lens, torch.int32, groups),
+                ("cu_groups", cu_groups, torch.int32, groups + 1))
+    _check_table(block_table, batch, dev)
+    if cu_q is not None:
+        _check_ints(dev, ("cu_q", cu_q, torch.int32, batch + 1))
+    elif n != batch:
+        raise ValueError(f"without cu_q every request has one row: q has {n}, seq_lens {batch}")
+    w_p = w_h = 0
+    if weights is not None:
+        if cu_q is not None:
+            raise ValueError("weights go with single tokens: paged_key_weights takes several of a request")
+        _check_weights(weights, pages, hkv, page_size, dev)
+        w_p, w_h, _ = weights.stride()
+    stream = _stream_handle(dev)
+    if out is None:
+        out = torch.empty(n, hq, d, dtype=torch.bfloat16, device=dev)
+    elif out.dtype is not torch.bfloat16 or tuple(out.shape) != (n, hq, d) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous bfloat16 [{n}, {hq}, {d}] tensor on {dev}")
+    need = lib.sp_shared_attn_workspace_bytes(n, batch, groups, hq, hkv, d, cu_q is None, 0 if weights is None else pages * page_size)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
+    q_h, q_n, _ = q.stride()
+    st = lib.sp_shared_attn_bf16(_lib.SHARED_ATTN_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+        shared_lens.data_ptr(), cu_groups.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(),
+        0 if ws is None else ws.data_ptr(), need, n, batch, groups, hq, hkv, d, pages, page_size, block_table.size(1), block_table.stride(0), q_n,
+        q_h, k_p, k_n, k_h, v_p, v_n, v_h, w_p, w_h, softmax_scale, stream))
+    if st:
+        _lib.check(st, "sp_shared_attn_bf16")
+    return out
+
+
 def rope_inplace(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> None:
     """Rotates q bf16 [Hq, N, D] and k bf16 [Hkv, N, D] (views with any token / head strides, contiguous head_dim)
     in place by the position embeddings cos / sin bf16 [N, D]:  x <- x*cos + rotate_half(x)*sin  with the roundings
