@@ -443,6 +443,44 @@ size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t gro
                                       int64_t pool_keys);
 int sp_shared_attn_bf16(const sp_shared_attn_args* args /* host */);
 
+/* What attention every cached key receives: for sequence b with rows cu_q[b] .. cu_q[b + 1] of q (null: one each), its last positions,
+ *   weight[j] = sum over its rows and the query heads of the kv group of softmax(q . k)[j] over the keys j' <= the row's position,
+ * for its keys j >= first[b] (null: all), at their places in the pages.  accumulate: added to what stands there, but for the places of the sequence's
+ * new tokens, which are set; else all are set.  Sequences without rows, and keys without a page, stay as they are; no such key may stand in pages
+ * of two sequences.  weights: fp32 [num_pages][hkv][page_size].  head_dim 64 or 128; at most 1024 sequences. */
+typedef struct sp_paged_key_weights_args {
+  const void *q, *k_pages;
+  const int32_t *block_table, *seq_lens, *cu_q, *first;
+  float* weights;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t tokens, batch, hq, hkv, d, num_pages, page_size, table_width, table_stride, accumulate;
+  int64_t q_stride_n, q_stride_h, k_stride_page, k_stride_slot, k_stride_h, w_stride_page, w_stride_h;
+  double softmax_scale;
+  sp_stream_t stream;
+} sp_paged_key_weights_args;
+size_t sp_paged_key_weights_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv);
+int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* args /* host */);
+
+/* Drops the lightest keys of every kv head of sequences that hold more than they may: of sequence b with seq_lens[b] keys the first first[b] (null: 0)
+ * and the last `recent` stay and of those between the `budget` heaviest by their weights (of equal ones the first; a weight that is negative or no
+ * number counts as 0).  What stays behind the first keys moves to the front of its pages, K, V and weights, in the order it stood in; places behind it keep
+ * what they held.  new_lens[b] is the length left, the same for all kv heads.  A sequence with a key behind the first ones that has no page stays as it is.
+ * Pages must not be shared but for those that hold nothing but first keys.  d a multiple of 8. */
+typedef struct sp_paged_evict_args {
+  void *k_pages, *v_pages;
+  float* weights;
+  const int32_t *block_table, *seq_lens, *first;
+  int32_t* new_lens;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int64_t batch, hkv, d, num_pages, page_size, table_width, table_stride, budget, recent;
+  int64_t k_stride_page, k_stride_slot, k_stride_h, v_stride_page, v_stride_slot, v_stride_h, w_stride_page, w_stride_h;
+  sp_stream_t stream;
+} sp_paged_evict_args;
+size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int64_t budget);
+int sp_paged_evict_bf16(const sp_paged_evict_args* args /* host */);
+
 /* ---- rotary position embedding in front of the attention function ---------------------------------
  * The reference's patched model produces (cos, sin) per position (model_patch.py:121) and leaves the rotation to
  * the Hugging Face attention layer, which evaluates  x*cos + rotate_half(x)*sin  (rotate_half(x) =

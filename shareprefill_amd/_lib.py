@@ -107,6 +107,10 @@ SIGNATURES = {
     "sp_window_attn_bf16": (_I32, [C.c_char_p]),
     "sp_shared_attn_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32, _I32, _I64]),
     "sp_shared_attn_bf16": (_I32, [C.c_char_p]),
+    "sp_paged_key_weights_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
+    "sp_paged_key_weights_bf16": (_I32, [C.c_char_p]),
+    "sp_paged_evict_workspace_bytes": (_SZ, [_I32, _I32, _I64]),
+    "sp_paged_evict_bf16": (_I32, [C.c_char_p]),
     "sp_rope_inplace_bf16": (_I32, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _P]),
     "sp_pivot_update": (_I32, [_ST, _P, _P, _P, _I32, _I32, _F, _P]),
     "sp_cover_select_rows": (_I32, [_P, _I32, _F, _P, _P]),
@@ -122,8 +126,10 @@ PAGED_TABLES_ARGS = struct.Struct("@10P7qP")
 PAGED_WRITE_ARGS = struct.Struct("@5P15qP")
 PAGED_ATTN_ARGS = struct.Struct("@8PQ19qdP")
 WINDOW_ATTN_ARGS = struct.Struct("@5PQ17qdP")
-# sp_shared_attn_args
+# sp_shared_attn_args, sp_paged_key_weights_args, sp_paged_evict_args
 SHARED_ATTN_ARGS = struct.Struct("@11PQ20qdP")
+KEY_WEIGHTS_ARGS = struct.Struct("@8PQ17qdP")
+EVICT_ARGS = struct.Struct("@8PQ17qP")
 
 _lib = None
 

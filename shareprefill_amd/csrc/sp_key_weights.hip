@@ -1,0 +1,423 @@
+// How much attention every cached key receives from a request's last queries (sp_paged_key_weights):
+//   weight[j] = sum over the rows r, (token, query head of the kv group) pairs, that see key j, of exp(scale q_r . k_j) / sum_j' exp(scale q_r . k_j').
+// A row's maximum and sum have to be known before its weights can be summed over the rows, so the keys are walked twice: once for
+// the rows' maxima and sums, once for the weights, S = K . Q^T formed anew (a second product costs less than 4 bytes a logit written and read
+// back once there are more than a few rows; the second walk of a cache that fits the 256 MB behind the L2 is read from there).
+// What bounds it: HBM for few rows (2 D bytes a key and kv head), else the matrix cores, two products of rows x keys x D.
+//
+// A wave has 32 keys, its K operands in registers, those of its next 32 keys on their way; the rows' queries lie in LDS, up to 256 of them, and serve all
+// keys of the workgroup's part.  Every key's sum is formed by one wave in one order: results do not depend on timing.  Requests' blocks of 128
+// keys lie on a line per kv head that is cut into equal parts, a workgroup each.
+#include <utility>
+
+#include "sp_ring.h"
+#include "sp_paged_plan.h"
+
+#define KW_WAVES 4
+#define KW_THREADS (KW_WAVES * SP_WAVE)
+#define KW_KEYS 32                       // of a wave
+#define KW_BLOCK (KW_WAVES * KW_KEYS)
+#define KW_TILES 16                      // row tiles of 16 in LDS
+#define KW_ROWS (16 * KW_TILES)
+#define KW_OVERHEAD 2                    // blocks' worth of a request beside its blocks: its queries, the rows' meeting
+#define KW_MAX_SEQS 1024
+#define KW_PLACES 512                    // workgroups: two a CU
+
+struct KwArgs {
+  const sp_bf16 *q, *k;
+  const int32_t *table, *lens, *cu, *first;
+  float* weights;
+  int64_t table_stride, sq_n, sq_h, sk_p, sk_n, sk_h, sw_p, sw_h;
+  int batch, tokens, width, num_pages, shift;
+  int hkv, group, accumulate, parts;
+  PgDivisor by_group;
+  float scale_log2;
+  float2* part_ml;   // [token][query head][part]: of the keys that fell to a part, counted from the request's first
+  float2* row_ml;    // [token][query head]: maximum, 1 / sum
+  int2* of_request;  // [batch + 1]: parts that the request's keys fell to, its first token
+};
+
+// ---- the line ----
+// Blocks of 128 keys of every request with new tokens, from block `from` on (the walk for the weights leaves out what lies in front of the
+// request's first wanted key).
+
+template <int D, bool SUMS>
+__global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwArgs a) {
+  constexpr int KS = D / 32, CHUNKS = D / 8;
+  extern __shared__ __attribute__((aligned(16))) char lds[];  // queries [KW_ROWS][D], swizzled; rows' maxima and sums; offsets and lengths
+  char* const q_lds = lds;
+  float2* const ml_s = reinterpret_cast<float2*>(lds + KW_ROWS * D * 2);  // [KW_WAVES][KW_ROWS]
+  int* const start_s = reinterpret_cast<int*>(ml_s + KW_WAVES * KW_ROWS);
+  int* const len_s = start_s + a.batch + 1;
+  __shared__ int64_t sums_s[KW_WAVES + 1];
+  __shared__ int found_s[1];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lq = lane & 15, gr = lane >> 4;
+  const int kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv, g = a.group, room = a.width << a.shift;
+  const int hq = a.hkv * g;
+
+  int back = 0;
+  for (int i = t; i <= a.batch; i += KW_THREADS) {
+    auto start = [&](int j) { return a.cu != nullptr ? pg_max(0, pg_min(a.cu[j], a.tokens)) : j; };
+    start_s[i] = start(i);
+    if (i < a.batch) len_s[i] = pg_max(0, pg_min(a.lens[i], PG_MAX_KEYS)), back |= start(i + 1) < start(i);
+  }
+  if (__syncthreads_or(back)) {  // (offsets that go back count as the largest in front of them)
+    if (t == 0)
+      for (int i = 1; i <= a.batch; ++i) start_s[i] = pg_max(start_s[i], start_s[i - 1]);
+    __syncthreads();
+  }
+  auto blocks = [&](int b, int* from) {
+    const int keys = pg_min(len_s[b], room);
+    *from = SUMS && a.first != nullptr ? pg_max(0, pg_min(a.first[b], keys)) / KW_BLOCK : 0;
+    return start_s[b + 1] > start_s[b] && keys > 0 ? (keys + KW_BLOCK - 1) / KW_BLOCK - *from : 0;
+  };
+  const int per = (a.batch + KW_THREADS - 1) / KW_THREADS, b0 = t * per, b1 = pg_min(b0 + per, a.batch);
+  int64_t mine = 0;
+  int from;
+  for (int b = b0; b < b1; ++b) {
+    const int n = blocks(b, &from);
+    mine += n > 0 ? n + KW_OVERHEAD : 0;
+  }
+  int64_t at = mine;
+#pragma unroll
+  for (int o = 1; o < SP_WAVE; o <<= 1) {
+    const int64_t y = __shfl_up(at, o, SP_WAVE);
+    if (lane >= o) at += y;
+  }
+  if (lane == SP_WAVE - 1) sums_s[wave] = at;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < KW_WAVES; ++w) {
+    if (w == wave) at += total;
+    total += sums_s[w];
+  }
+  at -= mine;
+  const int64_t parts = pg_parts(total, a.parts, 1 + KW_OVERHEAD);
+  const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
+  if (t == 0) found_s[0] = a.batch;
+  __syncthreads();
+  // units of a request: KW_OVERHEAD, then its blocks
+  auto steps = [&](int64_t start, int n, int64_t c0, int64_t c1, int* begin, int* end) {
+    *begin = c0 <= start + KW_OVERHEAD ? 0 : (int)pg_max(0, (int)(c0 - start < n + KW_OVERHEAD ? c0 - start - KW_OVERHEAD : n));
+    *end = c1 >= start + n + KW_OVERHEAD ? n : c1 <= start + KW_OVERHEAD ? 0 : (int)(c1 - start - KW_OVERHEAD);
+  };
+  // the part in which a request's first block lies
+  auto first_part = [&](int64_t start) {
+    const int64_t x = start + KW_OVERHEAD;  // (its unit)
+    int64_t p = (int64_t)((double)x / (double)total * (double)parts);
+    if (p >= parts) p = parts - 1;
+    while (p > 0 && pg_cut(total, parts, p) > x) --p;
+    while (p + 1 < parts && pg_cut(total, parts, p + 1) <= x) ++p;
+    return (int)p;
+  };
+  const bool tell = !SUMS && blockIdx.x == 0;
+  if (tell || (cut0 < cut1 && cut0 >= at && cut0 < at + mine)) {
+    int64_t u = at;
+    for (int b = b0; b < b1; ++b) {
+      const int n = blocks(b, &from);
+      const int64_t units = n > 0 ? n + KW_OVERHEAD : 0;
+      if (tell) {
+        int count = 0;
+        if (n > 0) {
+          const int64_t last = u + units - 1;
+          const int p0 = first_part(u);
+          int p1 = p0;
+          while (p1 + 1 < parts && pg_cut(total, parts, p1 + 1) <= last) ++p1;
+          count = p1 - p0 + 1;
+        }
+        a.of_request[b] = make_int2(count, start_s[b]);
+      }
+      if (cut0 >= u && cut0 < u + units) found_s[0] = b, sums_s[KW_WAVES] = u;
+      u += units;
+    }
+  }
+  if (tell && t == 0) a.of_request[a.batch] = make_int2(0, start_s[a.batch]);
+  __syncthreads();
+  int b = found_s[0];
+  int64_t unit = b < a.batch ? sums_s[KW_WAVES] : total;
+
+  for (; b < a.batch && unit < cut1; ++b) {
+    const int n = blocks(b, &from);
+    if (n == 0) continue;
+    const int64_t start_unit = unit;
+    unit += n + KW_OVERHEAD;
+    int begin, end;
+    steps(start_unit, n, cut0, cut1, &begin, &end);
+    if (begin >= end) continue;
+    const int start = start_s[b], q_len = start_s[b + 1] - start, len = len_s[b], rows = q_len * g, keys = pg_min(len, room);
+    const int rel = SUMS ? 0 : part - first_part(start_unit);
+    const int first_key = SUMS && a.first != nullptr ? pg_max(0, pg_min(a.first[b], keys)) : 0;
+    const int pos0 = len - q_len;  // of the first row
+    const sp_bf16* const kh = a.k + kvh * a.sk_h;
+    const int32_t* const table = a.table + (int64_t)b * a.table_stride;
+    // K operands of the wave's 32 keys of a block, and which of them there are
+    struct Keys {
+      dc_u32x4 r[2][KS];
+      uint32_t there;  // 16-key halves with a page (bits)
+    };
+    auto fetch = [&](int block, Keys& x) {
+      x.there = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = (from + block) * KW_BLOCK + wave * KW_KEYS + 16 * i, page = key >> a.shift;
+        const int id = page < a.width ? table[page] : -1;
+        const bool ok = (unsigned)id < (unsigned)a.num_pages;
+        if (ok) x.there |= 1u << i;
+        const sp_bf16* src = kh + (int64_t)(ok ? id : 0) * a.sk_p + (int64_t)((key & ((1 << a.shift) - 1)) + lq) * a.sk_n + 8 * gr;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x.r[i][ks] = *reinterpret_cast<const dc_u32x4*>(src + 32 * ks);
+      }
+    };
+    for (int row0 = 0; row0 < rows; row0 += KW_ROWS) {
+      const int here = pg_min(rows - row0, KW_ROWS), tiles = (here + 15) / 16;
+      Keys cur, nxt;
+      fetch(begin, cur);
+      __syncthreads();  // (the rows before are done with)
+      for (int i = t; i < tiles * 16 * CHUNKS; i += KW_THREADS) {
+        const int r = i / CHUNKS, c = i % CHUNKS, row = row0 + pg_min(r, here - 1), token = (int)pg_div((unsigned)row, a.by_group);
+        *reinterpret_cast<dc_u32x4*>(q_lds + r * (D * 2) + ((c ^ ds_swz_k<D>(r & 15)) << 4)) =
+            *reinterpret_cast<const dc_u32x4*>(a.q + (int64_t)(start + token) * a.sq_n + (int64_t)(kvh * g + (row - token * g)) * a.sq_h + 8 * c);
+      }
+      if constexpr (SUMS) {
+        for (int r = t; r < tiles * 16; r += KW_THREADS) {  // (rows that are none weigh nothing)
+          float2 ml = make_float2(INFINITY, 0.f);
+          if (r < here) {
+            const int row = row0 + r, token = (int)pg_div((unsigned)row, a.by_group);
+            ml = a.row_ml[(int64_t)(start + token) * hq + kvh * g + (row - token * g)];
+          }
+          ml_s[r] = ml;
+        }
+      }
+      __syncthreads();
+      float m[SUMS ? 1 : KW_TILES], l[SUMS ? 1 : KW_TILES];
+      if constexpr (!SUMS) {
+#pragma unroll
+        for (int i = 0; i < KW_TILES; ++i) m[i] = -INFINITY, l[i] = 0.f;
+      }
+      for (int block = begin; block < end; ++block) {
+        if (block + 1 < end) fetch(block + 1, nxt);
+        const int key0 = (from + block) * KW_BLOCK + wave * KW_KEYS;
+        const bool edge = key0 + KW_KEYS - 1 > pos0 + (int)pg_div((unsigned)row0, a.by_group) || cur.there != 3u;  // some row does not see some key
+        float acc[2][4] = {{0.f}};
+        auto tile = [&](int i) {
+          ds_floatx4 sc[2];
+          dc_bf16x8 qb[KS];
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            qb[ks] = *reinterpret_cast<const dc_bf16x8*>(q_lds + (16 * i + lq) * (D * 2) + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            sc[h] = (ds_floatx4){0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+              sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, cur.r[h][ks]), qb[ks], sc[h], 0, 0, 0);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sc[h][j] *= a.scale_log2;
+          if (edge) {
+            const int pos = pos0 + (int)pg_div((unsigned)pg_min(row0 + 16 * i + lq, rows - 1), a.by_group);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                sc[h][j] = key0 + 16 * h + 4 * gr + j <= pos && ((cur.there >> h) & 1u) ? sc[h][j] : -INFINITY;
+          }
+          return std::pair<ds_floatx4, ds_floatx4>(sc[0], sc[1]);
+        };
+        if constexpr (!SUMS) {
+#pragma unroll
+          for (int i = 0; i < KW_TILES; ++i) {
+            if (i < tiles) {
+              const auto [s0, s1] = tile(i);
+              float mx = fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])), fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3])));
+              mx = fmaxf(mx, m[i]);
+              const float base = mx == -INFINITY ? 0.f : mx;
+              float add = 0.f;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) add += __builtin_amdgcn_exp2f(s0[j] - base) + __builtin_amdgcn_exp2f(s1[j] - base);
+              l[i] = l[i] * __builtin_amdgcn_exp2f(m[i] - base) + add;
+              m[i] = mx;
+            }
+          }
+        } else {
+          for (int i = 0; i < tiles; ++i) {
+            const auto [s0, s1] = tile(i);
+            const float2 ml = ml_s[16 * i + lq];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              acc[0][j] += __builtin_amdgcn_exp2f(s0[j] - ml.x) * ml.y;
+              acc[1][j] += __builtin_amdgcn_exp2f(s1[j] - ml.x) * ml.y;
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int by = 1; by < 16; by <<= 1) acc[h][j] += __shfl_xor(acc[h][j], by, SP_WAVE);
+          // lanes 0 .. 7 of a group have a key each: 16 (lq / 4) + 4 gr + lq % 4
+          float sum = acc[0][0];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) sum = lq == i ? acc[i >> 2][i & 3] : sum;
+          const int key = key0 + 16 * (lq >> 2) + 4 * gr + (lq & 3);
+          if (lq < 8 && ((cur.there >> (lq >> 2)) & 1u) && key >= first_key && key < keys) {
+            float* const to = a.weights + (int64_t)table[key >> a.shift] * a.sw_p + kvh * a.sw_h + (key & ((1 << a.shift) - 1));
+            const bool adds = row0 > 0 || (a.accumulate && key < pos0);
+            *to = (adds ? *to : 0.f) + sum;
+          }
+        }
+        cur = nxt;
+      }
+      if constexpr (!SUMS) {
+#pragma unroll
+        for (int i = 0; i < KW_TILES; ++i) {
+          if (i < tiles) {
+#pragma unroll
+            for (int by = 16; by < SP_WAVE; by <<= 1) {
+              const float m1 = __shfl_xor(m[i], by, SP_WAVE), l1 = __shfl_xor(l[i], by, SP_WAVE), top = fmaxf(m[i], m1), base = top == -INFINITY ? 0.f : top;
+              l[i] = l[i] * __builtin_amdgcn_exp2f(m[i] - base) + l1 * __builtin_amdgcn_exp2f(m1 - base);
+              m[i] = top;
+          }
+          if (gr == 0) ml_s[wave * KW_ROWS + 16 * i + lq] = make_float2(m[i], l[i]);
+          }
+        }
+        __syncthreads();
+        for (int r = t; r < here; r += KW_THREADS) {
+          float top = -INFINITY, sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < KW_WAVES; ++w) top = fmaxf(top, ml_s[w * KW_ROWS + r].x);
+          const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+          for (int w = 0; w < KW_WAVES; ++w) sum += ml_s[w * KW_ROWS + r].y * __builtin_amdgcn_exp2f(ml_s[w * KW_ROWS + r].x - base);
+          const int row = row0 + r, token = (int)pg_div((unsigned)row, a.by_group);
+          a.part_ml[((int64_t)(start + token) * hq + kvh * g + (row - token * g)) * a.parts + rel] = make_float2(top, sum);
+        }
+      }
+    }
+  }
+}
+
+// A row's parts joined, a wave each: its maximum and 1 / sum (infinity and 0: it sees no key).
+__global__ __launch_bounds__(KW_THREADS) void sp_key_weights_join_kernel(const KwArgs a) {
+  const int lane = threadIdx.x & 63, hq = a.hkv * a.group;
+  const int64_t row = (int64_t)blockIdx.x * KW_WAVES + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.tokens * hq) return;
+  const int token = (int)(row / hq);
+  int b = token;
+  if (a.cu != nullptr) {
+    b = 0;
+    int hi = a.batch;
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (a.of_request[mid].y <= token)
+        b = mid;
+      else
+        hi = mid;
+    }
+  }
+  const int count = token >= a.of_request[b].y && token < a.of_request[b + 1].y ? a.of_request[b].x : 0;
+  float top = -INFINITY, sum = 0.f;
+  for (int i0 = 0; i0 < count; i0 += SP_WAVE) {
+    const float2 ml = i0 + lane < count ? a.part_ml[row * a.parts + i0 + lane] : make_float2(-INFINITY, 0.f);
+    const float to = fmaxf(top, sp_wave_max(ml.x)), base = to == -INFINITY ? 0.f : to;
+    sum = sum * __builtin_amdgcn_exp2f(top - base) + sp_wave_sum(ml.y * __builtin_amdgcn_exp2f(ml.x - base));
+    top = to;
+  }
+  if (lane == 0) a.row_ml[row] = make_float2(top == -INFINITY ? INFINITY : top, sum == 0.f ? 0.f : 1.0f / sum);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------
+static int kw_parts(int64_t hkv) { return hkv < KW_PLACES ? KW_PLACES / (int)hkv : 1; }
+struct KwSizes {
+  size_t part_ml, row_ml, of_request, bytes;
+};
+static KwSizes kw_sizes(int64_t tokens, int64_t batch, int64_t hq, int64_t hkv) {
+  KwSizes s;
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t here = at;
+    at += (n + 255) / 256 * 256;
+    return here;
+  };
+  s.part_ml = take((size_t)(tokens * hq) * kw_parts(hkv) * sizeof(float2));
+  s.row_ml = take((size_t)(tokens * hq) * sizeof(float2));
+  s.of_request = take((size_t)(batch + 1) * sizeof(int2));
+  s.bytes = at;
+  return s;
+}
+static bool kw_shape_ok(int64_t tokens, int64_t batch, int64_t hq, int64_t hkv) {
+  return tokens > 0 && tokens <= PG_MAX_KEYS && batch > 0 && batch <= KW_MAX_SEQS && hq > 0 && hkv > 0 && hq % hkv == 0 && hq <= 65536 &&
+         tokens * hq < (1ll << 31);
+}
+
+extern "C" size_t sp_paged_key_weights_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv) {
+  return kw_shape_ok(tokens, batch, hq, hkv) ? kw_sizes(tokens, batch, hq, hkv).bytes : 0;
+}
+
+extern "C" int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* x) {
+  const char* who = "sp_paged_key_weights_bf16";
+  SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(x->hq > 0 && x->hkv > 0 && x->hq % x->hkv == 0, SP_ERR_INVALID_ARGUMENT, "%s: bad shape hq=%lld hkv=%lld", who, (long long)x->hq,
+             (long long)x->hkv);
+  SP_REQUIRE(x->d == 64 || x->d == 128, SP_ERR_UNSUPPORTED, "%s: head_dim %lld unsupported (64 or 128)", who, (long long)x->d);
+  SP_REQUIRE((float)x->softmax_scale > 0.f, SP_ERR_INVALID_ARGUMENT, "%s: softmax_scale must be > 0", who);
+  SP_REQUIRE(x->batch > 0 && x->tokens >= 0 && x->table_width > 0 && x->num_pages > 0, SP_ERR_INVALID_ARGUMENT,
+             "%s: batch=%lld tokens=%lld table_width=%lld num_pages=%lld", who, (long long)x->batch, (long long)x->tokens, (long long)x->table_width,
+             (long long)x->num_pages);
+  SP_REQUIRE(x->batch <= KW_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %lld (at most %d)", who, (long long)x->batch, KW_MAX_SEQS);
+  int shift = 4;
+  while (shift <= 10 && x->page_size != 1ll << shift) ++shift;
+  SP_REQUIRE(shift <= 10, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
+  SP_REQUIRE(x->tokens <= PG_MAX_KEYS && x->num_pages <= 0x7fffffffll && x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS,
+             SP_ERR_UNSUPPORTED, "%s: tokens=%lld num_pages=%lld table_width=%lld too large", who, (long long)x->tokens, (long long)x->num_pages,
+             (long long)x->table_width);
+  SP_REQUIRE(x->cu_q != nullptr || x->tokens == x->batch, SP_ERR_INVALID_ARGUMENT, "%s: without cu_q every sequence has one token (%lld for %lld)",
+             who, (long long)x->tokens, (long long)x->batch);
+  if (x->tokens == 0) return SP_OK;
+  SP_REQUIRE(kw_shape_ok(x->tokens, x->batch, x->hq, x->hkv), SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who,
+             (long long)x->tokens, (long long)x->hq);
+  const int64_t q_n = pg_used_stride(x->q_stride_n, x->tokens), q_h = pg_used_stride(x->q_stride_h, x->hq);
+  const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);
+  SP_REQUIRE(x->q && x->k_pages && x->block_table && x->seq_lens && x->weights, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  SP_REQUIRE(((uintptr_t)x->q | (uintptr_t)x->k_pages) % 16 == 0 && (q_n | q_h | k_p | k_h | x->k_stride_slot) % 8 == 0, SP_ERR_UNSUPPORTED,
+             "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
+  const KwSizes s = kw_sizes(x->tokens, x->batch, x->hq, x->hkv);
+  SP_REQUIRE(x->workspace != nullptr && x->workspace_bytes >= s.bytes && (uintptr_t)x->workspace % 16 == 0, SP_ERR_WORKSPACE,
+             "%s: workspace missing, too small or misaligned", who);
+  char* const ws = (char*)x->workspace;
+  KwArgs a = {};
+  a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k_pages;
+  a.table = x->block_table, a.lens = x->seq_lens, a.cu = x->cu_q, a.first = x->first, a.weights = x->weights;
+  a.table_stride = x->table_stride, a.sq_n = q_n, a.sq_h = q_h, a.sk_p = k_p, a.sk_n = x->k_stride_slot, a.sk_h = k_h;
+  a.sw_p = pg_used_stride(x->w_stride_page, x->num_pages), a.sw_h = pg_used_stride(x->w_stride_h, x->hkv);
+  a.batch = (int)x->batch, a.tokens = (int)x->tokens, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
+  a.hkv = (int)x->hkv, a.group = (int)(x->hq / x->hkv), a.accumulate = x->accumulate != 0, a.parts = kw_parts(x->hkv);
+  a.by_group = pg_divisor((unsigned)a.group);
+  a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
+  a.part_ml = (float2*)(ws + s.part_ml), a.row_ml = (float2*)(ws + s.row_ml), a.of_request = (int2*)(ws + s.of_request);
+  auto lds = [](int d, int batch) { return (size_t)KW_ROWS * d * 2 + KW_WAVES * KW_ROWS * sizeof(float2) + (2 * (size_t)batch + 1) * sizeof(int); };
+  static bool attr_set[64] = {false};  // per device, once (idempotent)
+  int dev = 0;
+  SP_HIP(hipGetDevice(&dev));
+  SP_REQUIRE(dev >= 0 && dev < 64, SP_ERR_UNSUPPORTED, "%s: device index %d", who, dev);
+  if (!attr_set[dev]) {
+    for (const void* f : {(const void*)sp_key_weights_kernel<64, false>, (const void*)sp_key_weights_kernel<64, true>,
+                          (const void*)sp_key_weights_kernel<128, false>, (const void*)sp_key_weights_kernel<128, true>})
+      SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds(128, KW_MAX_SEQS)));
+    attr_set[dev] = true;
+  }
+  const hipStream_t stream = (hipStream_t)x->stream;
+  const unsigned grid = (unsigned)(a.parts * a.hkv), joins = (unsigned)sp_ceil_div(x->tokens * x->hq, KW_WAVES);
+  auto go = [&](auto stats, auto sums) {
+    hipLaunchKernelGGL(stats, dim3(grid), dim3(KW_THREADS), lds((int)x->d, a.batch), stream, a);
+    hipLaunchKernelGGL(sp_key_weights_join_kernel, dim3(joins), dim3(KW_THREADS), 0, stream, a);
+    hipLaunchKernelGGL(sums, dim3(grid), dim3(KW_THREADS), lds((int)x->d, a.batch), stream, a);
+  };
+  x->d == 64 ? go(sp_key_weights_kernel<64, false>, sp_key_weights_kernel<64, true>) : go(sp_key_weights_kernel<128, false>, sp_key_weights_kernel<128, true>);
+  SP_LAUNCH_CHECK();
+  return SP_OK;
+}

@@ -789,6 +789,86 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     return out
 
 
+def paged_key_weights(q: torch.Tensor, k_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, softmax_scale: float,
+                      weights: torch.Tensor, cu_q: Optional[torch.Tensor] = None, first: Optional[torch.Tensor] = None,
+                      accumulate: bool = False) -> torch.Tensor:
+    """How much attention the last tokens of every request pay to each of its cached keys: q bf16 [Hq, T, D] view as in paged_attention (the last
+    tokens of a prompt, say, once it is cached whole), weights fp32 [num_pages, Hkv, page_size] view, in place and returned.
+
+    At key j's place in the pages: the sum over the request's rows, cu_q[b] .. cu_q[b + 1] of q (None: one each), at its last positions, and over the kv
+    group's query heads of softmax(scale q . k)[j] (0 for rows in front of j).  accumulate: added to what stands there, but for keys of these
+    very tokens, which are set; without it all are set.  first int32 [B]: keys in front of first[b] stay as they are; so do requests
+    without rows, keys without a page and places of no key.  Keys that are written must not lie in pages of two requests.
+
+    At most 1024 requests; head_dim 64 or 128; lengths and pages are read on the device.  Every sum has 32 bits and one order.  Scratch memory, from
+    torch's allocator, for the call: 4 kB T Hq / Hkv."""
+    lib = _lib.load()
+    _check_hnd(q, "q")
+    hq, n, d = q.shape
+    dev = q.device
+    (pages, hkv, page_size, _), (k_p, k_h, k_n, _), _ = _check_pages(k_pages, k_pages, d, dev)
+    batch = seq_lens.numel()
+    _check_ints(dev, ("seq_lens", seq_lens, torch.int32, batch))
+    _check_table(block_table, batch, dev)
+    _check_weights(weights, pages, hkv, page_size, dev)
+    if first is not None:
+        _check_ints(dev, ("first", first, torch.int32, batch))
+    if cu_q is not None:
+        _check_ints(dev, ("cu_q", cu_q, torch.int32, batch + 1))
+    elif n != batch:
+        raise ValueError(f"without cu_q every request has one row: q has {n}, seq_lens {batch}")
+    stream = _stream_handle(dev)
+    need = lib.sp_paged_key_weights_workspace_bytes(n, batch, hq, hkv)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
+    q_h, q_n, _ = q.stride()
+    w_p, w_h, _ = weights.stride()
+    st = lib.sp_paged_key_weights_bf16(_lib.KEY_WEIGHTS_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+        0 if first is None else first.data_ptr(), weights.data_ptr(), 0 if ws is None else ws.data_ptr(), need, n, batch, hq, hkv, d, pages, page_size,
+        block_table.size(1), block_table.stride(0), bool(accumulate), q_n, q_h, k_p, k_n, k_h, w_p, w_h, softmax_scale, stream))
+    if st:
+        _lib.check(st, "sp_paged_key_weights_bf16")
+    return weights
+
+
+def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int,
+                recent: int, first: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Drops the lightest keys of requests that hold more than they may, in place: of a request's keys the first first[b] (int32 [B]; None: 0), the last
+    `recent` and, of those between, the `budget` heaviest stay, chosen for every kv head by itself.  -> the lengths left, int32 [B], the same for all heads.
+
+    weights fp32 [num_pages, Hkv, page_size] view (paged_key_weights, shared_prefix_attention).  Of equal weights the first stay; one that is negative or
+    NaN counts as 0.  Keys, values and weights that stay behind the first keys move to the front of their pages, in order; the pages behind the new
+    length may go back to the stack.  Keys are moved as they are, rotated for the positions they had: the next token's position is not the new length.
+    A request with a key behind the first ones that has no page stays as it is.  Only pages of nothing but first keys may be shared.
+
+    At most 4096 requests; head_dim a multiple of 8.  Scratch memory, from torch's allocator, for the call: 4 B Hkv budget bytes."""
+    lib = _lib.load()
+    if k_pages.dim() != 4 or not k_pages.is_cuda:
+        raise ValueError(f"k_pages must be [num_pages, Hkv, page_size, D] on the GPU, got {tuple(k_pages.shape)} on {k_pages.device}")
+    dev = k_pages.device
+    (pages, hkv, page_size, d), (k_p, k_h, k_n, _), (v_p, v_h, v_n, _) = _check_pages(k_pages, v_pages, k_pages.shape[3], dev)
+    batch = seq_lens.numel()
+    _check_ints(dev, ("seq_lens", seq_lens, torch.int32, batch))
+    _check_table(block_table, batch, dev)
+    _check_weights(weights, pages, hkv, page_size, dev)
+    if first is not None:
+        _check_ints(dev, ("first", first, torch.int32, batch))
+    if budget < 0 or recent < 0:
+        raise ValueError(f"budget {budget} and recent {recent} must not be negative")
+    stream = _stream_handle(dev)
+    new_lens = torch.empty(batch, dtype=torch.int32, device=dev)
+    need = lib.sp_paged_evict_workspace_bytes(batch, hkv, min(budget, block_table.size(1) * page_size))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
+    w_p, w_h, _ = weights.stride()
+    st = lib.sp_paged_evict_bf16(_lib.EVICT_ARGS.pack(
+        k_pages.data_ptr(), v_pages.data_ptr(), weights.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        0 if first is None else first.data_ptr(), new_lens.data_ptr(), 0 if ws is None else ws.data_ptr(), need, batch, hkv, d, pages, page_size,
+        block_table.size(1), block_table.stride(0), budget, recent, k_p, k_n, k_h, v_p, v_n, v_h, w_p, w_h, stream))
+    if st:
+        _lib.check(st, "sp_paged_evict_bf16")
+    return new_lens
+
+
 def rope_inplace(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> None:
     """Rotates q bf16 [Hq, N, D] and k bf16 [Hkv, N, D] (views with any token / head strides, contiguous head_dim)
     in place by the position embeddings cos / sin bf16 [N, D]:  x <- x*cos + rotate_half(x)*sin  with the roundings
