@@ -26,6 +26,11 @@ struct CkArgs {
   float2* ml_part;          // [workgroup][2][rows of a tile]
   int4* notes;              // [workgroup], and where by_slot is not null [row tile number][kv head]
   int4* by_slot;
+  // Groups of sequences over the keys that they share (sp_shared_prefix.hip): what is a sequence above is a group then, its rows' sums are left as they are
+  const int32_t* groups;    // first sequences, of n_seqs; a group's pages are those of its first
+  float* o_row;             // [token][hq][D], sums of the weights' values
+  float2* ml_row;           // [token][hq], maxima and sums of the weights
+  int n_seqs;
 };
 // Notes of a workgroup.  x: the part of its first row tile is no partial, the last of the row tile, or one in the middle; y: rows of the row
 // tile that starts here and goes on in the next part, 0: there is none; z: its first row in the sequence, w: the sequence's first token.
@@ -77,7 +82,7 @@ __device__ __forceinline__ int cm_parts(const CkArgs& a, int workgroups, int lan
     if (ends != 0ull) return first + __builtin_ctzll(ends) + 1;
   }
 }
-template <int D, int ROWS, int BAND>
+template <int D, int ROWS, int BAND, bool RAW = false>  // RAW: sums as they are, into o_row and ml_row
 __global__ __launch_bounds__(CM_THREADS) void sp_chunk_merge_kernel(const CkArgs a, int workgroups) {
   constexpr int C4 = D / 64, SETS = CM_THREADS / (16 * BAND);  // 16-byte pieces of a thread
   __shared__ __attribute__((aligned(16))) float o_s[SETS > 1 ? SETS - 1 : 1][BAND][D];
@@ -153,8 +158,15 @@ __global__ __launch_bounds__(CM_THREADS) void sp_chunk_merge_kernel(const CkArgs
       for (int c = 0; c < C4; ++c) acc[c] += *reinterpret_cast<const cm_floatx4*>(&o_s[i - 1][in_band][64 * c + c0]) * w;
     }
   }
-  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
   const int r = note.z + row, kvh = (int)(w0 % a.hkv), token = (int)pg_div((unsigned)r, a.by_group), head = kvh * a.group + (r - token * a.group);
+  if constexpr (RAW) {
+    const int64_t to = (int64_t)(note.w + token) * (a.hkv * a.group) + head;
+#pragma unroll
+    for (int c = 0; c < C4; ++c) *reinterpret_cast<cm_floatx4*>(a.o_row + to * D + 64 * c + c0) = acc[c];
+    if ((t & 15) == 0) a.ml_row[to] = make_float2(all, sum);
+    return;
+  }
+  const float inv = sum > 0.f || sum != sum ? 1.0f / sum : 0.f;
   sp_bf16* dst = a.out + ((int64_t)(note.w + token) * (a.hkv * a.group) + head) * D + c0;
 #pragma unroll
   for (int c = 0; c < C4; ++c)
@@ -163,6 +175,9 @@ __global__ __launch_bounds__(CM_THREADS) void sp_chunk_merge_kernel(const CkArgs
 
 // single tokens (sp_paged_decode.hip): groups of up to 16 heads
 #define PD_MAX_GROUP 16
+// groups over their shared keys (sp_chunk.hip): a's sequences are the groups, each row sees all of its group's keys
+size_t ck_groups_workspace_bytes(int32_t hkv, int32_t d);
+int ck_groups_launch(CkArgs& a, int32_t d, void* workspace, hipStream_t s);
 bool pd_takes(const CkArgs& a);
 size_t pd_workspace_bytes(int32_t hkv, int32_t d);
 int pd_launch(CkArgs& a, int64_t max_keys, int32_t d, void* workspace, hipStream_t s);

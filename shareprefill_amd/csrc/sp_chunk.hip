@@ -151,8 +151,16 @@ __device__ __forceinline__ int ck_sequence(const CkArgs& a, const int* cu, int x
 // WINDOWED: blocks are made of any two sub-tiles of a walk, so that a window's start and the sinks cost a sub-tile, not a block: 8192 tokens in a
 // window of 1024 with 4 sinks 155 -> 151 us.  Without a window a block is 128 keys in a row, and nothing asks for windows: a mixed batch of 64
 // channels 138 -> 133 us.
-template <int D, bool PAGED, bool WINDOWED>
-__global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a) {
+// GROUPS: a sequence is a group of them, its rows' positions lie behind all of its keys, and rows are left as sums (o_row, ml_row).
+// Of a group: its table row, and its first token.
+template <class Args>
+__device__ __forceinline__ int ck_group_row(const Args& a, int i) { return pg_max(0, pg_min(a.groups[i], a.n_seqs - 1)); }
+__device__ __forceinline__ int ck_group_start(const CkArgs& a, int i) {
+  const int b = pg_max(0, pg_min(a.groups[i], a.n_seqs));
+  return a.cu != nullptr ? pg_max(0, pg_min(a.cu[b], a.tokens)) : b;
+}
+template <int D, bool PAGED, bool WINDOWED, bool GROUPS>
+__device__ __forceinline__ void ck_attend(const CkArgs& a) {
   constexpr int WAVES = CK_WAVES, THREADS = CK_THREADS, TILE_ROWS = CK_ROWS;
   constexpr bool HALF = D == 64;
   constexpr int QT = 2;                    // 16-row tiles per wave
@@ -174,6 +182,15 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     return p;
   };
 
+  // positions of a row tile's first and last row, and of a token
+  auto positions = [&](int rt, int q_len, int len, int* p0, int* p1) {
+    if constexpr (GROUPS)
+      *p0 = *p1 = len - 1;
+    else
+      pg_tile_positions(rt, q_len, len, a.by_group, TILE_ROWS, p0, p1);
+  };
+  auto position = [](int q_len, int len, int token) { return GROUPS ? len - 1 : len - q_len + token; };
+
   // ---- which row tiles, and which blocks of the first and the last ----
   // On a line: row tiles x .. x_end, the first from block tile_begin on, of the last the blocks in front of tile_end.
   int x = 0, x_end = 0, tile_begin = 0, tile_end = 0, turn = 0;
@@ -185,9 +202,10 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     __shared__ int found[2][2];
     int back = 0;
     for (int i = t; i <= a.batch; i += THREADS) {
-      const int start = ck_start(a, i);
+      auto start_at = [&](int j) { return GROUPS ? ck_group_start(a, j) : ck_start(a, j); };
+      const int start = start_at(i);
       cu_s[i] = start;
-      if (i < a.batch) len_s[i] = ck_len(a, i), back |= ck_start(a, i + 1) < start;
+      if (i < a.batch) len_s[i] = GROUPS ? pg_min(ck_len(a, i), a.width << a.shift) : ck_len(a, i), back |= start_at(i + 1) < start;
     }
     // Searches need the offsets in order, and must all find the same: notes of row tiles that only some of them find stay unwritten, and the
     // merging launch would read where they happen to point.  An offset that goes back counts as the largest in front of it.
@@ -216,7 +234,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           continue;
         }
         int p0, p1;
-        pg_tile_positions(rt, q_len, len_s[b], a.by_group, TILE_ROWS, &p0, &p1);
+        positions(rt, q_len, len_s[b], &p0, &p1);
         const int blocks = ck_blocks(ck_span<WINDOWED>(a, p0, p1, CK_SUB));
         visit(i, blocks + PG_OVERHEAD, blocks);
       }
@@ -279,7 +297,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(at));
     return __builtin_amdgcn_readfirstlane(v);
   };
-  auto start_of = [&](int b) { return a.cu != nullptr ? from_lds(lds_cu + 4u * b) : b * a.n_queries; };
+  auto start_of = [&](int b) { return GROUPS || a.cu != nullptr ? from_lds(lds_cu + 4u * b) : b * a.n_queries; };
   int seq = a.parts == 0 || x >= a.slots ? 0 : __builtin_amdgcn_readfirstlane(ck_sequence<TILE_ROWS>(a, cu_s, x, lane));
   auto next_piece = [&](Piece& p) {  // false: there is none
     for (;;) {
@@ -312,7 +330,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         if (p.rt < 0 || p.rt >= pg_row_tiles(p.q_len, a.group, TILE_ROWS)) continue;
       }
       int p0, p1;
-      pg_tile_positions(p.rt, p.q_len, p.len, a.by_group, TILE_ROWS, &p0, &p1);
+      positions(p.rt, p.q_len, p.len, &p0, &p1);
       p.span = ck_span<WINDOWED>(a, p0, p1, CK_SUB);
       p.blocks = ck_blocks(p.span);
       p.i0 = begin;
@@ -368,7 +386,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     const int i = group * SP_WAVE + lane;
     if constexpr (!PAGED) return i;
     const auto r = args();
-    const int id = r->table[b * r->table_stride + pg_min(i, r->width - 1)];
+    const int id = r->table[(GROUPS ? ck_group_row(*r, b) : b) * r->table_stride + pg_min(i, r->width - 1)];
     return i < r->width && (unsigned)id < (unsigned)r->num_pages ? id : -1;
   };
   auto turn_to = [&](int b, int len, int group, int id) {
@@ -447,14 +465,14 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     const bool from_start = pc.i0 == 0, to_end = pc.i1 == pc.blocks;  // (uniform)
     const bool has_rows = wave * 32 < rows;  // (uniform in the wave)
     // positions of the wave's first and last row
-    const int w0 = len - q_len + (int)pg_div((unsigned)(rt * TILE_ROWS + pg_min(wave * 32, rows - 1)), a.by_group);
-    const int w1 = len - q_len + (int)pg_div((unsigned)(rt * TILE_ROWS + pg_min(wave * 32 + 31, rows - 1)), a.by_group);
+    const int w0 = position(q_len, len, (int)pg_div((unsigned)(rt * TILE_ROWS + pg_min(wave * 32, rows - 1)), a.by_group));
+    const int w1 = position(q_len, len, (int)pg_div((unsigned)(rt * TILE_ROWS + pg_min(wave * 32 + 31, rows - 1)), a.by_group));
     int pos[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
       int token, head;
       row_of(pc, wave * 32 + 16 * qt + lq, &token, &head);
-      pos[qt] = len - q_len + token;
+      pos[qt] = position(q_len, len, token);
     }
     const bool next_blocks = have_next && next_p.i1 > next_p.i0;  // the next piece has a first block to fetch
     const int ids_here = ids_first;
@@ -668,7 +686,12 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
       spoilt[qt] = spoilt[qt] && mine && l[qt] == l[qt];
       const float size = __builtin_fabsf(m[qt]);
       far[qt] = mine && l[qt] == l[qt] && size >= CK_FAR && size < INFINITY && m[qt] != CK_NO_MAX;
-      if (whole) {
+      if (GROUPS && whole && mine) {
+        const int64_t to = (int64_t)(start + token) * (a.hkv * a.group) + head;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<floatx4*>(dst_args->o_row + to * D + 16 * ct + 4 * g) = o[ct][qt];
+        if (g == 0) dst_args->ml_row[to] = make_float2(m[qt], l[qt]);
+      } else if (whole && !GROUPS) {
         const float inv_l = l[qt] > 0.f || l[qt] != l[qt] ? 1.0f / l[qt] : 0.f;
         // (lane groups 2i and 2i + 1 trade halves of two neighbouring channel tiles: 16 bytes a store, 64 contiguous ones a row)
         sp_bf16* dst = out + ((int64_t)(start + token) * (a.hkv * a.group) + head) * D + 16 * (g & 1) + 8 * (g >> 1);
@@ -715,7 +738,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           const auto c = args();
           int id = page;
           if constexpr (PAGED) {
-            id = page < c->width ? c->table[b * c->table_stride + page] : -1;
+            id = page < c->width ? c->table[(GROUPS ? ck_group_row(*c, b) : b) * c->table_stride + page] : -1;
             if ((unsigned)id >= (unsigned)c->num_pages) id = -1;
           }
           uint32_t bad = 0u;  // an exponent of ones: one more carries into the sign
@@ -731,7 +754,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           for (int qt = 0; qt < QT; ++qt)
             for (uint32_t rows_left = no_number[qt] & ~again[qt]; rows_left != 0u; rows_left &= rows_left - 1u) {
               const int r = rt * TILE_ROWS + wave * 32 + 16 * qt + __builtin_ctz(rows_left);
-              const int p = len - q_len + (int)pg_div((unsigned)r, a.by_group);
+              const int p = position(q_len, len, (int)pg_div((unsigned)r, a.by_group));
               if (__ballot(bad != 0u && !pg_sees(p, key, a.window, a.sinks)) != 0ull) again[qt] |= rows_left & (0u - rows_left);
             }
         }
@@ -746,7 +769,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         const int in_rows = wave * 32 + 16 * qt + __builtin_ctz(rows_left);
         rows_left &= rows_left - 1u;
         const int r = rt * TILE_ROWS + in_rows, token = (int)pg_div((unsigned)r, a.by_group), head = kvh * a.group + (r - token * a.group);
-        const int p = len - q_len + token;
+        const int p = position(q_len, len, token);
         const auto c = args();
         const sp_bf16* qrow = c->q + b * c->sq_b + (int64_t)((PAGED ? start : 0) + token) * c->sq_n + head * c->sq_h;
         constexpr int CL = D / SP_WAVE;  // channels of a lane
@@ -755,7 +778,7 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
           const int key = key_of(pc, 0, i) + lane, page = key >> a.shift;
           int id = page;
           if constexpr (PAGED) {
-            id = page < c->width ? c->table[b * c->table_stride + page] : -1;
+            id = page < c->width ? c->table[(GROUPS ? ck_group_row(*c, b) : b) * c->table_stride + page] : -1;
             if ((unsigned)id >= (unsigned)c->num_pages) id = -1;
           }
           const bool seen = id >= 0 && key < len && pg_sees(p, key, a.window, a.sinks);
@@ -809,11 +832,14 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
         }
 #pragma unroll
         for (int c = 0; c < CL; ++c) {
-          if (whole)
+          if (GROUPS && whole)
+            args()->o_row[((int64_t)(start + token) * (a.hkv * a.group) + head) * D + lane * CL + c] = acc[c];
+          else if (whole)
             out[((int64_t)(start + token) * (a.hkv * a.group) + head) * D + lane * CL + c] = sp_f32_to_bf16(sum == 0.f ? 0.f : acc[c] / sum);
           else
             o_to[in_rows * D + lane * CL + c] = acc[c];
         }
+        if (GROUPS && whole && lane == 0) args()->ml_row[(int64_t)(start + token) * (a.hkv * a.group) + head] = make_float2(top, sum);
         if (!whole && lane == 0) ml_to[in_rows] = make_float2(top, sum);
       }
     }
@@ -821,6 +847,14 @@ __global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a)
     have = have_next;
   }
   if (a.parts != 0 && t == 0) args()->notes[blockIdx.x] = note;
+}
+template <int D, bool PAGED, bool WINDOWED>
+__global__ __launch_bounds__(CK_THREADS, 1) void sp_chunk_kernel(const CkArgs a) {
+  ck_attend<D, PAGED, WINDOWED, false>(a);
+}
+template <int D>
+__global__ __launch_bounds__(CK_THREADS, 1) void sp_groups_kernel(const CkArgs a) {
+  ck_attend<D, true, false, true>(a);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
@@ -913,6 +947,45 @@ static int ck_launch(const char* who, CkArgs& a, int64_t max_keys, int32_t d, vo
   };
   auto wide = [&](auto width) { windowed ? pick(width, std::true_type{}) : pick(width, std::false_type{}); };
   d == 64 ? wide(std::integral_constant<int, 64>{}) : wide(std::integral_constant<int, 128>{});
+  SP_LAUNCH_CHECK();
+  return SP_OK;
+}
+
+size_t ck_groups_workspace_bytes(int32_t hkv, int32_t d) {
+  return (size_t)ck_workgroups(hkv) * hkv * (2 * (size_t)CK_ROWS * ((size_t)d * sizeof(float) + sizeof(float2)) + 2 * sizeof(int4));
+}
+// (a.batch groups; everything but what says how the call is cut is set)
+int ck_groups_launch(CkArgs& a, int32_t d, void* workspace, hipStream_t s) {
+  const int wgs = ck_workgroups(a.hkv), grid = wgs * a.hkv;
+  a.window = PG_NO_WINDOW;
+  a.workgroups = wgs;
+  a.by_group = pg_divisor((unsigned)a.group);
+  a.slots = (int)pg_slots(a.tokens, a.group, a.batch, CK_ROWS);
+  a.parts = wgs;
+  a.o_part = (float*)workspace;
+  a.ml_part = (float2*)(a.o_part + (size_t)grid * 2 * (size_t)CK_ROWS * d);
+  a.notes = (int4*)(a.ml_part + (size_t)grid * 2 * CK_ROWS);
+  const size_t lds = CK_LDS_BYTES(d) + (size_t)(2 * a.batch + 1) * sizeof(int);
+  const bool by_slot = (int64_t)a.slots * a.hkv < grid;
+  const int merges = by_slot ? a.slots * a.hkv : grid, band = merges <= 32 ? 16 : 64;  // (as in ck_launch)
+  a.by_slot = by_slot ? a.notes + grid : nullptr;
+  static bool attr_set[64] = {false};  // per device, once (idempotent)
+  int dev = 0;
+  SP_HIP(hipGetDevice(&dev));
+  SP_REQUIRE(dev >= 0 && dev < 64, SP_ERR_UNSUPPORTED, "device index %d", dev);
+  if (!attr_set[dev]) {
+    for (const void* f : {(const void*)sp_groups_kernel<64>, (const void*)sp_groups_kernel<128>})
+      SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, CK_LDS_BYTES(128) + (2 * CK_MAX_SEQS + 1) * (int)sizeof(int)));
+    attr_set[dev] = true;
+  }
+  auto go = [&](auto kernel, auto few, auto many) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(CK_THREADS), lds, s, a);
+    hipLaunchKernelGGL(band == 16 ? few : many, dim3((unsigned)merges, CK_ROWS / band), dim3(CM_THREADS), 0, s, a, grid);
+  };
+  if (d == 64)
+    go(sp_groups_kernel<64>, sp_chunk_merge_kernel<64, CK_ROWS, 16, true>, sp_chunk_merge_kernel<64, CK_ROWS, 64, true>);
+  else
+    go(sp_groups_kernel<128>, sp_chunk_merge_kernel<128, CK_ROWS, 16, true>, sp_chunk_merge_kernel<128, CK_ROWS, 64, true>);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }

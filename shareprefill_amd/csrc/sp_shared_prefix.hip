@@ -3,11 +3,13 @@
 // the sum over the shared keys formed once for all rows of the group and joined with that over the request's own: with running maxima m and
 // sums l of either side, out = (2^(m1 - m) o1 + 2^(m2 - m) o2) / (2^(m1 - m) l1 + 2^(m2 - m) l2).
 //
-// HBM-bound as long as a group has fewer than some 250 rows a kv head: shared keys are read once per tile of 64 rows, a request's own
-// once.  Tiles of 16 rows or fewer (a request's single token) take the loop of the single-token kernel (sp_paged_decode.hip): waves take steps of 32 keys
-// in turn, each with a ring of operands in LDS that direct loads fill, no barrier between them, and meet in LDS at the end.  In larger tiles a
-// step's operands serve two waves of two row tiles each, so that a group of 16 requests with four heads a kv head costs what one of them does;
-// the two share a SIMD, where the matrix instructions of one run under the exponentials of the other.
+// HBM-bound as long as a group has fewer than some 250 rows a kv head, (token, query head) pairs: shared keys are read once per tile of 64 rows, a
+// request's own once.  Tiles of 16 rows or fewer (a request's single token) take the loop of the single-token kernel (sp_paged_decode.hip): four waves
+// take steps of 32 keys in turn, each with a ring of operands in LDS that direct loads fill, no barrier between them, and meet in LDS at the end.  In
+// larger tiles two waves of 32 rows each share a ring, and all meet at a barrier every four steps; the two share a SIMD, where the matrix
+// instructions of one run under the exponentials of the other.  Groups of many rows go to sp_chunk.hip's loop first, in a launch of its own.
+//
+// The line that the workgroups' parts are cut from (sp_shared_plan.h) is formed by every wave for itself, 64 items at a time.
 #include "sp_chunk.h"
 #include "sp_ring.h"
 #include "sp_shared_plan.h"
@@ -18,23 +20,31 @@
 // (Probabilities up to 2^7 are as exact in bf16 as those below 1.)
 #define SH_SLACK 7.f
 
+struct ShRequest {
+  int first_own;            // its first key that no group sees to
+  int group, start0, end0;  // its group, that group's first token and the one behind its last
+  int start;                // its own first token
+  int pad[3];
+};
 struct ShArgs {
   const sp_bf16 *q, *k, *v;
   const int32_t *table, *lens, *cu, *shared, *groups;  // shared: keys of a group, [n_groups]; groups: first requests, [n_groups + 1]
   sp_bf16* out;
   int64_t table_stride, sq_n, sq_h, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;  // elements; _p between pages
   int batch, tokens, width, num_pages, shift, n_groups;
-  int hkv, group, dense;      // dense: single tokens, an item each
+  int hkv, group, dense;      // dense: single tokens, a row tile each
   PgDivisor by_group;
-  int shared_slots, slots;    // items of groups, items in all
+  int shared_slots;           // numbers of the groups' row tiles
   int parts;                  // of the line at most, and workgroups of a kv head
+  int apart;                  // groups have been seen to (o_row, ml_row)
   float scale_log2;
-  float* o_part;              // [part][kv head][2][SH_TILE][D]: an item that began in an earlier part, one that goes on in the next
+  float* o_part;              // [part][kv head][2][SH_TILE][D]: a row tile that began in an earlier part, one that goes on in the next
   float2* ml_part;            // [part][kv head][2][SH_TILE]
-  float* o_row;               // [2][token][query head][D]: items that lie in one part, of groups and of requests
+  float* o_row;               // [2][token][query head][D]: row tiles that lie in one part, of groups and of requests
   float2* ml_row;
-  int64_t* starts;            // [slots + 1]: the items' first units
-  int4* of_request;           // [batch + 1]: first own key, group, the group's first token, the request's first token
+  int2* parts_of;             // by row tile number: first and last part that hold steps of it
+  int4* cuts;                 // [parts]: item and step that a part begins with, those that it ends in front of
+  ShRequest* of_request;      // [batch + 1]
   float* weights;             // null, or [num_pages][kv head][page]
   float* logits;              // [num_pages][query head][page]: scaled logits of own keys, in octaves
 };
@@ -43,19 +53,19 @@ template <int D>
 using ShShape = DsShape<D, D / 16, SH_WAVES, 128>;
 // LDS: the rings, where the waves meet afterwards; their maxima and sums; what is known of the requests and groups
 #define SH_RING 131072
-#define SH_ML (SH_RING)                                      // [2][SH_WAVES][SH_TILE] floats
-#define SH_FOUND (SH_ML + 2 * SH_WAVES * SH_TILE * 4)        // 80 bytes
-#define SH_ARRAYS (SH_FOUND + 80)
-static size_t sh_lds_bytes(int batch, int groups) { return SH_ARRAYS + ((size_t)3 * (batch + 1) + 2 * ((size_t)groups + 1)) * sizeof(int); }
+#define SH_ML (SH_RING)                                // [2][SH_WAVES][SH_TILE] floats
+#define SH_ARRAYS (SH_ML + 2 * SH_WAVES * SH_TILE * 4)
+static size_t sh_lds_bytes(int batch, int groups) { return SH_ARRAYS + (2 * ((size_t)batch + 1) + 2 * ((size_t)groups + 1)) * sizeof(int); }
 static_assert(ShShape<128>::LDS_BYTES <= SH_RING && ShShape<64>::LDS_BYTES <= SH_RING && SH_WAVES * SH_TILE * 128 * 4 <= SH_RING, "");
 
 struct ShItem {
   int table_row;    // of the block table
-  int start;        // first token of the rows
-  int row0, rows;   // first row of the tile, rows from token `start` on
+  int start, rows;  // first token; rows from there on
   int key0, key1;   // keys that some row sees
   int pos;          // position of token `start`: its row and the following ones see keys up to pos, pos + 1, ..; groups: far behind the last key
-  int lo, n;        // first step, steps
+  int lo, n;        // first step, steps of a tile
+  int slot;         // number of its first row tile
+  int row0;         // first row of a tile
 };
 
 template <int D>
@@ -68,14 +78,13 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int lq = lane & 15, gr = lane >> 4;  // head (or key row, channel) in a 16-wide tile, lane group
   const int g = a.group, kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv;
-  const int room = a.width << a.shift;
+  const int room = a.width << a.shift, n_groups = a.apart ? 0 : a.n_groups, items = n_groups + a.batch;
 
   // ---- requests and groups ----
   int* const start_s = reinterpret_cast<int*>(lds + SH_ARRAYS);  // [batch + 1] first tokens
   int* const len_s = start_s + a.batch + 1;                      // [batch]
-  int* const first_s = len_s + a.batch + 1;                      // [batch] first own key
-  int* const group_s = first_s + a.batch + 1;                    // [n_groups + 1] first requests
-  int* const shared_s = group_s + a.n_groups + 1;                // [n_groups] shared keys, 0: nobody takes part
+  int* const group_s = len_s + a.batch + 1;                      // [n_groups + 1] first requests
+  int* const shared_s = group_s + a.n_groups + 1;                // [n_groups] shared keys
   int back = 0;
   for (int i = t; i <= a.batch; i += SH_THREADS) {
     auto start = [&](int j) { return a.cu != nullptr ? pg_max(0, pg_min(a.cu[j], a.tokens)) : j; };
@@ -85,7 +94,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   for (int i = a.n_groups > 0 ? t : 1; i <= a.n_groups; i += SH_THREADS) {
     auto first = [&](int j) { return pg_max(0, pg_min(a.groups[j], a.batch)); };
     group_s[i] = first(i);
-    if (i < a.n_groups) shared_s[i] = 0, back |= first(i + 1) < first(i);
+    if (i < a.n_groups) shared_s[i] = pg_max(0, pg_min(a.shared[i], room)), back |= first(i + 1) < first(i);
   }
   // (offsets that go back count as the largest in front of them: searches need them in order)
   if (__syncthreads_or(back)) {
@@ -95,111 +104,90 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
     __syncthreads();
   }
-  const bool tell = blockIdx.x == 0;
-  for (int b = t; b < a.batch; b += SH_THREADS) {
-    int4 what = make_int4(0, 0, 0, start_s[b]);
+  auto request = [&](int b) {
+    ShRequest r = {0, 0, 0, 0, start_s[b], {0, 0, 0}};
     if (a.n_groups > 0) {
       const int i = pg_holder(group_s, a.n_groups, b);
       if (group_s[i] <= b && b < group_s[i + 1]) {
-        const int shared = pg_max(0, pg_min(a.shared[i], room));
-        what.x = sh_first_own(len_s[b], start_s[b + 1] - start_s[b], shared);
-        what.y = i, what.z = start_s[group_s[i]];
-        if (what.x > 0 && start_s[b + 1] > start_s[b]) shared_s[i] = shared;  // (the same from all)
+        r.first_own = sh_first_own(len_s[b], start_s[b + 1] - r.start, shared_s[i]);
+        r.group = i, r.start0 = start_s[group_s[i]], r.end0 = start_s[group_s[i + 1]];
       }
     }
-    first_s[b] = what.x;
-    if (tell) a.of_request[b] = what;
-  }
-  if (tell && t == 0) a.of_request[a.batch] = make_int4(0, 0, 0, start_s[a.batch]);
-  __syncthreads();
-
-  // ---- items, and which of them fall to this workgroup ----
-  auto item = [&](int x, ShItem& p) {  // false: there is none of this number, or it has no keys
-    if (x < a.shared_slots) {
-      int i = 0, hi = a.n_groups;
-      while (hi - i > 1) {
-        const int mid = (i + hi) >> 1;
-        if (pg_first_slot(start_s[group_s[mid]], g, mid, SH_TILE) <= x)
-          i = mid;
-        else
-          hi = mid;
-      }
-      p.table_row = pg_min(group_s[i], a.batch - 1);
-      p.start = start_s[group_s[i]];
-      p.rows = (start_s[group_s[i + 1]] - p.start) * g;
-      p.row0 = (x - (int)pg_first_slot(p.start, g, i, SH_TILE)) * SH_TILE;
-      if (p.row0 < 0 || p.row0 >= p.rows) return false;
-      p.key0 = 0, p.key1 = shared_s[i], p.pos = PG_MAX_KEYS;
+    return r;
+  };
+  auto item = [&](int x) {
+    ShItem p;
+    p.row0 = 0;
+    if (x < n_groups) {
+      p.table_row = pg_min(group_s[x], a.batch - 1);
+      p.start = start_s[group_s[x]];
+      p.rows = (start_s[group_s[x + 1]] - p.start) * g;
+      p.key0 = 0, p.key1 = shared_s[x], p.pos = PG_MAX_KEYS;
+      p.slot = (int)pg_first_slot(p.start, g, x, SH_TILE);
     } else {
-      const int y = x - a.shared_slots;
-      int b = y;
-      if (!a.dense) {
-        b = 0;
-        int hi = a.batch;
-        while (hi - b > 1) {
-          const int mid = (b + hi) >> 1;
-          if (pg_first_slot(start_s[mid], g, mid, SH_TILE) <= y)
-            b = mid;
-          else
-            hi = mid;
-        }
-      }
-      const int q_len = start_s[b + 1] - start_s[b];
+      const int b = x - n_groups;
+      const ShRequest r = request(b);
+      const int q_len = start_s[b + 1] - r.start;
       p.table_row = b;
-      p.start = start_s[b];
+      p.start = r.start;
       p.rows = q_len * g;
-      p.row0 = (y - (int)sh_own_slot(p.start, g, b, a.dense)) * SH_TILE;
-      if (p.row0 < 0 || p.row0 >= p.rows) return false;
-      p.pos = len_s[b] - q_len;
-      p.key0 = first_s[b];
-      p.key1 = pg_min(p.pos + (int)pg_div((unsigned)(pg_min(p.row0 + SH_TILE, p.rows) - 1), a.by_group) + 1, room);
+      p.key0 = r.first_own, p.key1 = pg_min(len_s[b], room), p.pos = len_s[b] - q_len;
+      p.slot = a.shared_slots + (int)sh_own_slot(r.start, g, b, a.dense);
     }
     p.lo = p.key0 / SH_KEYS;
-    p.n = p.key1 > p.key0 ? (p.key1 + SH_KEYS - 1) / SH_KEYS - p.lo : 0;
-    return p.n > 0;
+    p.n = p.rows > 0 && p.key1 > p.key0 ? (p.key1 + SH_KEYS - 1) / SH_KEYS - p.lo : 0;
+    return p;
   };
-  int64_t* const found_s = reinterpret_cast<int64_t*>(lds + SH_FOUND);  // the waves' sums; then the first item's start
-  int* const item_s = reinterpret_cast<int*>(lds + SH_FOUND + 72);
-  int64_t cut0, cut1, at_unit;
-  int x, near;
+
+  // ---- which steps fall to this workgroup ----
+  int from[2], tile[2], at_step[2];  // item, tile and step that the part begins with, and that it ends in front of
+  int near;
   {
-    const int per = (a.slots + SH_THREADS - 1) / SH_THREADS, x0 = t * per, x1 = pg_min(x0 + per, a.slots);
-    ShItem p;
-    int64_t mine = 0;
-    for (int i = x0; i < x1; ++i) mine += item(i, p) ? p.n + SH_OVERHEAD : 0;
-    int64_t at = mine;
+    auto sums = [&](int i0, int* n, int64_t* units, int64_t* upto) {  // of the lane's item; units up to it, it included
+      *n = 0, *units = 0;
+      if (i0 + lane < items) {
+        const ShItem p = item(i0 + lane);
+        *n = p.n, *units = p.n > 0 ? (int64_t)(p.n + SH_OVERHEAD) * ((p.rows + SH_TILE - 1) / SH_TILE) : 0;
+      }
+      int64_t at = *units;
 #pragma unroll
-    for (int o = 1; o < SP_WAVE; o <<= 1) {
-      const int64_t y = __shfl_up(at, o, SP_WAVE);
-      if (lane >= o) at += y;
+      for (int o = 1; o < SP_WAVE; o <<= 1) {
+        const int64_t y = __shfl_up(at, o, SP_WAVE);
+        if (lane >= o) at += y;
+      }
+      *upto = at;
+    };
+    int n = 0;
+    int64_t units = 0, upto = 0, total = 0;
+    for (int i0 = 0; i0 < items; i0 += SP_WAVE) {
+      sums(i0, &n, &units, &upto);
+      total += __shfl(upto, SP_WAVE - 1, SP_WAVE);
     }
-    if (lane == SP_WAVE - 1) found_s[wave] = at;
-    __syncthreads();
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < 2 * WAVES; ++w) {
-      if (w == wave) at += total;
-      total += found_s[w];
-    }
-    at -= mine;
     const int64_t parts = pg_parts(total, a.parts, SH_MIN_SHARE);
     near = pg_near(total, parts);
-    cut0 = part < parts ? pg_cut(total, parts, part) : total;
-    cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
-    if (t == 0) item_s[0] = a.slots;
-    __syncthreads();
-    if (tell || (cut0 < cut1 && cut0 >= at && cut0 < at + mine)) {
-      for (int i = x0; i < x1; ++i) {
-        const int units = item(i, p) ? p.n + SH_OVERHEAD : 0;
-        if (tell) a.starts[i] = at;
-        if (cut0 >= at && cut0 < at + units) item_s[0] = i, found_s[8] = at;
-        at += units;
-      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t cut = part < parts ? pg_cut(total, parts, part + e) : total;
+      from[e] = items, tile[e] = 0, at_step[e] = 0;
+      int64_t before = 0;
+      if (cut < total)
+        for (int i0 = 0; i0 < items; i0 += SP_WAVE) {
+          if (items > SP_WAVE) sums(i0, &n, &units, &upto);
+          const uint64_t here = __ballot(cut < before + upto);
+          if (here != 0ull) {
+            const int i = __builtin_ctzll(here);
+            sh_place(cut - before - (__shfl(upto, i, SP_WAVE) - __shfl(units, i, SP_WAVE)), __shfl(n, i, SP_WAVE), near, &tile[e], &at_step[e]);
+            from[e] = i0 + i;
+            break;
+          }
+          before += __shfl(upto, SP_WAVE - 1, SP_WAVE);
+        }
+      from[e] = __builtin_amdgcn_readfirstlane(from[e]), tile[e] = __builtin_amdgcn_readfirstlane(tile[e]);
+      at_step[e] = __builtin_amdgcn_readfirstlane(at_step[e]);
     }
-    if (tell && t == 0) a.starts[a.slots] = total;
-    __syncthreads();
-    x = __builtin_amdgcn_readfirstlane(item_s[0]);
-    at_unit = (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)found_s[8]) | (int64_t)__builtin_amdgcn_readfirstlane((int)(found_s[8] >> 32)) << 32;
+    if (kvh == 0 && t == 0) a.cuts[part] = make_int4(from[0] - n_groups, at_step[0], from[1] - n_groups, at_step[1]);
+    if (blockIdx.x == 0)
+      for (int b = t; b <= a.batch; b += SH_THREADS) a.of_request[b] = b < a.batch ? request(b) : ShRequest{0, 0, 0, 0, start_s[a.batch], {0, 0, 0}};
   }
 
   // Arguments of what is done once an item are read where they are used: scalar registers do not suffice to keep them.
@@ -549,7 +537,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
         const float mw = m_s[w * SH_TILE + r];
-        const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);  // (a wave without keys, or without a finite logit: 0)
+        const float f = mw == -INFINITY && l_s[w * SH_TILE + r] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mw - top);  // (a wave without keys: 0)
         sum += l_s[w * SH_TILE + r] * f;
         acc += *reinterpret_cast<const ds_floatx4*>(o_s + (w * SH_TILE + r) * D + (c ^ (r & 15)) * 4) * f;
       }
@@ -568,189 +556,192 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
   };
 
-  for (ShItem p; x < a.slots && at_unit < cut1; ++x) {
-    if (!item(x, p)) continue;
-    int begin, end;
-    sh_steps(at_unit, p.n, cut0, cut1, near, &begin, &end);
-    at_unit += p.n + SH_OVERHEAD;
-    if (begin >= end) continue;
-    ShItem u;  // (uniform: out of vector registers)
-    u.table_row = __builtin_amdgcn_readfirstlane(p.table_row), u.start = __builtin_amdgcn_readfirstlane(p.start);
-    u.row0 = __builtin_amdgcn_readfirstlane(p.row0), u.rows = __builtin_amdgcn_readfirstlane(p.rows);
-    u.key0 = __builtin_amdgcn_readfirstlane(p.key0), u.key1 = __builtin_amdgcn_readfirstlane(p.key1);
-    u.pos = __builtin_amdgcn_readfirstlane(p.pos), u.lo = __builtin_amdgcn_readfirstlane(p.lo), u.n = __builtin_amdgcn_readfirstlane(p.n);
-    begin = __builtin_amdgcn_readfirstlane(begin), end = __builtin_amdgcn_readfirstlane(end);
-    if (u.rows - u.row0 <= 16)
-      run(std::integral_constant<int, 1>{}, u, begin, end, x < a.shared_slots);
-    else
-      run(std::integral_constant<int, SH_TILE / 32>{}, u, begin, end, x < a.shared_slots);
+  for (int x = from[0], first_tile = tile[0], begin = at_step[0]; x < items && x <= from[1]; ++x, first_tile = 0, begin = 0) {
+    ShItem p = item(x);
+    if (p.n == 0) continue;
+    // (uniform: out of vector registers)
+    p.table_row = __builtin_amdgcn_readfirstlane(p.table_row), p.start = __builtin_amdgcn_readfirstlane(p.start);
+    p.rows = __builtin_amdgcn_readfirstlane(p.rows), p.key0 = __builtin_amdgcn_readfirstlane(p.key0);
+    p.pos = __builtin_amdgcn_readfirstlane(p.pos), p.lo = __builtin_amdgcn_readfirstlane(p.lo), p.n = __builtin_amdgcn_readfirstlane(p.n);
+    p.slot = __builtin_amdgcn_readfirstlane(p.slot);
+    const int key1 = __builtin_amdgcn_readfirstlane(p.key1);
+    for (int at = first_tile; at * SH_TILE < p.rows; ++at, begin = 0) {
+      const bool last = x == from[1] && at == tile[1];
+      const int end = last ? pg_min(at_step[1], p.n) : p.n;
+      if (x == from[1] && at > tile[1]) break;
+      if (begin >= end) continue;
+      p.row0 = at * SH_TILE;
+      // (of a request's tile: up to its last row's position)
+      p.key1 = x < n_groups ? key1 : pg_min(key1, p.pos + (int)pg_div((unsigned)(pg_min(p.row0 + SH_TILE, p.rows) - 1), a.by_group) + 1);
+      if (kvh == 0 && t == 0) {
+        if (begin == 0) a.parts_of[p.slot + at].x = part;
+        if (end == p.n) a.parts_of[p.slot + at].y = part;
+      }
+      if (p.rows - p.row0 <= 16)
+        run(std::integral_constant<int, 1>{}, p, begin, end, x < n_groups);
+      else
+        run(std::integral_constant<int, SH_TILE / 32>{}, p, begin, end, x < n_groups);
+    }
   }
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------
-// What the parts of an item left of a row: visit(row of ml_part / o_part, row of ml_row / o_row, whole).
-struct ShLine {
-  int64_t total, parts;
-  int near;
-};
-__device__ __forceinline__ ShLine sh_line(const ShArgs& a) {
-  ShLine s;
-  s.total = a.starts[a.slots];
-  s.parts = s.total > 0 ? pg_parts(s.total, a.parts, SH_MIN_SHARE) : 0;
-  s.near = s.total > 0 ? pg_near(s.total, s.parts) : 0;
-  return s;
-}
-struct ShParts {  // of an item
-  int64_t start, first;
-  int n, count;  // steps; parts that may hold some of them
-};
-__device__ __forceinline__ ShParts sh_parts(const ShArgs& a, const ShLine& s, int x) {
-  ShParts p = {a.starts[x], 0, 0, 0};
-  const int64_t end = a.starts[x + 1];
-  if (end == p.start) return p;
-  p.n = (int)(end - p.start) - SH_OVERHEAD;
-  p.first = sh_part(p.start, s.total, s.parts);
-  p.count = (int)(sh_part(end - 1, s.total, s.parts) - p.first) + 1;
-  return p;
-}
-// Place i of an item's parts holds steps of it: where a row (of kv head kvh, place `in_tile` of its tile, number `row` among all) stands; < 0: it holds none.
-// Rows of ml_part come first, those of ml_row behind them.
-#define SH_NOWHERE (-1)
-__device__ __forceinline__ int64_t sh_place(const ShArgs& a, const ShLine& s, const ShParts& p, int i, int kvh, int in_tile, int64_t row, bool of_group,
-                                            bool* whole) {
-  int begin, end;
-  const int64_t part = p.first + i;
-  sh_steps(p.start, p.n, pg_cut(s.total, s.parts, part), pg_cut(s.total, s.parts, part + 1), s.near, &begin, &end);
-  *whole = begin == 0 && end == p.n;
-  if (begin >= end) return SH_NOWHERE;
-  if (*whole) return (of_group ? 0 : (int64_t)a.tokens * (a.hkv * a.group)) + row;
-  return ((part * a.hkv + kvh) * 2 + (begin == 0 ? 1 : 0)) * SH_TILE + in_tile;
-}
-// the items of a row: its group's (-1: it takes part in none) and its request's, and its places in their tiles
+// The number of a row's tile (group, or request), and the row's place in it.
 struct ShRow {
-  int item[2], in_tile[2];
+  int slot, in_tile;
 };
-__device__ __forceinline__ ShRow sh_row(const ShArgs& a, int b, int4 what, int token, int h) {
-  ShRow r;
-  const int in_group = (token - what.z) * a.group + h, in_own = (token - what.w) * a.group + h;
-  r.item[0] = what.x > 0 ? (int)pg_first_slot(what.z, a.group, what.y, SH_TILE) + in_group / SH_TILE : -1;
-  r.in_tile[0] = in_group % SH_TILE;
-  r.item[1] = a.shared_slots + (int)sh_own_slot(what.w, a.group, b, a.dense) + in_own / SH_TILE;
-  r.in_tile[1] = in_own % SH_TILE;
-  return r;
+__device__ __forceinline__ ShRow sh_group_row(const ShArgs& a, const ShRequest& r, int token, int h) {
+  const int row = (token - r.start0) * a.group + h;
+  return ShRow{(int)pg_first_slot(r.start0, a.group, r.group, SH_TILE) + row / SH_TILE, row % SH_TILE};
+}
+__device__ __forceinline__ ShRow sh_own_row(const ShArgs& a, const ShRequest& r, int b, int token, int h) {
+  const int row = (token - r.start) * a.group + h;
+  return ShRow{a.shared_slots + (int)sh_own_slot(r.start, a.group, b, a.dense) + row / SH_TILE, row % SH_TILE};
+}
+// Parts that hold some of it: (0, -1) where there are no keys.
+__device__ __forceinline__ int2 sh_group_parts(const ShArgs& a, const ShRequest& r, const ShRow& row) {
+  return r.first_own == 0 ? make_int2(0, -1) : a.apart ? make_int2(0, 0) : a.parts_of[row.slot];
+}
+__device__ __forceinline__ int2 sh_own_parts(const ShArgs& a, const ShRequest& r, int b, const ShRow& row) {
+  return pg_min(a.lens[b], a.width << a.shift) > r.first_own ? a.parts_of[row.slot] : make_int2(0, -1);
+}
+// Where part i of a tile that parts.x .. parts.y hold stands: in o_row and ml_row where there is but one, else in o_part and ml_part.
+__device__ __forceinline__ int64_t sh_slab(const ShArgs& a, int2 parts, int i, int kvh, int in_tile) {
+  return ((int64_t)((parts.x + i) * a.hkv + kvh) * 2 + (i == 0 ? 1 : 0)) * SH_TILE + in_tile;
 }
 
 #define SM_THREADS 256
-// A row's parts joined, D / 4 threads a row, and behind those workgroups, where weights are kept, one for every part of the line:
-//   weight[j] += sum over the group's heads of 2^(logit - m) / l for the own keys that fall to the part.
+// A row's parts joined, D / 4 threads a row.
 template <int D>
-__global__ __launch_bounds__(SM_THREADS) void sp_shared_join_kernel(const ShArgs a, int join_blocks) {
-  const int t = threadIdx.x;
-  const int hq = a.hkv * a.group;
-  const ShLine line = sh_line(a);
-  if ((int)blockIdx.x < join_blocks) {
-    constexpr int WIDTH = D / 4, PER = SM_THREADS / WIDTH;
-    const int64_t row = (int64_t)blockIdx.x * PER + t / WIDTH;
-    const int c = t % WIDTH * 4;
-    if (row >= (int64_t)a.tokens * hq) return;
-    const int token = (int)(row / hq), head = (int)(row % hq), kvh = head / a.group;
-    int b = token;
-    if (a.cu != nullptr) {
-      b = 0;
-      int hi = a.batch;
-      while (hi - b > 1) {
-        const int mid = (b + hi) >> 1;
-        if (a.of_request[mid].w <= token)
-          b = mid;
-        else
-          hi = mid;
-      }
+__device__ __forceinline__ void sh_join(const ShArgs& a) {
+  constexpr int WIDTH = D / 4, PER = SM_THREADS / WIDTH, AHEAD = 8;
+  const int t = threadIdx.x, hq = a.hkv * a.group, c = t % WIDTH * 4;
+  const unsigned row = blockIdx.x * PER + t / WIDTH;
+  if (row >= (unsigned)a.tokens * (unsigned)hq) return;
+  const int token = (int)(row / (unsigned)hq), head = (int)(row - (unsigned)token * (unsigned)hq), kvh = (int)pg_div((unsigned)head, a.by_group);
+  int b = token;
+  if (a.cu != nullptr) {
+    b = 0;
+    int hi = a.batch;
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if (a.of_request[mid].start <= token)
+        b = mid;
+      else
+        hi = mid;
     }
-    const int4 what = a.of_request[b];
-    if (token < what.w || token >= a.of_request[b + 1].w) return;  // (a row outside every request)
-    const ShRow r = sh_row(a, b, what, token, head - kvh * a.group);
-    float top = CK_NO_MAX, sum = 0.f;
-    ds_floatx4 acc = {0, 0, 0, 0};
-    for (int which = 0; which < 2; ++which) {
-      if (r.item[which] < 0) continue;
-      const ShParts p = sh_parts(a, line, r.item[which]);
-#pragma unroll 4
-      for (int i = 0; i < p.count; ++i) {
-        bool whole;
-        const int64_t at = sh_place(a, line, p, i, kvh, r.in_tile[which], row, which == 0, &whole);
-        if (at < 0) continue;
-        if (whole && which == 1 && what.x == 0) return;  // (the row is done)
-        const float2 ml = (whole ? a.ml_row : a.ml_part)[at];
-        const ds_floatx4 o = *reinterpret_cast<const ds_floatx4*>((whole ? a.o_row : a.o_part) + at * D + c);
-        const float to = fmaxf(top, ml.x), f0 = __builtin_amdgcn_exp2f(top - to), f1 = __builtin_amdgcn_exp2f(ml.x - to);
-        sum = sum * f0 + ml.y * f1;
-        acc = acc * f0 + o * f1;
-        top = to;
+  }
+  const ShRequest r = a.of_request[b];
+  const int end = a.of_request[b + 1].start;
+  if (token < r.start || token >= end) return;  // (a row outside every request)
+  const int h = head - kvh * a.group;
+  const ShRow own = sh_own_row(a, r, b, token, h), group = sh_group_row(a, r, token, h);
+  const int2 own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
+  if (r.first_own == 0 && own_parts.x == own_parts.y) return;  // (the row is done)
+  float top = CK_NO_MAX, sum = 0.f;
+  ds_floatx4 acc = {0, 0, 0, 0};
+  auto add = [&](const ShRow& it, int2 parts, bool of_group) {
+    const int count = parts.y - parts.x + 1;
+    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+      float2 ml[AHEAD];
+      ds_floatx4 o[AHEAD];
+      float to = top;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = pg_min(i0 + u, count - 1);
+        const int64_t at = count > 1 ? sh_slab(a, parts, i, kvh, it.in_tile) : (of_group ? 0 : (int64_t)a.tokens * hq) + row;
+        ml[u] = (count > 1 ? a.ml_part : a.ml_row)[at];
+        o[u] = *reinterpret_cast<const ds_floatx4*>((count > 1 ? a.o_part : a.o_row) + at * D + c);
       }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) to = fmaxf(to, ml[u].x);
+      const float before = __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      sum *= before;
+      acc *= before;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (i0 + u < count) {
+          const float f = __builtin_amdgcn_exp2f(ml[u].x - top);
+          sum += ml[u].y * f;
+          acc += o[u] * f;
+        }
     }
-    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(a.out + row * D + c) = make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
-    return;
-  }
-  // ---- weights of the own keys between two cuts (single tokens) ----
-  __shared__ float m_s[PD_MAX_GROUP], inv_s[PD_MAX_GROUP];
-  const int w = blockIdx.x - join_blocks, kvh = w % a.hkv, part = w / a.hkv, lane = t & 63, wave = t >> 6;
-  if (part >= line.parts) return;
-  const int64_t cut0 = pg_cut(line.total, line.parts, part), cut1 = pg_cut(line.total, line.parts, part + 1);
-  int x = a.shared_slots, hi = a.slots;
-  while (hi - x > 1) {  // the last request's item that starts at or in front of the cut
-    const int mid = (x + hi) >> 1;
-    if (a.starts[mid] <= cut0)
-      x = mid;
-    else
-      hi = mid;
-  }
-  for (; x < a.slots && a.starts[x] < cut1; ++x) {
-    const ShParts p = sh_parts(a, line, x);
-    if (p.count == 0) continue;
-    int begin, end;
-    sh_steps(p.start, p.n, cut0, cut1, line.near, &begin, &end);
-    if (begin >= end) continue;
-    const int b = x - a.shared_slots;
-    const int4 what = a.of_request[b];
-    const int len = pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS)), room = a.width << a.shift;
+  };
+  add(group, group_parts, true);
+  add(own, own_parts, false);
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(a.out + (int64_t)row * D + c) = make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
+}
+
+// Weights of the own keys that fell to part w / hkv of kv head w % hkv (single tokens):
+//   weight[j] += sum over the group's heads of 2^(logit - m) / l.
+__device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
+  __shared__ float2 ml_s[PD_MAX_GROUP];  // of a head: m, 1 / l
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, hq = a.hkv * a.group, kvh = w % a.hkv, part = w / a.hkv;
+  const int4 cut = a.cuts[part];
+  const int room = a.width << a.shift;
+  for (int b = pg_max(cut.x, 0); b < a.batch && b <= cut.z; ++b) {
+    const ShRequest r = a.of_request[b];
+    const int len = pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS));
+    const int lo = r.first_own / SH_KEYS, keys = pg_min(len, room);
+    const int begin = b == cut.x ? cut.y : 0, end = b == cut.z ? cut.w : PG_MAX_KEYS / SH_KEYS;
+    if (keys <= r.first_own || begin >= end) continue;
     __syncthreads();  // (the rows before are done with)
     for (int h = wave; h < a.group; h += SM_THREADS / SP_WAVE) {  // a lane a part
-      const ShRow r = sh_row(a, b, what, b, h);
+      const ShRow own = sh_own_row(a, r, b, b, h), group = sh_group_row(a, r, b, h);
+      const int2 own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
       float top = CK_NO_MAX, sum = 0.f;
-      for (int which = 0; which < 2; ++which) {
-        if (r.item[which] < 0) continue;
-        const ShParts q = sh_parts(a, line, r.item[which]);
-        for (int i0 = 0; i0 < q.count; i0 += SP_WAVE) {
+      auto add = [&](int in_tile, int2 held, bool of_group) {
+        const int count = held.y - held.x + 1;
+        for (int i0 = 0; i0 < count; i0 += SP_WAVE) {
           float2 ml = make_float2(CK_NO_MAX, 0.f);
-          bool whole;
-          const int64_t at = i0 + lane < q.count ? sh_place(a, line, q, i0 + lane, kvh, r.in_tile[which], (int64_t)b * hq + kvh * a.group + h, which == 0, &whole)
-                                                 : SH_NOWHERE;
-          if (at >= 0) ml = (whole ? a.ml_row : a.ml_part)[at];
+          if (i0 + lane < count)
+            ml = count > 1 ? a.ml_part[sh_slab(a, held, i0 + lane, kvh, in_tile)]
+                           : a.ml_row[(of_group ? 0 : (int64_t)a.tokens * hq) + (int64_t)b * hq + kvh * a.group + h];
           const float to = fmaxf(top, sp_wave_max(ml.x));
-          sum = sum * __builtin_amdgcn_exp2f(top - to) + sp_wave_sum(at >= 0 ? ml.y * __builtin_amdgcn_exp2f(ml.x - to) : 0.f);
+          sum = sum * __builtin_amdgcn_exp2f(top - to) + sp_wave_sum(i0 + lane < count ? ml.y * __builtin_amdgcn_exp2f(ml.x - to) : 0.f);
           top = to;
         }
-      }
-      if (lane == 0) m_s[h] = top, inv_s[h] = sum == 0.f ? 0.f : 1.0f / sum;
+      };
+      add(group.in_tile, group_parts, true);
+      add(own.in_tile, own_parts, false);
+      if (lane == 0) ml_s[h] = make_float2(top, sum == 0.f ? 0.f : 1.0f / sum);
     }
     __syncthreads();
-    const int lo = what.x / SH_KEYS, first = (lo + begin) * SH_KEYS, last = pg_min(pg_min((lo + end) * SH_KEYS, len), room);
+    const int first = (lo + begin) * SH_KEYS, last = (int)pg_min((int)(lo + end < keys / SH_KEYS + 1 ? (lo + end) * SH_KEYS : keys), keys);
     for (int key = first + 4 * t; key < last; key += 4 * SM_THREADS) {
       const int id = a.table[b * a.table_stride + (key >> a.shift)], in = key & ((1 << a.shift) - 1);
       if ((unsigned)id >= (unsigned)a.num_pages) continue;
+      const float* const from = a.logits + (((int64_t)id * a.hkv + kvh) * a.group << a.shift) + in;
       ds_floatx4 sum = {0, 0, 0, 0};
-      for (int h = 0; h < a.group; ++h) {
-        const ds_floatx4 s = *reinterpret_cast<const ds_floatx4*>(a.logits + (((int64_t)id * a.hkv + kvh) * a.group + h) * (1 << a.shift) + in);
+      for (int h0 = 0; h0 < a.group; h0 += 4) {
+        ds_floatx4 s[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[j] - m_s[h]) * inv_s[h];
+        for (int u = 0; u < 4; ++u) s[u] = *reinterpret_cast<const ds_floatx4*>(from + ((int64_t)pg_min(h0 + u, a.group - 1) << a.shift));
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (h0 + u < a.group) {
+            const float2 ml = ml_s[h0 + u];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[u][j] - ml.x) * ml.y;
+          }
       }
       float* const to = a.weights + id * a.sw_p + kvh * a.sw_h + in;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (key + j >= what.x && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
+        if (key + j >= r.first_own && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
     }
   }
+}
+
+// The workgroups behind the joining ones, where weights are kept: one for every part of the line.
+template <int D>
+__global__ __launch_bounds__(SM_THREADS) void sp_shared_join_kernel(const ShArgs a, int join_blocks) {
+  if ((int)blockIdx.x < join_blocks)
+    sh_join<D>(a);
+  else
+    sh_weigh(a, (int)blockIdx.x - join_blocks);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
@@ -759,12 +750,13 @@ static int sh_workgroups(int64_t hkv) { return hkv < SH_PLACES ? SH_PLACES / (in
 
 struct ShSizes {
   int64_t shared_slots, slots, logits;
-  size_t o_part, ml_part, o_row, ml_row, starts, of_request, bytes;
+  size_t o_part, ml_part, o_row, ml_row, parts_of, cuts, of_request, bytes;
 };
 static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d, bool single, int64_t pool_keys) {
   ShSizes s;
   const int64_t g = hq / hkv;
-  s.shared_slots = groups > 0 ? tokens * g / SH_TILE + groups : 0;
+  const bool apart = sh_apart(tokens, groups, g);
+  s.shared_slots = groups > 0 && !apart ? tokens * g / SH_TILE + groups : 0;
   s.slots = s.shared_slots + (single && g <= SH_TILE ? batch : tokens * g / SH_TILE + batch);
   const int64_t rows = (int64_t)sh_workgroups(hkv) * hkv * 2 * SH_TILE;
   size_t at = 0;
@@ -773,19 +765,21 @@ static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t h
     at += (n + 255) / 256 * 256;
     return here;
   };
-  s.o_part = take((size_t)rows * d * sizeof(float));
+  // (the groups' partials are joined before those of the requests are written)
+  s.o_part = take(apart ? ck_groups_workspace_bytes((int)hkv, (int)d) : (size_t)rows * d * sizeof(float));
   s.ml_part = take((size_t)rows * sizeof(float2));
   s.o_row = take(groups > 0 ? (size_t)(2 * tokens * hq) * d * sizeof(float) : 0);
   s.ml_row = take((size_t)(2 * tokens * hq) * sizeof(float2));
-  s.starts = take((size_t)(s.slots + 1) * sizeof(int64_t));
-  s.of_request = take((size_t)(batch + 1) * sizeof(int4));
+  s.parts_of = take((size_t)s.slots * sizeof(int2));
+  s.cuts = take((size_t)sh_workgroups(hkv) * sizeof(int4));
+  s.of_request = take((size_t)(batch + 1) * sizeof(ShRequest));
   s.logits = (int64_t)take((size_t)pool_keys * hq * sizeof(float));
   s.bytes = at;
   return s;
 }
 static bool sh_shape_ok(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d) {
   return tokens > 0 && batch > 0 && batch <= SH_MAX_SEQS && groups >= 0 && groups <= batch && hq > 0 && hkv > 0 && hq % hkv == 0 && (d == 64 || d == 128) &&
-         tokens <= PG_MAX_KEYS && hq <= 65536 && tokens * (hq / hkv) < (1ll << 31);
+         tokens <= PG_MAX_KEYS && hq <= 65536 && tokens * hq < (1ll << 31);
 }
 
 extern "C" size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t groups, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens,
@@ -849,11 +843,11 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   a.n_groups = (int)x->groups;
   a.hkv = (int)x->hkv, a.group = (int)g, a.dense = x->cu_q == nullptr && g <= SH_TILE;
   a.by_group = pg_divisor((unsigned)g);
-  a.shared_slots = (int)s.shared_slots, a.slots = (int)s.slots;
+  a.shared_slots = (int)s.shared_slots;
   a.parts = sh_workgroups(x->hkv);
   a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
   a.o_part = (float*)(ws + s.o_part), a.ml_part = (float2*)(ws + s.ml_part), a.o_row = (float*)(ws + s.o_row), a.ml_row = (float2*)(ws + s.ml_row);
-  a.starts = (int64_t*)(ws + s.starts), a.of_request = (int4*)(ws + s.of_request);
+  a.parts_of = (int2*)(ws + s.parts_of), a.cuts = (int4*)(ws + s.cuts), a.of_request = (ShRequest*)(ws + s.of_request);
   a.weights = x->weights, a.logits = (float*)(ws + s.logits);
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -868,6 +862,17 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   const int grid = a.parts * a.hkv;
   const int64_t join = sp_ceil_div(x->tokens * x->hq, SM_THREADS / (x->d / 4));
   SP_REQUIRE(join + grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens, (long long)x->hq);
+  a.apart = sh_apart(x->tokens, x->groups, g);
+  if (a.apart) {
+    CkArgs c = {};
+    c.q = a.q, c.k = a.k, c.v = a.v, c.table = a.table, c.lens = a.shared, c.cu = a.cu, c.groups = a.groups, c.o_row = a.o_row, c.ml_row = a.ml_row;
+    c.table_stride = a.table_stride, c.sq_n = a.sq_n, c.sq_h = a.sq_h;
+    c.sk_p = a.sk_p, c.sk_n = a.sk_n, c.sk_h = a.sk_h, c.sv_p = a.sv_p, c.sv_n = a.sv_n, c.sv_h = a.sv_h;
+    c.batch = a.n_groups, c.n_seqs = a.batch, c.tokens = a.tokens, c.width = a.width, c.num_pages = a.num_pages, c.shift = a.shift, c.n_queries = 1;
+    c.hkv = a.hkv, c.group = a.group, c.scale_log2 = a.scale_log2;
+    const int rc = ck_groups_launch(c, (int)x->d, ws + s.o_part, stream);
+    if (rc) return rc;
+  }
   const unsigned joins = (unsigned)(join + (a.weights != nullptr ? grid : 0));
   const size_t lds = sh_lds_bytes(a.batch, a.n_groups);
   if (x->d == 64) {
