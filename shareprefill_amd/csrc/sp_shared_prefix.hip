@@ -4,17 +4,19 @@
 // sums l of either side, out = (2^(m1 - m) o1 + 2^(m2 - m) o2) / (2^(m1 - m) l1 + 2^(m2 - m) l2).
 //
 // HBM-bound as long as a group has fewer than some 250 rows a kv head, (token, query head) pairs: shared keys are read once per tile of 64 rows, a
-// request's own once.  Tiles of 16 rows or fewer (a request's single token) take the loop of the single-token kernel (sp_paged_decode.hip): four waves
-// take steps of 32 keys in turn, each with a ring of operands in LDS that direct loads fill, no barrier between them, and meet in LDS at the end.  In
-// larger tiles two waves of 32 rows each share a ring, and all meet at a barrier every four steps; the two share a SIMD, where the matrix
-// instructions of one run under the exponentials of the other.  Groups of many rows go to sp_chunk.hip's loop first, in a launch of its own.
+// request's own once.  Three loops over steps of 32 keys, whose operands direct loads bring to rings in LDS:
+//   * single tokens of up to 16 heads over their own keys: a wave goes by itself through the steps of one request after the other, the next one's
+//     first keys on their way under the end of the one in front; no barrier, and nobody waits for a request to end;
+//   * other tiles of up to 16 rows: four waves take the tile's steps in turn and meet in LDS at the end;
+//   * larger tiles: two waves of 32 rows each share a ring, and all meet at a barrier every four steps; the two share a SIMD, where the matrix
+//     instructions of one run under the exponentials of the other.
+// Groups of many rows go to sp_chunk.hip's loop first, in a launch of its own.
 //
 // The line that the workgroups' parts are cut from (sp_shared_plan.h) is formed by every wave for itself, 64 items at a time.
 #include "sp_chunk.h"
 #include "sp_ring.h"
 #include "sp_shared_plan.h"
 
-#define SH_WAVES 4  // that share the keys
 #define SH_THREADS (2 * SH_WAVES * SP_WAVE)
 // Octaves by which a row's logits may pass its running maximum before that is moved and what has been summed is scaled: nearly all steps go without.
 // (Probabilities up to 2^7 are as exact in bf16 as those below 1.)
@@ -37,15 +39,19 @@ struct ShArgs {
   int shared_slots;           // numbers of the groups' row tiles
   int parts;                  // of the line at most, and workgroups of a kv head
   int apart;                  // groups have been seen to (o_row, ml_row)
+  int streams;                // single tokens of up to 16 heads: a request's parts are waves', four a workgroup
   float scale_log2;
   float* o_part;              // [part][kv head][2][SH_TILE][D]: a row tile that began in an earlier part, one that goes on in the next
   float2* ml_part;            // [part][kv head][2][SH_TILE]
+  float* o_stream;            // [part of a wave][kv head][2][16][D]
+  float2* ml_stream;
   float* o_row;               // [2][token][query head][D]: row tiles that lie in one part, of groups and of requests
   float2* ml_row;
   int2* parts_of;             // by row tile number: first and last part that hold steps of it
-  int4* cuts;                 // [parts]: item and step that a part begins with, those that it ends in front of
+  int4* cuts;                 // [part of a wave]: request and step that it begins with, those that it ends in front of
   ShRequest* of_request;      // [batch + 1]
   float* weights;             // null, or [num_pages][kv head][page]
+  int weights_by_four;        // four places side by side are one access
   float* logits;              // [num_pages][query head][page]: scaled logits of own keys, in octaves
 };
 
@@ -54,9 +60,17 @@ using ShShape = DsShape<D, D / 16, SH_WAVES, 128>;
 // LDS: the rings, where the waves meet afterwards; their maxima and sums; what is known of the requests and groups
 #define SH_RING 131072
 #define SH_ML (SH_RING)                                // [2][SH_WAVES][SH_TILE] floats
-#define SH_ARRAYS (SH_ML + 2 * SH_WAVES * SH_TILE * 4)
-static size_t sh_lds_bytes(int batch, int groups) { return SH_ARRAYS + (2 * ((size_t)batch + 1) + 2 * ((size_t)groups + 1)) * sizeof(int); }
-static_assert(ShShape<128>::LDS_BYTES <= SH_RING && ShShape<64>::LDS_BYTES <= SH_RING && SH_WAVES * SH_TILE * 128 * 4 <= SH_RING, "");
+#define SH_SUMS (SH_ML + 2 * SH_WAVES * SH_TILE * 4)  // [2 SH_WAVES + 1] int64
+#define SH_ARRAYS (SH_SUMS + 80)
+static size_t sh_lds_bytes(int batch, int groups) { return SH_ARRAYS + (3 * ((size_t)batch + 1) + 2 * ((size_t)groups + 1)) * sizeof(int); }
+static_assert(ShShape<128>::LDS_BYTES <= SH_RING && ShShape<64>::LDS_BYTES <= SH_RING && SH_WAVES * SH_TILE * 128 * 4 <= SH_RING && (2 * SH_MAX_SEQS + 1) * 8 <= SH_RING, "");
+
+template <int IMM>
+__device__ static __forceinline__ dc_u32x4 sh_read_k(uint32_t addr) {  // (as ds_read_k)
+  dc_u32x4 r;
+  asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(r) : "v"(addr), "n"(IMM));
+  return r;
+}
 
 struct ShItem {
   int table_row;    // of the block table
@@ -83,7 +97,8 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   // ---- requests and groups ----
   int* const start_s = reinterpret_cast<int*>(lds + SH_ARRAYS);  // [batch + 1] first tokens
   int* const len_s = start_s + a.batch + 1;                      // [batch]
-  int* const group_s = len_s + a.batch + 1;                      // [n_groups + 1] first requests
+  int* const first_s = len_s + a.batch + 1;                      // [batch] first own keys
+  int* const group_s = first_s + a.batch + 1;                    // [n_groups + 1] first requests
   int* const shared_s = group_s + a.n_groups + 1;                // [n_groups] shared keys
   int back = 0;
   for (int i = t; i <= a.batch; i += SH_THREADS) {
@@ -125,69 +140,100 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       p.key0 = 0, p.key1 = shared_s[x], p.pos = PG_MAX_KEYS;
       p.slot = (int)pg_first_slot(p.start, g, x, SH_TILE);
     } else {
-      const int b = x - n_groups;
-      const ShRequest r = request(b);
-      const int q_len = start_s[b + 1] - r.start;
+      const int b = x - n_groups, q_len = start_s[b + 1] - start_s[b];
       p.table_row = b;
-      p.start = r.start;
+      p.start = start_s[b];
       p.rows = q_len * g;
-      p.key0 = r.first_own, p.key1 = pg_min(len_s[b], room), p.pos = len_s[b] - q_len;
-      p.slot = a.shared_slots + (int)sh_own_slot(r.start, g, b, a.dense);
+      p.key0 = first_s[b], p.key1 = pg_min(len_s[b], room), p.pos = len_s[b] - q_len;
+      p.slot = a.shared_slots + (int)sh_own_slot(p.start, g, b, a.dense);
     }
     p.lo = p.key0 / SH_KEYS;
     p.n = p.rows > 0 && p.key1 > p.key0 ? (p.key1 + SH_KEYS - 1) / SH_KEYS - p.lo : 0;
     return p;
   };
 
-  // ---- which steps fall to this workgroup ----
-  int from[2], tile[2], at_step[2];  // item, tile and step that the part begins with, and that it ends in front of
-  int near;
+  // ---- the line: where every item starts, in the place of the rings ----
+  int64_t* const line_s = reinterpret_cast<int64_t*>(lds);  // [items + 1]
+  int64_t total = 0;
   {
-    auto sums = [&](int i0, int* n, int64_t* units, int64_t* upto) {  // of the lane's item; units up to it, it included
-      *n = 0, *units = 0;
-      if (i0 + lane < items) {
-        const ShItem p = item(i0 + lane);
-        *n = p.n, *units = p.n > 0 ? (int64_t)(p.n + SH_OVERHEAD) * ((p.rows + SH_TILE - 1) / SH_TILE) : 0;
+    int64_t* const sums_s = reinterpret_cast<int64_t*>(lds + SH_SUMS);
+    const int per = (items + SH_THREADS - 1) / SH_THREADS, x0 = t * per, x1 = pg_min(x0 + per, items);
+    int64_t at = 0;
+    for (int x = x0; x < x1; ++x) {
+      if (x >= n_groups) {
+        const ShRequest r = request(x - n_groups);
+        first_s[x - n_groups] = r.first_own;
+        if (blockIdx.x == 0) a.of_request[x - n_groups] = r;
       }
-      int64_t at = *units;
-#pragma unroll
-      for (int o = 1; o < SP_WAVE; o <<= 1) {
-        const int64_t y = __shfl_up(at, o, SP_WAVE);
-        if (lane >= o) at += y;
-      }
-      *upto = at;
-    };
-    int n = 0;
-    int64_t units = 0, upto = 0, total = 0;
-    for (int i0 = 0; i0 < items; i0 += SP_WAVE) {
-      sums(i0, &n, &units, &upto);
-      total += __shfl(upto, SP_WAVE - 1, SP_WAVE);
+      const ShItem p = item(x);
+      const int64_t units = sh_units(p.n, p.rows, a.streams && x >= n_groups);
+      line_s[x] = at;  // (of the thread's; completed below)
+      at += units;
     }
-    const int64_t parts = pg_parts(total, a.parts, SH_MIN_SHARE);
-    near = pg_near(total, parts);
+    const int64_t mine = at;
+#pragma unroll
+    for (int o = 1; o < SP_WAVE; o <<= 1) {
+      const int64_t y = __shfl_up(at, o, SP_WAVE);
+      if (lane >= o) at += y;
+    }
+    if (lane == SP_WAVE - 1) sums_s[wave] = at;
+    if (blockIdx.x == 0 && t == 0) a.of_request[a.batch] = ShRequest{0, 0, 0, 0, start_s[a.batch], {0, 0, 0}};
+    __syncthreads();
+    at -= mine;
+#pragma unroll
+    for (int w = 0; w < 2 * WAVES; ++w) {
+      if (w == wave) at += total;
+      total += sums_s[w];
+    }
+    for (int x = x0; x < x1; ++x) line_s[x] += at;
+    if (t == 0) line_s[items] = total;
+    __syncthreads();
+  }
+  auto uniform64 = [](int64_t x) {
+    return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+  };
+  total = uniform64(total);
+  auto find = [&](int64_t cut) {  // the item that unit `cut` < total of the line lies in: the last that starts at or in front of it, by 64 candidates at a time
+    int lo = 0, span = items;
+    while (span > 1) {
+      const int step = (span + SP_WAVE - 1) / SP_WAVE;
+      const int n = __builtin_popcountll(__ballot(lane * step < span && line_s[lo + lane * step] <= cut));
+      const int at = pg_max(n - 1, 0) * step;
+      span = pg_min(step, span - at);
+      lo += at;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+  };
+  const int64_t parts = pg_parts(total, a.parts, SH_MIN_SHARE);
+  const int near = pg_near(total, parts);
+  const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
+  // Of the streams the groups alone are the workgroup's matter, else all items are.
+  const int shared_items = a.streams ? n_groups : items;
+  const int64_t shared_units = uniform64(line_s[shared_items]);
+  int from[2], tile[2], at_step[2];  // item, tile and step that the part begins with, and that it ends in front of
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int64_t cut = e == 0 ? cut0 : cut1;
+    from[e] = shared_items, tile[e] = 0, at_step[e] = 0;
+    if (cut < shared_units) {
+      from[e] = find(cut);
+      sh_place(cut - line_s[from[e]], item(from[e]).n, near, &tile[e], &at_step[e]);
+    }
+    tile[e] = __builtin_amdgcn_readfirstlane(tile[e]), at_step[e] = __builtin_amdgcn_readfirstlane(at_step[e]);
+  }
+  int stream_b[2] = {a.batch, a.batch}, stream_step[2] = {0, 0};  // the same of a wave of the streams: request and step
+  if (a.streams && wave < WAVES) {
+    const int64_t own0 = cut0 > shared_units ? cut0 : shared_units, own1 = cut1 > shared_units ? cut1 : shared_units;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int64_t cut = part < parts ? pg_cut(total, parts, part + e) : total;
-      from[e] = items, tile[e] = 0, at_step[e] = 0;
-      int64_t before = 0;
-      if (cut < total)
-        for (int i0 = 0; i0 < items; i0 += SP_WAVE) {
-          if (items > SP_WAVE) sums(i0, &n, &units, &upto);
-          const uint64_t here = __ballot(cut < before + upto);
-          if (here != 0ull) {
-            const int i = __builtin_ctzll(here);
-            sh_place(cut - before - (__shfl(upto, i, SP_WAVE) - __shfl(units, i, SP_WAVE)), __shfl(n, i, SP_WAVE), near, &tile[e], &at_step[e]);
-            from[e] = i0 + i;
-            break;
-          }
-          before += __shfl(upto, SP_WAVE - 1, SP_WAVE);
-        }
-      from[e] = __builtin_amdgcn_readfirstlane(from[e]), tile[e] = __builtin_amdgcn_readfirstlane(tile[e]);
-      at_step[e] = __builtin_amdgcn_readfirstlane(at_step[e]);
+      const int64_t cut = uniform64(own0 + (own1 - own0) * (wave + e) / WAVES);
+      if (cut < total) {
+        const int x = find(cut);
+        stream_b[e] = x - n_groups;
+        stream_step[e] = __builtin_amdgcn_readfirstlane(sh_stream_step(cut - line_s[x], item(x).n));
+      }
     }
-    if (kvh == 0 && t == 0) a.cuts[part] = make_int4(from[0] - n_groups, at_step[0], from[1] - n_groups, at_step[1]);
-    if (blockIdx.x == 0)
-      for (int b = t; b <= a.batch; b += SH_THREADS) a.of_request[b] = b < a.batch ? request(b) : ShRequest{0, 0, 0, 0, start_s[a.batch], {0, 0, 0}};
+    if (kvh == 0 && lane == 0) a.cuts[part * WAVES + wave] = make_int4(stream_b[0], stream_step[0], stream_b[1], stream_step[1]);
   }
 
   // Arguments of what is done once an item are read where they are used: scalar registers do not suffice to keep them.
@@ -206,11 +252,220 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   float* const m_s = reinterpret_cast<float*>(lds + SH_ML);
   float* const l_s = m_s + WAVES * SH_TILE;
 
+  dc_bf16x8 ones = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  asm volatile("" : "+v"(ones));  // one register set throughout
+  const char* const kh = (const char*)(a.k + kvh * a.sk_h);
+  const char* const vh = (const char*)(a.v + kvh * a.sv_h);
+  struct Ids {
+    int id[2];
+  };
+  auto entries = [&](auto table, int key) {  // pages of a step's halves
+    Ids e;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) e.id[h] = table[pg_min((key + 16 * h) >> a.shift, a.width - 1)];
+    return e;
+  };
+  // The loads of the step at `key`, K's or V's or both, and which of its keys are any: those from key0 to key1 with a page.  The others are zeros, without a
+  // read, whatever stands there.
+  auto fetch = [&](uint32_t at, int key, int key0, int key1, Ids ids, bool with_k, bool with_v) {
+    auto low = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+    uint32_t seen = low(key1 - key) & ~low(key0 - key);
+    int64_t id[2];
+    int in[2], there[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int first = key + 16 * h;
+      const int page = first >> a.shift < a.width && (unsigned)ids.id[h] < (unsigned)a.num_pages ? ids.id[h] : -1;
+      in[h] = first & ((1 << a.shift) - 1);
+      there[h] = page < 0 ? 0 : pg_max(0, pg_min(key1 - first, 16));
+      if (page < 0) seen &= h == 0 ? 0xffff0000u : 0x0000ffffu;
+      id[h] = pg_max(page, 0);
+    }
+    auto load = [&](const char* from, int64_t page_bytes, uint32_t row_bytes, uint32_t to, auto&& chunk) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(from + id[h] * page_bytes + (uint64_t)(uint32_t)in[h] * row_bytes), 0,
+            there[h] > 0 ? (int)((uint32_t)(there[h] - 1) * row_bytes + 2u * D) : 0, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+          const int row = i * ROWS + lane / CHUNKS;
+          uint32_t off = (uint32_t)row * row_bytes + 16u * (uint32_t)chunk(16 * h + row);
+          off = (seen >> (16 * h + row)) & 1u ? off : 0x7ffffff0u;  // (past the buffer's end: zeros)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ds_lds_ptr)(uintptr_t)(to + (h * HALF + i) * 1024), 16, (int)off, 0, 0, 0);
+        }
+      }
+    };
+    if (with_k) load(kh, a.sk_p * 2, k_row, at, [&](int row) { return (lane % CHUNKS) ^ ds_swz_k<D>(row); });
+    if (with_v) load(vh, a.sv_p * 2, v_row, at + Shape::K_BYTES, [&](int row) { return (lane % CHUNKS) ^ (2 * ds_swz_v<CT>(row)); });
+    return seen;
+  };
+  // One step of a wave's rows, RT tiles of 16: its operands lie at `off` of the wave's ring, its first key is `key`, `mine` says which are seen; partly: some rows
+  // do not see some of them, those behind pos.  m, l: the rows' maxima and sums (the same four times).
+  auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits) {
+    constexpr int RT = decltype(tiles)::value;
+    constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
+    dc_u32x4 kr[2][KS];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint32_t at = k_at + off + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4);  // (16 rows further the swizzle is the same)
+        kr[i][ks] = i == 0 ? sh_read_k<0>(at) : sh_read_k<16 * D * 2>(at);
+      }
+    if constexpr (KS == 4)
+      asm volatile("s_waitcnt lgkmcnt(0)"
+                   : "+v"(kr[0][0]), "+v"(kr[0][1]), "+v"(kr[0][2]), "+v"(kr[0][3]), "+v"(kr[1][0]), "+v"(kr[1][1]), "+v"(kr[1][2]), "+v"(kr[1][3]));
+    else
+      asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(kr[0][0]), "+v"(kr[0][1]), "+v"(kr[1][0]), "+v"(kr[1][1]));
+    ds_floatx4 sc[RT][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        sc[rt][i] = (ds_floatx4){0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          sc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, kr[i][ks]), qb[rt][ks], sc[rt][i], 0, 0, 0);
+      }
+    const uint32_t bits = mine >> (4 * gr);  // the lane's keys: 16 i + 4 gr + j
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[rt][i][j] *= a.scale_log2;
+    if (mine != ~0u) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[rt][i][j] = bits & (1u << (16 * i + j)) ? sc[rt][i][j] : -INFINITY;
+    }
+    if (partly) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[rt][i][j] = key + 4 * gr + 16 * i + j <= pos[rt] ? sc[rt][i][j] : -INFINITY;
+    }
+    logits(sc);
+    float mx[RT];
+    bool moves = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      mx[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
+                     fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
+      moves |= mx[rt] > m[rt] + SH_SLACK;
+    }
+    // (the lanes of a row need its maximum only where one of them finds that it moves; a row that has seen no finite logit: m is -inf, every weight
+    // exp2(-inf) = 0)
+    if (__ballot(moves) != 0ull) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float to = fmaxf(m[rt], ds_quad_max(mx[rt])), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
+        m[rt] = to;
+        l[rt] *= alpha;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[rt][ct] *= alpha;
+      }
+    }
+    // V is asked for here, under the exponentials: no branch lies between these reads and the wait for them
+    ds_u32x2 vr[CT][2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const uint32_t at = v_at + off + ((ct ^ ds_swz_v<CT>(v_key)) << 5);
+      vr[ct][0] = ds_read_v<0>(at);
+      vr[ct][1] = ds_read_v<16 * CT * 32>(at);
+    }
+    dc_bf16x8 ph[RT], pl[1];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float base = m[rt] == -INFINITY ? 0.f : m[rt];
+      uint32_t hi[4], lw[4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(sc[rt][i][j] - base), p1 = __builtin_amdgcn_exp2f(sc[rt][i][j + 1] - base);
+          const uint32_t w = dc_pack2(p0, p1);
+          hi[2 * i + j / 2] = w;
+          if constexpr (TWO) lw[2 * i + j / 2] = dc_pack2(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
+        }
+      ph[rt] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){hi[0], hi[1], hi[2], hi[3]});
+      if constexpr (TWO) pl[0] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){lw[0], lw[1], lw[2], lw[3]});
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[ct][0]), "+v"(vr[ct][1]));
+    // Where a row does not see a key, 0 times a value that is no number would make a NaN of its sum: the product takes zeros in such places, and rows
+    // that do see such a key have a sum of weights that is none.
+    if (partly) {
+      uint32_t odd[2] = {0u, 0u};  // exponents of ones, of the lane's keys 16 h + 4 gr + 0 .. 3: bits 15, 31 of words 0 and 1
+      uint32_t any = 0u;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) any |= ((vr[ct][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+      if (__ballot(any != 0u) != 0ull) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t here = 0u;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              const uint32_t ones = ((vr[ct][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+              here |= ones;
+              vr[ct][h][e] &= ~((ones >> 15) * 0xffffu);
+            }
+            odd[h] |= here >> (15 * e);  // (keys 2 e and 2 e + 1: bits 15 - 15 e and 31 - 15 e)
+          }
+        uint32_t met = 0u;  // the lane's rows see such a key (bits)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int by = 1; by < 16; by <<= 1) odd[h] |= __shfl_xor(odd[h], by, SP_WAVE);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if ((odd[h] >> (15 - 15 * (j >> 1) + 16 * (j & 1))) & 1u) {
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                if (key + 16 * h + 4 * gr + j <= pos[rt]) met |= 1u << rt;
+            }
+        }
+        met |= __shfl_xor(met, 16, SP_WAVE);
+        met |= __shfl_xor(met, 32, SP_WAVE);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          if ((met >> rt) & 1u) l[rt] *= __builtin_nanf("");
+      }
+    }
+    // (the sums are those of what the product takes: an output is a mean of values, whatever its weights' roundings)
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, ph[rt], l[rt], 0, 0, 0);
+    if constexpr (TWO) l[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pl[0], l[0], 0, 0, 0);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, __builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3)),
+                                                            ph[rt], o[rt][ct], 0, 0, 0);
+    if constexpr (TWO) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        o[0][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(dc_bf16x8, ds_finite(__builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3))), pl[0], o[0][ct], 0, 0, 0);
+    }
+  };
+
   // RT: row tiles of 16 of a wave.  One: waves 0 .. 3 with a ring each.  Two: the waves of a slot have 32 rows each of its keys, one loads K and the other V, and
   // all meet at a barrier every block of four steps.
   auto run = [&](auto tiles, const ShItem& p, int begin, int s_end, bool of_group) {
     constexpr int RT = decltype(tiles)::value;
-    constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
     const int tile_row = RT == 1 ? 0 : 16 * RT * half;  // the wave's first row in the tile
     auto row_of = [&](int in_tile, int* token, int* head) {
       const int r = pg_min(p.row0 + in_tile, p.rows - 1);
@@ -232,230 +487,26 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       }
     }
     const int pos0 = p.pos + (int)pg_div((unsigned)p.row0, a.by_group);  // of the tile's first row
-    const char* const kh = (const char*)(a.k + kvh * a.sk_h);
-    const char* const vh = (const char*)(a.v + kvh * a.sv_h);
     // (scalar loads: nothing writes the table during the launch)
     const auto table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.table + (int64_t)p.table_row * a.table_stride);
-    struct Ids {
-      int id[2];
-    };
-    auto entries = [&](int s) {  // pages of a step's halves
-      Ids e;
-      const int key0 = (p.lo + s) * SH_KEYS;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) e.id[h] = table[pg_min((key0 + 16 * h) >> a.shift, a.width - 1)];
-      return e;
-    };
-    auto low = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
-    // A step's loads, K's or V's or both, and which of its keys any row sees: the others are zeros, without a read, whatever stands there.
-    auto fetch = [&](int buf, int s, Ids ids) {
-      const int key0 = (p.lo + s) * SH_KEYS;
-      uint32_t seen = low(p.key1 - key0) & ~low(p.key0 - key0);
-      const uint32_t at = ring + buf * Shape::STEP_BYTES;
-      int64_t id[2];
-      int in[2], there[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = key0 + 16 * h;
-        const int page = key >> a.shift < a.width && (unsigned)ids.id[h] < (unsigned)a.num_pages ? ids.id[h] : -1;
-        in[h] = key & ((1 << a.shift) - 1);
-        there[h] = page < 0 ? 0 : pg_max(0, pg_min(p.key1 - key, 16));
-        if (page < 0) seen &= h == 0 ? 0xffff0000u : 0x0000ffffu;
-        id[h] = pg_max(page, 0);
-      }
-      auto load = [&](const char* from, int64_t page_bytes, uint32_t row_bytes, uint32_t to, auto&& chunk) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-              (void*)(from + id[h] * page_bytes + (uint64_t)(uint32_t)in[h] * row_bytes), 0,
-              there[h] > 0 ? (int)((uint32_t)(there[h] - 1) * row_bytes + 2u * D) : 0, 0x00027000);
-#pragma unroll
-          for (int i = 0; i < HALF; ++i) {
-            const int row = i * ROWS + lane / CHUNKS;
-            uint32_t off = (uint32_t)row * row_bytes + 16u * (uint32_t)chunk(16 * h + row);
-            off = (seen >> (16 * h + row)) & 1u ? off : 0x7ffffff0u;  // (past the buffer's end: zeros)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ds_lds_ptr)(uintptr_t)(to + (h * HALF + i) * 1024), 16, (int)off, 0, 0, 0);
-          }
-        }
-      };
-      if (RT == 1 || half == 0) load(kh, a.sk_p * 2, k_row, at, [&](int row) { return (lane % CHUNKS) ^ ds_swz_k<D>(row); });
-      if (RT == 1 || half == 1) load(vh, a.sv_p * 2, v_row, at + Shape::K_BYTES, [&](int row) { return (lane % CHUNKS) ^ (2 * ds_swz_v<CT>(row)); });
-      return seen;
-    };
-
+    auto key_of = [&](int step) { return (p.lo + step) * SH_KEYS; };
     ds_floatx4 o[RT][CT];
-    float m[RT], l[RT];  // of the lane's rows; l: this lane group's keys
+    ds_floatx4 l[RT];
+    float m[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[rt][ct] = (ds_floatx4){0, 0, 0, 0};
-      m[rt] = -INFINITY, l[rt] = 0.f;
+      m[rt] = -INFINITY, l[rt] = (ds_floatx4){0, 0, 0, 0};
     }
 
-    // one step of the wave: its operands lie at `off` of its ring, `mine` says which keys are seen
-    auto step = [&](int s, uint32_t mine, uint32_t off) {
-      dc_u32x4 kr[2][KS];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kr[i][ks] = ds_read_k(k_at + off + i * 16 * (D * 2) + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4));
-      if constexpr (KS == 4)
-        asm volatile("s_waitcnt lgkmcnt(0)"
-                     : "+v"(kr[0][0]), "+v"(kr[0][1]), "+v"(kr[0][2]), "+v"(kr[0][3]), "+v"(kr[1][0]), "+v"(kr[1][1]), "+v"(kr[1][2]), "+v"(kr[1][3]));
-      else
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(kr[0][0]), "+v"(kr[0][1]), "+v"(kr[1][0]), "+v"(kr[1][1]));
-      ds_floatx4 sc[RT][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          sc[rt][i] = (ds_floatx4){0, 0, 0, 0};
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            sc[rt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, kr[i][ks]), qb[rt][ks], sc[rt][i], 0, 0, 0);
-        }
-      const int key0 = (p.lo + s) * SH_KEYS;
-      const uint32_t bits = mine >> (4 * gr);  // the lane's keys: 16 i + 4 gr + j
-      const bool partly = pg_min(key0 + SH_KEYS, p.key1) - 1 > pos0;  // (uniform: some row does not see a key that others see)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sc[rt][i][j] *= a.scale_log2;
-      if (mine != ~0u) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sc[rt][i][j] = bits & (1u << (16 * i + j)) ? sc[rt][i][j] : -INFINITY;
-      }
-      if (partly) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) sc[rt][i][j] = key0 + 4 * gr + 16 * i + j <= pos[rt] ? sc[rt][i][j] : -INFINITY;
-      }
-      if constexpr (RT == 1) {  // the logits themselves, for the keys' weights
-        if (a.weights != nullptr && !of_group) {
-          const auto r = args();
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int key = key0 + 16 * i + 4 * gr, page = table[pg_min((key0 + 16 * i) >> a.shift, a.width - 1)];
-            if (((mine >> (16 * i)) & 0xffffu) != 0u && lq < g)  // (no page: no key of it is seen)
-              *reinterpret_cast<ds_floatx4*>(r->logits + (((int64_t)page * a.hkv + kvh) * g + lq) * (1 << a.shift) + (key & ((1 << a.shift) - 1))) = sc[0][i];
-          }
-        }
-      }
-      float mx[RT];
-      bool moves = false;
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        mx[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
-                       fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
-        mx[rt] = ds_quad_max(mx[rt]);
-        moves |= mx[rt] > m[rt] + SH_SLACK;
-      }
-      // (a row that has seen no finite logit: m is -inf, every weight exp2(-inf) = 0)
-      if (__ballot(moves) != 0ull) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const float to = fmaxf(m[rt], mx[rt]), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[rt] - to);
-          m[rt] = to;
-          l[rt] *= alpha;
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) o[rt][ct] *= alpha;
-        }
-      }
-      // V is asked for here, under the exponentials: no branch lies between these reads and the wait for them
-      ds_u32x2 vr[CT][2];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        const uint32_t at = v_at + off + ((ct ^ ds_swz_v<CT>(v_key)) << 5);
-        vr[ct][0] = ds_read_v<0>(at);
-        vr[ct][1] = ds_read_v<16 * CT * 32>(at);
-      }
-      dc_bf16x8 ph[RT], pl[1];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float base = m[rt] == -INFINITY ? 0.f : m[rt];
-        uint32_t hi[4], lw[4];
-        float add = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; j += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(sc[rt][i][j] - base), p1 = __builtin_amdgcn_exp2f(sc[rt][i][j + 1] - base);
-            const uint32_t w = dc_pack2(p0, p1);
-            hi[2 * i + j / 2] = w;
-            const float q0 = __uint_as_float(w << 16), q1 = __uint_as_float(w & 0xffff0000u);
-            if constexpr (TWO) {
-              lw[2 * i + j / 2] = dc_pack2(p0 - q0, p1 - q1);
-              add += p0 + p1;
-            } else {
-              add += q0 + q1;  // (of what the product takes: an output is a mean of values, whatever its weights' roundings)
-            }
-          }
-        l[rt] += add;
-        ph[rt] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){hi[0], hi[1], hi[2], hi[3]});
-        if constexpr (TWO) pl[0] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){lw[0], lw[1], lw[2], lw[3]});
-      }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[ct][0]), "+v"(vr[ct][1]));
-      // Where a row does not see a key, 0 times a value that is no number would make a NaN of its sum: the product takes zeros in such places, and rows
-      // that do see such a key have a sum of weights that is none.
-      if (partly) {
-        uint32_t odd[2] = {0u, 0u};  // exponents of ones, of the lane's keys 16 h + 4 gr + 0 .. 3: bits 15, 31 of words 0 and 1
-        uint32_t any = 0u;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) any |= ((vr[ct][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-        if (__ballot(any != 0u) != 0ull) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint32_t here = 0u;
-#pragma unroll
-              for (int ct = 0; ct < CT; ++ct) {
-                const uint32_t ones = ((vr[ct][h][e] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-                here |= ones;
-                vr[ct][h][e] &= ~((ones >> 15) * 0xffffu);
-              }
-              odd[h] |= here >> (15 * e);  // (keys 2 e and 2 e + 1: bits 15 - 15 e and 31 - 15 e)
-            }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int by = 1; by < 16; by <<= 1) odd[h] |= __shfl_xor(odd[h], by, SP_WAVE);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if ((odd[h] >> (15 - 15 * (j >> 1) + 16 * (j & 1))) & 1u) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                  if (key0 + 16 * h + 4 * gr + j <= pos[rt]) l[rt] = __builtin_nanf("");
-              }
-          }
-        }
-      }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, __builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3)),
-                                                              ph[rt], o[rt][ct], 0, 0, 0);
-      if constexpr (TWO) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-          o[0][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(dc_bf16x8, ds_finite(__builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3))), pl[0], o[0][ct], 0, 0, 0);
-      }
+    auto ask = [&](int buf, int step, Ids ids) {
+      return fetch(ring + buf * Shape::STEP_BYTES, key_of(step), p.key0, p.key1, ids, RT == 1 || half == 0, RT == 1 || half == 1);
+    };
+    auto step = [&](int x, uint32_t mine, uint32_t off) {
+      const int key = key_of(x);
+      // (uniform: some row does not see a key that others see)
+      attend(tiles, off, key, mine, qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0, o, m, l, [](ds_floatx4 (&)[RT][2]) {});
     };
 
     __syncthreads();  // the rings are free
@@ -466,10 +517,10 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
 #pragma unroll
         for (int i = 0; i < NB - 1; ++i) {
           seen[i] = 0;
-          if (s0 + i * WAVES < s_end) seen[i] = fetch(i, s0 + i * WAVES, entries(s0 + i * WAVES));
+          if (s0 + i * WAVES < s_end) seen[i] = ask(i, s0 + i * WAVES, entries(table, key_of(s0 + i * WAVES)));
         }
         Ids next = {{0, 0}};
-        if (s0 + (NB - 1) * WAVES < s_end) next = entries(s0 + (NB - 1) * WAVES);
+        if (s0 + (NB - 1) * WAVES < s_end) next = entries(table, key_of(s0 + (NB - 1) * WAVES));
         int buf = 0;
         for (int s = s0; s < s_end; s += WAVES) {
           // the step's loads have landed, those of the NB - 2 behind it stay in flight (what is asked for returns in order)
@@ -482,8 +533,8 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
           for (int i = 0; i + 1 < NB - 1; ++i) seen[i] = seen[i + 1];
           // (the place that is filled here was read in the step before: those reads' results have been used)
           if (s + (NB - 1) * WAVES < s_end) {
-            seen[NB - 2] = fetch(buf == 0 ? NB - 1 : buf - 1, s + (NB - 1) * WAVES, next);
-            if (s + NB * WAVES < s_end) next = entries(s + NB * WAVES);
+            seen[NB - 2] = ask(buf == 0 ? NB - 1 : buf - 1, s + (NB - 1) * WAVES, next);
+            if (s + NB * WAVES < s_end) next = entries(table, key_of(s + NB * WAVES));
           }
           step(s, mine, buf * Shape::STEP_BYTES);
           buf = buf + 1 == NB ? 0 : buf + 1;
@@ -493,23 +544,21 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       const int blocks = (s_end - begin + WAVES - 1) / WAVES;
       const int s0 = begin + slot;
       uint32_t seen = 0, seen_next = 0;
-      if (s0 < s_end) seen_next = fetch(0, s0, entries(s0));
+      if (s0 < s_end) seen_next = ask(0, s0, entries(table, key_of(s0)));
       Ids next = {{0, 0}};
-      if (s0 + WAVES < s_end) next = entries(s0 + WAVES);
+      if (s0 + WAVES < s_end) next = entries(table, key_of(s0 + WAVES));
       for (int i = 0; i < blocks; ++i) {
         // everybody's loads of this block have landed, and everybody is past the block in front, whose place the next one's take
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         const int s = s0 + i * WAVES;
         seen = seen_next;
         if (s + WAVES < s_end) {
-          seen_next = fetch((i + 1) & 1, s + WAVES, next);
-          if (s + 2 * WAVES < s_end) next = entries(s + 2 * WAVES);
+          seen_next = ask((i + 1) & 1, s + WAVES, next);
+          if (s + 2 * WAVES < s_end) next = entries(table, key_of(s + 2 * WAVES));
         }
         if (s < s_end) step(s, seen, (i & 1) * Shape::STEP_BYTES);
       }
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) l[rt] = ds_quad_sum(l[rt]);
     __syncthreads();  // the rings are free
     // [slot][SH_TILE][D] floats, 16-byte pieces swizzled by the row
     float* const o_s = reinterpret_cast<float*>(lds);
@@ -519,7 +568,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
         const int r = slot * SH_TILE + tile_row + 16 * rt + lq;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<ds_floatx4*>(o_s + r * D + ((4 * ct + gr) ^ lq) * 4) = o[rt][ct];
-        if (gr == 0) m_s[r] = m[rt], l_s[r] = l[rt];
+        if (gr == 0) m_s[r] = m[rt], l_s[r] = l[rt][0];
       }
     }
     __syncthreads();
@@ -556,7 +605,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
   };
 
-  for (int x = from[0], first_tile = tile[0], begin = at_step[0]; x < items && x <= from[1]; ++x, first_tile = 0, begin = 0) {
+  for (int x = from[0], first_tile = tile[0], begin = at_step[0]; x < shared_items && x <= from[1]; ++x, first_tile = 0, begin = 0) {
     ShItem p = item(x);
     if (p.n == 0) continue;
     // (uniform: out of vector registers)
@@ -583,6 +632,132 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
         run(std::integral_constant<int, SH_TILE / 32>{}, p, begin, end, x < n_groups);
     }
   }
+  if (!a.streams) return;
+
+  // ---- single tokens over their own keys, a wave by itself ----
+  __syncthreads();  // the rings are free
+  if (half != 0) return;
+  const int b0 = stream_b[0], b1 = stream_b[1], step0 = stream_step[0], step1 = stream_step[1], wave_part = part * WAVES + slot;
+  struct At {  // a step of request b (b = batch: none is left): steps up to `end` of its n fall to the wave
+    int b, s, end, n, lo, key0, key1;
+  };
+  auto settle = [&](At& x) {
+    for (;; ++x.b, x.s = 0) {
+      if (x.b >= a.batch || x.b > b1 || (x.b == b1 && step1 == 0)) {
+        x.b = a.batch;
+        return;
+      }
+      x.key0 = __builtin_amdgcn_readfirstlane(first_s[x.b]), x.key1 = pg_min(__builtin_amdgcn_readfirstlane(len_s[x.b]), room);
+      x.lo = x.key0 / SH_KEYS, x.n = x.key1 > x.key0 ? (x.key1 + SH_KEYS - 1) / SH_KEYS - x.lo : 0;  // (as in item)
+      x.end = x.b == b1 ? pg_min(step1, x.n) : x.n;
+      if (x.s < x.end) return;
+    }
+  };
+  auto key_of = [](const At& x) { return (x.lo + x.s) * SH_KEYS; };
+  auto table_of = [&](int b) { return (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.table + (int64_t)b * a.table_stride); };
+  struct Step {  // on its way, or about to be computed on
+    int b, key;
+    uint32_t seen;
+    Ids ids;
+    bool first, last, from_start, to_end, alone;  // of the wave's steps of the request; they begin with its first, end with its last; no shared keys
+  };
+  At ahead = {b0, step0, 0, 0, 0, 0, 0};
+  settle(ahead);
+  Ids ids = {{0, 0}};
+  if (ahead.b < a.batch) ids = entries(table_of(ahead.b), key_of(ahead));
+  auto push = [&](int buf) {
+    Step x = {a.batch, 0, 0u, {{0, 0}}, false, false, false, false, false};
+    if (ahead.b < a.batch) {
+      const int key = key_of(ahead);
+      const bool from_start = ahead.b != b0 || step0 == 0;
+      x = {ahead.b, key, fetch(ring + buf * Shape::STEP_BYTES, key, ahead.key0, ahead.key1, ids, true, true), ids,
+           ahead.s == (from_start ? 0 : step0), ahead.s + 1 == ahead.end, from_start, ahead.end == ahead.n, ahead.key0 == 0};
+      if (++ahead.s >= ahead.end) {
+        ++ahead.b, ahead.s = 0;
+        settle(ahead);
+      }
+      if (ahead.b < a.batch) ids = entries(table_of(ahead.b), key_of(ahead));
+    }
+    return x;
+  };
+  dc_bf16x8 qb[1][KS], q_next[KS];
+  auto load_q = [&](int b) {
+    const auto r = args();
+    const sp_bf16* src = r->q + (int64_t)b * r->sq_n + (int64_t)(kvh * g + pg_min(lq, g - 1)) * r->sq_h + 8 * gr;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) q_next[ks] = *reinterpret_cast<const dc_bf16x8*>(src + 32 * ks);
+  };
+  if (ahead.b < a.batch) load_q(ahead.b);
+  Step queue[NB - 1];
+#pragma unroll
+  for (int i = 0; i < NB - 1; ++i) queue[i] = push(i);
+  ds_floatx4 o[1][CT];
+  ds_floatx4 l[1];
+  float m[1];
+  int pos[1] = {0};
+  int buf = 0;
+  bool wrote = false;  // at least CT stores are younger than all loads
+  while (queue[0].b < a.batch) {
+    // the step's loads have landed, those of the NB - 2 behind it stay in flight (what is asked for returns in order)
+    if (NB > 2 && queue[NB - 2].b < a.batch)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * Shape::LOADS) : "memory");
+    else if (NB == 2 && wrote)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CT) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const Step now = queue[0];
+#pragma unroll
+    for (int i = 0; i + 1 < NB - 1; ++i) queue[i] = queue[i + 1];
+    if (now.first) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qb[0][ks] = q_next[ks];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[0][ct] = (ds_floatx4){0, 0, 0, 0};
+      m[0] = -INFINITY, l[0] = (ds_floatx4){0, 0, 0, 0};
+    }
+    if (NB > 2 && queue[0].b < a.batch && queue[0].first) load_q(queue[0].b);
+    // (the place that is filled here was read in the step before: those reads' results have been used)
+    queue[NB - 2] = push(buf == 0 ? NB - 1 : buf - 1);
+    if (NB == 2 && queue[0].b < a.batch && queue[0].first) load_q(queue[0].b);
+    attend(std::integral_constant<int, 1>{}, buf * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l, [&](ds_floatx4 (&sc)[1][2]) {
+      if (a.weights == nullptr || lq >= g) return;  // the logits themselves, for the keys' weights
+      float* const to = args()->logits;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (((now.seen >> (16 * i)) & 0xffffu) != 0u)  // (no page: no key of it is seen)
+          *reinterpret_cast<ds_floatx4*>(to + ((((int64_t)now.ids.id[i] * a.hkv + kvh) * g + lq) << a.shift) + ((now.key + 16 * i + 4 * gr) & ((1 << a.shift) - 1))) = sc[0][i];
+    });
+    wrote = now.last;
+    if (now.last) {
+      const auto r = args();
+      const float sum = l[0][0];
+      const int64_t row = (int64_t)now.b * (a.hkv * g) + kvh * g + lq;
+      const bool whole = now.from_start && now.to_end, final = whole && now.alone;
+      if (lq < g) {
+        if (final) {
+          const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct)
+            *reinterpret_cast<uint2*>(r->out + row * D + 16 * ct + 4 * gr) =
+                make_uint2(dc_pack2(o[0][ct][0] * inv, o[0][ct][1] * inv), dc_pack2(o[0][ct][2] * inv, o[0][ct][3] * inv));
+        }
+        if (!final || a.weights != nullptr) {
+          const int64_t to = whole ? (int64_t)a.tokens * (a.hkv * g) + row : ((int64_t)(wave_part * a.hkv + kvh) * 2 + (now.from_start ? 1 : 0)) * 16 + lq;
+          if (!final) {
+            float* const dst = (whole ? r->o_row : r->o_stream) + to * D + 4 * gr;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<ds_floatx4*>(dst + 16 * ct) = o[0][ct];
+          }
+          if (gr == 0) (whole ? r->ml_row : r->ml_stream)[to] = make_float2(fmaxf(m[0], CK_NO_MAX), sum);
+        }
+      }
+      if (kvh == 0 && lane == 0) {
+        if (now.from_start) r->parts_of[a.shared_slots + now.b].x = wave_part;
+        if (now.to_end) r->parts_of[a.shared_slots + now.b].y = wave_part;
+      }
+    }
+    buf = buf + 1 == NB ? 0 : buf + 1;
+  }
 }
 
 // ---- joining ----------------------------------------------------------------------------------------------------
@@ -606,19 +781,21 @@ __device__ __forceinline__ int2 sh_own_parts(const ShArgs& a, const ShRequest& r
   return pg_min(a.lens[b], a.width << a.shift) > r.first_own ? a.parts_of[row.slot] : make_int2(0, -1);
 }
 // Where part i of a tile that parts.x .. parts.y hold stands: in o_row and ml_row where there is but one, else in o_part and ml_part.
-__device__ __forceinline__ int64_t sh_slab(const ShArgs& a, int2 parts, int i, int kvh, int in_tile) {
-  return ((int64_t)((parts.x + i) * a.hkv + kvh) * 2 + (i == 0 ? 1 : 0)) * SH_TILE + in_tile;
+__device__ __forceinline__ int64_t sh_slab(const ShArgs& a, int2 parts, int i, int kvh, int in_tile, int rows) {
+  return ((int64_t)((parts.x + i) * a.hkv + kvh) * 2 + (i == 0 ? 1 : 0)) * rows + in_tile;
 }
 
 #define SM_THREADS 256
-// A row's parts joined, D / 4 threads a row.
-template <int D>
+// A row's parts joined: D / 4 threads a row, SETS of them that take every so many parts, on a running maximum of their own, and meet in LDS.
+template <int D, int SETS>
 __device__ __forceinline__ void sh_join(const ShArgs& a) {
-  constexpr int WIDTH = D / 4, PER = SM_THREADS / WIDTH, AHEAD = 8;
-  const int t = threadIdx.x, hq = a.hkv * a.group, c = t % WIDTH * 4;
-  const unsigned row = blockIdx.x * PER + t / WIDTH;
-  if (row >= (unsigned)a.tokens * (unsigned)hq) return;
-  const int token = (int)(row / (unsigned)hq), head = (int)(row - (unsigned)token * (unsigned)hq), kvh = (int)pg_div((unsigned)head, a.by_group);
+  constexpr int WIDTH = D / 4, PER = SM_THREADS / (WIDTH * SETS), AHEAD = 4;
+  __shared__ float2 ml_s[SETS][PER];
+  __shared__ __attribute__((aligned(16))) float o_s[SETS > 1 ? SETS : 1][SETS > 1 ? PER : 1][D];
+  const int t = threadIdx.x, hq = a.hkv * a.group, c = t % WIDTH * 4, in_block = t / WIDTH % PER, set = t / (WIDTH * PER);
+  const unsigned row = blockIdx.x * PER + in_block;
+  const unsigned rows = (unsigned)a.tokens * (unsigned)hq;
+  const int token = (int)(pg_min((int)row, (int)rows - 1) / hq), head = pg_min((int)row, (int)rows - 1) - token * hq, kvh = (int)pg_div((unsigned)head, a.by_group);
   int b = token;
   if (a.cu != nullptr) {
     b = 0;
@@ -632,26 +809,29 @@ __device__ __forceinline__ void sh_join(const ShArgs& a) {
     }
   }
   const ShRequest r = a.of_request[b];
-  const int end = a.of_request[b + 1].start;
-  if (token < r.start || token >= end) return;  // (a row outside every request)
-  const int h = head - kvh * a.group;
+  const int end = a.of_request[b + 1].start, h = head - kvh * a.group;
   const ShRow own = sh_own_row(a, r, b, token, h), group = sh_group_row(a, r, token, h);
-  const int2 own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
-  if (r.first_own == 0 && own_parts.x == own_parts.y) return;  // (the row is done)
+  bool wanted = row < rows && token >= r.start && token < end;  // (a row outside every request)
+  int2 own_parts = make_int2(0, -1), group_parts = own_parts;
+  if (wanted) own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
+  if (r.first_own == 0 && own_parts.x == own_parts.y) wanted = false, own_parts.y = own_parts.x - 1;  // (the row is done)
   float top = CK_NO_MAX, sum = 0.f;
   ds_floatx4 acc = {0, 0, 0, 0};
   auto add = [&](const ShRow& it, int2 parts, bool of_group) {
     const int count = parts.y - parts.x + 1;
-    for (int i0 = 0; i0 < count; i0 += AHEAD) {
+    const bool stream = !of_group && a.streams;
+    const float2* const ml_from = count == 1 ? a.ml_row : stream ? a.ml_stream : a.ml_part;
+    const float* const o_from = count == 1 ? a.o_row : stream ? a.o_stream : a.o_part;
+    for (int i0 = set; i0 < count; i0 += SETS * AHEAD) {
       float2 ml[AHEAD];
       ds_floatx4 o[AHEAD];
       float to = top;
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        const int i = pg_min(i0 + u, count - 1);
-        const int64_t at = count > 1 ? sh_slab(a, parts, i, kvh, it.in_tile) : (of_group ? 0 : (int64_t)a.tokens * hq) + row;
-        ml[u] = (count > 1 ? a.ml_part : a.ml_row)[at];
-        o[u] = *reinterpret_cast<const ds_floatx4*>((count > 1 ? a.o_part : a.o_row) + at * D + c);
+        const int i = pg_min(i0 + u * SETS, count - 1);
+        const int64_t at = count > 1 ? sh_slab(a, parts, i, kvh, it.in_tile, stream ? 16 : SH_TILE) : (of_group ? 0 : (int64_t)a.tokens * hq) + row;
+        ml[u] = ml_from[at];
+        o[u] = *reinterpret_cast<const ds_floatx4*>(o_from + at * D + c);
       }
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) to = fmaxf(to, ml[u].x);
@@ -661,7 +841,7 @@ __device__ __forceinline__ void sh_join(const ShArgs& a) {
       acc *= before;
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
-        if (i0 + u < count) {
+        if (i0 + u * SETS < count) {
           const float f = __builtin_amdgcn_exp2f(ml[u].x - top);
           sum += ml[u].y * f;
           acc += o[u] * f;
@@ -670,11 +850,25 @@ __device__ __forceinline__ void sh_join(const ShArgs& a) {
   };
   add(group, group_parts, true);
   add(own, own_parts, false);
+  if constexpr (SETS > 1) {
+    *reinterpret_cast<ds_floatx4*>(&o_s[set][in_block][c]) = acc;
+    if (c == 0) ml_s[set][in_block] = make_float2(top, sum);
+    __syncthreads();
+    if (set > 0) return;
+    for (int i = 0; i < SETS; ++i) top = fmaxf(top, ml_s[i][in_block].x);
+    sum = 0.f, acc = (ds_floatx4){0, 0, 0, 0};
+    for (int i = 0; i < SETS; ++i) {
+      const float f = __builtin_amdgcn_exp2f(ml_s[i][in_block].x - top);
+      sum += ml_s[i][in_block].y * f;
+      acc += *reinterpret_cast<const ds_floatx4*>(&o_s[i][in_block][c]) * f;
+    }
+  }
+  if (!wanted) return;
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   *reinterpret_cast<uint2*>(a.out + (int64_t)row * D + c) = make_uint2(dc_pack2(acc[0] * inv, acc[1] * inv), dc_pack2(acc[2] * inv, acc[3] * inv));
 }
 
-// Weights of the own keys that fell to part w / hkv of kv head w % hkv (single tokens):
+// Weights of the own keys that fell to wave's part w / hkv of kv head w % hkv (single tokens):
 //   weight[j] += sum over the group's heads of 2^(logit - m) / l.
 __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
   __shared__ float2 ml_s[PD_MAX_GROUP];  // of a head: m, 1 / l
@@ -697,7 +891,7 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
         for (int i0 = 0; i0 < count; i0 += SP_WAVE) {
           float2 ml = make_float2(CK_NO_MAX, 0.f);
           if (i0 + lane < count)
-            ml = count > 1 ? a.ml_part[sh_slab(a, held, i0 + lane, kvh, in_tile)]
+            ml = count > 1 ? (of_group ? a.ml_part : a.ml_stream)[sh_slab(a, held, i0 + lane, kvh, in_tile, of_group ? SH_TILE : 16)]
                            : a.ml_row[(of_group ? 0 : (int64_t)a.tokens * hq) + (int64_t)b * hq + kvh * a.group + h];
           const float to = fmaxf(top, sp_wave_max(ml.x));
           sum = sum * __builtin_amdgcn_exp2f(top - to) + sp_wave_sum(i0 + lane < count ? ml.y * __builtin_amdgcn_exp2f(ml.x - to) : 0.f);
@@ -728,18 +922,22 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
           }
       }
       float* const to = a.weights + id * a.sw_p + kvh * a.sw_h + in;
+      if (a.weights_by_four && key >= r.first_own && key + 4 < len && key + 4 <= last) {
+        *reinterpret_cast<ds_floatx4*>(to) += sum;
+      } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (key + j >= r.first_own && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
+        for (int j = 0; j < 4; ++j)
+          if (key + j >= r.first_own && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
+      }
     }
   }
 }
 
-// The workgroups behind the joining ones, where weights are kept: one for every part of the line.
-template <int D>
+// The workgroups behind the joining ones, where weights are kept: one for every wave's part of the line.
+template <int D, int SETS>
 __global__ __launch_bounds__(SM_THREADS) void sp_shared_join_kernel(const ShArgs a, int join_blocks) {
   if ((int)blockIdx.x < join_blocks)
-    sh_join<D>(a);
+    sh_join<D, SETS>(a);
   else
     sh_weigh(a, (int)blockIdx.x - join_blocks);
 }
@@ -750,7 +948,7 @@ static int sh_workgroups(int64_t hkv) { return hkv < SH_PLACES ? SH_PLACES / (in
 
 struct ShSizes {
   int64_t shared_slots, slots, logits;
-  size_t o_part, ml_part, o_row, ml_row, parts_of, cuts, of_request, bytes;
+  size_t o_part, ml_part, o_stream, ml_stream, o_row, ml_row, parts_of, cuts, of_request, bytes;
 };
 static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d, bool single, int64_t pool_keys) {
   ShSizes s;
@@ -768,10 +966,13 @@ static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t h
   // (the groups' partials are joined before those of the requests are written)
   s.o_part = take(apart ? ck_groups_workspace_bytes((int)hkv, (int)d) : (size_t)rows * d * sizeof(float));
   s.ml_part = take((size_t)rows * sizeof(float2));
+  const bool streams = single && g <= PD_MAX_GROUP;
+  s.o_stream = take(streams ? (size_t)rows * d * sizeof(float) : 0);  // (as many rows: a quarter of them four times)
+  s.ml_stream = take(streams ? (size_t)rows * sizeof(float2) : 0);
   s.o_row = take(groups > 0 ? (size_t)(2 * tokens * hq) * d * sizeof(float) : 0);
   s.ml_row = take((size_t)(2 * tokens * hq) * sizeof(float2));
   s.parts_of = take((size_t)s.slots * sizeof(int2));
-  s.cuts = take((size_t)sh_workgroups(hkv) * sizeof(int4));
+  s.cuts = take((size_t)sh_workgroups(hkv) * SH_WAVES * sizeof(int4));
   s.of_request = take((size_t)(batch + 1) * sizeof(ShRequest));
   s.logits = (int64_t)take((size_t)pool_keys * hq * sizeof(float));
   s.bytes = at;
@@ -848,6 +1049,9 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
   a.o_part = (float*)(ws + s.o_part), a.ml_part = (float2*)(ws + s.ml_part), a.o_row = (float*)(ws + s.o_row), a.ml_row = (float2*)(ws + s.ml_row);
   a.parts_of = (int2*)(ws + s.parts_of), a.cuts = (int4*)(ws + s.cuts), a.of_request = (ShRequest*)(ws + s.of_request);
+  a.o_stream = (float*)(ws + s.o_stream), a.ml_stream = (float2*)(ws + s.ml_stream);
+  a.streams = x->cu_q == nullptr && g <= PD_MAX_GROUP;
+  a.weights_by_four = (uintptr_t)x->weights % 16 == 0 && (w_p | w_h) % 4 == 0;
   a.weights = x->weights, a.logits = (float*)(ws + s.logits);
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -860,8 +1064,11 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   }
   const hipStream_t stream = (hipStream_t)x->stream;
   const int grid = a.parts * a.hkv;
-  const int64_t join = sp_ceil_div(x->tokens * x->hq, SM_THREADS / (x->d / 4));
-  SP_REQUIRE(join + grid <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens, (long long)x->hq);
+  // few rows may have many parts each: a workgroup a row
+  const int sets = x->tokens * x->hq <= 512 ? SM_THREADS / ((int)x->d / 4) : 1;
+  const int64_t join = sp_ceil_div(x->tokens * x->hq * sets, SM_THREADS / (x->d / 4));
+  SP_REQUIRE(join + (int64_t)grid * SH_WAVES <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens,
+             (long long)x->hq);
   a.apart = sh_apart(x->tokens, x->groups, g);
   if (a.apart) {
     CkArgs c = {};
@@ -873,15 +1080,16 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
     const int rc = ck_groups_launch(c, (int)x->d, ws + s.o_part, stream);
     if (rc) return rc;
   }
-  const unsigned joins = (unsigned)(join + (a.weights != nullptr ? grid : 0));
+  const unsigned joins = (unsigned)(join + (a.weights != nullptr ? grid * SH_WAVES : 0));
   const size_t lds = sh_lds_bytes(a.batch, a.n_groups);
-  if (x->d == 64) {
-    hipLaunchKernelGGL(sp_shared_kernel<64>, dim3((unsigned)grid), dim3(SH_THREADS), lds, stream, a);
-    hipLaunchKernelGGL(sp_shared_join_kernel<64>, dim3(joins), dim3(SM_THREADS), 0, stream, a, (int)join);
-  } else {
-    hipLaunchKernelGGL(sp_shared_kernel<128>, dim3((unsigned)grid), dim3(SH_THREADS), lds, stream, a);
-    hipLaunchKernelGGL(sp_shared_join_kernel<128>, dim3(joins), dim3(SM_THREADS), 0, stream, a, (int)join);
-  }
+  auto go = [&](auto kernel, auto many, auto few) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(SH_THREADS), lds, stream, a);
+    hipLaunchKernelGGL(sets == 1 ? many : few, dim3(joins), dim3(SM_THREADS), 0, stream, a, (int)join);
+  };
+  if (x->d == 64)
+    go(sp_shared_kernel<64>, sp_shared_join_kernel<64, 1>, sp_shared_join_kernel<64, SM_THREADS / 16>);
+  else
+    go(sp_shared_kernel<128>, sp_shared_join_kernel<128, 1>, sp_shared_join_kernel<128, SM_THREADS / 32>);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
