@@ -301,8 +301,9 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     return seen;
   };
   // One step of a wave's rows, RT tiles of 16: its operands lie at `off` of the wave's ring, its first key is `key`, `mine` says which are seen; partly: some rows
-  // do not see some of them, those behind pos.  m, l: the rows' maxima and sums (the same four times).
-  auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits) {
+  // do not see some of them, those behind pos.  m, l: the rows' maxima and sums (the same four times).  logits(sc) is called with the logits, done() when the
+  // operands have been read.
+  auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits, auto&& done) {
     constexpr int RT = decltype(tiles)::value;
     constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
     dc_u32x4 kr[2][KS];
@@ -399,6 +400,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[ct][0]), "+v"(vr[ct][1]));
+    done();
     // Where a row does not see a key, 0 times a value that is no number would make a NaN of its sum: the product takes zeros in such places, and rows
     // that do see such a key have a sum of weights that is none.
     if (partly) {
@@ -503,60 +505,49 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     auto ask = [&](int buf, int step, Ids ids) {
       return fetch(ring + buf * Shape::STEP_BYTES, key_of(step), p.key0, p.key1, ids, RT == 1 || half == 0, RT == 1 || half == 1);
     };
-    auto step = [&](int x, uint32_t mine, uint32_t off) {
+    auto step = [&](int x, uint32_t mine, uint32_t off, auto&& done) {
       const int key = key_of(x);
       // (uniform: some row does not see a key that others see)
-      attend(tiles, off, key, mine, qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0, o, m, l, [](ds_floatx4 (&)[RT][2]) {});
+      attend(tiles, off, key, mine, qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0, o, m, l, [](ds_floatx4 (&)[RT][2]) {}, done);
     };
 
     __syncthreads();  // the rings are free
-    if constexpr (RT == 1) {
-      if (half == 0) {
-        const int s0 = begin + wave;
-        uint32_t seen[NB - 1];
+    // The ring holds NB steps; a step's place is filled again as soon as its operands have been read.
+    constexpr int MINE = RT == 1 ? Shape::LOADS : Shape::LOADS / 2;  // loads of the wave for a step
+    const int s0 = begin + slot;
+    if (RT > 1 || half == 0) {
+      uint32_t seen[NB];
 #pragma unroll
-        for (int i = 0; i < NB - 1; ++i) {
-          seen[i] = 0;
-          if (s0 + i * WAVES < s_end) seen[i] = ask(i, s0 + i * WAVES, entries(table, key_of(s0 + i * WAVES)));
-        }
-        Ids next = {{0, 0}};
-        if (s0 + (NB - 1) * WAVES < s_end) next = entries(table, key_of(s0 + (NB - 1) * WAVES));
-        int buf = 0;
-        for (int s = s0; s < s_end; s += WAVES) {
-          // the step's loads have landed, those of the NB - 2 behind it stay in flight (what is asked for returns in order)
-          if (s + (NB - 2) * WAVES < s_end)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * Shape::LOADS) : "memory");
-          else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          const uint32_t mine = seen[0];
-#pragma unroll
-          for (int i = 0; i + 1 < NB - 1; ++i) seen[i] = seen[i + 1];
-          // (the place that is filled here was read in the step before: those reads' results have been used)
-          if (s + (NB - 1) * WAVES < s_end) {
-            seen[NB - 2] = ask(buf == 0 ? NB - 1 : buf - 1, s + (NB - 1) * WAVES, next);
-            if (s + NB * WAVES < s_end) next = entries(table, key_of(s + NB * WAVES));
-          }
-          step(s, mine, buf * Shape::STEP_BYTES);
-          buf = buf + 1 == NB ? 0 : buf + 1;
-        }
+      for (int i = 0; i < NB; ++i) {
+        seen[i] = 0;
+        if (s0 + i * WAVES < s_end) seen[i] = ask(i, s0 + i * WAVES, entries(table, key_of(s0 + i * WAVES)));
       }
-    } else {
-      const int blocks = (s_end - begin + WAVES - 1) / WAVES;
-      const int s0 = begin + slot;
-      uint32_t seen = 0, seen_next = 0;
-      if (s0 < s_end) seen_next = ask(0, s0, entries(table, key_of(s0)));
       Ids next = {{0, 0}};
-      if (s0 + WAVES < s_end) next = entries(table, key_of(s0 + WAVES));
-      for (int i = 0; i < blocks; ++i) {
-        // everybody's loads of this block have landed, and everybody is past the block in front, whose place the next one's take
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        const int s = s0 + i * WAVES;
-        seen = seen_next;
-        if (s + WAVES < s_end) {
-          seen_next = ask((i + 1) & 1, s + WAVES, next);
-          if (s + 2 * WAVES < s_end) next = entries(table, key_of(s + 2 * WAVES));
-        }
-        if (s < s_end) step(s, seen, (i & 1) * Shape::STEP_BYTES);
+      if (s0 + NB * WAVES < s_end) next = entries(table, key_of(s0 + NB * WAVES));
+      int buf = 0;
+      // (of larger tiles all waves go through all blocks: they meet twice in each)
+      for (int s = s0; s < s_end || (RT > 1 && s - slot < s_end); s += WAVES) {
+        // the step's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
+        if (s + (NB - 1) * WAVES < s_end)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * MINE) : "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (RT > 1) asm volatile("s_barrier" ::: "memory");
+        const uint32_t mine = seen[0];
+        auto done = [&] {
+          if constexpr (RT > 1) asm volatile("s_barrier" ::: "memory");  // the other wave has read them too
+#pragma unroll
+          for (int i = 0; i + 1 < NB; ++i) seen[i] = seen[i + 1];
+          if (s + NB * WAVES < s_end) {
+            seen[NB - 1] = ask(buf, s + NB * WAVES, next);
+            if (s + (NB + 1) * WAVES < s_end) next = entries(table, key_of(s + (NB + 1) * WAVES));
+          }
+        };
+        if (s < s_end)
+          step(s, mine, buf * Shape::STEP_BYTES, done);
+        else
+          done();
+        buf = buf + 1 == NB ? 0 : buf + 1;
       }
     }
     __syncthreads();  // the rings are free
@@ -688,9 +679,9 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     for (int ks = 0; ks < KS; ++ks) q_next[ks] = *reinterpret_cast<const dc_bf16x8*>(src + 32 * ks);
   };
   if (ahead.b < a.batch) load_q(ahead.b);
-  Step queue[NB - 1];
+  Step queue[NB];
 #pragma unroll
-  for (int i = 0; i < NB - 1; ++i) queue[i] = push(i);
+  for (int i = 0; i < NB; ++i) queue[i] = push(i);
   ds_floatx4 o[1][CT];
   ds_floatx4 l[1];
   float m[1];
@@ -698,16 +689,17 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   int buf = 0;
   bool wrote = false;  // at least CT stores are younger than all loads
   while (queue[0].b < a.batch) {
-    // the step's loads have landed, those of the NB - 2 behind it stay in flight (what is asked for returns in order)
-    if (NB > 2 && queue[NB - 2].b < a.batch)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 2) * Shape::LOADS) : "memory");
-    else if (NB == 2 && wrote)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(CT) : "memory");
-    else
+    // the step's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
+    if (queue[NB - 1].b >= a.batch)
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else if (wrote)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * Shape::LOADS + CT) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * Shape::LOADS) : "memory");
     const Step now = queue[0];
 #pragma unroll
-    for (int i = 0; i + 1 < NB - 1; ++i) queue[i] = queue[i + 1];
+    for (int i = 0; i + 1 < NB; ++i) queue[i] = queue[i + 1];
+    queue[NB - 1].b = a.batch;
     if (now.first) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) qb[0][ks] = q_next[ks];
@@ -715,18 +707,18 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       for (int ct = 0; ct < CT; ++ct) o[0][ct] = (ds_floatx4){0, 0, 0, 0};
       m[0] = -INFINITY, l[0] = (ds_floatx4){0, 0, 0, 0};
     }
-    if (NB > 2 && queue[0].b < a.batch && queue[0].first) load_q(queue[0].b);
-    // (the place that is filled here was read in the step before: those reads' results have been used)
-    queue[NB - 2] = push(buf == 0 ? NB - 1 : buf - 1);
-    if (NB == 2 && queue[0].b < a.batch && queue[0].first) load_q(queue[0].b);
-    attend(std::integral_constant<int, 1>{}, buf * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l, [&](ds_floatx4 (&sc)[1][2]) {
-      if (a.weights == nullptr || lq >= g) return;  // the logits themselves, for the keys' weights
-      float* const to = args()->logits;
+    if (queue[0].b < a.batch && queue[0].first) load_q(queue[0].b);
+    attend(
+        std::integral_constant<int, 1>{}, buf * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l,
+        [&](ds_floatx4 (&sc)[1][2]) {
+          if (a.weights == nullptr || lq >= g) return;  // the logits themselves, for the keys' weights
+          float* const to = args()->logits;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (((now.seen >> (16 * i)) & 0xffffu) != 0u)  // (no page: no key of it is seen)
-          *reinterpret_cast<ds_floatx4*>(to + ((((int64_t)now.ids.id[i] * a.hkv + kvh) * g + lq) << a.shift) + ((now.key + 16 * i + 4 * gr) & ((1 << a.shift) - 1))) = sc[0][i];
-    });
+          for (int i = 0; i < 2; ++i)
+            if (((now.seen >> (16 * i)) & 0xffffu) != 0u)  // (no page: no key of it is seen)
+              *reinterpret_cast<ds_floatx4*>(to + ((((int64_t)now.ids.id[i] * a.hkv + kvh) * g + lq) << a.shift) + ((now.key + 16 * i + 4 * gr) & ((1 << a.shift) - 1))) = sc[0][i];
+        },
+        [&] { queue[NB - 1] = push(buf); });
     wrote = now.last;
     if (now.last) {
       const auto r = args();
