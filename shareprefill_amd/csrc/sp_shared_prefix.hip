@@ -92,6 +92,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int lq = lane & 15, gr = lane >> 4;  // head (or key row, channel) in a 16-wide tile, lane group
   const int g = a.group, kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv;
+  const int slot = wave % SH_WAVES, half = wave / SH_WAVES;  // the wave's keys of a block, and its rows where two waves share them
   const int room = a.width << a.shift, n_groups = a.apart ? 0 : a.n_groups, items = n_groups + a.batch;
 
   // ---- requests and groups ----
@@ -193,8 +194,20 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) | (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
   };
   total = uniform64(total);
-  auto find = [&](int64_t cut) {  // the item that unit `cut` < total of the line lies in: the last that starts at or in front of it, by 64 candidates at a time
-    int lo = 0, span = items;
+  const int64_t parts = pg_parts(total, a.parts, SH_MIN_SHARE);
+  const int near = pg_near(total, parts);
+  const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
+  // Of the streams the groups alone are the workgroup's matter, else all items are.
+  const int shared_items = a.streams ? n_groups : items;
+  const int64_t shared_units = uniform64(line_s[shared_items]);
+  // Where a unit of the line is: item, tile and step; behind the last one: items.
+  struct Place {
+    int item, tile, step;
+  };
+  auto find = [&](int64_t cut, bool stream) {
+    Place f = {items, 0, 0};
+    if (cut >= total) return f;
+    int lo = 0, span = items;  // the item is the last that starts at or in front of it, by 64 candidates at a time
     while (span > 1) {
       const int step = (span + SP_WAVE - 1) / SP_WAVE;
       const int n = __builtin_popcountll(__ballot(lane * step < span && line_s[lo + lane * step] <= cut));
@@ -202,39 +215,37 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       span = pg_min(step, span - at);
       lo += at;
     }
-    return __builtin_amdgcn_readfirstlane(lo);
+    f.item = __builtin_amdgcn_readfirstlane(lo);
+    const int n = item(f.item).n;
+    const int64_t off = cut - line_s[f.item];
+    if (stream)
+      f.step = sh_stream_step(off, n);
+    else
+      sh_place(off, n, near, &f.tile, &f.step);
+    f.tile = __builtin_amdgcn_readfirstlane(f.tile), f.step = __builtin_amdgcn_readfirstlane(f.step);
+    return f;
   };
-  const int64_t parts = pg_parts(total, a.parts, SH_MIN_SHARE);
-  const int near = pg_near(total, parts);
-  const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
-  // Of the streams the groups alone are the workgroup's matter, else all items are.
-  const int shared_items = a.streams ? n_groups : items;
-  const int64_t shared_units = uniform64(line_s[shared_items]);
-  int from[2], tile[2], at_step[2];  // item, tile and step that the part begins with, and that it ends in front of
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int64_t cut = e == 0 ? cut0 : cut1;
-    from[e] = shared_items, tile[e] = 0, at_step[e] = 0;
-    if (cut < shared_units) {
-      from[e] = find(cut);
-      sh_place(cut - line_s[from[e]], item(from[e]).n, near, &tile[e], &at_step[e]);
-    }
-    tile[e] = __builtin_amdgcn_readfirstlane(tile[e]), at_step[e] = __builtin_amdgcn_readfirstlane(at_step[e]);
-  }
-  int stream_b[2] = {a.batch, a.batch}, stream_step[2] = {0, 0};  // the same of a wave of the streams: request and step
-  if (a.streams && wave < WAVES) {
+  // What the workgroup begins with and ends in front of, and the same of a wave of the streams; kernels' first passes through their instructions are slow,
+  // so that one loop finds the four.
+  Place places[4];
+  {
     const int64_t own0 = cut0 > shared_units ? cut0 : shared_units, own1 = cut1 > shared_units ? cut1 : shared_units;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int64_t cut = uniform64(own0 + (own1 - own0) * (wave + e) / WAVES);
-      if (cut < total) {
-        const int x = find(cut);
-        stream_b[e] = x - n_groups;
-        stream_step[e] = __builtin_amdgcn_readfirstlane(sh_stream_step(cut - line_s[x], item(x).n));
-      }
+    Place f0 = {shared_items, 0, 0}, f1 = f0, f2 = {items, 0, 0}, f3 = f2;
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+      const int64_t cut = e == 0 ? cut0 : e == 1 ? cut1 : uniform64(own0 + (own1 - own0) * (slot + e - 2) / WAVES);
+      if (e < 2 ? cut >= shared_units : !a.streams) continue;
+      const Place f = find(cut, e >= 2);
+      if (e == 0) f0 = f;
+      if (e == 1) f1 = f;
+      if (e == 2) f2 = f;
+      if (e == 3) f3 = f;
     }
-    if (kvh == 0 && lane == 0) a.cuts[part * WAVES + wave] = make_int4(stream_b[0], stream_step[0], stream_b[1], stream_step[1]);
+    places[0] = f0, places[1] = f1, places[2] = f2, places[3] = f3;
   }
+  const Place &from = places[0], &to_place = places[1];
+  if (a.streams && half == 0 && kvh == 0 && lane == 0)
+    a.cuts[part * WAVES + slot] = make_int4(places[2].item - n_groups, places[2].step, places[3].item - n_groups, places[3].step);
 
   // Arguments of what is done once an item are read where they are used: scalar registers do not suffice to keep them.
   const auto kernel_args = (const __attribute__((address_space(4))) ShArgs*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -244,7 +255,6 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     return p;
   };
   const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
-  const int slot = wave % WAVES, half = wave / WAVES;  // the wave's keys of a block, and its rows where two waves share them
   const uint32_t ring = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds + slot * NB * Shape::STEP_BYTES;
   const uint32_t k_at = ring + lq * (D * 2);
   const int v_key = 4 * gr + (lq >> 2);  // row of the transposing read; 16 rows further the swizzle is the same
@@ -301,9 +311,8 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     return seen;
   };
   // One step of a wave's rows, RT tiles of 16: its operands lie at `off` of the wave's ring, its first key is `key`, `mine` says which are seen; partly: some rows
-  // do not see some of them, those behind pos.  m, l: the rows' maxima and sums (the same four times).  logits(sc) is called with the logits, done() when the
-  // operands have been read.
-  auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits, auto&& done) {
+  // do not see some of them, those behind pos.  m, l: the rows' maxima and sums (the same four times).  logits(sc) is called with the logits.
+  auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits) {
     constexpr int RT = decltype(tiles)::value;
     constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
     dc_u32x4 kr[2][KS];
@@ -400,7 +409,6 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[ct][0]), "+v"(vr[ct][1]));
-    done();
     // Where a row does not see a key, 0 times a value that is no number would make a NaN of its sum: the product takes zeros in such places, and rows
     // that do see such a key have a sum of weights that is none.
     if (partly) {
@@ -464,11 +472,10 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
   };
 
-  // RT: row tiles of 16 of a wave.  One: waves 0 .. 3 with a ring each.  Two: the waves of a slot have 32 rows each of its keys, one loads K and the other V, and
-  // all meet at a barrier every block of four steps.
-  auto run = [&](auto tiles, const ShItem& p, int begin, int s_end, bool of_group) {
-    constexpr int RT = decltype(tiles)::value;
-    const int tile_row = RT == 1 ? 0 : 16 * RT * half;  // the wave's first row in the tile
+  // A tile's steps: the two waves of a slot have 32 rows each of its keys, one loads K and the other V, and all meet twice in a block of four steps.
+  auto run = [&](const ShItem& p, int begin, int s_end, bool of_group) {
+    constexpr int RT = SH_TILE / 32;
+    const int tile_row = 16 * RT * half;  // the wave's first row in the tile
     auto row_of = [&](int in_tile, int* token, int* head) {
       const int r = pg_min(p.row0 + in_tile, p.rows - 1);
       *token = (int)pg_div((unsigned)r, a.by_group);
@@ -502,58 +509,42 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       m[rt] = -INFINITY, l[rt] = (ds_floatx4){0, 0, 0, 0};
     }
 
-    auto ask = [&](int buf, int step, Ids ids) {
-      return fetch(ring + buf * Shape::STEP_BYTES, key_of(step), p.key0, p.key1, ids, RT == 1 || half == 0, RT == 1 || half == 1);
-    };
-    auto step = [&](int x, uint32_t mine, uint32_t off, auto&& done) {
-      const int key = key_of(x);
-      // (uniform: some row does not see a key that others see)
-      attend(tiles, off, key, mine, qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0, o, m, l, [](ds_floatx4 (&)[RT][2]) {}, done);
-    };
-
     __syncthreads();  // the rings are free
-    // The ring holds NB steps; a step's place is filled again as soon as its operands have been read.
-    constexpr int MINE = RT == 1 ? Shape::LOADS : Shape::LOADS / 2;  // loads of the wave for a step
+    // The ring holds NB steps; a step's place is filled again when its operands have been read.  The first NB rounds do nothing but fill.
+    constexpr int MINE = Shape::LOADS / 2;  // loads of the wave for a step
     const int s0 = begin + slot;
-    if (RT > 1 || half == 0) {
-      uint32_t seen[NB];
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        seen[i] = 0;
-        if (s0 + i * WAVES < s_end) seen[i] = ask(i, s0 + i * WAVES, entries(table, key_of(s0 + i * WAVES)));
-      }
-      Ids next = {{0, 0}};
-      if (s0 + NB * WAVES < s_end) next = entries(table, key_of(s0 + NB * WAVES));
-      int buf = 0;
-      // (of larger tiles all waves go through all blocks: they meet twice in each)
-      for (int s = s0; s < s_end || (RT > 1 && s - slot < s_end); s += WAVES) {
+    uint32_t seen[NB];
+    Ids next = {{0, 0}};
+    if (s0 < s_end) next = entries(table, key_of(s0));
+    int buf = 0;
+    for (int s = s0 - NB * WAVES; s - slot < s_end; s += WAVES) {
+      if (s >= begin) {
         // the step's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
         if (s + (NB - 1) * WAVES < s_end)
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * MINE) : "memory");
+          asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NB - 1) * MINE) : "memory");
         else
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if constexpr (RT > 1) asm volatile("s_barrier" ::: "memory");
-        const uint32_t mine = seen[0];
-        auto done = [&] {
-          if constexpr (RT > 1) asm volatile("s_barrier" ::: "memory");  // the other wave has read them too
-#pragma unroll
-          for (int i = 0; i + 1 < NB; ++i) seen[i] = seen[i + 1];
-          if (s + NB * WAVES < s_end) {
-            seen[NB - 1] = ask(buf, s + NB * WAVES, next);
-            if (s + (NB + 1) * WAVES < s_end) next = entries(table, key_of(s + (NB + 1) * WAVES));
-          }
-        };
-        if (s < s_end)
-          step(s, mine, buf * Shape::STEP_BYTES, done);
-        else
-          done();
-        buf = buf + 1 == NB ? 0 : buf + 1;
+          asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s < s_end) {
+          const int key = key_of(s);
+          // (uniform: some row does not see a key that others see)
+          attend(std::integral_constant<int, RT>{}, buf * Shape::STEP_BYTES, key, seen[0], qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0, o, m, l,
+                 [](ds_floatx4 (&)[RT][2]) {});
+        }
+        asm volatile("s_barrier" ::: "memory");  // the other wave has read them too
       }
+#pragma unroll
+      for (int i = 0; i + 1 < NB; ++i) seen[i] = seen[i + 1];
+      const int ahead = s + NB * WAVES;
+      if (ahead < s_end) {
+        seen[NB - 1] = fetch(ring + buf * Shape::STEP_BYTES, key_of(ahead), p.key0, p.key1, next, half == 0, half == 1);
+        if (ahead + WAVES < s_end) next = entries(table, key_of(ahead + WAVES));
+      }
+      buf = buf + 1 == NB ? 0 : buf + 1;
     }
     __syncthreads();  // the rings are free
     // [slot][SH_TILE][D] floats, 16-byte pieces swizzled by the row
     float* const o_s = reinterpret_cast<float*>(lds);
-    if (RT > 1 || half == 0) {
+    {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int r = slot * SH_TILE + tile_row + 16 * rt + lq;
@@ -565,7 +556,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     __syncthreads();
     const auto to_args = args();
     const bool whole = begin == 0 && s_end == p.n;
-    const int rows = pg_min(p.rows - p.row0, RT == 1 ? 16 : SH_TILE);
+    const int rows = pg_min(p.rows - p.row0, SH_TILE);
     const int64_t slab = ((int64_t)(part * a.hkv + kvh) * 2 + (begin == 0 ? 1 : 0)) * SH_TILE;
     const bool final = whole && p.key0 == 0 && !of_group;
     for (int i = t; i < rows * (D / 4); i += SH_THREADS) {
@@ -596,7 +587,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
   };
 
-  for (int x = from[0], first_tile = tile[0], begin = at_step[0]; x < shared_items && x <= from[1]; ++x, first_tile = 0, begin = 0) {
+  for (int x = from.item, first_tile = from.tile, begin = from.step; x < shared_items && x <= to_place.item; ++x, first_tile = 0, begin = 0) {
     ShItem p = item(x);
     if (p.n == 0) continue;
     // (uniform: out of vector registers)
@@ -606,9 +597,8 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     p.slot = __builtin_amdgcn_readfirstlane(p.slot);
     const int key1 = __builtin_amdgcn_readfirstlane(p.key1);
     for (int at = first_tile; at * SH_TILE < p.rows; ++at, begin = 0) {
-      const bool last = x == from[1] && at == tile[1];
-      const int end = last ? pg_min(at_step[1], p.n) : p.n;
-      if (x == from[1] && at > tile[1]) break;
+      if (x == to_place.item && at > to_place.tile) break;
+      const int end = x == to_place.item && at == to_place.tile ? pg_min(to_place.step, p.n) : p.n;
       if (begin >= end) continue;
       p.row0 = at * SH_TILE;
       // (of a request's tile: up to its last row's position)
@@ -617,10 +607,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
         if (begin == 0) a.parts_of[p.slot + at].x = part;
         if (end == p.n) a.parts_of[p.slot + at].y = part;
       }
-      if (p.rows - p.row0 <= 16)
-        run(std::integral_constant<int, 1>{}, p, begin, end, x < n_groups);
-      else
-        run(std::integral_constant<int, SH_TILE / 32>{}, p, begin, end, x < n_groups);
+      run(p, begin, end, x < n_groups);
     }
   }
   if (!a.streams) return;
@@ -628,7 +615,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   // ---- single tokens over their own keys, a wave by itself ----
   __syncthreads();  // the rings are free
   if (half != 0) return;
-  const int b0 = stream_b[0], b1 = stream_b[1], step0 = stream_step[0], step1 = stream_step[1], wave_part = part * WAVES + slot;
+  const int b0 = places[2].item - n_groups, b1 = places[3].item - n_groups, step0 = places[2].step, step1 = places[3].step, wave_part = part * WAVES + slot;
   struct At {  // a step of request b (b = batch: none is left): steps up to `end` of its n fall to the wave
     int b, s, end, n, lo, key0, key1;
   };
@@ -681,46 +668,46 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   if (ahead.b < a.batch) load_q(ahead.b);
   Step queue[NB];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) queue[i] = push(i);
-  ds_floatx4 o[1][CT];
-  ds_floatx4 l[1];
+  for (int i = 0; i < NB; ++i) queue[i] = {-1, 0, 0u, {{0, 0}}, false, false, false, false, false};  // (the first NB rounds do nothing but fill)
+  ds_floatx4 o[1][CT], l[1];
   float m[1];
   int pos[1] = {0};
   int buf = 0;
   bool wrote = false;  // at least CT stores are younger than all loads
   while (queue[0].b < a.batch) {
-    // the step's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
-    if (queue[NB - 1].b >= a.batch)
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else if (wrote)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * Shape::LOADS + CT) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * Shape::LOADS) : "memory");
     const Step now = queue[0];
+    if (now.b >= 0) {
+      // the step's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
+      if (queue[NB - 1].b >= a.batch)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else if (wrote)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * Shape::LOADS + CT) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * Shape::LOADS) : "memory");
+      if (now.first) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qb[0][ks] = q_next[ks];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) o[0][ct] = (ds_floatx4){0, 0, 0, 0};
+        m[0] = -INFINITY, l[0] = (ds_floatx4){0, 0, 0, 0};
+      }
+        if (queue[1].b < a.batch && queue[1].first) load_q(queue[1].b);
+      attend(
+          std::integral_constant<int, 1>{}, buf * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l,
+          [&](ds_floatx4 (&sc)[1][2]) {
+            if (a.weights == nullptr || lq >= g) return;  // the logits themselves, for the keys' weights
+            float* const to = args()->logits;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (((now.seen >> (16 * i)) & 0xffffu) != 0u)  // (no page: no key of it is seen)
+                *reinterpret_cast<ds_floatx4*>(to + ((((int64_t)now.ids.id[i] * a.hkv + kvh) * g + lq) << a.shift) + ((now.key + 16 * i + 4 * gr) & ((1 << a.shift) - 1))) = sc[0][i];
+          });
+    }
 #pragma unroll
     for (int i = 0; i + 1 < NB; ++i) queue[i] = queue[i + 1];
-    queue[NB - 1].b = a.batch;
-    if (now.first) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qb[0][ks] = q_next[ks];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[0][ct] = (ds_floatx4){0, 0, 0, 0};
-      m[0] = -INFINITY, l[0] = (ds_floatx4){0, 0, 0, 0};
-    }
-    if (queue[0].b < a.batch && queue[0].first) load_q(queue[0].b);
-    attend(
-        std::integral_constant<int, 1>{}, buf * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l,
-        [&](ds_floatx4 (&sc)[1][2]) {
-          if (a.weights == nullptr || lq >= g) return;  // the logits themselves, for the keys' weights
-          float* const to = args()->logits;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (((now.seen >> (16 * i)) & 0xffffu) != 0u)  // (no page: no key of it is seen)
-              *reinterpret_cast<ds_floatx4*>(to + ((((int64_t)now.ids.id[i] * a.hkv + kvh) * g + lq) << a.shift) + ((now.key + 16 * i + 4 * gr) & ((1 << a.shift) - 1))) = sc[0][i];
-        },
-        [&] { queue[NB - 1] = push(buf); });
-    wrote = now.last;
-    if (now.last) {
+    queue[NB - 1] = push(buf);
+    wrote = now.b >= 0 && now.last;
+    if (wrote) {
       const auto r = args();
       const float sum = l[0][0];
       const int64_t row = (int64_t)now.b * (a.hkv * g) + kvh * g + lq;
