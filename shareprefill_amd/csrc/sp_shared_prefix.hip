@@ -3,13 +3,12 @@
 // the sum over the shared keys formed once for all rows of the group and joined with that over the request's own: with running maxima m and
 // sums l of either side, out = (2^(m1 - m) o1 + 2^(m2 - m) o2) / (2^(m1 - m) l1 + 2^(m2 - m) l2).
 //
-// HBM-bound as long as a group has fewer than some 250 rows a kv head, (token, query head) pairs: shared keys are read once per tile of 64 rows, a
-// request's own once.  Three loops over steps of 32 keys, whose operands direct loads bring to rings in LDS:
+// HBM-bound as long as a group has fewer than some 250 rows a kv head, (token, query head) pairs: shared keys are read once per tile of up to 128
+// rows, a request's own once.  Two loops over steps of 32 keys, whose operands direct loads bring to rings in LDS:
 //   * single tokens of up to 16 heads over their own keys: a wave goes by itself through the steps of one request after the other, the next one's
 //     first keys on their way under the end of the one in front; no barrier, and nobody waits for a request to end;
-//   * other tiles of up to 16 rows: four waves take the tile's steps in turn and meet in LDS at the end;
-//   * larger tiles: two waves of 32 rows each share a ring, and all meet at a barrier every four steps; the two share a SIMD, where the matrix
-//     instructions of one run under the exponentials of the other.
+//   * tiles of up to 128 rows: eight waves share blocks of four steps and meet twice in each; a wave has 32 rows, and the waves of the same rows
+//     share out the steps.  Two waves share a SIMD, where the matrix instructions of one run under the exponentials of the other.
 // Groups of many rows go to sp_chunk.hip's loop first, in a launch of its own.
 //
 // The line that the workgroups' parts are cut from (sp_shared_plan.h) is formed by every wave for itself, 64 items at a time.
@@ -41,8 +40,8 @@ struct ShArgs {
   int apart;                  // groups have been seen to (o_row, ml_row)
   int streams;                // single tokens of up to 16 heads: a request's parts are waves', four a workgroup
   float scale_log2;
-  float* o_part;              // [part][kv head][2][SH_TILE][D]: a row tile that began in an earlier part, one that goes on in the next
-  float2* ml_part;            // [part][kv head][2][SH_TILE]
+  float* o_part;              // [part][kv head][2][SH_ROWS][D]: a row tile that began in an earlier part, one that goes on in the next
+  float2* ml_part;            // [part][kv head][2][SH_ROWS]
   float* o_stream;            // [part of a wave][kv head][2][16][D]
   float2* ml_stream;
   float* o_row;               // [2][token][query head][D]: row tiles that lie in one part, of groups and of requests
@@ -59,11 +58,13 @@ template <int D>
 using ShShape = DsShape<D, D / 16, SH_WAVES, 128>;
 // LDS: the rings, where the waves meet afterwards; their maxima and sums; what is known of the requests and groups
 #define SH_RING 131072
-#define SH_ML (SH_RING)                                // [2][SH_WAVES][SH_TILE] floats
-#define SH_SUMS (SH_ML + 2 * SH_WAVES * SH_TILE * 4)  // [2 SH_WAVES + 1] int64
-#define SH_ARRAYS (SH_SUMS + 80)
+#define SH_MEET (2 * SH_WAVES * 32)  // rows that the waves bring together
+#define SH_ML (SH_RING)              // [2][SH_MEET] floats
+#define SH_SUMS (SH_ML + 2 * SH_MEET * 4)  // [2 SH_WAVES + 1] int64
+#define SH_SEEN (SH_SUMS + 80)                        // [SH_WAVES][4] words
+#define SH_ARRAYS (SH_SEEN + 64)
 static size_t sh_lds_bytes(int batch, int groups) { return SH_ARRAYS + (3 * ((size_t)batch + 1) + 2 * ((size_t)groups + 1)) * sizeof(int); }
-static_assert(ShShape<128>::LDS_BYTES <= SH_RING && ShShape<64>::LDS_BYTES <= SH_RING && SH_WAVES * SH_TILE * 128 * 4 <= SH_RING && (2 * SH_MAX_SEQS + 1) * 8 <= SH_RING, "");
+static_assert(ShShape<128>::LDS_BYTES <= SH_RING && ShShape<64>::LDS_BYTES <= SH_RING && SH_MEET * 128 * 4 <= SH_RING && (2 * SH_MAX_SEQS + 1) * 8 <= SH_RING, "");
 
 template <int IMM>
 __device__ static __forceinline__ dc_u32x4 sh_read_k(uint32_t addr) {  // (as ds_read_k)
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       p.start = start_s[group_s[x]];
       p.rows = (start_s[group_s[x + 1]] - p.start) * g;
       p.key0 = 0, p.key1 = shared_s[x], p.pos = PG_MAX_KEYS;
-      p.slot = (int)pg_first_slot(p.start, g, x, SH_TILE);
+      p.slot = (int)pg_first_slot(p.start, g, x, SH_UNIT);
     } else {
       const int b = x - n_groups, q_len = start_s[b + 1] - start_s[b];
       p.table_row = b;
@@ -216,12 +217,13 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       lo += at;
     }
     f.item = __builtin_amdgcn_readfirstlane(lo);
-    const int n = item(f.item).n;
+    const ShItem p = item(f.item);
+    const int n = p.n;
     const int64_t off = cut - line_s[f.item];
     if (stream)
       f.step = sh_stream_step(off, n);
     else
-      sh_place(off, n, near, &f.tile, &f.step);
+      sh_place(off, n, p.rows, near, &f.tile, &f.step);
     f.tile = __builtin_amdgcn_readfirstlane(f.tile), f.step = __builtin_amdgcn_readfirstlane(f.step);
     return f;
   };
@@ -255,15 +257,13 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     return p;
   };
   const uint32_t k_row = (uint32_t)a.sk_n * 2u, v_row = (uint32_t)a.sv_n * 2u;  // bytes
-  const uint32_t ring = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds + slot * NB * Shape::STEP_BYTES;
-  const uint32_t k_at = ring + lq * (D * 2);
+  const uint32_t rings = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds, ring = rings + slot * NB * Shape::STEP_BYTES;
+  const uint32_t k_at = rings + lq * (D * 2);
   const int v_key = 4 * gr + (lq >> 2);  // row of the transposing read; 16 rows further the swizzle is the same
-  const uint32_t v_at = ring + Shape::K_BYTES + v_key * (CT * 32) + 8 * (lq & 3);
+  const uint32_t v_at = rings + Shape::K_BYTES + v_key * (CT * 32) + 8 * (lq & 3);
   float* const m_s = reinterpret_cast<float*>(lds + SH_ML);
-  float* const l_s = m_s + WAVES * SH_TILE;
+  float* const l_s = m_s + SH_MEET;
 
-  dc_bf16x8 ones = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-  asm volatile("" : "+v"(ones));  // one register set throughout
   const char* const kh = (const char*)(a.k + kvh * a.sk_h);
   const char* const vh = (const char*)(a.v + kvh * a.sv_h);
   struct Ids {
@@ -291,6 +291,9 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       if (page < 0) seen &= h == 0 ? 0xffff0000u : 0x0000ffffu;
       id[h] = pg_max(page, 0);
     }
+    // (formed anew for every step: kept in registers they would crowd out what the loop needs)
+    int lane_here = lane;
+    asm volatile("" : "+v"(lane_here));
     auto load = [&](const char* from, int64_t page_bytes, uint32_t row_bytes, uint32_t to, auto&& chunk) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -299,19 +302,19 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
             there[h] > 0 ? (int)((uint32_t)(there[h] - 1) * row_bytes + 2u * D) : 0, 0x00027000);
 #pragma unroll
         for (int i = 0; i < HALF; ++i) {
-          const int row = i * ROWS + lane / CHUNKS;
+          const int row = i * ROWS + lane_here / CHUNKS;
           uint32_t off = (uint32_t)row * row_bytes + 16u * (uint32_t)chunk(16 * h + row);
           off = (seen >> (16 * h + row)) & 1u ? off : 0x7ffffff0u;  // (past the buffer's end: zeros)
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (ds_lds_ptr)(uintptr_t)(to + (h * HALF + i) * 1024), 16, (int)off, 0, 0, 0);
         }
       }
     };
-    if (with_k) load(kh, a.sk_p * 2, k_row, at, [&](int row) { return (lane % CHUNKS) ^ ds_swz_k<D>(row); });
-    if (with_v) load(vh, a.sv_p * 2, v_row, at + Shape::K_BYTES, [&](int row) { return (lane % CHUNKS) ^ (2 * ds_swz_v<CT>(row)); });
+    if (with_k) load(kh, a.sk_p * 2, k_row, at, [&](int row) { return (lane_here % CHUNKS) ^ ds_swz_k<D>(row); });
+    if (with_v) load(vh, a.sv_p * 2, v_row, at + Shape::K_BYTES, [&](int row) { return (lane_here % CHUNKS) ^ (2 * ds_swz_v<CT>(row)); });
     return seen;
   };
-  // One step of a wave's rows, RT tiles of 16: its operands lie at `off` of the wave's ring, its first key is `key`, `mine` says which are seen; partly: some rows
-  // do not see some of them, those behind pos.  m, l: the rows' maxima and sums (the same four times).  logits(sc) is called with the logits.
+  // One step of a wave's rows, RT tiles of 16: its operands lie at `off` of the rings, its first key is `key`, `mine` says which are seen; partly: some rows
+  // do not see some of them, those behind pos.  m, l: the rows' maxima, and the sums of this lane group's keys.  logits(sc) is called with the logits.
   auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits) {
     constexpr int RT = decltype(tiles)::value;
     constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
@@ -402,6 +405,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
           const float p0 = __builtin_amdgcn_exp2f(sc[rt][i][j] - base), p1 = __builtin_amdgcn_exp2f(sc[rt][i][j + 1] - base);
           const uint32_t w = dc_pack2(p0, p1);
           hi[2 * i + j / 2] = w;
+          l[rt] += p0 + p1;
           if constexpr (TWO) lw[2 * i + j / 2] = dc_pack2(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
         }
       ph[rt] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){hi[0], hi[1], hi[2], hi[3]});
@@ -447,17 +451,11 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
                 if (key + 16 * h + 4 * gr + j <= pos[rt]) met |= 1u << rt;
             }
         }
-        met |= __shfl_xor(met, 16, SP_WAVE);
-        met |= __shfl_xor(met, 32, SP_WAVE);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           if ((met >> rt) & 1u) l[rt] *= __builtin_nanf("");
       }
     }
-    // (the sums are those of what the product takes: an output is a mean of values, whatever its weights' roundings)
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) l[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, ph[rt], l[rt], 0, 0, 0);
-    if constexpr (TWO) l[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pl[0], l[0], 0, 0, 0);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -472,10 +470,12 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     }
   };
 
-  // A tile's steps: the two waves of a slot have 32 rows each of its keys, one loads K and the other V, and all meet twice in a block of four steps.
+  // A tile's steps: wave w has rows 32 (w / share) .. of the tile and of a block's four steps w % share, + share, ..; it fills K's or V's half of ring
+  // w % 4, and all meet twice in a block.
   auto run = [&](const ShItem& p, int begin, int s_end, bool of_group) {
-    constexpr int RT = SH_TILE / 32;
-    const int tile_row = 16 * RT * half;  // the wave's first row in the tile
+    constexpr int RT = 2;
+    const int tile = sh_tile(p.rows - p.row0), share = SH_MEET / tile;  // (as few rows as there are: waves without any would only wait)
+    const int mine_of = wave & (share - 1), tile_row = 32 * (wave / share);
     auto row_of = [&](int in_tile, int* token, int* head) {
       const int r = pg_min(p.row0 + in_tile, p.rows - 1);
       *token = (int)pg_div((unsigned)r, a.by_group);
@@ -500,77 +500,89 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     const auto table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.table + (int64_t)p.table_row * a.table_stride);
     auto key_of = [&](int step) { return (p.lo + step) * SH_KEYS; };
     ds_floatx4 o[RT][CT];
-    ds_floatx4 l[RT];
-    float m[RT];
+    float m[RT], l[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) o[rt][ct] = (ds_floatx4){0, 0, 0, 0};
-      m[rt] = -INFINITY, l[rt] = (ds_floatx4){0, 0, 0, 0};
+      m[rt] = -INFINITY, l[rt] = 0.f;
     }
 
     __syncthreads();  // the rings are free
     // The ring holds NB steps; a step's place is filled again when its operands have been read.  The first NB rounds do nothing but fill.
     constexpr int MINE = Shape::LOADS / 2;  // loads of the wave for a step
     const int s0 = begin + slot;
-    uint32_t seen[NB];
-    Ids next = {{0, 0}};
-    if (s0 < s_end) next = entries(table, key_of(s0));
+    const bool has_rows = p.row0 + tile_row < p.rows;
+    // which keys of a step are any: the wave that fetches it leaves a word for all (LDS accesses of its own: the compiler would wait for all loads in flight
+    // in front of them)
+    const uint32_t seen_at = rings + SH_SEEN;
+    auto any_of = [&](int j, int of_buf) {
+      uint32_t v;
+      asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(v) : "v"(seen_at + 4u * (uint32_t)(j * NB + of_buf)));
+      return (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+    };
+    Ids next[NB];  // pages of the wave's step of the blocks to come
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      if (s0 + i * WAVES < s_end) next[i] = entries(table, key_of(s0 + i * WAVES));
     int buf = 0;
     for (int s = s0 - NB * WAVES; s - slot < s_end; s += WAVES) {
       if (s >= begin) {
-        // the step's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
+        // the block's loads have landed, those of the NB - 1 behind it stay in flight (what is asked for returns in order)
         if (s + (NB - 1) * WAVES < s_end)
-          asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NB - 1) * MINE) : "memory");
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NB - 1) * MINE) : "memory");
         else
-          asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s < s_end) {
-          const int key = key_of(s);
-          // (uniform: some row does not see a key that others see)
-          attend(std::integral_constant<int, RT>{}, buf * Shape::STEP_BYTES, key, seen[0], qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0, o, m, l,
-                 [](ds_floatx4 (&)[RT][2]) {});
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (has_rows) {
+          for (int j = mine_of; j < WAVES && s - slot + j < s_end; j += share) {
+            const int key = key_of(s - slot + j);
+            // (uniform: some row does not see a key that others see)
+            attend(std::integral_constant<int, RT>{}, (j * NB + buf) * Shape::STEP_BYTES, key, any_of(j, buf), qb, pos, pg_min(key + SH_KEYS, p.key1) - 1 > pos0,
+                   o, m, l, [](ds_floatx4 (&)[RT][2]) {});
+          }
         }
-        asm volatile("s_barrier" ::: "memory");  // the other wave has read them too
+        asm volatile("s_barrier" ::: "memory");  // the others have read them too
       }
-#pragma unroll
-      for (int i = 0; i + 1 < NB; ++i) seen[i] = seen[i + 1];
       const int ahead = s + NB * WAVES;
       if (ahead < s_end) {
-        seen[NB - 1] = fetch(ring + buf * Shape::STEP_BYTES, key_of(ahead), p.key0, p.key1, next, half == 0, half == 1);
-        if (ahead + WAVES < s_end) next = entries(table, key_of(ahead + WAVES));
+        const uint32_t seen = fetch(ring + buf * Shape::STEP_BYTES, key_of(ahead), p.key0, p.key1, next[0], half == 0, half == 1);
+        if (half == 0) asm volatile("ds_write_b32 %0, %1" ::"v"(seen_at + 4u * (uint32_t)(slot * NB + buf)), "v"(seen) : "memory");
       }
+#pragma unroll
+      for (int i = 0; i + 1 < NB; ++i) next[i] = next[i + 1];
+      if (ahead + NB * WAVES < s_end) next[NB - 1] = entries(table, key_of(ahead + NB * WAVES));
       buf = buf + 1 == NB ? 0 : buf + 1;
     }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l[rt] = ds_quad_sum(l[rt]);
     __syncthreads();  // the rings are free
-    // [slot][SH_TILE][D] floats, 16-byte pieces swizzled by the row
+    // [share][tile][D] floats, 16-byte pieces swizzled by the row
     float* const o_s = reinterpret_cast<float*>(lds);
     {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const int r = slot * SH_TILE + tile_row + 16 * rt + lq;
+        const int r = mine_of * tile + tile_row + 16 * rt + lq;
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) *reinterpret_cast<ds_floatx4*>(o_s + r * D + ((4 * ct + gr) ^ lq) * 4) = o[rt][ct];
-        if (gr == 0) m_s[r] = m[rt], l_s[r] = l[rt][0];
+        if (gr == 0) m_s[r] = m[rt], l_s[r] = l[rt];
       }
     }
     __syncthreads();
     const auto to_args = args();
     const bool whole = begin == 0 && s_end == p.n;
-    const int rows = pg_min(p.rows - p.row0, SH_TILE);
-    const int64_t slab = ((int64_t)(part * a.hkv + kvh) * 2 + (begin == 0 ? 1 : 0)) * SH_TILE;
+    const int rows = pg_min(p.rows - p.row0, tile);
+    const int64_t slab = ((int64_t)(part * a.hkv + kvh) * 2 + (begin == 0 ? 1 : 0)) * SH_ROWS;
     const bool final = whole && p.key0 == 0 && !of_group;
     for (int i = t; i < rows * (D / 4); i += SH_THREADS) {
       const int r = i / (D / 4), c = i % (D / 4);
       float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) top = fmaxf(top, m_s[w * SH_TILE + r]);
+      for (int w = 0; w < share; ++w) top = fmaxf(top, m_s[w * tile + r]);
       ds_floatx4 acc = {0, 0, 0, 0};
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        const float mw = m_s[w * SH_TILE + r];
-        const float f = mw == -INFINITY && l_s[w * SH_TILE + r] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mw - top);  // (a wave without keys: 0)
-        sum += l_s[w * SH_TILE + r] * f;
-        acc += *reinterpret_cast<const ds_floatx4*>(o_s + (w * SH_TILE + r) * D + (c ^ (r & 15)) * 4) * f;
+      for (int w = 0; w < share; ++w) {
+        const float mw = m_s[w * tile + r];
+        const float f = mw == -INFINITY && l_s[w * tile + r] == 0.f ? 0.f : __builtin_amdgcn_exp2f(mw - top);  // (a wave without keys: 0)
+        sum += l_s[w * tile + r] * f;
+        acc += *reinterpret_cast<const ds_floatx4*>(o_s + (w * tile + r) * D + (c ^ (r & 15)) * 4) * f;
       }
       int token, head;
       row_of(r, &token, &head);
@@ -596,16 +608,17 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     p.pos = __builtin_amdgcn_readfirstlane(p.pos), p.lo = __builtin_amdgcn_readfirstlane(p.lo), p.n = __builtin_amdgcn_readfirstlane(p.n);
     p.slot = __builtin_amdgcn_readfirstlane(p.slot);
     const int key1 = __builtin_amdgcn_readfirstlane(p.key1);
-    for (int at = first_tile; at * SH_TILE < p.rows; ++at, begin = 0) {
+    const int tile = sh_tile(p.rows);
+    for (int at = first_tile; at * tile < p.rows; ++at, begin = 0) {
       if (x == to_place.item && at > to_place.tile) break;
       const int end = x == to_place.item && at == to_place.tile ? pg_min(to_place.step, p.n) : p.n;
       if (begin >= end) continue;
-      p.row0 = at * SH_TILE;
+      p.row0 = at * tile;
       // (of a request's tile: up to its last row's position)
-      p.key1 = x < n_groups ? key1 : pg_min(key1, p.pos + (int)pg_div((unsigned)(pg_min(p.row0 + SH_TILE, p.rows) - 1), a.by_group) + 1);
+      p.key1 = x < n_groups ? key1 : pg_min(key1, p.pos + (int)pg_div((unsigned)(pg_min(p.row0 + tile, p.rows) - 1), a.by_group) + 1);
       if (kvh == 0 && t == 0) {
-        if (begin == 0) a.parts_of[p.slot + at].x = part;
-        if (end == p.n) a.parts_of[p.slot + at].y = part;
+        if (begin == 0) a.parts_of[p.slot + p.row0 / SH_UNIT].x = part;
+        if (end == p.n) a.parts_of[p.slot + p.row0 / SH_UNIT].y = part;
       }
       run(p, begin, end, x < n_groups);
     }
@@ -669,8 +682,8 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   Step queue[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) queue[i] = {-1, 0, 0u, {{0, 0}}, false, false, false, false, false};  // (the first NB rounds do nothing but fill)
-  ds_floatx4 o[1][CT], l[1];
-  float m[1];
+  ds_floatx4 o[1][CT];
+  float m[1], l[1];
   int pos[1] = {0};
   int buf = 0;
   bool wrote = false;  // at least CT stores are younger than all loads
@@ -689,11 +702,11 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
         for (int ks = 0; ks < KS; ++ks) qb[0][ks] = q_next[ks];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) o[0][ct] = (ds_floatx4){0, 0, 0, 0};
-        m[0] = -INFINITY, l[0] = (ds_floatx4){0, 0, 0, 0};
+        m[0] = -INFINITY, l[0] = 0.f;
       }
         if (queue[1].b < a.batch && queue[1].first) load_q(queue[1].b);
       attend(
-          std::integral_constant<int, 1>{}, buf * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l,
+          std::integral_constant<int, 1>{}, (slot * NB + buf) * Shape::STEP_BYTES, now.key, now.seen, qb, pos, false, o, m, l,
           [&](ds_floatx4 (&sc)[1][2]) {
             if (a.weights == nullptr || lq >= g) return;  // the logits themselves, for the keys' weights
             float* const to = args()->logits;
@@ -709,7 +722,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     wrote = now.b >= 0 && now.last;
     if (wrote) {
       const auto r = args();
-      const float sum = l[0][0];
+      const float sum = ds_quad_sum(l[0]);
       const int64_t row = (int64_t)now.b * (a.hkv * g) + kvh * g + lq;
       const bool whole = now.from_start && now.to_end, final = whole && now.alone;
       if (lq < g) {
@@ -745,12 +758,12 @@ struct ShRow {
   int slot, in_tile;
 };
 __device__ __forceinline__ ShRow sh_group_row(const ShArgs& a, const ShRequest& r, int token, int h) {
-  const int row = (token - r.start0) * a.group + h;
-  return ShRow{(int)pg_first_slot(r.start0, a.group, r.group, SH_TILE) + row / SH_TILE, row % SH_TILE};
+  const int row = (token - r.start0) * a.group + h, first = row & -sh_tile((r.end0 - r.start0) * a.group);
+  return ShRow{(int)pg_first_slot(r.start0, a.group, r.group, SH_UNIT) + first / SH_UNIT, row - first};
 }
-__device__ __forceinline__ ShRow sh_own_row(const ShArgs& a, const ShRequest& r, int b, int token, int h) {
-  const int row = (token - r.start) * a.group + h;
-  return ShRow{a.shared_slots + (int)sh_own_slot(r.start, a.group, b, a.dense) + row / SH_TILE, row % SH_TILE};
+__device__ __forceinline__ ShRow sh_own_row(const ShArgs& a, const ShRequest& r, int end, int b, int token, int h) {
+  const int row = (token - r.start) * a.group + h, first = row & -sh_tile((end - r.start) * a.group);
+  return ShRow{a.shared_slots + (int)sh_own_slot(r.start, a.group, b, a.dense) + first / SH_UNIT, row - first};
 }
 // Parts that hold some of it: (0, -1) where there are no keys.
 __device__ __forceinline__ int2 sh_group_parts(const ShArgs& a, const ShRequest& r, const ShRow& row) {
@@ -789,7 +802,7 @@ __device__ __forceinline__ void sh_join(const ShArgs& a) {
   }
   const ShRequest r = a.of_request[b];
   const int end = a.of_request[b + 1].start, h = head - kvh * a.group;
-  const ShRow own = sh_own_row(a, r, b, token, h), group = sh_group_row(a, r, token, h);
+  const ShRow own = sh_own_row(a, r, end, b, token, h), group = sh_group_row(a, r, token, h);
   bool wanted = row < rows && token >= r.start && token < end;  // (a row outside every request)
   int2 own_parts = make_int2(0, -1), group_parts = own_parts;
   if (wanted) own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
@@ -808,7 +821,7 @@ __device__ __forceinline__ void sh_join(const ShArgs& a) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int i = pg_min(i0 + u * SETS, count - 1);
-        const int64_t at = count > 1 ? sh_slab(a, parts, i, kvh, it.in_tile, stream ? 16 : SH_TILE) : (of_group ? 0 : (int64_t)a.tokens * hq) + row;
+        const int64_t at = count > 1 ? sh_slab(a, parts, i, kvh, it.in_tile, stream ? 16 : SH_ROWS) : (of_group ? 0 : (int64_t)a.tokens * hq) + row;
         ml[u] = ml_from[at];
         o[u] = *reinterpret_cast<const ds_floatx4*>(o_from + at * D + c);
       }
@@ -862,7 +875,7 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
     if (keys <= r.first_own || begin >= end) continue;
     __syncthreads();  // (the rows before are done with)
     for (int h = wave; h < a.group; h += SM_THREADS / SP_WAVE) {  // a lane a part
-      const ShRow own = sh_own_row(a, r, b, b, h), group = sh_group_row(a, r, b, h);
+      const ShRow own = sh_own_row(a, r, r.start + 1, b, b, h), group = sh_group_row(a, r, b, h);
       const int2 own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
       float top = CK_NO_MAX, sum = 0.f;
       auto add = [&](int in_tile, int2 held, bool of_group) {
@@ -870,7 +883,7 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
         for (int i0 = 0; i0 < count; i0 += SP_WAVE) {
           float2 ml = make_float2(CK_NO_MAX, 0.f);
           if (i0 + lane < count)
-            ml = count > 1 ? (of_group ? a.ml_part : a.ml_stream)[sh_slab(a, held, i0 + lane, kvh, in_tile, of_group ? SH_TILE : 16)]
+            ml = count > 1 ? (of_group ? a.ml_part : a.ml_stream)[sh_slab(a, held, i0 + lane, kvh, in_tile, of_group ? SH_ROWS : 16)]
                            : a.ml_row[(of_group ? 0 : (int64_t)a.tokens * hq) + (int64_t)b * hq + kvh * a.group + h];
           const float to = fmaxf(top, sp_wave_max(ml.x));
           sum = sum * __builtin_amdgcn_exp2f(top - to) + sp_wave_sum(i0 + lane < count ? ml.y * __builtin_amdgcn_exp2f(ml.x - to) : 0.f);
@@ -932,10 +945,10 @@ struct ShSizes {
 static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d, bool single, int64_t pool_keys) {
   ShSizes s;
   const int64_t g = hq / hkv;
-  const bool apart = sh_apart(tokens, groups, g);
-  s.shared_slots = groups > 0 && !apart ? tokens * g / SH_TILE + groups : 0;
-  s.slots = s.shared_slots + (single && g <= SH_TILE ? batch : tokens * g / SH_TILE + batch);
-  const int64_t rows = (int64_t)sh_workgroups(hkv) * hkv * 2 * SH_TILE;
+  const bool apart = sh_apart(tokens, groups, g, pool_keys > 0);
+  s.shared_slots = groups > 0 && !apart ? tokens * g / SH_UNIT + groups : 0;
+  s.slots = s.shared_slots + (single && g <= SH_UNIT ? batch : tokens * g / SH_UNIT + batch);
+  const int64_t rows = (int64_t)sh_workgroups(hkv) * hkv * 2 * SH_ROWS;
   size_t at = 0;
   auto take = [&](size_t n) {
     const size_t here = at;
@@ -946,8 +959,9 @@ static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t h
   s.o_part = take(apart ? ck_groups_workspace_bytes((int)hkv, (int)d) : (size_t)rows * d * sizeof(float));
   s.ml_part = take((size_t)rows * sizeof(float2));
   const bool streams = single && g <= PD_MAX_GROUP;
-  s.o_stream = take(streams ? (size_t)rows * d * sizeof(float) : 0);  // (as many rows: a quarter of them four times)
-  s.ml_stream = take(streams ? (size_t)rows * sizeof(float2) : 0);
+  const int64_t stream_rows = streams ? (int64_t)sh_workgroups(hkv) * hkv * SH_WAVES * 2 * PD_MAX_GROUP : 0;
+  s.o_stream = take((size_t)stream_rows * d * sizeof(float));
+  s.ml_stream = take((size_t)stream_rows * sizeof(float2));
   s.o_row = take(groups > 0 ? (size_t)(2 * tokens * hq) * d * sizeof(float) : 0);
   s.ml_row = take((size_t)(2 * tokens * hq) * sizeof(float2));
   s.parts_of = take((size_t)s.slots * sizeof(int2));
@@ -1021,7 +1035,7 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   a.sk_p = k_p, a.sk_n = x->k_stride_slot, a.sk_h = k_h, a.sv_p = v_p, a.sv_n = x->v_stride_slot, a.sv_h = v_h, a.sw_p = w_p, a.sw_h = w_h;
   a.batch = (int)x->batch, a.tokens = (int)x->tokens, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
   a.n_groups = (int)x->groups;
-  a.hkv = (int)x->hkv, a.group = (int)g, a.dense = x->cu_q == nullptr && g <= SH_TILE;
+  a.hkv = (int)x->hkv, a.group = (int)g, a.dense = x->cu_q == nullptr && g <= SH_UNIT;
   a.by_group = pg_divisor((unsigned)g);
   a.shared_slots = (int)s.shared_slots;
   a.parts = sh_workgroups(x->hkv);
@@ -1048,7 +1062,7 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   const int64_t join = sp_ceil_div(x->tokens * x->hq * sets, SM_THREADS / (x->d / 4));
   SP_REQUIRE(join + (int64_t)grid * SH_WAVES <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens,
              (long long)x->hq);
-  a.apart = sh_apart(x->tokens, x->groups, g);
+  a.apart = sh_apart(x->tokens, x->groups, g, x->weights != nullptr);
   if (a.apart) {
     CkArgs c = {};
     c.q = a.q, c.k = a.k, c.v = a.v, c.table = a.table, c.lens = a.shared, c.cu = a.cu, c.groups = a.groups, c.o_row = a.o_row, c.ml_row = a.ml_row;
