@@ -863,8 +863,7 @@ __device__ __forceinline__ void sh_join(const ShArgs& a) {
 // Weights of the own keys that fell to wave's part w / hkv of kv head w % hkv (single tokens):
 //   weight[j] += sum over the group's heads of 2^(logit - m) / l.
 __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
-  __shared__ float2 ml_s[PD_MAX_GROUP];  // of a head: m, 1 / l
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, hq = a.hkv * a.group, kvh = w % a.hkv, part = w / a.hkv;
+  const int t = threadIdx.x, lane = t & 63, hq = a.hkv * a.group, kvh = w % a.hkv, part = w / a.hkv;
   const int4 cut = a.cuts[part];
   const int room = a.width << a.shift;
   for (int b = pg_max(cut.x, 0); b < a.batch && b <= cut.z; ++b) {
@@ -873,33 +872,48 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
     const int lo = r.first_own / SH_KEYS, keys = pg_min(len, room);
     const int begin = b == cut.x ? cut.y : 0, end = b == cut.z ? cut.w : PG_MAX_KEYS / SH_KEYS;
     if (keys <= r.first_own || begin >= end) continue;
-    __syncthreads();  // (the rows before are done with)
-    for (int h = wave; h < a.group; h += SM_THREADS / SP_WAVE) {  // a lane a part
+    // Maxima and sums of the group's heads, by every wave for itself: lane 16 q + h takes every fourth part of head h from q on.
+    float top = CK_NO_MAX, inv = 0.f;
+    {
+      const int h = pg_min(lane & 15, a.group - 1);
       const ShRow own = sh_own_row(a, r, r.start + 1, b, b, h), group = sh_group_row(a, r, b, h);
       const int2 own_parts = sh_own_parts(a, r, b, own), group_parts = sh_group_parts(a, r, group);
-      float top = CK_NO_MAX, sum = 0.f;
+      float sum = 0.f;
       auto add = [&](int in_tile, int2 held, bool of_group) {
         const int count = held.y - held.x + 1;
-        for (int i0 = 0; i0 < count; i0 += SP_WAVE) {
-          float2 ml = make_float2(CK_NO_MAX, 0.f);
-          if (i0 + lane < count)
-            ml = count > 1 ? (of_group ? a.ml_part : a.ml_stream)[sh_slab(a, held, i0 + lane, kvh, in_tile, of_group ? SH_ROWS : 16)]
-                           : a.ml_row[(of_group ? 0 : (int64_t)a.tokens * hq) + (int64_t)b * hq + kvh * a.group + h];
-          const float to = fmaxf(top, sp_wave_max(ml.x));
-          sum = sum * __builtin_amdgcn_exp2f(top - to) + sp_wave_sum(i0 + lane < count ? ml.y * __builtin_amdgcn_exp2f(ml.x - to) : 0.f);
+        for (int i0 = lane >> 4; i0 < count; i0 += 16) {
+          float2 ml[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            ml[u] = count > 1 ? (of_group ? a.ml_part : a.ml_stream)[sh_slab(a, held, pg_min(i0 + 4 * u, count - 1), kvh, in_tile, of_group ? SH_ROWS : 16)]
+                              : a.ml_row[(of_group ? 0 : (int64_t)a.tokens * hq) + (int64_t)b * hq + kvh * a.group + h];
+          float to = top;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) to = fmaxf(to, ml[u].x);
+          sum *= __builtin_amdgcn_exp2f(top - to);
           top = to;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sum += i0 + 4 * u < count ? ml[u].y * __builtin_amdgcn_exp2f(ml[u].x - top) : 0.f;
         }
       };
       add(group.in_tile, group_parts, true);
       add(own.in_tile, own_parts, false);
-      if (lane == 0) ml_s[h] = make_float2(top, sum == 0.f ? 0.f : 1.0f / sum);
+#pragma unroll
+      for (int by = 16; by < SP_WAVE; by <<= 1) {
+        const float top1 = __shfl_xor(top, by, SP_WAVE), sum1 = __shfl_xor(sum, by, SP_WAVE), to = fmaxf(top, top1);
+        sum = sum * __builtin_amdgcn_exp2f(top - to) + sum1 * __builtin_amdgcn_exp2f(top1 - to);
+        top = to;
+      }
+      inv = sum == 0.f ? 0.f : 1.0f / sum;
     }
-    __syncthreads();
     const int first = (lo + begin) * SH_KEYS, last = (int)pg_min((int)(lo + end < keys / SH_KEYS + 1 ? (lo + end) * SH_KEYS : keys), keys);
-    for (int key = first + 4 * t; key < last; key += 4 * SM_THREADS) {
-      const int id = a.table[b * a.table_stride + (key >> a.shift)], in = key & ((1 << a.shift) - 1);
-      if ((unsigned)id >= (unsigned)a.num_pages) continue;
-      const float* const from = a.logits + (((int64_t)id * a.hkv + kvh) * a.group << a.shift) + in;
+    // (all lanes go through the loop together: they hold the heads' maxima and sums for each other)
+    for (int at = first; at < last; at += 4 * SM_THREADS) {
+      const int key = at + 4 * t, in = key & ((1 << a.shift) - 1), page = pg_min(key >> a.shift, a.width - 1);
+      int id = a.table[b * a.table_stride + page];
+      const bool there = key < last && (unsigned)id < (unsigned)a.num_pages;
+      id = there ? id : 0;
+      const float* const from = a.logits + ((((int64_t)id * a.hkv + kvh) * a.group) << a.shift) + in;
       ds_floatx4 sum = {0, 0, 0, 0};
       for (int h0 = 0; h0 < a.group; h0 += 4) {
         ds_floatx4 s[4];
@@ -908,11 +922,13 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           if (h0 + u < a.group) {
-            const float2 ml = ml_s[h0 + u];
+            const float m = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), h0 + u));
+            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inv), h0 + u));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[u][j] - ml.x) * ml.y;
+            for (int j = 0; j < 4; ++j) sum[j] += __builtin_amdgcn_exp2f(s[u][j] - m) * f;
           }
       }
+      if (!there) continue;
       float* const to = a.weights + id * a.sw_p + kvh * a.sw_h + in;
       if (a.weights_by_four && key >= r.first_own && key + 4 < len && key + 4 <= last) {
         *reinterpret_cast<ds_floatx4*>(to) += sum;
