@@ -1,19 +1,25 @@
 // Eviction from a paged cache by accumulated attention weight (sp_paged_evict_bf16): of every kv head of a request the first keys, the last ones and
 // the `budget` heaviest of those between stay, moved to the front of the request's pages in the order they stood in.
 //
-// The heaviest are those above the budget-th largest weight T and as many of those equal to it as there is room for, lowest place first.  T is
-// found by its bits from above, 11, 10 and 10 of the weight's pattern (finite floats without a sign are ordered as their patterns are), a
-// histogram each.  Moving is a gather in place: a kept key comes from its place or further back, so rows are moved front to
-// back in tiles that are read before they are written, by one workgroup, and what other rows still need is never overwritten.
-// Rows are cut across instead: 64 channels of K or V are a workgroup's.  HBM-bound: kept rows once in and out, weights once in.
+// The heaviest are those above the budget-th largest weight T and as many of those equal to it as there is room for, lowest place first.  Finite
+// floats without a sign are ordered as their patterns are: a histogram of the patterns' upper 11 bits says which of its bins T lies in; the keys of that
+// bin and of those above it are listed in order, some hundredths more than stay; and two histograms of 10 bits over the list find T and what of it goes.
+// So the weights are read twice, by as many workgroups as a kv head's keys are shared out to, and the list by one.  Moving is a gather in place: a kept key
+// comes from its place or further back, so rows are moved front to back in tiles that are read before they are written, by one workgroup, and what other rows
+// still need is never overwritten.  Rows are cut across instead, into as many slices as fill the card.
+// Moving is HBM-bound where there are many kv heads in all, kept rows once in and out; one request's is latency: chains of three loads, a tile after the other.
 #include "sp_common.h"
 #include "sp_paged_plan.h"
 
 #define EV_THREADS 1024
 #define EV_WAVES (EV_THREADS / SP_WAVE)
 #define EV_MAX_SEQS 4096
+#define EV_BINS 2048        // of the first histogram: bits 20 .. 30 of a weight's pattern
+#define EV_RUN 16           // places of a thread, which lie in one page
+#define EV_MAX_SHARES 16    // workgroups that share a kv head's keys
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
+typedef float ev_floatx4 __attribute__((ext_vector_type(4)));
 
 struct EvArgs {
   sp_bf16 *k, *v;
@@ -21,8 +27,12 @@ struct EvArgs {
   const int32_t *table, *lens, *first;
   int32_t* new_lens;
   int64_t table_stride, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;
-  int batch, hkv, d, width, num_pages, shift, budget, recent;
-  int32_t* list;  // [request][kv head][budget]: places of the heaviest, behind the first keys
+  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slice;
+  // By place in the pages, [num_pages][kv head][page]: entry i of a request's list stands at the place of its i-th key behind the first ones.  First
+  // pattern and place of what is listed, then where a kept key comes from, page << shift + place in it.
+  uint64_t* list;
+  uint32_t* hists;  // [request][kv head][share][EV_BINS]
+  int32_t* counts;  // [request][kv head][share]: entries of the list
 };
 
 // What becomes of a request: keys first .. first + mid - 1 may go, `keep` of them stay (keep == mid: nothing moves).
@@ -45,144 +55,312 @@ __device__ __forceinline__ bool ev_has_pages(const EvArgs& a, int b, const EvReq
       missing |= (unsigned)a.table[b * a.table_stride + i] >= (unsigned)a.num_pages;
   return __syncthreads_or(missing) == 0;
 }
-
-__global__ __launch_bounds__(EV_THREADS) void sp_evict_select_kernel(const EvArgs a) {
-  __shared__ int hist[2048];
-  __shared__ int wave_s[2][EV_WAVES];
-  __shared__ int found_s[2];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int b = blockIdx.x / a.hkv, kvh = blockIdx.x % a.hkv;
-  const EvRequest r = ev_request(a, b);
-  const bool goes = r.keep < r.mid && ev_has_pages(a, b, r);
-  if (kvh == 0 && t == 0) a.new_lens[b] = goes ? r.len - r.mid + r.keep : r.len;
-  if (!goes || r.keep == 0) return;
-  const int32_t* const table = a.table + b * a.table_stride;
-  const float* const w = a.weights + kvh * a.sw_h;
-  auto key_at = [&](int i) {  // pattern of the weight at place i behind the first keys
+// A request's kv head, one of a.batch * a.hkv.
+struct EvPair {
+  const EvArgs& a;
+  const int32_t* table;
+  int kvh;
+  EvRequest r;
+  __device__ __forceinline__ int64_t place(int j) const {  // of key j in the pages: of a kv head, of all of them where there are a.hkv side by side
+    return ((int64_t)table[j >> a.shift] << a.shift) + (j & ((1 << a.shift) - 1));
+  }
+  __device__ __forceinline__ uint64_t* entry(int i) const {
     const int j = r.first + i;
-    return sp_sort_key(w[(int64_t)table[j >> a.shift] * a.sw_p + (j & ((1 << a.shift) - 1))]);
-  };
-  uint32_t top = 0;     // bits of T that are known
-  int left = r.keep;    // the left-th largest of those that share them is T
-  int shift = 20;
-  for (int pass = 0; pass < 3; ++pass) {
-    const int bits = pass == 0 ? 11 : 10;
-    for (int i = t; i < 1 << bits; i += EV_THREADS) hist[i] = 0;
-    __syncthreads();
-    for (int i = t; i < r.mid; i += EV_THREADS) {
-      const uint32_t key = key_at(i);
-      if (pass == 0 || key >> (shift + bits) == top) atomicAdd(&hist[(key >> shift) & ((1 << bits) - 1)], 1);
+    return a.list + ((((int64_t)table[j >> a.shift] * a.hkv + kvh) << a.shift) + (j & ((1 << a.shift) - 1)));
+  }
+  // Patterns of keys j .. j + EV_RUN - 1 (j a multiple of EV_RUN); those outside lo .. hi - 1 are left as they are.
+  __device__ __forceinline__ void load(int j, int lo, int hi, uint32_t (&key)[EV_RUN]) const {
+    if (j + EV_RUN <= lo || j >= hi) return;
+    const float* const w = a.weights + (int64_t)table[j >> a.shift] * a.sw_p + kvh * a.sw_h + (j & ((1 << a.shift) - 1));
+    float x[EV_RUN];
+    if (a.by_four) {
+#pragma unroll
+      for (int e = 0; e < EV_RUN; e += 4) {
+        const ev_floatx4 y = *reinterpret_cast<const ev_floatx4*>(w + e);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[e + u] = y[u];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e) x[e] = w[e];
     }
-    __syncthreads();
-    // bins from above, two a thread in the first pass
-    const int each = pass == 0 ? 2 : 1, bins = 1 << bits;
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e)
+      if (j + e >= lo && j + e < hi) key[e] = sp_sort_key(x[e]);
+  }
+  // keys of a share, from .. to
+  __device__ __forceinline__ int share_start(int s) const {
+    const int64_t at = (int64_t)r.mid * s / a.shares;
+    return r.first + (int)at;
+  }
+};
+
+// bins of a histogram in LDS from above: the one that holds the left-th largest, and which of it that is
+struct EvBin {
+  int bin, left;
+};
+template <int BINS>
+__device__ __forceinline__ EvBin ev_find(const uint32_t* hist, int left, int* wave_s, int* found_s) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  constexpr int EACH = BINS / EV_THREADS;
+  int mine = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) mine += hist[BINS - 1 - (t * EACH + e)];
+  int at = mine;
+#pragma unroll
+  for (int o = 1; o < SP_WAVE; o <<= 1) {
+    const int y = __shfl_up(at, o, SP_WAVE);
+    if (lane >= o) at += y;
+  }
+  if (lane == SP_WAVE - 1) wave_s[wave] = at;
+  __syncthreads();
+  for (int x = 0; x < wave; ++x) at += wave_s[x];
+  at -= mine;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int bin = BINS - 1 - (t * EACH + e), n = hist[bin];
+    if (at < left && left <= at + n) found_s[0] = bin, found_s[1] = left - at;
+    at += n;
+  }
+  __syncthreads();
+  const EvBin f = {found_s[0], found_s[1]};
+  __syncthreads();
+  return f;
+}
+// the histogram of a share, in LDS
+__device__ __forceinline__ void ev_hist(const EvPair& p, int from, int to, uint32_t* hist) {
+  for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+  __syncthreads();
+  for (int j = (from & -EV_RUN) + (int)threadIdx.x * EV_RUN; j < to; j += EV_THREADS * EV_RUN) {
+    uint32_t key[EV_RUN];
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e) key[e] = ~0u;
+    p.load(j, from, to, key);
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e)
+      if (key[e] != ~0u) atomicAdd(&hist[key[e] >> 20], 1u);
+  }
+  __syncthreads();
+}
+// Lists the keys of a share that lie in bin `bin` or above, in order; -> how many
+__device__ __forceinline__ int ev_gather(const EvPair& p, int from, int to, uint32_t bin, int* wave_s) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  int listed = 0;
+  for (int j0 = from & -EV_RUN; j0 < to; j0 += EV_THREADS * EV_RUN) {
+    const int j = j0 + t * EV_RUN;
+    uint32_t key[EV_RUN];
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e) key[e] = ~0u;
+    p.load(j, from, to, key);
     int mine = 0;
-    for (int e = 0; e < each; ++e) mine += hist[bins - 1 - (t * each + e)];
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e) mine += key[e] != ~0u && key[e] >> 20 >= bin;
     int at = mine;
 #pragma unroll
     for (int o = 1; o < SP_WAVE; o <<= 1) {
       const int y = __shfl_up(at, o, SP_WAVE);
       if (lane >= o) at += y;
     }
-    if (lane == SP_WAVE - 1) wave_s[0][wave] = at;
+    if (lane == SP_WAVE - 1) wave_s[wave] = at;
     __syncthreads();
-    for (int x = 0; x < wave; ++x) at += wave_s[0][x];
-    at -= mine;
-    for (int e = 0; e < each; ++e) {
-      const int bin = bins - 1 - (t * each + e), n = hist[bin];
-      if (at < left && left <= at + n) found_s[0] = bin, found_s[1] = left - at;
-      at += n;
-    }
-    __syncthreads();
-    top = pass == 0 ? (uint32_t)found_s[0] : top << bits | (uint32_t)found_s[0];
-    left = found_s[1];
-    shift -= 10;
-    __syncthreads();
-  }
-  // `left` of those equal to T stay
-  int32_t* const list = a.list + (int64_t)blockIdx.x * a.budget;
-  int kept = 0, equal = 0;  // in front of this chunk
-  for (int i0 = 0; i0 < r.mid; i0 += EV_THREADS) {
-    const int i = i0 + t;
-    const uint32_t key = i < r.mid ? key_at(i) : 0u;
-    const bool over = i < r.mid && key > top, same = i < r.mid && key == top;
-    const uint64_t overs = __ballot(over), sames = __ballot(same), below = (1ull << lane) - 1ull;
-    if (lane == 0) wave_s[0][wave] = __builtin_popcountll(overs), wave_s[1][wave] = __builtin_popcountll(sames);
-    __syncthreads();
-    int over_at = 0, same_at = equal, overs_all = 0, sames_all = 0;
+    int all = 0;
 #pragma unroll
     for (int x = 0; x < EV_WAVES; ++x) {
-      const int n = wave_s[0][x], m = wave_s[1][x];
-      if (x < wave) over_at += n, same_at += m;
-      overs_all += n, sames_all += m;
+      if (x == wave) at += all;
+      all += wave_s[x];
     }
-    // (those equal to T that stay, in front of the lane)
-    over_at += __builtin_popcountll(overs & below);
-    same_at += __builtin_popcountll(sames & below);
-    const int place = kept + over_at + pg_min(same_at, left) - pg_min(equal, left);
-    if (over || (same && same_at < left)) list[place] = i;
-    kept += overs_all + pg_min(equal + sames_all, left) - pg_min(equal, left);
-    equal += sames_all;
+    at += listed - mine + (from - p.r.first);
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e)
+      if (key[e] != ~0u && key[e] >> 20 >= bin) *p.entry(at++) = (uint64_t)key[e] << 32 | (uint32_t)(j + e);
+    listed += all;
     __syncthreads();
+  }
+  return listed;
+}
+
+__device__ __forceinline__ EvPair ev_pair(const EvArgs& a, int pair) {
+  const int b = pair / a.hkv;
+  return EvPair{a, a.table + b * a.table_stride, pair % a.hkv, ev_request(a, b)};
+}
+
+__global__ __launch_bounds__(EV_THREADS) void sp_evict_hist_kernel(const EvArgs a) {
+  __shared__ uint32_t hist[EV_BINS];
+  const int pair = blockIdx.x / a.shares, share = blockIdx.x % a.shares;
+  const EvPair p = ev_pair(a, pair);
+  if (p.r.keep == p.r.mid || p.r.keep == 0 || !ev_has_pages(a, pair / a.hkv, p.r)) return;
+  ev_hist(p, p.share_start(share), p.share_start(share + 1), hist);
+  for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) a.hists[(int64_t)blockIdx.x * EV_BINS + i] = hist[i];
+}
+// (a kv head's shares find the same bin)
+__device__ __forceinline__ EvBin ev_first_bin(const EvArgs& a, int pair, int keep, uint32_t* hist, int* wave_s, int* found_s) {
+  for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) {
+    uint32_t n = 0;
+    for (int x = 0; x < a.shares; ++x) n += a.hists[((int64_t)pair * a.shares + x) * EV_BINS + i];
+    hist[i] = n;
+  }
+  __syncthreads();
+  return ev_find<EV_BINS>(hist, keep, wave_s, found_s);
+}
+__global__ __launch_bounds__(EV_THREADS) void sp_evict_gather_kernel(const EvArgs a) {
+  __shared__ uint32_t hist[EV_BINS];
+  __shared__ int wave_s[EV_WAVES], found_s[2];
+  const int pair = blockIdx.x / a.shares, share = blockIdx.x % a.shares;
+  const EvPair p = ev_pair(a, pair);
+  if (p.r.keep == p.r.mid || p.r.keep == 0 || !ev_has_pages(a, pair / a.hkv, p.r)) return;
+  const EvBin f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
+  const int n = ev_gather(p, p.share_start(share), p.share_start(share + 1), (uint32_t)f.bin, wave_s);
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
+}
+
+// One workgroup a kv head: T, and the list of what stays.  With one share it forms the histogram and the first list itself.
+__global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArgs a) {
+  __shared__ uint32_t hist[EV_BINS];
+  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, pair = blockIdx.x, b = pair / a.hkv;
+  const EvPair p = ev_pair(a, pair);
+  const bool goes = p.r.keep < p.r.mid && ev_has_pages(a, b, p.r);
+  if (p.kvh == 0 && t == 0) a.new_lens[b] = goes ? p.r.len - p.r.mid + p.r.keep : p.r.len;
+  if (!goes || p.r.keep == 0) return;
+  EvBin f;
+  if (a.shares == 1) {
+    ev_hist(p, p.r.first, p.r.first + p.r.mid, hist);
+    f = ev_find<EV_BINS>(hist, p.r.keep, wave_s, found_s);
+    const int n = ev_gather(p, p.r.first, p.r.first + p.r.mid, (uint32_t)f.bin, wave_s);
+    if (t == 0) count_s[0] = n;
+  } else {
+    f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
+    if (t < a.shares) count_s[t] = a.counts[pair * a.shares + t];
+  }
+  __syncthreads();
+  uint32_t top = (uint32_t)f.bin;  // bits of T that are known
+  int left = f.left;               // the left-th largest of those that share them is T
+  for (int shift = 10; shift >= 0; shift -= 10) {
+    for (int i = t; i < 1024; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
+    for (int s = 0; s < a.shares; ++s) {
+      const int base = p.share_start(s) - p.r.first;
+      for (int i = t; i < count_s[s]; i += EV_THREADS) {
+        const uint32_t key = (uint32_t)(*p.entry(base + i) >> 32);
+        if (key >> (shift + 10) == top) atomicAdd(&hist[(key >> shift) & 1023u], 1u);
+      }
+    }
+    __syncthreads();
+    f = ev_find<1024>(hist, left, wave_s, found_s);
+    top = top << 10 | (uint32_t)f.bin;
+    left = f.left;
+  }
+  // `left` of those equal to T stay.  The list becomes where they come from, in place: an entry is written at or in front of where it was read.
+  int kept = 0, equal = 0;  // in front of this round
+  for (int s = 0; s < a.shares; ++s) {
+    const int base = p.share_start(s) - p.r.first;
+    for (int i0 = 0; i0 < count_s[s]; i0 += EV_THREADS) {
+      const int i = i0 + t;
+      const bool there = i < count_s[s];
+      const uint64_t x = there ? *p.entry(base + i) : 0ull;
+      const uint32_t key = (uint32_t)(x >> 32);
+      const bool over = there && key > top, same = there && key == top;
+      const uint64_t overs = __ballot(over), sames = __ballot(same), below = (1ull << lane) - 1ull;
+      if (lane == 0) wave_s[wave] = __builtin_popcountll(overs), wave_s[EV_WAVES + wave] = __builtin_popcountll(sames);
+      __syncthreads();  // (the round's entries are read)
+      int over_at = 0, same_at = equal, overs_all = 0, sames_all = 0;
+#pragma unroll
+      for (int y = 0; y < EV_WAVES; ++y) {
+        const int n = wave_s[y], m = wave_s[EV_WAVES + y];
+        if (y < wave) over_at += n, same_at += m;
+        overs_all += n, sames_all += m;
+      }
+      over_at += __builtin_popcountll(overs & below);
+      same_at += __builtin_popcountll(sames & below);
+      if (over || (same && same_at < left)) *p.entry(kept + over_at + pg_min(same_at, left) - pg_min(equal, left)) = (uint64_t)p.place((int)(uint32_t)x);
+      kept += overs_all + pg_min(equal + sames_all, left) - pg_min(equal, left);
+      equal += sames_all;
+      __syncthreads();
+    }
   }
 }
 
 #define EV_AHEAD 8  // rows of a thread in flight
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs a) {
-  const int t = threadIdx.x, slices = (a.d + 63) / 64, per = 2 * slices + 1;  // K's, V's, the weights
-  const int pair = blockIdx.x / per, part = blockIdx.x % per, b = pair / a.hkv, kvh = pair % a.hkv;
-  const EvRequest r = ev_request(a, b);
+  // (the slices of a kv head side by side in the same XCD's L2, where the kv heads are a multiple of eight)
+  const int t = threadIdx.x, pairs = a.batch * a.hkv, pair = blockIdx.x % pairs, part = blockIdx.x / pairs;
+  const int lanes = a.slice / 8, slices = (a.d + a.slice - 1) / a.slice, b = pair / a.hkv;
+  const EvPair p = ev_pair(a, pair);
+  const EvRequest& r = p.r;
   if (!(r.keep < r.mid && ev_has_pages(a, b, r))) return;
-  const int32_t* const table = a.table + b * a.table_stride;
-  const int32_t* const list = a.list + (int64_t)pair * a.budget;
   const int rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
-  auto from = [&](int i) { return r.first + (i < r.keep ? list[i] : r.mid + (i - r.keep)); };
-  if (part == per - 1) {
-    float* const w = a.weights + kvh * a.sw_h;
-    auto at = [&](int j) { return (int64_t)table[j >> a.shift] * a.sw_p + (j & in); };
+  // where kept key i goes and comes from
+  auto from = [&](int i, int64_t to) {
+    return i < r.keep ? (int64_t)a.list[((((to >> a.shift) * a.hkv + p.kvh) << a.shift) + (to & in))] : p.place(r.first + r.mid + (i - r.keep));
+  };
+  if (part == 2 * slices) {
+    float* const w = a.weights + p.kvh * a.sw_h;
+    auto at = [&](int64_t x) { return (x >> a.shift) * a.sw_p + (x & in); };
     for (int i0 = 0; i0 < rows; i0 += EV_THREADS * EV_AHEAD) {
       float x[EV_AHEAD];
+      int64_t to[EV_AHEAD];
 #pragma unroll
       for (int u = 0; u < EV_AHEAD; ++u) {
-        const int i = i0 + u * EV_THREADS + t;
-        if (i < rows) x[u] = w[at(from(i))];
+        const int i = pg_min(i0 + u * EV_THREADS + t, rows - 1);
+        to[u] = p.place(r.first + i);
+        x[u] = w[at(from(i, to[u]))];
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tile is read
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < EV_AHEAD; ++u) {
-        const int i = i0 + u * EV_THREADS + t;
-        if (i < rows) w[at(r.first + i)] = x[u];
-      }
+      for (int u = 0; u < EV_AHEAD; ++u)
+        if (i0 + u * EV_THREADS + t < rows) w[at(to[u])] = x[u];
     }
     return;
   }
   const bool is_v = part >= slices;
-  const int c = (part % slices) * 64 + (t & 7) * 8;
+  const int c = (part % slices) * a.slice + t % lanes * 8, row = t / lanes, per = EV_THREADS / lanes;
   const int64_t page_at = is_v ? a.sv_p : a.sk_p, slot_at = is_v ? a.sv_n : a.sk_n;
-  sp_bf16* const x = (is_v ? a.v + kvh * a.sv_h : a.k + kvh * a.sk_h) + c;
-  auto at = [&](int j) { return x + (int64_t)table[j >> a.shift] * page_at + (int64_t)(j & in) * slot_at; };
-  constexpr int ROWS = EV_THREADS / 8;
-  for (int i0 = 0; i0 < rows; i0 += ROWS * EV_AHEAD) {
+  sp_bf16* const x = (is_v ? a.v + p.kvh * a.sv_h : a.k + p.kvh * a.sk_h) + c;
+  auto at = [&](int64_t y) { return x + (y >> a.shift) * page_at + (y & in) * slot_at; };
+  const bool mine = c < a.d;
+  for (int i0 = 0; i0 < rows; i0 += per * EV_AHEAD) {
     ev_u32x4 y[EV_AHEAD];
+    int64_t to[EV_AHEAD];
 #pragma unroll
     for (int u = 0; u < EV_AHEAD; ++u) {
-      const int i = i0 + u * ROWS + (t >> 3);
-      if (i < rows && c < a.d) y[u] = *reinterpret_cast<const ev_u32x4*>(at(from(i)));
+      const int i = pg_min(i0 + u * per + row, rows - 1);
+      to[u] = p.place(r.first + i);
+      const int64_t come = from(i, to[u]);
+      if (mine) y[u] = *reinterpret_cast<const ev_u32x4*>(at(come));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tile is read
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < EV_AHEAD; ++u) {
-      const int i = i0 + u * ROWS + (t >> 3);
-      if (i < rows && c < a.d) *reinterpret_cast<ev_u32x4*>(at(r.first + i)) = y[u];
-    }
+    for (int u = 0; u < EV_AHEAD; ++u)
+      if (i0 + u * per + row < rows && mine) *reinterpret_cast<ev_u32x4*>(at(to[u])) = y[u];
   }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
-extern "C" size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int64_t budget) {
-  return batch <= 0 || hkv <= 0 || budget <= 0 ? 0 : (size_t)batch * hkv * (size_t)budget * sizeof(int32_t);
+// Workgroups that share a kv head's keys: as many as fill the card, of some 8192 keys at least by what the table has room for.  One launch of one workgroup each
+// instead of three: us, one / 16 shares, a kv head's 2000 keys of 8 12 / 18, 8000 of 64 17 / 25, 131072 of 8 84 / 26.
+static int ev_shares(int64_t pairs, int64_t room) {
+  const int64_t by_keys = room / 8192, by_card = 256 / pairs;
+  const int64_t n = by_keys < by_card ? by_keys : by_card;
+  return n < 1 ? 1 : n > EV_MAX_SHARES ? EV_MAX_SHARES : (int)n;
+}
+struct EvSizes {
+  size_t list, hists, counts, bytes;
+};
+static EvSizes ev_sizes(int64_t pairs, int64_t hkv, int64_t pool_keys, int shares) {
+  EvSizes s;
+  s.list = 0;
+  s.hists = (size_t)(hkv * pool_keys) * sizeof(uint64_t);
+  s.counts = s.hists + (shares > 1 ? (size_t)(pairs * shares) * EV_BINS * sizeof(uint32_t) : 0);
+  s.bytes = s.counts + (shares > 1 ? ((size_t)(pairs * shares) * sizeof(int32_t) + 15) / 16 * 16 : 0);
+  return s;
+}
+extern "C" size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int64_t num_pages, int64_t page_size, int64_t table_width) {
+  if (batch <= 0 || hkv <= 0 || num_pages <= 0 || page_size <= 0 || table_width <= 0 || num_pages > 0x7fffffffll || page_size > 1024 || table_width > PG_MAX_KEYS)
+    return 0;
+  const int64_t pairs = (int64_t)batch * hkv;
+  return ev_sizes(pairs, hkv, num_pages * page_size, ev_shares(pairs, table_width * page_size)).bytes;
 }
 
 extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
@@ -197,7 +375,11 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   while (shift <= 10 && x->page_size != 1ll << shift) ++shift;
   SP_REQUIRE(shift <= 10, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
   SP_REQUIRE(x->batch <= EV_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %lld (at most %d)", who, (long long)x->batch, EV_MAX_SEQS);
-  const int64_t pairs = x->batch * x->hkv, per = 2 * ((x->d + 63) / 64) + 1;
+  const int64_t pairs = x->batch * x->hkv;
+  // 128 bytes of a row, or fewer where that leaves most of the card idle
+  int slice = 64;
+  while (slice > 16 && pairs * 2 * ((x->d + slice - 1) / slice) < 256) slice /= 2;
+  const int64_t per = 2 * ((x->d + slice - 1) / slice) + 1;
   SP_REQUIRE(x->hkv <= 65536 && x->num_pages <= 0x7fffffffll && x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS &&
                  pairs * per <= 0x7fffffffll,
              SP_ERR_UNSUPPORTED, "%s: hkv=%lld num_pages=%lld table_width=%lld too large", who, (long long)x->hkv, (long long)x->num_pages,
@@ -208,10 +390,9 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   SP_REQUIRE(x->new_lens != x->seq_lens && x->new_lens != x->first, SP_ERR_INVALID_ARGUMENT, "%s: an output is an input", who);
   SP_REQUIRE(((uintptr_t)x->k_pages | (uintptr_t)x->v_pages) % 16 == 0 && (k_p | k_h | x->k_stride_slot | v_p | v_h | x->v_stride_slot) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
-  // (a table cannot hold more keys than its width, so no list is longer)
-  const int64_t budget = x->budget < x->table_width << shift ? x->budget : x->table_width << shift;
-  const size_t need = sp_paged_evict_workspace_bytes((int)x->batch, (int)x->hkv, budget);
-  SP_REQUIRE(need == 0 || (x->workspace != nullptr && x->workspace_bytes >= need && (uintptr_t)x->workspace % 16 == 0), SP_ERR_WORKSPACE,
+  const int shares = ev_shares(pairs, x->table_width << shift);
+  const EvSizes sizes = ev_sizes(pairs, x->hkv, x->num_pages << shift, shares);
+  SP_REQUIRE(x->workspace != nullptr && x->workspace_bytes >= sizes.bytes && (uintptr_t)x->workspace % 16 == 0, SP_ERR_WORKSPACE,
              "%s: workspace missing, too small or misaligned", who);
   EvArgs a = {};
   a.k = (sp_bf16*)x->k_pages, a.v = (sp_bf16*)x->v_pages, a.weights = x->weights;
@@ -219,10 +400,18 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   a.sk_p = k_p, a.sk_n = x->k_stride_slot, a.sk_h = k_h, a.sv_p = v_p, a.sv_n = x->v_stride_slot, a.sv_h = v_h;
   a.sw_p = pg_used_stride(x->w_stride_page, x->num_pages), a.sw_h = pg_used_stride(x->w_stride_h, x->hkv);
   a.batch = (int)x->batch, a.hkv = (int)x->hkv, a.d = (int)x->d, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
-  a.budget = (int)budget, a.recent = (int)(x->recent < PG_MAX_KEYS ? x->recent : PG_MAX_KEYS);
-  a.list = (int32_t*)x->workspace;
-  hipLaunchKernelGGL(sp_evict_select_kernel, dim3((unsigned)pairs), dim3(EV_THREADS), 0, (hipStream_t)x->stream, a);
-  hipLaunchKernelGGL(sp_evict_move_kernel, dim3((unsigned)(pairs * per)), dim3(EV_THREADS), 0, (hipStream_t)x->stream, a);
+  a.budget = (int)(x->budget < PG_MAX_KEYS ? x->budget : PG_MAX_KEYS), a.recent = (int)(x->recent < PG_MAX_KEYS ? x->recent : PG_MAX_KEYS);
+  a.shares = shares, a.slice = slice;
+  a.by_four = (uintptr_t)x->weights % 16 == 0 && (a.sw_p | a.sw_h) % 4 == 0;
+  char* const ws = (char*)x->workspace;
+  a.list = (uint64_t*)(ws + sizes.list), a.hists = (uint32_t*)(ws + sizes.hists), a.counts = (int32_t*)(ws + sizes.counts);
+  const hipStream_t stream = (hipStream_t)x->stream;
+  if (shares > 1) {
+    hipLaunchKernelGGL(sp_evict_hist_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), 0, stream, a);
+    hipLaunchKernelGGL(sp_evict_gather_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), 0, stream, a);
+  }
+  hipLaunchKernelGGL(sp_evict_choose_kernel, dim3((unsigned)pairs), dim3(EV_THREADS), 0, stream, a);
+  hipLaunchKernelGGL(sp_evict_move_kernel, dim3((unsigned)(pairs * per)), dim3(EV_THREADS), 0, stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }

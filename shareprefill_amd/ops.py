@@ -841,7 +841,8 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     length may go back to the stack.  Keys are moved as they are, rotated for the positions they had: the next token's position is not the new length.
     A request with a key behind the first ones that has no page stays as it is.  Only pages of nothing but first keys may be shared.
 
-    At most 4096 requests; head_dim a multiple of 8.  Scratch memory, from torch's allocator, for the call: 4 B Hkv budget bytes."""
+    At most 4096 requests; head_dim a multiple of 8.  Scratch memory, from torch's allocator, for the call: 8 bytes a key and kv head
+    of the pools, and up to 2 MB."""
     lib = _lib.load()
     if k_pages.dim() != 4 or not k_pages.is_cuda:
         raise ValueError(f"k_pages must be [num_pages, Hkv, page_size, D] on the GPU, got {tuple(k_pages.shape)} on {k_pages.device}")
@@ -857,7 +858,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
         raise ValueError(f"budget {budget} and recent {recent} must not be negative")
     stream = _stream_handle(dev)
     new_lens = torch.empty(batch, dtype=torch.int32, device=dev)
-    need = lib.sp_paged_evict_workspace_bytes(batch, hkv, min(budget, block_table.size(1) * page_size))
+    need = lib.sp_paged_evict_workspace_bytes(batch, hkv, pages, page_size, block_table.size(1))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
     w_p, w_h, _ = weights.stride()
     st = lib.sp_paged_evict_bf16(_lib.EVICT_ARGS.pack(
