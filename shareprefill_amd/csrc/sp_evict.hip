@@ -15,7 +15,8 @@
 #define EV_WAVES (EV_THREADS / SP_WAVE)
 #define EV_MAX_SEQS 4096
 #define EV_BINS 2048        // of the first histogram: bits 20 .. 30 of a weight's pattern
-#define EV_RUN 16           // places of a thread, which lie in one page
+#define EV_RUN 16           // keys of a thread, which lie in one page
+#define EV_CHUNK (EV_THREADS * EV_RUN)
 #define EV_MAX_SHARES 16    // workgroups that share a kv head's keys
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
@@ -29,7 +30,7 @@ struct EvArgs {
   int64_t table_stride, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;
   int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slice;
   // By place in the pages, [num_pages][kv head][page]: entry i of a request's list stands at the place of its i-th key behind the first ones.  First
-  // pattern and place of what is listed, then where a kept key comes from, page << shift + place in it.
+  // pattern << 32 | place of what is listed, then the place that a kept key comes from; a place is page << shift + place in it.
   uint64_t* list;
   uint32_t* hists;  // [request][kv head][share][EV_BINS]
   int32_t* counts;  // [request][kv head][share]: entries of the list
@@ -55,6 +56,8 @@ __device__ __forceinline__ bool ev_has_pages(const EvArgs& a, int b, const EvReq
       missing |= (unsigned)a.table[b * a.table_stride + i] >= (unsigned)a.num_pages;
   return __syncthreads_or(missing) == 0;
 }
+// A kv head whose keys a workgroup's registers hold is done by the choosing launch alone.
+__device__ __forceinline__ bool ev_in_registers(const EvRequest& r) { return ((r.first + r.mid + EV_RUN - 1) & -EV_RUN) - (r.first & -EV_RUN) <= EV_CHUNK; }
 // A request's kv head, one of a.batch * a.hkv.
 struct EvPair {
   const EvArgs& a;
@@ -68,9 +71,9 @@ struct EvPair {
     const int j = r.first + i;
     return a.list + ((((int64_t)table[j >> a.shift] * a.hkv + kvh) << a.shift) + (j & ((1 << a.shift) - 1)));
   }
-  // Patterns of keys j .. j + EV_RUN - 1 (j a multiple of EV_RUN); those outside lo .. hi - 1 are left as they are.
-  __device__ __forceinline__ void load(int j, int lo, int hi, uint32_t (&key)[EV_RUN]) const {
-    if (j + EV_RUN <= lo || j >= hi) return;
+  // Patterns of keys j .. j + EV_RUN - 1 (j a multiple of EV_RUN); those outside lo .. hi - 1 are left as they are.  -> place of key j
+  __device__ __forceinline__ uint32_t load(int j, int lo, int hi, uint32_t (&key)[EV_RUN]) const {
+    if (j + EV_RUN <= lo || j >= hi) return 0u;
     const float* const w = a.weights + (int64_t)table[j >> a.shift] * a.sw_p + kvh * a.sw_h + (j & ((1 << a.shift) - 1));
     float x[EV_RUN];
     if (a.by_four) {
@@ -87,6 +90,7 @@ struct EvPair {
 #pragma unroll
     for (int e = 0; e < EV_RUN; ++e)
       if (j + e >= lo && j + e < hi) key[e] = sp_sort_key(x[e]);
+    return (uint32_t)place(j);
   }
   // keys of a share, from .. to
   __device__ __forceinline__ int share_start(int s) const {
@@ -142,37 +146,45 @@ __device__ __forceinline__ void ev_hist(const EvPair& p, int from, int to, uint3
   }
   __syncthreads();
 }
-// Lists the keys of a share that lie in bin `bin` or above, in order; -> how many
-__device__ __forceinline__ int ev_gather(const EvPair& p, int from, int to, uint32_t bin, int* wave_s) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// sums of the threads in front, and over all of them (two barriers)
+__device__ __forceinline__ int ev_scan(int mine, int* wave_s, int* all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int at = mine;
+#pragma unroll
+  for (int o = 1; o < SP_WAVE; o <<= 1) {
+    const int y = __shfl_up(at, o, SP_WAVE);
+    if (lane >= o) at += y;
+  }
+  if (lane == SP_WAVE - 1) wave_s[wave] = at;
+  __syncthreads();
+  *all = 0;
+#pragma unroll
+  for (int x = 0; x < EV_WAVES; ++x) {
+    if (x == wave) at += *all;
+    *all += wave_s[x];
+  }
+  __syncthreads();
+  return at - mine;
+}
+// Lists the keys of a share that lie in bin `bin` or above, in order; -> how many.  stage: EV_CHUNK entries of LDS, so that threads side by side write them.
+__device__ __forceinline__ int ev_gather(const EvPair& p, int from, int to, uint32_t bin, int* wave_s, uint64_t* stage) {
   int listed = 0;
-  for (int j0 = from & -EV_RUN; j0 < to; j0 += EV_THREADS * EV_RUN) {
-    const int j = j0 + t * EV_RUN;
+  for (int j0 = from & -EV_RUN; j0 < to; j0 += EV_CHUNK) {
+    const int j = j0 + (int)threadIdx.x * EV_RUN;
     uint32_t key[EV_RUN];
 #pragma unroll
     for (int e = 0; e < EV_RUN; ++e) key[e] = ~0u;
-    p.load(j, from, to, key);
-    int mine = 0;
+    const uint32_t place = p.load(j, from, to, key);
+    int mine = 0, all;
 #pragma unroll
     for (int e = 0; e < EV_RUN; ++e) mine += key[e] != ~0u && key[e] >> 20 >= bin;
-    int at = mine;
-#pragma unroll
-    for (int o = 1; o < SP_WAVE; o <<= 1) {
-      const int y = __shfl_up(at, o, SP_WAVE);
-      if (lane >= o) at += y;
-    }
-    if (lane == SP_WAVE - 1) wave_s[wave] = at;
-    __syncthreads();
-    int all = 0;
-#pragma unroll
-    for (int x = 0; x < EV_WAVES; ++x) {
-      if (x == wave) at += all;
-      all += wave_s[x];
-    }
-    at += listed - mine + (from - p.r.first);
+    int at = ev_scan(mine, wave_s, &all);
 #pragma unroll
     for (int e = 0; e < EV_RUN; ++e)
-      if (key[e] != ~0u && key[e] >> 20 >= bin) *p.entry(at++) = (uint64_t)key[e] << 32 | (uint32_t)(j + e);
+      if (key[e] != ~0u && key[e] >> 20 >= bin) stage[at++] = (uint64_t)key[e] << 32 | (place + e);
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < all; i += EV_THREADS) *p.entry(from - p.r.first + listed + i) = stage[i];
     listed += all;
     __syncthreads();
   }
@@ -188,7 +200,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_hist_kernel(const EvArgs 
   __shared__ uint32_t hist[EV_BINS];
   const int pair = blockIdx.x / a.shares, share = blockIdx.x % a.shares;
   const EvPair p = ev_pair(a, pair);
-  if (p.r.keep == p.r.mid || p.r.keep == 0 || !ev_has_pages(a, pair / a.hkv, p.r)) return;
+  if (p.r.keep == p.r.mid || p.r.keep == 0 || ev_in_registers(p.r) || !ev_has_pages(a, pair / a.hkv, p.r)) return;
   ev_hist(p, p.share_start(share), p.share_start(share + 1), hist);
   for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) a.hists[(int64_t)blockIdx.x * EV_BINS + i] = hist[i];
 }
@@ -196,43 +208,110 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_hist_kernel(const EvArgs 
 __device__ __forceinline__ EvBin ev_first_bin(const EvArgs& a, int pair, int keep, uint32_t* hist, int* wave_s, int* found_s) {
   for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) {
     uint32_t n = 0;
-    for (int x = 0; x < a.shares; ++x) n += a.hists[((int64_t)pair * a.shares + x) * EV_BINS + i];
+#pragma unroll
+    for (int x = 0; x < EV_MAX_SHARES; ++x)
+      if (x < a.shares) n += a.hists[((int64_t)pair * a.shares + x) * EV_BINS + i];
     hist[i] = n;
   }
   __syncthreads();
   return ev_find<EV_BINS>(hist, keep, wave_s, found_s);
 }
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_gather_kernel(const EvArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint64_t stage[];
   __shared__ uint32_t hist[EV_BINS];
   __shared__ int wave_s[EV_WAVES], found_s[2];
   const int pair = blockIdx.x / a.shares, share = blockIdx.x % a.shares;
   const EvPair p = ev_pair(a, pair);
-  if (p.r.keep == p.r.mid || p.r.keep == 0 || !ev_has_pages(a, pair / a.hkv, p.r)) return;
+  if (p.r.keep == p.r.mid || p.r.keep == 0 || ev_in_registers(p.r) || !ev_has_pages(a, pair / a.hkv, p.r)) return;
   const EvBin f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
-  const int n = ev_gather(p, p.share_start(share), p.share_start(share + 1), (uint32_t)f.bin, wave_s);
+  const int n = ev_gather(p, p.share_start(share), p.share_start(share + 1), (uint32_t)f.bin, wave_s, stage);
   if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
 }
 
-// One workgroup a kv head: T, and the list of what stays.  With one share it forms the histogram and the first list itself.
+// One workgroup a kv head: T, and the list of what stays.  Up to EV_CHUNK keys, a kv head's own or those that are listed, stay in registers for all of it.
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint64_t stage[];
   __shared__ uint32_t hist[EV_BINS];
-  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES];
+  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES], start_s[EV_MAX_SHARES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, pair = blockIdx.x, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   const bool goes = p.r.keep < p.r.mid && ev_has_pages(a, b, p.r);
   if (p.kvh == 0 && t == 0) a.new_lens[b] = goes ? p.r.len - p.r.mid + p.r.keep : p.r.len;
   if (!goes || p.r.keep == 0) return;
   EvBin f;
-  if (a.shares == 1) {
-    ev_hist(p, p.r.first, p.r.first + p.r.mid, hist);
-    f = ev_find<EV_BINS>(hist, p.r.keep, wave_s, found_s);
-    const int n = ev_gather(p, p.r.first, p.r.first + p.r.mid, (uint32_t)f.bin, wave_s);
-    if (t == 0) count_s[0] = n;
-  } else {
-    f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
-    if (t < a.shares) count_s[t] = a.counts[pair * a.shares + t];
+  const bool whole = ev_in_registers(p.r);
+  int listed = 0;  // (uniform)
+  if (!whole) {
+    if (a.shares == 1) {
+      ev_hist(p, p.r.first, p.r.first + p.r.mid, hist);
+      f = ev_find<EV_BINS>(hist, p.r.keep, wave_s, found_s);
+      const int n = ev_gather(p, p.r.first, p.r.first + p.r.mid, (uint32_t)f.bin, wave_s, stage);
+      if (t == 0) count_s[0] = n;
+    } else {
+      if (t < a.shares) count_s[t] = a.counts[pair * a.shares + t];
+    }
+    __syncthreads();
+    for (int s = 0; s < a.shares; ++s) {
+      if (t == 0) start_s[s] = listed;
+      listed += count_s[s];
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  if (whole || listed <= EV_CHUNK) {
+    uint32_t key[EV_RUN], place[EV_RUN];
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e) key[e] = ~0u, place[e] = 0u;
+    if (whole) {
+      const int j = (p.r.first & -EV_RUN) + t * EV_RUN;
+      const uint32_t first = p.load(j, p.r.first, p.r.first + p.r.mid, key);
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e) place[e] = first + e;
+    } else {
+      // (threads side by side read entries side by side, then each its own out of LDS)
+#pragma unroll 4
+      for (int i = t; i < listed; i += EV_THREADS) {
+        int s = 0;
+#pragma unroll
+        for (int step = EV_MAX_SHARES / 2; step > 0; step /= 2)
+          if (s + step < a.shares && start_s[s + step] <= i) s += step;
+        stage[i] = *p.entry(p.share_start(s) - p.r.first + i - start_s[s]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e)
+        if (t * EV_RUN + e < listed) key[e] = (uint32_t)(stage[t * EV_RUN + e] >> 32), place[e] = (uint32_t)stage[t * EV_RUN + e];
+    }
+    uint32_t top = 0;
+    int left = p.r.keep;
+    for (int shift = 20; shift >= 0; shift -= 10) {
+      for (int i = t; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e)
+        if (key[e] != ~0u && (shift == 20 || key[e] >> (shift + 10) == top)) atomicAdd(&hist[(key[e] >> shift) & (shift == 20 ? 2047u : 1023u)], 1u);
+      __syncthreads();
+      f = ev_find<EV_BINS>(hist, left, wave_s, found_s);
+      top = top << 10 | (uint32_t)f.bin;
+      left = f.left;
+    }
+    // `left` of those equal to T stay, the first
+    int overs = 0, sames = 0, all;
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e) overs += key[e] != ~0u && key[e] > top, sames += key[e] == top;
+    const int in_front = ev_scan(overs | sames << 16, wave_s, &all);  // (neither reaches 2^16: EV_CHUNK is 2^14)
+    int over_at = in_front & 0xffff, same_at = in_front >> 16;
+#pragma unroll
+    for (int e = 0; e < EV_RUN; ++e) {
+      const bool over = key[e] != ~0u && key[e] > top, same = key[e] == top;
+      if (over || (same && same_at < left)) stage[over_at + pg_min(same_at, left)] = place[e];
+      over_at += over, same_at += same;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = t; i < p.r.keep; i += EV_THREADS) *p.entry(i) = stage[i];
+    return;
+  }
+  if (a.shares > 1) f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
   uint32_t top = (uint32_t)f.bin;  // bits of T that are known
   int left = f.left;               // the left-th largest of those that share them is T
   for (int shift = 10; shift >= 0; shift -= 10) {
@@ -272,7 +351,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
       }
       over_at += __builtin_popcountll(overs & below);
       same_at += __builtin_popcountll(sames & below);
-      if (over || (same && same_at < left)) *p.entry(kept + over_at + pg_min(same_at, left) - pg_min(equal, left)) = (uint64_t)p.place((int)(uint32_t)x);
+      if (over || (same && same_at < left)) *p.entry(kept + over_at + pg_min(same_at, left) - pg_min(equal, left)) = (uint32_t)x;
       kept += overs_all + pg_min(equal + sames_all, left) - pg_min(equal, left);
       equal += sames_all;
       __syncthreads();
@@ -381,7 +460,7 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   while (slice > 16 && pairs * 2 * ((x->d + slice - 1) / slice) < 256) slice /= 2;
   const int64_t per = 2 * ((x->d + slice - 1) / slice) + 1;
   SP_REQUIRE(x->hkv <= 65536 && x->num_pages <= 0x7fffffffll && x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS &&
-                 pairs * per <= 0x7fffffffll,
+                 x->num_pages << shift <= 0xffffffffll && pairs * per <= 0x7fffffffll,
              SP_ERR_UNSUPPORTED, "%s: hkv=%lld num_pages=%lld table_width=%lld too large", who, (long long)x->hkv, (long long)x->num_pages,
              (long long)x->table_width);
   const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);
@@ -406,11 +485,21 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   char* const ws = (char*)x->workspace;
   a.list = (uint64_t*)(ws + sizes.list), a.hists = (uint32_t*)(ws + sizes.hists), a.counts = (int32_t*)(ws + sizes.counts);
   const hipStream_t stream = (hipStream_t)x->stream;
+  constexpr int lds = EV_CHUNK * (int)sizeof(uint64_t);
+  static bool attr_set[64] = {false};  // per device, once (idempotent)
+  int dev = 0;
+  SP_HIP(hipGetDevice(&dev));
+  SP_REQUIRE(dev >= 0 && dev < 64, SP_ERR_UNSUPPORTED, "%s: device index %d", who, dev);
+  if (!attr_set[dev]) {
+    for (const void* f : {(const void*)sp_evict_gather_kernel, (const void*)sp_evict_choose_kernel})
+      SP_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    attr_set[dev] = true;
+  }
   if (shares > 1) {
     hipLaunchKernelGGL(sp_evict_hist_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), 0, stream, a);
-    hipLaunchKernelGGL(sp_evict_gather_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), 0, stream, a);
+    hipLaunchKernelGGL(sp_evict_gather_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), lds, stream, a);
   }
-  hipLaunchKernelGGL(sp_evict_choose_kernel, dim3((unsigned)pairs), dim3(EV_THREADS), 0, stream, a);
+  hipLaunchKernelGGL(sp_evict_choose_kernel, dim3((unsigned)pairs), dim3(EV_THREADS), lds, stream, a);
   hipLaunchKernelGGL(sp_evict_move_kernel, dim3((unsigned)(pairs * per)), dim3(EV_THREADS), 0, stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;

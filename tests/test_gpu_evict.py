@@ -75,6 +75,42 @@ def test_lengths_around_the_tiles(gpu_device):
     _run(gpu_device, [9000], 8500, 20, hkv=1, d=16, page=64)  # (nearly all stay: tiles that overlap what they come from)
 
 
+def _fast(dev, n, budget, recent, first, weight, width=0, page=64, seed=0):
+    """One long request of one kv head, against torch's stable sort."""
+    from shareprefill_amd import ops
+
+    gen = torch.Generator().manual_seed(seed)
+    pages = -(-n // page)
+    table = torch.randperm(pages, generator=gen).to(torch.int32)
+    wide = torch.full((1, max(width, pages)), -1, dtype=torch.int32)
+    wide[0, :pages] = table
+    k, v = (torch.randn(pages, 1, page, 8, generator=gen).to(torch.bfloat16) for _ in range(2))
+    w = weight((pages, 1, page))
+    live = [x.to(dev) for x in (k, v, w)]
+    got = ops.paged_evict(*live, wide.to(dev), _ints(dev, [n]), budget, recent, first=_ints(dev, [first]))
+    place = lambda x: x[table.long(), 0].reshape(-1, *x.shape[3:])  # in the order of the keys
+    mid = n - first - recent
+    stay = torch.sort(place(w)[first:first + mid], descending=True, stable=True).indices[:budget].sort().values
+    src = torch.cat((torch.arange(first), stay + first, torch.arange(first + mid, n)))
+    assert got.tolist() == [src.numel()]
+    for x, y in zip(live, (k, v, w)):
+        want = place(y).clone()
+        want[:src.numel()] = place(y)[src]
+        assert torch.equal(place(x.cpu()), want)
+
+
+@pytest.mark.parametrize("n", [16384, 16385, 16400, 40000, 140000])
+@pytest.mark.parametrize("first", [0, 5, 64])
+def test_long_requests(gpu_device, n, first):
+    """Keys of a kv head that one workgroup's registers hold, and more, which are listed by one workgroup or by several."""
+    gen = torch.Generator().manual_seed(n + first)
+    spread = lambda shape: torch.exp(2 * torch.randn(shape, generator=gen))
+    for weight in (spread, lambda shape: torch.full(shape, 0.25), lambda shape: 1.0 + torch.randint(0, 900, shape, generator=gen).float() * 2.0 ** -22):
+        _fast(gpu_device, n, n // 16, 33, first, weight)
+        _fast(gpu_device, n, n - first - 50, 33, first, weight)
+    _fast(gpu_device, n, 700, 0, first, spread, width=4000)  # a table that has room for much more
+
+
 def test_equal_weights_keep_the_first(gpu_device):
     _run(gpu_device, [3000, 700], 300, 20, weight=lambda shape: torch.zeros(shape))
     gen = torch.Generator().manual_seed(3)
