@@ -6,10 +6,8 @@
 // What bounds it: HBM for few rows (2 D bytes a key and kv head), else the matrix cores, two products of rows x keys x D.
 //
 // A wave has 32 keys, its K operands in registers, those of its next 32 keys on their way; the rows' queries lie in LDS, up to 256 of them, and serve all
-// keys of the workgroup's part.  Every key's sum is formed by one wave in one order: results do not depend on timing.  Requests' blocks of 128
+// keys of the workgroup's part; two row tiles are on their way at a time, one's products under the other's exponentials.  Every key's sum is formed by one wave in one order: results do not depend on timing.  Requests' blocks of 128
 // keys lie on a line per kv head that is cut into equal parts, a workgroup each.
-#include <utility>
-
 #include "sp_ring.h"
 #include "sp_paged_plan.h"
 
@@ -18,8 +16,10 @@
 #define KW_KEYS 32                       // of a wave
 #define KW_BLOCK (KW_WAVES * KW_KEYS)
 #define KW_TILES 16                      // row tiles of 16 in LDS
+#define KW_SLACK 7.f
 #define KW_ROWS (16 * KW_TILES)
 #define KW_OVERHEAD 2                    // blocks' worth of a request beside its blocks: its queries, the rows' meeting
+#define KW_SHARE 2                       // units of a part at least
 #define KW_MAX_SEQS 1024
 #define KW_PLACES 512                    // workgroups: two a CU
 
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     total += sums_s[w];
   }
   at -= mine;
-  const int64_t parts = pg_parts(total, a.parts, 1 + KW_OVERHEAD);
+  const int64_t parts = pg_parts(total, a.parts, KW_SHARE);
   const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
   if (t == 0) found_s[0] = a.batch;
   __syncthreads();
@@ -171,10 +171,11 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
       }
     };
     for (int row0 = 0; row0 < rows; row0 += KW_ROWS) {
-      const int here = pg_min(rows - row0, KW_ROWS), tiles = (here + 15) / 16;
+      const int here = pg_min(rows - row0, KW_ROWS), tiles = (here + 31) / 32 * 2;  // (an even number)
       Keys cur, nxt;
       fetch(begin, cur);
       __syncthreads();  // (the rows before are done with)
+#pragma unroll 4
       for (int i = t; i < tiles * 16 * CHUNKS; i += KW_THREADS) {
         const int r = i / CHUNKS, c = i % CHUNKS, row = row0 + pg_min(r, here - 1), token = (int)pg_div((unsigned)row, a.by_group);
         *reinterpret_cast<dc_u32x4*>(q_lds + r * (D * 2) + ((c ^ ds_swz_k<D>(r & 15)) << 4)) =
@@ -201,56 +202,84 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
         const int key0 = (from + block) * KW_BLOCK + wave * KW_KEYS;
         const bool edge = key0 + KW_KEYS - 1 > pos0 + (int)pg_div((unsigned)row0, a.by_group) || cur.there != 3u;  // some row does not see some key
         float acc[2][4] = {{0.f}};
-        auto tile = [&](int i) {
-          ds_floatx4 sc[2];
-          dc_bf16x8 qb[KS];
+        // the logits of row tiles i and i + 1, in octaves: keys 16 h + 4 gr + j of row lq
+        auto pair = [&](int i, ds_floatx4 (&sc)[2][2]) {
+          dc_bf16x8 qb[2][KS];
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-            qb[ks] = *reinterpret_cast<const dc_bf16x8*>(q_lds + (16 * i + lq) * (D * 2) + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            sc[h] = (ds_floatx4){0, 0, 0, 0};
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-              sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, cur.r[h][ks]), qb[ks], sc[h], 0, 0, 0);
-          }
+              qb[u][ks] = *reinterpret_cast<const dc_bf16x8*>(q_lds + (16 * (i + u) + lq) * (D * 2) + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4));
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sc[h][j] *= a.scale_log2;
-          if (edge) {
-            const int pos = pos0 + (int)pg_div((unsigned)pg_min(row0 + 16 * i + lq, rows - 1), a.by_group);
+            for (int h = 0; h < 2; ++h) sc[u][h] = (ds_floatx4){0, 0, 0, 0};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                sc[u][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, cur.r[h][ks]), qb[u][ks], sc[u][h], 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                sc[h][j] = key0 + 16 * h + 4 * gr + j <= pos && ((cur.there >> h) & 1u) ? sc[h][j] : -INFINITY;
+              for (int j = 0; j < 4; ++j) sc[u][h][j] *= a.scale_log2;
+          if (edge) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int pos = pos0 + (int)pg_div((unsigned)pg_min(row0 + 16 * (i + u) + lq, rows - 1), a.by_group);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  sc[u][h][j] = key0 + 16 * h + 4 * gr + j <= pos && ((cur.there >> h) & 1u) ? sc[u][h][j] : -INFINITY;
+            }
           }
-          return std::pair<ds_floatx4, ds_floatx4>(sc[0], sc[1]);
         };
         if constexpr (!SUMS) {
 #pragma unroll
-          for (int i = 0; i < KW_TILES; ++i) {
+          for (int i = 0; i < KW_TILES; i += 2) {
             if (i < tiles) {
-              const auto [s0, s1] = tile(i);
-              float mx = fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])), fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3])));
-              mx = fmaxf(mx, m[i]);
-              const float base = mx == -INFINITY ? 0.f : mx;
-              float add = 0.f;
+              ds_floatx4 sc[2][2];
+              pair(i, sc);
+              float mx[2];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) add += __builtin_amdgcn_exp2f(s0[j] - base) + __builtin_amdgcn_exp2f(s1[j] - base);
-              l[i] = l[i] * __builtin_amdgcn_exp2f(m[i] - base) + add;
-              m[i] = mx;
+              for (int u = 0; u < 2; ++u)
+                mx[u] = fmaxf(fmaxf(fmaxf(sc[u][0][0], sc[u][0][1]), fmaxf(sc[u][0][2], sc[u][0][3])),
+                              fmaxf(fmaxf(sc[u][1][0], sc[u][1][1]), fmaxf(sc[u][1][2], sc[u][1][3])));
+              // (a lane's maximum moves when a logit passes it by seven octaves, which few do: sums of 2^7 are as exact)
+              if (__ballot(mx[0] > m[i] + KW_SLACK || mx[1] > m[i + 1] + KW_SLACK) != 0ull) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                  const float to = fmaxf(m[i + u], mx[u]);
+                  l[i + u] *= to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i + u] - to);
+                  m[i + u] = to;
+                }
+              }
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const float base = m[i + u] == -INFINITY ? 0.f : m[i + u];
+                float add = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) add += __builtin_amdgcn_exp2f(sc[u][0][j] - base) + __builtin_amdgcn_exp2f(sc[u][1][j] - base);
+                l[i + u] += add;
+              }
             }
           }
         } else {
-          for (int i = 0; i < tiles; ++i) {
-            const auto [s0, s1] = tile(i);
-            const float2 ml = ml_s[16 * i + lq];
+          for (int i = 0; i < tiles; i += 2) {
+            ds_floatx4 sc[2][2];
+            pair(i, sc);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              acc[0][j] += __builtin_amdgcn_exp2f(s0[j] - ml.x) * ml.y;
-              acc[1][j] += __builtin_amdgcn_exp2f(s1[j] - ml.x) * ml.y;
+            for (int u = 0; u < 2; ++u) {
+              const float2 ml = ml_s[16 * (i + u) + lq];
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[h][j] += __builtin_amdgcn_exp2f(sc[u][h][j] - ml.x) * ml.y;
             }
           }
 #pragma unroll
@@ -281,8 +310,8 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
               const float m1 = __shfl_xor(m[i], by, SP_WAVE), l1 = __shfl_xor(l[i], by, SP_WAVE), top = fmaxf(m[i], m1), base = top == -INFINITY ? 0.f : top;
               l[i] = l[i] * __builtin_amdgcn_exp2f(m[i] - base) + l1 * __builtin_amdgcn_exp2f(m1 - base);
               m[i] = top;
-          }
-          if (gr == 0) ml_s[wave * KW_ROWS + 16 * i + lq] = make_float2(m[i], l[i]);
+            }
+            if (gr == 0) ml_s[wave * KW_ROWS + 16 * i + lq] = make_float2(m[i], l[i]);
           }
         }
         __syncthreads();
