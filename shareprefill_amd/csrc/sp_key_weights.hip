@@ -151,21 +151,31 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     const int first_key = SUMS && a.first != nullptr ? pg_max(0, pg_min(a.first[b], keys)) : 0;
     const int pos0 = len - q_len;  // of the first row
     const sp_bf16* const kh = a.k + kvh * a.sk_h;
-    const int32_t* const table = a.table + (int64_t)b * a.table_stride;
-    // K operands of the wave's 32 keys of a block, and which of them there are
-    struct Keys {
-      dc_u32x4 r[2][KS];
-      uint32_t there;  // 16-key halves with a page (bits)
+    // (scalar loads: nothing writes the table during the launch)
+    const auto table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.table + (int64_t)__builtin_amdgcn_readfirstlane(b) * a.table_stride);
+    struct Ids {
+      int id[2];  // pages of the wave's 16-key halves of a block, -1: none
     };
-    auto fetch = [&](int block, Keys& x) {
-      x.there = 0;
+    struct Keys {  // K operands of the wave's 32 keys of a block
+      dc_u32x4 r[2][KS];
+      Ids ids;
+    };
+    auto entries = [&](int block) {
+      Ids x;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int key = (from + block) * KW_BLOCK + wave * KW_KEYS + 16 * i, page = key >> a.shift;
-        const int id = page < a.width ? table[page] : -1;
-        const bool ok = (unsigned)id < (unsigned)a.num_pages;
-        if (ok) x.there |= 1u << i;
-        const sp_bf16* src = kh + (int64_t)(ok ? id : 0) * a.sk_p + (int64_t)((key & ((1 << a.shift) - 1)) + lq) * a.sk_n + 8 * gr;
+        const int page = ((from + block) * KW_BLOCK + wave * KW_KEYS + 16 * i) >> a.shift;
+        const int id = table[pg_min(page, a.width - 1)];
+        x.id[i] = page < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
+      }
+      return x;
+    };
+    auto fetch = [&](int block, Ids ids, Keys& x) {
+      x.ids = ids;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = (from + block) * KW_BLOCK + wave * KW_KEYS + 16 * i;
+        const sp_bf16* src = kh + (int64_t)pg_max(ids.id[i], 0) * a.sk_p + (int64_t)((key & ((1 << a.shift) - 1)) + lq) * a.sk_n + 8 * gr;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) x.r[i][ks] = *reinterpret_cast<const dc_u32x4*>(src + 32 * ks);
       }
@@ -173,7 +183,8 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     for (int row0 = 0; row0 < rows; row0 += KW_ROWS) {
       const int here = pg_min(rows - row0, KW_ROWS), tiles = (here + 31) / 32 * 2;  // (an even number)
       Keys cur, nxt;
-      fetch(begin, cur);
+      fetch(begin, entries(begin), cur);
+      Ids ids = entries(pg_min(begin + 1, end - 1));
       __syncthreads();  // (the rows before are done with)
 #pragma unroll 4
       for (int i = t; i < tiles * 16 * CHUNKS; i += KW_THREADS) {
@@ -198,9 +209,11 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
         for (int i = 0; i < KW_TILES; ++i) m[i] = -INFINITY, l[i] = 0.f;
       }
       for (int block = begin; block < end; ++block) {
-        if (block + 1 < end) fetch(block + 1, nxt);
+        // (the last block asks for itself again: were it not to ask, the wait for this block's keys would be one for the next one's too)
+        fetch(pg_min(block + 1, end - 1), ids, nxt);
+        ids = entries(pg_min(block + 2, end - 1));
         const int key0 = (from + block) * KW_BLOCK + wave * KW_KEYS;
-        const bool edge = key0 + KW_KEYS - 1 > pos0 + (int)pg_div((unsigned)row0, a.by_group) || cur.there != 3u;  // some row does not see some key
+        const bool edge = key0 + KW_KEYS - 1 > pos0 + (int)pg_div((unsigned)row0, a.by_group) || (cur.ids.id[0] | cur.ids.id[1]) < 0;  // some row does not see some key
         float acc[2][4] = {{0.f}};
         // the logits of row tiles i and i + 1, in octaves: keys 16 h + 4 gr + j of row lq
         auto pair = [&](int i, ds_floatx4 (&sc)[2][2]) {
@@ -235,7 +248,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
               for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  sc[u][h][j] = key0 + 16 * h + 4 * gr + j <= pos && ((cur.there >> h) & 1u) ? sc[u][h][j] : -INFINITY;
+                  sc[u][h][j] = key0 + 16 * h + 4 * gr + j <= pos && cur.ids.id[h] >= 0 ? sc[u][h][j] : -INFINITY;
             }
           }
         };
@@ -293,8 +306,9 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
           for (int i = 1; i < 8; ++i) sum = lq == i ? acc[i >> 2][i & 3] : sum;
           const int key = key0 + 16 * (lq >> 2) + 4 * gr + (lq & 3);
-          if (lq < 8 && ((cur.there >> (lq >> 2)) & 1u) && key >= first_key && key < keys) {
-            float* const to = a.weights + (int64_t)table[key >> a.shift] * a.sw_p + kvh * a.sw_h + (key & ((1 << a.shift) - 1));
+          const int id = lq < 4 ? cur.ids.id[0] : cur.ids.id[1];
+          if (lq < 8 && id >= 0 && key >= first_key && key < keys) {
+            float* const to = a.weights + (int64_t)id * a.sw_p + kvh * a.sw_h + (key & ((1 << a.shift) - 1));
             const bool adds = row0 > 0 || (a.accumulate && key < pos0);
             *to = (adds ? *to : 0.f) + sum;
           }
