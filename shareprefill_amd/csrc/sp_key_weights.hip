@@ -19,7 +19,8 @@
 #define KW_SLACK 7.f
 #define KW_ROWS (16 * KW_TILES)
 #define KW_OVERHEAD 2                    // blocks' worth of a request beside its blocks: its queries, the rows' meeting
-#define KW_SHARE 2                       // units of a part at least
+#define KW_UNITS(rows) (((rows) + 31) / 32 + 1)  // of a block: pairs of row tiles, and its keys
+#define KW_SHARE 4                       // units of a part at least
 #define KW_MAX_SEQS 1024
 #define KW_PLACES 512                    // workgroups: two a CU
 
@@ -72,12 +73,13 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     *from = SUMS && a.first != nullptr ? pg_max(0, pg_min(a.first[b], keys)) / KW_BLOCK : 0;
     return start_s[b + 1] > start_s[b] && keys > 0 ? (keys + KW_BLOCK - 1) / KW_BLOCK - *from : 0;
   };
+  auto units_of = [&](int b, int n) { return n > 0 ? (int64_t)(n + KW_OVERHEAD) * KW_UNITS((start_s[b + 1] - start_s[b]) * g) : 0; };
   const int per = (a.batch + KW_THREADS - 1) / KW_THREADS, b0 = t * per, b1 = pg_min(b0 + per, a.batch);
   int64_t mine = 0;
   int from;
   for (int b = b0; b < b1; ++b) {
     const int n = blocks(b, &from);
-    mine += n > 0 ? n + KW_OVERHEAD : 0;
+    mine += units_of(b, n);
   }
   int64_t at = mine;
 #pragma unroll
@@ -98,15 +100,19 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
   const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
   if (t == 0) found_s[0] = a.batch;
   __syncthreads();
-  // units of a request: KW_OVERHEAD, then its blocks
-  auto steps = [&](int64_t start, int n, int64_t c0, int64_t c1, int* begin, int* end) {
-    *begin = c0 <= start + KW_OVERHEAD ? 0 : (int)pg_max(0, (int)(c0 - start < n + KW_OVERHEAD ? c0 - start - KW_OVERHEAD : n));
-    *end = c1 >= start + n + KW_OVERHEAD ? n : c1 <= start + KW_OVERHEAD ? 0 : (int)(c1 - start - KW_OVERHEAD);
+  // of a request whose blocks have `each` units: KW_OVERHEAD blocks' worth, then its blocks; a part may fall between two cuts of one block and hold none
+  auto steps = [&](int64_t start, int n, int each, int64_t c0, int64_t c1, int* begin, int* end) {
+    auto block = [&](int64_t c) {
+      const int64_t off = c - start, at = off <= 0 ? 0 : off < PG_SHORT_LINE ? (int64_t)((unsigned)off / (unsigned)each) : off / each;
+      return (int)(at <= KW_OVERHEAD ? 0 : at - KW_OVERHEAD < n ? at - KW_OVERHEAD : n);
+    };
+    *begin = block(c0);
+    *end = block(c1);
   };
-  // the part in which a request's first block lies
-  auto first_part = [&](int64_t start) {
-    const int64_t x = start + KW_OVERHEAD;  // (its unit)
-    int64_t p = (int64_t)((double)x / (double)total * (double)parts);
+  // the part that a request's first block ends in
+  auto first_part = [&](int64_t start, int each) {
+    const int64_t x = start + (int64_t)(KW_OVERHEAD + 1) * each - 1;  // (its last unit)
+    int64_t p = total < PG_SHORT_LINE ? (int64_t)((uint64_t)(unsigned)x * (unsigned)parts / (unsigned)total) : (int64_t)((double)x / (double)total * (double)parts);
     if (p >= parts) p = parts - 1;
     while (p > 0 && pg_cut(total, parts, p) > x) --p;
     while (p + 1 < parts && pg_cut(total, parts, p + 1) <= x) ++p;
@@ -117,12 +123,12 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     int64_t u = at;
     for (int b = b0; b < b1; ++b) {
       const int n = blocks(b, &from);
-      const int64_t units = n > 0 ? n + KW_OVERHEAD : 0;
+      const int64_t units = units_of(b, n);
       if (tell) {
         int count = 0;
         if (n > 0) {
           const int64_t last = u + units - 1;
-          const int p0 = first_part(u);
+          const int p0 = first_part(u, KW_UNITS((start_s[b + 1] - start_s[b]) * g));
           int p1 = p0;
           while (p1 + 1 < parts && pg_cut(total, parts, p1 + 1) <= last) ++p1;
           count = p1 - p0 + 1;
@@ -141,13 +147,20 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
   for (; b < a.batch && unit < cut1; ++b) {
     const int n = blocks(b, &from);
     if (n == 0) continue;
+    const int start = start_s[b], q_len = start_s[b + 1] - start, len = len_s[b], rows = q_len * g, keys = pg_min(len, room), each = KW_UNITS(rows);
     const int64_t start_unit = unit;
-    unit += n + KW_OVERHEAD;
+    unit += units_of(b, n);
     int begin, end;
-    steps(start_unit, n, cut0, cut1, &begin, &end);
-    if (begin >= end) continue;
-    const int start = start_s[b], q_len = start_s[b + 1] - start, len = len_s[b], rows = q_len * g, keys = pg_min(len, room);
-    const int rel = SUMS ? 0 : part - first_part(start_unit);
+    steps(start_unit, n, each, cut0, cut1, &begin, &end);
+    const int rel = SUMS ? 0 : part - first_part(start_unit, each);
+    if (begin >= end) {
+      if (!SUMS && rel >= 0)  // (a part between the others' that holds nothing)
+        for (int r = t; r < rows; r += KW_THREADS) {
+          const int token = (int)pg_div((unsigned)r, a.by_group);
+          a.part_ml[((int64_t)(start + token) * hq + kvh * g + (r - token * g)) * a.parts + rel] = make_float2(-INFINITY, 0.f);
+        }
+      continue;
+    }
     const int first_key = SUMS && a.first != nullptr ? pg_max(0, pg_min(a.first[b], keys)) : 0;
     const int pos0 = len - q_len;  // of the first row
     const sp_bf16* const kh = a.k + kvh * a.sk_h;
