@@ -8,13 +8,23 @@
     cache.begin_step(active=running)                        # a token of each running request, rows request by request
     cache.release(finished)
 
-A step (begin_step, write, attend) reads no device value on the host, so it can be recorded into a HIP graph and replayed with other lengths;
-release runs between steps.  The reference keeps no cache of its own (its decode step reads a contiguous one, shareprefill_attn.py:146-155).
+Requests that share the start of their prompt are rows of a group (group_sizes): the first row caches it, share() gives its whole pages to the others, and
+attend reads them once for the group.  With key_weights the cache knows what attention every key has received, from each next token (attend) and from a
+prompt's last ones (observe), and evict() keeps the heaviest of a request's keys when it holds too many:
+
+    cache = PagedKVCache(..., group_sizes=[16, 16], key_weights=True)
+    cache.begin_step(prompt_lens, max_new_tokens=8192)      # the common start, to rows 0 and 16
+    ...
+    cache.share(0, 4000), cache.share(1, 2500)              # rows 1 .. 15 and 17 .. 31 begin behind it
+    cache.evict(budget=2048, recent=128, sinks=4)
+
+A step (begin_step, write, attend, observe) reads no device value on the host, so it can be recorded into a HIP graph and replayed with other lengths;
+share, join, evict and release run between steps.  The reference keeps no cache of its own (its decode step reads a contiguous one, shareprefill_attn.py:146-155).
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -25,7 +35,8 @@ class PagedKVCache:
     """Requests are rows 0 .. max_requests - 1 of the block table; one model runs its steps in order on one stream."""
 
     def __init__(self, num_layers: int, num_pages: int, num_kv_heads: int, head_dim: int, max_requests: int, max_tokens: int,
-                 page_size: int = 64, device="cuda"):
+                 page_size: int = 64, device="cuda", group_sizes: Optional[Sequence[int]] = None, key_weights: bool = False):
+        """group_sizes: rows that share prompts' starts, group after group from row 0 on; rows behind them share nothing."""
         if min(num_layers, num_pages, num_kv_heads, head_dim, max_requests, max_tokens) < 1:
             raise ValueError("every size of a PagedKVCache must be at least 1")
         self.page_size, self.num_pages, self.max_requests = page_size, num_pages, max_requests
@@ -40,6 +51,21 @@ class PagedKVCache:
         self.tables: Optional[ops.PageTables] = None
         self._cu_q: Optional[torch.Tensor] = None
         self._seen_lens: Optional[torch.Tensor] = None  # of a step: keys that a request's rows may see
+        sizes = list(group_sizes or [])
+        if any(n < 1 for n in sizes) or sum(sizes) > max_requests:
+            raise ValueError(f"group_sizes {sizes} must be at least 1 each and {max_requests} in all at most")
+        starts = [sum(sizes[:i]) for i in range(len(sizes) + 1)]
+        ints = lambda x, dtype: torch.tensor(x, dtype=dtype, device=dev)
+        self._group_starts = starts
+        self.cu_groups = ints(starts, torch.int32)
+        self.shared_lens = torch.zeros(len(sizes), dtype=torch.int32, device=dev)
+        group_of = [i for i, n in enumerate(sizes) for _ in range(n)]
+        self._group_of = ints(group_of + [len(sizes)] * (max_requests - len(group_of)), torch.int64)  # (none: one past the last)
+        self._holder = ints([starts[i] for i in group_of] + list(range(len(group_of), max_requests)), torch.int64)
+        # what attention every key has received, by its place in the pages (None: not kept), and how many keys evictions have taken from a request
+        self.weights = torch.zeros(num_layers, num_pages, num_kv_heads, page_size, dtype=torch.float32, device=dev) if key_weights else None
+        self.dropped = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self._last = None  # of a step: rows of its requests' last tokens (observe)
 
     def _check_mask(self, mask: torch.Tensor, name: str) -> None:
         if mask.dtype is not torch.bool or tuple(mask.shape) != (self.max_requests,) or mask.device != self.lens.device:
@@ -54,7 +80,8 @@ class PagedKVCache:
 
         max_new_tokens: how many there can be in all, the T of the step's q, k and v; tokens past it, of the last requests, are left out (the
         result's cu_new says what each request brought, and its lens grow by that).  Whether the pages sufficed is in the result's free_left
-        (negative: they did not; tokens without a slot are not cached and seen by nobody)."""
+        (negative: they did not; tokens without a slot are not cached and seen by nobody).  positions count what evictions have dropped: a token's
+        place in its request, not in the cache."""
         singles = new_lens is None
         if active is not None:
             if not singles:
@@ -74,7 +101,15 @@ class PagedKVCache:
             place = t.cu_new[:-1]
             t = t._replace(slots=torch.where(active, t.slots.index_select(0, place), -1), positions=t.positions.index_select(0, place) * new_lens)
             self._seen_lens = t.seq_lens * new_lens
-        self.tables, self._cu_q = t, None if singles else t.cu_new
+        if self.weights is not None:
+            # (places without a token stay at 0)
+            if singles:
+                t = t._replace(positions=t.positions + self.dropped * new_lens)
+            else:
+                token = torch.arange(t.positions.numel(), dtype=torch.int32, device=self.lens.device)
+                row = torch.searchsorted(t.cu_new[1:], token, right=True).clamp_(max=self.max_requests - 1)
+                t = t._replace(positions=t.positions + torch.where(token < t.cu_new[-1:], self.dropped[row], 0))
+        self.tables, self._cu_q, self._last = t, None if singles else t.cu_new, None
         return t
 
     def _pools_of(self, layer: int):
@@ -88,21 +123,116 @@ class PagedKVCache:
 
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, window: Optional[int] = None, sinks: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """q: bf16 [Hq, T, D] view -> bf16 [T, Hq, D]: every new token over what its request has cached up to it (ops.paged_attention)."""
+        """q: bf16 [Hq, T, D] view -> bf16 [T, Hq, D]: every new token over what its request has cached up to it (ops.paged_attention; with groups or
+        key_weights, where there is no window, ops.shared_prefix_attention).  A step of single tokens adds what they attend to to the keys' weights; one
+        with new_lens leaves them to observe, and so does one with a window."""
         pools = self._pools_of(layer)
         if q.dim() == 3 and q.shape[1] != self.tables.slots.numel():
             raise ValueError(f"q has {q.shape[1]} rows, the step {self.tables.slots.numel()}")
+        if window is None and (self.shared_lens.numel() > 0 or self.weights is not None):
+            return ops.shared_prefix_attention(q, *pools, self.block_table, self._seen_lens, self.shared_lens, self.cu_groups, softmax_scale,
+                                               cu_q=self._cu_q, weights=self.weights[layer] if self.weights is not None and self._cu_q is None else None,
+                                               out=out)
         return ops.paged_attention(q, *pools, self.block_table, self._seen_lens, softmax_scale, cu_q=self._cu_q,
                                    window=window, sinks=sinks, out=out)
 
-    def release(self, finished: torch.Tensor) -> None:
-        """Puts the pages of the requests with finished[r] (bool [max_requests]) back on the stack; their rows are empty again.
-        Not for a captured graph."""
-        self._check_mask(finished, "finished")
-        back = finished[:, None] & (self.block_table >= 0)
+    def _shared_of(self) -> torch.Tensor:
+        """int32 [max_requests]: keys that a request's group shares (0: it is in none)."""
+        return torch.cat((self.shared_lens, self.shared_lens.new_zeros(1)))[self._group_of]
+
+    def _check_weights(self) -> torch.Tensor:
+        if self.weights is None:
+            raise RuntimeError("key_weights=True makes a cache that knows its keys' weights")
+        return self.weights
+
+    def observe(self, layer: int, q: torch.Tensor, softmax_scale: float, last: int = 32, accumulate: bool = False) -> None:
+        """Sets the keys' weights of the requests that bring tokens to what the last `last` tokens of each attend to (all of them, where it brings
+        fewer); accumulate: on top of what keys in front of those tokens have (ops.paged_key_weights).  q as for attend, behind write.  Keys that a group
+        shares have none."""
+        weights = self._check_weights()
+        pools = self._pools_of(layer)
+        if last < 1:
+            raise ValueError(f"last must be at least 1, got {last}")
+        if q.dim() != 3 or q.shape[1] != self.tables.slots.numel():
+            raise ValueError(f"q must be [Hq, {self.tables.slots.numel()}, D], got {tuple(q.shape)}")
+        cu = self._cu_q
+        if cu is not None:
+            if self._last is None or self._last[0] != last:
+                count = (cu[1:] - cu[:-1]).clamp(max=last)
+                starts = torch.cat((cu[:1], torch.cumsum(count, 0, dtype=torch.int32)))
+                token = torch.arange(min(self.max_requests * last, q.shape[1]), dtype=torch.int32, device=q.device)
+                row = torch.searchsorted(starts[1:], token, right=True).clamp_(max=self.max_requests - 1)
+                source = (cu[1:][row] - count[row] + token - starts[row]).clamp_(0, max(q.shape[1] - 1, 0))
+                self._last = (last, starts, source)
+            cu, q = self._last[1], q.transpose(0, 1).index_select(0, self._last[2]).transpose(0, 1)
+        ops.paged_key_weights(q, pools[0], self.block_table, self._seen_lens, softmax_scale, weights[layer], cu_q=cu, first=self._shared_of(),
+                              accumulate=accumulate)
+
+    def share(self, group: int, tokens: int) -> None:
+        """The first `tokens` keys of the group's first row, as many as fill whole pages, become those of all its rows: the others, which must be empty,
+        begin behind them.  The first row must have them cached; it may go on as a request of its own, and its end is the end of the sharing (release)."""
+        if not 0 <= group < self.shared_lens.numel():
+            raise ValueError(f"there are {self.shared_lens.numel()} groups, no group {group}")
+        if not 0 <= tokens <= self.block_table.shape[1] * self.page_size:
+            raise ValueError(f"{tokens} tokens are none that a request can have")
+        first, end = self._group_starts[group:group + 2]
+        self.shared_lens[group:group + 1].fill_(tokens // self.page_size * self.page_size)
+        rows = torch.zeros(self.max_requests, dtype=torch.bool, device=self.lens.device)
+        rows[first + 1:end] = True
+        self.join(rows)
+
+    def join(self, rows: torch.Tensor) -> None:
+        """Rows (bool [max_requests], empty ones, as release leaves them) begin behind what their group shares; a group's first row stays as it is."""
+        self._check_mask(rows, "rows")
+        rows = rows & (self._holder != torch.arange(self.max_requests, device=self._holder.device))
+        shared = self._shared_of()
+        place = torch.arange(self.block_table.shape[1], device=self.lens.device)[None, :]
+        named = torch.where(place * self.page_size < shared[:, None], self.block_table[self._holder], -1)
+        self.block_table.copy_(torch.where(rows[:, None], named, self.block_table))
+        self.lens.copy_(torch.where(rows, shared, self.lens))
+
+    def evict(self, budget: int, recent: int, sinks: int = 0, rows: Optional[torch.Tensor] = None) -> None:
+        """Drops keys of requests (rows bool [max_requests]; None: all) that hold more than they may, in every layer and kv head by itself: the first
+        `sinks` and what a group shares stay, the last `recent`, and of the others the `budget` heaviest (ops.paged_evict).  Their pages go back.
+        A window of attend counts places in the cache, which later keys of such a request have nearer to each other than their positions."""
+        weights = self._check_weights()
+        if rows is not None:
+            self._check_mask(rows, "rows")
+        lens = self.lens if rows is None else self.lens * rows
+        first = torch.clamp(self._shared_of(), min=sinks)
+        left = lens
+        for layer in range(self.pools.shape[0]):
+            left = ops.paged_evict(*self.pools[layer].unbind(0), weights[layer], self.block_table, lens, budget, recent, first=first)
+        if rows is not None:
+            left = torch.where(rows, left, self.lens)
+        self.dropped += self.lens - left
+        self.lens.copy_(left)
+        place = torch.arange(self.block_table.shape[1], device=left.device)[None, :]
+        self._give_back(place * self.page_size >= left[:, None])
+
+    def _give_back(self, entries: torch.Tensor) -> None:
+        """Puts the pages of entries of the block table (bool, its shape) back on the stack, those that no other entry names, each once."""
+        back = entries & (self.block_table >= 0)
+        page = torch.where(self.block_table >= 0, self.block_table, self.num_pages).reshape(-1).long()
+        if self.shared_lens.numel() > 0:
+            kept = torch.zeros(self.num_pages + 1, dtype=torch.bool, device=page.device)
+            kept[torch.where(entries.reshape(-1), self.num_pages, page)] = True
+            place = torch.arange(page.numel(), device=page.device)
+            first = torch.full((self.num_pages + 1,), page.numel(), dtype=torch.int64, device=page.device)
+            first.scatter_reduce_(0, torch.where(back.reshape(-1), page, self.num_pages), place, "amin")
+            back &= (~kept[page] & (first[page] == place)).reshape(back.shape)
         count = torch.cumsum(back.reshape(-1), 0, dtype=torch.int32)
         place = torch.where(back.reshape(-1), self.free_count + count - 1, self.num_pages)
         self._stack[place.long()] = self.block_table.reshape(-1)
         self.free_count += count[-1:]
-        self.block_table.masked_fill_(finished[:, None], -1)
+        self.block_table.masked_fill_(entries, -1)
+
+    def release(self, finished: torch.Tensor) -> None:
+        """Puts the pages of the requests with finished[r] (bool [max_requests]) back on the stack, but for those that others share; their rows are empty
+        again.  Where a group's first row finishes its rows share no longer.  Not for a captured graph."""
+        self._check_mask(finished, "finished")
+        self._give_back(finished[:, None].expand_as(self.block_table))
         self.lens.masked_fill_(finished, 0)
+        self.dropped.masked_fill_(finished, 0)
+        if self.shared_lens.numel() > 0:
+            self.shared_lens.masked_fill_(finished[self.cu_groups[:-1].long()], 0)
