@@ -22,7 +22,10 @@
 #define KW_UNITS(rows) (((rows) + 31) / 32 + 1)  // of a block: pairs of row tiles, and its keys
 #define KW_SHARE 4                       // units of a part at least
 #define KW_MAX_SEQS 1024
+#define KW_FEW 16                        // parts that the second walk joins by itself
 #define KW_PLACES 512                    // workgroups: two a CU
+
+typedef const __attribute__((address_space(1))) void* kw_gbl_ptr;
 
 struct KwArgs {
   const sp_bf16 *q, *k;
@@ -30,7 +33,7 @@ struct KwArgs {
   float* weights;
   int64_t table_stride, sq_n, sq_h, sk_p, sk_n, sk_h, sw_p, sw_h;
   int batch, tokens, width, num_pages, shift;
-  int hkv, group, accumulate, parts;
+  int hkv, group, accumulate, parts, few;
   PgDivisor by_group;
   float scale_log2;
   float2* part_ml;   // [token][query head][part]: of the keys that fell to a part, counted from the request's first
@@ -42,6 +45,37 @@ struct KwArgs {
 // Blocks of 128 keys of every request with new tokens, from block `from` on (the walk for the weights leaves out what lies in front of the
 // request's first wanted key).
 
+// (a NaN passes, and makes the lane's sum one: no other logit of the row counts then)
+__device__ static __forceinline__ float kw_max(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
+__device__ static __forceinline__ float kw_max(ds_floatx4 v) { return __builtin_elementwise_maximum(kw_max(v[0], v[1], v[2]), v[3]); }
+
+__device__ static __forceinline__ int64_t kw_lane(int64_t v, int lane) {  // (a lane that all agree on)
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+
+// over the 16 lanes of a row, each in an order of its own
+__device__ static __forceinline__ float kw_row_sum(float v) {
+#define KW_ROTATED(n) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x120 + n, 0xf, 0xf, true))
+  v += KW_ROTATED(8), v += KW_ROTATED(4), v += KW_ROTATED(2), v += KW_ROTATED(1);
+#undef KW_ROTATED
+  return v;
+}
+
+// A row's parts joined where there are KW_FEW at most: maximum and 1 / sum, infinity and 0 of a row that sees no key.
+__device__ static __forceinline__ float2 kw_joined(float top, float sum) { return make_float2(top == -INFINITY ? INFINITY : top, sum == 0.f ? 0.f : 1.0f / sum); }
+__device__ static __forceinline__ float2 kw_join(const float2* parts, int count) {
+  float2 p[KW_FEW];
+#pragma unroll
+  for (int i = 0; i < KW_FEW; ++i) p[i] = i < count ? parts[i] : make_float2(-INFINITY, 0.f);
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < KW_FEW; ++i) top = fmaxf(top, p[i].x);
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int i = 0; i < KW_FEW; ++i) sum += p[i].y * __builtin_amdgcn_exp2f(p[i].x - base);
+  return kw_joined(top, sum);
+}
+
 template <int D, bool SUMS>
 __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwArgs a) {
   constexpr int KS = D / 32, CHUNKS = D / 8;
@@ -50,8 +84,6 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
   float2* const ml_s = reinterpret_cast<float2*>(lds + KW_ROWS * D * 2);  // [KW_WAVES][KW_ROWS]
   int* const start_s = reinterpret_cast<int*>(ml_s + KW_WAVES * KW_ROWS);
   int* const len_s = start_s + a.batch + 1;
-  __shared__ int64_t sums_s[KW_WAVES + 1];
-  __shared__ int found_s[1];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int lq = lane & 15, gr = lane >> 4;
   const int kvh = blockIdx.x % a.hkv, part = blockIdx.x / a.hkv, g = a.group, room = a.width << a.shift;
@@ -74,12 +106,15 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     return start_s[b + 1] > start_s[b] && keys > 0 ? (keys + KW_BLOCK - 1) / KW_BLOCK - *from : 0;
   };
   auto units_of = [&](int b, int n) { return n > 0 ? (int64_t)(n + KW_OVERHEAD) * KW_UNITS((start_s[b + 1] - start_s[b]) * g) : 0; };
-  const int per = (a.batch + KW_THREADS - 1) / KW_THREADS, b0 = t * per, b1 = pg_min(b0 + per, a.batch);
-  int64_t mine = 0;
+  // the line, by every wave for itself: a lane has some requests side by side
+  const int per = (a.batch + SP_WAVE - 1) / SP_WAVE, b0 = lane * per, b1 = pg_min(b0 + per, a.batch);
+  int64_t mine = 0, lead = 0;
   int from;
   for (int b = b0; b < b1; ++b) {
     const int n = blocks(b, &from);
-    mine += units_of(b, n);
+    const int64_t units = units_of(b, n);
+    if (mine == 0 && n > 0) lead = (int64_t)KW_OVERHEAD * KW_UNITS((start_s[b + 1] - start_s[b]) * g);
+    mine += units;
   }
   int64_t at = mine;
 #pragma unroll
@@ -87,19 +122,14 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     const int64_t y = __shfl_up(at, o, SP_WAVE);
     if (lane >= o) at += y;
   }
-  if (lane == SP_WAVE - 1) sums_s[wave] = at;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < KW_WAVES; ++w) {
-    if (w == wave) at += total;
-    total += sums_s[w];
-  }
+  const int64_t total = kw_lane(at, SP_WAVE - 1);
   at -= mine;
-  const int64_t parts = pg_parts(total, a.parts, KW_SHARE);
-  const int64_t cut0 = part < parts ? pg_cut(total, parts, part) : total, cut1 = part < parts ? pg_cut(total, parts, part + 1) : total;
-  if (t == 0) found_s[0] = a.batch;
-  __syncthreads();
+  // what the line's first request has beside its blocks every part has: the parts begin behind it
+  const uint64_t some = __ballot(mine > 0);
+  lead = some != 0ull ? kw_lane(lead, __builtin_ctzll(some)) : 0;
+  const int64_t shared = total - lead, parts = pg_parts(shared, a.parts, KW_SHARE);
+  auto cut = [&](int64_t p) { return lead + pg_cut(shared, parts, p); };
+  const int64_t cut0 = part < parts ? cut(part) : total, cut1 = part < parts ? cut(part + 1) : total;
   // of a request whose blocks have `each` units: KW_OVERHEAD blocks' worth, then its blocks; a part may fall between two cuts of one block and hold none
   auto steps = [&](int64_t start, int n, int each, int64_t c0, int64_t c1, int* begin, int* end) {
     auto block = [&](int64_t c) {
@@ -109,40 +139,35 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     *begin = block(c0);
     *end = block(c1);
   };
-  // the part that a request's first block ends in
-  auto first_part = [&](int64_t start, int each) {
-    const int64_t x = start + (int64_t)(KW_OVERHEAD + 1) * each - 1;  // (its last unit)
-    int64_t p = total < PG_SHORT_LINE ? (int64_t)((uint64_t)(unsigned)x * (unsigned)parts / (unsigned)total) : (int64_t)((double)x / (double)total * (double)parts);
+  // the part that unit x lies in, and the one that a request's first block ends in
+  auto part_of = [&](int64_t x) {
+    int64_t p = (int64_t)((float)(x - lead) * (float)parts * __builtin_amdgcn_rcpf((float)shared));  // within one: parts are KW_PLACES at most
     if (p >= parts) p = parts - 1;
-    while (p > 0 && pg_cut(total, parts, p) > x) --p;
-    while (p + 1 < parts && pg_cut(total, parts, p + 1) <= x) ++p;
+    while (p > 0 && cut(p) > x) --p;
+    while (p + 1 < parts && cut(p + 1) <= x) ++p;
     return (int)p;
   };
-  const bool tell = !SUMS && blockIdx.x == 0;
-  if (tell || (cut0 < cut1 && cut0 >= at && cut0 < at + mine)) {
+  auto first_part = [&](int64_t start, int each) { return part_of(start + (int64_t)(KW_OVERHEAD + 1) * each - 1); };
+  const bool holds = cut0 < cut1 && cut0 >= at && cut0 < at + mine;
+  const bool tell = !SUMS && blockIdx.x == gridDim.x - 1;  // (the one that small calls leave idle)
+  int b = a.batch;
+  int64_t unit = at;
+  if (holds || tell) {
     int64_t u = at;
-    for (int b = b0; b < b1; ++b) {
-      const int n = blocks(b, &from);
-      const int64_t units = units_of(b, n);
-      if (tell) {
-        int count = 0;
-        if (n > 0) {
-          const int64_t last = u + units - 1;
-          const int p0 = first_part(u, KW_UNITS((start_s[b + 1] - start_s[b]) * g));
-          int p1 = p0;
-          while (p1 + 1 < parts && pg_cut(total, parts, p1 + 1) <= last) ++p1;
-          count = p1 - p0 + 1;
-        }
-        a.of_request[b] = make_int2(count, start_s[b]);
-      }
-      if (cut0 >= u && cut0 < u + units) found_s[0] = b, sums_s[KW_WAVES] = u;
+    for (int i = b0; i < b1; ++i) {
+      const int n = blocks(i, &from);
+      const int64_t units = units_of(i, n);
+      if (tell && wave == 0)
+        a.of_request[i] = make_int2(n > 0 ? part_of(u + units - 1) - first_part(u, KW_UNITS((start_s[i + 1] - start_s[i]) * g)) + 1 : 0, start_s[i]);
+      if (holds && cut0 >= u && cut0 < u + units) b = i, unit = u;
       u += units;
     }
   }
   if (tell && t == 0) a.of_request[a.batch] = make_int2(0, start_s[a.batch]);
-  __syncthreads();
-  int b = found_s[0];
-  int64_t unit = b < a.batch ? sums_s[KW_WAVES] : total;
+  const uint64_t holder = __ballot(holds);
+  const int held = holder != 0ull ? __builtin_ctzll(holder) : 0;  // (the lanes' b is the batch where none holds)
+  b = __builtin_amdgcn_readlane(b, held);
+  unit = kw_lane(unit, held);
 
   for (; b < a.batch && unit < cut1; ++b) {
     const int n = blocks(b, &from);
@@ -196,25 +221,28 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     for (int row0 = 0; row0 < rows; row0 += KW_ROWS) {
       const int here = pg_min(rows - row0, KW_ROWS), tiles = (here + 31) / 32 * 2;  // (an even number)
       Keys cur, nxt;
+      __syncthreads();  // (the rows before are done with)
+      for (int i = t; i < tiles * 16 * CHUNKS; i += KW_THREADS) {
+        const int r = i / CHUNKS, row = row0 + pg_min(r, here - 1), token = (int)pg_div((unsigned)row, a.by_group);
+        __builtin_amdgcn_global_load_lds((kw_gbl_ptr)(a.q + (int64_t)(start + token) * a.sq_n + (int64_t)(kvh * g + (row - token * g)) * a.sq_h +
+                                                      8 * ((i % CHUNKS) ^ ds_swz_k<D>(r & 15))),
+                                         (ds_lds_ptr)(q_lds + (i - lane) * 16), 16, 0, 0);
+      }
       fetch(begin, entries(begin), cur);
       Ids ids = entries(pg_min(begin + 1, end - 1));
-      __syncthreads();  // (the rows before are done with)
-#pragma unroll 4
-      for (int i = t; i < tiles * 16 * CHUNKS; i += KW_THREADS) {
-        const int r = i / CHUNKS, c = i % CHUNKS, row = row0 + pg_min(r, here - 1), token = (int)pg_div((unsigned)row, a.by_group);
-        *reinterpret_cast<dc_u32x4*>(q_lds + r * (D * 2) + ((c ^ ds_swz_k<D>(r & 15)) << 4)) =
-            *reinterpret_cast<const dc_u32x4*>(a.q + (int64_t)(start + token) * a.sq_n + (int64_t)(kvh * g + (row - token * g)) * a.sq_h + 8 * c);
-      }
       if constexpr (SUMS) {
+        const int count = a.few ? a.of_request[b].x : 0;
         for (int r = t; r < tiles * 16; r += KW_THREADS) {  // (rows that are none weigh nothing)
           float2 ml = make_float2(INFINITY, 0.f);
           if (r < here) {
             const int row = row0 + r, token = (int)pg_div((unsigned)row, a.by_group);
-            ml = a.row_ml[(int64_t)(start + token) * hq + kvh * g + (row - token * g)];
+            const int64_t at = (int64_t)(start + token) * hq + kvh * g + (row - token * g);
+            ml = a.few ? kw_join(a.part_ml + at * a.parts, count) : a.row_ml[at];
           }
           ml_s[r] = ml;
         }
       }
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the queries
       __syncthreads();
       float m[SUMS ? 1 : KW_TILES], l[SUMS ? 1 : KW_TILES];
       if constexpr (!SUMS) {
@@ -228,7 +256,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
         const int key0 = (from + block) * KW_BLOCK + wave * KW_KEYS;
         const bool edge = key0 + KW_KEYS - 1 > pos0 + (int)pg_div((unsigned)row0, a.by_group) || (cur.ids.id[0] | cur.ids.id[1]) < 0;  // some row does not see some key
         float acc[2][4] = {{0.f}};
-        // the logits of row tiles i and i + 1, in octaves: keys 16 h + 4 gr + j of row lq
+        // the products of row tiles i and i + 1: keys 16 h + 4 gr + j of row lq
         auto pair = [&](int i, ds_floatx4 (&sc)[2][2]) {
           dc_bf16x8 qb[2][KS];
 #pragma unroll
@@ -236,6 +264,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
               qb[u][ks] = *reinterpret_cast<const dc_bf16x8*>(q_lds + (16 * (i + u) + lq) * (D * 2) + (((4 * ks + gr) ^ ds_swz_k<D>(lq)) << 4));
+          __builtin_amdgcn_sched_barrier(0);  // (all on their way at once)
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -247,12 +276,6 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
               for (int h = 0; h < 2; ++h)
                 sc[u][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, cur.r[h][ks]), qb[u][ks], sc[u][h], 0, 0, 0);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) sc[u][h][j] *= a.scale_log2;
           if (edge) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -274,8 +297,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
               float mx[2];
 #pragma unroll
               for (int u = 0; u < 2; ++u)
-                mx[u] = fmaxf(fmaxf(fmaxf(sc[u][0][0], sc[u][0][1]), fmaxf(sc[u][0][2], sc[u][0][3])),
-                              fmaxf(fmaxf(sc[u][1][0], sc[u][1][1]), fmaxf(sc[u][1][2], sc[u][1][3])));
+                mx[u] = a.scale_log2 * kw_max(kw_max(kw_max(sc[u][0]), sc[u][1][0], sc[u][1][1]), sc[u][1][2], sc[u][1][3]);
               // (a lane's maximum moves when a logit passes it by seven octaves, which few do: sums of 2^7 are as exact)
               if (__ballot(mx[0] > m[i] + KW_SLACK || mx[1] > m[i + 1] + KW_SLACK) != 0ull) {
 #pragma unroll
@@ -290,7 +312,8 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
                 const float base = m[i + u] == -INFINITY ? 0.f : m[i + u];
                 float add = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) add += __builtin_amdgcn_exp2f(sc[u][0][j] - base) + __builtin_amdgcn_exp2f(sc[u][1][j] - base);
+                for (int j = 0; j < 4; ++j)
+                  add += __builtin_amdgcn_exp2f(fmaf(sc[u][0][j], a.scale_log2, -base)) + __builtin_amdgcn_exp2f(fmaf(sc[u][1][j], a.scale_log2, -base));
                 l[i + u] += add;
               }
             }
@@ -305,15 +328,14 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[h][j] += __builtin_amdgcn_exp2f(sc[u][h][j] - ml.x) * ml.y;
+                for (int j = 0; j < 4; ++j) acc[h][j] += __builtin_amdgcn_exp2f(fmaf(sc[u][h][j], a.scale_log2, -ml.x)) * ml.y;
             }
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int by = 1; by < 16; by <<= 1) acc[h][j] += __shfl_xor(acc[h][j], by, SP_WAVE);
+              acc[h][j] = kw_row_sum(acc[h][j]);
           // lanes 0 .. 7 of a group have a key each: 16 (lq / 4) + 4 gr + lq % 4
           float sum = acc[0][0];
 #pragma unroll
@@ -332,13 +354,8 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
         for (int i = 0; i < KW_TILES; ++i) {
           if (i < tiles) {
-#pragma unroll
-            for (int by = 16; by < SP_WAVE; by <<= 1) {
-              const float m1 = __shfl_xor(m[i], by, SP_WAVE), l1 = __shfl_xor(l[i], by, SP_WAVE), top = fmaxf(m[i], m1), base = top == -INFINITY ? 0.f : top;
-              l[i] = l[i] * __builtin_amdgcn_exp2f(m[i] - base) + l1 * __builtin_amdgcn_exp2f(m1 - base);
-              m[i] = top;
-            }
-            if (gr == 0) ml_s[wave * KW_ROWS + 16 * i + lq] = make_float2(m[i], l[i]);
+            const float top = ds_quad_max(m[i]), sum = ds_quad_sum(l[i] * __builtin_amdgcn_exp2f(m[i] - (top == -INFINITY ? 0.f : top)));
+            if (gr == 0) ml_s[wave * KW_ROWS + 16 * i + lq] = make_float2(top, sum);
           }
         }
         __syncthreads();
@@ -383,7 +400,7 @@ __global__ __launch_bounds__(KW_THREADS) void sp_key_weights_join_kernel(const K
     sum = sum * __builtin_amdgcn_exp2f(top - base) + sp_wave_sum(ml.y * __builtin_amdgcn_exp2f(ml.x - base));
     top = to;
   }
-  if (lane == 0) a.row_ml[row] = make_float2(top == -INFINITY ? INFINITY : top, sum == 0.f ? 0.f : 1.0f / sum);
+  if (lane == 0) a.row_ml[row] = kw_joined(top, sum);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
@@ -455,6 +472,9 @@ extern "C" int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* x) {
   a.by_group = pg_divisor((unsigned)a.group);
   a.scale_log2 = (float)x->softmax_scale * 1.4426950408889634f;
   a.part_ml = (float2*)(ws + s.part_ml), a.row_ml = (float2*)(ws + s.row_ml), a.of_request = (int2*)(ws + s.of_request);
+  // parts of a request: two ends and what lies between them, of KW_SHARE - 1 units at least (n units make ceil(n / KW_SHARE) parts: three parts of 9)
+  const int64_t blocks = ((x->table_width << shift) + KW_BLOCK - 1) / KW_BLOCK + KW_OVERHEAD;
+  a.few = blocks * KW_UNITS(x->tokens * a.group) / (KW_SHARE - 1) + 2 <= KW_FEW;
   auto lds = [](int d, int batch) { return (size_t)KW_ROWS * d * 2 + KW_WAVES * KW_ROWS * sizeof(float2) + (2 * (size_t)batch + 1) * sizeof(int); };
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
@@ -470,7 +490,7 @@ extern "C" int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* x) {
   const unsigned grid = (unsigned)(a.parts * a.hkv), joins = (unsigned)sp_ceil_div(x->tokens * x->hq, KW_WAVES);
   auto go = [&](auto stats, auto sums) {
     hipLaunchKernelGGL(stats, dim3(grid), dim3(KW_THREADS), lds((int)x->d, a.batch), stream, a);
-    hipLaunchKernelGGL(sp_key_weights_join_kernel, dim3(joins), dim3(KW_THREADS), 0, stream, a);
+    if (!a.few) hipLaunchKernelGGL(sp_key_weights_join_kernel, dim3(joins), dim3(KW_THREADS), 0, stream, a);
     hipLaunchKernelGGL(sums, dim3(grid), dim3(KW_THREADS), lds((int)x->d, a.batch), stream, a);
   };
   x->d == 64 ? go(sp_key_weights_kernel<64, false>, sp_key_weights_kernel<64, true>) : go(sp_key_weights_kernel<128, false>, sp_key_weights_kernel<128, true>);
