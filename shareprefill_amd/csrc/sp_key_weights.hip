@@ -53,6 +53,17 @@ __device__ static __forceinline__ int64_t kw_lane(int64_t v, int lane) {  // (a 
   return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
 }
 
+__device__ static __forceinline__ double kw_inverse(double v) {
+  const double r = __builtin_amdgcn_rcp(v);
+  return __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
+}
+// x / by with 1 / by to 2^-24 at least, quotients below 2^24
+__device__ static __forceinline__ int64_t kw_quotient(int64_t x, int by, double inverse) {
+  int64_t q = (int64_t)((double)x * inverse);
+  const int64_t left = x - q * by;
+  return q + (left >= by) - (left < 0);
+}
+
 // over the 16 lanes of a row, each in an order of its own
 __device__ static __forceinline__ float kw_row_sum(float v) {
 #define KW_ROTATED(n) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x120 + n, 0xf, 0xf, true))
@@ -117,23 +128,27 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     mine += units;
   }
   int64_t at = mine;
-#pragma unroll
-  for (int o = 1; o < SP_WAVE; o <<= 1) {
+  for (int o = 1; o < a.batch && o < SP_WAVE; o <<= 1) {
     const int64_t y = __shfl_up(at, o, SP_WAVE);
     if (lane >= o) at += y;
   }
-  const int64_t total = kw_lane(at, SP_WAVE - 1);
+  const int64_t total = kw_lane(at, pg_min(a.batch, SP_WAVE) - 1);
   at -= mine;
   // what the line's first request has beside its blocks every part has: the parts begin behind it
   const uint64_t some = __ballot(mine > 0);
   lead = some != 0ull ? kw_lane(lead, __builtin_ctzll(some)) : 0;
-  const int64_t shared = total - lead, parts = pg_parts(shared, a.parts, KW_SHARE);
-  auto cut = [&](int64_t p) { return lead + pg_cut(shared, parts, p); };
-  const int64_t cut0 = part < parts ? cut(part) : total, cut1 = part < parts ? cut(part + 1) : total;
+  const int64_t shared = total - lead, full = (shared + KW_SHARE - 1) / KW_SHARE;
+  const int parts = full < a.parts ? pg_max((int)full, 1) : a.parts;
+  // Part p begins at unit shared * p / parts, in doubles (divisions of 64 bits take a hundred instructions each, which every launch fetches anew): exact for
+  // fewer than 2^36 units, behind which equal cuts need not be, only the same wherever they are formed.  (Quotients are multiples of 1 / 512 at least.)
+  const double inv = kw_inverse((double)parts);
+  auto cut = [&](int p) { return p >= parts ? total : lead + (int64_t)__builtin_fma((double)shared * (double)p, inv, 1.0 / 1024); };
+  const int64_t cut0 = cut(part), cut1 = cut(part + 1);
   // of a request whose blocks have `each` units: KW_OVERHEAD blocks' worth, then its blocks; a part may fall between two cuts of one block and hold none
   auto steps = [&](int64_t start, int n, int each, int64_t c0, int64_t c1, int* begin, int* end) {
+    const double by = __builtin_amdgcn_rcp((double)each);
     auto block = [&](int64_t c) {
-      const int64_t off = c - start, at = off <= 0 ? 0 : off < PG_SHORT_LINE ? (int64_t)((unsigned)off / (unsigned)each) : off / each;
+      const int64_t off = c - start, at = off > 0 ? kw_quotient(off, each, by) : 0;
       return (int)(at <= KW_OVERHEAD ? 0 : at - KW_OVERHEAD < n ? at - KW_OVERHEAD : n);
     };
     *begin = block(c0);
@@ -141,11 +156,11 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
   };
   // the part that unit x lies in, and the one that a request's first block ends in
   auto part_of = [&](int64_t x) {
-    int64_t p = (int64_t)((float)(x - lead) * (float)parts * __builtin_amdgcn_rcpf((float)shared));  // within one: parts are KW_PLACES at most
-    if (p >= parts) p = parts - 1;
+    int p = (int)((float)(x - lead) * (float)parts * __builtin_amdgcn_rcpf((float)shared));  // within one: parts are KW_PLACES at most
+    p = pg_min(p, parts - 1);
     while (p > 0 && cut(p) > x) --p;
     while (p + 1 < parts && cut(p + 1) <= x) ++p;
-    return (int)p;
+    return p;
   };
   auto first_part = [&](int64_t start, int each) { return part_of(start + (int64_t)(KW_OVERHEAD + 1) * each - 1); };
   const bool holds = cut0 < cut1 && cut0 >= at && cut0 < at + mine;
@@ -192,7 +207,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     // (scalar loads: nothing writes the table during the launch)
     const auto table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(a.table + (int64_t)__builtin_amdgcn_readfirstlane(b) * a.table_stride);
     struct Ids {
-      int id[2];  // pages of the wave's 16-key halves of a block, -1: none
+      int id[2];  // pages of the wave's 16-key halves of a block, in Keys -1: none
     };
     struct Keys {  // K operands of the wave's 32 keys of a block
       dc_u32x4 r[2][KS];
@@ -203,17 +218,16 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int page = ((from + block) * KW_BLOCK + wave * KW_KEYS + 16 * i) >> a.shift;
-        const int id = table[pg_min(page, a.width - 1)];
-        x.id[i] = page < a.width && (unsigned)id < (unsigned)a.num_pages ? id : -1;
+        x.id[i] = table[pg_min(page, a.width - 1)];
       }
       return x;
     };
     auto fetch = [&](int block, Ids ids, Keys& x) {
-      x.ids = ids;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int key = (from + block) * KW_BLOCK + wave * KW_KEYS + 16 * i;
-        const sp_bf16* src = kh + (int64_t)pg_max(ids.id[i], 0) * a.sk_p + (int64_t)((key & ((1 << a.shift) - 1)) + lq) * a.sk_n + 8 * gr;
+        x.ids.id[i] = key >> a.shift < a.width && (unsigned)ids.id[i] < (unsigned)a.num_pages ? ids.id[i] : -1;
+        const sp_bf16* src = kh + (int64_t)pg_max(x.ids.id[i], 0) * a.sk_p + (int64_t)((key & ((1 << a.shift) - 1)) + lq) * a.sk_n + 8 * gr;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) x.r[i][ks] = *reinterpret_cast<const dc_u32x4*>(src + 32 * ks);
       }
@@ -221,15 +235,18 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     for (int row0 = 0; row0 < rows; row0 += KW_ROWS) {
       const int here = pg_min(rows - row0, KW_ROWS), tiles = (here + 31) / 32 * 2;  // (an even number)
       Keys cur, nxt;
+      Ids ids = entries(begin);
       __syncthreads();  // (the rows before are done with)
-      for (int i = t; i < tiles * 16 * CHUNKS; i += KW_THREADS) {
-        const int r = i / CHUNKS, row = row0 + pg_min(r, here - 1), token = (int)pg_div((unsigned)row, a.by_group);
+      // (workgroups side by side begin at rows of their own: all of them ask for the same ones)
+      const int runs = tiles * 16 * CHUNKS / KW_THREADS;
+      for (int j = 0, at = part % runs; j < runs; ++j, at = at + 1 < runs ? at + 1 : 0) {
+        const int i = at * KW_THREADS + t, r = i / CHUNKS, row = row0 + pg_min(r, here - 1), token = (int)pg_div((unsigned)row, a.by_group);
         __builtin_amdgcn_global_load_lds((kw_gbl_ptr)(a.q + (int64_t)(start + token) * a.sq_n + (int64_t)(kvh * g + (row - token * g)) * a.sq_h +
                                                       8 * ((i % CHUNKS) ^ ds_swz_k<D>(r & 15))),
                                          (ds_lds_ptr)(q_lds + (i - lane) * 16), 16, 0, 0);
       }
-      fetch(begin, entries(begin), cur);
-      Ids ids = entries(pg_min(begin + 1, end - 1));
+      fetch(begin, ids, cur);
+      ids = entries(pg_min(begin + 1, end - 1));
       if constexpr (SUMS) {
         const int count = a.few ? a.of_request[b].x : 0;
         for (int r = t; r < tiles * 16; r += KW_THREADS) {  // (rows that are none weigh nothing)
