@@ -49,14 +49,6 @@ struct KwArgs {
 __device__ static __forceinline__ float kw_max(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 __device__ static __forceinline__ float kw_max(ds_floatx4 v) { return __builtin_elementwise_maximum(kw_max(v[0], v[1], v[2]), v[3]); }
 
-__device__ static __forceinline__ int64_t kw_lane(int64_t v, int lane) {  // (a lane that all agree on)
-  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
-}
-
-__device__ static __forceinline__ double kw_inverse(double v) {
-  const double r = __builtin_amdgcn_rcp(v);
-  return __builtin_fma(__builtin_fma(-v, r, 1.0), r, r);
-}
 // x / by with 1 / by to 2^-24 at least, quotients below 2^24
 __device__ static __forceinline__ int64_t kw_quotient(int64_t x, int by, double inverse) {
   int64_t q = (int64_t)((double)x * inverse);
@@ -132,17 +124,15 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
     const int64_t y = __shfl_up(at, o, SP_WAVE);
     if (lane >= o) at += y;
   }
-  const int64_t total = kw_lane(at, pg_min(a.batch, SP_WAVE) - 1);
+  const int64_t total = ds_lane64(at, pg_min(a.batch, SP_WAVE) - 1);
   at -= mine;
   // what the line's first request has beside its blocks every part has: the parts begin behind it
   const uint64_t some = __ballot(mine > 0);
-  lead = some != 0ull ? kw_lane(lead, __builtin_ctzll(some)) : 0;
+  lead = some != 0ull ? ds_lane64(lead, __builtin_ctzll(some)) : 0;
   const int64_t shared = total - lead, full = (shared + KW_SHARE - 1) / KW_SHARE;
   const int parts = full < a.parts ? pg_max((int)full, 1) : a.parts;
-  // Part p begins at unit shared * p / parts, in doubles (divisions of 64 bits take a hundred instructions each, which every launch fetches anew): exact for
-  // fewer than 2^36 units, behind which equal cuts need not be, only the same wherever they are formed.  (Quotients are multiples of 1 / 512 at least.)
-  const double inv = kw_inverse((double)parts);
-  auto cut = [&](int p) { return p >= parts ? total : lead + (int64_t)__builtin_fma((double)shared * (double)p, inv, 1.0 / 1024); };
+  const PgCuts cuts = pg_cuts(shared, parts);
+  auto cut = [&](int p) { return lead + pg_cut_at(cuts, p); };
   const int64_t cut0 = cut(part), cut1 = cut(part + 1);
   // of a request whose blocks have `each` units: KW_OVERHEAD blocks' worth, then its blocks; a part may fall between two cuts of one block and hold none
   auto steps = [&](int64_t start, int n, int each, int64_t c0, int64_t c1, int* begin, int* end) {
@@ -182,7 +172,7 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
   const uint64_t holder = __ballot(holds);
   const int held = holder != 0ull ? __builtin_ctzll(holder) : 0;  // (the lanes' b is the batch where none holds)
   b = __builtin_amdgcn_readlane(b, held);
-  unit = kw_lane(unit, held);
+  unit = ds_lane64(unit, held);
 
   for (; b < a.batch && unit < cut1; ++b) {
     const int n = blocks(b, &from);

@@ -112,6 +112,27 @@ PG_FN int64_t pg_cut(int64_t total, int64_t parts, int64_t p) {
   }
   return total / parts * p + total % parts * p / parts;
 }
+// The same cuts in doubles, for kernels that form few of them in long programs (a division of 64 bits is a hundred instructions, which every launch fetches
+// anew): equal to pg_cut's for lines of fewer than 2^36 units, as a quotient by up to 512 that is not whole is 1 / 512 off at least; longer lines' parts
+// need not be equal, only lie side by side.
+struct PgCuts {
+  int64_t total;
+  double inverse;
+  int parts;
+};
+PG_FN PgCuts pg_cuts(int64_t total, int parts) {
+  PgCuts c = {total, 0.0, parts};
+#ifdef __HIP_DEVICE_COMPILE__
+  const double r = __builtin_amdgcn_rcp((double)parts);  // to 2^-24
+  c.inverse = __builtin_fma(__builtin_fma(-(double)parts, r, 1.0), r, r);
+#else
+  c.inverse = 1.0 / parts;
+#endif
+  return c;
+}
+PG_FN int64_t pg_cut_at(const PgCuts& c, int p) {
+  return p >= c.parts ? c.total : (int64_t)__builtin_fma((double)c.total * (double)p, c.inverse, 1.0 / 1024);
+}
 // How near: a cut leaves partials behind that are written, read and merged, some four units' worth, and is not worth a quarter of a part.
 PG_FN int pg_near(int64_t total, int64_t parts) {
   const int64_t four = 16 * parts;

@@ -52,6 +52,10 @@ __device__ static __forceinline__ float ds_quad_sum(float v) {
   return __builtin_bit_cast(float, (uint32_t)b[0]) + __builtin_bit_cast(float, (uint32_t)b[1]);
 }
 
+__device__ static __forceinline__ int64_t ds_lane64(int64_t v, int lane) {  // (a lane that all agree on)
+  return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
+}
+
 // LDS reads the compiler does not track: it would wait for every direct-to-LDS load in flight before each
 __device__ static __forceinline__ dc_u32x4 ds_read_k(uint32_t addr) {
   dc_u32x4 r;

@@ -136,3 +136,29 @@ def test_very_long_lines(ask):
     for streams in (20, 110):
         pieces = ask([(items, streams, 32)])[0]
         assert sum(end - begin for kind, _, _, _, begin, end in pieces) == 20 * 6 * n + 90 * n
+
+
+def test_cuts_in_doubles_are_the_cuts(tmp_path):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    (tmp_path / "cuts.cpp").write_text("""
+#include <stdio.h>
+#include "sp_paged_plan.h"
+int main() {
+  uint64_t x = 1;
+  long bad = 0;
+  for (int i = 0; i < 20000; ++i) {
+    x = x * 6364136223846793005ull + 1442695040888963407ull;
+    const int parts = 1 + (int)(x >> 40) % 512;
+    const int64_t total = (int64_t)((x >> 8) & ((1ull << (1 + i % 36)) - 1)) / (i % 3 ? 1 : parts) * (i % 3 ? 1 : parts);
+    const PgCuts cuts = pg_cuts(total, parts);
+    for (int p = 0; p <= parts + 1; ++p) bad += pg_cut_at(cuts, p) != (p > parts ? total : (int64_t)((unsigned __int128)total * p / parts));
+  }
+  const PgCuts cuts = pg_cuts((1ll << 59) + 12345, 511);  // (beyond: in order, from 0 to the end)
+  for (int p = 0; p < 511; ++p) bad += pg_cut_at(cuts, p + 1) < pg_cut_at(cuts, p);
+  bad += pg_cut_at(cuts, 0) != 0 || pg_cut_at(cuts, 511) != (1ll << 59) + 12345;
+  printf("%ld\\n", bad);
+}
+""")
+    subprocess.run(["g++", "-O2", "-Wall", "-I", CSRC, str(tmp_path / "cuts.cpp"), "-o", str(tmp_path / "cuts")], check=True)
+    assert subprocess.run([str(tmp_path / "cuts")], capture_output=True, text=True, check=True).stdout.strip() == "0"
