@@ -2,7 +2,7 @@
 // that a plain C++ compiler takes as well.
 //
 // Rows are (token, query head of the kv group) pairs, the heads of a token side by side, 64 or 128 of them a tile.  Items are the groups, over their
-// shared keys, and behind them the requests, over their own.  An item has as many units as its tiles have steps of 32 keys, and SH_OVERHEAD beside them a
+// shared keys, and behind them the requests, over their own.  An item has as many units as its tiles have steps of 32 keys, and SH_OVERHEAD (SH_OWN_OVERHEAD) beside them a
 // tile, for its queries, its first loads and the waves' meeting; the items lie on a line that is cut into equal parts, one workgroup of a kv head each.
 // Single tokens whose heads fit 16 rows are no matter of the workgroup's but of its waves: four of them have a quarter each of what of the requests falls to
 // it, go through it step by step and count one unit beside an item's steps (SH_STREAM_OVERHEAD).
@@ -13,7 +13,12 @@
 #define SH_ROWS 128      // of a tile at most
 #define SH_KEYS 32       // of a step
 #define SH_MAX_SEQS 1024
+enum { SH_GROUP, SH_OWN, SH_STREAM };  // items: a group's shared keys, a request's own, the same as a matter of waves
+// Units of a tile beside its steps.  (us, 6 / 10 / 14 / 20 of a request's: two tokens each of 40 requests over 120 own keys, most behind 17378 shared
+// ones 57 / 48 / 48 / 50, nine of 20 over a few 37 / 32 / 34 / 33, two of 37 over 1336 40 / 39 / 40 / 40; 6 / 7 / 8 of a group's: eight tokens behind 1024 keys
+// 20 / 22 / 22.)
 #define SH_OVERHEAD 6
+#define SH_OWN_OVERHEAD 10
 #define SH_STREAM_OVERHEAD 1
 #define SH_MIN_SHARE 8   // units of a part at least
 #define SH_WAVES 4       // that share a workgroup's keys
@@ -22,17 +27,18 @@
 PG_FN int sh_tile(int rows) { return rows <= SH_UNIT ? SH_UNIT : SH_ROWS; }
 PG_FN int sh_step_units(int rows) { return rows <= SH_UNIT ? 1 : 2; }
 // Where a cut `off` units into an item stands whose tiles have n steps each: in front of a step of a tile (the n-th: behind the tile).
-PG_FN void sh_place(int64_t off, int n, int rows, int near, int* tile, int* step) {
-  const int of_step = sh_step_units(rows);
-  const int64_t each = (int64_t)n * of_step + SH_OVERHEAD, at = off < PG_SHORT_LINE ? (int64_t)((unsigned)off / (unsigned)each) : off / each;
+PG_FN int sh_overhead(int kind) { return kind == SH_GROUP ? SH_OVERHEAD : kind == SH_OWN ? SH_OWN_OVERHEAD : SH_STREAM_OVERHEAD; }
+PG_FN void sh_place(int64_t off, int n, int rows, int kind, int near, int* tile, int* step) {
+  const int of_step = sh_step_units(rows), overhead = sh_overhead(kind);
+  const int64_t each = (int64_t)n * of_step + overhead, at = off < PG_SHORT_LINE ? (int64_t)((unsigned)off / (unsigned)each) : off / each;
   const int64_t in = off - at * each;
   *tile = (int)at;
-  *step = pg_snap(in < SH_OVERHEAD ? 0 : SH_OVERHEAD + (in - SH_OVERHEAD) / of_step, n, SH_OVERHEAD, near);
+  *step = pg_snap(in < overhead ? 0 : overhead + (in - overhead) / of_step, n, overhead, near);
 }
 // The same of a request's steps among those of a wave.
 PG_FN int sh_stream_step(int64_t off, int n) { return pg_snap(off, n, SH_STREAM_OVERHEAD, 1); }
-PG_FN int64_t sh_units(int n, int rows, int streams) {
-  return n <= 0 ? 0 : streams ? n + SH_STREAM_OVERHEAD : ((int64_t)n * sh_step_units(rows) + SH_OVERHEAD) * ((rows + sh_tile(rows) - 1) / sh_tile(rows));
+PG_FN int64_t sh_units(int n, int rows, int kind) {
+  return n <= 0 ? 0 : kind == SH_STREAM ? n + SH_STREAM_OVERHEAD : ((int64_t)n * sh_step_units(rows) + sh_overhead(kind)) * ((rows + sh_tile(rows) - 1) / sh_tile(rows));
 }
 // A request whose first new token stands behind its group's shared keys takes part in the group; any other sees to all of its keys by itself.
 PG_FN int sh_first_own(int len, int q_len, int shared) { return len - q_len >= shared ? shared : 0; }

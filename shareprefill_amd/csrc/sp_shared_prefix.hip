@@ -168,7 +168,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
         if (blockIdx.x == 0) a.of_request[x - n_groups] = r;
       }
       const ShItem p = item(x);
-      const int64_t units = sh_units(p.n, p.rows, a.streams && x >= n_groups);
+      const int64_t units = sh_units(p.n, p.rows, x < n_groups ? SH_GROUP : a.streams ? SH_STREAM : SH_OWN);
       line_s[x] = at;  // (of the thread's; completed below)
       at += units;
     }
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     if (wanted) {
       f.item = lo;
       if (gr < 2)
-        sh_place(off, p.n, p.rows, near, &f.tile, &f.step);
+        sh_place(off, p.n, p.rows, lo < n_groups ? SH_GROUP : SH_OWN, near, &f.tile, &f.step);
       else
         f.step = sh_stream_step(off, p.n);
     }

@@ -13,15 +13,15 @@ PROGRAM = """
 #include <stdio.h>
 #include <vector>
 #include "sp_shared_plan.h"
-// items of `rows` rows and n steps a tile, those from `streams` on waves'; room: workgroups.  Prints every piece: part (of a wave), item, tile, begin, end.
+// items of `rows` rows and n steps a tile, the first `groups` of them groups, those from `streams` on waves'; room: workgroups.  Prints every piece: part (of a wave), item, tile, begin, end.
 int main() {
-  long items, streams, room;
-  while (scanf("%ld %ld %ld", &items, &streams, &room) == 3) {
+  long items, groups, streams, room;
+  while (scanf("%ld %ld %ld %ld", &items, &groups, &streams, &room) == 4) {
     std::vector<long> n(items), rows(items);
     std::vector<int64_t> line(items + 1);
     for (long i = 0; i < items; ++i) {
       if (scanf("%ld %ld", &n[i], &rows[i]) != 2) return 1;
-      line[i + 1] = line[i] + (n[i] > 0 && rows[i] > 0 ? sh_units((int)n[i], (int)rows[i], i >= streams) : 0);
+      line[i + 1] = line[i] + (n[i] > 0 && rows[i] > 0 ? sh_units((int)n[i], (int)rows[i], i < groups ? SH_GROUP : i < streams ? SH_OWN : SH_STREAM) : 0);
     }
     const int64_t total = line[items], parts = pg_parts(total, room, SH_MIN_SHARE);
     const int near = pg_near(total, parts);
@@ -39,7 +39,7 @@ int main() {
         from[e] = streams, tile[e] = step[e] = 0;
         if (cut[e] < line[streams]) {
           from[e] = holder(cut[e]);
-          sh_place(cut[e] - line[from[e]], (int)n[from[e]], (int)rows[from[e]], near, &tile[e], &step[e]);
+          sh_place(cut[e] - line[from[e]], (int)n[from[e]], (int)rows[from[e]], from[e] < groups ? SH_GROUP : SH_OWN, near, &tile[e], &step[e]);
         }
       }
       for (long x = from[0], t0 = tile[0], begin = step[0]; x < streams && x <= from[1]; ++x, t0 = 0, begin = 0)
@@ -79,7 +79,7 @@ def ask(tmp_path_factory):
                     str(tmp / "plan.cpp"), "-o", str(tmp / "plan")], check=True)
 
     def run(cases):
-        text = "".join(f"{len(items)} {streams} {room} " + " ".join(f"{n} {rows}" for n, rows in items) + "\n" for items, streams, room in cases)
+        text = "".join(f"{len(items)} {min(streams, len(items) // 2)} {streams} {room} " + " ".join(f"{n} {rows}" for n, rows in items) + "\n" for items, streams, room in cases)
         out = subprocess.run([str(tmp / "plan")], input=text, capture_output=True, text=True, check=True).stdout
         found, here = [], []
         for line in out.splitlines():
