@@ -478,7 +478,7 @@ typedef struct sp_paged_evict_args {
   int64_t k_stride_page, k_stride_slot, k_stride_h, v_stride_page, v_stride_slot, v_stride_h, w_stride_page, w_stride_h;
   sp_stream_t stream;
 } sp_paged_evict_args;
-size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int64_t num_pages, int64_t page_size, int64_t table_width);
+size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int32_t d, int64_t num_pages, int64_t page_size, int64_t table_width);
 int sp_paged_evict_bf16(const sp_paged_evict_args* args /* host */);
 
 /* ---- rotary position embedding in front of the attention function ---------------------------------

@@ -18,6 +18,9 @@
 #define EV_RUN 16           // keys of a thread, which lie in one page
 #define EV_CHUNK (EV_THREADS * EV_RUN)
 #define EV_MAX_SHARES 16    // workgroups that share a kv head's keys
+#define EV_SLICE 512        // channels of a row that a workgroup moves
+#define EV_AHEAD 8          // rows of a thread
+#define EV_FEW 256          // workgroups that move: one a CU
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
 typedef float ev_floatx4 __attribute__((ext_vector_type(4)));
@@ -28,12 +31,14 @@ struct EvArgs {
   const int32_t *table, *lens, *first;
   int32_t* new_lens;
   int64_t table_stride, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;
-  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slice;
+  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slices, streams, chunks;
   // By place in the pages, [num_pages][kv head][page]: entry i of a request's list stands at the place of its i-th key behind the first ones.  First
   // pattern << 32 | place of what is listed, then the place that a kept key comes from; a place is page << shift + place in it.
   uint64_t* list;
   uint32_t* hists;  // [request][kv head][share][EV_BINS]
   int32_t* counts;  // [request][kv head][share]: entries of the list
+  int2* bins;       // [request][kv head]: what ev_find says of the first histogram
+  int32_t *tickets, *done;  // [stream] chunks that were taken, [stream][chunk] those that are read; a stream: a kv head's K, V (by EV_SLICE channels) or weights
 };
 
 // What becomes of a request: keys first .. first + mid - 1 may go, `keep` of them stay (keep == mid: nothing moves).
@@ -226,6 +231,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_gather_kernel(const EvArg
   const EvBin f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
   const int n = ev_gather(p, p.share_start(share), p.share_start(share + 1), (uint32_t)f.bin, wave_s, stage);
   if (threadIdx.x == 0) a.counts[blockIdx.x] = n;
+  if (threadIdx.x == 0 && share == 0) a.bins[pair] = make_int2(f.bin, f.left);
 }
 
 // One workgroup a kv head: T, and the list of what stays.  Up to EV_CHUNK keys, a kv head's own or those that are listed, stay in registers for all of it.
@@ -235,6 +241,11 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
   __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES], start_s[EV_MAX_SHARES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, pair = blockIdx.x, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
+  for (int part = 0; part <= 2 * a.slices; ++part) {
+    const int stream = part * a.batch * a.hkv + pair;
+    if (t == 0) a.tickets[stream] = 0;
+    for (int i = t; i < a.chunks; i += EV_THREADS) a.done[(int64_t)stream * a.chunks + i] = 0;
+  }
   const bool goes = p.r.keep < p.r.mid && ev_has_pages(a, b, p.r);
   if (p.kvh == 0 && t == 0) a.new_lens[b] = goes ? p.r.len - p.r.mid + p.r.keep : p.r.len;
   if (!goes || p.r.keep == 0) return;
@@ -248,12 +259,16 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
       const int n = ev_gather(p, p.r.first, p.r.first + p.r.mid, (uint32_t)f.bin, wave_s, stage);
       if (t == 0) count_s[0] = n;
     } else {
+      const int2 bin = a.bins[pair];
+      f = {bin.x, bin.y};
       if (t < a.shares) count_s[t] = a.counts[pair * a.shares + t];
     }
     __syncthreads();
-    for (int s = 0; s < a.shares; ++s) {
-      if (t == 0) start_s[s] = listed;
-      listed += count_s[s];
+#pragma unroll
+    for (int s = 0; s < EV_MAX_SHARES; ++s) {
+      const int n = s < a.shares ? count_s[s] : 0;
+      if (t == s) start_s[s] = listed;
+      listed += n;
     }
     __syncthreads();
   }
@@ -268,22 +283,26 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
       for (int e = 0; e < EV_RUN; ++e) place[e] = first + e;
     } else {
       // (threads side by side read entries side by side, then each its own out of LDS)
-#pragma unroll 4
-      for (int i = t; i < listed; i += EV_THREADS) {
+      uint64_t x[EV_RUN];
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e) {
+        const int i = pg_min(t + e * EV_THREADS, listed - 1);
         int s = 0;
 #pragma unroll
         for (int step = EV_MAX_SHARES / 2; step > 0; step /= 2)
           if (s + step < a.shares && start_s[s + step] <= i) s += step;
-        stage[i] = *p.entry(p.share_start(s) - p.r.first + i - start_s[s]);
+        x[e] = *p.entry(p.share_start(s) - p.r.first + i - start_s[s]);
       }
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e) stage[t + e * EV_THREADS] = x[e];
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < EV_RUN; ++e)
         if (t * EV_RUN + e < listed) key[e] = (uint32_t)(stage[t * EV_RUN + e] >> 32), place[e] = (uint32_t)stage[t * EV_RUN + e];
     }
-    uint32_t top = 0;
-    int left = p.r.keep;
-    for (int shift = 20; shift >= 0; shift -= 10) {
+    uint32_t top = whole ? 0 : (uint32_t)f.bin;
+    int left = whole ? p.r.keep : f.left;
+    for (int shift = whole ? 20 : 10; shift >= 0; shift -= 10) {
       for (int i = t; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
       __syncthreads();
 #pragma unroll
@@ -307,11 +326,10 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
       over_at += over, same_at += same;
     }
     __syncthreads();
-#pragma unroll 4
+#pragma unroll 8
     for (int i = t; i < p.r.keep; i += EV_THREADS) *p.entry(i) = stage[i];
     return;
   }
-  if (a.shares > 1) f = ev_first_bin(a, pair, p.r.keep, hist, wave_s, found_s);
   uint32_t top = (uint32_t)f.bin;  // bits of T that are known
   int left = f.left;               // the left-th largest of those that share them is T
   for (int shift = 10; shift >= 0; shift -= 10) {
@@ -359,60 +377,56 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
   }
 }
 
-#define EV_AHEAD 8  // rows of a thread in flight
+// A workgroup moves a chunk of a kv head's kept rows: reads them all, waits until the chunks in front of it have read theirs, which alone may need what it
+// writes over, and writes.  A chunk is taken when its workgroup has begun, so that whoever is waited for runs, and waits for nobody before it has read.
+template <int AHEAD>
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs a) {
-  // (the slices of a kv head side by side in the same XCD's L2, where the kv heads are a multiple of eight)
-  const int t = threadIdx.x, pairs = a.batch * a.hkv, pair = blockIdx.x % pairs, part = blockIdx.x / pairs;
-  const int lanes = a.slice / 8, slices = (a.d + a.slice - 1) / a.slice, b = pair / a.hkv;
+  __shared__ int chunk_s;
+  const int t = threadIdx.x, pairs = a.batch * a.hkv, stream = blockIdx.x % a.streams, pair = stream % pairs, part = stream / pairs, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   const EvRequest& r = p.r;
+  // (the look at the table has its entries at hand when the ticket comes: 30 us for 44 where the launch before this one had told what it says)
+  if (t == 0) chunk_s = __hip_atomic_fetch_add(a.tickets + stream, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (!(r.keep < r.mid && ev_has_pages(a, b, r))) return;
-  const int rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
-  // where kept key i goes and comes from
-  auto from = [&](int i, int64_t to) {
-    return i < r.keep ? (int64_t)a.list[((((to >> a.shift) * a.hkv + p.kvh) << a.shift) + (to & in))] : p.place(r.first + r.mid + (i - r.keep));
-  };
-  if (part == 2 * slices) {
-    float* const w = a.weights + p.kvh * a.sw_h;
-    auto at = [&](int64_t x) { return (x >> a.shift) * a.sw_p + (x & in); };
-    for (int i0 = 0; i0 < rows; i0 += EV_THREADS * EV_AHEAD) {
-      float x[EV_AHEAD];
-      int64_t to[EV_AHEAD];
+  const int chunk = chunk_s, rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
+  auto move = [&](auto type, int lanes, auto at) {  // elements of a row side by side, one a thread
+    const int per = EV_THREADS / lanes, row = t / lanes;
+    const int64_t i0 = (int64_t)chunk * (per * AHEAD);
+    if (i0 >= rows) return;
+    decltype(type) y[AHEAD] = {};
+    uint32_t to[AHEAD];
 #pragma unroll
-      for (int u = 0; u < EV_AHEAD; ++u) {
-        const int i = pg_min(i0 + u * EV_THREADS + t, rows - 1);
-        to[u] = p.place(r.first + i);
-        x[u] = w[at(from(i, to[u]))];
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tile is read
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < EV_AHEAD; ++u)
-        if (i0 + u * EV_THREADS + t < rows) w[at(to[u])] = x[u];
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = (int)i0 + u * per + row;
+      to[u] = 0;
+      if (row >= per || i >= rows) continue;
+      const int64_t goes = p.place(r.first + i);
+      const int64_t come = i < r.keep ? (int64_t)a.list[((((goes >> a.shift) * a.hkv + p.kvh) << a.shift) + (goes & in))] : p.place(r.first + r.mid + (i - r.keep));
+      to[u] = (uint32_t)goes;
+      y[u] = *at(come);
     }
-    return;
-  }
-  const bool is_v = part >= slices;
-  const int c = (part % slices) * a.slice + t % lanes * 8, row = t / lanes, per = EV_THREADS / lanes;
-  const int64_t page_at = is_v ? a.sv_p : a.sk_p, slot_at = is_v ? a.sv_n : a.sk_n;
-  sp_bf16* const x = (is_v ? a.v + p.kvh * a.sv_h : a.k + p.kvh * a.sk_h) + c;
-  auto at = [&](int64_t y) { return x + (y >> a.shift) * page_at + (y & in) * slot_at; };
-  const bool mine = c < a.d;
-  for (int i0 = 0; i0 < rows; i0 += per * EV_AHEAD) {
-    ev_u32x4 y[EV_AHEAD];
-    int64_t to[EV_AHEAD];
-#pragma unroll
-    for (int u = 0; u < EV_AHEAD; ++u) {
-      const int i = pg_min(i0 + u * per + row, rows - 1);
-      to[u] = p.place(r.first + i);
-      const int64_t come = from(i, to[u]);
-      if (mine) y[u] = *reinterpret_cast<const ev_u32x4*>(at(come));
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tile is read
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // the chunk is read
+    int32_t* const done = a.done + (int64_t)stream * a.chunks;
+    if (t == 0) __hip_atomic_store(done + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (t < SP_WAVE)
+      for (int i = t; i < chunk; i += SP_WAVE)
+        while (__hip_atomic_load(done + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(1);
+    asm volatile("" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < EV_AHEAD; ++u)
-      if (i0 + u * per + row < rows && mine) *reinterpret_cast<ev_u32x4*>(at(to[u])) = y[u];
+    for (int u = 0; u < AHEAD; ++u)
+      if (row < per && i0 + u * per + row < rows) *at(to[u]) = y[u];
+  };
+  if (part == 2 * a.slices) {
+    float* const w = a.weights + p.kvh * a.sw_h;
+    move(0.f, 1, [&](int64_t x) { return w + (x >> a.shift) * a.sw_p + (x & in); });
+  } else {
+    const bool is_v = part >= a.slices;
+    const int c = part % a.slices * EV_SLICE, lanes = pg_min(a.d - c, EV_SLICE) / 8;
+    const int64_t page_at = is_v ? a.sv_p : a.sk_p, slot_at = is_v ? a.sv_n : a.sk_n;
+    sp_bf16* const x = (is_v ? a.v + p.kvh * a.sv_h : a.k + p.kvh * a.sk_h) + c + t % lanes * 8;
+    move(ev_u32x4{}, lanes, [&](int64_t y) { return reinterpret_cast<ev_u32x4*>(x + (y >> a.shift) * page_at + (y & in) * slot_at); });
   }
 }
 
@@ -424,22 +438,42 @@ static int ev_shares(int64_t pairs, int64_t room) {
   const int64_t n = by_keys < by_card ? by_keys : by_card;
   return n < 1 ? 1 : n > EV_MAX_SHARES ? EV_MAX_SHARES : (int)n;
 }
-struct EvSizes {
-  size_t list, hists, counts, bytes;
+struct EvMove {
+  int64_t slices, streams, ahead, chunks;
 };
-static EvSizes ev_sizes(int64_t pairs, int64_t hkv, int64_t pool_keys, int shares) {
+// Chunks of `kept` rows at most, as many as the widest stream needs.  A thread has EV_AHEAD rows in flight, or one where few workgroups are enough all the same: us,
+// one / 2 / 4 / 8 / 16, eight kv heads' 320 rows of 128 channels 8 / 9 / 10 / 11 / 11, their 8192 rows 45 / 36 / 34 / 30 / 36, 64 kv heads' 2000 rows 67 / 50 / 44 /
+// 40 / 46.
+static EvMove ev_move(int64_t pairs, int64_t d, int64_t kept) {
+  EvMove m;
+  m.slices = (d + EV_SLICE - 1) / EV_SLICE, m.streams = pairs * (2 * m.slices + 1);
+  const int64_t rows = EV_THREADS / ((d < EV_SLICE ? d : EV_SLICE) / 8);
+  m.ahead = m.streams * ((kept + rows - 1) / rows) <= EV_FEW ? 1 : EV_AHEAD;
+  m.chunks = (kept + rows * m.ahead - 1) / (rows * m.ahead);
+  return m;
+}
+struct EvSizes {
+  size_t list, hists, counts, bins, tickets, done, bytes;
+};
+static EvSizes ev_sizes(int64_t batch, int64_t hkv, int64_t pool_keys, int shares, const EvMove& m) {
   EvSizes s;
+  const int64_t pairs = batch * hkv;
   s.list = 0;
   s.hists = (size_t)(hkv * pool_keys) * sizeof(uint64_t);
   s.counts = s.hists + (shares > 1 ? (size_t)(pairs * shares) * EV_BINS * sizeof(uint32_t) : 0);
-  s.bytes = s.counts + (shares > 1 ? ((size_t)(pairs * shares) * sizeof(int32_t) + 15) / 16 * 16 : 0);
+  s.bins = s.counts + (shares > 1 ? ((size_t)(pairs * shares) * sizeof(int32_t) + 15) / 16 * 16 : 0);
+  s.tickets = s.bins + (shares > 1 ? ((size_t)pairs * sizeof(int2) + 15) / 16 * 16 : 0);
+  s.done = s.tickets + ((size_t)m.streams * sizeof(int32_t) + 15) / 16 * 16;
+  const int64_t chunks = m.streams * m.chunks;
+  s.bytes = s.done + ((size_t)(chunks > EV_FEW ? chunks : EV_FEW) * sizeof(int32_t) + 15) / 16 * 16;  // (those of fewer rows than the most may be more)
   return s;
 }
-extern "C" size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int64_t num_pages, int64_t page_size, int64_t table_width) {
-  if (batch <= 0 || hkv <= 0 || num_pages <= 0 || page_size <= 0 || table_width <= 0 || num_pages > 0x7fffffffll || page_size > 1024 || table_width > PG_MAX_KEYS)
+extern "C" size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int32_t d, int64_t num_pages, int64_t page_size, int64_t table_width) {
+  if (batch <= 0 || hkv <= 0 || d <= 0 || d % 8 || d > 65536 || num_pages <= 0 || page_size <= 0 || table_width <= 0 || num_pages > 0x7fffffffll || page_size > 1024 || table_width > PG_MAX_KEYS)
     return 0;
   const int64_t pairs = (int64_t)batch * hkv;
-  return ev_sizes(pairs, hkv, num_pages * page_size, ev_shares(pairs, table_width * page_size)).bytes;
+  const int64_t room = table_width * page_size;
+  return ev_sizes(batch, hkv, num_pages * page_size, ev_shares(pairs, room), ev_move(pairs, d, room)).bytes;
 }
 
 extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
@@ -455,12 +489,8 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   SP_REQUIRE(shift <= 10, SP_ERR_UNSUPPORTED, "%s: page size %lld (a power of two from 16 to 1024)", who, (long long)x->page_size);
   SP_REQUIRE(x->batch <= EV_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %lld (at most %d)", who, (long long)x->batch, EV_MAX_SEQS);
   const int64_t pairs = x->batch * x->hkv;
-  // 128 bytes of a row, or fewer where that leaves most of the card idle
-  int slice = 64;
-  while (slice > 16 && pairs * 2 * ((x->d + slice - 1) / slice) < 256) slice /= 2;
-  const int64_t per = 2 * ((x->d + slice - 1) / slice) + 1;
   SP_REQUIRE(x->hkv <= 65536 && x->num_pages <= 0x7fffffffll && x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS &&
-                 x->num_pages << shift <= 0xffffffffll && pairs * per <= 0x7fffffffll,
+                 x->num_pages << shift <= 0xffffffffll && pairs <= (1 << 22),
              SP_ERR_UNSUPPORTED, "%s: hkv=%lld num_pages=%lld table_width=%lld too large", who, (long long)x->hkv, (long long)x->num_pages,
              (long long)x->table_width);
   const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);
@@ -470,7 +500,11 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   SP_REQUIRE(((uintptr_t)x->k_pages | (uintptr_t)x->v_pages) % 16 == 0 && (k_p | k_h | x->k_stride_slot | v_p | v_h | x->v_stride_slot) % 8 == 0,
              SP_ERR_UNSUPPORTED, "%s: tensors must be 16-byte aligned, strides multiple of 8", who);
   const int shares = ev_shares(pairs, x->table_width << shift);
-  const EvSizes sizes = ev_sizes(pairs, x->hkv, x->num_pages << shift, shares);
+  const int64_t room = x->table_width << shift, most = x->budget > room || x->recent > room || x->budget + x->recent > room ? room : x->budget + x->recent;
+  const EvMove move = ev_move(pairs, x->d, most);  // (rows that are kept beside the first ones, at most)
+  SP_REQUIRE(move.streams * move.chunks <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld rows of %lld kv heads are too many", who, (long long)most,
+             (long long)pairs);
+  const EvSizes sizes = ev_sizes(x->batch, x->hkv, x->num_pages << shift, shares, move);
   SP_REQUIRE(x->workspace != nullptr && x->workspace_bytes >= sizes.bytes && (uintptr_t)x->workspace % 16 == 0, SP_ERR_WORKSPACE,
              "%s: workspace missing, too small or misaligned", who);
   EvArgs a = {};
@@ -480,10 +514,11 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   a.sw_p = pg_used_stride(x->w_stride_page, x->num_pages), a.sw_h = pg_used_stride(x->w_stride_h, x->hkv);
   a.batch = (int)x->batch, a.hkv = (int)x->hkv, a.d = (int)x->d, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
   a.budget = (int)(x->budget < PG_MAX_KEYS ? x->budget : PG_MAX_KEYS), a.recent = (int)(x->recent < PG_MAX_KEYS ? x->recent : PG_MAX_KEYS);
-  a.shares = shares, a.slice = slice;
+  a.shares = shares, a.slices = (int)move.slices, a.streams = (int)move.streams, a.chunks = (int)move.chunks;
   a.by_four = (uintptr_t)x->weights % 16 == 0 && (a.sw_p | a.sw_h) % 4 == 0;
   char* const ws = (char*)x->workspace;
   a.list = (uint64_t*)(ws + sizes.list), a.hists = (uint32_t*)(ws + sizes.hists), a.counts = (int32_t*)(ws + sizes.counts);
+  a.bins = (int2*)(ws + sizes.bins), a.tickets = (int32_t*)(ws + sizes.tickets), a.done = (int32_t*)(ws + sizes.done);
   const hipStream_t stream = (hipStream_t)x->stream;
   constexpr int lds = EV_CHUNK * (int)sizeof(uint64_t);
   static bool attr_set[64] = {false};  // per device, once (idempotent)
@@ -500,7 +535,8 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
     hipLaunchKernelGGL(sp_evict_gather_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), lds, stream, a);
   }
   hipLaunchKernelGGL(sp_evict_choose_kernel, dim3((unsigned)pairs), dim3(EV_THREADS), lds, stream, a);
-  hipLaunchKernelGGL(sp_evict_move_kernel, dim3((unsigned)(pairs * per)), dim3(EV_THREADS), 0, stream, a);
+  if (move.chunks > 0)
+    hipLaunchKernelGGL(move.ahead == 1 ? sp_evict_move_kernel<1> : sp_evict_move_kernel<EV_AHEAD>, dim3((unsigned)(move.streams * move.chunks)), dim3(EV_THREADS), 0, stream, a);
   SP_LAUNCH_CHECK();
   return SP_OK;
 }

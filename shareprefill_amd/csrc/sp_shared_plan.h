@@ -44,7 +44,11 @@ PG_FN int64_t sh_units(int n, int rows, int kind) {
 PG_FN int sh_first_own(int len, int q_len, int shared) { return len - q_len >= shared ? shared : 0; }
 // Numbers of row tiles, by 64 rows (a larger one has that of its first): every sequence has room for its last, partly filled one (pg_first_slot); single tokens whose heads fit a tile have one each.
 PG_FN int64_t sh_own_slot(int64_t start, int g, int b, int dense) { return dense ? b : pg_first_slot(start, g, b, SH_UNIT); }
-// Groups of many rows are left to the kernel that has matrix products' rate (sp_chunk.hip, tiles of 256 rows) and a launch of its own, but where keys are
-// weighed: its sums are those of probabilities rounded to bf16.  us, within one launch / apart: 128 requests of four heads a kv head over 32768 shared keys
-// and some hundred of their own 199 / 156, 64 over 8192 and a thousand 90 / 114, drafted tokens of 32 requests of 64 channels over 16001 85 / 73.
-PG_FN bool sh_apart(int64_t tokens, int64_t groups, int64_t g, bool weighed) { return !weighed && groups > 0 && tokens * g > 256 * groups; }
+// Groups of many rows are left to the kernel that has matrix products' rate (sp_chunk.hip, tiles of 256 rows) where the table has room for enough keys to pay
+// for two launches more, but not where keys are weighed: its sums are those of probabilities rounded to bf16.  By rows x keys x channels, in units of 10^9, us
+// within one launch / apart: 32 heads over 8 of 128 channels 0.7 37 / 56, 3.3 46 / 60, 6.3 76 / 73, 8.4 91 / 78, 17 142 / 105, 67 292 / 186; 28 over 4 1.2 36 / 48,
+// 4.6 67 / 71, 7.3 80 / 73; of 64 channels 1.6 44 / 52, 3.1 55 / 58, 4.2 68 / 61, 8.4 113 / 82.  At 256 rows and fewer tiles of 256 are not full.
+PG_FN bool sh_may_be_apart(int64_t tokens, int64_t groups, int64_t g, bool weighed) { return !weighed && groups > 0 && tokens * g > 256 * groups; }
+PG_FN bool sh_apart(int64_t tokens, int64_t groups, int64_t hq, int64_t hkv, int64_t d, int64_t room, bool weighed) {
+  return sh_may_be_apart(tokens, groups, hq / hkv, weighed) && (double)(tokens * hq * d) * (double)room > 5e9;
+}

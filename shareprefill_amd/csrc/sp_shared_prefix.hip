@@ -948,10 +948,9 @@ struct ShSizes {
   int64_t shared_slots, slots, logits;
   size_t o_part, ml_part, o_stream, ml_stream, o_row, ml_row, parts_of, cuts, of_request, bytes;
 };
-static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d, bool single, int64_t pool_keys) {
+static ShSizes sh_sizes(int64_t tokens, int64_t batch, int64_t groups, int64_t hq, int64_t hkv, int64_t d, bool single, int64_t pool_keys, bool apart) {
   ShSizes s;
   const int64_t g = hq / hkv;
-  const bool apart = sh_apart(tokens, groups, g, pool_keys > 0);
   s.shared_slots = groups > 0 && !apart ? tokens * g / SH_UNIT + groups : 0;
   s.slots = s.shared_slots + (single && g <= SH_UNIT ? batch : tokens * g / SH_UNIT + batch);
   const int64_t rows = (int64_t)sh_workgroups(hkv) * hkv * 2 * SH_ROWS;
@@ -984,9 +983,11 @@ static bool sh_shape_ok(int64_t tokens, int64_t batch, int64_t groups, int64_t h
 
 extern "C" size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t groups, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens,
                                                  int64_t pool_keys) {
-  return sh_shape_ok(tokens, batch, groups, hq, hkv, d) && pool_keys >= 0 && pool_keys <= (1ll << 40)
-             ? sh_sizes(tokens, batch, groups, hq, hkv, d, single_tokens != 0, pool_keys).bytes
-             : 0;
+  if (!sh_shape_ok(tokens, batch, groups, hq, hkv, d) || pool_keys < 0 || pool_keys > (1ll << 40)) return 0;
+  const size_t one = sh_sizes(tokens, batch, groups, hq, hkv, d, single_tokens != 0, pool_keys, false).bytes;
+  if (!sh_may_be_apart(tokens, groups, hq / hkv, pool_keys > 0)) return one;
+  const size_t apart = sh_sizes(tokens, batch, groups, hq, hkv, d, single_tokens != 0, pool_keys, true).bytes;
+  return one > apart ? one : apart;
 }
 
 extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
@@ -1027,8 +1028,9 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   for (const int64_t n : {x->k_stride_slot, x->v_stride_slot})
     SP_REQUIRE(n >= 0 && n < (1ll << 24) && n * x->page_size < (1ll << 30) && n % 8 == 0, SP_ERR_UNSUPPORTED, "%s: slot stride %lld unsupported", who,
                (long long)n);
+  const bool apart = sh_apart(x->tokens, x->groups, x->hq, x->hkv, x->d, x->table_width << shift, x->weights != nullptr);
   const ShSizes s = sh_sizes(x->tokens, x->batch, x->groups, x->hq, x->hkv, x->d, x->cu_q == nullptr,
-                             x->weights != nullptr ? x->num_pages << shift : 0);
+                             x->weights != nullptr ? x->num_pages << shift : 0, apart);
   SP_REQUIRE(s.slots <= 0x7ffffff0ll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens, (long long)x->hq);
   SP_REQUIRE(x->workspace != nullptr && x->workspace_bytes >= s.bytes && (uintptr_t)x->workspace % 16 == 0, SP_ERR_WORKSPACE,
              "%s: workspace missing, too small or misaligned", who);
@@ -1068,7 +1070,7 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   const int64_t join = sp_ceil_div(x->tokens * x->hq * sets, SM_THREADS / (x->d / 4));
   SP_REQUIRE(join + (int64_t)grid * SH_WAVES <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens,
              (long long)x->hq);
-  a.apart = sh_apart(x->tokens, x->groups, g, x->weights != nullptr);
+  a.apart = apart;
   if (a.apart) {
     CkArgs c = {};
     c.q = a.q, c.k = a.k, c.v = a.v, c.table = a.table, c.lens = a.shared, c.cu = a.cu, c.groups = a.groups, c.o_row = a.o_row, c.ml_row = a.ml_row;

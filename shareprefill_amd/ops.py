@@ -858,7 +858,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
         raise ValueError(f"budget {budget} and recent {recent} must not be negative")
     stream = _stream_handle(dev)
     new_lens = torch.empty(batch, dtype=torch.int32, device=dev)
-    need = lib.sp_paged_evict_workspace_bytes(batch, hkv, pages, page_size, block_table.size(1))
+    need = lib.sp_paged_evict_workspace_bytes(batch, hkv, d, pages, page_size, block_table.size(1))
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
     w_p, w_h, _ = weights.stride()
     st = lib.sp_paged_evict_bf16(_lib.EVICT_ARGS.pack(

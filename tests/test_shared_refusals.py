@@ -71,7 +71,7 @@ def test_key_weights_refuse(code, kw):
     (-1, dict(batch=0)), (-2, dict(batch=4097)), (-1, dict(hkv=0)), (-1, dict(budget=-1)), (-1, dict(recent=-1)), (-2, dict(d=4)), (-2, dict(d=0)),
     (-2, dict(page_size=24)), (-2, dict(table_width=1 << 27)), (-1, dict(k_pages=0)), (-1, dict(v_pages=0)), (-1, dict(weights=0)), (-1, dict(block_table=0)),
     (-1, dict(seq_lens=0)), (-1, dict(new_lens=0)), (-1, dict(new_lens=P)), (-1, dict(first=P + 64)), (-2, dict(k_pages=P + 8)), (-2, dict(v_stride_slot=4)),
-    (-4, dict(workspace=0)), (-4, dict(workspace_bytes=100)), (-2, dict(num_pages=1 << 29))])
+    (-4, dict(workspace=0)), (-4, dict(workspace_bytes=100)), (-2, dict(num_pages=1 << 29)), (-2, dict(d=65544))])
 def test_eviction_refuses(code, kw):
     assert _evict(**kw) == code and "sp_paged_evict_bf16" in _message(), _message()
 
@@ -84,6 +84,6 @@ def test_nothing_to_do_is_no_error():
 def test_workspaces_of_calls_that_are_refused_are_none():
     lib = _lib.load()
     assert lib.sp_shared_attn_workspace_bytes(4, 4, 2, 8, 3, 128, 1, 0) == 0 and lib.sp_shared_attn_workspace_bytes(4, 2000, 2, 8, 2, 128, 1, 0) == 0
-    assert lib.sp_paged_key_weights_workspace_bytes(4, 0, 8, 2) == 0 and lib.sp_paged_evict_workspace_bytes(0, 2, 50, 16, 9) == 0
+    assert lib.sp_paged_key_weights_workspace_bytes(4, 0, 8, 2) == 0 and lib.sp_paged_evict_workspace_bytes(0, 2, 128, 50, 16, 9) == 0
     assert lib.sp_shared_attn_workspace_bytes(4, 4, 2, 8, 2, 128, 1, 800) > lib.sp_shared_attn_workspace_bytes(4, 4, 2, 8, 2, 128, 1, 0) > 0
-    assert lib.sp_paged_evict_workspace_bytes(4, 2, 50, 16, 9) == 8 * 2 * 50 * 16
+    assert lib.sp_paged_evict_workspace_bytes(4, 2, 128, 50, 16, 9) == 8 * 2 * 50 * 16 + 8 * 3 * 4 + 4 * 256
