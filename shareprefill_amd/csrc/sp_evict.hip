@@ -19,7 +19,7 @@
 #define EV_CHUNK (EV_THREADS * EV_RUN)
 #define EV_MAX_SHARES 16    // workgroups that share a kv head's keys
 #define EV_SLICE 512        // channels of a row that a workgroup moves
-#define EV_AHEAD 8          // rows of a thread
+#define EV_AHEAD 6          // rows of a thread
 #define EV_FEW 256          // workgroups that move: one a CU
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
@@ -69,13 +69,12 @@ struct EvPair {
   const int32_t* table;
   int kvh;
   EvRequest r;
+  int each, more;  // keys of a share; so many shares have one more
   __device__ __forceinline__ int64_t place(int j) const {  // of key j in the pages: of a kv head, of all of them where there are a.hkv side by side
     return ((int64_t)table[j >> a.shift] << a.shift) + (j & ((1 << a.shift) - 1));
   }
-  __device__ __forceinline__ uint64_t* entry(int i) const {
-    const int j = r.first + i;
-    return a.list + ((((int64_t)table[j >> a.shift] * a.hkv + kvh) << a.shift) + (j & ((1 << a.shift) - 1)));
-  }
+  __device__ __forceinline__ uint64_t* entry(int page, int j) const { return a.list + ((((int64_t)page * a.hkv + kvh) << a.shift) + (j & ((1 << a.shift) - 1))); }
+  __device__ __forceinline__ uint64_t* entry(int i) const { return entry(table[(r.first + i) >> a.shift], r.first + i); }
   // Patterns of keys j .. j + EV_RUN - 1 (j a multiple of EV_RUN); those outside lo .. hi - 1 are left as they are.  -> place of key j
   __device__ __forceinline__ uint32_t load(int j, int lo, int hi, uint32_t (&key)[EV_RUN]) const {
     if (j + EV_RUN <= lo || j >= hi) return 0u;
@@ -99,8 +98,7 @@ struct EvPair {
   }
   // keys of a share, from .. to
   __device__ __forceinline__ int share_start(int s) const {
-    const int64_t at = (int64_t)r.mid * s / a.shares;
-    return r.first + (int)at;
+    return r.first + each * s + pg_min(s, more);
   }
 };
 
@@ -198,7 +196,9 @@ __device__ __forceinline__ int ev_gather(const EvPair& p, int from, int to, uint
 
 __device__ __forceinline__ EvPair ev_pair(const EvArgs& a, int pair) {
   const int b = pair / a.hkv;
-  return EvPair{a, a.table + b * a.table_stride, pair % a.hkv, ev_request(a, b)};
+  const EvRequest r = ev_request(a, b);
+  const int each = a.shares > 1 ? (int)((unsigned)r.mid / (unsigned)a.shares) : r.mid;
+  return EvPair{a, a.table + b * a.table_stride, pair % a.hkv, r, each, r.mid - each * a.shares};
 }
 
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_hist_kernel(const EvArgs a) {
@@ -212,10 +212,12 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_hist_kernel(const EvArgs 
 // (a kv head's shares find the same bin)
 __device__ __forceinline__ EvBin ev_first_bin(const EvArgs& a, int pair, int keep, uint32_t* hist, int* wave_s, int* found_s) {
   for (int i = threadIdx.x; i < EV_BINS; i += EV_THREADS) {
-    uint32_t n = 0;
+    uint32_t part[EV_MAX_SHARES], n = 0;
 #pragma unroll
-    for (int x = 0; x < EV_MAX_SHARES; ++x)
-      if (x < a.shares) n += a.hists[((int64_t)pair * a.shares + x) * EV_BINS + i];
+    for (int x = 0; x < EV_MAX_SHARES; ++x) part[x] = a.hists[((int64_t)pair * a.shares + pg_min(x, a.shares - 1)) * EV_BINS + i];
+    __builtin_amdgcn_sched_barrier(0);  // (all on their way at once)
+#pragma unroll
+    for (int x = 0; x < EV_MAX_SHARES; ++x) n += x < a.shares ? part[x] : 0;
     hist[i] = n;
   }
   __syncthreads();
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_gather_kernel(const EvArg
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint64_t stage[];
   __shared__ uint32_t hist[EV_BINS];
-  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES], start_s[EV_MAX_SHARES];
+  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES], start_s[EV_MAX_SHARES], list_s[EV_MAX_SHARES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, pair = blockIdx.x, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   for (int part = 0; part <= 2 * a.slices; ++part) {
@@ -267,7 +269,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 #pragma unroll
     for (int s = 0; s < EV_MAX_SHARES; ++s) {
       const int n = s < a.shares ? count_s[s] : 0;
-      if (t == s) start_s[s] = listed;
+      if (t == s) start_s[s] = listed, list_s[s] = s < a.shares ? p.share_start(s) - p.r.first - listed : 0;
       listed += n;
     }
     __syncthreads();
@@ -283,7 +285,9 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
       for (int e = 0; e < EV_RUN; ++e) place[e] = first + e;
     } else {
       // (threads side by side read entries side by side, then each its own out of LDS)
+      // (pages, then entries: asked for one after the other each waits for the last)
       uint64_t x[EV_RUN];
+      int at[EV_RUN], page[EV_RUN];
 #pragma unroll
       for (int e = 0; e < EV_RUN; ++e) {
         const int i = pg_min(t + e * EV_THREADS, listed - 1);
@@ -291,8 +295,12 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 #pragma unroll
         for (int step = EV_MAX_SHARES / 2; step > 0; step /= 2)
           if (s + step < a.shares && start_s[s + step] <= i) s += step;
-        x[e] = *p.entry(p.share_start(s) - p.r.first + i - start_s[s]);
+        at[e] = p.r.first + list_s[s] + i;
+        page[e] = p.table[at[e] >> a.shift];
       }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int e = 0; e < EV_RUN; ++e) x[e] = *p.entry(page[e], at[e]);
 #pragma unroll
       for (int e = 0; e < EV_RUN; ++e) stage[t + e * EV_THREADS] = x[e];
       __syncthreads();
@@ -385,7 +393,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
   const int t = threadIdx.x, pairs = a.batch * a.hkv, stream = blockIdx.x % a.streams, pair = stream % pairs, part = stream / pairs, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   const EvRequest& r = p.r;
-  // (the look at the table has its entries at hand when the ticket comes: 30 us for 44 where the launch before this one had told what it says)
+  // (the look at the table brings its entries near while the ticket is on its way: 30 us for 44 where the launch before this one had told what it says)
   if (t == 0) chunk_s = __hip_atomic_fetch_add(a.tickets + stream, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   if (!(r.keep < r.mid && ev_has_pages(a, b, r))) return;
   const int chunk = chunk_s, rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
@@ -393,17 +401,24 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
     const int per = EV_THREADS / lanes, row = t / lanes;
     const int64_t i0 = (int64_t)chunk * (per * AHEAD);
     if (i0 >= rows) return;
-    decltype(type) y[AHEAD] = {};
-    uint32_t to[AHEAD];
+    // (a thread without a row reads the last one's.  Every row's page, then every row's source, then every row: asked for row by row each waits for the last)
+    decltype(type) y[AHEAD];
+    uint32_t to[AHEAD], come[AHEAD];
+    int last[AHEAD];  // page that a last key comes from
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int i = (int)i0 + u * per + row;
-      to[u] = 0;
-      if (row >= per || i >= rows) continue;
-      const int64_t goes = p.place(r.first + i);
-      const int64_t come = i < r.keep ? (int64_t)a.list[((((goes >> a.shift) * a.hkv + p.kvh) << a.shift) + (goes & in))] : p.place(r.first + r.mid + (i - r.keep));
-      to[u] = (uint32_t)goes;
-      y[u] = *at(come);
+      const int i = pg_min((int)i0 + u * per + row, rows - 1);
+      to[u] = (uint32_t)p.place(r.first + i);
+      last[u] = p.table[(r.first + r.mid + pg_max(i - r.keep, 0)) >> a.shift];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) come[u] = (uint32_t)a.list[(((int64_t)(to[u] >> a.shift) * a.hkv + p.kvh) << a.shift) + (to[u] & in)];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = pg_min((int)i0 + u * per + row, rows - 1);
+      y[u] = *at(i < r.keep ? come[u] : ((uint32_t)last[u] << a.shift) + ((r.first + r.mid + (i - r.keep)) & in));
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the chunk is read
@@ -442,8 +457,8 @@ struct EvMove {
   int64_t slices, streams, ahead, chunks;
 };
 // Chunks of `kept` rows at most, as many as the widest stream needs.  A thread has EV_AHEAD rows in flight, or one where few workgroups are enough all the same: us,
-// one / 2 / 4 / 8 / 16, eight kv heads' 320 rows of 128 channels 8 / 9 / 10 / 11 / 11, their 8192 rows 45 / 36 / 34 / 30 / 36, 64 kv heads' 2000 rows 67 / 50 / 44 /
-// 40 / 46.
+// one / 2 / 4 / 6 / 8, eight kv heads' 320 rows of 128 channels 7 / 9 / 10 / 11 / 11, their 8192 rows 45 / 34 / 31 / 29 / 30, 64 kv heads' 2000 rows 67 / 45 / 37 /
+// 36 / 38.
 static EvMove ev_move(int64_t pairs, int64_t d, int64_t kept) {
   EvMove m;
   m.slices = (d + EV_SLICE - 1) / EV_SLICE, m.streams = pairs * (2 * m.slices + 1);
