@@ -18,6 +18,7 @@
 #define EV_RUN 16           // keys of a thread, which lie in one page
 #define EV_CHUNK (EV_THREADS * EV_RUN)
 #define EV_MAX_SHARES 16    // workgroups that share a kv head's keys
+#define EV_TURN 10          // entries of a lane on their way
 #define EV_SLICE 512        // channels of a row that a workgroup moves
 #define EV_AHEAD 6          // rows of a thread
 #define EV_FEW 256          // workgroups that move: one a CU
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_gather_kernel(const EvArg
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint64_t stage[];
   __shared__ uint32_t hist[EV_BINS];
-  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES], start_s[EV_MAX_SHARES], list_s[EV_MAX_SHARES];
+  __shared__ int wave_s[2 * EV_WAVES], found_s[2], count_s[EV_MAX_SHARES], start_s[EV_MAX_SHARES];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, pair = blockIdx.x, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   for (int part = 0; part <= 2 * a.slices; ++part) {
@@ -269,7 +270,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 #pragma unroll
     for (int s = 0; s < EV_MAX_SHARES; ++s) {
       const int n = s < a.shares ? count_s[s] : 0;
-      if (t == s) start_s[s] = listed, list_s[s] = s < a.shares ? p.share_start(s) - p.r.first - listed : 0;
+      if (t == s) start_s[s] = listed;
       listed += n;
     }
     __syncthreads();
@@ -284,25 +285,24 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 #pragma unroll
       for (int e = 0; e < EV_RUN; ++e) place[e] = first + e;
     } else {
-      // (threads side by side read entries side by side, then each its own out of LDS)
-      // (pages, then entries: asked for one after the other each waits for the last)
-      uint64_t x[EV_RUN];
-      int at[EV_RUN], page[EV_RUN];
+      // Some waves a share, whose lanes read entries side by side; then every thread its own out of LDS.  (Pages, then entries: asked for one after the other
+      // each waits for the last.)
+      const int of = EV_WAVES / a.shares, s = wave / of, stride = of * SP_WAVE;
+      if (s < a.shares) {
+        const int count = count_s[s], base = p.share_start(s), to = start_s[s];
+        for (int i0 = wave % of * SP_WAVE + lane; i0 < count; i0 += EV_TURN * stride) {
+          int page[EV_TURN];
+          uint64_t x[EV_TURN];
 #pragma unroll
-      for (int e = 0; e < EV_RUN; ++e) {
-        const int i = pg_min(t + e * EV_THREADS, listed - 1);
-        int s = 0;
+          for (int e = 0; e < EV_TURN; ++e) page[e] = p.table[(base + pg_min(i0 + e * stride, count - 1)) >> a.shift];
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int step = EV_MAX_SHARES / 2; step > 0; step /= 2)
-          if (s + step < a.shares && start_s[s + step] <= i) s += step;
-        at[e] = p.r.first + list_s[s] + i;
-        page[e] = p.table[at[e] >> a.shift];
+          for (int e = 0; e < EV_TURN; ++e) x[e] = *p.entry(page[e], base + pg_min(i0 + e * stride, count - 1));
+#pragma unroll
+          for (int e = 0; e < EV_TURN; ++e)
+            if (i0 + e * stride < count) stage[to + i0 + e * stride] = x[e];
+        }
       }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int e = 0; e < EV_RUN; ++e) x[e] = *p.entry(page[e], at[e]);
-#pragma unroll
-      for (int e = 0; e < EV_RUN; ++e) stage[t + e * EV_THREADS] = x[e];
       __syncthreads();
 #pragma unroll
       for (int e = 0; e < EV_RUN; ++e)
