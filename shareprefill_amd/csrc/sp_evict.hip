@@ -18,6 +18,7 @@
 #define EV_RUN 16           // keys of a thread, which lie in one page
 #define EV_CHUNK (EV_THREADS * EV_RUN)
 #define EV_MAX_SHARES 16    // workgroups that share a kv head's keys
+#define EV_ONE 49152        // keys that one workgroup goes through at least
 #define EV_TURN 10          // entries of a lane on their way
 #define EV_SLICE 512        // channels of a row that a workgroup moves
 #define EV_AHEAD 6          // rows of a thread
@@ -122,7 +123,8 @@ __device__ __forceinline__ EvBin ev_find(const uint32_t* hist, int left, int* wa
   }
   if (lane == SP_WAVE - 1) wave_s[wave] = at;
   __syncthreads();
-  for (int x = 0; x < wave; ++x) at += wave_s[x];
+#pragma unroll
+  for (int x = 0; x < EV_WAVES; ++x) at += x < wave ? wave_s[x] : 0;
   at -= mine;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
@@ -446,10 +448,11 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
 }
 
 // ---- host -------------------------------------------------------------------------------------------------
-// Workgroups that share a kv head's keys: as many as fill the card, of some 8192 keys at least by what the table has room for.  One launch of one workgroup each
-// instead of three: us, one / 16 shares, a kv head's 2000 keys of 8 12 / 18, 8000 of 64 17 / 25, 131072 of 8 84 / 26.
+// Workgroups that share a kv head's keys, by what the table has room for: as many as fill the card, of some 8192 keys at least, where they pay for the two launches
+// more.  us for the whole call, one / shared, eight kv heads' 8000 keys 22 / 26, 20000 33 / 37, 32000 37 / 40, 65000 53 / 47, 131072 87 / 70; 64 kv heads' 20000
+// 43 / 50.
 static int ev_shares(int64_t pairs, int64_t room) {
-  const int64_t by_keys = room / 8192, by_card = 256 / pairs;
+  const int64_t by_keys = room < EV_ONE ? 1 : room / 8192, by_card = 256 / pairs;
   const int64_t n = by_keys < by_card ? by_keys : by_card;
   return n < 1 ? 1 : n > EV_MAX_SHARES ? EV_MAX_SHARES : (int)n;
 }

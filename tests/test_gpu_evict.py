@@ -99,7 +99,7 @@ def _fast(dev, n, budget, recent, first, weight, width=0, page=64, seed=0):
         assert torch.equal(place(x.cpu()), want)
 
 
-@pytest.mark.parametrize("n", [16384, 16385, 16400, 40000, 140000])
+@pytest.mark.parametrize("n", [16384, 16385, 16400, 40000, 60000, 140000])
 @pytest.mark.parametrize("first", [0, 5, 64])
 def test_long_requests(gpu_device, n, first):
     """Keys of a kv head that one workgroup's registers hold, and more, which are listed by one workgroup or by several."""
