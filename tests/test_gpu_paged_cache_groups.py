@@ -227,3 +227,79 @@ def test_a_captured_step_of_groups(gpu_device):
             cache.release(torch.tensor([False, True, False, False], device=gpu_device))
             cache.join(torch.tensor([False, True, False, False], device=gpu_device))
             assert cache.lens.tolist()[1] == 64
+
+
+def test_requests_of_a_group_that_share_nothing(gpu_device):
+    """A group's first row ends before the others, which keep its pages through evictions, and rows of the group take requests that share nothing."""
+    from shareprefill_amd import PagedKVCache
+
+    gen = torch.Generator().manual_seed(6)
+    hq, hkv, d, page, rows, scale = 8, 2, 64, 16, 4, default_scale(64)
+    cache = PagedKVCache(1, 60, hkv, d, rows, 300, page, device=gpu_device, group_sizes=[4], key_weights=True)
+    held = Held(1, rows, hkv, d)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu_device)
+    mask = lambda *r: torch.tensor([i in r for i in range(rows)], device=gpu_device)
+    front = [0] * rows  # keys in pages of several
+
+    def step(new=None, active=None):
+        singles = new is None
+        counts = [int(r in active) for r in range(rows)] if singles else new
+        total = rows if singles else sum(new)
+        tables = cache.begin_step(active=mask(*active)) if singles else cache.begin_step(ints(new), total)
+        assert tables.free_left.item() >= 0
+        q, k, v = (torch.randn(total, h, d, generator=gen).to(torch.bfloat16).transpose(0, 1) for h in (hq, hkv, hkv))
+        cache.write(0, k.to(gpu_device), v.to(gpu_device))
+        out, at = cache.attend(0, q.to(gpu_device), scale).cpu(), 0
+        if not singles:
+            cache.observe(0, q.to(gpu_device), scale, last=4)
+        for r, n in enumerate(counts):
+            mine = slice(r, r + n) if singles else slice(at, at + n)
+            if n:
+                held.add(r, 0, k[:, mine], v[:, mine])
+                check(out[mine], *reference(q[:, mine], *held.of[r][0][:2], scale, 0, 0), f"request {r}")
+                seen = q[:, mine] if singles else q[:, mine][:, -4:]
+                held.weigh(r, 0, seen, scale, front[r], singles)
+            at += n
+
+    def evict(budget, recent):
+        got = [_check_weights(cache, held, r, 0, front[r]) for r in range(rows)]
+        cache.evict(budget, recent)
+        for r in range(rows):
+            k, v, w, room = held.of[r][0]
+            n, first = k.shape[1], front[r]
+            mid = max(n - first - recent, 0)
+            keep = min(mid, budget)
+            stay = torch.tensor([list(range(first)) + sorted(first + i for i in sorted(range(mid), key=lambda i: (-got[r][h, first + i].item(), i))[:keep])
+                                 + list(range(first + mid, n)) for h in range(hkv)])
+            held.of[r] = [tuple(torch.stack([x[h, stay[h]] for h in range(hkv)]) for x in (k, v, w, room))]
+            assert cache.lens[r].item() == stay.shape[1]
+
+    step(new=[70, 0, 0, 0])
+    cache.share(0, 70)
+    front = [64] * rows
+    for r in (1, 2, 3):
+        held.of[r] = [tuple(x[:, :64].clone() for x in layer) for layer in held.of[0]]
+    step(new=[2, 30, 25, 1])
+    step(active=[0, 1, 2])
+    cache.release(mask(0, 3))
+    for r in (0, 3):
+        held.of[r], front[r] = held.empty(), 0
+    step(new=[150, 1, 3, 0])  # a request that shares nothing, in the first row
+    step(new=[1, 1, 1, 90])   # and in another one
+    for _ in range(3):
+        step(active=[0, 1, 2, 3])
+    evict(12, 5)
+    step(active=[0, 1, 2, 3])
+    cache.release(mask(2))
+    held.of[2] = held.empty()
+    cache.share(0, 16)  # of what the first row has now, to row 2 alone
+    front[0] = front[2] = 16
+    held.of[2] = [tuple(x[:, :16].clone() for x in layer) for layer in held.of[0]]
+    assert cache.lens[2].item() == 16
+    for _ in range(3):
+        step(active=[0, 1, 2, 3])
+    evict(3, 1)
+    step(active=[1, 2, 3])
+    step(new=[3, 4, 5, 6])
+    cache.release(torch.ones(rows, dtype=torch.bool, device=gpu_device))
+    assert cache.free_count.item() == 60

@@ -230,3 +230,24 @@ def test_a_captured_step(gpu_device):
         kept, replayed = weights.clone(), out.clone()
         weights.zero_()
         assert torch.equal(call(None), replayed) and torch.equal(weights, kept), "a replay differs from the eager call"
+
+
+@pytest.mark.parametrize("single", [True, False])
+def test_requests_that_have_not_joined(gpu_device, single):
+    """They go through all of their keys by themselves, though the group's are as long."""
+    from shareprefill_amd import ops
+
+    dev, (hq, hkv, d), page = gpu_device, (8, 2, 128), 16
+    gen = torch.Generator().manual_seed(12)
+    pools, table, lens, shared, cu, kv, prefix = make_shared([(64, [30, 20])], [90, 70], hkv, d, page, gen)
+    new = [1] * 4 if single else [2, 5, 3, 1]
+    q = torch.randn(sum(new), hq, d, generator=gen).to(torch.bfloat16).transpose(0, 1)
+    weights = torch.zeros(pools[0].shape[:3], device=dev) if single else None
+    # (all four rows are the group's; the last two share nothing with it)
+    out = ops.shared_prefix_attention(q.to(dev), pools[0].to(dev), pools[1].to(dev), table.to(dev), _ints(dev, lens), _ints(dev, shared), _ints(dev, [0, 4]),
+                                      default_scale(d), cu_q=None if single else _ints(dev, starts(new)), weights=weights, joined=_ints(dev, [64, 90, 63, -5]))
+    want, bound = references(q, kv, new, default_scale(d))
+    check(out, want, bound)
+    if single:
+        total = sum(hq - key_weights(q[:, b:b + 1], kv[b][0], default_scale(d))[:, :prefix[b]].sum().item() for b in range(4))
+        assert abs(weights.double().sum().item() - total) < 1e-3  # (8 rows of weights that sum to one, 2^-20 each at most)

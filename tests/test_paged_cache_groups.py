@@ -79,3 +79,32 @@ def test_refusals():
         cache.evict(4, 4)
     with pytest.raises(RuntimeError):
         cache.observe(0, torch.zeros(1, 1, 64), 0.1)
+
+
+def test_keys_in_pages_of_several_requests_stay_apart_behind_the_end_of_a_first_row():
+    cache = _cache()
+    _fill(cache, 0, 4, 60)
+    cache.dropped[0] = 7
+    cache.share(0, 50)
+    assert cache._held.tolist() == cache._joined.tolist() == [48, 48, 48, 0, 0, 0]
+    assert cache.dropped.tolist() == [7, 7, 7, 0, 0, 0]  # (positions go on from the first row's)
+    cache.release(_mask(0))
+    assert cache._held.tolist() == [0, 48, 48, 0, 0, 0] and cache._joined.tolist() == [0] * 6 and cache.dropped.tolist() == [0, 7, 7, 0, 0, 0]
+    _fill(cache, 0, 2, 32)
+    cache.share(0, 16)  # the others are not empty: they keep what they have and are none of this start's
+    assert cache.shared_lens.tolist() == [16, 0] and cache._joined.tolist() == [16, 0, 0, 0, 0, 0] and cache._held.tolist() == [16, 48, 48, 0, 0, 0]
+    assert cache.lens.tolist() == [32, 48, 48, 0, 0, 0] and cache.dropped.tolist() == [0, 7, 7, 0, 0, 0]
+    assert not set(cache.block_table[0, :2].tolist()) & set(cache.block_table[1, :3].tolist())
+    cache.release(_mask(2))
+    cache.join(_mask(1, 2))
+    assert cache.lens.tolist() == [32, 48, 16, 0, 0, 0] and cache._joined.tolist() == [16, 0, 16, 0, 0, 0]
+    _whole(cache)
+    cache.release(_mask(0, 1, 2))
+    assert cache.free_count.item() == 20 and cache._held.tolist() == [0] * 6
+
+
+def test_more_requests_than_groups_and_weights_take():
+    for kw in (dict(group_sizes=[2]), dict(group_sizes=None, key_weights=True)):
+        with pytest.raises(ValueError, match="1024"):
+            _cache(max_requests=1025, **kw)
+    assert _cache(max_requests=1025, group_sizes=None).max_requests == 1025

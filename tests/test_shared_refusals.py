@@ -9,7 +9,7 @@ P = 1 << 20  # an address, 16-byte aligned
 
 
 def _shared(**kw):
-    a = dict(q=P, k_pages=P, v_pages=P, block_table=P, seq_lens=P, cu_q=0, shared_lens=P, cu_groups=P, weights=P, out=P, workspace=P, workspace_bytes=1 << 40,
+    a = dict(q=P, k_pages=P, v_pages=P, block_table=P, seq_lens=P, cu_q=0, shared_lens=P, cu_groups=P, joined=0, weights=P, out=P, workspace=P, workspace_bytes=1 << 40,
              tokens=4, batch=4, groups=2, hq=8, hkv=2, d=128, num_pages=50, page_size=16, table_width=9, table_stride=9, q_stride_n=1024, q_stride_h=128,
              k_stride_page=4096, k_stride_slot=128, k_stride_h=2048, v_stride_page=4096, v_stride_slot=128, v_stride_h=2048, w_stride_page=32, w_stride_h=16,
              softmax_scale=0.1, stream=0)
