@@ -303,3 +303,31 @@ def test_requests_of_a_group_that_share_nothing(gpu_device):
     step(new=[3, 4, 5, 6])
     cache.release(torch.ones(rows, dtype=torch.bool, device=gpu_device))
     assert cache.free_count.item() == 60
+
+
+def test_new_keys_have_no_weight(gpu_device):
+    """Places that earlier owners left weights in: 0 until something attends to the key."""
+    from shareprefill_amd import PagedKVCache
+
+    gen = torch.Generator().manual_seed(7)
+    hq, hkv, d, page, rows, scale = 8, 2, 64, 16, 3, default_scale(64)
+    cache = PagedKVCache(2, 20, hkv, d, rows, 100, page, device=gpu_device, key_weights=True)
+    make = lambda n: [torch.randn(n, h, d, generator=gen).to(torch.bfloat16).to(gpu_device).transpose(0, 1) for h in (hq, hkv, hkv)]
+
+    def step(window, **kw):
+        tables = cache.begin_step(**kw)
+        for layer in range(2):
+            q, k, v = make(tables.slots.numel())
+            cache.write(layer, k, v)
+            cache.attend(layer, q, scale, window=window)
+
+    cache.weights.fill_(float("nan"))
+    step(None, new_lens=torch.tensor([20, 0, 35], dtype=torch.int32, device=gpu_device), max_new_tokens=60)
+    seen = lambda: [torch.stack([cache.weights[layer].cpu()[_places(cache, r, n)[0], :, _places(cache, r, n)[1]] for layer in range(2)])
+                    for r, n in enumerate(cache.lens.tolist())]
+    assert all((w == 0).all() for w in seen()) and cache.weights.isnan().sum().item() == 2 * hkv * (20 * page - 55)
+    step(10, active=torch.tensor([True, False, True], device=gpu_device))
+    assert [w.shape[1] for w in seen()] == [21, 0, 36] and all((w == 0).all() for w in seen())
+    step(None, active=torch.tensor([True, True, True], device=gpu_device))
+    for w in seen():  # the single tokens' weights sum to one a query head
+        assert (w.double().sum(1) - hq // hkv).abs().max() < 1e-4
