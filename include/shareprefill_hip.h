@@ -422,7 +422,7 @@ int sp_window_attn_bf16(const sp_window_attn_args* args /* host */);
 /* Attention of new tokens where requests have their first keys in common: as sp_paged_attn_bf16 without a window, the shared keys read once for a
  * whole group.  Group i is the sequences cu_groups[i] .. cu_groups[i + 1] (int32, groups + 1 of them, in order; sequences outside share
  * nothing); the first shared_lens[i] keys of each are those that the table row of its first sequence names.  A sequence with a new token at a place
- * in front of that sees to all of its keys by itself.  At most 1024 sequences.
+ * in front of that sees to all of its keys by itself, and so does sequence b with joined[b] < shared_lens[i] (null: none).  At most 1024 sequences.
  * weights (null, or fp32 [num_pages][hkv][page_size] with element strides for the page and head axes): for calls without cu_q and up to 16
  * query heads to a kv head.  For every sequence and each of its keys j that is not shared, at its place in the pages,
  *   weights[j] += sum over the query heads of the kv group of softmax(q . k)[j];
@@ -430,7 +430,7 @@ int sp_window_attn_bf16(const sp_window_attn_args* args /* host */);
  * single_tokens: for calls without cu_q; pool_keys: num_pages * page_size where weights are given, else 0. */
 typedef struct sp_shared_attn_args {
   const void *q, *k_pages, *v_pages;
-  const int32_t *block_table, *seq_lens, *cu_q, *shared_lens, *cu_groups;
+  const int32_t *block_table, *seq_lens, *cu_q, *shared_lens, *cu_groups, *joined;
   float* weights;
   void *out, *workspace;
   uint64_t workspace_bytes;

@@ -127,7 +127,7 @@ PAGED_WRITE_ARGS = struct.Struct("@5P15qP")
 PAGED_ATTN_ARGS = struct.Struct("@8PQ19qdP")
 WINDOW_ATTN_ARGS = struct.Struct("@5PQ17qdP")
 # sp_shared_attn_args, sp_paged_key_weights_args, sp_paged_evict_args
-SHARED_ATTN_ARGS = struct.Struct("@11PQ20qdP")
+SHARED_ATTN_ARGS = struct.Struct("@12PQ20qdP")
 KEY_WEIGHTS_ARGS = struct.Struct("@8PQ17qdP")
 EVICT_ARGS = struct.Struct("@8PQ17qP")
 

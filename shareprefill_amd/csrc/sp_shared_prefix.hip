@@ -29,7 +29,7 @@ struct ShRequest {
 };
 struct ShArgs {
   const sp_bf16 *q, *k, *v;
-  const int32_t *table, *lens, *cu, *shared, *groups;  // shared: keys of a group, [n_groups]; groups: first requests, [n_groups + 1]
+  const int32_t *table, *lens, *cu, *shared, *groups, *joined;  // shared: keys of a group, [n_groups]; groups: first requests, [n_groups + 1]
   sp_bf16* out;
   int64_t table_stride, sq_n, sq_h, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;  // elements; _p between pages
   int batch, tokens, width, num_pages, shift, n_groups;
@@ -106,7 +106,10 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   for (int i = t; i <= a.batch; i += SH_THREADS) {
     auto start = [&](int j) { return a.cu != nullptr ? pg_max(0, pg_min(a.cu[j], a.tokens)) : j; };
     start_s[i] = start(i);
-    if (i < a.batch) len_s[i] = pg_max(0, pg_min(a.lens[i], PG_MAX_KEYS)), back |= start(i + 1) < start(i);
+    if (i < a.batch) {
+      len_s[i] = pg_max(0, pg_min(a.lens[i], PG_MAX_KEYS)), back |= start(i + 1) < start(i);
+      first_s[i] = a.joined != nullptr ? a.joined[i] : PG_MAX_KEYS;  // (until the line is formed)
+    }
   }
   for (int i = a.n_groups > 0 ? t : 1; i <= a.n_groups; i += SH_THREADS) {
     auto first = [&](int j) { return pg_max(0, pg_min(a.groups[j], a.batch)); };
@@ -126,7 +129,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
     if (a.n_groups > 0) {
       const int i = pg_holder(group_s, a.n_groups, b);
       if (group_s[i] <= b && b < group_s[i + 1]) {
-        r.first_own = sh_first_own(len_s[b], start_s[b + 1] - r.start, shared_s[i]);
+        r.first_own = first_s[b] >= shared_s[i] ? sh_first_own(len_s[b], start_s[b + 1] - r.start, shared_s[i]) : 0;
         r.group = i, r.start0 = start_s[group_s[i]], r.end0 = start_s[group_s[i + 1]];
       }
     }
@@ -1037,7 +1040,7 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   char* const ws = (char*)x->workspace;
   ShArgs a = {};
   a.q = (const sp_bf16*)x->q, a.k = (const sp_bf16*)x->k_pages, a.v = (const sp_bf16*)x->v_pages;
-  a.table = x->block_table, a.lens = x->seq_lens, a.cu = x->cu_q, a.shared = x->shared_lens, a.groups = x->cu_groups;
+  a.table = x->block_table, a.lens = x->seq_lens, a.cu = x->cu_q, a.shared = x->shared_lens, a.groups = x->cu_groups, a.joined = x->joined;
   a.out = (sp_bf16*)x->out;
   a.table_stride = x->table_stride, a.sq_n = q_n, a.sq_h = q_h;
   a.sk_p = k_p, a.sk_n = x->k_stride_slot, a.sk_h = k_h, a.sv_p = v_p, a.sv_n = x->v_stride_slot, a.sv_h = v_h, a.sw_p = w_p, a.sw_h = w_h;

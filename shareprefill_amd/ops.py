@@ -734,12 +734,14 @@ def _check_weights(weights: torch.Tensor, pages: int, hkv: int, page_size: int, 
 
 def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                             shared_lens: torch.Tensor, cu_groups: torch.Tensor, softmax_scale: float, cu_q: Optional[torch.Tensor] = None,
-                            weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                            weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                            joined: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_attention (without a window) where groups of requests have their first keys in common, which are read once for a group instead of once
     for each of its requests.  Requests cu_groups[i] .. cu_groups[i + 1] - 1 are group i (int32 [G + 1], in order; requests outside share nothing;
     G may be 0), and the first shared_lens[i] keys (int32 [G]) of each of them are those in the pages that the block table names for the group's
     first request.  Usually their rows of the table name the same pages; a last one that is shared in part is a copy of everyone's own.  A request
-    with a new token at a place in front of its group's shared_lens takes no part and is computed by itself, so idle rows (seq_lens 0) do no harm.
+    with a new token at a place in front of its group's shared_lens takes no part and is computed by itself, so idle rows (seq_lens 0) do no harm; nor
+    does a request with joined[b] < shared_lens[i] (int32 [B]; None: all do).
 
     weights (fp32 [num_pages, Hkv, page_size] view, for single tokens in groups of up to 16 query heads): what attention each key has received.
     Every key that a request does not share gets, at its place in the pages, the sum of its softmax weights over the kv group's query heads added; the
@@ -747,7 +749,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     requests must not lie in one page then, but for shared ones.
 
     At most 1024 requests; head_dim 64 or 128; lengths, offsets and pages are read on the device.  Scratch memory, from torch's allocator, for the
-    call: 17 MB with 256 kv heads or fewer and 8 Hq (D + 2) bytes a token, with weights 4 Hq num_pages page_size beside it.
+    call: 52 MB at 128 channels with 256 kv heads or fewer (86 MB where groups have more than 256 rows), half of it at 64, 8 Hq (D + 2) bytes a token, and
+    with weights 4 Hq num_pages page_size.
 
     Precision: sums, maxima and partial results have 32 bits; probabilities enter the product with V as one bf16 value, as two where a request (or a
     group) has no more than 16 rows (tokens times query heads of a kv group).  A value that is not finite makes the rows that see it not finite, and
@@ -761,6 +764,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     _check_ints(dev, ("seq_lens", seq_lens, torch.int32, batch), ("shared_lens", shared_lens, torch.int32, groups),
                 ("cu_groups", cu_groups, torch.int32, groups + 1))
     _check_table(block_table, batch, dev)
+    if joined is not None:
+        _check_ints(dev, ("joined", joined, torch.int32, batch))
     if cu_q is not None:
         _check_ints(dev, ("cu_q", cu_q, torch.int32, batch + 1))
     elif n != batch:
@@ -781,7 +786,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     q_h, q_n, _ = q.stride()
     st = lib.sp_shared_attn_bf16(_lib.SHARED_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
-        shared_lens.data_ptr(), cu_groups.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(),
+        shared_lens.data_ptr(), cu_groups.data_ptr(), 0 if joined is None else joined.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(),
         0 if ws is None else ws.data_ptr(), need, n, batch, groups, hq, hkv, d, pages, page_size, block_table.size(1), block_table.stride(0), q_n,
         q_h, k_p, k_n, k_h, v_p, v_n, v_h, w_p, w_h, softmax_scale, stream))
     if st:
@@ -842,7 +847,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     A request with a key behind the first ones that has no page stays as it is.  Only pages of nothing but first keys may be shared.
 
     At most 4096 requests; head_dim a multiple of 8.  Scratch memory, from torch's allocator, for the call: 8 bytes a key and kv head
-    of the pools, and up to 2 MB."""
+    of the pools, up to 2 MB, and 12 bytes for every 384 keys (at 128 channels) and kv head that the table has room for."""
     lib = _lib.load()
     if k_pages.dim() != 4 or not k_pages.is_cuda:
         raise ValueError(f"k_pages must be [num_pages, Hkv, page_size, D] on the GPU, got {tuple(k_pages.shape)} on {k_pages.device}")

@@ -54,6 +54,8 @@ class PagedKVCache:
         sizes = list(group_sizes or [])
         if any(n < 1 for n in sizes) or sum(sizes) > max_requests:
             raise ValueError(f"group_sizes {sizes} must be at least 1 each and {max_requests} in all at most")
+        if (sizes or key_weights) and max_requests > 1024:
+            raise ValueError(f"max_requests {max_requests}: with group_sizes or key_weights there are at most 1024")
         starts = [sum(sizes[:i]) for i in range(len(sizes) + 1)]
         ints = lambda x, dtype: torch.tensor(x, dtype=dtype, device=dev)
         self._group_starts = starts
@@ -61,11 +63,16 @@ class PagedKVCache:
         self.shared_lens = torch.zeros(len(sizes), dtype=torch.int32, device=dev)
         group_of = [i for i, n in enumerate(sizes) for _ in range(n)]
         self._group_of = ints(group_of + [len(sizes)] * (max_requests - len(group_of)), torch.int64)  # (none: one past the last)
+        # keys at the front of a request that lie in pages of several, and that its group shares as long as the first row is there
+        self._held = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self._joined = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self._shared_dropped = torch.zeros(len(sizes) + 1, dtype=torch.int32, device=dev)
         self._holder = ints([starts[i] for i in group_of] + list(range(len(group_of), max_requests)), torch.int64)
         # what attention every key has received, by its place in the pages (None: not kept), and how many keys evictions have taken from a request
         self.weights = torch.zeros(num_layers, num_pages, num_kv_heads, page_size, dtype=torch.float32, device=dev) if key_weights else None
         self.dropped = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self._last = None  # of a step: rows of its requests' last tokens (observe)
+        self._fresh = None  # of a step: places that its tokens' keys come to
 
     def _check_mask(self, mask: torch.Tensor, name: str) -> None:
         if mask.dtype is not torch.bool or tuple(mask.shape) != (self.max_requests,) or mask.device != self.lens.device:
@@ -109,7 +116,7 @@ class PagedKVCache:
                 token = torch.arange(t.positions.numel(), dtype=torch.int32, device=self.lens.device)
                 row = torch.searchsorted(t.cu_new[1:], token, right=True).clamp_(max=self.max_requests - 1)
                 t = t._replace(positions=t.positions + torch.where(token < t.cu_new[-1:], self.dropped[row], 0))
-        self.tables, self._cu_q, self._last = t, None if singles else t.cu_new, None
+        self.tables, self._cu_q, self._last, self._fresh = t, None if singles else t.cu_new, None, None
         return t
 
     def _pools_of(self, layer: int):
@@ -120,25 +127,41 @@ class PagedKVCache:
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v: bf16 [Hkv, T, D] views of the step's tokens."""
         ops.paged_cache_write(k, v, *self._pools_of(layer), self.tables.slots)
+        if self.weights is not None and self._cu_q is not None:
+            self._clear_weights(layer)
+
+    def _clear_weights(self, layer: int) -> None:
+        """The step's new keys have received nothing yet, whatever an earlier owner of their places left."""
+        if self._fresh is None:
+            places, slots = self.num_pages * self.page_size, self.tables.slots
+            fresh = torch.zeros(places + 1, dtype=torch.bool, device=slots.device)
+            fresh[torch.where(slots < 0, places, slots).long()] = True
+            self._fresh = fresh[:-1].view(self.num_pages, 1, self.page_size)
+        self.weights[layer].masked_fill_(self._fresh, 0)
 
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, window: Optional[int] = None, sinks: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q: bf16 [Hq, T, D] view -> bf16 [T, Hq, D]: every new token over what its request has cached up to it (ops.paged_attention; with groups or
-        key_weights, where there is no window, ops.shared_prefix_attention).  A step of single tokens adds what they attend to to the keys' weights; one
-        with new_lens leaves them to observe, and so does one with a window."""
+        key_weights, where there is no window and a step brings few tokens, ops.shared_prefix_attention).  A step of single tokens adds what they attend to to the keys' weights; one
+        with new_lens leaves them to observe, and so does one with a window: its own keys' are 0 until then.  (What keys in pages of several requests have
+        received is not kept.)"""
         pools = self._pools_of(layer)
         if q.dim() == 3 and q.shape[1] != self.tables.slots.numel():
             raise ValueError(f"q has {q.shape[1]} rows, the step {self.tables.slots.numel()}")
-        if window is None and (self.shared_lens.numel() > 0 or self.weights is not None):
+        if window is None and (self.shared_lens.numel() > 0 or self.weights is not None) and not self._many_rows(q):
             return ops.shared_prefix_attention(q, *pools, self.block_table, self._seen_lens, self.shared_lens, self.cu_groups, softmax_scale,
                                                cu_q=self._cu_q, weights=self.weights[layer] if self.weights is not None and self._cu_q is None else None,
-                                               out=out)
+                                               out=out, joined=self._joined)
+        if self.weights is not None and self._cu_q is None:
+            self._clear_weights(layer)
         return ops.paged_attention(q, *pools, self.block_table, self._seen_lens, softmax_scale, cu_q=self._cu_q,
                                    window=window, sinks=sinks, out=out)
 
-    def _shared_of(self) -> torch.Tensor:
-        """int32 [max_requests]: keys that a request's group shares (0: it is in none)."""
-        return torch.cat((self.shared_lens, self.shared_lens.new_zeros(1)))[self._group_of]
+    def _many_rows(self, q: torch.Tensor) -> bool:
+        """Chunks of prompts: the kernel with matrix products' rate takes less time to read shared keys once a request than the other to read them once.
+        us, shared / paged, by rows (tokens x query heads of a kv head) a request: 16 of 32 heads over 8 behind 4096 keys 16: 38 / 63, 32: 51 / 64, 64: 69 / 66,
+        128: 100 / 72, 2048: 812 / 524; 4 behind 32768 keys 32: 60 / 93, 64: 105 / 97, 2048: 980 / 893; 16 of 14 over 2 behind 4096 28: 26 / 26, 56: 30 / 28."""
+        return self._cu_q is not None and q.dim() == 3 and q.shape[1] * q.shape[0] > 48 * self.max_requests * self.pools.shape[3]
 
     def _check_weights(self) -> torch.Tensor:
         if self.weights is None:
@@ -147,8 +170,8 @@ class PagedKVCache:
 
     def observe(self, layer: int, q: torch.Tensor, softmax_scale: float, last: int = 32, accumulate: bool = False) -> None:
         """Sets the keys' weights of the requests that bring tokens to what the last `last` tokens of each attend to (all of them, where it brings
-        fewer); accumulate: on top of what keys in front of those tokens have (ops.paged_key_weights).  q as for attend, behind write.  Keys that a group
-        shares have none."""
+        fewer); accumulate: on top of what keys in front of those tokens have (ops.paged_key_weights).  q as for attend, behind write.  Keys in pages of
+        several requests have none."""
         weights = self._check_weights()
         pools = self._pools_of(layer)
         if last < 1:
@@ -165,41 +188,48 @@ class PagedKVCache:
                 source = (cu[1:][row] - count[row] + token - starts[row]).clamp_(0, max(q.shape[1] - 1, 0))
                 self._last = (last, starts, source)
             cu, q = self._last[1], q.transpose(0, 1).index_select(0, self._last[2]).transpose(0, 1)
-        ops.paged_key_weights(q, pools[0], self.block_table, self._seen_lens, softmax_scale, weights[layer], cu_q=cu, first=self._shared_of(),
+        ops.paged_key_weights(q, pools[0], self.block_table, self._seen_lens, softmax_scale, weights[layer], cu_q=cu, first=self._held,
                               accumulate=accumulate)
 
     def share(self, group: int, tokens: int) -> None:
-        """The first `tokens` keys of the group's first row, as many as fill whole pages, become those of all its rows: the others, which must be empty,
-        begin behind them.  The first row must have them cached; it may go on as a request of its own, and its end is the end of the sharing (release)."""
+        """The first `tokens` keys of the group's first row, as many as fill whole pages, become those of all its rows: the others begin behind them, if they
+        are empty.  The first row must have them cached; it may go on as a request of its own, and its end is the end of the sharing (release)."""
         if not 0 <= group < self.shared_lens.numel():
             raise ValueError(f"there are {self.shared_lens.numel()} groups, no group {group}")
         if not 0 <= tokens <= self.block_table.shape[1] * self.page_size:
             raise ValueError(f"{tokens} tokens are none that a request can have")
         first, end = self._group_starts[group:group + 2]
-        self.shared_lens[group:group + 1].fill_(tokens // self.page_size * self.page_size)
+        whole = tokens // self.page_size * self.page_size
+        self.shared_lens[group:group + 1].fill_(whole)
+        self._joined[first:first + 1].fill_(whole)
+        self._held[first:first + 1].clamp_(min=whole)
+        self._shared_dropped[group:group + 1].copy_(self.dropped[first:first + 1])
         rows = torch.zeros(self.max_requests, dtype=torch.bool, device=self.lens.device)
         rows[first + 1:end] = True
         self.join(rows)
 
     def join(self, rows: torch.Tensor) -> None:
-        """Rows (bool [max_requests], empty ones, as release leaves them) begin behind what their group shares; a group's first row stays as it is."""
+        """Rows (bool [max_requests]) that are empty, as release leaves them, begin behind what their group shares; others stay as they are, a group's first
+        row too.  (An empty row of a group may as well take a request that shares nothing, without joining.)"""
         self._check_mask(rows, "rows")
-        rows = rows & (self._holder != torch.arange(self.max_requests, device=self._holder.device))
-        shared = self._shared_of()
+        rows = rows & (self.lens == 0) & (self._holder != torch.arange(self.max_requests, device=self._holder.device))
+        shared = torch.cat((self.shared_lens, self.shared_lens.new_zeros(1)))[self._group_of]
         place = torch.arange(self.block_table.shape[1], device=self.lens.device)[None, :]
         named = torch.where(place * self.page_size < shared[:, None], self.block_table[self._holder], -1)
         self.block_table.copy_(torch.where(rows[:, None], named, self.block_table))
-        self.lens.copy_(torch.where(rows, shared, self.lens))
+        for x in (self.lens, self._held, self._joined):
+            x.copy_(torch.where(rows, shared, x))
+        self.dropped.copy_(torch.where(rows, self._shared_dropped[self._group_of], self.dropped))
 
     def evict(self, budget: int, recent: int, sinks: int = 0, rows: Optional[torch.Tensor] = None) -> None:
         """Drops keys of requests (rows bool [max_requests]; None: all) that hold more than they may, in every layer and kv head by itself: the first
-        `sinks` and what a group shares stay, the last `recent`, and of the others the `budget` heaviest (ops.paged_evict).  Their pages go back.
+        `sinks` and those in pages of several requests stay, the last `recent`, and of the others the `budget` heaviest (ops.paged_evict).  Their pages go back.
         A window of attend counts places in the cache, which later keys of such a request have nearer to each other than their positions."""
         weights = self._check_weights()
         if rows is not None:
             self._check_mask(rows, "rows")
         lens = self.lens if rows is None else self.lens * rows
-        first = torch.clamp(self._shared_of(), min=sinks)
+        first = torch.clamp(self._held, min=sinks)
         left = lens
         for layer in range(self.pools.shape[0]):
             left = ops.paged_evict(*self.pools[layer].unbind(0), weights[layer], self.block_table, lens, budget, recent, first=first)
@@ -233,6 +263,8 @@ class PagedKVCache:
         self._check_mask(finished, "finished")
         self._give_back(finished[:, None].expand_as(self.block_table))
         self.lens.masked_fill_(finished, 0)
-        self.dropped.masked_fill_(finished, 0)
+        for x in (self.dropped, self._held, self._joined):
+            x.masked_fill_(finished, 0)
         if self.shared_lens.numel() > 0:
             self.shared_lens.masked_fill_(finished[self.cu_groups[:-1].long()], 0)
+            self._joined.masked_fill_(finished[self._holder], 0)
