@@ -1031,7 +1031,7 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   for (const int64_t n : {x->k_stride_slot, x->v_stride_slot})
     SP_REQUIRE(n >= 0 && n < (1ll << 24) && n * x->page_size < (1ll << 30) && n % 8 == 0, SP_ERR_UNSUPPORTED, "%s: slot stride %lld unsupported", who,
                (long long)n);
-  const bool apart = sh_apart(x->tokens, x->groups, x->hq, x->hkv, x->d, x->table_width << shift, x->weights != nullptr);
+  const bool apart = sh_apart(x->tokens, x->groups, x->hq, x->hkv, x->table_width << shift, x->weights != nullptr);
   const ShSizes s = sh_sizes(x->tokens, x->batch, x->groups, x->hq, x->hkv, x->d, x->cu_q == nullptr,
                              x->weights != nullptr ? x->num_pages << shift : 0, apart);
   SP_REQUIRE(s.slots <= 0x7ffffff0ll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens, (long long)x->hq);

@@ -14,9 +14,8 @@ def _ints(dev, x):
 
 
 def _room(table, tokens, heads, page):
-    """The table, wide enough for tokens x heads x channels x keys to pass 5e9; what lies behind a request's pages is never read."""
-    hq, _, d = heads
-    width = max(table.shape[1], int(5.1e9 / (tokens * hq * d * page)) + 1)
+    """The table, wide enough for tokens x heads x keys to pass 5e7; what lies behind a request's pages is never read."""
+    width = max(table.shape[1], int(5.1e7 / (tokens * heads[0] * page)) + 1)
     assert width * page < 1 << 26
     return torch.cat((table, torch.full((table.shape[0], width - table.shape[1]), 1 << 30, dtype=torch.int32)), 1)
 
