@@ -5,9 +5,12 @@
 // floats without a sign are ordered as their patterns are: a histogram of the patterns' upper 11 bits says which of its bins T lies in; the keys of that
 // bin and of those above it are listed in order, some hundredths more than stay; and two histograms of 10 bits over the list find T and what of it goes.
 // So the weights are read twice, by as many workgroups as a kv head's keys are shared out to, and the list by one.  Moving is a gather in place: a kept key
-// comes from its place or further back, so rows are moved front to back in tiles that are read before they are written, by one workgroup, and what other rows
-// still need is never overwritten.  Rows are cut across instead, into as many slices as fill the card.
-// Moving is HBM-bound where there are many kv heads in all, kept rows once in and out; one request's is latency: chains of three loads, a tile after the other.
+// comes from its place or further back, so that a row may be written once the rows in front of it have been read.  Chunks of rows are read all at a time, by a
+// workgroup each, and written behind a wait for the chunks in front (sp_evict_move_kernel).
+// Moving is HBM-bound where there are many kv heads in all, kept rows once in and out; one request's is latency: chains of three loads.
+//
+// Measured, 128 channels, on rows that have not been moved before: 16 requests of up to 8001 keys, 4 kv heads, 2064 rows left, 133 MB: choosing 15 us, moving 36, 3.7 TB/s;
+// one of 131072 keys, 8 kv heads, 8192 left: two reads of the weights 6 and 10, choosing 20, moving 29; one of 2000, 320 left: choosing 14, moving 7.
 #include "sp_common.h"
 #include "sp_paged_plan.h"
 
@@ -287,22 +290,24 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 #pragma unroll
       for (int e = 0; e < EV_RUN; ++e) place[e] = first + e;
     } else {
-      // Some waves a share, whose lanes read entries side by side; then every thread its own out of LDS.  (Pages, then entries: asked for one after the other
-      // each waits for the last.)
-      const int of = EV_WAVES / a.shares, s = wave / of, stride = of * SP_WAVE;
-      if (s < a.shares) {
-        const int count = count_s[s], base = p.share_start(s), to = start_s[s];
-        for (int i0 = wave % of * SP_WAVE + lane; i0 < count; i0 += EV_TURN * stride) {
+      // A wave has as many entries as any, of one share or of several, and lanes side by side read entries side by side; then every thread its own out of LDS.
+      // (Pages, then entries: asked for one after the other each waits for the last.)
+      const int r0 = listed * wave / EV_WAVES, r1 = listed * (wave + 1) / EV_WAVES;
+      const int starts = lane < a.shares ? start_s[lane] : 0, ends = lane < a.shares ? starts + count_s[lane] : 0;
+      for (uint64_t of = __ballot(starts < r1 && ends > r0); of != 0ull; of &= of - 1ull) {
+        const int s = __builtin_ctzll(of), start = __builtin_amdgcn_readlane(starts, s), base = p.share_start(s) - start;
+        const int lo = pg_max(r0, start), hi = pg_min(r1, __builtin_amdgcn_readlane(ends, s));
+        for (int i0 = lo; i0 < hi; i0 += EV_TURN * SP_WAVE) {
           int page[EV_TURN];
           uint64_t x[EV_TURN];
 #pragma unroll
-          for (int e = 0; e < EV_TURN; ++e) page[e] = p.table[(base + pg_min(i0 + e * stride, count - 1)) >> a.shift];
+          for (int e = 0; e < EV_TURN; ++e) page[e] = p.table[(base + pg_min(i0 + e * SP_WAVE + lane, hi - 1)) >> a.shift];
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int e = 0; e < EV_TURN; ++e) x[e] = *p.entry(page[e], base + pg_min(i0 + e * stride, count - 1));
+          for (int e = 0; e < EV_TURN; ++e) x[e] = *p.entry(page[e], base + pg_min(i0 + e * SP_WAVE + lane, hi - 1));
 #pragma unroll
           for (int e = 0; e < EV_TURN; ++e)
-            if (i0 + e * stride < count) stage[to + i0 + e * stride] = x[e];
+            if (i0 + e * SP_WAVE + lane < hi) stage[i0 + e * SP_WAVE + lane] = x[e];
         }
       }
       __syncthreads();
