@@ -862,7 +862,11 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
   const int t = threadIdx.x, lane = t & 63, hq = a.hkv * a.group, kvh = w % a.hkv, part = w / a.hkv;
   const int4 cut = a.cuts[part];
   const int room = a.width << a.shift;
-  for (int b = pg_max(cut.x, 0); b < a.batch && b <= cut.z; ++b) {
+  // the part's requests side by side: for each all waves, two or one (each is a chain of six loads: 12 us one after the other)
+  const int b0 = pg_max(cut.x, 0), span = pg_min(cut.w > 0 ? cut.z : cut.z - 1, a.batch - 1) - b0 + 1;
+  const int waves = span <= 1 ? SM_THREADS / SP_WAVE : span == 2 ? SM_THREADS / SP_WAVE / 2 : 1, threads = waves * SP_WAVE;
+  for (int i = __builtin_amdgcn_readfirstlane(t / threads); i < span; i += SM_THREADS / threads) {
+    const int b = b0 + i;
     const ShRequest r = a.of_request[b];
     const int len = pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS));
     const int lo = r.first_own / SH_KEYS, keys = pg_min(len, room);
@@ -904,8 +908,8 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
     }
     const int first = (lo + begin) * SH_KEYS, last = (int)pg_min((int)(lo + end < keys / SH_KEYS + 1 ? (lo + end) * SH_KEYS : keys), keys);
     // (all lanes go through the loop together: they hold the heads' maxima and sums for each other)
-    for (int at = first; at < last; at += 4 * SM_THREADS) {
-      const int key = at + 4 * t, in = key & ((1 << a.shift) - 1), page = pg_min(key >> a.shift, a.width - 1);
+    for (int at = first; at < last; at += 4 * threads) {
+      const int key = at + 4 * (t % threads), in = key & ((1 << a.shift) - 1), page = pg_min(key >> a.shift, a.width - 1);
       int id = a.table[b * a.table_stride + page];
       const bool there = key < last && (unsigned)id < (unsigned)a.num_pages;
       id = there ? id : 0;
