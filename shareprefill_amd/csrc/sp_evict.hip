@@ -25,6 +25,7 @@
 #define EV_TURN 10          // entries of a lane on their way
 #define EV_SLICE 512        // channels of a row that a workgroup moves
 #define EV_AHEAD 6          // rows of a thread
+#define EV_POLLS (1 << 20)
 #define EV_FEW 256          // workgroups that move: one a CU
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
@@ -431,9 +432,10 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
     __syncthreads();  // the chunk is read
     int32_t* const done = a.done + (int64_t)stream * a.chunks;
     if (t == 0) __hip_atomic_store(done + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // (some microseconds; the bound, of a second, is for a workspace that something else writes to meanwhile)
     if (t < SP_WAVE)
       for (int i = t; i < chunk; i += SP_WAVE)
-        while (__hip_atomic_load(done + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0) __builtin_amdgcn_s_sleep(1);
+        for (int polls = 0; polls < EV_POLLS && __hip_atomic_load(done + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0; ++polls) __builtin_amdgcn_s_sleep(1);
     asm volatile("" ::: "memory");
     __syncthreads();
 #pragma unroll
