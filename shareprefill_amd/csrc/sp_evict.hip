@@ -364,7 +364,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
     left = f.left;
   }
   // `left` of those equal to T stay.  The list becomes where they come from, in place: an entry is written at or in front of where it was read.
-  int kept = 0, equal = 0;  // in front of this round
+  int kept = 0, equal = 0;  // in front of this turn
   for (int s = 0; s < a.shares; ++s) {
     const int base = p.share_start(s) - p.r.first;
     for (int i0 = 0; i0 < count_s[s]; i0 += EV_THREADS) {
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
       const bool over = there && key > top, same = there && key == top;
       const uint64_t overs = __ballot(over), sames = __ballot(same), below = (1ull << lane) - 1ull;
       if (lane == 0) wave_s[wave] = __builtin_popcountll(overs), wave_s[EV_WAVES + wave] = __builtin_popcountll(sames);
-      __syncthreads();  // (the round's entries are read)
+      __syncthreads();  // (the turn's entries are read)
       int over_at = 0, same_at = equal, overs_all = 0, sames_all = 0;
 #pragma unroll
       for (int y = 0; y < EV_WAVES; ++y) {
