@@ -401,9 +401,10 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
   const int t = threadIdx.x, pairs = a.batch * a.hkv, stream = blockIdx.x % a.streams, pair = stream % pairs, part = stream / pairs, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   const EvRequest& r = p.r;
+  if (r.keep >= r.mid) return;
   // (the look at the table brings its entries near while the ticket is on its way: 30 us for 44 where the launch before this one had told what it says)
   if (t == 0) chunk_s = __hip_atomic_fetch_add(a.tickets + stream, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (!(r.keep < r.mid && ev_has_pages(a, b, r))) return;
+  if (!ev_has_pages(a, b, r)) return;
   const int chunk = chunk_s, rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
   auto move = [&](auto type, int lanes, auto at) {  // elements of a row side by side, one a thread
     const int per = EV_THREADS / lanes, row = t / lanes;
