@@ -752,8 +752,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     call: 52 MB at 128 channels with 256 kv heads or fewer (86 MB where groups have more than 256 rows), half of it at 64, 8 Hq (D + 2) bytes a token, and
     with weights 4 Hq num_pages page_size.
 
-    Precision: sums, maxima and partial results have 32 bits; probabilities enter the product with V as one bf16 value, as two where a request (or a
-    group) has no more than 16 rows (tokens times query heads of a kv group).  A value that is not finite makes the rows that see it not finite, and
+    Precision: sums, maxima and partial results have 32 bits; probabilities enter the product with V as one bf16 value, as two over the own keys of
+    single tokens with up to 16 query heads a kv head.  A value that is not finite makes the rows that see it not finite, and
     no others."""
     lib = _lib.load()
     _check_hnd(q, "q")
