@@ -418,7 +418,7 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
     for (int u = 0; u < AHEAD; ++u) {
       const int i = pg_min((int)i0 + u * per + row, rows - 1);
       to[u] = (uint32_t)p.place(r.first + i);
-      last[u] = p.table[(r.first + r.mid + pg_max(i - r.keep, 0)) >> a.shift];
+      last[u] = p.table[pg_min(r.first + r.mid + pg_max(i - r.keep, 0), r.len - 1) >> a.shift];  // (there may be no last keys)
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

@@ -177,3 +177,10 @@ def test_a_replayed_eviction(gpu_device):
         torch.cuda.synchronize()
         want, lefts = definition([x.cpu() for x in start], table.cpu(), n, None, 60, 10, page)
         assert left.tolist() == lefts and all(torch.equal(x.cpu(), y) for x, y in zip((k, v, w), want))
+
+
+def test_a_table_that_is_full_to_its_last_place(gpu_device):
+    """No last keys that stay, in requests as long as the table has room for."""
+    for first in ([0, 0], [16, 5]):
+        _run(gpu_device, [64, 64], 20, 0, first=first)
+        _run(gpu_device, [1024, 1000], 700, 0, first=first, page=16)
