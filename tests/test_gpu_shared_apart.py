@@ -138,3 +138,22 @@ def test_a_captured_step(gpu_device):
         eager = torch.zeros_like(out)
         call(eager)
         assert torch.equal(eager, out)
+
+
+def test_offsets_that_go_back(gpu_device):
+    """An offset counts as the largest in front of it: tokens that two requests seem to have are the first one's, and so is their group."""
+    hq, hkv, d = heads = (8, 2, 128)
+    gen = torch.Generator().manual_seed(34)
+    pools, table, lens, shared, cu, kv, _ = make_shared([(64, [40, 30]), (96, [50] * 8)], [60], hkv, d, 16, gen)
+    offsets = [0, 30, 22, 60, 50, 80, 90, 100, 110, 150, 160, 162]
+    new, top = [], 0
+    for a, b in zip(offsets, offsets[1:]):
+        top = max(top, a)
+        new.append(max(b - top, 0))
+    q = torch.randn(162, hq, d, generator=gen).to(torch.bfloat16).transpose(0, 1)
+    from shareprefill_amd import ops
+    out = ops.shared_prefix_attention(q.to(gpu_device), pools[0].to(gpu_device), pools[1].to(gpu_device), _room(table, 162, heads, 16).to(gpu_device),
+                                      _ints(gpu_device, lens), _ints(gpu_device, shared), _ints(gpu_device, cu), default_scale(d), cu_q=_ints(gpu_device, offsets))
+    assert len(new) == 11 and sum(new) == 162
+    want, bound = references(q, kv, new, default_scale(d))
+    check(out, want, bound)
