@@ -207,11 +207,25 @@ __device__ __forceinline__ void ck_attend(const CkArgs& a) {
       cu_s[i] = start;
       if (i < a.batch) len_s[i] = GROUPS ? pg_min(ck_len(a, i), a.width << a.shift) : ck_len(a, i), back |= start_at(i + 1) < start;
     }
+    if constexpr (GROUPS) {
+      if (a.cu != nullptr)
+        for (int i = t; i < a.n_seqs; i += THREADS) back |= ck_start(a, i + 1) < ck_start(a, i);
+    }
     // Searches need the offsets in order, and must all find the same: notes of row tiles that only some of them find stay unwritten, and the
     // merging launch would read where they happen to point.  An offset that goes back counts as the largest in front of it.
     if (__syncthreads_or(back)) {
-      if (t == 0)
-        for (int i = 1; i <= a.batch; ++i) cu_s[i] = pg_max(cu_s[i], cu_s[i - 1]);
+      if (t == 0) {
+        if constexpr (GROUPS) {  // (of the requests' offsets, up to each group's first one)
+          int b = 0, at = 0;
+          for (int i = 0; i <= a.batch; ++i) {
+            const int first = pg_max(0, pg_min(a.groups[i], a.n_seqs));
+            for (; b <= first; ++b) at = pg_max(at, a.cu != nullptr ? ck_start(a, b) : b);
+            cu_s[i] = at;
+          }
+        } else {
+          for (int i = 1; i <= a.batch; ++i) cu_s[i] = pg_max(cu_s[i], cu_s[i - 1]);
+        }
+      }
       __syncthreads();
     }
     // every thread some row tiles in a row: their units, then the line's prefix sums
