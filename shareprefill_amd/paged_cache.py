@@ -135,7 +135,7 @@ class PagedKVCache:
         if self._fresh is None:
             places, slots = self.num_pages * self.page_size, self.tables.slots
             fresh = torch.zeros(places + 1, dtype=torch.bool, device=slots.device)
-            fresh[torch.where(slots < 0, places, slots).long()] = True
+            fresh.index_fill_(0, torch.where(slots < 0, places, slots).long(), True)
             self._fresh = fresh[:-1].view(self.num_pages, 1, self.page_size)
         self.weights[layer].masked_fill_(self._fresh, 0)
 

@@ -331,3 +331,44 @@ def test_new_keys_have_no_weight(gpu_device):
     step(None, active=torch.tensor([True, True, True], device=gpu_device))
     for w in seen():  # the single tokens' weights sum to one a query head
         assert (w.double().sum(1) - hq // hkv).abs().max() < 1e-4
+
+
+def test_a_captured_step_of_chunks(gpu_device):
+    """A step of several tokens a request with its keys' weights, recorded once: every replay leaves what an eager twin has."""
+    from shareprefill_amd import PagedKVCache
+
+    gen = torch.Generator().manual_seed(8)
+    hq, hkv, d, page, rows, most, scale = 8, 2, 64, 16, 4, 60, default_scale(64)
+    caches = [PagedKVCache(1, 60, hkv, d, rows, 200, page, device=gpu_device, group_sizes=[3], key_weights=True) for _ in range(2)]
+    q, k, v = (torch.zeros(most, h, d, dtype=torch.bfloat16, device=gpu_device).transpose(0, 1) for h in (hq, hkv, hkv))
+    new, out = torch.zeros(rows, dtype=torch.int32, device=gpu_device), torch.zeros(most, hq, d, dtype=torch.bfloat16, device=gpu_device)
+
+    def step(cache, to):
+        cache.begin_step(new, most)
+        cache.write(0, k, v)
+        cache.attend(0, q, scale, out=to)
+        cache.observe(0, q, scale, last=5, accumulate=True)
+
+    step(caches[0], out)  # (nobody brings anything)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(caches[0], out)
+    for i, counts in enumerate(([40, 0, 0, 7], [3, 20, 9, 1], [1, 2, 3, 4], [0, 5, 30, 25], [1, 1, 1, 1])):
+        new.copy_(torch.tensor(counts, dtype=torch.int32))
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape[1], x.shape[0], d, generator=gen).to(torch.bfloat16).transpose(0, 1))
+        twin = torch.zeros_like(out)
+        graph.replay()
+        torch.cuda.synchronize()
+        step(caches[1], twin)
+        n = sum(counts)
+        assert torch.equal(out[:n], twin[:n]), counts
+        assert torch.equal(caches[0].weights, caches[1].weights) and torch.equal(caches[0].block_table, caches[1].block_table)
+        assert torch.equal(caches[0].lens, caches[1].lens) and torch.equal(caches[0].pools, caches[1].pools)
+        if i == 0:
+            for c in caches:
+                c.share(0, 33)
+        if i == 2:
+            for c in caches:
+                c.evict(8, 4)
