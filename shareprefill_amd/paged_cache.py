@@ -67,6 +67,7 @@ class PagedKVCache:
         self._held = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self._joined = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self._shared_dropped = torch.zeros(len(sizes) + 1, dtype=torch.int32, device=dev)
+        self._in_place = torch.zeros(max_requests, dtype=torch.int32, device=dev)  # of what has dropped some: keys at its front in front of all of them
         self._holder = ints([starts[i] for i in group_of] + list(range(len(group_of), max_requests)), torch.int64)
         # what attention every key has received, by its place in the pages (None: not kept), and how many keys evictions have taken from a request
         self.weights = torch.zeros(num_layers, num_pages, num_kv_heads, page_size, dtype=torch.float32, device=dev) if key_weights else None
@@ -203,7 +204,8 @@ class PagedKVCache:
         self.shared_lens[group:group + 1].fill_(whole)
         self._joined[first:first + 1].fill_(whole)
         self._held[first:first + 1].clamp_(min=whole)
-        self._shared_dropped[group:group + 1].copy_(self.dropped[first:first + 1])
+        # (keys in front of all that evictions have taken stand where they stood in the prompt)
+        self._shared_dropped[group:group + 1].copy_(self.dropped[first:first + 1] * (self._in_place[first:first + 1] < whole))
         rows = torch.zeros(self.max_requests, dtype=torch.bool, device=self.lens.device)
         rows[first + 1:end] = True
         self.join(rows)
@@ -219,7 +221,7 @@ class PagedKVCache:
         self.block_table.copy_(torch.where(rows[:, None], named, self.block_table))
         for x in (self.lens, self._held, self._joined):
             x.copy_(torch.where(rows, shared, x))
-        self.dropped.copy_(torch.where(rows, self._shared_dropped[self._group_of], self.dropped))
+        self.dropped.copy_(torch.where(rows & (shared > 0), self._shared_dropped[self._group_of], self.dropped))
 
     def evict(self, budget: int, recent: int, sinks: int = 0, rows: Optional[torch.Tensor] = None) -> None:
         """Drops keys of requests (rows bool [max_requests]; None: all) that hold more than they may, in every layer and kv head by itself: the first
@@ -235,6 +237,8 @@ class PagedKVCache:
             left = ops.paged_evict(*self.pools[layer].unbind(0), weights[layer], self.block_table, lens, budget, recent, first=first)
         if rows is not None:
             left = torch.where(rows, left, self.lens)
+        in_front = torch.where(self.dropped > 0, torch.minimum(self._in_place, first), first)
+        self._in_place.copy_(torch.where(left < self.lens, in_front, self._in_place))
         self.dropped += self.lens - left
         self.lens.copy_(left)
         place = torch.arange(self.block_table.shape[1], device=left.device)[None, :]
@@ -266,5 +270,7 @@ class PagedKVCache:
         for x in (self.dropped, self._held, self._joined):
             x.masked_fill_(finished, 0)
         if self.shared_lens.numel() > 0:
-            self.shared_lens.masked_fill_(finished[self.cu_groups[:-1].long()], 0)
+            ended = finished[self.cu_groups[:-1].long()]
+            self.shared_lens.masked_fill_(ended, 0)
+            self._shared_dropped[:-1].masked_fill_(ended, 0)
             self._joined.masked_fill_(finished[self._holder], 0)
