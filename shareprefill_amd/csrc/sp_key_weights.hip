@@ -269,8 +269,9 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
         const int key0 = (from + block) * KW_BLOCK + wave * KW_KEYS;
         const bool edge = key0 + KW_KEYS - 1 > pos0 + (int)pg_div((unsigned)row0, a.by_group) || (cur.ids.id[0] | cur.ids.id[1]) < 0;  // some row does not see some key
         float acc[2][4] = {{0.f}};
-        // the products of row tiles i and i + 1: keys 16 h + 4 gr + j of row lq
+        // the products of row tiles i and i + 1: keys 16 h + 4 gr + j of row lq.  -> where `edge`: bit 8 u + 4 h + j says that row lq of tile i + u sees that key
         auto pair = [&](int i, ds_floatx4 (&sc)[2][2]) {
+          uint32_t seen = 0u;
           dc_bf16x8 qb[2][KS];
 #pragma unroll
           for (int u = 0; u < 2; ++u)
@@ -296,10 +297,14 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
 #pragma unroll
               for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  sc[u][h][j] = key0 + 16 * h + 4 * gr + j <= pos && cur.ids.id[h] >= 0 ? sc[u][h][j] : -INFINITY;
+                for (int j = 0; j < 4; ++j) {
+                  const bool sees = key0 + 16 * h + 4 * gr + j <= pos && cur.ids.id[h] >= 0;
+                  sc[u][h][j] = sees ? sc[u][h][j] : -INFINITY;
+                  seen |= (uint32_t)sees << (8 * u + 4 * h + j);
+                }
             }
           }
+          return seen;
         };
         if constexpr (!SUMS) {
 #pragma unroll
@@ -334,15 +339,22 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
         } else {
           for (int i = 0; i < tiles; i += 2) {
             ds_floatx4 sc[2][2];
-            pair(i, sc);
+            const uint32_t seen = pair(i, sc);
+            auto add = [&](auto some) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const float2 ml = ml_s[16 * (i + u) + lq];
+              for (int u = 0; u < 2; ++u) {
+                const float2 ml = ml_s[16 * (i + u) + lq];
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[h][j] += __builtin_amdgcn_exp2f(fmaf(sc[u][h][j], a.scale_log2, -ml.x)) * ml.y;
-            }
+                  for (int j = 0; j < 4; ++j) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][h][j], a.scale_log2, -ml.x)) * ml.y;
+                    acc[h][j] += !decltype(some)::value || (seen >> (8 * u + 4 * h + j)) & 1u ? w : 0.f;
+                  }
+              }
+            };
+            // (a row that is no number makes none of the keys it sees, and of no others: 0 times its sum's reciprocal would be none too)
+            edge ? add(std::true_type{}) : add(std::false_type{});
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h)
