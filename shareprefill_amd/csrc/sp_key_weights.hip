@@ -23,6 +23,9 @@
 #define KW_BLOCK (KW_WAVES * KW_KEYS)
 #define KW_TILES 16                      // row tiles of 16 in LDS
 #define KW_SLACK 7.f
+// The exponent takes a logit's exact product with the scale and the row's maximum rounded, half a step of the maximum apart for all of its keys alike: 8 octaves
+// below 2^28, more than an exponential holds from 2^31 on.  Rows that lie further out take rounded products.
+#define KW_FAR 0x1p28f
 #define KW_ROWS (16 * KW_TILES)
 #define KW_OVERHEAD 2                    // blocks' worth of a request beside its blocks: its queries, the rows' meeting
 #define KW_UNITS(rows) (((rows) + 31) / 32 + 1)  // of a block: pairs of row tiles, and its keys
@@ -60,6 +63,14 @@ __device__ static __forceinline__ int64_t kw_quotient(int64_t x, int by, double 
   int64_t q = (int64_t)((double)x * inverse);
   const int64_t left = x - q * by;
   return q + (left >= by) - (left < 0);
+}
+
+__device__ static __forceinline__ bool kw_far(float m) { return __builtin_fabsf(m) >= KW_FAR && __builtin_fabsf(m) < INFINITY; }
+
+__device__ static __forceinline__ float kw_octaves(float x, float scale, float m) {  // (the product is rounded)
+#pragma clang fp contract(off)
+  const float p = x * scale;
+  return p - m;
 }
 
 // over the 16 lanes of a row, each in an order of its own
@@ -258,9 +269,14 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the queries
       __syncthreads();
       float m[SUMS ? 1 : KW_TILES], l[SUMS ? 1 : KW_TILES];
+      // (uniform) some row of the wave lies far out; in the walk for the weights: or is no number
+      bool odd = false;
       if constexpr (!SUMS) {
 #pragma unroll
         for (int i = 0; i < KW_TILES; ++i) m[i] = -INFINITY, l[i] = 0.f;
+      } else {
+        for (int r = lane; r < tiles * 16; r += SP_WAVE) odd |= kw_far(ml_s[r].x) || ml_s[r].y != ml_s[r].y;
+        odd = __ballot(odd) != 0ull;
       }
       for (int block = begin; block < end; ++block) {
         // (the last block asks for itself again: were it not to ask, the wait for this block's keys would be one for the next one's too)
@@ -323,39 +339,49 @@ __global__ __launch_bounds__(KW_THREADS, 2) void sp_key_weights_kernel(const KwA
                   const float to = fmaxf(m[i + u], mx[u]);
                   l[i + u] *= to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i + u] - to);
                   m[i + u] = to;
+                  odd |= __ballot(kw_far(to)) != 0ull;
                 }
               }
+              auto add = [&](auto far_out) {
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const float base = m[i + u] == -INFINITY ? 0.f : m[i + u];
-                float add = 0.f;
+                for (int u = 0; u < 2; ++u) {
+                  const float base = m[i + u] == -INFINITY ? 0.f : m[i + u];
+                  const bool far = decltype(far_out)::value && kw_far(base);
+                  auto octaves = [&](float x) { return far ? kw_octaves(x, a.scale_log2, base) : fmaf(x, a.scale_log2, -base); };
+                  float more = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  add += __builtin_amdgcn_exp2f(fmaf(sc[u][0][j], a.scale_log2, -base)) + __builtin_amdgcn_exp2f(fmaf(sc[u][1][j], a.scale_log2, -base));
-                l[i + u] += add;
-              }
+                  for (int j = 0; j < 4; ++j) more += __builtin_amdgcn_exp2f(octaves(sc[u][0][j])) + __builtin_amdgcn_exp2f(octaves(sc[u][1][j]));
+                  l[i + u] += more;
+                }
+              };
+              if (__builtin_expect(odd, false))
+                add(std::true_type{});
+              else
+                add(std::false_type{});
             }
           }
         } else {
-          for (int i = 0; i < tiles; i += 2) {
-            ds_floatx4 sc[2][2];
-            const uint32_t seen = pair(i, sc);
-            auto add = [&](auto some) {
+          auto walk = [&](auto any) {
+            for (int i = 0; i < tiles; i += 2) {
+              ds_floatx4 sc[2][2];
+              const uint32_t seen = pair(i, sc);
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 const float2 ml = ml_s[16 * (i + u) + lq];
+                const bool far = decltype(any)::value && kw_far(ml.x);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                   for (int j = 0; j < 4; ++j) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[u][h][j], a.scale_log2, -ml.x)) * ml.y;
-                    acc[h][j] += !decltype(some)::value || (seen >> (8 * u + 4 * h + j)) & 1u ? w : 0.f;
+                    const float x = far ? kw_octaves(sc[u][h][j], a.scale_log2, ml.x) : fmaf(sc[u][h][j], a.scale_log2, -ml.x);
+                    const float w = __builtin_amdgcn_exp2f(x) * ml.y;
+                    // (a row that is no number makes none of the keys it sees, and of no others: 0 times its sum's reciprocal would be none too)
+                    acc[h][j] += decltype(any)::value && edge && !((seen >> (8 * u + 4 * h + j)) & 1u) ? 0.f : w;
                   }
               }
-            };
-            // (a row that is no number makes none of the keys it sees, and of no others: 0 times its sum's reciprocal would be none too)
-            edge ? add(std::true_type{}) : add(std::false_type{});
-          }
+            }
+          };
+          if (__builtin_expect(odd, false)) walk(std::true_type{}); else walk(std::false_type{});
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
