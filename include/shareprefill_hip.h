@@ -442,6 +442,8 @@ typedef struct sp_shared_attn_args {
 size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t groups, int32_t hq, int32_t hkv, int32_t d, int32_t single_tokens,
                                       int64_t pool_keys);
 int sp_shared_attn_bf16(const sp_shared_attn_args* args /* host */);
+/* The same where keys in front of first[b] (int32 [batch], null: 0) of sequence b are not weighed either: they may stand in pages of several sequences. */
+int sp_shared_attn_from_bf16(const sp_shared_attn_args* args /* host */, const int32_t* first);
 
 /* What attention every cached key receives: for sequence b with rows cu_q[b] .. cu_q[b + 1] of q (null: one each), its last positions,
  *   weight[j] = sum over its rows and the query heads of the kv group of softmax(q . k)[j] over the keys j' <= the row's position,

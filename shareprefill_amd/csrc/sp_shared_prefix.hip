@@ -54,6 +54,7 @@ struct ShArgs {
   int4* cuts;                 // [part of a wave]: request and step that it begins with, those that it ends in front of
   ShRequest* of_request;      // [batch + 1]
   float* weights;             // null, or [num_pages][kv head][page]
+  const int32_t* weigh_from;  // null, or [batch]: a request's keys in front of that are not weighed
   int weights_by_four;        // four places side by side are one access
   float* logits;              // [num_pages][query head][page]: scaled logits of own keys, in octaves
 };
@@ -627,7 +628,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   if (half != 0) return;
   const int b0 = places[2].item - n_groups, b1 = places[3].item - n_groups, step0 = places[2].step, step1 = places[3].step, wave_part = part * WAVES + slot;
   struct At {  // a step of request b (b = batch: none is left): steps up to `end` of its n fall to the wave
-    int b, s, end, n, lo, key0, key1;
+    int b, s, end, n, lo, key0, key1, weigh0;
   };
   auto settle = [&](At& x) {
     for (;; ++x.b, x.s = 0) {
@@ -638,6 +639,8 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       x.key0 = __builtin_amdgcn_readfirstlane(first_s[x.b]), x.key1 = pg_min(__builtin_amdgcn_readfirstlane(len_s[x.b]), room);
       x.lo = x.key0 / SH_KEYS, x.n = x.key1 > x.key0 ? (x.key1 + SH_KEYS - 1) / SH_KEYS - x.lo : 0;  // (as in item)
       x.end = x.b == b1 ? pg_min(step1, x.n) : x.n;
+      const auto weigh_from = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)args()->weigh_from;
+      x.weigh0 = weigh_from != nullptr ? weigh_from[x.b] : 0;
       if (x.s < x.end) return;
     }
   };
@@ -646,10 +649,10 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   struct Step {  // on its way, or about to be computed on
     int b, key;
     uint32_t seen;
-    Ids ids;
+    Ids ids;  // pages of halves that hold keys to be weighed, else -1
     bool first, last, from_start, to_end, alone;  // of the wave's steps of the request; they begin with its first, end with its last; no shared keys
   };
-  At ahead = {b0, step0, 0, 0, 0, 0, 0};
+  At ahead = {b0, step0, 0, 0, 0, 0, 0, 0};
   settle(ahead);
   Ids ids = {{0, 0}};
   if (ahead.b < a.batch) ids = entries(table_of(ahead.b), key_of(ahead));
@@ -660,6 +663,10 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       const bool from_start = ahead.b != b0 || step0 == 0;
       x = {ahead.b, key, fetch(ring + buf * Shape::STEP_BYTES, key, ahead.key0, ahead.key1, ids, true, true), ids,
            ahead.s == (from_start ? 0 : step0), ahead.s + 1 == ahead.end, from_start, ahead.end == ahead.n, ahead.key0 == 0};
+      // (no page: no key is seen.  The logits' scratch goes by places in the pages: what lies in front of the weighed keys may be several requests')
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (((x.seen >> (16 * i)) & 0xffffu) == 0u || key + 16 * i + 16 <= ahead.weigh0) x.ids.id[i] = -1;
       if (++ahead.s >= ahead.end) {
         ++ahead.b, ahead.s = 0;
         settle(ahead);
@@ -709,7 +716,7 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
             float* const to = args()->logits;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (((now.seen >> (16 * i)) & 0xffffu) != 0u)  // (no page: no key of it is seen)
+              if (now.ids.id[i] >= 0)
                 *reinterpret_cast<ds_floatx4*>(to + ((((int64_t)now.ids.id[i] * a.hkv + kvh) * g + lq) << a.shift) + ((now.key + 16 * i + 4 * gr) & ((1 << a.shift) - 1))) = sc[0][i];
           });
     }
@@ -872,7 +879,8 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
     const int len = pg_max(0, pg_min(a.lens[b], PG_MAX_KEYS));
     const int lo = r.first_own / SH_KEYS, keys = pg_min(len, room);
     const int begin = b == cut.x ? cut.y : 0, end = b == cut.z ? cut.w : PG_MAX_KEYS / SH_KEYS;
-    if (keys <= r.first_own || begin >= end) continue;
+    const int weigh0 = a.weigh_from != nullptr ? pg_max(a.weigh_from[b], r.first_own) : r.first_own;
+    if (keys <= weigh0 || begin >= end) continue;
     // Maxima and sums of the group's heads, by every wave for itself: lane 16 q + h takes every fourth part of head h from q on.
     float top = CK_NO_MAX, inv = 0.f;
     {
@@ -907,7 +915,7 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
       }
       inv = sum == 0.f ? 0.f : 1.0f / sum;
     }
-    const int first = (lo + begin) * SH_KEYS, last = (int)pg_min((int)(lo + end < keys / SH_KEYS + 1 ? (lo + end) * SH_KEYS : keys), keys);
+    const int first = pg_max((lo + begin) * SH_KEYS, weigh0 / SH_KEYS * SH_KEYS), last = (int)pg_min((int)(lo + end < keys / SH_KEYS + 1 ? (lo + end) * SH_KEYS : keys), keys);
     // (all lanes go through the loop together: they hold the heads' maxima and sums for each other)
     for (int at = first; at < last; at += 4 * threads) {
       const int key = at + 4 * (t % threads), in = key & ((1 << a.shift) - 1), page = pg_min(key >> a.shift, a.width - 1);
@@ -931,12 +939,12 @@ __device__ __forceinline__ void sh_weigh(const ShArgs& a, int w) {
       }
       if (!there) continue;
       float* const to = a.weights + id * a.sw_p + kvh * a.sw_h + in;
-      if (a.weights_by_four && key >= r.first_own && key + 4 < len && key + 4 <= last) {
+      if (a.weights_by_four && key >= weigh0 && key + 4 < len && key + 4 <= last) {
         *reinterpret_cast<ds_floatx4*>(to) += sum;
       } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (key + j >= r.first_own && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
+          if (key + j >= weigh0 && key + j < last) to[j] = (key + j == len - 1 ? 0.f : to[j]) + sum[j];  // (the newest key's starts here)
       }
     }
   }
@@ -1001,7 +1009,9 @@ extern "C" size_t sp_shared_attn_workspace_bytes(int64_t tokens, int32_t batch, 
   return one > apart ? one : apart;
 }
 
-extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
+extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) { return sp_shared_attn_from_bf16(x, nullptr); }
+
+extern "C" int sp_shared_attn_from_bf16(const sp_shared_attn_args* x, const int32_t* first) {
   const char* who = "sp_shared_attn_bf16";
   SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   SP_REQUIRE(x->hq > 0 && x->hkv > 0 && x->hq % x->hkv == 0, SP_ERR_INVALID_ARGUMENT, "%s: bad shape hq=%lld hkv=%lld", who, (long long)x->hq,
@@ -1064,7 +1074,7 @@ extern "C" int sp_shared_attn_bf16(const sp_shared_attn_args* x) {
   a.o_stream = (float*)(ws + s.o_stream), a.ml_stream = (float2*)(ws + s.ml_stream);
   a.streams = x->cu_q == nullptr && g <= PD_MAX_GROUP;
   a.weights_by_four = (uintptr_t)x->weights % 16 == 0 && (w_p | w_h) % 4 == 0;
-  a.weights = x->weights, a.logits = (float*)(ws + s.logits);
+  a.weights = x->weights, a.weigh_from = x->weights != nullptr ? first : nullptr, a.logits = (float*)(ws + s.logits);
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
   SP_HIP(hipGetDevice(&dev));

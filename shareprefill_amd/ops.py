@@ -735,7 +735,7 @@ def _check_weights(weights: torch.Tensor, pages: int, hkv: int, page_size: int, 
 def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                             shared_lens: torch.Tensor, cu_groups: torch.Tensor, softmax_scale: float, cu_q: Optional[torch.Tensor] = None,
                             weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                            joined: Optional[torch.Tensor] = None) -> torch.Tensor:
+                            joined: Optional[torch.Tensor] = None, first: Optional[torch.Tensor] = None) -> torch.Tensor:
     """paged_attention (without a window) where groups of requests have their first keys in common, which are read once for a group instead of once
     for each of its requests.  Requests cu_groups[i] .. cu_groups[i + 1] - 1 are group i (int32 [G + 1], in order; requests outside share nothing;
     G may be 0), and the first shared_lens[i] keys (int32 [G]) of each of them are those in the pages that the block table names for the group's
@@ -745,8 +745,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
 
     weights (fp32 [num_pages, Hkv, page_size] view, for single tokens in groups of up to 16 query heads): what attention each key has received.
     Every key that a request does not share gets, at its place in the pages, the sum of its softmax weights over the kv group's query heads added; the
-    newest key, whose place may hold what an earlier owner of the page left, is set to it.  Places of no key stay as they are.  Keys of two
-    requests must not lie in one page then, but for shared ones.
+    newest key, whose place may hold what an earlier owner of the page left, is set to it.  Places of no key stay as they are, and so do those of keys in
+    front of first[b] (int32 [B]; None: 0).  Keys of two requests must not lie in one page then, but for shared ones and those.
 
     At most 1024 requests; head_dim 64 or 128; lengths, offsets and pages are read on the device.  Scratch memory, from torch's allocator, for the
     call: 52 MB at 128 channels with 256 kv heads or fewer (86 MB where groups have more than 256 rows), half of it at 64, 8 Hq (D + 2) bytes a token, and
@@ -766,6 +766,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     _check_table(block_table, batch, dev)
     if joined is not None:
         _check_ints(dev, ("joined", joined, torch.int32, batch))
+    if first is not None:
+        _check_ints(dev, ("first", first, torch.int32, batch))
     if cu_q is not None:
         _check_ints(dev, ("cu_q", cu_q, torch.int32, batch + 1))
     elif n != batch:
@@ -784,11 +786,11 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     need = lib.sp_shared_attn_workspace_bytes(n, batch, groups, hq, hkv, d, cu_q is None, 0 if weights is None else pages * page_size)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None  # (of this call's own, as in paged_attention)
     q_h, q_n, _ = q.stride()
-    st = lib.sp_shared_attn_bf16(_lib.SHARED_ATTN_ARGS.pack(
+    st = lib.sp_shared_attn_from_bf16(_lib.SHARED_ATTN_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
         shared_lens.data_ptr(), cu_groups.data_ptr(), 0 if joined is None else joined.data_ptr(), 0 if weights is None else weights.data_ptr(), out.data_ptr(),
         0 if ws is None else ws.data_ptr(), need, n, batch, groups, hq, hkv, d, pages, page_size, block_table.size(1), block_table.stride(0), q_n,
-        q_h, k_p, k_n, k_h, v_p, v_n, v_h, w_p, w_h, softmax_scale, stream))
+        q_h, k_p, k_n, k_h, v_p, v_n, v_h, w_p, w_h, softmax_scale, stream), 0 if first is None else first.data_ptr())
     if st:
         _lib.check(st, "sp_shared_attn_bf16")
     return out

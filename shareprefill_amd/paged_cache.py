@@ -153,7 +153,7 @@ class PagedKVCache:
             weights = self.weights[layer] if self.weights is not None and self._cu_q is None else None
             together = q.dim() == 3 and q.shape[0] <= 16 * self.pools.shape[3]  # (attention weighs the keys of up to 16 query heads a kv head)
             out = ops.shared_prefix_attention(q, *pools, self.block_table, self._seen_lens, self.shared_lens, self.cu_groups, softmax_scale,
-                                              cu_q=self._cu_q, weights=weights if together else None, out=out, joined=self._joined)
+                                              cu_q=self._cu_q, weights=weights if together else None, out=out, joined=self._joined, first=self._held)
             if weights is not None and not together:
                 ops.paged_key_weights(q, pools[0], self.block_table, self._seen_lens, softmax_scale, weights, first=self._held, accumulate=True)
             return out
