@@ -467,7 +467,7 @@ int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* args /* host */);
 /* Drops the lightest keys of every kv head of sequences that hold more than they may: of sequence b with seq_lens[b] keys the first first[b] (null: 0)
  * and the last `recent` stay and of those between the `budget` heaviest by their weights (of equal ones the first; a weight that is negative or no
  * number counts as 0).  What stays behind the first keys moves to the front of its pages, K, V and weights, in the order it stood in; places behind it keep
- * what they held.  new_lens[b] is the length left, the same for all kv heads.  A sequence with a key behind the first ones that has no page stays as it is.
+ * what they held.  new_lens[b] is the length left, the same for all kv heads (-1: see sp_paged_evict_bounded_bf16).  A sequence with a key behind the first ones that has no page stays as it is.
  * Pages must not be shared but for those that hold nothing but first keys.  d a multiple of 8. */
 typedef struct sp_paged_evict_args {
   void *k_pages, *v_pages;
@@ -482,6 +482,10 @@ typedef struct sp_paged_evict_args {
 } sp_paged_evict_args;
 size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int32_t d, int64_t num_pages, int64_t page_size, int64_t table_width);
 int sp_paged_evict_bf16(const sp_paged_evict_args* args /* host */);
+/* The same with the bound of its waits given: rows that stay are moved by workgroups that wait for each other's reads, some microseconds.  One that has
+ * looked `polls` times in vain (sp_paged_evict_bf16: 2^20 times, a second or more) writes nothing, and new_lens[b] is -1: the keys behind the first ones of
+ * sequence b are lost. */
+int sp_paged_evict_bounded_bf16(const sp_paged_evict_args* args /* host */, int32_t polls);
 
 /* ---- rotary position embedding in front of the attention function ---------------------------------
  * The reference's patched model produces (cos, sin) per position (model_patch.py:121) and leaves the rotation to

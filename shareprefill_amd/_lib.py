@@ -112,6 +112,7 @@ SIGNATURES = {
     "sp_paged_key_weights_bf16": (_I32, [C.c_char_p]),
     "sp_paged_evict_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I64, _I64, _I64]),
     "sp_paged_evict_bf16": (_I32, [C.c_char_p]),
+    "sp_paged_evict_bounded_bf16": (_I32, [C.c_char_p, _I32]),
     "sp_rope_inplace_bf16": (_I32, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _P]),
     "sp_pivot_update": (_I32, [_ST, _P, _P, _P, _I32, _I32, _F, _P]),
     "sp_cover_select_rows": (_I32, [_P, _I32, _F, _P, _P]),

@@ -25,7 +25,7 @@
 #define EV_TURN 10          // entries of a lane on their way
 #define EV_SLICE 512        // channels of a row that a workgroup moves
 #define EV_AHEAD 6          // rows of a thread
-#define EV_POLLS (1 << 20)
+#define EV_POLLS (1 << 20)  // looks that a lane of a workgroup that waits has for all of its wait: a second or more
 #define EV_FEW 256          // workgroups that move: one a CU
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
@@ -37,7 +37,7 @@ struct EvArgs {
   const int32_t *table, *lens, *first;
   int32_t* new_lens;
   int64_t table_stride, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;
-  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slices, streams, chunks;
+  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slices, streams, chunks, polls;
   // By place in the pages, [num_pages][kv head][page]: entry i of a request's list stands at the place of its i-th key behind the first ones.  First
   // pattern << 32 | place of what is listed, then the place that a kept key comes from; a place is page << shift + place in it.
   uint64_t* list;
@@ -394,10 +394,11 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 }
 
 // A workgroup moves a chunk of a kv head's kept rows: reads them all, waits until the chunks in front of it have read theirs, which alone may need what it
-// writes over, and writes.  A chunk is taken when its workgroup has begun, so that whoever is waited for runs, and waits for nobody before it has read.
+// writes over, and writes.  A chunk is taken when its workgroup has begun, so that whoever is waited for runs, and waits for nobody before it has read: a wait
+// of some microseconds.  It is bounded all the same; a workgroup that has waited in vain does not write, and the request's length is -1.
 template <int AHEAD>
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs a) {
-  __shared__ int chunk_s;
+  __shared__ int chunk_s, in_vain_s;
   const int t = threadIdx.x, pairs = a.batch * a.hkv, stream = blockIdx.x % a.streams, pair = stream % pairs, part = stream / pairs, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   const EvRequest& r = p.r;
@@ -433,12 +434,26 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
     __syncthreads();  // the chunk is read
     int32_t* const done = a.done + (int64_t)stream * a.chunks;
     if (t == 0) __hip_atomic_store(done + chunk, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // (some microseconds; the bound, of a second, is for a workspace that something else writes to meanwhile)
-    if (t < SP_WAVE)
-      for (int i = t; i < chunk; i += SP_WAVE)
-        for (int polls = 0; polls < EV_POLLS && __hip_atomic_load(done + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0; ++polls) __builtin_amdgcn_s_sleep(1);
+    if (t < SP_WAVE) {
+      int polls = a.polls;
+      bool in_vain = false;
+      for (int i = t; i < chunk; i += SP_WAVE) {
+        bool read = false;
+        while (!read && polls > 0) {
+          read = __hip_atomic_load(done + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != 0;
+          if (!read) --polls, __builtin_amdgcn_s_sleep(1);
+        }
+        in_vain |= !read;
+      }
+      const bool any = __ballot(in_vain) != 0ull;
+      if (t == 0) in_vain_s = any;
+    }
     asm volatile("" ::: "memory");
     __syncthreads();
+    if (in_vain_s) {
+      if (t == 0) a.new_lens[b] = -1;
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
       if (row < per && i0 + u * per + row < rows) *at(to[u]) = y[u];
@@ -502,13 +517,16 @@ extern "C" size_t sp_paged_evict_workspace_bytes(int32_t batch, int32_t hkv, int
   return ev_sizes(batch, hkv, num_pages * page_size, ev_shares(pairs, room), ev_move(pairs, d, room)).bytes;
 }
 
-extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
+extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) { return sp_paged_evict_bounded_bf16(x, EV_POLLS); }
+
+extern "C" int sp_paged_evict_bounded_bf16(const sp_paged_evict_args* x, int32_t polls) {
   const char* who = "sp_paged_evict_bf16";
   SP_REQUIRE(x != nullptr, SP_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   SP_REQUIRE(x->batch > 0 && x->hkv > 0 && x->table_width > 0 && x->num_pages > 0, SP_ERR_INVALID_ARGUMENT,
              "%s: batch=%lld hkv=%lld table_width=%lld num_pages=%lld", who, (long long)x->batch, (long long)x->hkv, (long long)x->table_width,
              (long long)x->num_pages);
   SP_REQUIRE(x->budget >= 0 && x->recent >= 0, SP_ERR_INVALID_ARGUMENT, "%s: budget=%lld recent=%lld", who, (long long)x->budget, (long long)x->recent);
+  SP_REQUIRE(polls >= 0, SP_ERR_INVALID_ARGUMENT, "%s: polls %d", who, (int)polls);
   SP_REQUIRE(x->d > 0 && x->d % 8 == 0 && x->d <= 65536, SP_ERR_UNSUPPORTED, "%s: head_dim %lld (a multiple of 8)", who, (long long)x->d);
   int shift = 4;
   while (shift <= 10 && x->page_size != 1ll << shift) ++shift;
@@ -540,7 +558,7 @@ extern "C" int sp_paged_evict_bf16(const sp_paged_evict_args* x) {
   a.sw_p = pg_used_stride(x->w_stride_page, x->num_pages), a.sw_h = pg_used_stride(x->w_stride_h, x->hkv);
   a.batch = (int)x->batch, a.hkv = (int)x->hkv, a.d = (int)x->d, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
   a.budget = (int)(x->budget < PG_MAX_KEYS ? x->budget : PG_MAX_KEYS), a.recent = (int)(x->recent < PG_MAX_KEYS ? x->recent : PG_MAX_KEYS);
-  a.shares = shares, a.slices = (int)move.slices, a.streams = (int)move.streams, a.chunks = (int)move.chunks;
+  a.shares = shares, a.slices = (int)move.slices, a.streams = (int)move.streams, a.chunks = (int)move.chunks, a.polls = polls;
   a.by_four = (uintptr_t)x->weights % 16 == 0 && (a.sw_p | a.sw_h) % 4 == 0;
   char* const ws = (char*)x->workspace;
   a.list = (uint64_t*)(ws + sizes.list), a.hists = (uint32_t*)(ws + sizes.hists), a.counts = (int32_t*)(ws + sizes.counts);

@@ -847,6 +847,7 @@ def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Ten
     NaN counts as 0.  Keys, values and weights that stay behind the first keys move to the front of their pages, in order; the pages behind the new
     length may go back to the stack.  Keys are moved as they are, rotated for the positions they had: the next token's position is not the new length.
     A request with a key behind the first ones that has no page stays as it is.  Only pages of nothing but first keys may be shared.
+    A length of -1: the card stood still for a second or more while the request's rows were moved, and its keys behind the first ones are lost.
 
     At most 4096 requests; head_dim a multiple of 8.  Scratch memory, from torch's allocator, for the call: 8 bytes a key and kv head
     of the pools, up to 2 MB, and 12 bytes for every 384 keys (at 128 channels) and kv head that the table has room for."""

@@ -72,6 +72,7 @@ class PagedKVCache:
         # what attention every key has received, by its place in the pages (None: not kept), and how many keys evictions have taken from a request
         self.weights = torch.zeros(num_layers, num_pages, num_kv_heads, page_size, dtype=torch.float32, device=dev) if key_weights else None
         self.dropped = torch.zeros(max_requests, dtype=torch.int32, device=dev)
+        self.lost = torch.zeros(max_requests, dtype=torch.bool, device=dev)  # requests whose keys an eviction has spoilt
         self._last = None  # of a step: rows of its requests' last tokens (observe)
         self._fresh = None  # of a step: places that its tokens' keys come to
 
@@ -230,15 +231,18 @@ class PagedKVCache:
     def evict(self, budget: int, recent: int, sinks: int = 0, rows: Optional[torch.Tensor] = None) -> None:
         """Drops keys of requests (rows bool [max_requests]; None: all) that hold more than they may, in every layer and kv head by itself: the first
         `sinks` and those in pages of several requests stay, the last `recent`, and of the others the `budget` heaviest (ops.paged_evict).  Their pages go back.
-        A window of attend counts places in the cache, which later keys of such a request have nearer to each other than their positions."""
+        A window of attend counts places in the cache, which later keys of such a request have nearer to each other than their positions.
+        A request whose rows could not be moved (ops.paged_evict: a length of -1) has its first keys alone, and lost[r] until its release."""
         weights = self._check_weights()
         if rows is not None:
             self._check_mask(rows, "rows")
         lens = self.lens if rows is None else self.lens * rows
         first = torch.clamp(self._held, min=sinks)
-        left = lens
-        for layer in range(self.pools.shape[0]):
-            left = ops.paged_evict(*self.pools[layer].unbind(0), weights[layer], self.block_table, lens, budget, recent, first=first)
+        left = torch.stack([ops.paged_evict(*self.pools[layer].unbind(0), weights[layer], self.block_table, lens, budget, recent, first=first)
+                            for layer in range(self.pools.shape[0])]).amin(0)
+        lost = left < 0
+        self.lost |= lost
+        left = torch.where(lost, torch.minimum(first, lens), left)
         if rows is not None:
             left = torch.where(rows, left, self.lens)
         in_front = torch.where(self.dropped > 0, torch.minimum(self._in_place, first), first)
@@ -271,7 +275,7 @@ class PagedKVCache:
         self._check_mask(finished, "finished")
         self._give_back(finished[:, None].expand_as(self.block_table))
         self.lens.masked_fill_(finished, 0)
-        for x in (self.dropped, self._held, self._joined):
+        for x in (self.dropped, self._held, self._joined, self.lost):
             x.masked_fill_(finished, 0)
         if self.shared_lens.numel() > 0:
             ended = finished[self.cu_groups[:-1].long()]

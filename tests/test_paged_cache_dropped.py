@@ -70,3 +70,17 @@ def test_a_start_in_front_of_all_that_went_counts_nothing(evicting):
     cache.evict(budget=10, recent=10, sinks=2, rows=_mask(3))
     cache.share(1, 16)
     assert cache.lens.tolist()[3:5] == [22, 16] and cache.dropped.tolist()[3:5] == [68, 68]
+
+
+def test_a_request_that_an_eviction_has_spoilt(monkeypatch):
+    """One layer of it is enough; its first keys stay, its pages go back, and its release ends it."""
+    cache = _cache(key_weights=True, num_layers=3)
+    _fill(cache, 0, 6, 90)
+    _fill(cache, 5, 5, 80)
+    left = iter([[30, 0, 0, 0, 0, 80], [-1, 0, 0, 0, 0, 80], [30, 0, 0, 0, 0, 80]])
+    monkeypatch.setattr(ops, "paged_evict", lambda *a, **kw: torch.tensor(next(left), dtype=torch.int32))
+    cache.evict(budget=20, recent=2, sinks=8)
+    assert cache.lens.tolist() == [8, 0, 0, 0, 0, 80] and cache.lost.tolist() == [True] + [False] * 5
+    assert (cache.block_table[0] >= 0).sum() == 1 and cache.free_count.item() == 20 - 6 and cache.dropped.tolist()[0] == 82
+    cache.release(_mask(0))
+    assert cache.lost.tolist() == [False] * 6 and cache.free_count.item() == 20 - 5
