@@ -27,6 +27,7 @@
 #define EV_AHEAD 6          // rows of a thread
 #define EV_POLLS (1 << 20)  // looks that a lane of a workgroup that waits has for all of its wait: a second or more
 #define EV_FEW 256          // workgroups that move: one a CU
+#define EV_MOST 8192        // workgroups that move at most, but for one a stream: 16 times as many as the card holds
 
 typedef uint32_t ev_u32x4 __attribute__((ext_vector_type(4)));
 typedef float ev_floatx4 __attribute__((ext_vector_type(4)));
@@ -37,7 +38,7 @@ struct EvArgs {
   const int32_t *table, *lens, *first;
   int32_t* new_lens;
   int64_t table_stride, sk_p, sk_n, sk_h, sv_p, sv_n, sv_h, sw_p, sw_h;
-  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slices, streams, chunks, polls;
+  int batch, hkv, d, width, num_pages, shift, budget, recent, shares, by_four, slices, chunks, polls;
   // By place in the pages, [num_pages][kv head][page]: entry i of a request's list stands at the place of its i-th key behind the first ones.  First
   // pattern << 32 | place of what is listed, then the place that a kept key comes from; a place is page << shift + place in it.
   uint64_t* list;
@@ -396,21 +397,24 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_choose_kernel(const EvArg
 // A workgroup moves a chunk of a kv head's kept rows: reads them all, waits until the chunks in front of it have read theirs, which alone may need what it
 // writes over, and writes.  A chunk is taken when its workgroup has begun, so that whoever is waited for runs, and waits for nobody before it has read: a wait
 // of some microseconds.  It is bounded all the same; a workgroup that has waited in vain does not write, and the request's length is -1.
-template <int AHEAD>
+template <int AHEAD, bool MORE>  // MORE: a stream has more chunks than workgroups, which take another behind each (it costs those that have had their own 6 us of 46)
 __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs a) {
   __shared__ int chunk_s, in_vain_s;
-  const int t = threadIdx.x, pairs = a.batch * a.hkv, stream = blockIdx.x % a.streams, pair = stream % pairs, part = stream / pairs, b = pair / a.hkv;
+  const int t = threadIdx.x, pair = blockIdx.x, part = blockIdx.y, stream = part * gridDim.x + pair, b = pair / a.hkv;
   const EvPair p = ev_pair(a, pair);
   const EvRequest& r = p.r;
   if (r.keep >= r.mid) return;
   // (the look at the table brings its entries near while the ticket is on its way: 30 us for 44 where the launch before this one had told what it says)
-  if (t == 0) chunk_s = __hip_atomic_fetch_add(a.tickets + stream, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  auto take = [&] {
+    if (t == 0) chunk_s = __hip_atomic_fetch_add(a.tickets + stream, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  take();
   if (!ev_has_pages(a, b, r)) return;
-  const int chunk = chunk_s, rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
-  auto move = [&](auto type, int lanes, auto at) {  // elements of a row side by side, one a thread
-    const int per = EV_THREADS / lanes, row = t / lanes;
+  const int rows = r.keep + r.len - r.first - r.mid, in = (1 << a.shift) - 1;
+  auto move_chunk = [&](auto type, int lanes, auto at) {  // elements of a row side by side, one a thread.  -> there may be another chunk
+    const int per = EV_THREADS / lanes, row = t / lanes, chunk = chunk_s;
     const int64_t i0 = (int64_t)chunk * (per * AHEAD);
-    if (i0 >= rows) return;
+    if (i0 >= rows) return false;
     // (a thread without a row reads the last one's.  Every row's page, then every row's source, then every row: asked for row by row each waits for the last)
     decltype(type) y[AHEAD];
     uint32_t to[AHEAD], come[AHEAD];
@@ -452,11 +456,18 @@ __global__ __launch_bounds__(EV_THREADS) void sp_evict_move_kernel(const EvArgs 
     __syncthreads();
     if (in_vain_s) {
       if (t == 0) a.new_lens[b] = -1;
-      return;
+      return false;
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u)
       if (row < per && i0 + u * per + row < rows) *at(to[u]) = y[u];
+    return MORE && i0 + per * AHEAD < rows;
+  };
+  auto move = [&](auto type, int lanes, auto at) {
+    while (move_chunk(type, lanes, at)) {
+      take();
+      __syncthreads();
+    }
   };
   if (part == 2 * a.slices) {
     float* const w = a.weights + p.kvh * a.sw_h;
@@ -534,7 +545,7 @@ extern "C" int sp_paged_evict_bounded_bf16(const sp_paged_evict_args* x, int32_t
   SP_REQUIRE(x->batch <= EV_MAX_SEQS, SP_ERR_UNSUPPORTED, "%s: batch %lld (at most %d)", who, (long long)x->batch, EV_MAX_SEQS);
   const int64_t pairs = x->batch * x->hkv;
   SP_REQUIRE(x->hkv <= 65536 && x->num_pages <= 0x7fffffffll && x->table_width <= PG_MAX_KEYS && x->table_width << shift <= PG_MAX_KEYS &&
-                 x->num_pages << shift <= 0xffffffffll && pairs <= (1 << 22),
+                 x->num_pages << shift <= 0xffffffffll && pairs * EV_THREADS < (1ll << 32),
              SP_ERR_UNSUPPORTED, "%s: hkv=%lld num_pages=%lld table_width=%lld too large", who, (long long)x->hkv, (long long)x->num_pages,
              (long long)x->table_width);
   const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);
@@ -558,7 +569,7 @@ extern "C" int sp_paged_evict_bounded_bf16(const sp_paged_evict_args* x, int32_t
   a.sw_p = pg_used_stride(x->w_stride_page, x->num_pages), a.sw_h = pg_used_stride(x->w_stride_h, x->hkv);
   a.batch = (int)x->batch, a.hkv = (int)x->hkv, a.d = (int)x->d, a.width = (int)x->table_width, a.num_pages = (int)x->num_pages, a.shift = shift;
   a.budget = (int)(x->budget < PG_MAX_KEYS ? x->budget : PG_MAX_KEYS), a.recent = (int)(x->recent < PG_MAX_KEYS ? x->recent : PG_MAX_KEYS);
-  a.shares = shares, a.slices = (int)move.slices, a.streams = (int)move.streams, a.chunks = (int)move.chunks, a.polls = polls;
+  a.shares = shares, a.slices = (int)move.slices, a.chunks = (int)move.chunks, a.polls = polls;
   a.by_four = (uintptr_t)x->weights % 16 == 0 && (a.sw_p | a.sw_h) % 4 == 0;
   char* const ws = (char*)x->workspace;
   a.list = (uint64_t*)(ws + sizes.list), a.hists = (uint32_t*)(ws + sizes.hists), a.counts = (int32_t*)(ws + sizes.counts);
@@ -579,8 +590,11 @@ extern "C" int sp_paged_evict_bounded_bf16(const sp_paged_evict_args* x, int32_t
     hipLaunchKernelGGL(sp_evict_gather_kernel, dim3((unsigned)(pairs * shares)), dim3(EV_THREADS), lds, stream, a);
   }
   hipLaunchKernelGGL(sp_evict_choose_kernel, dim3((unsigned)pairs), dim3(EV_THREADS), lds, stream, a);
-  if (move.chunks > 0)
-    hipLaunchKernelGGL(move.ahead == 1 ? sp_evict_move_kernel<1> : sp_evict_move_kernel<EV_AHEAD>, dim3((unsigned)(move.streams * move.chunks)), dim3(EV_THREADS), 0, stream, a);
+  if (move.chunks > 0) {
+    const int64_t each = EV_MOST / move.streams, of_stream = move.chunks < each ? move.chunks : each < 1 ? 1 : each;
+    const auto kernel = of_stream < move.chunks ? sp_evict_move_kernel<EV_AHEAD, true> : move.ahead == 1 ? sp_evict_move_kernel<1, false> : sp_evict_move_kernel<EV_AHEAD, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)pairs, (unsigned)(move.streams / pairs), (unsigned)of_stream), dim3(EV_THREADS), 0, stream, a);
+  }
   SP_LAUNCH_CHECK();
   return SP_OK;
 }
