@@ -502,7 +502,8 @@ extern "C" int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* x) {
   SP_REQUIRE(x->cu_q != nullptr || x->tokens == x->batch, SP_ERR_INVALID_ARGUMENT, "%s: without cu_q every sequence has one token (%lld for %lld)",
              who, (long long)x->tokens, (long long)x->batch);
   if (x->tokens == 0) return SP_OK;
-  SP_REQUIRE(kw_shape_ok(x->tokens, x->batch, x->hq, x->hkv), SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who,
+  SP_REQUIRE(kw_shape_ok(x->tokens, x->batch, x->hq, x->hkv) && (x->tokens * x->hq + KW_WAVES - 1) * SP_WAVE < (1ll << 32), SP_ERR_UNSUPPORTED,  // (the joining launch)
+             "%s: %lld tokens of %lld heads are too many", who,
              (long long)x->tokens, (long long)x->hq);
   const int64_t q_n = pg_used_stride(x->q_stride_n, x->tokens), q_h = pg_used_stride(x->q_stride_h, x->hq);
   const int64_t k_p = pg_used_stride(x->k_stride_page, x->num_pages), k_h = pg_used_stride(x->k_stride_h, x->hkv);

@@ -1075,6 +1075,13 @@ extern "C" int sp_shared_attn_from_bf16(const sp_shared_attn_args* x, const int3
   a.streams = x->cu_q == nullptr && g <= PD_MAX_GROUP;
   a.weights_by_four = (uintptr_t)x->weights % 16 == 0 && (w_p | w_h) % 4 == 0;
   a.weights = x->weights, a.weigh_from = x->weights != nullptr ? first : nullptr, a.logits = (float*)(ws + s.logits);
+  const int grid = a.parts * a.hkv;
+  // few rows may have many parts each: a workgroup a row
+  const int sets = x->tokens * x->hq <= 512 ? SM_THREADS / ((int)x->d / 4) : 1;
+  const int64_t join = sp_ceil_div(x->tokens * x->hq * sets, SM_THREADS / (x->d / 4));
+  const int64_t joins = join + (x->weights != nullptr ? (int64_t)grid * SH_WAVES : 0);
+  SP_REQUIRE(joins * SM_THREADS < (1ll << 32), SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens,
+             (long long)x->hq);  // (a launch has fewer threads than that)
   static bool attr_set[64] = {false};  // per device, once (idempotent)
   int dev = 0;
   SP_HIP(hipGetDevice(&dev));
@@ -1085,12 +1092,6 @@ extern "C" int sp_shared_attn_from_bf16(const sp_shared_attn_args* x, const int3
     attr_set[dev] = true;
   }
   const hipStream_t stream = (hipStream_t)x->stream;
-  const int grid = a.parts * a.hkv;
-  // few rows may have many parts each: a workgroup a row
-  const int sets = x->tokens * x->hq <= 512 ? SM_THREADS / ((int)x->d / 4) : 1;
-  const int64_t join = sp_ceil_div(x->tokens * x->hq * sets, SM_THREADS / (x->d / 4));
-  SP_REQUIRE(join + (int64_t)grid * SH_WAVES <= 0x7fffffffll, SP_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads are too many", who, (long long)x->tokens,
-             (long long)x->hq);
   a.apart = apart;
   if (a.apart) {
     CkArgs c = {};
@@ -1102,11 +1103,10 @@ extern "C" int sp_shared_attn_from_bf16(const sp_shared_attn_args* x, const int3
     const int rc = ck_groups_launch(c, (int)x->d, ws + s.o_part, stream);
     if (rc) return rc;
   }
-  const unsigned joins = (unsigned)(join + (a.weights != nullptr ? grid * SH_WAVES : 0));
   const size_t lds = sh_lds_bytes(a.batch, a.n_groups);
   auto go = [&](auto kernel, auto many, auto few) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(SH_THREADS), lds, stream, a);
-    hipLaunchKernelGGL(sets == 1 ? many : few, dim3(joins), dim3(SM_THREADS), 0, stream, a, (int)join);
+    hipLaunchKernelGGL(sets == 1 ? many : few, dim3((unsigned)joins), dim3(SM_THREADS), 0, stream, a, (int)join);
   };
   if (x->d == 64)
     go(sp_shared_kernel<64>, sp_shared_join_kernel<64, 1>, sp_shared_join_kernel<64, SM_THREADS / 16>);
