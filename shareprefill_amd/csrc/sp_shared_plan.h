@@ -23,9 +23,10 @@ enum { SH_GROUP, SH_OWN, SH_STREAM };  // items: a group's shared keys, a reques
 #define SH_MIN_SHARE 8   // units of a part at least
 #define SH_WAVES 4       // that share a workgroup's keys
 
-// Rows of a tile where there are `rows` of them: with more than 64 keys are read half as often for a step's work twice as long, which its steps count.
+// Rows of a tile where there are `rows` of them: with more than 64 keys are read half as often for a step's work twice as long or more, which its steps count.
+// (us, 2 / 3 / 4 units: 64 single tokens of 32 heads over 8 behind 8192 keys 95 / 86 / 95, four groups of 16 of 28 over 4 behind 4000 42 / 42 / 40.)
 PG_FN int sh_tile(int rows) { return rows <= SH_UNIT ? SH_UNIT : SH_ROWS; }
-PG_FN int sh_step_units(int rows) { return rows <= SH_UNIT ? 1 : 2; }
+PG_FN int sh_step_units(int rows) { return rows <= SH_UNIT ? 1 : 3; }
 // Where a cut `off` units into an item stands whose tiles have n steps each: in front of a step of a tile (the n-th: behind the tile).
 PG_FN int sh_overhead(int kind) { return kind == SH_GROUP ? SH_OVERHEAD : kind == SH_OWN ? SH_OWN_OVERHEAD : SH_STREAM_OVERHEAD; }
 PG_FN void sh_place(int64_t off, int n, int rows, int kind, int near, int* tile, int* step) {

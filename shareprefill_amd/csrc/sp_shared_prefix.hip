@@ -315,7 +315,6 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
   // do not see some of them, those behind pos.  m, l: the rows' maxima, and the sums of this lane group's keys.  logits(sc) is called with the logits.
   auto attend = [&](auto tiles, uint32_t off, int key, uint32_t mine, auto& qb, auto& pos, bool partly, auto& o, auto& m, auto& l, auto&& logits) {
     constexpr int RT = decltype(tiles)::value;
-    constexpr bool TWO = RT == 1;  // probabilities as two bf16 values
     dc_u32x4 kr[2][KS];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -391,7 +390,9 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
       vr[ct][0] = ds_read_v<0>(at);
       vr[ct][1] = ds_read_v<16 * CT * 32>(at);
     }
-    dc_bf16x8 ph[RT], pl[1];
+    // Probabilities enter the product as two bf16 values: what truncation leaves of them, and the rest, of at least 2^-23 of the probability: an infinite value
+    // has met its weight in the first product, and zero or a negative number times infinity would make a NaN of the sum.
+    dc_bf16x8 ph[RT], pl[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float base = m[rt] == -INFINITY ? 0.f : m[rt];
@@ -401,13 +402,13 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
 #pragma unroll
         for (int j = 0; j < 4; j += 2) {
           const float p0 = __builtin_amdgcn_exp2f(sc[rt][i][j] - base), p1 = __builtin_amdgcn_exp2f(sc[rt][i][j + 1] - base);
-          const uint32_t w = dc_pack2(p0, p1);
-          hi[2 * i + j / 2] = w;
+          const uint32_t b0 = __float_as_uint(p0), b1 = __float_as_uint(p1);
+          hi[2 * i + j / 2] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
           l[rt] += p0 + p1;
-          if constexpr (TWO) lw[2 * i + j / 2] = dc_pack2(p0 - __uint_as_float(w << 16), p1 - __uint_as_float(w & 0xffff0000u));
+          lw[2 * i + j / 2] = dc_pack2(fmaf(p0, 0x1.000002p0f, -__uint_as_float(b0 & 0xffff0000u)), fmaf(p1, 0x1.000002p0f, -__uint_as_float(b1 & 0xffff0000u)));
         }
       ph[rt] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){hi[0], hi[1], hi[2], hi[3]});
-      if constexpr (TWO) pl[0] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){lw[0], lw[1], lw[2], lw[3]});
+      pl[rt] = __builtin_bit_cast(dc_bf16x8, (dc_u32x4){lw[0], lw[1], lw[2], lw[3]});
     }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(vr[ct][0]), "+v"(vr[ct][1]));
@@ -454,18 +455,15 @@ __global__ __launch_bounds__(SH_THREADS, 1) void sp_shared_kernel(const ShArgs a
           if ((met >> rt) & 1u) l[rt] *= __builtin_nanf("");
       }
     }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, __builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3)),
-                                                            ph[rt], o[rt][ct], 0, 0, 0);
-    if constexpr (TWO) {
+    auto weigh = [&](const dc_bf16x8 (&p)[RT]) {
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct)
-        o[0][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            __builtin_bit_cast(dc_bf16x8, ds_finite(__builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3))), pl[0], o[0][ct], 0, 0, 0);
-    }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, __builtin_shufflevector(vr[ct][0], vr[ct][1], 0, 1, 2, 3)),
+                                                              p[rt], o[rt][ct], 0, 0, 0);
+    };
+    weigh(ph), weigh(pl);
   };
 
   // A tile's steps: wave w has rows 32 (w / share) .. of the tile and of a block's four steps w % share, + share, ..; it fills K's or V's half of ring
