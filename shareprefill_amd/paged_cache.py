@@ -219,7 +219,8 @@ class PagedKVCache:
         """Rows (bool [max_requests]) that are empty, as release leaves them, begin behind what their group shares; others stay as they are, a group's first
         row too.  (An empty row of a group may as well take a request that shares nothing, without joining.)"""
         self._check_mask(rows, "rows")
-        rows = rows & (self.lens == 0) & (self._holder != torch.arange(self.max_requests, device=self._holder.device))
+        # (what an eviction has left nothing of is a request all the same)
+        rows = rows & (self.lens == 0) & (self.dropped == 0) & (self._holder != torch.arange(self.max_requests, device=self._holder.device))
         shared = torch.cat((self.shared_lens, self.shared_lens.new_zeros(1)))[self._group_of]
         place = torch.arange(self.block_table.shape[1], device=self.lens.device)[None, :]
         named = torch.where(place * self.page_size < shared[:, None], self.block_table[self._holder], -1)

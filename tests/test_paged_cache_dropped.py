@@ -84,3 +84,17 @@ def test_a_request_that_an_eviction_has_spoilt(monkeypatch):
     assert (cache.block_table[0] >= 0).sum() == 1 and cache.free_count.item() == 20 - 6 and cache.dropped.tolist()[0] == 82
     cache.release(_mask(0))
     assert cache.lost.tolist() == [False] * 6 and cache.free_count.item() == 20 - 5
+
+
+def test_a_request_that_an_eviction_left_nothing_of_is_no_empty_row(evicting):
+    cache = evicting
+    _fill(cache, 0, 3, 40)
+    _fill(cache, 1, 2, 30)
+    cache.evict(budget=0, recent=0, rows=_mask(1))
+    assert cache.lens.tolist()[:2] == [40, 0] and cache.dropped.tolist()[:2] == [0, 30]
+    cache.share(0, 40)
+    cache.join(_mask(1))
+    assert cache.lens.tolist()[:3] == [40, 0, 32] and cache.dropped.tolist()[:3] == [0, 30, 0] and (cache.block_table[1] == -1).all()
+    cache.release(_mask(1))
+    cache.join(_mask(1))
+    assert cache.lens.tolist()[:3] == [40, 32, 32] and cache.dropped.tolist()[:3] == [0, 0, 0]
