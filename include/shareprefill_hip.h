@@ -463,6 +463,9 @@ typedef struct sp_paged_key_weights_args {
 } sp_paged_key_weights_args;
 size_t sp_paged_key_weights_workspace_bytes(int64_t tokens, int32_t batch, int32_t hq, int32_t hkv);
 int sp_paged_key_weights_bf16(const sp_paged_key_weights_args* args /* host */);
+/* weights (as above, element strides for the page and head axes): 0 at slots[t] (int64 [tokens]) in every head; a slot outside the pool is skipped. */
+int sp_paged_weights_clear(float* weights, const int64_t* slots, int64_t tokens, int64_t hkv, int64_t num_pages, int64_t page_size, int64_t w_stride_page,
+                           int64_t w_stride_h, sp_stream_t stream);
 
 /* Drops the lightest keys of every kv head of sequences that hold more than they may: of sequence b with seq_lens[b] keys the first first[b] (null: 0)
  * and the last `recent` stay and of those between the `budget` heaviest by their weights (of equal ones the first; a weight that is negative or no

@@ -110,6 +110,7 @@ SIGNATURES = {
     "sp_shared_attn_from_bf16": (_I32, [C.c_char_p, _P]),
     "sp_paged_key_weights_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32]),
     "sp_paged_key_weights_bf16": (_I32, [C.c_char_p]),
+    "sp_paged_weights_clear": (_I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "sp_paged_evict_workspace_bytes": (_SZ, [_I32, _I32, _I32, _I64, _I64, _I64]),
     "sp_paged_evict_bf16": (_I32, [C.c_char_p]),
     "sp_paged_evict_bounded_bf16": (_I32, [C.c_char_p, _I32]),

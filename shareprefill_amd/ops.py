@@ -839,6 +839,20 @@ def paged_key_weights(q: torch.Tensor, k_pages: torch.Tensor, block_table: torch
     return weights
 
 
+def paged_weights_clear(weights: torch.Tensor, slots: torch.Tensor) -> None:
+    """What new keys have received, whatever an earlier owner of their places left: weights fp32 [num_pages, Hkv, page_size] view becomes 0 at their slots
+    (int64 [T], page_tables) in every head.  Slots outside the pool are left out."""
+    lib = _lib.load()
+    if weights.dim() != 3 or not weights.is_cuda:
+        raise ValueError(f"weights must be [num_pages, Hkv, page_size] on the GPU, got {tuple(weights.shape)} on {weights.device}")
+    (pages, hkv, page_size), dev = weights.shape, weights.device
+    _check_weights(weights, pages, hkv, page_size, dev)
+    _check_ints(dev, ("slots", slots, torch.int64, slots.numel()))
+    st = lib.sp_paged_weights_clear(weights.data_ptr(), slots.data_ptr(), slots.numel(), hkv, pages, page_size, weights.stride(0), weights.stride(1), _stream_handle(dev))
+    if st:
+        _lib.check(st, "sp_paged_weights_clear")
+
+
 def paged_evict(k_pages: torch.Tensor, v_pages: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int,
                 recent: int, first: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Drops the lightest keys of requests that hold more than they may, in place: of a request's keys the first first[b] (int32 [B]; None: 0), the last

@@ -74,7 +74,6 @@ class PagedKVCache:
         self.dropped = torch.zeros(max_requests, dtype=torch.int32, device=dev)
         self.lost = torch.zeros(max_requests, dtype=torch.bool, device=dev)  # requests whose keys an eviction has spoilt
         self._last = None  # of a step: rows of its requests' last tokens (observe)
-        self._fresh = None  # of a step: places that its tokens' keys come to
 
     def _check_mask(self, mask: torch.Tensor, name: str) -> None:
         if mask.dtype is not torch.bool or tuple(mask.shape) != (self.max_requests,) or mask.device != self.lens.device:
@@ -118,7 +117,7 @@ class PagedKVCache:
                 token = torch.arange(t.positions.numel(), dtype=torch.int32, device=self.lens.device)
                 row = torch.searchsorted(t.cu_new[1:], token, right=True).clamp_(max=self.max_requests - 1)
                 t = t._replace(positions=t.positions + torch.where(token < t.cu_new[-1:], self.dropped[row], 0))
-        self.tables, self._cu_q, self._last, self._fresh = t, None if singles else t.cu_new, None, None
+        self.tables, self._cu_q, self._last = t, None if singles else t.cu_new, None
         return t
 
     def _pools_of(self, layer: int):
@@ -130,16 +129,7 @@ class PagedKVCache:
         """k, v: bf16 [Hkv, T, D] views of the step's tokens."""
         ops.paged_cache_write(k, v, *self._pools_of(layer), self.tables.slots)
         if self.weights is not None and self._cu_q is not None:
-            self._clear_weights(layer)
-
-    def _clear_weights(self, layer: int) -> None:
-        """The step's new keys have received nothing yet, whatever an earlier owner of their places left."""
-        if self._fresh is None:
-            places, slots = self.num_pages * self.page_size, self.tables.slots
-            fresh = torch.zeros(places + 1, dtype=torch.bool, device=slots.device)
-            fresh.index_fill_(0, torch.where(slots < 0, places, slots).long(), True)
-            self._fresh = fresh[:-1].view(self.num_pages, 1, self.page_size)
-        self.weights[layer].masked_fill_(self._fresh, 0)
+            ops.paged_weights_clear(self.weights[layer], self.tables.slots)
 
     def attend(self, layer: int, q: torch.Tensor, softmax_scale: float, window: Optional[int] = None, sinks: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -159,7 +149,7 @@ class PagedKVCache:
                 ops.paged_key_weights(q, pools[0], self.block_table, self._seen_lens, softmax_scale, weights, first=self._held, accumulate=True)
             return out
         if self.weights is not None and self._cu_q is None:
-            self._clear_weights(layer)
+            ops.paged_weights_clear(self.weights[layer], self.tables.slots)
         return ops.paged_attention(q, *pools, self.block_table, self._seen_lens, softmax_scale, cu_q=self._cu_q,
                                    window=window, sinks=sinks, out=out)
 
