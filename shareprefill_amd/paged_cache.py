@@ -187,9 +187,10 @@ class PagedKVCache:
         ops.paged_key_weights(q, pools[0], self.block_table, self._seen_lens, softmax_scale, weights[layer], cu_q=cu, first=self._held,
                               accumulate=accumulate)
 
-    def share(self, group: int, tokens: int) -> None:
+    def share(self, group: int, tokens: int) -> int:
         """The first `tokens` keys of the group's first row, as many as fill whole pages, become those of all its rows: the others begin behind them, if they
-        are empty.  The first row must have them cached; it may go on as a request of its own, and its end is the end of the sharing (release)."""
+        are empty.  The first row must have them cached; it may go on as a request of its own, and its end is the end of the sharing (release).  -> how many
+        they are: the tokens from there on are the other rows' own to bring."""
         if not 0 <= group < self.shared_lens.numel():
             raise ValueError(f"there are {self.shared_lens.numel()} groups, no group {group}")
         if not 0 <= tokens <= self.block_table.shape[1] * self.page_size:
@@ -204,6 +205,7 @@ class PagedKVCache:
         rows = torch.zeros(self.max_requests, dtype=torch.bool, device=self.lens.device)
         rows[first + 1:end] = True
         self.join(rows)
+        return whole
 
     def join(self, rows: torch.Tensor) -> None:
         """Rows (bool [max_requests]) that are empty, as release leaves them, begin behind what their group shares; others stay as they are, a group's first

@@ -98,3 +98,10 @@ def test_a_request_that_an_eviction_left_nothing_of_is_no_empty_row(evicting):
     cache.release(_mask(1))
     cache.join(_mask(1))
     assert cache.lens.tolist()[:3] == [40, 32, 32] and cache.dropped.tolist()[:3] == [0, 0, 0]
+
+
+def test_share_says_where_the_other_rows_begin():
+    cache = _cache()
+    _fill(cache, 0, 4, 60)
+    assert [cache.share(0, n) for n in (0, 15, 16, 55)] == [0, 0, 16, 48]
+    assert cache.lens.tolist()[:3] == [60, 16, 16]  # (rows that are no longer empty stay as they are)
