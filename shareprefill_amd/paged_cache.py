@@ -248,8 +248,8 @@ class PagedKVCache:
     def _give_back(self, entries: torch.Tensor) -> None:
         """Puts the pages of entries of the block table (bool, its shape) back on the stack, those that no other entry names, each once."""
         back = entries & (self.block_table >= 0)
-        page = torch.where(self.block_table >= 0, self.block_table, self.num_pages).reshape(-1).long()
         if self.shared_lens.numel() > 0:
+            page = torch.where(self.block_table >= 0, self.block_table, self.num_pages).reshape(-1).long()
             kept = torch.zeros(self.num_pages + 1, dtype=torch.bool, device=page.device)
             kept[torch.where(entries.reshape(-1), self.num_pages, page)] = True
             place = torch.arange(page.numel(), device=page.device)
@@ -268,8 +268,9 @@ class PagedKVCache:
         self._check_mask(finished, "finished")
         self._give_back(finished[:, None].expand_as(self.block_table))
         self.lens.masked_fill_(finished, 0)
-        for x in (self.dropped, self._held, self._joined, self.lost):
-            x.masked_fill_(finished, 0)
+        if self.weights is not None or self.shared_lens.numel() > 0:  # (else they stay 0)
+            for x in (self.dropped, self._held, self._joined, self.lost):
+                x.masked_fill_(finished, 0)
         if self.shared_lens.numel() > 0:
             ended = finished[self.cu_groups[:-1].long()]
             self.shared_lens.masked_fill_(ended, 0)
