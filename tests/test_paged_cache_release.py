@@ -22,8 +22,9 @@ def test_what_only_groups_and_weights_need_is_left_out():
         cache = _cache(**kw)
         _fill(cache, 1, 3, 40)
         _fill(cache, 4, 2, 20)
+        finished = _mask(1)
         with _Count() as ops:
-            cache.release(_mask(1))
+            cache.release(finished)
         counts[name] = ops.n
         assert cache.free_count.item() == 18 and cache.lens.tolist() == [0, 0, 0, 0, 20, 0]
     # one each: >=, &, cumsum, +, -, where and its scalar, a cast, the pages put back, the count, the entries, the lengths
