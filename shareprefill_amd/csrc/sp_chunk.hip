@@ -106,8 +106,8 @@ __device__ __forceinline__ void ck_qk_only(const Addr& ad, const bf16x8 (&qb)[2]
     AT_PIN();
   });
 }
-template <int VB, int KT, bool HALF, class Addr>
-__device__ __forceinline__ void ck_pv_only(const Addr& ad, const bf16x8 (&p)[2], floatx4 (&o)[9][2], const bf16x8& ones) {
+template <int VB, int KT, bool HALF, class Addr, int PN>
+__device__ __forceinline__ void ck_pv_only(const Addr& ad, const bf16x8 (&p)[PN], floatx4 (&o)[9][2], const bf16x8& ones) {
   constexpr int PS = HALF ? 4 : 8;
   bf16x8 a[PS];  // slot i: channel tile i
   auto fetch = [&](auto kc) {
@@ -122,9 +122,13 @@ __device__ __forceinline__ void ck_pv_only(const Addr& ad, const bf16x8 (&p)[2],
     AT_PIN();
     if constexpr (i + 2 < PS) fetch(std::integral_constant<int, i + 2>{});
 #pragma unroll
-    for (int qt = 0; qt < 2; ++qt) at_mfma_acc(o[i][qt], a[i], p[qt]);
+    for (int part = 0; part < PN; ++part) at_mfma_acc(o[i][part & 1], a[i], p[part]);
     AT_PIN();
   });
+  if constexpr (PN == 4) {
+    at_mfma_acc(o[8][0], ones, p[2]);
+    at_mfma_acc(o[8][1], ones, p[3]);
+  }
   at_mfma_acc(o[8][0], ones, p[0]);
   at_mfma_acc_settled(o[8][1], ones, p[1]);  // the end of the walk: the epilogue reads O next
 }
@@ -625,7 +629,7 @@ __device__ __forceinline__ void ck_attend(const CkArgs& a) {
         if (have_next) load_q(next_p);
       } else {
         floatx4 sa[2][2], sb[2][2];  // [key tile][row tile]
-        bf16x8 pa[2], pb[2];         // [row tile]
+        bf16x8 pa[GROUPS ? 4 : 2], pb[GROUPS ? 4 : 2];  // [row tile], of groups in two parts
         bf16x8 pre[2];
         Block old = cur;
         bool some = partly(cur), some_old = some;

@@ -42,6 +42,14 @@ __device__ __forceinline__ uint32_t at_pack2(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
 }
 
+// The same as two bf16 values each: what truncation leaves, and the rest, of at least 2^-23 of the whole (an infinite value of V has met its weight in the first one's
+// product, and zero or a negative number times infinity would make a NaN of the sum).
+__device__ __forceinline__ void at_split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  hi = __builtin_amdgcn_perm(y, x, 0x07060302u);
+  lo = at_pack2(__builtin_fmaf(a, 0x1.000002p0f, -__uint_as_float(x & 0xffff0000u)), __builtin_fmaf(b, 0x1.000002p0f, -__uint_as_float(y & 0xffff0000u)));
+}
+
 // compile-time loop: f(std::integral_constant<int, K>) for K = 0 .. N-1
 template <int K, int N, typename F>
 __device__ __forceinline__ void at_static_for(F&& f) {
@@ -133,9 +141,10 @@ __device__ __forceinline__ void at_prefetch_qk(const Addr& ad, bf16x8 (&pre)[2])
 // Addr: where the operands of a block lie in LDS.  k<KQ, KS, T>() fetches channel step KS of key tile T of quarter KQ, v<VB, KT, I>() channel
 // tile I of half KT of buffer VB, both unseen by the compiler; V_READS: LDS reads of the latter.
 // EARLY: they are asked for two slots in front of the stage's end, and have landed there: no branch finds them on their way.
-template <bool DO_QK, bool DO_PV, int KQ, int VB, int KT, bool PRE, int NEXT, bool HALF, bool SETTLE, bool EARLY, class Addr>
+// PN: 2, probabilities of a query tile each, or 4, their first and then their second parts (at_split2), with a product more for either.
+template <bool DO_QK, bool DO_PV, int KQ, int VB, int KT, bool PRE, int NEXT, bool HALF, bool SETTLE, bool EARLY, class Addr, int PN>
 __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4], floatx4 (&s_out)[2][2],
-                                         const floatx4 (&s_in)[2][2], const bf16x8 (&p_prev)[2], bf16x8 (&p_out)[2],
+                                         const floatx4 (&s_in)[2][2], const bf16x8 (&p_prev)[PN], bf16x8 (&p_out)[PN],
                                          floatx4 (&o)[9][2], float sc, const float (&neg_m)[2], uint32_t (&det)[2],
                                          const bf16x8& ones, bf16x8 (&pre)[2]) {
   static_assert(!PRE || DO_QK, "only stages that start with the S product take prefetched operands");
@@ -147,7 +156,8 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
   constexpr int AHEAD = 2;      // LDS operands are fetched this many slots before their MFMAs
   bf16x8 opnd[NP];
   float x[16], e[16];
-  uint32_t pk[8];
+  uint32_t pk[8], pl[8];
+  constexpr bool TWO = PN == 4;
   auto fetch = [&](auto kc) {
     constexpr int k = decltype(kc)::value;
     constexpr bool qk = k < QS;
@@ -206,7 +216,10 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
       if (idx >= 1) e[idx - 1] = __builtin_amdgcn_exp2f(x[idx - 1]);
       if (idx >= 3 && ((idx - 3) & 1) == 0) {
         const int m = (idx - 3) >> 1;
-        pk[m] = at_pack2(e[idx - 3], e[idx - 2]);
+        if constexpr (TWO)
+          at_split2(e[idx - 3], e[idx - 2], pk[m], pl[m]);
+        else
+          pk[m] = at_pack2(e[idx - 3], e[idx - 2]);
         // OR of the packed probabilities: any exponent >= 128 (P >= 2, inf, NaN) shows in bit 14 or 30
         // (three words at a time: one three-input instruction)
         if ((m & 3) == 2) det[m >> 2] = pk[m - 2] | pk[m - 1] | pk[m];
@@ -220,11 +233,20 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
           asm volatile("" : "+v"(pk[(idx - 3) >> 1]), "+v"(det[(idx - 3) >> 3]));
         else
           asm volatile("" : "+v"(pk[(idx - 3) >> 1]));
+        if constexpr (TWO) asm volatile("" : "+v"(pl[(idx - 3) >> 1]));
       }
     }
     AT_PIN();
     mfma(std::integral_constant<int, 1 - (k & 1)>{}, std::integral_constant<bool, SETTLE && !DO_PV && k == NP - 1>{});
+    if constexpr (TWO && !qk) {
+      at_mfma_acc(o[i][k & 1], opnd[k], p_prev[2 + (k & 1)]);
+      at_mfma_acc(o[i][1 - (k & 1)], opnd[k], p_prev[3 - (k & 1)]);
+    }
     if constexpr (DO_PV && k == NP - 1) {  // row sums of P(j-1) as rounded for the P.V product: ones . P
+      if constexpr (TWO) {
+        at_mfma_acc(o[8][0], ones, p_prev[2]);
+        at_mfma_acc(o[8][1], ones, p_prev[3]);
+      }
       at_mfma_acc(o[8][0], ones, p_prev[0]);
       if constexpr (SETTLE)
         at_mfma_acc_settled(o[8][1], ones, p_prev[1]);
@@ -241,7 +263,10 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
     AT_PIN();
   }
   e[15] = __builtin_amdgcn_exp2f(x[15]);
-  pk[7] = at_pack2(e[14], e[15]);
+  if constexpr (TWO)
+    at_split2(e[14], e[15], pk[7], pl[7]);
+  else
+    pk[7] = at_pack2(e[14], e[15]);
   det[1] |= pk[7];
   static_assert(!(DO_QK && !DO_PV) || SETTLE, "a run's first stage: the next stage's softmax reads S_out at once");
   at_u32x4 w0, w1;
@@ -252,6 +277,10 @@ __device__ __forceinline__ void at_fused(const Addr& ad, const bf16x8 (&qb)[2][4
   }
   p_out[0] = __builtin_bit_cast(bf16x8, w0);
   p_out[1] = __builtin_bit_cast(bf16x8, w1);
+  if constexpr (TWO) {
+    p_out[2] = __builtin_bit_cast(bf16x8, (at_u32x4){pl[0], pl[1], pl[2], pl[3]});
+    p_out[3] = __builtin_bit_cast(bf16x8, (at_u32x4){pl[4], pl[5], pl[6], pl[7]});
+  }
 }
 
 // max over the lane's 8 keys of each query tile
@@ -298,8 +327,8 @@ __device__ __forceinline__ float at_groupmax(float mx) {
 // kernel) follows every rescale.
 // MODE: bit 0 = PIVOT, bit 1 = HALF (see at_fused), bit 2 = FINE (sp_attn.hip), bits 4 .. 6 = SLACK: octaves that a moved max is set above the
 // largest logit
-template <int MODE>
-__device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 (&p)[2], uint32_t (&det)[2],
+template <int MODE, int PN>
+__device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 (&p)[PN], uint32_t (&det)[2],
                                           floatx4 (&o)[9][2], float scale_log2, float (&m_run)[2],
                                           float (&l_mark)[2]) {
   constexpr bool PIVOT = (MODE & 1) != 0, HALF = (MODE & 2) != 0;
@@ -321,7 +350,7 @@ __device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 
     at_settle_o(o);
     // m_run = AT_NO_MAX on a row's first keys: alpha = 0 (O and the sums are still zero then)
     const float alpha[2] = {__builtin_amdgcn_exp2f(m_run[0] - m_new[0]), __builtin_amdgcn_exp2f(m_run[1] - m_new[1])};
-    uint32_t pk[8];
+    uint32_t pk[8], pl[8];
 #pragma unroll
     for (int qt = 0; qt < 2; ++qt) {
       if constexpr (PIVOT) l_mark[qt] *= alpha[qt];
@@ -336,12 +365,22 @@ __device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 
       for (int j = 0; j < 8; ++j)
         e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(AT_SVAL(s_prev, 8 * qt + j), scale_log2, -m_new[qt]));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) pk[4 * qt + j] = at_pack2(e[2 * j], e[2 * j + 1]);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (PN == 4)
+          at_split2(e[2 * j], e[2 * j + 1], pk[4 * qt + j], pl[4 * qt + j]);
+        else
+          pk[4 * qt + j] = at_pack2(e[2 * j], e[2 * j + 1]);
+      }
       m_run[qt] = m_new[qt];
     }
     at_settle_o(o);
     p[0] = __builtin_bit_cast(bf16x8, (at_u32x4){pk[0], pk[1], pk[2], pk[3]});
     p[1] = __builtin_bit_cast(bf16x8, (at_u32x4){pk[4], pk[5], pk[6], pk[7]});
+    if constexpr (PN == 4) {
+      p[2] = __builtin_bit_cast(bf16x8, (at_u32x4){pl[0], pl[1], pl[2], pl[3]});
+      p[3] = __builtin_bit_cast(bf16x8, (at_u32x4){pl[4], pl[5], pl[6], pl[7]});
+      asm volatile("" : "+v"(p[2]), "+v"(p[3]));
+    }
     asm volatile("s_nop 4" : "+v"(p[0]), "+v"(p[1]));  // vector writes of P are complete before an MFMA reads them
   }
   det[0] = 0u;
@@ -352,9 +391,9 @@ __device__ __forceinline__ void at_commit(const floatx4 (&s_prev)[2][2], bf16x8 
 // packed words; s_out still holds S(j-1) on entry and S(j+1) on return, p_out = P(j) with its OR in det.
 // The fused stage exists once per step: O never lives in two register sets that would have to be merged.
 // mask(s): takes out what the half-tile's queries do not see of its keys.
-template <bool DO_QK, bool HAVE_PREV, int KQ, int VB, int KT, int MODE, bool PRE = false, int NEXT = -1, bool EARLY = false, class Addr, class Mask>
+template <bool DO_QK, bool HAVE_PREV, int KQ, int VB, int KT, int MODE, bool PRE = false, int NEXT = -1, bool EARLY = false, class Addr, class Mask, int PN>
 __device__ __forceinline__ void at_step(const Addr& ad, const bf16x8 (&qb)[2][4], floatx4 (&s_out)[2][2],
-                                        floatx4 (&s_in)[2][2], bf16x8 (&p_prev)[2], bf16x8 (&p_out)[2],
+                                        floatx4 (&s_in)[2][2], bf16x8 (&p_prev)[PN], bf16x8 (&p_out)[PN],
                                         floatx4 (&o)[9][2], float scale_log2, float (&m_run)[2], uint32_t (&det)[2],
                                         const bf16x8& ones, Mask&& mask, float (&l_mark)[2], bf16x8 (&pre)[2]) {
   if (HAVE_PREV) at_commit<MODE>(s_out, p_prev, det, o, scale_log2, m_run, l_mark);

@@ -46,10 +46,10 @@ PG_FN int sh_first_own(int len, int q_len, int shared) { return len - q_len >= s
 // Numbers of row tiles, by 64 rows (a larger one has that of its first): every sequence has room for its last, partly filled one (pg_first_slot); single tokens whose heads fit a tile have one each.
 PG_FN int64_t sh_own_slot(int64_t start, int g, int b, int dense) { return dense ? b : pg_first_slot(start, g, b, SH_UNIT); }
 // Groups of many rows are left to the kernel that has matrix products' rate (sp_chunk.hip, tiles of 256 rows) where the table has room for enough keys to pay
-// for two launches more, but not where keys are weighed: its sums are those of probabilities rounded to bf16.  By rows x keys of all kv heads, in millions, us
-// within one launch / apart: 32 heads over 8 of 128 channels 5 37 / 56, 26 46 / 60, 34 69 / 69, 49 76 / 73, 66 91 / 78, 131 142 / 105, 524 292 / 186; 28 over 4 9
-// 36 / 48, 36 67 / 71, 57 80 / 73; of 64 channels 25 44 / 52, 49 55 / 58, 58 73 / 69, 66 68 / 61, 131 113 / 82.  At 256 rows and fewer tiles of 256 are not full.
+// for two launches more, but not where keys are weighed: its sums are those of probabilities rounded to two bf16 values.  By rows x keys of all kv heads, in millions, us
+// within one launch / apart: 32 heads over 8 of 128 channels 6 37 / 58, 26 68 / 75, 34 78 / 79, 49 100 / 91, 66 128 / 103, 132 202 / 131, 526 714 / 379; 28 over 4 9
+// 39 / 52, 36 87 / 77, 57 121 / 97; of 64 channels 26 56 / 58, 49 85 / 72, 58 99 / 77, 66 107 / 81, 132 169 / 96.  At 256 rows and fewer tiles of 256 are not full.
 PG_FN bool sh_may_be_apart(int64_t tokens, int64_t groups, int64_t g, bool weighed) { return !weighed && groups > 0 && tokens * g > 256 * groups; }
 PG_FN bool sh_apart(int64_t tokens, int64_t groups, int64_t hq, int64_t hkv, int64_t room, bool weighed) {
-  return sh_may_be_apart(tokens, groups, hq / hkv, weighed) && (double)(tokens * hq) * (double)room > 5e7;
+  return sh_may_be_apart(tokens, groups, hq / hkv, weighed) && (double)(tokens * hq) * (double)room > 3e7;
 }

@@ -752,10 +752,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     call: 52 MB at 128 channels with 256 kv heads or fewer (86 MB where groups have more than 256 rows), half of it at 64, 8 Hq (D + 2) bytes a token, and
     with weights 4 Hq num_pages page_size.
 
-    Precision: sums, maxima and partial results have 32 bits.  Probabilities enter the product with V as two bf16 values (outputs some 1.7e-3 from 64 bits, nearly all of
-    it their own rounding), as one over the shared keys of groups that have more than 256 rows (tokens x query heads of a kv head) on average, where the
-    table has room for many keys: 5e7 and more, times tokens and heads (some 2.3e-3).  A value that is not finite makes the rows that see it not finite,
-    and no others."""
+    Precision: sums, maxima and partial results have 32 bits.  Probabilities enter the product with V as two bf16 values (outputs some 1.7e-3 from 64 bits, nearly
+    all of it their own rounding).  A value that is not finite makes the rows that see it not finite, and no others."""
     lib = _lib.load()
     _check_hnd(q, "q")
     hq, n, d = q.shape

@@ -17,10 +17,21 @@ def _ints(dev, x):
 @pytest.mark.parametrize("new", [1, 3])
 @pytest.mark.parametrize("at", [(35, 50), (75, 90), (20, 99)])  # (shared, side by side: one running maximum; own; one of either)
 def test_two_keys_that_cancel(gpu_device, hq, hkv, d, new, at):
+    _check_cancelling(gpu_device, hq, hkv, d, new, at, 4, 0)
+
+
+@pytest.mark.parametrize("hq,hkv,d,new,members", [(8, 2, 128, 1, 70), (14, 2, 64, 3, 14), (24, 1, 64, 1, 12)])
+@pytest.mark.parametrize("at", [(35, 50), (20, 99)])
+def test_two_keys_that_cancel_in_a_launch_of_their_own(gpu_device, hq, hkv, d, new, members, at):
+    """More than 256 rows, and a table with room for 3e7 keys times tokens and heads."""
+    _check_cancelling(gpu_device, hq, hkv, d, new, at, members, 160000)
+
+
+def _check_cancelling(gpu_device, hq, hkv, d, new, at, members, room_of_table):
     """Two keys of nearly the same weight have all of it, and values of either sign: what is left of them is small, and a weight's rounding shows."""
     from shareprefill_amd import ops
 
-    dev, page, members = gpu_device, 16, 4
+    dev, page = gpu_device, 16
     gen = torch.Generator().manual_seed(hq + new)
     pools, table, lens, shared, cu, kv, _ = make_shared([(70, [40 + i for i in range(members)])], [], hkv, d, page, gen)
     q = 0.125 * torch.randn(members * new, hq, d, generator=gen)
@@ -37,6 +48,8 @@ def test_two_keys_that_cancel(gpu_device, hq, hkv, d, new, at):
         for i, j in enumerate(at):
             kv[b][0][:, j], kv[b][1][:, j] = one[i].to(torch.bfloat16), value[i].to(torch.bfloat16)
             pools[0][table[b, j // page], :, j % page], pools[1][table[b, j // page], :, j % page] = one[i].to(torch.bfloat16), value[i].to(torch.bfloat16)
+    if room_of_table:
+        table = torch.cat((table, torch.full((members, room_of_table // page - table.shape[1]), -1, dtype=torch.int32)), 1).contiguous()
     out = ops.shared_prefix_attention(q.to(dev), *(x.to(dev) for x in pools), table.to(dev), _ints(dev, lens), _ints(dev, shared), _ints(dev, cu), 1.0,
                                       cu_q=None if new == 1 else _ints(dev, [new * b for b in range(members + 1)]))
     for b, n in enumerate(lens):
