@@ -155,9 +155,10 @@ class PagedKVCache:
 
     def _many_rows(self, q: torch.Tensor) -> bool:
         """Chunks of prompts: the kernel with matrix products' rate takes less time to read shared keys once a request than the other to read them once.
-        us, shared / paged, by rows (tokens x query heads of a kv head) a request: 16 of 32 heads over 8 behind 4096 keys 16: 38 / 63, 32: 51 / 64, 64: 69 / 66,
-        128: 100 / 72, 2048: 812 / 524; 4 behind 32768 keys 32: 60 / 93, 64: 105 / 97, 2048: 980 / 893; 16 of 14 over 2 behind 4096 28: 26 / 26, 56: 30 / 28."""
-        return self._cu_q is not None and q.dim() == 3 and q.shape[1] * q.shape[0] > 48 * self.max_requests * self.pools.shape[3]
+        us, shared / paged, by rows (tokens x query heads of a kv head) a request: 16 of 32 heads over 8 behind 4096 keys 16: 40 / 57, 32: 54 / 57, 48: 83 / 58,
+        128: 102 / 66, 2048: 1021 / 519; 4 behind 32768 keys 32: 72 / 91, 48: 92 / 94, 64: 111 / 94, 2048: 1308 / 879; 16 of 14 over 2 behind 4096 28: 28 / 26, 56:
+        34 / 26."""
+        return self._cu_q is not None and q.dim() == 3 and q.shape[1] * q.shape[0] > 32 * self.max_requests * self.pools.shape[3]
 
     def _check_weights(self) -> torch.Tensor:
         if self.weights is None:
