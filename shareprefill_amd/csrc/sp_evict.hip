@@ -9,8 +9,8 @@
 // workgroup each, and written behind a wait for the chunks in front (sp_evict_move_kernel).
 // Moving is HBM-bound where there are many kv heads in all, kept rows once in and out; one request's is latency: chains of three loads.
 //
-// Measured, 128 channels, on rows that have not been moved before: 16 requests of up to 8001 keys, 4 kv heads, 2064 rows left, 133 MB: choosing 15 us, moving 36, 3.7 TB/s;
-// one of 131072 keys, 8 kv heads, 8192 left: two reads of the weights 6 and 10, choosing 20, moving 29; one of 2000, 320 left: choosing 14, moving 7.
+// Measured, 128 channels, on rows that have not been moved before: 16 requests of up to 8001 keys, 4 kv heads, 2064 rows left, 133 MB: choosing 14 us, moving 35, 3.8 TB/s;
+// one of 131072 keys, 8 kv heads, 8192 left: two reads of the weights 7 and 10, choosing 21, moving 27; one of 2000, 320 left: choosing 13, moving 6.
 #include "sp_common.h"
 #include "sp_paged_plan.h"
 

@@ -11,9 +11,9 @@
 // waves the queries would be staged half as often, which took as long.  Every key's sum is formed by one wave in one order: results do not depend on timing.
 // Requests' blocks of 128 keys lie on a line per kv head that is cut into equal parts, a workgroup each.
 //
-// Measured (first walk, rows' parts joined, second walk): 32 queries of 28 heads over 4 of 128 channels over 32768 keys 23.5 + 4.9 + 20.4 us, 15 GFLOP in both
+// Measured (first walk, rows' parts joined, second walk): 32 queries of 28 heads over 4 of 128 channels over 32768 keys 23.9 + 4.8 + 19.6 us, 15 GFLOP in both
 // products; of a walk 3 us are the line, 5 the queries and first keys, 4 a block of 224 rows.  64 queries each of 8 requests of 32 heads over 8 of 64 channels over up
-// to 8001 keys 29.8 + 5.6 + 25.4; 16 over 1025 keys of 32 heads over 8 11.4 + 10.0, all of it latency.
+// to 8001 keys 31.2 + 5.9 + 26.1; 16 over 1025 keys of 32 heads over 8 10.6 + 10.4, all of it latency.
 #include "sp_ring.h"
 #include "sp_paged_plan.h"
 

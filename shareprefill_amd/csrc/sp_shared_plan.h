@@ -14,9 +14,8 @@
 #define SH_KEYS 32       // of a step
 #define SH_MAX_SEQS 1024
 enum { SH_GROUP, SH_OWN, SH_STREAM };  // items: a group's shared keys, a request's own, the same as a matter of waves
-// Units of a tile beside its steps.  (us, 6 / 10 / 14 / 20 of a request's: two tokens each of 40 requests over 120 own keys, most behind 17378 shared
-// ones 57 / 48 / 48 / 50, nine of 20 over a few 37 / 32 / 34 / 33, two of 37 over 1336 40 / 39 / 40 / 40; 6 / 7 / 8 of a group's: eight tokens behind 1024 keys
-// 20 / 22 / 22.)
+// Units of a tile beside its steps.  (us, 32 heads over 8, 6 / 10 / 14 / 20 of a request's: nine tokens each of 20 requests behind 2000 shared keys 65 / 51 / 51 / 49, two of 37
+// over 1336 own ones 49 / 50 / 50 / 50, of 14 heads over 2 22 / 22 / 22 / 24; 6 / 7 / 8 of a group's: eight tokens each of 8 requests behind 1024 keys 30 / 33 / 33.)
 #define SH_OVERHEAD 6
 #define SH_OWN_OVERHEAD 10
 #define SH_STREAM_OVERHEAD 1

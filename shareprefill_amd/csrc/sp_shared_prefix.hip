@@ -11,9 +11,9 @@
 //     share out the steps.  Two waves share a SIMD, where the matrix instructions of one run under the exponentials of the other.
 // Groups of many rows over many keys go to sp_chunk.hip's loop first, in a launch of its own (sh_apart).
 //
-// Measured, 32 heads over 8 of 128 channels, this launch and the joining one: 64 single tokens behind 8192 shared keys and up to 2000 own, 365 MB, 82.6 + 6.3 us,
-// 4.1 TB/s (a copy 5.05); 8 behind 1024 and up to 200 15.2 + 4.4 us, of which 3.5 are the line, 2 the launch, 9 a part of the group: its queries and first keys,
-// two blocks, its end; 128 behind 32768, 52 us for the requests and 86 + 11 for the group (69 GFLOP, 800 TFLOP/s).  Without groups 64 single tokens over
+// Measured, 32 heads over 8 of 128 channels, this launch and the joining one: 64 single tokens behind 8192 shared keys and up to 2000 own, 365 MB, 79 + 6.9 us,
+// 4.3 TB/s (a copy 5.05); 8 behind 1024 and up to 200 15.3 + 4.3 us, of which 3.5 are the line, 2 the launch, 9 a part of the group: its queries and first keys,
+// two blocks, its end; 128 behind 32768, 55 us for the requests and 117 + 11 for the group (69 GFLOP and half as many for the probabilities' second parts, 880 TFLOP/s).  Without groups 64 single tokens over
 // 500 to 2000 keys take 67 us, sp_paged_decode.hip's kernels 70; 8 over 50 to 200 keys 14 and 7, 32 of 64 channels over 250 to 1000
 // 23 and 12: the line, and a joining launch whether anything was cut or not.
 #include "sp_chunk.h"
